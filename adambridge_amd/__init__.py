@@ -8,7 +8,9 @@ of parameters per launch.  The public API mirrors the reference package
 
 from . import native, precision
 from .engine import StepStats
+from .experts import Routing, combine, dispatch, expert_mm, route
 from .losses import causal_lm_loss
+from .norms import layer_norm
 from .optimizer import AdamBridge, AutoTuneConfig, LionBridge, OptiComputeAdamW
 from .precision import bytes_per_param
 
@@ -22,6 +24,12 @@ __all__ = [
     "StepStats",
     "bytes_per_param",
     "causal_lm_loss",
+    "layer_norm",
+    "Routing",
+    "route",
+    "dispatch",
+    "expert_mm",
+    "combine",
     "native",
     "precision",
     "__version__",

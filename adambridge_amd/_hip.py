@@ -122,6 +122,9 @@ EXPORTS = (
     "adambridge_convert_plane", "adambridge_capabilities", "adambridge_cross_entropy_work",
     "adambridge_cross_entropy", "adambridge_cross_entropy_backward", "adambridge_unpack_state",
     "adambridge_pack_state", "adambridge_matmul_work", "adambridge_matmul",
+    "adambridge_layer_norm", "adambridge_layer_norm_work", "adambridge_layer_norm_backward", "adambridge_route_work",
+    "adambridge_route", "adambridge_route_backward", "adambridge_dispatch", "adambridge_combine",
+    "adambridge_combine_backward", "adambridge_expert_mm", "adambridge_expert_mm_dx", "adambridge_expert_mm_dw",
 )
 
 
@@ -169,6 +172,18 @@ def open_library(path: Path = LIB_PATH) -> ctypes.CDLL:
         "adambridge_cross_entropy_work": (i64, [i64, i64]),
         "adambridge_cross_entropy": (ctypes.c_int, [vp, i32, vp, i64, i64, i64, vp, vp, vp]),
         "adambridge_cross_entropy_backward": (ctypes.c_int, [vp, i32, vp, i64, i64, i64, vp, vp, vp]),
+        "adambridge_layer_norm": (ctypes.c_int, [vp, i32, vp, vp, i32, i64, i64, ctypes.c_float, vp, vp]),
+        "adambridge_layer_norm_work": (i64, [i64, i64, i32]),
+        "adambridge_layer_norm_backward": (ctypes.c_int, [vp, vp, i32, vp, i32, vp, i64, i64, vp, vp, vp, vp]),
+        "adambridge_route_work": (i64, [i64, i64, i64]),
+        "adambridge_route": (ctypes.c_int, [vp, i32, i64, i64, i64, i32, vp, vp, vp, vp, vp, vp]),
+        "adambridge_route_backward": (ctypes.c_int, [vp, vp, vp, vp, i32, i64, i64, i64, i32, vp]),
+        "adambridge_dispatch": (ctypes.c_int, [vp, i32, vp, i64, i64, i64, vp]),
+        "adambridge_combine": (ctypes.c_int, [vp, i32, vp, vp, i64, i64, i64, vp]),
+        "adambridge_combine_backward": (ctypes.c_int, [vp, vp, i32, vp, vp, i64, i64, i64, vp, vp]),
+        "adambridge_expert_mm": (ctypes.c_int, [vp, vp, vp, vp, i32, i64, i64, i64, i64]),
+        "adambridge_expert_mm_dx": (ctypes.c_int, [vp, vp, vp, vp, i32, i64, i64, i64, i64]),
+        "adambridge_expert_mm_dw": (ctypes.c_int, [vp, vp, vp, vp, i32, i64, i64, i64, i64]),
     }
     for name in EXPORTS:
         fn = getattr(lib, name)
@@ -454,6 +469,155 @@ class HipKernels:
                       work.data_ptr())
         self._check(rc, "adambridge_matmul")
 
+    # -- expert blocks ---------------------------------------------------------
+
+    def _work(self, device: torch.device, name: str, *sizes) -> torch.Tensor | None:
+        """Scratch of the call ``name``_work gives the bytes of."""
+        nbytes = getattr(self._lib, name + "_work")(*sizes)
+        if nbytes < 0:
+            self._check(nbytes, name + "_work")
+        return torch.empty(-(-nbytes // 4), dtype=torch.int32, device=device) if nbytes else None
+
+    def layer_norm(self, x: torch.Tensor, weight: torch.Tensor | None, bias: torch.Tensor | None, eps: float,
+                   with_stats: bool) -> tuple[torch.Tensor, torch.Tensor | None]:
+        """Layer norm of contiguous [rows, cols] float32 or bfloat16 values on the current stream
+        (adambridge_layer_norm): the result and, ``with_stats``, the rows' mean and rstd."""
+        rows, cols = x.shape
+        self._operand("x", x, tuple(_DTYPE_CODES), (rows, cols), x.device)
+        w_dtype = x.dtype if weight is None and bias is None else (bias if weight is None else weight).dtype
+        for name, t in (("weight", weight), ("bias", bias)):
+            if t is not None:
+                self._operand(name, t, tuple(_DTYPE_CODES) if weight is None or t is weight else (w_dtype,), (cols,), x.device)
+        y = torch.empty_like(x)
+        stats = torch.empty(rows, 2, dtype=torch.float32, device=x.device) if with_stats else None
+        rc = self._on(x.device, self._lib.adambridge_layer_norm, x.data_ptr(), _DTYPE_CODES[x.dtype], _address(weight),
+                      _address(bias), _DTYPE_CODES[w_dtype], rows, cols, eps, y.data_ptr(), _address(stats))
+        self._check(rc, "adambridge_layer_norm")
+        return y, stats
+
+    def layer_norm_backward(self, gout: torch.Tensor, x: torch.Tensor, weight: torch.Tensor | None, stats: torch.Tensor,
+                            w_dtype: torch.dtype, wanted: tuple) -> tuple:
+        """The gradients of :meth:`layer_norm` to x, weight and bias (of ``w_dtype``), those ``wanted``
+        (adambridge_layer_norm_backward)."""
+        rows, cols = x.shape
+        self._operand("x", x, tuple(_DTYPE_CODES), (rows, cols), x.device)
+        self._operand("gout", gout, (x.dtype,), (rows, cols), x.device)
+        self._operand("stats", stats, (torch.float32,), (rows, 2), x.device)
+        if weight is not None:
+            self._operand("weight", weight, (w_dtype,), (cols,), x.device)
+        dx = torch.empty_like(x) if wanted[0] else None
+        dw, db = (torch.empty(cols, dtype=w_dtype, device=x.device) if want else None for want in wanted[1:])
+        work = self._work(x.device, "adambridge_layer_norm", rows, cols, _DTYPE_CODES[x.dtype]) if any(wanted[1:]) else None
+        rc = self._on(x.device, self._lib.adambridge_layer_norm_backward, gout.data_ptr(), x.data_ptr(), _DTYPE_CODES[x.dtype],
+                      _address(weight), _DTYPE_CODES[w_dtype], stats.data_ptr(), rows, cols, _address(dx), _address(dw),
+                      _address(db), _address(work))
+        self._check(rc, "adambridge_layer_norm_backward")
+        return dx, dw, db
+
+    def route(self, logits: torch.Tensor, top_k: int, normalize: bool) -> tuple:
+        """Weights, chosen experts, ends, order and position of contiguous [tokens, experts] logits
+        (adambridge_route)."""
+        tokens, experts = logits.shape
+        self._operand("logits", logits, tuple(_DTYPE_CODES), (tokens, experts), logits.device)
+        work = self._work(logits.device, "adambridge_route", tokens, experts, top_k)
+        weights = torch.empty(tokens, top_k, dtype=torch.float32, device=logits.device)
+        ints = torch.empty(3 * tokens * top_k + experts, dtype=torch.int32, device=logits.device)
+        n = tokens * top_k
+        chosen, position = ints[:n].view(tokens, top_k), ints[n:2 * n].view(tokens, top_k)
+        order, ends = ints[2 * n:3 * n], ints[3 * n:]
+        rc = self._on(logits.device, self._lib.adambridge_route, logits.data_ptr(), _DTYPE_CODES[logits.dtype], tokens, experts,
+                      top_k, int(normalize), weights.data_ptr(), chosen.data_ptr(), ends.data_ptr(), order.data_ptr(),
+                      position.data_ptr(), _address(work))
+        self._check(rc, "adambridge_route")
+        return weights, chosen, ends, order, position
+
+    def route_backward(self, weights: torch.Tensor, chosen: torch.Tensor, gout: torch.Tensor, logits: torch.Tensor | None,
+                       dtype: torch.dtype, experts: int, normalize: bool) -> torch.Tensor:
+        """The logits' gradient (of ``dtype``) from the weights' (adambridge_route_backward)."""
+        tokens, top_k = weights.shape
+        self._operand("weights", weights, (torch.float32,), (tokens, top_k), weights.device)
+        self._operand("gout", gout, (torch.float32,), (tokens, top_k), weights.device)
+        self._operand("chosen", chosen, (torch.int32,), (tokens, top_k), weights.device)
+        if not normalize:
+            self._operand("logits", logits, (dtype,), (tokens, experts), weights.device)
+        grad = torch.empty(tokens, experts, dtype=dtype, device=weights.device)
+        rc = self._on(weights.device, self._lib.adambridge_route_backward, weights.data_ptr(), chosen.data_ptr(), gout.data_ptr(),
+                      _address(logits), _DTYPE_CODES[dtype], tokens, experts, top_k, int(normalize), grad.data_ptr())
+        self._check(rc, "adambridge_route_backward")
+        return grad
+
+    def dispatch(self, x: torch.Tensor, position: torch.Tensor) -> torch.Tensor:
+        """The rows ``position`` [tokens, top_k] gives each token of contiguous [tokens, cols] values
+        (adambridge_dispatch)."""
+        (tokens, cols), top_k = x.shape, position.shape[1]
+        self._operand("x", x, tuple(_DTYPE_CODES), (tokens, cols), x.device)
+        self._operand("position", position, (torch.int32,), (tokens, top_k), x.device)
+        rows = torch.empty(tokens * top_k, cols, dtype=x.dtype, device=x.device)
+        rc = self._on(x.device, self._lib.adambridge_dispatch, x.data_ptr(), _DTYPE_CODES[x.dtype], position.data_ptr(), tokens,
+                      top_k, cols, rows.data_ptr())
+        self._check(rc, "adambridge_dispatch")
+        return rows
+
+    def combine(self, rows: torch.Tensor, weights: torch.Tensor | None, position: torch.Tensor) -> torch.Tensor:
+        """Each token's weighted sum of its rows (adambridge_combine)."""
+        (tokens, top_k), cols = position.shape, rows.shape[1]
+        self._operand("rows", rows, tuple(_DTYPE_CODES), (tokens * top_k, cols), rows.device)
+        self._operand("position", position, (torch.int32,), (tokens, top_k), rows.device)
+        if weights is not None:
+            self._operand("weights", weights, (torch.float32,), (tokens, top_k), rows.device)
+        out = torch.empty(tokens, cols, dtype=rows.dtype, device=rows.device)
+        rc = self._on(rows.device, self._lib.adambridge_combine, rows.data_ptr(), _DTYPE_CODES[rows.dtype], _address(weights),
+                      position.data_ptr(), tokens, top_k, cols, out.data_ptr())
+        self._check(rc, "adambridge_combine")
+        return out
+
+    def combine_backward(self, gout: torch.Tensor, rows: torch.Tensor | None, weights: torch.Tensor, position: torch.Tensor,
+                         wanted: tuple) -> tuple:
+        """The gradients of :meth:`combine` to the rows and to the weights (which take ``rows``), those
+        ``wanted`` (adambridge_combine_backward)."""
+        (tokens, top_k), cols = position.shape, gout.shape[1]
+        self._operand("gout", gout, tuple(_DTYPE_CODES), (tokens, cols), gout.device)
+        self._operand("position", position, (torch.int32,), (tokens, top_k), gout.device)
+        self._operand("weights", weights, (torch.float32,), (tokens, top_k), gout.device)
+        if wanted[1]:
+            self._operand("rows", rows, (gout.dtype,), (tokens * top_k, cols), gout.device)
+        drows = torch.empty(tokens * top_k, cols, dtype=gout.dtype, device=gout.device) if wanted[0] else None
+        dweights = torch.empty_like(weights) if wanted[1] else None
+        rc = self._on(gout.device, self._lib.adambridge_combine_backward, gout.data_ptr(), _address(rows), _DTYPE_CODES[gout.dtype],
+                      weights.data_ptr(), position.data_ptr(), tokens, top_k, cols, _address(drows), _address(dweights))
+        self._check(rc, "adambridge_combine_backward")
+        return drows, dweights
+
+    def expert_mm(self, x: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
+        """Each expert's contiguous rows times its weights' transpose (adambridge_expert_mm)."""
+        (experts, n, k), rows = weight.shape, x.shape[0]
+        out = torch.empty(rows, n, dtype=x.dtype, device=x.device)
+        self._expert("adambridge_expert_mm", ("x", x, (rows, k)), ("weight", weight, (experts, n, k)), ends, out, experts, n, k)
+        return out
+
+    def expert_mm_backward(self, gout: torch.Tensor, x: torch.Tensor | None, weight: torch.Tensor, ends: torch.Tensor,
+                           wanted: tuple) -> tuple:
+        """The gradients of :meth:`expert_mm` to x and to the weights (which take ``x``), those ``wanted``
+        (adambridge_expert_mm_dx, adambridge_expert_mm_dw)."""
+        (experts, n, k), rows = weight.shape, gout.shape[0]
+        dx = dw = None
+        if wanted[0]:
+            dx = torch.empty(rows, k, dtype=gout.dtype, device=gout.device)
+            self._expert("adambridge_expert_mm_dx", ("gout", gout, (rows, n)), ("weight", weight, (experts, n, k)), ends, dx,
+                         experts, n, k)
+        if wanted[1]:
+            dw = torch.empty(experts, n, k, dtype=gout.dtype, device=gout.device)
+            self._expert("adambridge_expert_mm_dw", ("gout", gout, (rows, n)), ("x", x, (rows, k)), ends, dw, experts, n, k)
+        return dx, dw
+
+    def _expert(self, name: str, a: tuple, b: tuple, ends: torch.Tensor, out: torch.Tensor, experts: int, n: int, k: int) -> None:
+        for what, t, shape in (a, b):
+            self._operand(what, t, tuple(_DTYPE_CODES) if t is a[1] else (a[1].dtype,), shape, out.device)
+        self._operand("ends", ends, (torch.int32,), (experts,), out.device)
+        rc = self._on(out.device, getattr(self._lib, name), a[1].data_ptr(), b[1].data_ptr(), ends.data_ptr(), out.data_ptr(),
+                      _DTYPE_CODES[out.dtype], a[1].shape[0], experts, n, k)
+        self._check(rc, name)
+
     def fused_adamw(self, master: torch.Tensor, grad: torch.Tensor, m: torch.Tensor, v: torch.Tensor,
                     out: torch.Tensor | None, hp: HParams, lo: int, hi: int) -> None:
         """Update elements ``[lo, hi)`` of flat contiguous device tensors in place, synchronously
@@ -495,6 +659,10 @@ class HipKernels:
         if rc != 0:
             detail = self.last_error() if rc in (-20, -22) else ""   # codes that set the error text
             raise RuntimeError(f"{what} rejected the update (code {rc}){': ' + detail if detail else ''}")
+
+
+def _address(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 def _stream_handle(stream) -> int | None:

@@ -1,0 +1,517 @@
+// abh_route.hip -- tokens to experts and back: the router's choice, the order of the chosen, and the rows'
+// way there (dispatch) and back (combine).
+//
+// A token's top_k largest logits are chosen (the lower index of equal ones; a NaN counts as the largest), and
+// their weights are the softmax over the chosen or over all.  The T k assignments, token by token, are sorted by
+// expert, stably, so that an expert's rows lie together in the tokens' order:
+//
+//   ends[e]      = how many assignments have experts 0 .. e
+//   order[r]     = the assignment t k + j that row r is
+//   position[t, j] = its row
+//
+// Bytes bound all of it: the logits once; x once and its k copies; k rows and their sum.  Nothing depends on
+// the order of atomics: 64 tokens are a block, an expert's tokens in a block are one 64-bit mask (set by or, whose order
+// does not matter), a token's rank among them the bits below its own, and the blocks' counts are summed
+// in order.  Up to 64 tokens are one launch; more are three: choice and counts, the counts' prefix
+// sums, and the places.
+
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "../../include/adambridge_hip.h"
+#include "abh_device.hpp"
+#include "abh_host.hpp"
+#include "abh_rows.hpp"
+
+namespace abh {
+
+constexpr int kBlockTokens = 64;
+constexpr int kRouteThreads = 256;
+constexpr int kMostExperts = 1024;
+constexpr int kMostChosen = 64;
+constexpr float kRouteLog2e = 1.4426950408889634f;
+constexpr float kRouteNegInf = -__builtin_inff();
+
+struct RouteArgs {
+    const void* logits;
+    int64_t tokens;
+    int32_t experts, top_k, normalize, blocks;
+    float* weights;      // tokens x top_k
+    int32_t* chosen;     // tokens x top_k
+    int32_t* ends;       // experts
+    int32_t* order;      // tokens top_k
+    int32_t* position;   // tokens x top_k
+    uint8_t* counts;     // experts x blocks
+    int32_t* bases;      // experts x blocks
+};
+
+// A total order of floats as integers: -inf lowest but 0 (nothing), +0 and -0 equal, NaN above all.
+__device__ __forceinline__ uint32_t order_key(float x)
+{
+    if (x != x) return 0xffffffffu;
+    const uint32_t u = fbits(x + 0.0f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// exp(x - m) with m = -inf taken as 0, so that a row without any finite logit has weights 0 and not NaN.
+__device__ __forceinline__ float exp_below(float x, float m)
+{
+    return __builtin_amdgcn_exp2f((x - (m == kRouteNegInf ? 0.0f : m)) * kRouteLog2e);
+}
+
+template <int G>
+__device__ __forceinline__ uint32_t group_max(uint32_t x)
+{
+#pragma unroll
+    for (int d = 1; d < G; d *= 2) {
+        const uint32_t y = (uint32_t)__shfl_xor((int)x, d);
+        x = x > y ? x : y;
+    }
+    return x;
+}
+
+template <int G>
+__device__ __forceinline__ float group_sum(float x)
+{
+#pragma unroll
+    for (int d = 1; d < G; d *= 2) x += __shfl_xor(x, d);
+    return x;
+}
+
+// Masks of a block's tokens by expert, and the rows of its assignments: base[e] + the bits below.
+__device__ __forceinline__ void place_block(const RouteArgs& A, const uint64_t* mask, const int32_t* base, int64_t base_stride,
+                                            int64_t t0, int tokens)
+{
+    for (int i = threadIdx.x; i < tokens * A.top_k; i += kRouteThreads) {
+        const int64_t a = t0 * A.top_k + i;
+        const int e = A.chosen[a], t = i / A.top_k;
+        const int row = base[(int64_t)e * base_stride] + __builtin_popcountll(mask[e] & (((uint64_t)1 << t) - 1));
+        A.position[a] = row;
+        A.order[row] = (int32_t)a;
+    }
+}
+
+// 64 tokens a workgroup, G lanes a token, NV logits a lane (expert lane * NV + v).
+template <int DT, int G, int NV>
+__global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs A)
+{
+    __shared__ uint64_t mask[kMostExperts];
+    __shared__ int32_t base[kMostExperts];
+    constexpr int kPass = kRouteThreads / G;   // tokens at a time
+    const int lane = threadIdx.x % G, sub = threadIdx.x / G;
+    const int64_t t0 = (int64_t)blockIdx.x * kBlockTokens;
+    const int tokens = (int)(A.tokens - t0 < kBlockTokens ? A.tokens - t0 : kBlockTokens);
+    for (int e = threadIdx.x; e < A.experts; e += kRouteThreads) mask[e] = 0;
+    __syncthreads();
+    for (int t = sub; t < kBlockTokens; t += kPass) {   // the same for all lanes: whole groups take part in the sums
+        const bool real = t < tokens;
+        float x[NV];
+        uint32_t key[NV];
+        const int64_t row = (t0 + (real ? t : 0)) * A.experts;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+            const int e = lane * NV + v;
+            x[v] = e < A.experts ? get<DT>(A.logits, row + e) : kRouteNegInf;
+            key[v] = e < A.experts ? order_key(x[v]) : 0u;
+        }
+        float top = 0.0f, sum = 0.0f, mine = 0.0f;
+        int my_expert = 0;
+        for (int j = 0; j < A.top_k; ++j) {
+            uint32_t best = key[0];
+            float value = x[0];
+            int at_v = 0;
+#pragma unroll
+            for (int v = 1; v < NV; ++v) {
+                const bool more = key[v] > best;   // equal: the lower index stays
+                best = more ? key[v] : best;
+                value = more ? x[v] : value;
+                at_v = more ? v : at_v;
+            }
+            const uint32_t most = group_max<G>(best);
+            const uint64_t holders = __builtin_amdgcn_ballot_w64(best == most) >> ((threadIdx.x & 63) / G * G);
+            const int winner = __builtin_ctzll(holders);   // the lowest lane of this group that holds it
+            const int e = __shfl(lane * NV + at_v, winner, G);
+            value = __shfl(value, winner, G);
+#pragma unroll
+            for (int v = 0; v < NV; ++v) key[v] = lane * NV + v == e ? 0u : key[v];
+            if (j == 0) {
+                top = value;
+                if (!A.normalize) {   // the sum over all experts
+#pragma unroll
+                    for (int v = 0; v < NV; ++v) sum += exp_below(x[v], top);
+                    sum = group_sum<G>(sum);
+                }
+            }
+            const float w = exp_below(value, top);
+            if (A.normalize) sum += w;
+            if (lane == j) {
+                mine = w;
+                my_expert = e;
+            }
+        }
+        if (real && lane < A.top_k) {
+            const int64_t a = (t0 + t) * A.top_k + lane;
+            A.weights[a] = top == kRouteNegInf ? 0.0f : mine / sum;
+            A.chosen[a] = my_expert;
+            atomicOr(reinterpret_cast<unsigned long long*>(&mask[my_expert]), 1ull << t);
+        }
+    }
+    __syncthreads();
+    if (A.blocks > 1) {
+        for (int e = threadIdx.x; e < A.experts; e += kRouteThreads)
+            A.counts[(int64_t)e * A.blocks + blockIdx.x] = (uint8_t)__builtin_popcountll(mask[e]);
+        return;
+    }
+    if (threadIdx.x < kWave) {   // one wavefront sums the experts' counts
+        int32_t before = 0;
+        for (int e0 = 0; e0 < A.experts; e0 += kWave) {
+            const int e = e0 + (int)threadIdx.x;
+            const int32_t n = e < A.experts ? (int32_t)__builtin_popcountll(mask[e]) : 0;
+            int32_t s = n;
+#pragma unroll
+            for (int d = 1; d < kWave; d *= 2) {
+                const int32_t y = __shfl_up(s, d);
+                if ((int)threadIdx.x >= d) s += y;
+            }
+            if (e < A.experts) {
+                base[e] = before + s - n;
+                A.ends[e] = before + s;
+            }
+            before += __shfl(s, kWave - 1);
+        }
+    }
+    __threadfence_block();
+    __syncthreads();
+    place_block(A, mask, base, 1, t0, tokens);
+}
+
+// One expert a workgroup: the rows of the experts before it, then its blocks' prefix sums.
+__global__ __launch_bounds__(1024) void k_route_bases(RouteArgs A)
+{
+    constexpr int T = 1024;
+    __shared__ int32_t part[T / kWave];
+    const int e = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
+    // bytes 0 .. e * blocks, four at a time where they are aligned (the array is)
+    const int64_t n = (int64_t)e * A.blocks;
+    int32_t s = 0;
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(A.counts);
+    for (int64_t i = threadIdx.x; i < n / 4; i += T) {
+        const uint32_t w = words[i];
+        s += (int32_t)((w & 255u) + (w >> 8 & 255u) + (w >> 16 & 255u) + (w >> 24));
+    }
+    for (int64_t i = n / 4 * 4 + threadIdx.x; i < n; i += T) s += A.counts[i];
+#pragma unroll
+    for (int d = 1; d < kWave; d *= 2) s += __shfl_xor(s, d);
+    if (lane == 0) part[wave] = s;
+    __syncthreads();
+    int32_t before = 0;
+    for (int w = 0; w < T / kWave; ++w) before += part[w];
+    for (int b0 = 0; b0 < A.blocks; b0 += T) {
+        const int b = b0 + (int)threadIdx.x;
+        const int32_t c = b < A.blocks ? A.counts[n + b] : 0;
+        int32_t x = c;
+#pragma unroll
+        for (int d = 1; d < kWave; d *= 2) {
+            const int32_t y = __shfl_up(x, d);
+            if (lane >= d) x += y;
+        }
+        __syncthreads();
+        if (lane == kWave - 1) part[wave] = x;
+        __syncthreads();
+        int32_t waves = 0, all = 0;
+        for (int w = 0; w < T / kWave; ++w) {
+            if (w < wave) waves += part[w];
+            all += part[w];
+        }
+        if (b < A.blocks) A.bases[n + b] = before + waves + x - c;
+        before += all;
+    }
+    if (threadIdx.x == 0) A.ends[e] = before;
+}
+
+__global__ __launch_bounds__(kRouteThreads) void k_route_places(RouteArgs A)
+{
+    __shared__ uint64_t mask[kMostExperts];
+    const int64_t t0 = (int64_t)blockIdx.x * kBlockTokens;
+    const int tokens = (int)(A.tokens - t0 < kBlockTokens ? A.tokens - t0 : kBlockTokens);
+    for (int e = threadIdx.x; e < A.experts; e += kRouteThreads) mask[e] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < tokens * A.top_k; i += kRouteThreads)
+        atomicOr(reinterpret_cast<unsigned long long*>(&mask[A.chosen[t0 * A.top_k + i]]), 1ull << (i / A.top_k));
+    __syncthreads();
+    place_block(A, mask, A.bases + blockIdx.x, A.blocks, t0, tokens);
+}
+
+// dlogits of the chosen's softmax, w_j (g_j - sum w g), or of all's, p_e ([e = chosen_j] g_j - sum p g).
+// A wavefront a token.
+template <int DT>
+__global__ __launch_bounds__(256) void k_route_back(const float* weights, const int32_t* chosen, const float* gout,
+                                                    const void* logits, int64_t tokens, int32_t experts, int32_t top_k,
+                                                    int32_t normalize, void* grad)
+{
+    const int lane = threadIdx.x & 63;
+    const int64_t t = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+    if (t >= tokens) return;
+    const float w = lane < top_k ? weights[t * top_k + lane] : 0.0f;
+    const float g = lane < top_k ? gout[t * top_k + lane] : 0.0f;
+    const int at = lane < top_k ? chosen[t * top_k + lane] : -1;
+    const float total = wave_sum(lane < top_k ? w * g : 0.0f);
+    const int64_t row = t * experts;
+    float top = 0.0f, inv = 0.0f;
+    if (!normalize) {
+        float most = kRouteNegInf, sum = 0.0f;
+        bool nan = false;
+        for (int e = lane; e < experts; e += kWave) {
+            const float x = get<DT>(logits, row + e);
+            most = __builtin_fmaxf(most, x);
+            nan |= x != x;
+        }
+#pragma unroll
+        for (int d = 1; d < kWave; d *= 2) most = __builtin_fmaxf(most, __shfl_xor(most, d));
+        top = __builtin_amdgcn_ballot_w64(nan) ? __builtin_nanf("") : most;
+        for (int e = lane; e < experts; e += kWave) sum += exp_below(get<DT>(logits, row + e), top);
+        sum = wave_sum(sum);
+        inv = top == kRouteNegInf ? 0.0f : 1.0f / sum;
+    }
+    for (int e0 = 0; e0 < experts; e0 += kWave) {
+        const int e = e0 + lane;
+        float seed = 0.0f;   // w g of the assignment to e, if there is one
+        float own = 0.0f;
+        for (int j = 0; j < top_k; ++j) {
+            const int c = __shfl(at, j);
+            const float wj = __shfl(w, j), gj = __shfl(g, j);
+            if (c == e) {
+                seed = wj * gj;
+                own = wj;
+            }
+        }
+        if (e >= experts) continue;
+        if (!normalize) own = exp_below(get<DT>(logits, row + e), top) * inv;
+        put<DT>(grad, row + e, seed - own * total);
+    }
+}
+
+// ---------------------------------------------------------------- dispatch and combine
+
+struct ShuffleArgs {
+    const void* x;            // tokens x cols, or rows x cols
+    const void* g;
+    const float* weights;     // tokens x top_k
+    const int32_t* position;  // tokens x top_k
+    void* out;
+    float* dw;
+    int64_t tokens, cols;
+    int32_t top_k;
+};
+
+// The row of an assignment; -1 where it is none (a position that no routing gives): nothing is read or written there.
+__device__ __forceinline__ int64_t row_of(const ShuffleArgs& A, int64_t a)
+{
+    const int64_t r = A.position[a];
+    return r >= 0 && r < A.tokens * A.top_k ? r : -1;
+}
+
+// out[position[t, j]] = x[t]: the token's row read once, written top_k times.  A wavefront takes 64 vectors of a token.
+template <int DT>
+__global__ __launch_bounds__(256) void k_dispatch(ShuffleArgs A)
+{
+    constexpr int K = kLane<DT>;
+    const int64_t t = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+    const int64_t c = ((int64_t)blockIdx.y * kWave + (threadIdx.x & 63)) * K;
+    if (t >= A.tokens || c >= A.cols) return;
+    float v[K];
+    load_vec<DT>(at<DT>(A.x, t * A.cols), c, A.cols, v);
+    for (int j = 0; j < A.top_k; ++j) {
+        const int64_t r = row_of(A, t * A.top_k + j);
+        if (r >= 0) store_vec<DT>(at<DT>(A.out, r * A.cols), c, A.cols, v);
+    }
+}
+
+// out[t] = sum over j of weights[t, j] x[position[t, j]] (without weights: of the rows), in order, rounded once.
+template <int DT>
+__global__ __launch_bounds__(256) void k_combine(ShuffleArgs A)
+{
+    constexpr int K = kLane<DT>;
+    const int64_t t = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+    const int64_t c = ((int64_t)blockIdx.y * kWave + (threadIdx.x & 63)) * K;
+    if (t >= A.tokens || c >= A.cols) return;
+    float s[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) s[k] = 0.0f;
+    for (int j = 0; j < A.top_k; ++j) {
+        const int64_t a = t * A.top_k + j, r = row_of(A, a);
+        if (r < 0) continue;
+        const float w = A.weights ? A.weights[a] : 1.0f;
+        float v[K];
+        load_vec<DT>(at<DT>(A.x, r * A.cols), c, A.cols, v);
+#pragma unroll
+        for (int k = 0; k < K; ++k) s[k] = __builtin_fmaf(w, v[k], s[k]);
+    }
+    store_vec<DT>(at<DT>(A.out, t * A.cols), c, A.cols, s);
+}
+
+// An assignment a wavefront: out[row] = w g[t], dw = <g[t], x[row]>.
+template <int DT>
+__global__ __launch_bounds__(256) void k_combine_back(ShuffleArgs A)
+{
+    constexpr int K = kLane<DT>;
+    const int lane = threadIdx.x & 63;
+    const int64_t a = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+    if (a >= A.tokens * A.top_k) return;
+    const int64_t t = a / A.top_k, r = row_of(A, a);
+    float dot = 0.0f;
+    if (r >= 0) {
+        const float w = A.weights[a];
+        for (int64_t c = (int64_t)lane * K; c < A.cols; c += kWave * K) {
+            float g[K], v[K];
+            load_vec<DT>(at<DT>(A.g, t * A.cols), c, A.cols, g);
+            if (A.dw) {
+                load_vec<DT>(at<DT>(A.x, r * A.cols), c, A.cols, v);
+#pragma unroll
+                for (int k = 0; k < K; ++k) dot = __builtin_fmaf(g[k], v[k], dot);
+            }
+            if (A.out) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) g[k] *= w;
+                store_vec<DT>(at<DT>(A.out, r * A.cols), c, A.cols, g);
+            }
+        }
+    }
+    if (A.dw) {
+        dot = wave_sum(dot);
+        if (lane == 0) A.dw[a] = dot;
+    }
+}
+
+static bool route_type_ok(int32_t t) { return t == ADAMBRIDGE_DT_F32 || t == ADAMBRIDGE_DT_BF16; }
+
+static int route_sizes(int64_t tokens, int64_t experts, int64_t top_k)
+{
+    const int64_t most = ((int64_t)1 << 31) - 1;
+    return tokens >= 1 && tokens <= most && experts >= 1 && experts <= kMostExperts && top_k >= 1 && top_k <= kMostChosen &&
+           top_k <= experts && tokens * top_k <= most ? 0 : ADAMBRIDGE_EBADN;
+}
+
+template <int DT>
+static void launch_route(const RouteArgs& A)
+{
+    // a token's lanes: 16 while its logits and its choices fit them, so that four tokens share a wavefront
+#define ABH_ROUTE(G, NV)                                                                                        \
+    if (A.experts <= G * NV && A.top_k <= G) {                                                                  \
+        hipLaunchKernelGGL((k_route<DT, G, NV>), dim3(A.blocks), dim3(kRouteThreads), 0, t_stream, A);           \
+        return;                                                                                                 \
+    }
+    ABH_ROUTE(16, 1) ABH_ROUTE(16, 2) ABH_ROUTE(16, 4) ABH_ROUTE(32, 4) ABH_ROUTE(64, 4) ABH_ROUTE(64, 16)
+#undef ABH_ROUTE
+}
+
+static int done(const char* what)
+{
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? 0 : hip_fail(e, what);
+}
+
+static int shuffle_check(const void* a, const void* out, const int32_t* position, int32_t dtype, int64_t tokens, int64_t top_k,
+                         int64_t cols)
+{
+    const int rc = route_sizes(tokens, kMostExperts, top_k);
+    if (rc || cols < 1 || cols > (int64_t)1 << 22) return ADAMBRIDGE_EBADN;
+    if (!route_type_ok(dtype)) return ADAMBRIDGE_EMVDTYPE;
+    return a && out && position ? 0 : ADAMBRIDGE_ENULL;
+}
+
+static dim3 shuffle_grid(const ShuffleArgs& A, int32_t dtype)
+{
+    const int64_t a_wave = kWave * (dtype == ADAMBRIDGE_DT_BF16 ? kLane<DT_BF16> : kLane<DT_F32>);
+    return dim3((unsigned)((A.tokens + 3) / 4), (unsigned)((A.cols + a_wave - 1) / a_wave));
+}
+
+}  // namespace abh
+
+using namespace abh;
+
+extern "C" {
+
+ADAMBRIDGE_API int64_t adambridge_route_work(int64_t tokens, int64_t experts, int64_t top_k)
+{
+    if (route_sizes(tokens, experts, top_k)) return ADAMBRIDGE_EBADN;
+    const int64_t blocks = (tokens + kBlockTokens - 1) / kBlockTokens;
+    return blocks == 1 ? 0 : (experts * blocks + 3) / 4 * 4 + experts * blocks * 4;
+}
+
+ADAMBRIDGE_API int adambridge_route(const void* logits, int32_t dtype, int64_t tokens, int64_t experts, int64_t top_k,
+                                    int32_t normalize, float* weights, int32_t* chosen, int32_t* ends, int32_t* order,
+                                    int32_t* position, void* work)
+{
+    if (route_sizes(tokens, experts, top_k)) return ADAMBRIDGE_EBADN;
+    if (!route_type_ok(dtype)) return ADAMBRIDGE_EMVDTYPE;
+    const int64_t blocks = (tokens + kBlockTokens - 1) / kBlockTokens;
+    if (!logits || !weights || !chosen || !ends || !order || !position || (blocks > 1 && !work)) return ADAMBRIDGE_ENULL;
+    if ((uintptr_t)work % 4) return ADAMBRIDGE_EALIGN;
+    RouteArgs A{logits, tokens, (int32_t)experts, (int32_t)top_k, normalize != 0, (int32_t)blocks, weights, chosen, ends, order,
+                position, static_cast<uint8_t*>(work), nullptr};
+    if (blocks > 1) A.bases = reinterpret_cast<int32_t*>(A.counts + (experts * blocks + 3) / 4 * 4);
+    if (dtype == ADAMBRIDGE_DT_BF16) launch_route<DT_BF16>(A);
+    else launch_route<DT_F32>(A);
+    if (blocks > 1) {
+        hipLaunchKernelGGL(k_route_bases, dim3((unsigned)experts), dim3(1024), 0, t_stream, A);
+        hipLaunchKernelGGL(k_route_places, dim3((unsigned)blocks), dim3(kRouteThreads), 0, t_stream, A);
+    }
+    return done("hipLaunchKernelGGL (route)");
+}
+
+ADAMBRIDGE_API int adambridge_route_backward(const float* weights, const int32_t* chosen, const float* gout, const void* logits,
+                                             int32_t dtype, int64_t tokens, int64_t experts, int64_t top_k, int32_t normalize,
+                                             void* grad)
+{
+    if (route_sizes(tokens, experts, top_k)) return ADAMBRIDGE_EBADN;
+    if (!route_type_ok(dtype)) return ADAMBRIDGE_EMVDTYPE;
+    if (!weights || !chosen || !gout || !grad || (!normalize && !logits)) return ADAMBRIDGE_ENULL;
+    const dim3 grid((unsigned)((tokens + 3) / 4));
+    if (dtype == ADAMBRIDGE_DT_BF16)
+        hipLaunchKernelGGL((k_route_back<DT_BF16>), grid, dim3(256), 0, t_stream, weights, chosen, gout, logits, tokens,
+                           (int32_t)experts, (int32_t)top_k, normalize, grad);
+    else
+        hipLaunchKernelGGL((k_route_back<DT_F32>), grid, dim3(256), 0, t_stream, weights, chosen, gout, logits, tokens,
+                           (int32_t)experts, (int32_t)top_k, normalize, grad);
+    return done("hipLaunchKernelGGL (route's gradient)");
+}
+
+ADAMBRIDGE_API int adambridge_dispatch(const void* x, int32_t dtype, const int32_t* position, int64_t tokens, int64_t top_k,
+                                       int64_t cols, void* rows)
+{
+    if (const int rc = shuffle_check(x, rows, position, dtype, tokens, top_k, cols)) return rc;
+    const ShuffleArgs A{x, nullptr, nullptr, position, rows, nullptr, tokens, cols, (int32_t)top_k};
+    if (dtype == ADAMBRIDGE_DT_BF16) hipLaunchKernelGGL((k_dispatch<DT_BF16>), shuffle_grid(A, dtype), dim3(256), 0, t_stream, A);
+    else hipLaunchKernelGGL((k_dispatch<DT_F32>), shuffle_grid(A, dtype), dim3(256), 0, t_stream, A);
+    return done("hipLaunchKernelGGL (dispatch)");
+}
+
+ADAMBRIDGE_API int adambridge_combine(const void* rows, int32_t dtype, const float* weights, const int32_t* position,
+                                      int64_t tokens, int64_t top_k, int64_t cols, void* out)
+{
+    if (const int rc = shuffle_check(rows, out, position, dtype, tokens, top_k, cols)) return rc;
+    const ShuffleArgs A{rows, nullptr, weights, position, out, nullptr, tokens, cols, (int32_t)top_k};
+    if (dtype == ADAMBRIDGE_DT_BF16) hipLaunchKernelGGL((k_combine<DT_BF16>), shuffle_grid(A, dtype), dim3(256), 0, t_stream, A);
+    else hipLaunchKernelGGL((k_combine<DT_F32>), shuffle_grid(A, dtype), dim3(256), 0, t_stream, A);
+    return done("hipLaunchKernelGGL (combine)");
+}
+
+ADAMBRIDGE_API int adambridge_combine_backward(const void* gout, const void* rows, int32_t dtype, const float* weights,
+                                               const int32_t* position, int64_t tokens, int64_t top_k, int64_t cols, void* drows,
+                                               float* dweights)
+{
+    if (const int rc = shuffle_check(gout, weights, position, dtype, tokens, top_k, cols)) return rc;
+    if (dweights && !rows) return ADAMBRIDGE_ENULL;
+    if (!drows && !dweights) return 0;
+    const ShuffleArgs A{rows, gout, weights, position, drows, dweights, tokens, cols, (int32_t)top_k};
+    const dim3 grid((unsigned)((tokens * top_k + 3) / 4));
+    if (dtype == ADAMBRIDGE_DT_BF16) hipLaunchKernelGGL((k_combine_back<DT_BF16>), grid, dim3(256), 0, t_stream, A);
+    else hipLaunchKernelGGL((k_combine_back<DT_F32>), grid, dim3(256), 0, t_stream, A);
+    return done("hipLaunchKernelGGL (combine's gradient)");
+}
+
+}  // extern "C"

@@ -1,0 +1,298 @@
+"""Expert layers: the router's choice, the rows' way to the experts and back, and the experts' products.
+
+An expert MLP of ``top_k`` experts a token is::
+
+    r = route(x @ router.T, top_k)                  # which experts, with what weights, in what order
+    rows = dispatch(x, r)                           # [tokens * top_k, hidden], sorted by expert
+    rows = expert_mm(F.gelu(expert_mm(rows, up, r.ends)), down, r.ends)
+    y = combine(rows, r)                            # each token's weighted sum
+
+Nothing of it waits for the device: how many rows an expert has is read there (``r.ends``).  On plain GPU
+tensors of float32 or bfloat16 the library's kernels compute it (csrc/abh_route.hip, csrc/abh_experts.hip);
+elsewhere, and where an operation is traced, transformed or differentiated twice, torch operations do.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _hip
+from .losses import _observed, _plain_backward
+from .norms import plain
+
+__all__ = ["Routing", "route", "dispatch", "expert_mm", "combine"]
+
+_MOST_EXPERTS, _MOST_CHOSEN, _MOST_ASSIGNED = 1024, 64, (1 << 31) - 1   # adambridge_route's
+_MOST_ROWS, _MOST_SIZE, _MOST_MM_EXPERTS = 1 << 30, 1 << 22, 4096       # adambridge_expert_mm's
+
+
+class Routing(NamedTuple):
+    """Where tokens go.  The assignments ``(t, j)``, numbered ``t * top_k + j``, are sorted by expert, stably.
+
+    ``weights``: ``[tokens, top_k]`` float32 (float64 from float64 logits), differentiable; ``experts``: ``[tokens, top_k]``, largest weight first;
+    ``ends``: ``[experts]``, one past each expert's last row; ``order``: ``[tokens * top_k]``, the assignment
+    that is each row; ``position``: ``[tokens, top_k]``, each assignment's row.  The last four are int32."""
+
+    weights: torch.Tensor
+    experts: torch.Tensor
+    ends: torch.Tensor
+    order: torch.Tensor
+    position: torch.Tensor
+
+
+# ----------------------------------------------------------------------- route
+
+def _torch_route(logits, top_k, normalize):
+    """The definition in torch operations."""
+    wide = logits.to(torch.promote_types(logits.dtype, torch.float32))
+    tokens, experts = wide.shape
+    chosen = torch.sort(wide.detach() + 0.0, dim=1, descending=True, stable=True).indices[:, :top_k]
+    values = torch.gather(wide, 1, chosen)
+    top = values[:, :1].detach()
+    shift = torch.where(top == -torch.inf, 0.0, top)   # a row without any finite logit: weights 0
+    e = torch.exp(values - shift)
+    total = (e if normalize else torch.exp(wide - shift)).sum(1, keepdim=True)
+    weights = e / torch.where(total == 0.0, 1.0, total)
+    flat = chosen.reshape(-1)
+    order = torch.sort(flat, stable=True).indices
+    at = torch.arange(tokens * top_k, device=logits.device)
+    position = torch.empty_like(order).scatter_(0, order, at).view(tokens, top_k)
+    ends = torch.zeros(experts, dtype=torch.int64, device=logits.device).scatter_add_(0, flat, torch.ones_like(flat)).cumsum(0)
+    return Routing(weights, chosen.int(), ends.int(), order.int(), position.int())
+
+
+class _Route(torch.autograd.Function):
+    """Keeps the weights and the choice, and the logits if the softmax is over all of them."""
+
+    @staticmethod
+    def forward(ctx, logits, top_k, normalize):
+        out = _hip.load().route(logits, top_k, normalize)
+        ctx.mark_non_differentiable(*out[1:])
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(out[0], out[1], None if normalize else logits)
+        ctx.dtype, ctx.experts, ctx.normalize = logits.dtype, logits.shape[1], normalize
+        return out
+
+    @staticmethod
+    def backward(ctx, gout, *_):
+        weights, chosen, logits = ctx.saved_tensors
+        if gout is None:
+            return None, None, None
+        if _plain_backward(gout):
+            return _hip.load().route_backward(weights, chosen, gout.contiguous(), logits, ctx.dtype, ctx.experts,
+                                              ctx.normalize), None, None
+        seed = weights * gout
+        total = seed.sum(1, keepdim=True)
+        spread = weights.new_zeros(weights.shape[0], ctx.experts)
+        if ctx.normalize:
+            return spread.scatter(1, chosen.long(), seed - weights * total).to(ctx.dtype), None, None
+        wide = logits.float()
+        top = wide.detach().amax(1, keepdim=True)
+        e = torch.exp(wide - torch.where(top == -torch.inf, 0.0, top))
+        norm = e.sum(1, keepdim=True)
+        p = e / torch.where(norm == 0.0, 1.0, norm)
+        return (spread.scatter(1, chosen.long(), seed) - p * total).to(ctx.dtype), None, None
+
+
+@torch.compiler.disable
+def route(logits: torch.Tensor, top_k: int, normalize: bool = True) -> Routing:
+    """The ``top_k`` largest of each token's ``logits`` (``[tokens, experts]``; the lower index of equal ones, a NaN
+    counting as the largest), their softmax weights -- over the chosen if ``normalize``, else over all experts --
+    and the order of the assignments by expert.
+
+    An expert masked by ``-inf`` has weight 0 and is chosen only where nothing else is left; a token all of
+    whose logits are ``-inf`` has weights 0 and no gradient."""
+    if logits.dim() != 2 or not logits.is_floating_point() or logits.shape[1] < 1:
+        raise ValueError(f"logits must be floating-point [tokens, experts], got {logits.dtype} {tuple(logits.shape)}")
+    tokens, experts = logits.shape
+    if isinstance(top_k, bool) or not isinstance(top_k, int) or not 1 <= top_k <= experts:
+        raise ValueError(f"top_k must be an int from 1 to the number of experts, {experts}, got {top_k!r}")
+    if tokens * top_k > _MOST_ASSIGNED:
+        raise ValueError(f"tokens * top_k must be below 2^31, got {tokens * top_k}")
+    if not plain(logits) or not tokens or experts > _MOST_EXPERTS or top_k > _MOST_CHOSEN or _observed():
+        return _torch_route(logits, top_k, normalize)
+    logits = logits.contiguous()
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return Routing(*_Route.apply(logits, top_k, bool(normalize)))
+    return Routing(*_hip.load().route(logits, top_k, normalize))
+
+
+# -------------------------------------------------------- dispatch and combine
+
+def _checked_position(name: str, routing: Routing, device: torch.device) -> tuple[int, int]:
+    position = routing.position
+    if position.dim() != 2 or position.dtype != torch.int32 or position.device != device:
+        raise ValueError(f"the routing's position must be int32 [tokens, top_k] on {name}'s device, {device}, got "
+                         f"{position.dtype} {tuple(position.shape)} on {position.device}")
+    if not 1 <= position.shape[1]:
+        raise ValueError("the routing assigns no rows")
+    return position.shape
+
+
+def _fits(tokens: int, top_k: int, cols: int) -> bool:
+    return tokens > 0 and top_k <= _MOST_CHOSEN and 0 < cols <= _MOST_SIZE and tokens * top_k <= _MOST_ASSIGNED
+
+
+def _torch_dispatch(x, position):
+    token = torch.empty_like(position.reshape(-1), dtype=torch.int64)
+    at = torch.arange(position.numel(), device=x.device)
+    token = token.scatter(0, position.reshape(-1).long(), at // position.shape[1])
+    return x.index_select(0, token)
+
+
+def _torch_gather_sum(rows, weights, position):
+    wide = torch.promote_types(rows.dtype, torch.float32)
+    picked = rows.to(wide).index_select(0, position.reshape(-1).long()).view(*position.shape, rows.shape[1])
+    if weights is not None:
+        picked = picked * weights[:, :, None]   # never narrower than FP32
+    return picked.sum(1).to(rows.dtype)
+
+
+class _Dispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, position):
+        ctx.save_for_backward(position)
+        return _hip.load().dispatch(x, position)
+
+    @staticmethod
+    def backward(ctx, gout):
+        position, = ctx.saved_tensors
+        if _plain_backward(gout):
+            return _hip.load().combine(gout.contiguous(), None, position), None
+        return _torch_gather_sum(gout, None, position), None
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, weights, position):
+        ctx.save_for_backward(rows if ctx.needs_input_grad[1] else None, weights, position)
+        return _hip.load().combine(rows, weights, position)
+
+    @staticmethod
+    def backward(ctx, gout):
+        rows, weights, position = ctx.saved_tensors
+        wanted = ctx.needs_input_grad[:2]
+        if _plain_backward(gout):
+            return (*_hip.load().combine_backward(gout.contiguous(), rows, weights, position, wanted), None)
+        g = gout.float()
+        drows = dweights = None
+        if wanted[0]:
+            flat = position.reshape(-1).long()
+            inverse = torch.empty_like(flat).scatter(0, flat, torch.arange(flat.numel(), device=flat.device))
+            drows = (weights[:, :, None] * g[:, None, :]).flatten(0, 1).index_select(0, inverse).to(gout.dtype)
+        if wanted[1]:
+            picked = rows.float().index_select(0, position.reshape(-1).long()).view(*position.shape, rows.shape[1])
+            dweights = (picked * g[:, None, :]).sum(2)
+        return drows, dweights, None
+
+
+@torch.compiler.disable
+def dispatch(x: torch.Tensor, routing: Routing) -> torch.Tensor:
+    """Each token's row of ``x`` (``[tokens, hidden]``) at its ``top_k`` rows of the experts' order:
+    ``[tokens * top_k, hidden]``."""
+    if x.dim() != 2 or not x.is_floating_point():
+        raise ValueError(f"x must be floating-point [tokens, hidden], got {x.dtype} {tuple(x.shape)}")
+    tokens, top_k = _checked_position("x", routing, x.device)
+    if x.shape[0] != tokens:
+        raise ValueError(f"x has {x.shape[0]} tokens, the routing {tokens}")
+    if not plain(x) or not _fits(tokens, top_k, x.shape[1]) or _observed():
+        return _torch_dispatch(x, routing.position)
+    x, position = x.contiguous(), routing.position.contiguous()
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _Dispatch.apply(x, position)
+    return _hip.load().dispatch(x, position)
+
+
+@torch.compiler.disable
+def combine(rows: torch.Tensor, routing: Routing) -> torch.Tensor:
+    """Each token's sum of its ``rows`` (``[tokens * top_k, hidden]``, in the experts' order), weighted by the routing's
+    weights, summed in FP32 in the order of its choices and rounded once: ``[tokens, hidden]``."""
+    if rows.dim() != 2 or not rows.is_floating_point():
+        raise ValueError(f"rows must be floating-point [tokens * top_k, hidden], got {rows.dtype} {tuple(rows.shape)}")
+    tokens, top_k = _checked_position("rows", routing, rows.device)
+    if rows.shape[0] != tokens * top_k:
+        raise ValueError(f"rows must be the routing's {tokens * top_k}, got {rows.shape[0]}")
+    weights = routing.weights
+    if (tuple(weights.shape) != (tokens, top_k) or weights.device != rows.device
+            or weights.dtype not in (torch.float32, torch.promote_types(rows.dtype, torch.float32))):
+        raise ValueError(f"the routing's weights must be float32 [{tokens}, {top_k}] on {rows.device}, got {weights.dtype} "
+                         f"{tuple(weights.shape)} on {weights.device}")
+    if not plain(rows, weights) or not _fits(tokens, top_k, rows.shape[1]) or _observed():
+        return _torch_gather_sum(rows, weights, routing.position)
+    rows, weights, position = rows.contiguous(), weights.contiguous(), routing.position.contiguous()
+    if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
+        return _Combine.apply(rows, weights, position)
+    return _hip.load().combine(rows, weights, position)
+
+
+# ------------------------------------------------------------------- expert_mm
+
+def _bounds(rows: int, ends: torch.Tensor) -> list[tuple[int, int]]:
+    """Each expert's rows; ends out of range or order pulled to the nearest that are not, as the kernels do."""
+    out, lo = [], 0
+    for end in ends.tolist():
+        lo = min(max(lo, 0), rows)
+        out.append((lo, min(max(end, lo), rows)))
+        lo = end
+    return out
+
+
+def _torch_rows(x, weight, ends):
+    """``x`` times each expert's ``weight[e]`` (rows x k by k x n); zeros for the rows that are no expert's."""
+    parts = [x[lo:hi] @ weight[e] for e, (lo, hi) in enumerate(_bounds(x.shape[0], ends))]
+    out = torch.cat(parts)
+    return torch.cat((out, out.new_zeros(x.shape[0] - out.shape[0], out.shape[1]))) if out.shape[0] < x.shape[0] else out
+
+
+def _torch_weights(gout, x, ends):
+    return torch.stack([gout[lo:hi].t() @ x[lo:hi] for lo, hi in _bounds(x.shape[0], ends)])
+
+
+class _ExpertMM(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, ends):
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, weight, ends)
+        return _hip.load().expert_mm(x, weight, ends)
+
+    @staticmethod
+    def backward(ctx, gout):
+        x, weight, ends = ctx.saved_tensors
+        wanted = ctx.needs_input_grad[:2]
+        if _plain_backward(gout):
+            return (*_hip.load().expert_mm_backward(gout.contiguous(), x, weight, ends, wanted), None)
+        with torch.autocast(gout.device.type, enabled=False):
+            return (_torch_rows(gout, weight, ends) if wanted[0] else None,
+                    _torch_weights(gout, x, ends) if wanted[1] else None, None)
+
+
+@torch.compiler.disable
+def expert_mm(x: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
+    """``x[r] @ weight[e].T`` for each row ``r`` of each expert ``e``: ``x`` ``[rows, in]`` sorted by expert, ``weight``
+    ``[experts, out, in]`` (stacked Linear weights), expert ``e``'s rows ``ends[e - 1]`` to ``ends[e] - 1`` (``ends``: int32
+    ``[experts]``, not decreasing, on the device).  Rows from the last end on give zeros.
+
+    Sums are FP32, rounded once.  Differentiable in ``x`` and ``weight``; an expert without rows has zero gradients.
+    Under autocast both operands are taken in autocast's type, as a Linear's are."""
+    if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2]:
+        raise ValueError(f"expert_mm takes x [rows, in] and weight [experts, out, in], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if ends.dim() != 1 or ends.shape[0] != weight.shape[0] or ends.dtype != torch.int32:
+        raise ValueError(f"ends must be int32 [{weight.shape[0]}], got {ends.dtype} {tuple(ends.shape)}")
+    if not weight.shape[0] or not weight.shape[1] or not weight.shape[2]:
+        raise ValueError(f"weight must not be empty, got {tuple(weight.shape)}")
+    if weight.device != x.device or ends.device != x.device:
+        raise ValueError(f"x, weight and ends must be on one device, got {x.device}, {weight.device} and {ends.device}")
+    if torch.is_autocast_enabled(x.device.type):
+        cast = torch.get_autocast_dtype(x.device.type)
+        x, weight = x.to(cast), weight.to(cast)
+    if x.dtype != weight.dtype or not x.is_floating_point():
+        raise ValueError(f"x and weight must be of one floating-point type, got {x.dtype} and {weight.dtype}")
+    experts, n, k = weight.shape
+    if (not plain(x, weight) or x.shape[0] > _MOST_ROWS or experts > _MOST_MM_EXPERTS or n > _MOST_SIZE or k > _MOST_SIZE
+            or _observed()):
+        return _torch_rows(x, weight.transpose(1, 2), ends)
+    x, weight, ends = x.contiguous(), weight.contiguous(), ends.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return _ExpertMM.apply(x, weight, ends)
+    return _hip.load().expert_mm(x, weight, ends)

@@ -502,6 +502,61 @@ ADAMBRIDGE_API int adambridge_cross_entropy_backward(const void* logits, int32_t
                                                      int64_t rows, int64_t vocab, int64_t ignore_index,
                                                      const float* stats, const float* gout, void* grad);
 
+/* Operators of an expert block, for training and for single tokens.  The reference has none.  Values are
+ * ADAMBRIDGE_DT_F32 or _BF16, row-major and contiguous, at any element's address; sums, statistics and weights are FP32
+ * and each result is rounded once.  All on the calling thread's stream (asynchronous); results do not depend on
+ * scheduling.  Return 0, ADAMBRIDGE_EBADN (a size out of its range), _EMVDTYPE, _ENULL, _EALIGN (work not at a
+ * 4-byte boundary) or _EHIP; the _work functions the bytes of scratch a call takes, or ADAMBRIDGE_EBADN / _EMVDTYPE. */
+
+/* Layer norm over rows of cols values (each 1 .. 2^30): y = (x - mean) rstd weight + bias with rstd = 1 / sqrt(var + eps),
+ * var the mean of squared deviations.  weight and bias: cols values of w_dtype, or NULL (1 and 0).  stats: NULL, or the
+ * rows' mean and rstd for the gradient.  The backward call writes what is not NULL of dx (rows x cols of dtype), dweight and
+ * dbias (cols values of w_dtype; work: adambridge_layer_norm_work bytes, NULL without them). */
+ADAMBRIDGE_API int adambridge_layer_norm(const void* x, int32_t dtype, const void* weight, const void* bias, int32_t w_dtype,
+                                         int64_t rows, int64_t cols, float eps, void* y, float* stats);
+ADAMBRIDGE_API int64_t adambridge_layer_norm_work(int64_t rows, int64_t cols, int32_t dtype);
+ADAMBRIDGE_API int adambridge_layer_norm_backward(const void* gout, const void* x, int32_t dtype, const void* weight,
+                                                  int32_t w_dtype, const float* stats, int64_t rows, int64_t cols, void* dx,
+                                                  void* dweight, void* dbias, void* work);
+
+/* The top_k (1 .. 64) largest of each token's logits (experts: 1 .. 1024; tokens x top_k below 2^31), the lower index of
+ * equal ones, a NaN the largest: chosen and their weights, tokens x top_k, largest first.  The weights are the softmax
+ * over the chosen (normalize) or over all experts (0 in a row without any logit above -inf).  The assignments (t, j),
+ * numbered t top_k + j, are sorted by expert, stably: order holds the number at each row, position each assignment's
+ * row, ends one past each expert's last row.  The backward call takes gout, tokens x top_k, the gradient at the
+ * weights; it reads logits only without normalize. */
+ADAMBRIDGE_API int64_t adambridge_route_work(int64_t tokens, int64_t experts, int64_t top_k);
+ADAMBRIDGE_API int adambridge_route(const void* logits, int32_t dtype, int64_t tokens, int64_t experts, int64_t top_k,
+                                    int32_t normalize, float* weights, int32_t* chosen, int32_t* ends, int32_t* order,
+                                    int32_t* position, void* work);
+ADAMBRIDGE_API int adambridge_route_backward(const float* weights, const int32_t* chosen, const float* gout, const void* logits,
+                                             int32_t dtype, int64_t tokens, int64_t experts, int64_t top_k, int32_t normalize,
+                                             void* grad);
+
+/* dispatch: rows[position[t, j]] = x[t] (x: tokens x cols, cols 1 .. 2^22; rows: tokens top_k x cols).  combine: out[t] =
+ * the sum over j, in order, of weights[t, j] rows[position[t, j]] (weights NULL: 1, dispatch's gradient).
+ * combine_backward: drows[position[t, j]] = weights[t, j] gout[t] and dweights[t, j] = <gout[t], rows[position[t, j]]>, either
+ * NULL if not wanted.  A position outside 0 .. tokens top_k - 1 counts as a row of zeros and nothing is written for it. */
+ADAMBRIDGE_API int adambridge_dispatch(const void* x, int32_t dtype, const int32_t* position, int64_t tokens, int64_t top_k,
+                                       int64_t cols, void* rows);
+ADAMBRIDGE_API int adambridge_combine(const void* rows, int32_t dtype, const float* weights, const int32_t* position,
+                                      int64_t tokens, int64_t top_k, int64_t cols, void* out);
+ADAMBRIDGE_API int adambridge_combine_backward(const void* gout, const void* rows, int32_t dtype, const float* weights,
+                                               const int32_t* position, int64_t tokens, int64_t top_k, int64_t cols, void* drows,
+                                               float* dweights);
+
+/* Products grouped by expert (1 .. 4096): rows (0 .. 2^30) sorted by expert, expert e's being ends[e - 1] .. ends[e] - 1 (ends
+ * in device memory, none below the one before it; the first expert's start at 0); weight: experts x n x k (n and k 1 ..
+ * 2^22).  y = x weight[e]^T (x: rows x k, y: rows x n); dx = gout weight[e] (gout: rows x n); dw[e] = gout^T x over e's
+ * rows, zeros where there are none.  Rows from the last end on give zeros.  Ends that break the rule give
+ * unspecified values, and nothing outside the arrays is touched. */
+ADAMBRIDGE_API int adambridge_expert_mm(const void* x, const void* weight, const int32_t* ends, void* y, int32_t dtype,
+                                        int64_t rows, int64_t experts, int64_t n, int64_t k);
+ADAMBRIDGE_API int adambridge_expert_mm_dx(const void* gout, const void* weight, const int32_t* ends, void* dx, int32_t dtype,
+                                           int64_t rows, int64_t experts, int64_t n, int64_t k);
+ADAMBRIDGE_API int adambridge_expert_mm_dw(const void* gout, const void* x, const int32_t* ends, void* dw, int32_t dtype,
+                                           int64_t rows, int64_t experts, int64_t n, int64_t k);
+
 #ifdef __cplusplus
 }
 #endif
