@@ -309,6 +309,190 @@ __global__ __launch_bounds__(kMmThreads2, 2) void k_experts_any(ExpertArgs A)
     }
 }
 
+// ------------------------------------------------------------- BF16 rows of whole 16-byte pieces
+//
+// Tiles of 256 x 256, eight wavefronts of 128 x 64 (2 x 4), 64 terms a step, two buffers of 64 KB in the LDS.  A step's
+// tiles go from memory to the LDS past the registers while the step before is multiplied; what lies outside an
+// operand is out of its buffer's range and arrives as zeros.  A wavefront's 8 matrix products of 32 x 32 x 16
+// take 6 KB from the LDS, three quarters of the time the products take.
+//
+// A long operand's tile is 256 rows of 128 bytes, its 16-byte pieces exchanged by the row (piece c at place c ^ row mod 8), so
+// that the reads of 8 rows meet 8 different places.  One across its rows is 64 terms of 512 bytes, read transposed
+// (ds_read_b64_tr_b16: 16 lanes take 4 terms x 16 values, a lane 4 terms of one value), its pieces exchanged in
+// pairs by the term's bits 0, 1 and 3, in which the terms of one read differ.
+
+constexpr int kFast = 256, kFastStep = 64, kFastThreads = 512;
+constexpr int kFastBytes = kFast * kFastStep * 2;   // of an operand's tile
+constexpr uint32_t kOutside = 0x80000000u;          // an offset outside every buffer
+
+typedef float mm_f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 mm_bf16x4 __attribute__((ext_vector_type(4)));
+
+template <bool LONG>
+struct Feed {
+    const uint8_t* base;   // the tile's first value
+    uint32_t offset[4];    // of this lane's pieces
+    int64_t left;          // !LONG: bytes from base to the operand's end
+    int32_t pitch;         // bytes
+    bool past;             // LONG: whether this lane's pieces are past the end in the last step
+
+    // rows: LONG: the tile's rows; else the operand's terms.  lead: !LONG: bytes before base in its first row.
+    __device__ __forceinline__ void start(const uint8_t* p, int64_t pitch_bytes, int rows, int len, int64_t lead)
+    {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
+        base = p;
+        pitch = (int32_t)pitch_bytes;
+        const int piece = LONG ? (lane & 7) ^ (lane >> 3) : 0;
+        past = LONG && len % kFastStep && piece * 8 >= len % kFastStep;
+        left = LONG ? (int64_t)(rows < kFast ? rows : kFast) * pitch_bytes : (int64_t)rows * pitch_bytes - lead;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if constexpr (LONG) {
+                const int row = (q * 8 + wave) * 8 + (lane >> 3);
+                offset[q] = (uint32_t)(row * pitch + piece * 16);
+            } else {
+                const int term = (q * 8 + wave) * 2 + (lane >> 5), swap = (term & 3) | ((term >> 3) & 1) << 2;
+                offset[q] = (uint32_t)(term * pitch + ((lane & 31) ^ (swap << 1)) * 16);
+            }
+        }
+    }
+    __device__ __forceinline__ void issue(int step, bool last, uint8_t* lds) const
+    {
+        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+        const int64_t skip = LONG ? 0 : (int64_t)step * kFastStep * pitch;
+        const int64_t bytes = left - skip;
+        const int32_t range = (int32_t)(bytes < 0x7fffffff ? bytes : 0x7fffffff);
+        const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base + skip), 0, range, 0x00020000);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                buffer, (__attribute__((address_space(3))) void*)(lds + (q * 8 + wave) * 1024), 16,
+                LONG && last && past ? kOutside : offset[q], LONG ? step * kFastStep * 2 : 0, 0, 0);
+    }
+};
+
+// Reads of a wavefront's fragments: 32 rows, from row `first` of the tile, by 16 terms.
+template <bool LONG, int N>
+struct Fragments {
+    uint32_t place[LONG ? 4 : N];
+    __device__ __forceinline__ void start(int first)
+    {
+        const int lane = threadIdx.x & 63;
+        if constexpr (LONG) {
+#pragma unroll
+            for (int h = 0; h < 4; ++h) place[h] = (first + (lane & 31)) * 128 + (((2 * h + (lane >> 5)) ^ (lane & 7)) * 16);
+        } else {
+            const int within = (lane & 15) >> 2, term = 8 * (lane >> 5) + within, swap = within | (lane >> 5) << 2;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int piece = (first + 32 * i) / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+                place[i] = term * 512 + ((piece ^ (swap << 1)) * 16) + (lane & 1) * 8;
+            }
+        }
+    }
+    __device__ __forceinline__ mm_bf16x8 read(const uint8_t* lds, int i, int h) const
+    {
+        if constexpr (LONG) {
+            return __builtin_bit_cast(mm_bf16x8, *reinterpret_cast<const raw16*>(lds + place[h] + i * 4096));
+        } else {
+            typedef __attribute__((address_space(3))) mm_bf16x4* Local;
+            const uint8_t* p = lds + place[i] + h * 8192;
+            const mm_bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Local)(p));
+            const mm_bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Local)(p + 2048));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+};
+
+template <int MODE>
+__global__ __launch_bounds__(kFastThreads, 2) void k_experts_fast(ExpertArgs A)
+{
+    constexpr bool ALONG = MODE != MODE_DW, BLONG = MODE == MODE_Y;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * kFastBytes];
+    Tile t;
+    if (!(MODE == MODE_DW ? find_weight_tile(A, t) : find_row_tile<kFast>(A, t))) return;
+    const int i0 = t.ti * kFast, j0 = t.tj * kFast;
+    const int limit_i = MODE == MODE_DW ? A.ni - i0 : t.hi - t.lo - i0, limit_j = A.nj - j0;
+    const int len = MODE == MODE_DW ? t.hi - t.lo : t.e < A.experts ? A.len : 0;
+    const int steps = (len + kFastStep - 1) / kFastStep;
+    Feed<ALONG> fa;
+    Feed<BLONG> fb;
+    if constexpr (MODE == MODE_DW) {
+        fa.start(at<DT_BF16>(A.a, (int64_t)t.lo * A.ni + i0), (int64_t)A.ni * 2, len, len, (int64_t)i0 * 2);
+        fb.start(at<DT_BF16>(A.b, (int64_t)t.lo * A.nj + j0), (int64_t)A.nj * 2, len, len, (int64_t)j0 * 2);
+    } else {
+        const uint8_t* w = at<DT_BF16>(A.b, (int64_t)(t.e < A.experts ? t.e : 0) * A.len * A.nj);
+        fa.start(at<DT_BF16>(A.a, (int64_t)(t.lo + i0) * A.len), (int64_t)A.len * 2, limit_i, len, 0);
+        if constexpr (MODE == MODE_Y) fb.start(w + (int64_t)j0 * A.len * 2, (int64_t)A.len * 2, limit_j, len, 0);
+        else fb.start(w + (int64_t)j0 * 2, (int64_t)A.nj * 2, len, len, (int64_t)j0 * 2);
+    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
+    const int wi = (wave & 1) * 128, wj = (wave >> 1) * 64;
+    Fragments<ALONG, 4> ra;
+    Fragments<BLONG, 2> rb;
+    ra.start(wi);
+    rb.start(wj);
+    mm_f32x16 acc[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+    if (steps > 0) {
+        fa.issue(0, steps == 1, lds);
+        fb.issue(0, steps == 1, lds + kFastBytes);
+    }
+    for (int s = 0; s < steps; ++s) {
+        uint8_t* now = lds + (s & 1) * 2 * kFastBytes;
+        uint8_t* next = lds + ((s & 1) ^ 1) * 2 * kFastBytes;
+        __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this step's pieces have arrived
+        __syncthreads();                      // everyone's, and the step before has been read
+        if (s + 1 < steps) {
+            fa.issue(s + 1, s + 2 == steps, next);
+            fb.issue(s + 1, s + 2 == steps, next + kFastBytes);
+        }
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            mm_bf16x8 a[4], b[2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] = ra.read(now, i, h);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) b[j] = rb.read(now + kFastBytes, j, h);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
+        }
+    }
+    // a lane has row lane mod 32 and, of each 8 columns, 4: the two halves exchange fours for whole 16 bytes
+    uint8_t* out = MODE == MODE_DW ? at<DT_BF16>(A.c, ((int64_t)t.e * A.ni + i0) * A.nj + j0)
+                                   : at<DT_BF16>(A.c, (int64_t)(t.lo + i0) * A.nj + j0);
+    const int half = lane >> 5;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = wi + 32 * i + (lane & 31);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int q = 0; q < 4; q += 2) {
+                uint32_t x[2][2];
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    x[p][0] = bf16x2_rne(acc[i][j][4 * (q + p)], acc[i][j][4 * (q + p) + 1]);
+                    x[p][1] = bf16x2_rne(acc[i][j][4 * (q + p) + 2], acc[i][j][4 * (q + p) + 3]);
+                }
+                // half 0 keeps its four of the first eight and takes half 1's; half 1 those of the second
+                const auto s0 = __builtin_amdgcn_permlane32_swap(x[0][0], x[1][0], false, false);
+                const auto s1 = __builtin_amdgcn_permlane32_swap(x[0][1], x[1][1], false, false);
+                const int c = wj + 32 * j + 8 * (q + half);
+                if (row < limit_i && c < limit_j)
+                    store_raw<DT_BF16>(out, (int64_t)row * A.nj + c, raw16{s0[0], s1[0], s0[1], s1[1]});
+            }
+        }
+    }
+}
+
 // --------------------------------------------------------------------- launches
 
 template <int MODE>
@@ -331,14 +515,19 @@ static int experts_mm(const void* a, const void* b, const int32_t* ends, void* c
     A.ni = (int32_t)n;
     A.nj = (int32_t)(MODE == MODE_Y ? n : k);
     A.len = (int32_t)(MODE == MODE_Y ? k : n);
-    A.tiles_j = (A.nj + kTile - 1) / kTile;
-    A.tiles_i = (A.ni + kTile - 1) / kTile;
+    // rows of whole 16-byte pieces, 256 of them within a buffer's offsets
+    const bool fast = dtype == ADAMBRIDGE_DT_BF16 && n % 8 == 0 && k % 8 == 0 && n <= (int64_t)1 << 21 && k <= (int64_t)1 << 21 &&
+                      ((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) % 16 == 0;
+    const int tile = fast ? kFast : kTile;
+    A.tiles_j = (A.nj + tile - 1) / tile;
+    A.tiles_i = (A.ni + tile - 1) / tile;
     // every expert, and the rows that are no expert's, may have a partial tile
     const int64_t tiles = MODE == MODE_DW ? experts * A.tiles_i * A.tiles_j
-                                          : std::min(rows, rows / kTile + experts + 1) * A.tiles_j;
+                                          : std::min(rows, rows / tile + experts + 1) * A.tiles_j;
     if (tiles > ((int64_t)1 << 31) - 64) return ADAMBRIDGE_EBADN;
     const dim3 grid((unsigned)((tiles + kXcd - 1) / kXcd * kXcd));
-    if (dtype == ADAMBRIDGE_DT_BF16) hipLaunchKernelGGL((k_experts_any<DT_BF16, MODE>), grid, dim3(kMmThreads2), 0, t_stream, A);
+    if (fast) hipLaunchKernelGGL((k_experts_fast<MODE>), grid, dim3(kFastThreads), 0, t_stream, A);
+    else if (dtype == ADAMBRIDGE_DT_BF16) hipLaunchKernelGGL((k_experts_any<DT_BF16, MODE>), grid, dim3(kMmThreads2), 0, t_stream, A);
     else hipLaunchKernelGGL((k_experts_any<DT_F32, MODE>), grid, dim3(kMmThreads2), 0, t_stream, A);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : hip_fail(e, "hipLaunchKernelGGL (expert product)");
