@@ -19,6 +19,7 @@
 #include <algorithm>
 #include <type_traits>
 
+
 #include "../../include/adambridge_hip.h"
 #include "abh_device.hpp"
 #include "abh_host.hpp"
@@ -115,17 +116,15 @@ __device__ __forceinline__ bool find_row_tile(const ExpertArgs& A, Tile& t)
     return false;
 }
 
-// A tile of dW: expert by expert, an expert's tiles on one XCD.
+// A tile of dW.  The XCDs share every expert's tiles evenly, because experts differ in rows and so in work.
 __device__ __forceinline__ bool find_weight_tile(const ExpertArgs& A, Tile& t)
 {
-    const int an = A.tiles_i * A.tiles_j;
-    const int tiles = an * A.experts;
-    const int per = (tiles + kXcd - 1) / kXcd;
+    const int an = A.tiles_i * A.tiles_j, per = (an + kXcd - 1) / kXcd;
     const int slot = (int)(blockIdx.x / kXcd);
-    const int idx = (int)(blockIdx.x % kXcd) * per + slot;
-    if (slot >= per || idx >= tiles) return false;
-    t.e = idx / an;
-    const int local = idx - t.e * an;
+    t.e = slot / per;
+    if (t.e >= A.experts) return false;
+    const int local = (int)((blockIdx.x + t.e) % kXcd) * per + slot - t.e * per;   // the first XCD changes: an may be below 8
+    if (local >= an) return false;
     const int g = local / (kGroupTiles * A.tiles_j), first = g * kGroupTiles;
     const int wide = A.tiles_i - first < kGroupTiles ? A.tiles_i - first : kGroupTiles;
     const int r = local - first * A.tiles_j;
@@ -311,30 +310,53 @@ __global__ __launch_bounds__(kMmThreads2, 2) void k_experts_any(ExpertArgs A)
 
 // ------------------------------------------------------------- BF16 rows of whole 16-byte pieces
 //
-// Tiles of 256 x 256, eight wavefronts of 128 x 64 (2 x 4), 64 terms a step, two buffers of 64 KB in the LDS.  A step's
-// tiles go from memory to the LDS past the registers while the step before is multiplied; what lies outside an
-// operand is out of its buffer's range and arrives as zeros.  A wavefront's 8 matrix products of 32 x 32 x 16
-// take 6 KB from the LDS, three quarters of the time the products take.
+// Tiles of 256 x 256, eight wavefronts of 128 x 64 (2 x 4), 32 terms a step, four buffers of 32 KB in the LDS.  A step's
+// tiles go from memory to the LDS past the registers, three steps ahead of the one that is multiplied; what lies
+// outside an operand is out of its buffer's range and arrives as zeros.  A wavefront reads the fragments of its next
+// 8 matrix products of 32 x 32 x 16 while the matrix cores work on these.
 //
-// A long operand's tile is 256 rows of 128 bytes, its 16-byte pieces exchanged by the row (piece c at place c ^ row mod 8), so
-// that the reads of 8 rows meet 8 different places.  One across its rows is 64 terms of 512 bytes, read transposed
+// Measured on MI355X, one expert, 8192^3: y 873 us (1259 TFLOP/s), dx 827 (1329), dW 821 (1339); the matrix cores are busy
+// 73% of the cycles, at 1.6 GHz of 2.4: power is the bound.  Slower: 64 terms a step with two buffers 891 (y),
+// wavefronts of 128 x 128 (one a SIMD) 890, tiles of 128 x 256 with two workgroups a CU 1010, three buffers 989; five
+// buffers change nothing.
+//
+// A long operand's tile is its rows by 64 bytes, a row's 16-byte pieces exchanged by the row, so that the reads of
+// neighbouring rows meet different banks.  One across its rows is 32 terms by its rows, read transposed
 // (ds_read_b64_tr_b16: 16 lanes take 4 terms x 16 values, a lane 4 terms of one value), its pieces exchanged in
-// pairs by the term's bits 0, 1 and 3, in which the terms of one read differ.
+// fours by the term mod 4: the 4 terms x 2 pairs of pieces of 32 lanes then cover the 256 bytes of all banks.
 
-constexpr int kFast = 256, kFastStep = 64, kFastThreads = 512;
-constexpr int kFastBytes = kFast * kFastStep * 2;   // of an operand's tile
 constexpr uint32_t kOutside = 0x80000000u;          // an offset outside every buffer
 
 typedef float mm_f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 mm_bf16x4 __attribute__((ext_vector_type(4)));
 
-template <bool LONG>
+// Tile BM x BN by BK terms, NB buffers, WI x WJ wavefronts.
+template <int BM_, int BN_, int BK_, int NB_, int WI_, int WJ_, int OCC_>
+struct Config {
+    static constexpr int BM = BM_, BN = BN_, BK = BK_, NB = NB_, WI = WI_, WJ = WJ_, OCC = OCC_, W = WI * WJ, T = W * kWave;
+    static constexpr int NI = BM / WI / 32, NJ = BN / WJ / 32;
+    static constexpr int LOADS = (BM + BN) * BK * 2 / 1024 / W;   // of a wavefront and step
+    static constexpr int BYTES = (BM + BN) * BK * 2;
+};
+
+// vmcnt(n): all but the last n of this wavefront's loads have arrived.
+template <int N>
+__device__ __forceinline__ void wait_loads()
+{
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
+}
+
+// One operand's tile of R rows by BK terms, on its way to the LDS in W wavefronts' pieces of 1 KB.
+template <bool LONG, int R, int BK, int W>
 struct Feed {
+    static constexpr int N = R * BK * 2 / 1024 / W, CH = BK / 8;
     const uint8_t* base;   // the tile's first value
-    uint32_t offset[4];    // of this lane's pieces
+    uint32_t offset[N];    // of this lane's pieces
     int64_t left;          // !LONG: bytes from base to the operand's end
     int32_t pitch;         // bytes
     bool past;             // LONG: whether this lane's pieces are past the end in the last step
+
+    static __device__ __forceinline__ int swap_of_row(int row) { return BK == 64 ? row & 7 : (row >> 2) & 3; }
 
     // rows: LONG: the tile's rows; else the operand's terms.  lead: !LONG: bytes before base in its first row.
     __device__ __forceinline__ void start(const uint8_t* p, int64_t pitch_bytes, int rows, int len, int64_t lead)
@@ -342,81 +364,104 @@ struct Feed {
         const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
         base = p;
         pitch = (int32_t)pitch_bytes;
-        const int piece = LONG ? (lane & 7) ^ (lane >> 3) : 0;
-        past = LONG && len % kFastStep && piece * 8 >= len % kFastStep;
-        left = LONG ? (int64_t)(rows < kFast ? rows : kFast) * pitch_bytes : (int64_t)rows * pitch_bytes - lead;
+        past = false;
+        left = LONG ? (int64_t)(rows < R ? rows : R) * pitch_bytes : (int64_t)rows * pitch_bytes - lead;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < N; ++q) {
             if constexpr (LONG) {
-                const int row = (q * 8 + wave) * 8 + (lane >> 3);
+                const int row = (q * W + wave) * (64 / CH) + lane / CH, piece = (lane % CH) ^ swap_of_row(row);
                 offset[q] = (uint32_t)(row * pitch + piece * 16);
+                if (q == 0) past = len % BK && piece * 8 >= len % BK;   // the same piece in all of them
             } else {
-                const int term = (q * 8 + wave) * 2 + (lane >> 5), swap = (term & 3) | ((term >> 3) & 1) << 2;
-                offset[q] = (uint32_t)(term * pitch + ((lane & 31) ^ (swap << 1)) * 16);
+                const int term = (q * W + wave) * (512 / R) + lane / (R / 8);
+                offset[q] = (uint32_t)(term * pitch + ((lane % (R / 8)) ^ (term & 3) << 2) * 16);
             }
         }
     }
-    __device__ __forceinline__ void issue(int step, bool last, uint8_t* lds) const
+    __device__ __forceinline__ void issue(int step, int steps, uint8_t* lds) const
     {
         const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
-        const int64_t skip = LONG ? 0 : (int64_t)step * kFastStep * pitch;
+        const int64_t skip = LONG ? 0 : (int64_t)step * BK * pitch;
         const int64_t bytes = left - skip;
-        const int32_t range = (int32_t)(bytes < 0x7fffffff ? bytes : 0x7fffffff);
-        const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base + skip), 0, range, 0x00020000);
+        const int32_t range = step >= steps ? 0 : (int32_t)(bytes < 0x7fffffff ? bytes : 0x7fffffff);   // past the end: zeros
+        const uint64_t first = (uint64_t)(base + skip);
+        const raw16 buffer = {(uint32_t)first, (uint32_t)(first >> 32) & 0xffffu, (uint32_t)range, 0x00020000u};
+        const uint32_t along = LONG ? (uint32_t)step * BK * 2 : 0u;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                buffer, (__attribute__((address_space(3))) void*)(lds + (q * 8 + wave) * 1024), 16,
-                LONG && last && past ? kOutside : offset[q], LONG ? step * kFastStep * 2 : 0, 0, 0);
+        for (int q = 0; q < N; ++q) {
+            // In assembly, so that the compiler does not wait for it before each transposed read: no register is written, and
+            // the arrival is waited for by wait_loads.
+            const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)(lds + (q * W + wave) * 1024);
+            const uint32_t from = LONG && step + 1 == steps && past ? kOutside : offset[q];
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                         :: "s"(to), "v"(from), "s"(buffer), "s"(along) : "memory");
+        }
     }
 };
 
-// Reads of a wavefront's fragments: 32 rows, from row `first` of the tile, by 16 terms.
-template <bool LONG, int N>
+// Reads of a wavefront's fragments: 32 rows, from row `first` of the tile of R rows, by 16 terms.
+template <bool LONG, int R, int BK, int N>
 struct Fragments {
-    uint32_t place[LONG ? 4 : N];
+    uint32_t place[LONG ? BK / 16 : N];
     __device__ __forceinline__ void start(int first)
     {
         const int lane = threadIdx.x & 63;
         if constexpr (LONG) {
+            const int row = first + (lane & 31);   // first and the fragments are multiples of 32 apart: the same exchange
 #pragma unroll
-            for (int h = 0; h < 4; ++h) place[h] = (first + (lane & 31)) * 128 + (((2 * h + (lane >> 5)) ^ (lane & 7)) * 16);
+            for (int h = 0; h < BK / 16; ++h)
+                place[h] = row * BK * 2 + (((2 * h + (lane >> 5)) ^ Feed<LONG, R, BK, 1>::swap_of_row(row)) * 16);
         } else {
-            const int within = (lane & 15) >> 2, term = 8 * (lane >> 5) + within, swap = within | (lane >> 5) << 2;
+            const int within = (lane & 15) >> 2, term = 8 * (lane >> 5) + within;   // within: the term mod 4
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int piece = (first + 32 * i) / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-                place[i] = term * 512 + ((piece ^ (swap << 1)) * 16) + (lane & 1) * 8;
+                place[i] = term * R * 2 + ((piece ^ within << 2) * 16) + (lane & 1) * 8;
             }
         }
     }
     __device__ __forceinline__ mm_bf16x8 read(const uint8_t* lds, int i, int h) const
     {
         if constexpr (LONG) {
-            return __builtin_bit_cast(mm_bf16x8, *reinterpret_cast<const raw16*>(lds + place[h] + i * 4096));
+            return __builtin_bit_cast(mm_bf16x8, *reinterpret_cast<const raw16*>(lds + place[h] + i * 32 * BK * 2));
         } else {
             typedef __attribute__((address_space(3))) mm_bf16x4* Local;
-            const uint8_t* p = lds + place[i] + h * 8192;
+            const uint8_t* p = lds + place[i] + h * 16 * R * 2;
             const mm_bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Local)(p));
-            const mm_bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Local)(p + 2048));
+            const mm_bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Local)(p + 4 * R * 2));
             return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     }
 };
 
-template <int MODE>
-__global__ __launch_bounds__(kFastThreads, 2) void k_experts_fast(ExpertArgs A)
+typedef Config<256, 256, 32, 4, 2, 4, 2> FastConfig;
+
+// Asks the scheduler for READS reads of the LDS spread among the next PRODUCTS matrix products.
+template <int READS, int PRODUCTS, int M = 0>
+__device__ __forceinline__ void spread_reads()
+{
+    if constexpr (M < PRODUCTS) {
+        constexpr int n = READS * (M + 1) / PRODUCTS - READS * M / PRODUCTS;
+        if constexpr (n > 0) __builtin_amdgcn_sched_group_barrier(0x100, n, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        spread_reads<READS, PRODUCTS, M + 1>();
+    }
+}
+
+template <int MODE, class C>
+__global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
 {
     constexpr bool ALONG = MODE != MODE_DW, BLONG = MODE == MODE_Y;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[4 * kFastBytes];
+    constexpr int BM = C::BM, BN = C::BN, BK = C::BK, NB = C::NB;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[NB * C::BYTES];
     Tile t;
-    if (!(MODE == MODE_DW ? find_weight_tile(A, t) : find_row_tile<kFast>(A, t))) return;
-    const int i0 = t.ti * kFast, j0 = t.tj * kFast;
+    if (!(MODE == MODE_DW ? find_weight_tile(A, t) : find_row_tile<BM>(A, t))) return;
+    const int i0 = t.ti * BM, j0 = t.tj * BN;
     const int limit_i = MODE == MODE_DW ? A.ni - i0 : t.hi - t.lo - i0, limit_j = A.nj - j0;
     const int len = MODE == MODE_DW ? t.hi - t.lo : t.e < A.experts ? A.len : 0;
-    const int steps = (len + kFastStep - 1) / kFastStep;
-    Feed<ALONG> fa;
-    Feed<BLONG> fb;
+    const int steps = (len + BK - 1) / BK;
+    Feed<ALONG, BM, BK, C::W> fa;
+    Feed<BLONG, BN, BK, C::W> fb;
     if constexpr (MODE == MODE_DW) {
         fa.start(at<DT_BF16>(A.a, (int64_t)t.lo * A.ni + i0), (int64_t)A.ni * 2, len, len, (int64_t)i0 * 2);
         fb.start(at<DT_BF16>(A.b, (int64_t)t.lo * A.nj + j0), (int64_t)A.nj * 2, len, len, (int64_t)j0 * 2);
@@ -427,53 +472,82 @@ __global__ __launch_bounds__(kFastThreads, 2) void k_experts_fast(ExpertArgs A)
         else fb.start(w + (int64_t)j0 * 2, (int64_t)A.nj * 2, len, len, (int64_t)j0 * 2);
     }
     const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
-    const int wi = (wave & 1) * 128, wj = (wave >> 1) * 64;
-    Fragments<ALONG, 4> ra;
-    Fragments<BLONG, 2> rb;
+    const int wi = wave % C::WI * (BM / C::WI), wj = wave / C::WI * (BN / C::WJ);
+    Fragments<ALONG, BM, BK, C::NI> ra;
+    Fragments<BLONG, BN, BK, C::NJ> rb;
     ra.start(wi);
     rb.start(wj);
-    mm_f32x16 acc[4][2];
+    mm_f32x16 acc[C::NI][C::NJ];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < C::NI; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < C::NJ; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+    constexpr int H = BK / 16;
+    auto issue = [&](int s, int buffer) {
+        fa.issue(s, steps, lds + buffer * C::BYTES);
+        fb.issue(s, steps, lds + buffer * C::BYTES + BM * BK * 2);
+    };
+    // fragments are read one product ahead, so that the LDS works while the matrix cores do
+    mm_bf16x8 a[2][C::NI], b[2][C::NJ];
+    auto fetch = [&](int set, int buffer, int h) {
+        const uint8_t* la = lds + buffer * C::BYTES;
+#pragma unroll
+        for (int i = 0; i < C::NI; ++i) a[set][i] = ra.read(la, i, h);
+#pragma unroll
+        for (int j = 0; j < C::NJ; ++j) b[set][j] = rb.read(la + BM * BK * 2, j, h);
+    };
+    auto multiply = [&](int set) {
+#pragma unroll
+        for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+            for (int j = 0; j < C::NJ; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[set][j], a[set][i], acc[i][j], 0, 0, 0);
+    };
+    constexpr int READS = (ALONG ? 1 : 2) * C::NI + (BLONG ? 1 : 2) * C::NJ, PRODUCTS = C::NI * C::NJ;
+    auto interleave = [&]() { spread_reads<READS, PRODUCTS>(); };
     if (steps > 0) {
-        fa.issue(0, steps == 1, lds);
-        fb.issue(0, steps == 1, lds + kFastBytes);
-    }
-    for (int s = 0; s < steps; ++s) {
-        uint8_t* now = lds + (s & 1) * 2 * kFastBytes;
-        uint8_t* next = lds + ((s & 1) ^ 1) * 2 * kFastBytes;
-        __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this step's pieces have arrived
-        __syncthreads();                      // everyone's, and the step before has been read
-        if (s + 1 < steps) {
-            fa.issue(s + 1, s + 2 == steps, next);
-            fb.issue(s + 1, s + 2 == steps, next + kFastBytes);
+#pragma unroll
+        for (int s = 0; s < NB - 1; ++s) issue(s, s);
+        wait_loads<(NB - 2) * C::LOADS>();
+        __syncthreads();
+        fetch(0, 0, 0);
+        int now = 0, next = 1, ahead = NB - 1;
+        for (int s = 0; s + 1 < steps; ++s) {
+#pragma unroll
+            for (int h = 0; h + 1 < H; ++h) {
+                fetch((h + 1) & 1, now, h + 1);
+                multiply(h & 1);
+                interleave();
+            }
+            // the next step's pieces have arrived, everyone's after the barrier, and the step before has been read
+            wait_loads<(NB - 3) * C::LOADS>();
+            __syncthreads();
+            issue(s + NB - 1, ahead);
+            fetch(0, next, 0);
+            multiply((H - 1) & 1);
+            interleave();
+            now = next;
+            next = next + 1 == NB ? 0 : next + 1;
+            ahead = ahead + 1 == NB ? 0 : ahead + 1;
         }
 #pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            mm_bf16x8 a[4], b[2];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] = ra.read(now, i, h);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) b[j] = rb.read(now + kFastBytes, j, h);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[j], a[i], acc[i][j], 0, 0, 0);
+        for (int h = 0; h < H; ++h) {
+            if (h + 1 < H) fetch((h + 1) & 1, now, h + 1);
+            multiply(h & 1);
         }
+        wait_loads<0>();   // nothing is on its way to the LDS when the workgroup ends
     }
     // a lane has row lane mod 32 and, of each 8 columns, 4: the two halves exchange fours for whole 16 bytes
     uint8_t* out = MODE == MODE_DW ? at<DT_BF16>(A.c, ((int64_t)t.e * A.ni + i0) * A.nj + j0)
                                    : at<DT_BF16>(A.c, (int64_t)(t.lo + i0) * A.nj + j0);
     const int half = lane >> 5;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < C::NI; ++i) {
         const int row = wi + 32 * i + (lane & 31);
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < C::NJ; ++j) {
 #pragma unroll
             for (int q = 0; q < 4; q += 2) {
                 uint32_t x[2][2];
@@ -492,6 +566,11 @@ __global__ __launch_bounds__(kFastThreads, 2) void k_experts_fast(ExpertArgs A)
         }
     }
 }
+
+// (named here: the host's compilation leaves out their launch functions otherwise)
+template __global__ void k_experts_fast<MODE_Y, FastConfig>(ExpertArgs);
+template __global__ void k_experts_fast<MODE_DX, FastConfig>(ExpertArgs);
+template __global__ void k_experts_fast<MODE_DW, FastConfig>(ExpertArgs);
 
 // --------------------------------------------------------------------- launches
 
@@ -518,15 +597,16 @@ static int experts_mm(const void* a, const void* b, const int32_t* ends, void* c
     // rows of whole 16-byte pieces, 256 of them within a buffer's offsets
     const bool fast = dtype == ADAMBRIDGE_DT_BF16 && n % 8 == 0 && k % 8 == 0 && n <= (int64_t)1 << 21 && k <= (int64_t)1 << 21 &&
                       ((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) % 16 == 0;
-    const int tile = fast ? kFast : kTile;
-    A.tiles_j = (A.nj + tile - 1) / tile;
-    A.tiles_i = (A.ni + tile - 1) / tile;
+    typedef FastConfig C;
+    const int tile_i = fast ? C::BM : kTile, tile_j = fast ? C::BN : kTile;
+    A.tiles_j = (A.nj + tile_j - 1) / tile_j;
+    A.tiles_i = (A.ni + tile_i - 1) / tile_i;
     // every expert, and the rows that are no expert's, may have a partial tile
-    const int64_t tiles = MODE == MODE_DW ? experts * A.tiles_i * A.tiles_j
-                                          : std::min(rows, rows / tile + experts + 1) * A.tiles_j;
+    const int64_t tiles = MODE == MODE_DW ? experts * (((int64_t)A.tiles_i * A.tiles_j + kXcd - 1) / kXcd * kXcd)
+                                          : std::min(rows, rows / tile_i + experts + 1) * A.tiles_j;
     if (tiles > ((int64_t)1 << 31) - 64) return ADAMBRIDGE_EBADN;
     const dim3 grid((unsigned)((tiles + kXcd - 1) / kXcd * kXcd));
-    if (fast) hipLaunchKernelGGL((k_experts_fast<MODE>), grid, dim3(kFastThreads), 0, t_stream, A);
+    if (fast) hipLaunchKernelGGL((k_experts_fast<MODE, C>), grid, dim3(C::T), 0, t_stream, A);
     else if (dtype == ADAMBRIDGE_DT_BF16) hipLaunchKernelGGL((k_experts_any<DT_BF16, MODE>), grid, dim3(kMmThreads2), 0, t_stream, A);
     else hipLaunchKernelGGL((k_experts_any<DT_F32, MODE>), grid, dim3(kMmThreads2), 0, t_stream, A);
     const hipError_t e = hipGetLastError();
