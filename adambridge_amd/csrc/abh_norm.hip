@@ -31,13 +31,14 @@ struct NormArgs {
     const void* b;
     void* y;        // or dx
     float* stats;   // mean, rstd a row
+    void* dw;
+    void* db;
     float* part;    // P x 2 x cols: sums of g xh, of g
     int64_t rows, cols;
     float eps;
 };
 
-// G lanes a row, NV vectors a lane.  A row of up to 64 lanes has a wavefront (four a workgroup), a longer one
-// a workgroup.
+// G lanes a row, NV vectors a lane: a wavefront a row (four rows a workgroup) or a workgroup.
 template <int G>
 constexpr int kNormThreads = G < 256 ? 256 : G;
 
@@ -45,30 +46,38 @@ template <int DT, int WT, int G, int NV>
 __global__ __launch_bounds__(kNormThreads<G>) void k_norm(NormArgs A)
 {
     constexpr int K = kLane<DT>, T = kNormThreads<G>;
-    __shared__ float part[2 * T / kWave];
+    __shared__ float part[2][2 * T / kWave];
     const int lane = threadIdx.x % G;
     const int64_t row = (int64_t)blockIdx.x * (T / G) + threadIdx.x / G;
     if (G < T && row >= A.rows) return;   // whole wavefronts, and no barrier follows
     const void* x = at<DT>(A.x, row * A.cols);
-    float v[NV][K];
+    raw16 v[NV];
     float sum = 0.0f, none = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load_vec<DT>(x, (int64_t)(i * G + lane) * K, A.cols, v[i]);
+    for (int i = 0; i < NV; ++i) v[i] = load_vec_raw<DT>(x, (int64_t)(i * G + lane) * K, A.cols);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+        float f[K];
+        to_floats<DT>(v[i], f);
 #pragma unroll
-        for (int k = 0; k < K; ++k) sum += v[i][k];
-    block_sum2<G>(sum, none, part);
+        for (int k = 0; k < K; ++k) sum += f[k];
+    }
+    block_sum2<G>(sum, none, part[0], lane);
     const float mean = sum / (float)A.cols;
     float sq = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+        float f[K];
+        hold(v[i]);
+        to_floats<DT>(v[i], f);
+        const int64_t c = (int64_t)(i * G + lane) * K;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            v[i][k] -= mean;
-            if ((int64_t)(i * G + lane) * K + k < A.cols) sq = __builtin_fmaf(v[i][k], v[i][k], sq);
+            const float d = c + k < A.cols ? f[k] - mean : 0.0f;
+            sq = __builtin_fmaf(d, d, sq);
         }
-    block_sum2<G>(sq, none, part);
+    }
+    block_sum2<G>(sq, none, part[1], lane);
     const float rstd = 1.0f / sqrtf(sq / (float)A.cols + A.eps);
     if (A.stats && lane == 0) {
         A.stats[2 * row] = mean;
@@ -79,12 +88,14 @@ __global__ __launch_bounds__(kNormThreads<G>) void k_norm(NormArgs A)
     for (int i = 0; i < NV; ++i) {
         const int64_t c = (int64_t)(i * G + lane) * K;
         if (c >= A.cols) break;
-        float w[K], b[K];
+        float f[K], w[K], b[K];
+        hold(v[i]);
+        to_floats<DT>(v[i], f);
         load_like<WT, K>(A.w, c, A.cols, 1.0f, w);
         load_like<WT, K>(A.b, c, A.cols, 0.0f, b);
 #pragma unroll
-        for (int k = 0; k < K; ++k) w[k] = __builtin_fmaf(v[i][k] * rstd, w[k], b[k]);
-        store_vec<DT>(y, c, A.cols, w);
+        for (int k = 0; k < K; ++k) w[k] = __builtin_fmaf((f[k] - mean) * rstd, w[k], b[k]);
+        stream_vec<DT>(y, c, A.cols, w);
     }
 }
 
@@ -93,7 +104,7 @@ template <int DT, int WT>
 __global__ __launch_bounds__(1024) void k_norm_long(NormArgs A)
 {
     constexpr int K = kLane<DT>, T = 1024;
-    __shared__ float part[2 * T / kWave];
+    __shared__ float part[2][2 * T / kWave];
     const int64_t row = blockIdx.x;
     const void* x = at<DT>(A.x, row * A.cols);
     float sum = 0.0f, sq = 0.0f, none = 0.0f, v[K];
@@ -102,7 +113,7 @@ __global__ __launch_bounds__(1024) void k_norm_long(NormArgs A)
 #pragma unroll
         for (int k = 0; k < K; ++k) sum += v[k];
     }
-    block_sum2<T>(sum, none, part);
+    block_sum2<T>(sum, none, part[0], threadIdx.x);
     const float mean = sum / (float)A.cols;
     for (int64_t c = (int64_t)threadIdx.x * K; c < A.cols; c += T * K) {
         load_vec<DT>(x, c, A.cols, v);
@@ -110,7 +121,7 @@ __global__ __launch_bounds__(1024) void k_norm_long(NormArgs A)
         for (int k = 0; k < K; ++k)
             if (c + k < A.cols) sq = __builtin_fmaf(v[k] - mean, v[k] - mean, sq);
     }
-    block_sum2<T>(sq, none, part);
+    block_sum2<T>(sq, none, part[1], threadIdx.x);
     const float rstd = 1.0f / sqrtf(sq / (float)A.cols + A.eps);
     if (A.stats && threadIdx.x == 0) {
         A.stats[2 * row] = mean;
@@ -124,50 +135,69 @@ __global__ __launch_bounds__(1024) void k_norm_long(NormArgs A)
         load_like<WT, K>(A.b, c, A.cols, 0.0f, b);
 #pragma unroll
         for (int k = 0; k < K; ++k) v[k] = __builtin_fmaf((v[k] - mean) * rstd, w[k], b[k]);
-        store_vec<DT>(y, c, A.cols, v);
+        stream_vec<DT>(y, c, A.cols, v);
     }
 }
 
-// dx and this workgroup's partial sums of dw and db.
-template <int DT, int WT, int G, int NV>
-__global__ __launch_bounds__(kNormThreads<G>) void k_norm_back(NormArgs A)
+// dx and this workgroup's partial sums of dw and db: T lanes, T / G rows at a time, every gridDim.x-th of them.  The next
+// rows are on their way while these are worked on (but in workgroups of 1024 lanes, which have no registers for
+// it, nor for the weights).
+template <int DT, int WT, int G, int NV, int T>
+__global__ __launch_bounds__(T) void k_norm_back(NormArgs A)
 {
-    constexpr int K = kLane<DT>, T = kNormThreads<G>, R = T / G;
-    __shared__ float part[2 * T / kWave];
+    constexpr int K = kLane<DT>, R = T / G;
+    constexpr bool AHEAD = T < 1024;
+    __shared__ float part[2][R][2 * G / kWave];
     __shared__ float cross[R > 1 ? 2 * R * G * K : 1];
     const int lane = threadIdx.x % G, sub = threadIdx.x / G;
     float w[NV][K], dw[NV][K], db[NV][K];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        load_like<WT, K>(A.w, (int64_t)(i * G + lane) * K, A.cols, 1.0f, w[i]);
+        if (AHEAD) load_like<WT, K>(A.w, (int64_t)(i * G + lane) * K, A.cols, 1.0f, w[i]);
 #pragma unroll
         for (int k = 0; k < K; ++k) dw[i][k] = db[i][k] = 0.0f;
     }
     const float inv = 1.0f / (float)A.cols;
-    for (int64_t row = (int64_t)blockIdx.x * R + sub; row < A.rows; row += (int64_t)gridDim.x * R) {
-        const void* xr = at<DT>(A.x, row * A.cols);
-        const void* gr = at<DT>(A.g, row * A.cols);
-        const float mean = A.stats[2 * row], rstd = A.stats[2 * row + 1];
+    const int64_t step = (int64_t)gridDim.x * R;
+    raw16 xr[NV], gr[NV];
+    float mean = 0.0f, rstd = 0.0f;
+    auto read = [&](int64_t r) {   // past the last row: zeros, which add nothing
+        const int64_t n = r < A.rows ? A.cols : 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            xr[i] = load_vec_raw<DT>(at<DT>(A.x, r * A.cols), (int64_t)(i * G + lane) * K, n);
+            gr[i] = load_vec_raw<DT>(at<DT>(A.g, r * A.cols), (int64_t)(i * G + lane) * K, n);
+        }
+        mean = n ? A.stats[2 * r] : 0.0f;
+        rstd = n ? A.stats[2 * r + 1] : 0.0f;
+    };
+    int64_t first = (int64_t)blockIdx.x * R;   // of the rows taken at a time: the same turns for all lanes
+    if (AHEAD && first < A.rows) read(first + sub);
+    for (int turn = 0; first < A.rows; first += step, turn ^= 1) {
+        const int64_t row = first + sub;
+        if (!AHEAD) read(row);
+        const float scale = rstd;
         float x[NV][K], g[NV][K];
         float c1 = 0.0f, c2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            load_vec<DT>(xr, (int64_t)(i * G + lane) * K, A.cols, x[i]);
-            load_vec<DT>(gr, (int64_t)(i * G + lane) * K, A.cols, g[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < NV; ++i)
+            to_floats<DT>(xr[i], x[i]);
+            to_floats<DT>(gr[i], g[i]);
+            if (!AHEAD) load_like<WT, K>(A.w, (int64_t)(i * G + lane) * K, A.cols, 1.0f, w[i]);
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                x[i][k] = (x[i][k] - mean) * rstd;
+                x[i][k] = (x[i][k] - mean) * scale;
                 dw[i][k] = __builtin_fmaf(g[i][k], x[i][k], dw[i][k]);
                 db[i][k] += g[i][k];
                 g[i][k] *= w[i][k];
                 c1 += g[i][k];
                 c2 = __builtin_fmaf(g[i][k], x[i][k], c2);
             }
+        }
+        if (AHEAD && first + step < A.rows) read(row + step);
         if (A.y) {
-            block_sum2<G>(c1, c2, part);
+            block_sum2<G>(c1, c2, part[turn][sub], lane);
+            if (row >= A.rows) continue;
             c1 *= inv;
             c2 *= inv;
             void* dx = at<DT>(A.y, row * A.cols);
@@ -176,17 +206,16 @@ __global__ __launch_bounds__(kNormThreads<G>) void k_norm_back(NormArgs A)
                 const int64_t c = (int64_t)(i * G + lane) * K;
                 if (c >= A.cols) break;
 #pragma unroll
-                for (int k = 0; k < K; ++k) g[i][k] = rstd * (g[i][k] - c1 - x[i][k] * c2);
-                store_vec<DT>(dx, c, A.cols, g[i]);
+                for (int k = 0; k < K; ++k) g[i][k] = scale * (g[i][k] - c1 - x[i][k] * c2);
+                stream_vec<DT>(dx, c, A.cols, g[i]);
             }
         }
     }
-    if (!A.part) return;
-    float* out = A.part + (int64_t)blockIdx.x * 2 * A.cols;
+    if (!A.dw && !A.db) return;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int64_t c = (int64_t)(i * G + lane) * K;
-        if constexpr (R > 1) {   // the wavefronts' sums, added in order
+        if constexpr (R > 1) {   // the rows' sums, added in order
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < K; ++k) {
@@ -204,13 +233,14 @@ __global__ __launch_bounds__(kNormThreads<G>) void k_norm_back(NormArgs A)
                     }
             }
         }
-        if (sub == 0) {
-#pragma unroll
-            for (int k = 0; k < K; ++k)
-                if (c + k < A.cols) {
-                    out[c + k] = dw[i][k];
-                    out[A.cols + c + k] = db[i][k];
-                }
+        if (sub > 0 || c >= A.cols) continue;
+        if (gridDim.x == 1) {   // the only workgroup: its sums are the gradients
+            if (A.dw) store_like<WT, K>(A.dw, c, A.cols, dw[i]);
+            if (A.db) store_like<WT, K>(A.db, c, A.cols, db[i]);
+        } else {
+            float* out = A.part + (int64_t)blockIdx.x * 2 * A.cols;
+            store_like<DT_F32, K>(out, c, A.cols, dw[i]);
+            store_like<DT_F32, K>(out + A.cols, c, A.cols, db[i]);
         }
     }
 }
@@ -220,7 +250,7 @@ template <int DT, int WT>
 __global__ __launch_bounds__(1024) void k_norm_back_long(NormArgs A)
 {
     constexpr int K = kLane<DT>, T = 1024;
-    __shared__ float part[2 * T / kWave];
+    __shared__ float part[2][2 * T / kWave];
     const int64_t row = blockIdx.x;
     const void* xr = at<DT>(A.x, row * A.cols);
     const void* gr = at<DT>(A.g, row * A.cols);
@@ -236,7 +266,7 @@ __global__ __launch_bounds__(1024) void k_norm_back_long(NormArgs A)
             c2 = __builtin_fmaf(g[k] * w[k], (x[k] - mean) * rstd, c2);
         }
     }
-    block_sum2<T>(c1, c2, part);
+    block_sum2<T>(c1, c2, part[0], threadIdx.x);
     c1 /= (float)A.cols;
     c2 /= (float)A.cols;
     void* dx = at<DT>(A.y, row * A.cols);
@@ -246,7 +276,7 @@ __global__ __launch_bounds__(1024) void k_norm_back_long(NormArgs A)
         load_like<WT, K>(A.w, c, A.cols, 1.0f, w);
 #pragma unroll
         for (int k = 0; k < K; ++k) g[k] = rstd * (g[k] * w[k] - c1 - (x[k] - mean) * rstd * c2);
-        store_vec<DT>(dx, c, A.cols, g);
+        stream_vec<DT>(dx, c, A.cols, g);
     }
 }
 
@@ -279,85 +309,122 @@ __global__ __launch_bounds__(256) void k_norm_columns(NormArgs A)
         }
 }
 
-// The P partial sums of 64 columns a workgroup: 16 lanes a column each take every 16th, then a tree.
-constexpr int kSumLanes = 16;
-
-template <int WT>
-__global__ __launch_bounds__(64 * kSumLanes) void k_norm_sums(const float* part, int32_t parts, int64_t cols, void* dw, void* db)
+// The P partial sums of 64 columns a workgroup: L lanes of 4 columns each take every L-th, then their sums in order.
+template <int WT, int L>
+__global__ __launch_bounds__(16 * L) void k_norm_sums(NormArgs A, int32_t parts)
 {
-    __shared__ float tree[kSumLanes][64];
-    const int col = threadIdx.x & 63, at_row = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + col;   // of 2 cols: dw's, then db's
-    float s = 0.0f;
-    if (c < 2 * cols)
-        for (int p = at_row; p < parts; p += kSumLanes) s += part[(int64_t)p * 2 * cols + c];
-    tree[at_row][col] = s;
-    for (int d = kSumLanes / 2; d; d /= 2) {
-        __syncthreads();
-        if (at_row < d) tree[at_row][col] += tree[at_row + d][col];
+    __shared__ float sums[L][64 + 4];
+    const int col = (threadIdx.x & 15) * 4, at_row = threadIdx.x >> 4;
+    const int64_t c0 = (int64_t)blockIdx.x * 64;   // of 2 cols: dw's, then db's
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (c0 + col < 2 * A.cols) {
+#pragma unroll 4
+        for (int p = at_row; p < parts; p += L) {
+            float x[4];
+            load_vec<DT_F32>(A.part + (int64_t)p * 2 * A.cols, c0 + col, 2 * A.cols, x);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[k] += x[k];
+        }
     }
-    if (at_row == 0 && c < 2 * cols) {
-        void* out = c < cols ? dw : db;
-        if (out) put<WT>(out, c < cols ? c : c - cols, tree[0][col]);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) sums[at_row][col + k] = s[k];
+    __syncthreads();
+    if constexpr (L > 16) {   // sixteen at a time first
+        float some = 0.0f;
+        const int g = threadIdx.x >> 6, cc = threadIdx.x & 63;
+        if (g < L / 16)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) some += sums[16 * g + i][cc];
+        __syncthreads();
+        if (g < L / 16) sums[g][cc] = some;
+        __syncthreads();
+    }
+    const int64_t c = c0 + threadIdx.x;
+    if (threadIdx.x < 64 && c < 2 * A.cols) {
+        float all = 0.0f;
+#pragma unroll
+        for (int i = 0; i < (L > 16 ? L / 16 : 16); ++i) all += sums[i][threadIdx.x];
+        void* out = c < A.cols ? A.dw : A.db;
+        if (out) put<WT>(out, c < A.cols ? c : c - A.cols, all);
     }
 }
 
 static bool type_ok(int32_t t) { return t == ADAMBRIDGE_DT_F32 || t == ADAMBRIDGE_DT_BF16; }
 
-// Lanes a row (0: the long form) and vectors a lane.  Backward, whose lanes hold five values a column, the
-// registers of 1024 lanes end at two.
+// Lanes a row (0: the long form), values a lane, lanes of a workgroup.
 struct Shape {
-    int lanes, vectors;
+    int lanes, values, group;
 };
 
-static Shape norm_shape(int64_t cols, int32_t dtype, bool back)
+// Few rows are spread over more lanes: what counts then is how long one row takes.
+static Shape norm_shape(int64_t rows, int64_t cols)
 {
-    const int64_t v = (cols + (dtype == ADAMBRIDGE_DT_BF16 ? 7 : 3)) / (dtype == ADAMBRIDGE_DT_BF16 ? 8 : 4);
-    if (v <= 64) return {64, 1};
-    if (v <= 128) return {64, 2};
-    if (v <= 256) return {64, 4};
-    if (v <= 512) return {256, 2};
-    if (v <= 1024) return {256, 4};
-    if (v <= 2048) return {1024, 2};
-    if (v <= 4096 && !back) return {1024, 4};
-    return {0, 0};
+    if (cols <= 512) return {64, 8, 256};
+    if (cols <= 1024) return {64, 16, 256};
+    if (rows < 1024) {
+        if (cols <= 2048) return {256, 8, 256};
+        if (cols <= 4096) return {256, 16, 256};
+        if (cols <= 8192) return {512, 16, 512};
+        if (cols <= 16384) return {1024, 16, 1024};
+        return {0, 0, 0};
+    }
+    if (cols <= 2048) return {64, 32, 256};
+    if (cols <= 4096) return {64, 64, 256};
+    if (cols <= 8192) return {256, 32, 256};
+    if (cols <= 16384) return {512, 32, 512};
+    return {0, 0, 0};
 }
 
-// Workgroups of the backward pass, each with its partial sums.
-static int norm_parts(int64_t rows, int64_t cols, int32_t dtype)
+// Backward a lane holds five values a column and the next row's two: fewer columns a lane.
+static Shape norm_back_shape(int64_t cols)
 {
-    const Shape s = norm_shape(cols, dtype, true);
-    const int64_t a_group = s.lanes == 64 ? 4 : 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(512, (rows + a_group * 4 - 1) / (a_group * 4)));
+    if (cols <= 512) return {64, 8, 512};
+    if (cols <= 1024) return {64, 16, 512};
+    if (cols <= 2048) return {256, 8, 512};
+    if (cols <= 4096) return {256, 16, 512};
+    if (cols <= 8192) return {512, 16, 512};
+    if (cols <= 16384) return {1024, 16, 1024};
+    return {0, 0, 0};
+}
+
+// Workgroups of the backward pass, each with its partial sums: one a CU, of two turns at least (65536 x 4096 BF16: 287 us; 512
+// workgroups 294, 768 325 and 1024 350, as the partial sums grow and more rows compete).
+static int norm_parts(int64_t rows, int64_t cols)
+{
+    const Shape s = norm_back_shape(cols);
+    const int64_t at_a_time = s.lanes ? s.group / s.lanes : 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(256, (rows + at_a_time * 2 - 1) / (at_a_time * 2)));
 }
 
 template <int DT, int WT>
 static void launch_norm(const NormArgs& A, bool back, int parts)
 {
-    const Shape s = norm_shape(A.cols, DT, back);
-#define ABH_NORM(G, NV)                                                                                                 \
-    if (!back && s.lanes == G && s.vectors == NV) {                                                                     \
+    constexpr int K = kLane<DT>;
+    const Shape s = back ? norm_back_shape(A.cols) : norm_shape(A.rows, A.cols);
+#define ABH_NORM(G, N)                                                                                                  \
+    if (!back && s.lanes == G && s.values == N) {                                                                       \
         constexpr int R = kNormThreads<G> / G;                                                                          \
-        hipLaunchKernelGGL((k_norm<DT, WT, G, NV>), dim3((unsigned)((A.rows + R - 1) / R)), dim3(kNormThreads<G>), 0,    \
+        hipLaunchKernelGGL((k_norm<DT, WT, G, N / K>), dim3((unsigned)((A.rows + R - 1) / R)), dim3(kNormThreads<G>), 0, \
                            t_stream, A);                                                                                \
         return;                                                                                                         \
     }
-    ABH_NORM(64, 1) ABH_NORM(64, 2) ABH_NORM(64, 4) ABH_NORM(256, 2) ABH_NORM(256, 4) ABH_NORM(1024, 2) ABH_NORM(1024, 4)
+    ABH_NORM(64, 8) ABH_NORM(64, 16) ABH_NORM(64, 32) ABH_NORM(64, 64) ABH_NORM(256, 8) ABH_NORM(256, 16) ABH_NORM(256, 32)
+    ABH_NORM(512, 16) ABH_NORM(512, 32) ABH_NORM(1024, 16)
 #undef ABH_NORM
-#define ABH_NORM_BACK(G, NV)                                                                                            \
-    if (back && s.lanes == G && s.vectors == NV) {                                                                      \
-        hipLaunchKernelGGL((k_norm_back<DT, WT, G, NV>), dim3(parts), dim3(kNormThreads<G>), 0, t_stream, A);            \
+#define ABH_NORM_BACK(G, N, T)                                                                                          \
+    if (back && s.lanes == G && s.values == N && s.group == T) {                                                        \
+        hipLaunchKernelGGL((k_norm_back<DT, WT, G, N / K, T>), dim3(parts), dim3(T), 0, t_stream, A);                    \
         return;                                                                                                         \
     }
-    ABH_NORM_BACK(64, 1) ABH_NORM_BACK(64, 2) ABH_NORM_BACK(64, 4) ABH_NORM_BACK(256, 2) ABH_NORM_BACK(256, 4)
-    ABH_NORM_BACK(1024, 2)
+    ABH_NORM_BACK(64, 8, 512) ABH_NORM_BACK(64, 16, 512) ABH_NORM_BACK(256, 8, 512) ABH_NORM_BACK(256, 16, 512)
+    ABH_NORM_BACK(512, 16, 512) ABH_NORM_BACK(1024, 16, 1024)
 #undef ABH_NORM_BACK
     if (!back) {
         hipLaunchKernelGGL((k_norm_long<DT, WT>), dim3((unsigned)A.rows), dim3(1024), 0, t_stream, A);
         return;
     }
     if (A.y) hipLaunchKernelGGL((k_norm_back_long<DT, WT>), dim3((unsigned)A.rows), dim3(1024), 0, t_stream, A);
-    if (A.part)
+    if (A.dw || A.db)
         hipLaunchKernelGGL((k_norm_columns<DT>), dim3((unsigned)((A.cols + 256 * kLane<DT> - 1) / (256 * kLane<DT>)), (unsigned)parts),
                            dim3(256), 0, t_stream, A);
 }
@@ -385,7 +452,7 @@ ADAMBRIDGE_API int adambridge_layer_norm(const void* x, int32_t dtype, const voi
     if (rows < 1 || cols < 1 || rows > kNormMost || cols > kNormMost) return ADAMBRIDGE_EBADN;
     if (!type_ok(dtype) || !type_ok(w_dtype)) return ADAMBRIDGE_EMVDTYPE;
     if (!x || !y) return ADAMBRIDGE_ENULL;
-    const NormArgs A{x, nullptr, weight, bias, y, stats, nullptr, rows, cols, eps};
+    const NormArgs A{x, nullptr, weight, bias, y, stats, nullptr, nullptr, nullptr, rows, cols, eps};
     norm_by_type(A, dtype, w_dtype, false, 0);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : hip_fail(e, "hipLaunchKernelGGL (layer norm)");
@@ -395,7 +462,7 @@ ADAMBRIDGE_API int64_t adambridge_layer_norm_work(int64_t rows, int64_t cols, in
 {
     if (rows < 1 || cols < 1 || rows > kNormMost || cols > kNormMost) return ADAMBRIDGE_EBADN;
     if (!type_ok(dtype)) return ADAMBRIDGE_EMVDTYPE;
-    return (int64_t)norm_parts(rows, cols, dtype) * 2 * cols * 4;
+    return (int64_t)norm_parts(rows, cols) * 2 * cols * 4;
 }
 
 ADAMBRIDGE_API int adambridge_layer_norm_backward(const void* gout, const void* x, int32_t dtype, const void* weight,
@@ -407,16 +474,17 @@ ADAMBRIDGE_API int adambridge_layer_norm_backward(const void* gout, const void* 
     const bool sums = dweight || dbias;
     if (!gout || !x || !stats || (sums && !work)) return ADAMBRIDGE_ENULL;
     if (!dx && !sums) return 0;
-    const int parts = norm_parts(rows, cols, dtype);
-    const NormArgs A{x, gout, weight, nullptr, dx, const_cast<float*>(stats), sums ? static_cast<float*>(work) : nullptr,
+    const int parts = norm_parts(rows, cols);
+    const NormArgs A{x, gout, weight, nullptr, dx, const_cast<float*>(stats), dweight, dbias, static_cast<float*>(work),
                      rows, cols, 0.0f};
     norm_by_type(A, dtype, w_dtype, true, parts);
-    if (sums) {
-        const dim3 grid((unsigned)((2 * cols + 63) / 64)), block(64 * kSumLanes);
-        if (w_dtype == ADAMBRIDGE_DT_BF16)
-            hipLaunchKernelGGL((k_norm_sums<DT_BF16>), grid, block, 0, t_stream, A.part, parts, cols, dweight, dbias);
-        else
-            hipLaunchKernelGGL((k_norm_sums<DT_F32>), grid, block, 0, t_stream, A.part, parts, cols, dweight, dbias);
+    if (sums && (parts > 1 || !norm_back_shape(cols).lanes)) {
+        const dim3 grid((unsigned)((2 * cols + 63) / 64));
+        const bool bf = w_dtype == ADAMBRIDGE_DT_BF16, few = parts <= 64;
+        if (bf && few) hipLaunchKernelGGL((k_norm_sums<DT_BF16, 16>), grid, dim3(256), 0, t_stream, A, parts);
+        else if (bf) hipLaunchKernelGGL((k_norm_sums<DT_BF16, 64>), grid, dim3(1024), 0, t_stream, A, parts);
+        else if (few) hipLaunchKernelGGL((k_norm_sums<DT_F32, 16>), grid, dim3(256), 0, t_stream, A, parts);
+        else hipLaunchKernelGGL((k_norm_sums<DT_F32, 64>), grid, dim3(1024), 0, t_stream, A, parts);
     }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : hip_fail(e, "hipLaunchKernelGGL (layer norm's gradient)");

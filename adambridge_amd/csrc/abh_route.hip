@@ -29,7 +29,7 @@
 namespace abh {
 
 constexpr int kBlockTokens = 64;
-constexpr int kRouteThreads = 256;
+constexpr int kRouteThreads = 1024;   // so that a block of tokens is chosen from in few passes: blocks are few
 constexpr int kMostExperts = 1024;
 constexpr int kMostChosen = 64;
 constexpr float kRouteLog2e = 1.4426950408889634f;
@@ -65,20 +65,7 @@ __device__ __forceinline__ float exp_below(float x, float m)
 template <int G>
 __device__ __forceinline__ uint32_t group_max(uint32_t x)
 {
-#pragma unroll
-    for (int d = 1; d < G; d *= 2) {
-        const uint32_t y = (uint32_t)__shfl_xor((int)x, d);
-        x = x > y ? x : y;
-    }
-    return x;
-}
-
-template <int G>
-__device__ __forceinline__ float group_sum(float x)
-{
-#pragma unroll
-    for (int d = 1; d < G; d *= 2) x += __shfl_xor(x, d);
-    return x;
+    return group_reduce<G>(x, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
 
 // Masks of a block's tokens by expert, and the rows of its assignments: base[e] + the bits below.
@@ -106,8 +93,9 @@ __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs A)
     const int tokens = (int)(A.tokens - t0 < kBlockTokens ? A.tokens - t0 : kBlockTokens);
     for (int e = threadIdx.x; e < A.experts; e += kRouteThreads) mask[e] = 0;
     __syncthreads();
-    for (int t = sub; t < kBlockTokens; t += kPass) {   // the same for all lanes: whole groups take part in the sums
+    for (int t = sub; t < kBlockTokens; t += kPass) {
         const bool real = t < tokens;
+        if (!__builtin_amdgcn_ballot_w64(real)) break;   // a wavefront's groups go on together: they share its sums' lanes
         float x[NV];
         uint32_t key[NV];
         const int64_t row = (t0 + (real ? t : 0)) * A.experts;
@@ -203,8 +191,7 @@ __global__ __launch_bounds__(1024) void k_route_bases(RouteArgs A)
         s += (int32_t)((w & 255u) + (w >> 8 & 255u) + (w >> 16 & 255u) + (w >> 24));
     }
     for (int64_t i = n / 4 * 4 + threadIdx.x; i < n; i += T) s += A.counts[i];
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) s += __shfl_xor(s, d);
+    s = group_reduce<kWave>(s, [](int32_t a, int32_t b) { return a + b; });
     if (lane == 0) part[wave] = s;
     __syncthreads();
     int32_t before = 0;
@@ -269,8 +256,7 @@ __global__ __launch_bounds__(256) void k_route_back(const float* weights, const 
             most = __builtin_fmaxf(most, x);
             nan |= x != x;
         }
-#pragma unroll
-        for (int d = 1; d < kWave; d *= 2) most = __builtin_fmaxf(most, __shfl_xor(most, d));
+        most = group_reduce<kWave>(most, [](float a, float b) { return __builtin_fmaxf(a, b); });
         top = __builtin_amdgcn_ballot_w64(nan) ? __builtin_nanf("") : most;
         for (int e = lane; e < experts; e += kWave) sum += exp_below(get<DT>(logits, row + e), top);
         sum = wave_sum(sum);
@@ -280,13 +266,10 @@ __global__ __launch_bounds__(256) void k_route_back(const float* weights, const 
         const int e = e0 + lane;
         float seed = 0.0f;   // w g of the assignment to e, if there is one
         float own = 0.0f;
-        for (int j = 0; j < top_k; ++j) {
-            const int c = __shfl(at, j);
-            const float wj = __shfl(w, j), gj = __shfl(g, j);
-            if (c == e) {
-                seed = wj * gj;
-                own = wj;
-            }
+        for (int j = 0; j < top_k; ++j) {   // of one token: scalars
+            const bool mine = __builtin_amdgcn_readlane(at, j) == e;
+            seed = mine ? bitsf(__builtin_amdgcn_readlane(fbits(w * g), j)) : seed;
+            own = mine ? bitsf(__builtin_amdgcn_readlane(fbits(w), j)) : own;
         }
         if (e >= experts) continue;
         if (!normalize) own = exp_below(get<DT>(logits, row + e), top) * inv;
@@ -307,76 +290,128 @@ struct ShuffleArgs {
     int32_t top_k;
 };
 
-// The row of an assignment; -1 where it is none (a position that no routing gives): nothing is read or written there.
-__device__ __forceinline__ int64_t row_of(const ShuffleArgs& A, int64_t a)
+// The rows of a token's assignments, one a lane; -1 where it is none (a position that no routing gives): nothing is
+// read or written there.  One load for all of them, not one before each row.
+__device__ __forceinline__ int rows_of(const ShuffleArgs& A, int64_t t)
 {
-    const int64_t r = A.position[a];
+    const int lane = threadIdx.x & 63;
+    const int r = lane < A.top_k ? A.position[t * A.top_k + lane] : -1;
     return r >= 0 && r < A.tokens * A.top_k ? r : -1;
 }
 
-// out[position[t, j]] = x[t]: the token's row read once, written top_k times.  A wavefront takes 64 vectors of a token.
+// Tokens have a wavefront each, which takes `vectors` vectors of a lane of it (blockIdx.y the ones after).
+struct Place {
+    int64_t t, c0, c1;
+};
+
 template <int DT>
-__global__ __launch_bounds__(256) void k_dispatch(ShuffleArgs A)
+__device__ __forceinline__ bool place_of(const ShuffleArgs& A, int vectors, Place& p)
+{
+    constexpr int64_t a_load = kWave * kLane<DT>;
+    p.t = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    p.c0 = (int64_t)blockIdx.y * vectors * a_load + (threadIdx.x & 63) * kLane<DT>;
+    p.c1 = ((int64_t)blockIdx.y + 1) * vectors * a_load;
+    p.c1 = p.c1 < A.cols ? p.c1 : A.cols;
+    return p.t < A.tokens;
+}
+
+// out[position[t, j]] = x[t]: the token's row read once, written top_k times.
+template <int DT>
+__global__ __launch_bounds__(256) void k_dispatch(ShuffleArgs A, int vectors)
 {
     constexpr int K = kLane<DT>;
-    const int64_t t = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
-    const int64_t c = ((int64_t)blockIdx.y * kWave + (threadIdx.x & 63)) * K;
-    if (t >= A.tokens || c >= A.cols) return;
-    float v[K];
-    load_vec<DT>(at<DT>(A.x, t * A.cols), c, A.cols, v);
-    for (int j = 0; j < A.top_k; ++j) {
-        const int64_t r = row_of(A, t * A.top_k + j);
-        if (r >= 0) store_vec<DT>(at<DT>(A.out, r * A.cols), c, A.cols, v);
+    Place p;
+    if (!place_of<DT>(A, vectors, p)) return;
+    const int rows = rows_of(A, p.t);
+    for (int64_t c = p.c0; c < p.c1; c += kWave * K) {
+        const raw16 v = load_vec_raw<DT>(at<DT>(A.x, p.t * A.cols), c, A.cols);
+        float f[K];
+        to_floats<DT>(v, f);
+        for (int j = 0; j < A.top_k; ++j) {
+            const int r = __builtin_amdgcn_readlane(rows, j);
+            if (r < 0) continue;
+            void* out = at<DT>(A.out, (int64_t)r * A.cols);
+            if (c + K <= A.cols) stream_raw<DT>(out, c, v);
+            else stream_vec<DT>(out, c, A.cols, f);
+        }
     }
 }
 
-// out[t] = sum over j of weights[t, j] x[position[t, j]] (without weights: of the rows), in order, rounded once.
+// out[t] = sum over j of weights[t, j] x[position[t, j]] (without weights: of the rows), in order, rounded once.  The
+// rows of four choices are on their way at a time.
 template <int DT>
-__global__ __launch_bounds__(256) void k_combine(ShuffleArgs A)
+__global__ __launch_bounds__(256) void k_combine(ShuffleArgs A, int vectors)
 {
-    constexpr int K = kLane<DT>;
-    const int64_t t = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
-    const int64_t c = ((int64_t)blockIdx.y * kWave + (threadIdx.x & 63)) * K;
-    if (t >= A.tokens || c >= A.cols) return;
-    float s[K];
+    constexpr int K = kLane<DT>, U = 4;
+    Place p;
+    if (!place_of<DT>(A, vectors, p)) return;
+    const int rows = rows_of(A, p.t), lane = threadIdx.x & 63;
+    const float weight = !A.weights ? 1.0f : lane < A.top_k ? A.weights[p.t * A.top_k + lane] : 0.0f;
+    for (int64_t c = p.c0; c < p.c1; c += kWave * K) {
+        float s[K];
 #pragma unroll
-    for (int k = 0; k < K; ++k) s[k] = 0.0f;
-    for (int j = 0; j < A.top_k; ++j) {
-        const int64_t a = t * A.top_k + j, r = row_of(A, a);
-        if (r < 0) continue;
-        const float w = A.weights ? A.weights[a] : 1.0f;
-        float v[K];
-        load_vec<DT>(at<DT>(A.x, r * A.cols), c, A.cols, v);
+        for (int k = 0; k < K; ++k) s[k] = 0.0f;
+        for (int j0 = 0; j0 < A.top_k; j0 += U) {
+            raw16 v[U];
+            int r[U];
 #pragma unroll
-        for (int k = 0; k < K; ++k) s[k] = __builtin_fmaf(w, v[k], s[k]);
+            for (int u = 0; u < U; ++u) {
+                r[u] = j0 + u < A.top_k ? __builtin_amdgcn_readlane(rows, j0 + u) : -1;
+                if (r[u] >= 0) v[u] = load_vec_raw<DT>(at<DT>(A.x, (int64_t)r[u] * A.cols), c, A.cols);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if (r[u] < 0) continue;
+                const float w = bitsf(__builtin_amdgcn_readlane(fbits(weight), j0 + u));
+                float f[K];
+                to_floats<DT>(v[u], f);
+#pragma unroll
+                for (int k = 0; k < K; ++k) s[k] = __builtin_fmaf(w, f[k], s[k]);
+            }
+        }
+        stream_vec<DT>(at<DT>(A.out, p.t * A.cols), c, A.cols, s);
     }
-    store_vec<DT>(at<DT>(A.out, t * A.cols), c, A.cols, s);
 }
 
 // An assignment a wavefront: out[row] = w g[t], dw = <g[t], x[row]>.
 template <int DT>
 __global__ __launch_bounds__(256) void k_combine_back(ShuffleArgs A)
 {
-    constexpr int K = kLane<DT>;
+    constexpr int K = kLane<DT>, U = 4;
     const int lane = threadIdx.x & 63;
-    const int64_t a = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
+    const int64_t a = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if (a >= A.tokens * A.top_k) return;
-    const int64_t t = a / A.top_k, r = row_of(A, a);
+    const int64_t t = a / A.top_k, r = A.position[a];
     float dot = 0.0f;
-    if (r >= 0) {
+    if (r >= 0 && r < A.tokens * A.top_k) {
         const float w = A.weights[a];
-        for (int64_t c = (int64_t)lane * K; c < A.cols; c += kWave * K) {
-            float g[K], v[K];
-            load_vec<DT>(at<DT>(A.g, t * A.cols), c, A.cols, g);
-            if (A.dw) {
-                load_vec<DT>(at<DT>(A.x, r * A.cols), c, A.cols, v);
+        const void* gt = at<DT>(A.g, t * A.cols);
+        const void* xr = at<DT>(A.x, r * A.cols);
+        for (int64_t c = (int64_t)lane * K; c < A.cols; c += U * kWave * K) {
+            raw16 g[U], v[U];
 #pragma unroll
-                for (int k = 0; k < K; ++k) dot = __builtin_fmaf(g[k], v[k], dot);
+            for (int u = 0; u < U; ++u) {
+                const int64_t cu = c + u * kWave * K;
+                if (cu >= A.cols) continue;
+                g[u] = load_vec_raw<DT>(gt, cu, A.cols);
+                if (A.dw) v[u] = load_vec_raw<DT>(xr, cu, A.cols);
             }
-            if (A.out) {
 #pragma unroll
-                for (int k = 0; k < K; ++k) g[k] *= w;
-                store_vec<DT>(at<DT>(A.out, r * A.cols), c, A.cols, g);
+            for (int u = 0; u < U; ++u) {
+                const int64_t cu = c + u * kWave * K;
+                if (cu >= A.cols) continue;
+                float gf[K], vf[K];
+                to_floats<DT>(g[u], gf);
+                if (A.dw) {
+                    to_floats<DT>(v[u], vf);
+#pragma unroll
+                    for (int k = 0; k < K; ++k) dot = __builtin_fmaf(gf[k], vf[k], dot);
+                }
+                if (A.out) {
+#pragma unroll
+                    for (int k = 0; k < K; ++k) gf[k] *= w;
+                    stream_vec<DT>(at<DT>(A.out, r * A.cols), cu, A.cols, gf);
+                }
             }
         }
     }
@@ -423,9 +458,13 @@ static int shuffle_check(const void* a, const void* out, const int32_t* position
     return a && out && position ? 0 : ADAMBRIDGE_ENULL;
 }
 
-static dim3 shuffle_grid(const ShuffleArgs& A, int32_t dtype)
+// Many tokens: a wavefront takes `many` vectors a lane of a token.  Few: one, so that more wavefronts share them.
+static int shuffle_vectors(const ShuffleArgs& A, int many) { return A.tokens >= 2048 ? many : 1; }
+constexpr int kDispatchVectors = 1 << 20, kCombineVectors = 8;
+
+static dim3 shuffle_grid(const ShuffleArgs& A, int32_t dtype, int vectors)
 {
-    const int64_t a_wave = kWave * (dtype == ADAMBRIDGE_DT_BF16 ? kLane<DT_BF16> : kLane<DT_F32>);
+    const int64_t a_wave = (int64_t)vectors * kWave * (dtype == ADAMBRIDGE_DT_BF16 ? kLane<DT_BF16> : kLane<DT_F32>);
     return dim3((unsigned)((A.tokens + 3) / 4), (unsigned)((A.cols + a_wave - 1) / a_wave));
 }
 
@@ -485,8 +524,9 @@ ADAMBRIDGE_API int adambridge_dispatch(const void* x, int32_t dtype, const int32
 {
     if (const int rc = shuffle_check(x, rows, position, dtype, tokens, top_k, cols)) return rc;
     const ShuffleArgs A{x, nullptr, nullptr, position, rows, nullptr, tokens, cols, (int32_t)top_k};
-    if (dtype == ADAMBRIDGE_DT_BF16) hipLaunchKernelGGL((k_dispatch<DT_BF16>), shuffle_grid(A, dtype), dim3(256), 0, t_stream, A);
-    else hipLaunchKernelGGL((k_dispatch<DT_F32>), shuffle_grid(A, dtype), dim3(256), 0, t_stream, A);
+    const int vectors = shuffle_vectors(A, kDispatchVectors);
+    if (dtype == ADAMBRIDGE_DT_BF16) hipLaunchKernelGGL((k_dispatch<DT_BF16>), shuffle_grid(A, dtype, vectors), dim3(256), 0, t_stream, A, vectors);
+    else hipLaunchKernelGGL((k_dispatch<DT_F32>), shuffle_grid(A, dtype, vectors), dim3(256), 0, t_stream, A, vectors);
     return done("hipLaunchKernelGGL (dispatch)");
 }
 
@@ -495,8 +535,9 @@ ADAMBRIDGE_API int adambridge_combine(const void* rows, int32_t dtype, const flo
 {
     if (const int rc = shuffle_check(rows, out, position, dtype, tokens, top_k, cols)) return rc;
     const ShuffleArgs A{rows, nullptr, weights, position, out, nullptr, tokens, cols, (int32_t)top_k};
-    if (dtype == ADAMBRIDGE_DT_BF16) hipLaunchKernelGGL((k_combine<DT_BF16>), shuffle_grid(A, dtype), dim3(256), 0, t_stream, A);
-    else hipLaunchKernelGGL((k_combine<DT_F32>), shuffle_grid(A, dtype), dim3(256), 0, t_stream, A);
+    const int vectors = shuffle_vectors(A, kCombineVectors);
+    if (dtype == ADAMBRIDGE_DT_BF16) hipLaunchKernelGGL((k_combine<DT_BF16>), shuffle_grid(A, dtype, vectors), dim3(256), 0, t_stream, A, vectors);
+    else hipLaunchKernelGGL((k_combine<DT_F32>), shuffle_grid(A, dtype, vectors), dim3(256), 0, t_stream, A, vectors);
     return done("hipLaunchKernelGGL (combine)");
 }
 

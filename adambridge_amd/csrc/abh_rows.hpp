@@ -94,6 +94,13 @@ __device__ __forceinline__ void store_raw(void* base, int64_t i, raw16 w)
 {
     *reinterpret_cast<typename Vec16<DT>::type*>(at<DT>(base, i)) = w;
 }
+// For results that the kernel does not read again: not kept in the caches in place of what it reads (4096 x 2048 layer norm
+// 9.8 -> 7.7 us, combine of 16384 x 4 rows of 2048 79 -> 51; reads of that kind gained in none).
+template <int DT>
+__device__ __forceinline__ void stream_raw(void* base, int64_t i, raw16 w)
+{
+    __builtin_nontemporal_store(w, reinterpret_cast<typename Vec16<DT>::type*>(at<DT>(base, i)));
+}
 
 // Values i .. i + kLane - 1 of a row of n, zeros past its end.
 template <int DT>
@@ -108,15 +115,25 @@ __device__ __forceinline__ void load_vec(const void* row, int64_t i, int64_t n, 
 }
 
 template <int DT>
-__device__ __forceinline__ void store_vec(void* row, int64_t i, int64_t n, const float* x)
+__device__ __forceinline__ void stream_vec(void* row, int64_t i, int64_t n, const float* x)
 {
     if (i + kLane<DT> <= n) {
-        store_raw<DT>(row, i, to_raw<DT>(x));
+        stream_raw<DT>(row, i, to_raw<DT>(x));
     } else {
 #pragma unroll
         for (int k = 0; k < kLane<DT>; ++k)
             if (i + k < n) put<DT>(row, i + k, x[k]);
     }
+}
+
+// The same as they lie in memory.
+template <int DT>
+__device__ __forceinline__ raw16 load_vec_raw(const void* row, int64_t i, int64_t n)
+{
+    if (i + kLane<DT> <= n) return load_raw<DT>(row, i);
+    float x[kLane<DT>];
+    load_vec<DT>(row, i, n, x);
+    return to_raw<DT>(x);   // exact
 }
 
 // N values of WT at i .. of a row of n (N a lane's values of another type), `none` without a row.
@@ -140,25 +157,69 @@ __device__ __forceinline__ void load_like(const void* row, int64_t i, int64_t n,
     }
 }
 
-__device__ __forceinline__ float wave_sum(float x)
+// A value of another lane, chosen by a pattern of the data-parallel primitives (no LDS): the lanes paired are each
+// other's, so that a sum over pairs is the same in both.
+template <int PATTERN, class T>
+__device__ __forceinline__ T paired(T x)
 {
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) x += __shfl_xor(x, d);
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    return __builtin_bit_cast(T, (uint32_t)__builtin_amdgcn_update_dpp((int)u, (int)u, PATTERN, 0xf, 0xf, false));
+}
+
+// op over groups of G (2 .. 64) neighbouring lanes, the same result in every lane of a group.
+template <int G, class T, class Op>
+__device__ __forceinline__ T group_reduce(T x, Op op)
+{
+    if constexpr (G >= 2) x = op(x, paired<0xb1>(x));    // lanes 1 0 3 2
+    if constexpr (G >= 4) x = op(x, paired<0x4e>(x));    // 2 3 0 1
+    if constexpr (G >= 8) x = op(x, paired<0x141>(x));   // 7 - i of 8
+    if constexpr (G >= 16) x = op(x, paired<0x140>(x));  // 15 - i of 16
+    if constexpr (G >= 32) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, x);
+        const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);   // even sixteens' and odd sixteens'
+        x = op(__builtin_bit_cast(T, (uint32_t)s[0]), __builtin_bit_cast(T, (uint32_t)s[1]));
+    }
+    if constexpr (G >= 64) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, x);
+        const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        x = op(__builtin_bit_cast(T, (uint32_t)s[0]), __builtin_bit_cast(T, (uint32_t)s[1]));
+    }
     return x;
 }
 
-// Two sums over a workgroup of T lanes, for every lane, in an order of their own whatever the schedule.  `part` is
-// 2 T / 64 floats of LDS; a workgroup of one wavefront uses none.
+template <int G>
+__device__ __forceinline__ float group_sum(float x)
+{
+    return group_reduce<G>(x, [](float a, float b) { return a + b; });
+}
+// The other way: N values to a row of n of another type.
+template <int WT, int N>
+__device__ __forceinline__ void store_like(void* row, int64_t i, int64_t n, const float* x)
+{
+    if (i + N <= n && N >= kLane<WT>) {
+#pragma unroll
+        for (int k = 0; k < N; k += kLane<WT>) store_raw<WT>(row, i + k, to_raw<WT>(x + k));
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+            if (i + k < n) put<WT>(row, i + k, x[k]);
+    }
+}
+
+__device__ __forceinline__ float wave_sum(float x) { return group_sum<kWave>(x); }
+
+// Two sums over T lanes of a workgroup whose lanes all take part (in groups of T, this one's number `lane` in its own), for
+// each of them, in an order of its own whatever the schedule.  `part` is the group's 2 T / 64 floats of LDS, not
+// those of the call before: two that take turns need one barrier a call.  One wavefront uses none.
 template <int T>
-__device__ __forceinline__ void block_sum2(float& a, float& b, float* part)
+__device__ __forceinline__ void block_sum2(float& a, float& b, float* part, int lane)
 {
     a = wave_sum(a);
     b = wave_sum(b);
     if constexpr (T > kWave) {
-        __syncthreads();   // the sums before these have been read
-        if ((threadIdx.x & (kWave - 1)) == 0) {
-            part[threadIdx.x / kWave] = a;
-            part[T / kWave + threadIdx.x / kWave] = b;
+        if (lane % kWave == 0) {
+            part[lane / kWave] = a;
+            part[T / kWave + lane / kWave] = b;
         }
         __syncthreads();
         a = b = 0.0f;
@@ -169,5 +230,8 @@ __device__ __forceinline__ void block_sum2(float& a, float& b, float* part)
         }
     }
 }
+
+// Keeps a value in its register as it is: what is computed from it again later is computed again, not kept.
+__device__ __forceinline__ void hold(raw16& w) { asm volatile("" : "+v"(w)); }
 
 }  // namespace abh
