@@ -56,6 +56,11 @@ __device__ __forceinline__ uint32_t order_key(float x)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+__device__ __forceinline__ float key_value(uint32_t key)
+{
+    return key == 0xffffffffu ? __builtin_nanf("") : bitsf(key & 0x80000000u ? key & 0x7fffffffu : ~key);
+}
+
 // exp(x - m) with m = -inf taken as 0, so that a row without any finite logit has weights 0 and not NaN.
 __device__ __forceinline__ float exp_below(float x, float m)
 {
@@ -81,7 +86,8 @@ __device__ __forceinline__ void place_block(const RouteArgs& A, const uint64_t* 
     }
 }
 
-// 64 tokens a workgroup, G lanes a token, NV logits a lane (expert lane * NV + v).
+// 64 tokens a workgroup, G lanes a token, NV logits a lane (expert lane * NV + v).  Bound by its instructions, not by its
+// bytes: few lanes a token, so that a step over the lanes serves several tokens.
 template <int DT, int G, int NV>
 __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs A)
 {
@@ -98,38 +104,36 @@ __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs A)
         if (!__builtin_amdgcn_ballot_w64(real)) break;   // a wavefront's groups go on together: they share its sums' lanes
         float x[NV];
         uint32_t key[NV];
-        const int64_t row = (t0 + (real ? t : 0)) * A.experts;
+        const void* row = at<DT>(A.logits, (t0 + (real ? t : 0)) * A.experts);
+        if constexpr (NV % kLane<DT> == 0) {
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int e = lane * NV + v;
-            x[v] = e < A.experts ? get<DT>(A.logits, row + e) : kRouteNegInf;
-            key[v] = e < A.experts ? order_key(x[v]) : 0u;
+            for (int v = 0; v < NV; v += kLane<DT>) load_vec<DT>(row, lane * NV + v, A.experts, x + v);
+        } else {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) x[v] = lane * NV + v < A.experts ? get<DT>(row, lane * NV + v) : 0.0f;
         }
+#pragma unroll
+        for (int v = 0; v < NV; ++v) key[v] = lane * NV + v < A.experts ? order_key(x[v]) : 0u;
         float top = 0.0f, sum = 0.0f, mine = 0.0f;
         int my_expert = 0;
         for (int j = 0; j < A.top_k; ++j) {
-            uint32_t best = key[0];
-            float value = x[0];
-            int at_v = 0;
+            uint32_t most = key[0];
 #pragma unroll
-            for (int v = 1; v < NV; ++v) {
-                const bool more = key[v] > best;   // equal: the lower index stays
-                best = more ? key[v] : best;
-                value = more ? x[v] : value;
-                at_v = more ? v : at_v;
-            }
-            const uint32_t most = group_max<G>(best);
-            const uint64_t holders = __builtin_amdgcn_ballot_w64(best == most) >> ((threadIdx.x & 63) / G * G);
-            const int winner = __builtin_ctzll(holders);   // the lowest lane of this group that holds it
-            const int e = __shfl(lane * NV + at_v, winner, G);
-            value = __shfl(value, winner, G);
+            for (int v = 1; v < NV; ++v) most = most > key[v] ? most : key[v];
+            most = group_max<G>(most);
+            uint32_t e = ~0u;   // the lowest index that has it
 #pragma unroll
-            for (int v = 0; v < NV; ++v) key[v] = lane * NV + v == e ? 0u : key[v];
+            for (int v = NV - 1; v >= 0; --v) e = key[v] == most ? (uint32_t)v : e;
+            e = e == ~0u ? e : lane * NV + e;
+            e = group_reduce<G>(e, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+#pragma unroll
+            for (int v = 0; v < NV; ++v) key[v] = e == (uint32_t)(lane * NV + v) ? 0u : key[v];
+            const float value = key_value(most);
             if (j == 0) {
                 top = value;
                 if (!A.normalize) {   // the sum over all experts
 #pragma unroll
-                    for (int v = 0; v < NV; ++v) sum += exp_below(x[v], top);
+                    for (int v = 0; v < NV; ++v) sum += lane * NV + v < A.experts ? exp_below(x[v], top) : 0.0f;
                     sum = group_sum<G>(sum);
                 }
             }
@@ -137,7 +141,7 @@ __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs A)
             if (A.normalize) sum += w;
             if (lane == j) {
                 mine = w;
-                my_expert = e;
+                my_expert = (int)e;
             }
         }
         if (real && lane < A.top_k) {
@@ -232,49 +236,45 @@ __global__ __launch_bounds__(kRouteThreads) void k_route_places(RouteArgs A)
     place_block(A, mask, A.bases + blockIdx.x, A.blocks, t0, tokens);
 }
 
-// dlogits of the chosen's softmax, w_j (g_j - sum w g), or of all's, p_e ([e = chosen_j] g_j - sum p g).
-// A wavefront a token.
+// dlogits of the chosen's softmax, w_j (g_j - sum w g), or of all's, [e = chosen_j] w_j g_j - p_e sum w g.  A wavefront a
+// token, which spreads the chosen's values over the experts in its part of the LDS.
 template <int DT>
 __global__ __launch_bounds__(256) void k_route_back(const float* weights, const int32_t* chosen, const float* gout,
                                                     const void* logits, int64_t tokens, int32_t experts, int32_t top_k,
                                                     int32_t normalize, void* grad)
 {
-    const int lane = threadIdx.x & 63;
-    const int64_t t = (int64_t)blockIdx.x * 4 + threadIdx.x / kWave;
-    if (t >= tokens) return;
-    const float w = lane < top_k ? weights[t * top_k + lane] : 0.0f;
-    const float g = lane < top_k ? gout[t * top_k + lane] : 0.0f;
-    const int at = lane < top_k ? chosen[t * top_k + lane] : -1;
-    const float total = wave_sum(lane < top_k ? w * g : 0.0f);
+    __shared__ float spread[4][kMostExperts];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
+    const int64_t t = (int64_t)blockIdx.x * 4 + wave;
+    const bool real = t < tokens, picks = real && lane < top_k;
+    const float w = picks ? weights[t * top_k + lane] : 0.0f;
+    const float g = picks ? gout[t * top_k + lane] : 0.0f;
+    const int at_e = picks ? chosen[t * top_k + lane] : -1;
+    for (int e = lane; e < experts; e += kWave) spread[wave][e] = 0.0f;
+    const float total = wave_sum(picks ? w * g : 0.0f);
+    __syncthreads();   // zeros before values, values before reads
+    if (picks && at_e >= 0 && at_e < experts) spread[wave][at_e] = normalize ? w * (g - total) : w * g;
+    __syncthreads();
+    if (!real) return;
     const int64_t row = t * experts;
-    float top = 0.0f, inv = 0.0f;
-    if (!normalize) {
-        float most = kRouteNegInf, sum = 0.0f;
-        bool nan = false;
-        for (int e = lane; e < experts; e += kWave) {
-            const float x = get<DT>(logits, row + e);
-            most = __builtin_fmaxf(most, x);
-            nan |= x != x;
-        }
-        most = group_reduce<kWave>(most, [](float a, float b) { return __builtin_fmaxf(a, b); });
-        top = __builtin_amdgcn_ballot_w64(nan) ? __builtin_nanf("") : most;
-        for (int e = lane; e < experts; e += kWave) sum += exp_below(get<DT>(logits, row + e), top);
-        sum = wave_sum(sum);
-        inv = top == kRouteNegInf ? 0.0f : 1.0f / sum;
+    if (normalize) {
+        for (int e = lane; e < experts; e += kWave) put<DT>(grad, row + e, spread[wave][e]);
+        return;
     }
-    for (int e0 = 0; e0 < experts; e0 += kWave) {
-        const int e = e0 + lane;
-        float seed = 0.0f;   // w g of the assignment to e, if there is one
-        float own = 0.0f;
-        for (int j = 0; j < top_k; ++j) {   // of one token: scalars
-            const bool mine = __builtin_amdgcn_readlane(at, j) == e;
-            seed = mine ? bitsf(__builtin_amdgcn_readlane(fbits(w * g), j)) : seed;
-            own = mine ? bitsf(__builtin_amdgcn_readlane(fbits(w), j)) : own;
-        }
-        if (e >= experts) continue;
-        if (!normalize) own = exp_below(get<DT>(logits, row + e), top) * inv;
-        put<DT>(grad, row + e, seed - own * total);
+    float most = kRouteNegInf, sum = 0.0f;
+    bool nan = false;
+    for (int e = lane; e < experts; e += kWave) {
+        const float x = get<DT>(logits, row + e);
+        most = __builtin_fmaxf(most, x);
+        nan |= x != x;
     }
+    most = group_reduce<kWave>(most, [](float a, float b) { return __builtin_fmaxf(a, b); });
+    const float top = __builtin_amdgcn_ballot_w64(nan) ? __builtin_nanf("") : most;
+    for (int e = lane; e < experts; e += kWave) sum += exp_below(get<DT>(logits, row + e), top);
+    sum = wave_sum(sum);
+    const float inv = top == kRouteNegInf ? 0.0f : 1.0f / sum;
+    for (int e = lane; e < experts; e += kWave)
+        put<DT>(grad, row + e, spread[wave][e] - exp_below(get<DT>(logits, row + e), top) * inv * total);
 }
 
 // ---------------------------------------------------------------- dispatch and combine
@@ -433,13 +433,13 @@ static int route_sizes(int64_t tokens, int64_t experts, int64_t top_k)
 template <int DT>
 static void launch_route(const RouteArgs& A)
 {
-    // a token's lanes: 16 while its logits and its choices fit them, so that four tokens share a wavefront
+    // 16 lanes a token while its choices fit them and its logits their registers: four tokens share a wavefront
 #define ABH_ROUTE(G, NV)                                                                                        \
     if (A.experts <= G * NV && A.top_k <= G) {                                                                  \
         hipLaunchKernelGGL((k_route<DT, G, NV>), dim3(A.blocks), dim3(kRouteThreads), 0, t_stream, A);           \
         return;                                                                                                 \
     }
-    ABH_ROUTE(16, 1) ABH_ROUTE(16, 2) ABH_ROUTE(16, 4) ABH_ROUTE(32, 4) ABH_ROUTE(64, 4) ABH_ROUTE(64, 16)
+    ABH_ROUTE(16, 1) ABH_ROUTE(16, 2) ABH_ROUTE(16, 4) ABH_ROUTE(16, 8) ABH_ROUTE(16, 16) ABH_ROUTE(64, 16)
 #undef ABH_ROUTE
 }
 
