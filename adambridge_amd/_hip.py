@@ -701,3 +701,23 @@ def bind():
                                "run `python -m adambridge_amd.build` (or __graft_entry__.build())") from exc
         _bind_module = _bind
     return _bind_module
+
+
+_ops_module = None
+
+
+def ops():
+    """The host module _ops (csrc/abh_ops.cpp) over the loaded library.  Raises RuntimeError if either is not built."""
+    global _ops_module
+    if _ops_module is None:
+        lib = load()._lib
+        try:
+            from . import _ops
+        except ImportError as exc:
+            raise RuntimeError(f"adambridge_amd/_ops.so is not built or does not load ({exc}): "
+                               "run `python -m adambridge_amd.build` (or __graft_entry__.build())") from exc
+        from . import experts, norms
+        _ops.connect({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in EXPORTS},
+                     {**norms.BACKWARD, **experts.BACKWARD})
+        _ops_module = _ops
+    return _ops_module

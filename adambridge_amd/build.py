@@ -24,6 +24,8 @@ SOURCES = [PKG / "csrc" / name for name in ("adambridge_hip.hip", "abh_state.hip
 LIB = PKG / "libadambridge_hip.so"
 BIND_SOURCE = PKG / "csrc" / "abh_bind.cpp"   # host code over torch's C++ tensors: the Python module _bind
 BIND = PKG / "_bind.so"
+OPS_SOURCE = PKG / "csrc" / "abh_ops.cpp"     # the operators' host work and autograd functions: the module _ops
+OPS = PKG / "_ops.so"
 ARCH = os.environ.get("ADAMBRIDGE_HIP_ARCH", "gfx950")
 
 
@@ -41,25 +43,34 @@ def flags() -> list[str]:
             f"-I{ROOT / 'include'}"]
 
 
-def bind_command(out: Path) -> list[str]:
+def module_command(source: Path, out: Path, *more: str) -> list[str]:
     import torch
     from torch.utils import cpp_extension
 
     lib = Path(torch.__file__).resolve().parent / "lib"
     includes = [f"-I{d}" for d in (ROOT / "include", *cpp_extension.include_paths(), sysconfig.get_paths()["include"])]
     return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-fvisibility=hidden",
-            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *includes, str(BIND_SOURCE),
-            "-o", str(out), f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *includes, str(source),
+            "-o", str(out), f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10", *more]
+
+
+def bind_command(out: Path) -> list[str]:
+    return module_command(BIND_SOURCE, out)
+
+
+def ops_command(out: Path) -> list[str]:
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    return module_command(OPS_SOURCE, out, "-lc10_hip", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f"-I{rocm}/include")
 
 
 def build(verbose: bool = False) -> Path:
-    """Compile the library and the host module (always; a stale one is never reused): the sources side by
+    """Compile the library and the host modules (always; a stale one is never reused): the sources side by
     side, then one link."""
     with tempfile.TemporaryDirectory(prefix="adambridge_build_") as work:
         objects = [Path(work) / (src.stem + ".o") for src in SOURCES]
         compiles = [[hipcc(), *flags(), "-c", str(src), "-o", str(obj)] for src, obj in zip(SOURCES, objects)]
-        tmp, bind = LIB.with_suffix(".so.tmp"), BIND.with_suffix(".so.tmp")
-        compiles.append(bind_command(bind))
+        tmp, bind, ops = (path.with_suffix(".so.tmp") for path in (LIB, BIND, OPS))
+        compiles += [bind_command(bind), ops_command(ops)]
         link = [hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objects), "-o", str(tmp)]
         if verbose:
             print("\n".join(" ".join(cmd) for cmd in [*compiles, link]), file=sys.stderr)
@@ -75,6 +86,7 @@ def build(verbose: bool = False) -> Path:
                 raise RuntimeError(f"the compiler failed ({code}):\n{output}")
         os.replace(tmp, LIB)
         os.replace(bind, BIND)
+        os.replace(ops, OPS)
     return LIB
 
 

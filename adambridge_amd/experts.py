@@ -8,8 +8,8 @@ An expert MLP of ``top_k`` experts a token is::
     y = combine(rows, r)                            # each token's weighted sum
 
 Nothing of it waits for the device: how many rows an expert has is read there (``r.ends``).  On plain GPU
-tensors of float32 or bfloat16 the library's kernels compute it (csrc/abh_route.hip, csrc/abh_experts.hip);
-elsewhere, and where an operation is traced, transformed or differentiated twice, torch operations do.
+tensors of float32 or bfloat16 the library's kernels compute it (csrc/abh_route.hip, csrc/abh_experts.hip, called by
+csrc/abh_ops.cpp); elsewhere, and where an operation is traced, transformed or differentiated twice, torch operations do.
 """
 
 from __future__ import annotations
@@ -19,7 +19,7 @@ from typing import NamedTuple
 import torch
 
 from . import _hip
-from .losses import _observed, _plain_backward
+from .losses import _observed
 from .norms import plain
 
 __all__ = ["Routing", "route", "dispatch", "expert_mm", "combine"]
@@ -40,6 +40,12 @@ class Routing(NamedTuple):
     ends: torch.Tensor
     order: torch.Tensor
     position: torch.Tensor
+
+
+@torch.compiler.disable
+def _uncompiled(fn, *args):
+    """``fn`` outside a compiled graph, which breaks there."""
+    return fn(*args)
 
 
 # ----------------------------------------------------------------------- route
@@ -63,40 +69,21 @@ def _torch_route(logits, top_k, normalize):
     return Routing(weights, chosen.int(), ends.int(), order.int(), position.int())
 
 
-class _Route(torch.autograd.Function):
-    """Keeps the weights and the choice, and the logits if the softmax is over all of them."""
-
-    @staticmethod
-    def forward(ctx, logits, top_k, normalize):
-        out = _hip.load().route(logits, top_k, normalize)
-        ctx.mark_non_differentiable(*out[1:])
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(out[0], out[1], None if normalize else logits)
-        ctx.dtype, ctx.experts, ctx.normalize = logits.dtype, logits.shape[1], normalize
-        return out
-
-    @staticmethod
-    def backward(ctx, gout, *_):
-        weights, chosen, logits = ctx.saved_tensors
-        if gout is None:
-            return None, None, None
-        if _plain_backward(gout):
-            return _hip.load().route_backward(weights, chosen, gout.contiguous(), logits, ctx.dtype, ctx.experts,
-                                              ctx.normalize), None, None
-        seed = weights * gout
-        total = seed.sum(1, keepdim=True)
-        spread = weights.new_zeros(weights.shape[0], ctx.experts)
-        if ctx.normalize:
-            return spread.scatter(1, chosen.long(), seed - weights * total).to(ctx.dtype), None, None
-        wide = logits.float()
-        top = wide.detach().amax(1, keepdim=True)
-        e = torch.exp(wide - torch.where(top == -torch.inf, 0.0, top))
-        norm = e.sum(1, keepdim=True)
-        p = e / torch.where(norm == 0.0, 1.0, norm)
-        return (spread.scatter(1, chosen.long(), seed) - p * total).to(ctx.dtype), None, None
+def _route_backward(gout, weights, chosen, logits, experts, normalize, dtype):
+    """The logits' gradient in torch operations, differentiable in turn."""
+    seed = weights * gout
+    total = seed.sum(1, keepdim=True)
+    spread = weights.new_zeros(weights.shape[0], experts)
+    if normalize:
+        return spread.scatter(1, chosen.long(), seed - weights * total).to(dtype), None, None
+    wide = logits.float()
+    top = wide.detach().amax(1, keepdim=True)
+    e = torch.exp(wide - torch.where(top == -torch.inf, 0.0, top))
+    norm = e.sum(1, keepdim=True)
+    p = e / torch.where(norm == 0.0, 1.0, norm)
+    return (spread.scatter(1, chosen.long(), seed) - p * total).to(dtype), None, None
 
 
-@torch.compiler.disable
 def route(logits: torch.Tensor, top_k: int, normalize: bool = True) -> Routing:
     """The ``top_k`` largest of each token's ``logits`` (``[tokens, experts]``; the lower index of equal ones, a NaN
     counting as the largest), their softmax weights -- over the chosen if ``normalize``, else over all experts --
@@ -104,6 +91,12 @@ def route(logits: torch.Tensor, top_k: int, normalize: bool = True) -> Routing:
 
     An expert masked by ``-inf`` has weight 0 and is chosen only where nothing else is left; a token all of
     whose logits are ``-inf`` has weights 0 and no gradient."""
+    if torch.compiler.is_compiling():
+        return _uncompiled(route, logits, top_k, normalize)
+    if logits.is_cuda:
+        out = _hip.ops().route(logits, top_k, bool(normalize))
+        if out is not None:
+            return Routing(*out)
     if logits.dim() != 2 or not logits.is_floating_point() or logits.shape[1] < 1:
         raise ValueError(f"logits must be floating-point [tokens, experts], got {logits.dtype} {tuple(logits.shape)}")
     tokens, experts = logits.shape
@@ -113,10 +106,8 @@ def route(logits: torch.Tensor, top_k: int, normalize: bool = True) -> Routing:
         raise ValueError(f"tokens * top_k must be below 2^31, got {tokens * top_k}")
     if not plain(logits) or not tokens or experts > _MOST_EXPERTS or top_k > _MOST_CHOSEN or _observed():
         return _torch_route(logits, top_k, normalize)
-    logits = logits.contiguous()
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return Routing(*_Route.apply(logits, top_k, bool(normalize)))
-    return Routing(*_hip.load().route(logits, top_k, normalize))
+    out = _hip.ops().route(logits.contiguous(), top_k, bool(normalize))
+    return _torch_route(logits, top_k, normalize) if out is None else Routing(*out)
 
 
 # -------------------------------------------------------- dispatch and combine
@@ -150,48 +141,33 @@ def _torch_gather_sum(rows, weights, position):
     return picked.sum(1).to(rows.dtype)
 
 
-class _Dispatch(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, position):
-        ctx.save_for_backward(position)
-        return _hip.load().dispatch(x, position)
-
-    @staticmethod
-    def backward(ctx, gout):
-        position, = ctx.saved_tensors
-        if _plain_backward(gout):
-            return _hip.load().combine(gout.contiguous(), None, position), None
-        return _torch_gather_sum(gout, None, position), None
+def _dispatch_backward(gout, position):
+    return _torch_gather_sum(gout, None, position), None
 
 
-class _Combine(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, rows, weights, position):
-        ctx.save_for_backward(rows if ctx.needs_input_grad[1] else None, weights, position)
-        return _hip.load().combine(rows, weights, position)
-
-    @staticmethod
-    def backward(ctx, gout):
-        rows, weights, position = ctx.saved_tensors
-        wanted = ctx.needs_input_grad[:2]
-        if _plain_backward(gout):
-            return (*_hip.load().combine_backward(gout.contiguous(), rows, weights, position, wanted), None)
-        g = gout.float()
-        drows = dweights = None
-        if wanted[0]:
-            flat = position.reshape(-1).long()
-            inverse = torch.empty_like(flat).scatter(0, flat, torch.arange(flat.numel(), device=flat.device))
-            drows = (weights[:, :, None] * g[:, None, :]).flatten(0, 1).index_select(0, inverse).to(gout.dtype)
-        if wanted[1]:
-            picked = rows.float().index_select(0, position.reshape(-1).long()).view(*position.shape, rows.shape[1])
-            dweights = (picked * g[:, None, :]).sum(2)
-        return drows, dweights, None
+def _combine_backward(gout, rows, weights, position, want_rows, want_weights):
+    """Both gradients in torch operations, differentiable in turn."""
+    g = gout.float()
+    drows = dweights = None
+    if want_rows:
+        flat = position.reshape(-1).long()
+        inverse = torch.empty_like(flat).scatter(0, flat, torch.arange(flat.numel(), device=flat.device))
+        drows = (weights[:, :, None] * g[:, None, :]).flatten(0, 1).index_select(0, inverse).to(gout.dtype)
+    if want_weights:
+        picked = rows.float().index_select(0, position.reshape(-1).long()).view(*position.shape, rows.shape[1])
+        dweights = (picked * g[:, None, :]).sum(2)
+    return drows, dweights, None
 
 
-@torch.compiler.disable
 def dispatch(x: torch.Tensor, routing: Routing) -> torch.Tensor:
     """Each token's row of ``x`` (``[tokens, hidden]``) at its ``top_k`` rows of the experts' order:
     ``[tokens * top_k, hidden]``."""
+    if torch.compiler.is_compiling():
+        return _uncompiled(dispatch, x, routing)
+    if x.is_cuda:
+        rows = _hip.ops().dispatch(x, routing.position)
+        if rows is not None:
+            return rows
     if x.dim() != 2 or not x.is_floating_point():
         raise ValueError(f"x must be floating-point [tokens, hidden], got {x.dtype} {tuple(x.shape)}")
     tokens, top_k = _checked_position("x", routing, x.device)
@@ -199,16 +175,19 @@ def dispatch(x: torch.Tensor, routing: Routing) -> torch.Tensor:
         raise ValueError(f"x has {x.shape[0]} tokens, the routing {tokens}")
     if not plain(x) or not _fits(tokens, top_k, x.shape[1]) or _observed():
         return _torch_dispatch(x, routing.position)
-    x, position = x.contiguous(), routing.position.contiguous()
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _Dispatch.apply(x, position)
-    return _hip.load().dispatch(x, position)
+    out = _hip.ops().dispatch(x.contiguous(), routing.position.contiguous())
+    return _torch_dispatch(x, routing.position) if out is None else out
 
 
-@torch.compiler.disable
 def combine(rows: torch.Tensor, routing: Routing) -> torch.Tensor:
     """Each token's sum of its ``rows`` (``[tokens * top_k, hidden]``, in the experts' order), weighted by the routing's
     weights, summed in FP32 in the order of its choices and rounded once: ``[tokens, hidden]``."""
+    if torch.compiler.is_compiling():
+        return _uncompiled(combine, rows, routing)
+    if rows.is_cuda:
+        out = _hip.ops().combine(rows, routing.weights, routing.position)
+        if out is not None:
+            return out
     if rows.dim() != 2 or not rows.is_floating_point():
         raise ValueError(f"rows must be floating-point [tokens * top_k, hidden], got {rows.dtype} {tuple(rows.shape)}")
     tokens, top_k = _checked_position("rows", routing, rows.device)
@@ -221,10 +200,8 @@ def combine(rows: torch.Tensor, routing: Routing) -> torch.Tensor:
                          f"{tuple(weights.shape)} on {weights.device}")
     if not plain(rows, weights) or not _fits(tokens, top_k, rows.shape[1]) or _observed():
         return _torch_gather_sum(rows, weights, routing.position)
-    rows, weights, position = rows.contiguous(), weights.contiguous(), routing.position.contiguous()
-    if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
-        return _Combine.apply(rows, weights, position)
-    return _hip.load().combine(rows, weights, position)
+    out = _hip.ops().combine(rows.contiguous(), weights.contiguous(), routing.position.contiguous())
+    return _torch_gather_sum(rows, weights, routing.position) if out is None else out
 
 
 # ------------------------------------------------------------------- expert_mm
@@ -250,24 +227,18 @@ def _torch_weights(gout, x, ends):
     return torch.stack([gout[lo:hi].t() @ x[lo:hi] for lo, hi in _bounds(x.shape[0], ends)])
 
 
-class _ExpertMM(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, ends):
-        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, weight, ends)
-        return _hip.load().expert_mm(x, weight, ends)
-
-    @staticmethod
-    def backward(ctx, gout):
-        x, weight, ends = ctx.saved_tensors
-        wanted = ctx.needs_input_grad[:2]
-        if _plain_backward(gout):
-            return (*_hip.load().expert_mm_backward(gout.contiguous(), x, weight, ends, wanted), None)
-        with torch.autocast(gout.device.type, enabled=False):
-            return (_torch_rows(gout, weight, ends) if wanted[0] else None,
-                    _torch_weights(gout, x, ends) if wanted[1] else None, None)
+def _expert_mm_backward(gout, x, weight, ends, want_x, want_w):
+    """Both gradients in torch operations, differentiable in turn."""
+    with torch.autocast(gout.device.type, enabled=False):
+        return (_torch_rows(gout, weight, ends) if want_x else None,
+                _torch_weights(gout, x, ends) if want_w else None, None)
 
 
-@torch.compiler.disable
+# for the backward passes that the kernels do not take
+BACKWARD = {"route": _route_backward, "dispatch": _dispatch_backward, "combine": _combine_backward,
+            "expert_mm": _expert_mm_backward}
+
+
 def expert_mm(x: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
     """``x[r] @ weight[e].T`` for each row ``r`` of each expert ``e``: ``x`` ``[rows, in]`` sorted by expert, ``weight``
     ``[experts, out, in]`` (stacked Linear weights), expert ``e``'s rows ``ends[e - 1]`` to ``ends[e] - 1`` (``ends``: int32
@@ -275,6 +246,12 @@ def expert_mm(x: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) -> torc
 
     Sums are FP32, rounded once.  Differentiable in ``x`` and ``weight``; an expert without rows has zero gradients.
     Under autocast both operands are taken in autocast's type, as a Linear's are."""
+    if torch.compiler.is_compiling():
+        return _uncompiled(expert_mm, x, weight, ends)
+    if x.is_cuda:
+        out = _hip.ops().expert_mm(x, weight, ends)
+        if out is not None:
+            return out
     if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2]:
         raise ValueError(f"expert_mm takes x [rows, in] and weight [experts, out, in], got {tuple(x.shape)} and {tuple(weight.shape)}")
     if ends.dim() != 1 or ends.shape[0] != weight.shape[0] or ends.dtype != torch.int32:
@@ -292,7 +269,6 @@ def expert_mm(x: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) -> torc
     if (not plain(x, weight) or x.shape[0] > _MOST_ROWS or experts > _MOST_MM_EXPERTS or n > _MOST_SIZE or k > _MOST_SIZE
             or _observed()):
         return _torch_rows(x, weight.transpose(1, 2), ends)
-    x, weight, ends = x.contiguous(), weight.contiguous(), ends.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        return _ExpertMM.apply(x, weight, ends)
-    return _hip.load().expert_mm(x, weight, ends)
+    with torch.autocast("cuda", enabled=False):
+        out = _hip.ops().expert_mm(x.contiguous(), weight.contiguous(), ends.contiguous())
+    return _torch_rows(x, weight.transpose(1, 2), ends) if out is None else out

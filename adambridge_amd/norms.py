@@ -1,4 +1,4 @@
-"""Layer norm and its gradients by the library's kernels (csrc/abh_norm.hip).
+"""Layer norm and its gradients by the library's kernels (csrc/abh_norm.hip, called by csrc/abh_ops.cpp).
 
 Elsewhere than on plain GPU tensors of float32 or bfloat16, and where an operation is traced, transformed or
 differentiated twice, the same values come from torch operations.
@@ -10,7 +10,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _hip
-from .losses import _observed, _plain_backward
+from .losses import _observed
 
 __all__ = ["layer_norm"]
 
@@ -33,31 +33,26 @@ def _torch_layer_norm(x, weight, bias, eps):
     return F.layer_norm(x.to(wide), x.shape[-1:], *cast, eps).to(x.dtype)
 
 
-class _LayerNorm(torch.autograd.Function):
-    """Keeps x and the rows' mean and rstd."""
+def _backward(gout, x, weight, eps, want_x, want_w, want_b, w_dtype):
+    """The gradients in torch operations, differentiable in turn."""
+    with torch.autocast(x.device.type, enabled=False):
+        xf, g = x.float(), gout.float()
+        var, mean = torch.var_mean(xf, -1, correction=0, keepdim=True)
+        rstd = (var + eps).rsqrt()
+        xh = (xf - mean) * rstd
+        gw = g if weight is None else g * weight.float()
+        rows = tuple(range(x.dim() - 1))   # of none, a single row's sum is itself
+        dx = dw = db = None
+        if want_x:
+            dx = (rstd * (gw - gw.mean(-1, keepdim=True) - xh * (gw * xh).mean(-1, keepdim=True))).to(x.dtype)
+        if want_w:
+            dw = ((g * xh).sum(rows) if rows else g * xh).to(w_dtype)
+        if want_b:
+            db = (g.sum(rows) if rows else g).to(w_dtype)
+        return dx, dw, db
 
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, stats = _hip.load().layer_norm(x, weight, bias, eps, with_stats=True)
-        ctx.save_for_backward(x, weight, stats)
-        ctx.eps, ctx.w_dtype = eps, (x if weight is None and bias is None else bias if weight is None else weight).dtype
-        return y
 
-    @staticmethod
-    def backward(ctx, gout):
-        x, weight, stats = ctx.saved_tensors
-        wanted = ctx.needs_input_grad[:3]
-        if _plain_backward(gout):
-            return (*_hip.load().layer_norm_backward(gout.contiguous(), x, weight, stats, ctx.w_dtype, wanted), None)
-        with torch.autocast(x.device.type, enabled=False):
-            xf, g = x.float(), gout.float()
-            var, mean = torch.var_mean(xf, 1, correction=0, keepdim=True)
-            rstd = (var + ctx.eps).rsqrt()
-            xh = (xf - mean) * rstd
-            gw = g if weight is None else g * weight.float()
-            dx = rstd * (gw - gw.mean(1, keepdim=True) - xh * (gw * xh).mean(1, keepdim=True))
-            return (dx.to(x.dtype), (g * xh).sum(0).to(ctx.w_dtype) if wanted[1] else None,
-                    g.sum(0).to(ctx.w_dtype) if wanted[2] else None, None)
+BACKWARD = {"layer_norm": _backward}   # for the backward passes that the kernels do not take
 
 
 def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.Tensor | None = None,
@@ -68,6 +63,10 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     ``weight`` and ``bias`` are of one type, ``x``'s or another.  Differentiable in all three; the backward pass
     reads ``x`` and the gradient once and sums the weight's and the bias's gradients over all rows in FP32.
     """
+    if x.is_cuda and not torch.compiler.is_compiling():
+        y = _hip.ops().layer_norm(x, weight, bias, float(eps))
+        if y is not None:
+            return y
     cols = x.shape[-1] if x.dim() else 0
     if cols < 1 or not x.is_floating_point():
         raise ValueError(f"x must hold floating-point rows of one value or more, got {x.dtype} {tuple(x.shape)}")
@@ -81,8 +80,5 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
     rows = x.numel() // cols
     if not plain(x, weight, bias) or not 0 < rows <= _MOST or cols > _MOST or _observed():
         return _torch_layer_norm(x, weight, bias, eps)
-    flat = x.reshape(rows, cols).contiguous()
-    weight, bias = (t if t is None else t.contiguous() for t in (weight, bias))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
-        return _LayerNorm.apply(flat, weight, bias, eps).view(x.shape)
-    return _hip.load().layer_norm(flat, weight, bias, eps, with_stats=False)[0].view(x.shape)
+    y = _hip.ops().layer_norm(*(t if t is None else t.contiguous() for t in (x, weight, bias)), float(eps))
+    return _torch_layer_norm(x, weight, bias, eps) if y is None else y
