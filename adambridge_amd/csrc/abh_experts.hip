@@ -47,6 +47,8 @@ struct ExpertArgs {
     int32_t ni, nj;     // MODE_DW: C's rows (n); columns of C
     int32_t len;        // the sum's length, but for MODE_DW
     int32_t tiles_i, tiles_j;
+    int32_t splits;     // MODE_DW: parts of an expert's rows, each with its own sums ...
+    float* part;        // ... splits x experts x ni x nj
 };
 
 // Rows lo .. hi of expert e (e = experts: the rows that are no expert's).  Ends outside 0 .. rows, or one below the
@@ -62,6 +64,10 @@ __device__ __forceinline__ void expert_rows(const ExpertArgs& A, int e, int& lo,
 struct Tile {
     int e, lo, hi, ti, tj;
 };
+
+// The tile's numbers in scalar registers: divisions leave them, the same in all lanes, in vector ones, where the addresses made
+// of them cannot describe a buffer.
+__device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // This workgroup's row tile of BM rows: consecutive tiles go to one XCD, whose L2 then holds an expert's weights for
 // the tiles of its rows.  Every wavefront finds it for itself.
@@ -107,8 +113,8 @@ __device__ __forceinline__ bool find_row_tile(const ExpertArgs& A, Tile& t)
             const int g = idx / (kGroupTiles * A.tiles_j), first = g * kGroupTiles;
             const int wide = mine - first < kGroupTiles ? mine - first : kGroupTiles;
             const int r = idx - first * A.tiles_j;
-            t.ti = first + r % wide;
-            t.tj = r / wide;
+            t.ti = scalar(first + r % wide);
+            t.tj = scalar(r / wide);
             return true;
         }
         before += __builtin_amdgcn_readlane(s, kWave - 1);
@@ -116,24 +122,63 @@ __device__ __forceinline__ bool find_row_tile(const ExpertArgs& A, Tile& t)
     return false;
 }
 
-// A tile of dW.  The XCDs share every expert's tiles evenly, because experts differ in rows and so in work.
-__device__ __forceinline__ bool find_weight_tile(const ExpertArgs& A, Tile& t)
+// A tile of dW (and of one of the parts of its expert's rows).  The XCDs share every expert's tiles evenly, because
+// experts differ in rows and so in work.
+struct WeightTile : Tile {
+    int split;
+};
+
+__device__ __forceinline__ bool find_weight_tile(const ExpertArgs& A, WeightTile& t)
 {
     const int an = A.tiles_i * A.tiles_j, per = (an + kXcd - 1) / kXcd;
-    const int slot = (int)(blockIdx.x / kXcd);
-    t.e = slot / per;
-    if (t.e >= A.experts) return false;
-    const int local = (int)((blockIdx.x + t.e) % kXcd) * per + slot - t.e * per;   // the first XCD changes: an may be below 8
+    const int slot = (int)(blockIdx.x / kXcd), turn = slot / per;
+    if (turn >= A.experts * A.splits) return false;
+    const int local = (int)((blockIdx.x + turn) % kXcd) * per + slot - turn * per;   // the first XCD changes: an may be below 8
     if (local >= an) return false;
+    t.e = turn / A.splits;
+    t.split = turn - t.e * A.splits;
     const int g = local / (kGroupTiles * A.tiles_j), first = g * kGroupTiles;
     const int wide = A.tiles_i - first < kGroupTiles ? A.tiles_i - first : kGroupTiles;
     const int r = local - first * A.tiles_j;
-    t.ti = first + r % wide;
-    t.tj = r / wide;
-    expert_rows(A, t.e, t.lo, t.hi);
-    t.lo = __builtin_amdgcn_readfirstlane(t.lo);
-    t.hi = __builtin_amdgcn_readfirstlane(t.hi);
+    t.ti = scalar(first + r % wide);
+    t.tj = scalar(r / wide);
+    t.e = scalar(t.e);
+    t.split = scalar(t.split);
+    int lo, hi;
+    expert_rows(A, t.e, lo, hi);
+    lo = scalar(lo);
+    hi = scalar(hi);
+    const int chunk = ((hi - lo + A.splits - 1) / A.splits + 31) / 32 * 32;   // whole steps of 32 rows
+    t.lo = scalar(chunk * t.split < hi - lo ? lo + chunk * t.split : hi);
+    t.hi = scalar(t.lo + chunk < hi ? t.lo + chunk : hi);
     return true;
+}
+
+template <int MODE>
+using TileOf = typename std::conditional<MODE == MODE_DW, WeightTile, Tile>::type;
+
+// Where this part's sums go: FP32, rows of nj.
+__device__ __forceinline__ float* part_of(const ExpertArgs& A, const WeightTile& t)
+{
+    return A.part + ((int64_t)t.split * A.experts + t.e) * A.ni * A.nj;
+}
+
+// c = the parts' sums, in order, rounded once.
+template <int DT>
+__global__ __launch_bounds__(256) void k_experts_sum(const float* part, int64_t size, int32_t splits, void* c)
+{
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= size) return;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p = 0; p < splits; ++p) {
+        float x[4];
+        load_vec<DT_F32>(part + p * size, i, size, x);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[k] += x[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (i + k < size) put<DT>(c, i + k, s[k]);
 }
 
 // ------------------------------------------------------------- any sizes, any alignment
@@ -220,8 +265,12 @@ __global__ __launch_bounds__(kMmThreads2, 2) void k_experts_any(ExpertArgs A)
 {
     constexpr bool ALONG = MODE != MODE_DW, BLONG = MODE == MODE_Y;
     __shared__ __attribute__((aligned(16))) Element<DT> la[kTile * kPitch<DT>], lb[kTile * kPitch<DT>];
-    Tile t;
-    if (!(MODE == MODE_DW ? find_weight_tile(A, t) : find_row_tile<kTile>(A, t))) return;
+    TileOf<MODE> t;
+    if constexpr (MODE == MODE_DW) {
+        if (!find_weight_tile(A, t)) return;
+    } else {
+        if (!find_row_tile<kTile>(A, t)) return;
+    }
     const int i0 = t.ti * kTile, j0 = t.tj * kTile;
     const int limit_i = MODE == MODE_DW ? A.ni - i0 : t.hi - t.lo - i0, limit_j = A.nj - j0;
     const int len = MODE == MODE_DW ? t.hi - t.lo : t.e < A.experts ? A.len : 0;
@@ -308,6 +357,118 @@ __global__ __launch_bounds__(kMmThreads2, 2) void k_experts_any(ExpertArgs A)
     }
 }
 
+// ---------------------------------------------------------------------------- few rows
+//
+// y of few rows is its experts' weights read once: no tile to share, so they go to the registers in 16-byte pieces,
+// 16 columns of C a workgroup, whose four wavefronts split the sum and add their parts in order.  The rows are the
+// matrix instruction's other side, 16 at a time (whatever their number costs nothing beside the weights) and up to
+// 64 for one reading.  Any size and alignment; a workgroup finds the expert that is the blockIdx-th with rows.
+
+constexpr int kFewColumns = 16, kFewWaves = 4, kFewAhead = 8;
+constexpr uint32_t kOutside = 0x80000000u;   // an offset outside every buffer
+
+// 16-byte pieces of rows of a matrix: whole ones through a buffer, whose range ends them, or (EVEN false) rows of any
+// length at any address.
+template <int DT, bool EVEN>
+struct Pieces {
+    const uint8_t* base;
+    uint32_t bytes;
+    int64_t len;
+    int rows;
+    // Values k .. of row `row`; zeros past the rows' end and past the row's.
+    __device__ __forceinline__ raw16 load(int row, int k, bool real) const
+    {
+        if constexpr (EVEN) {
+            const __amdgpu_buffer_rsrc_t buffer = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, (int)bytes, 0x00020000);
+            const uint32_t offset = real && k < len ? (uint32_t)((row * (int)len + k) * kSize<DT>) : kOutside;
+            return __builtin_bit_cast(raw16, __builtin_amdgcn_raw_buffer_load_b128(buffer, offset, 0, 0));
+        } else {
+            return load_vec_raw<DT>(base + (int64_t)(row < rows ? row : 0) * len * kSize<DT>, k, real && row < rows ? len : 0);
+        }
+    }
+};
+
+template <int DT, bool EVEN>
+__global__ __launch_bounds__(kFewWaves * kWave) void k_experts_few(ExpertArgs A)
+{
+    constexpr int V = kLane<DT>, STEP = 4 * V, CH = 4, U = kFewAhead, W = kFewWaves;
+    __shared__ mm_f32x4 parts[W - 1][CH][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+    const int col = lane & 15, quarter = lane >> 4;
+    const int tj = (int)blockIdx.x % A.tiles_j;
+    int skip = (int)blockIdx.x / A.tiles_j;
+    int e = -1, lo = 0, hi = 0;
+    for (int e0 = 0; e0 <= A.experts; e0 += kWave) {
+        int l, h;
+        expert_rows(A, e0 + lane, l, h);
+        const uint64_t with = __builtin_amdgcn_ballot_w64(h > l);
+        const int count = __builtin_popcountll(with);
+        if (skip < count) {
+            const int before = __builtin_popcountll(with & (((uint64_t)1 << lane) - 1));
+            const int at_lane = __builtin_ctzll(__builtin_amdgcn_ballot_w64(h > l && before == skip));
+            e = e0 + at_lane;
+            lo = __builtin_amdgcn_readlane(l, at_lane);
+            hi = __builtin_amdgcn_readlane(h, at_lane);
+            break;
+        }
+        skip -= count;
+    }
+    if (e < 0) return;
+    const int steps = e < A.experts ? (A.len + STEP - 1) / STEP : 0;   // rows that are no expert's: zeros
+    const int s0 = steps * wave / W, s1 = steps * (wave + 1) / W;
+    const int j0 = tj * kFewColumns, columns = A.nj - j0 < kFewColumns ? A.nj - j0 : kFewColumns;
+    const Pieces<DT, EVEN> w{at<DT>(A.b, ((int64_t)(e < A.experts ? e : 0) * A.nj + j0) * A.len), (uint32_t)(columns * A.len * kSize<DT>),
+                             A.len, columns};
+    const Pieces<DT, EVEN> x{at<DT>(A.a, (int64_t)lo * A.len), (uint32_t)((hi - lo) * A.len * kSize<DT>), A.len, hi - lo};
+    for (int r0 = 0; r0 < hi - lo; r0 += 16 * CH) {
+        mm_f32x4 acc[CH];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) acc[c] = mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s = s0; s < s1; s += U) {
+            raw16 wv[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) wv[u] = w.load(col, (s + u) * STEP + quarter * V, s + u < s1);
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                if (r0 + 16 * c >= hi - lo) break;
+                raw16 xv[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) xv[u] = x.load(r0 + 16 * c + col, (s + u) * STEP + quarter * V, s + u < s1);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if constexpr (DT == DT_BF16) {
+                        acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mm_bf16x8, wv[u]),
+                                                                         __builtin_bit_cast(mm_bf16x8, xv[u]), acc[c], 0, 0, 0);
+                    } else {
+                        const mm_f32x4 wf = __builtin_bit_cast(mm_f32x4, wv[u]), xf = __builtin_bit_cast(mm_f32x4, xv[u]);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[q], xf[q], acc[c], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        if (r0 > 0) __syncthreads();   // the parts before have been read
+        if (wave > 0)
+#pragma unroll
+            for (int c = 0; c < CH; ++c)
+                if (r0 + 16 * c < hi - lo) parts[wave - 1][c][lane] = acc[c];
+        __syncthreads();
+        if (wave > 0) continue;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            if (r0 + 16 * c >= hi - lo) break;
+            const int row = r0 + 16 * c + col, j4 = j0 + 4 * quarter;
+#pragma unroll
+            for (int p = 0; p < W - 1; ++p) acc[c] += parts[p][c][lane];
+            if (row >= hi - lo) continue;
+            void* y = at<DT>(A.c, (int64_t)(lo + row) * A.nj);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (j4 + r < A.nj) put<DT>(y, j4 + r, acc[c][r]);
+        }
+    }
+}
+
 // ------------------------------------------------------------- BF16 rows of whole 16-byte pieces
 //
 // Tiles of 256 x 256, eight wavefronts of 128 x 64 (2 x 4), 32 terms a step, four buffers of 32 KB in the LDS.  A step's
@@ -324,8 +485,6 @@ __global__ __launch_bounds__(kMmThreads2, 2) void k_experts_any(ExpertArgs A)
 // neighbouring rows meet different banks.  One across its rows is 32 terms by its rows, read transposed
 // (ds_read_b64_tr_b16: 16 lanes take 4 terms x 16 values, a lane 4 terms of one value), its pieces exchanged in
 // fours by the term mod 4: the 4 terms x 2 pairs of pieces of 32 lanes then cover the 256 bytes of all banks.
-
-constexpr uint32_t kOutside = 0x80000000u;          // an offset outside every buffer
 
 typedef float mm_f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 mm_bf16x4 __attribute__((ext_vector_type(4)));
@@ -346,6 +505,19 @@ __device__ __forceinline__ void wait_loads()
     __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);
 }
 
+// How the 16-byte pieces of a row of CH of them, or of a term of R rows, change places in the LDS.
+template <int CH>
+__device__ __forceinline__ int swap_of_row(int row)
+{
+    return CH == 8 ? (row >> 1) & 7 : (row >> 2) & 3;   // 16 rows' pieces of a number: 16 places of the 256 bytes of all banks
+}
+template <int DT, int R>
+__device__ __forceinline__ int swap_of_term(int term)
+{
+    if (DT == DT_F32) return (term & 4) << 1;              // read a value a lane: terms 4 apart, 128 bytes of each
+    return R >= 128 ? (term & 3) << 2 : (term & 2) << 1;   // read transposed
+}
+
 // One operand's tile of R rows by BK terms, on its way to the LDS in W wavefronts' pieces of 1 KB.
 template <bool LONG, int R, int BK, int W>
 struct Feed {
@@ -355,8 +527,6 @@ struct Feed {
     int64_t left;          // !LONG: bytes from base to the operand's end
     int32_t pitch;         // bytes
     bool past;             // LONG: whether this lane's pieces are past the end in the last step
-
-    static __device__ __forceinline__ int swap_of_row(int row) { return BK == 64 ? row & 7 : (row >> 2) & 3; }
 
     // rows: LONG: the tile's rows; else the operand's terms.  lead: !LONG: bytes before base in its first row.
     __device__ __forceinline__ void start(const uint8_t* p, int64_t pitch_bytes, int rows, int len, int64_t lead)
@@ -369,12 +539,12 @@ struct Feed {
 #pragma unroll
         for (int q = 0; q < N; ++q) {
             if constexpr (LONG) {
-                const int row = (q * W + wave) * (64 / CH) + lane / CH, piece = (lane % CH) ^ swap_of_row(row);
+                const int row = (q * W + wave) * (64 / CH) + lane / CH, piece = (lane % CH) ^ swap_of_row<CH>(row);
                 offset[q] = (uint32_t)(row * pitch + piece * 16);
                 if (q == 0) past = len % BK && piece * 8 >= len % BK;   // the same piece in all of them
             } else {
                 const int term = (q * W + wave) * (512 / R) + lane / (R / 8);
-                offset[q] = (uint32_t)(term * pitch + ((lane % (R / 8)) ^ (term & 3) << 2) * 16);
+                offset[q] = (uint32_t)(term * pitch + ((lane % (R / 8)) ^ swap_of_term<DT_BF16, R>(term)) * 16);
             }
         }
     }
@@ -399,6 +569,89 @@ struct Feed {
     }
 };
 
+// The same tile, of rows of any length (a piece or more) of BF16 or FP32 at any address: through the registers, a step ahead of
+// the LDS.  A piece over the end of its row is the row's last whole one, moved down once it has arrived.
+template <int DT, bool LONG, int R, int BK, int W>
+struct StagedFeed {
+    static constexpr int V = kLane<DT>, S = kSize<DT>, N = R * BK * S / 1024 / W, CH = BK / V, RH = R / V;
+    const uint8_t* base;   // LONG: the tile's first row; else the operand's first term (whole rows)
+    uint32_t offset[N];    // of this lane's pieces from there, bytes
+    int32_t moved[N];      // !LONG: values to move down
+    int32_t pitch, len;    // values of a row; terms
+    bool edge;             // !LONG: whether any piece of the tile is over the end of its row
+    raw16 piece[N];
+
+    static __device__ __forceinline__ void where(int q, int& row, int& term)
+    {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
+        if constexpr (LONG) {
+            row = (q * W + wave) * (64 / CH) + lane / CH;
+            term = ((lane % CH) ^ swap_of_row<CH>(row)) * V;
+        } else {
+            term = (q * W + wave) * (64 / RH) + lane / RH;
+            row = ((lane % RH) ^ swap_of_term<DT, R>(term)) * V;
+        }
+    }
+    // first: the tile's first row; rows: how many there are in all of the operand (from LONG: the tile's) on
+    __device__ __forceinline__ void start(const uint8_t* p, int pitch_values, int first, int rows, int terms)
+    {
+        base = p;
+        pitch = pitch_values;
+        len = terms;
+        edge = !LONG && first + R > rows;
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+            int row, term;
+            where(q, row, term);
+            if constexpr (LONG) {
+                offset[q] = (uint32_t)((row < rows ? row : 0) * pitch + term) * (uint32_t)S;   // past the end: any, not stored
+                moved[q] = 0;
+            } else {
+                const int from = first + row < rows - V ? first + row : rows - V;
+                offset[q] = (uint32_t)(term * pitch + from) * (uint32_t)S;
+                moved[q] = first + row - from < V ? first + row - from : V;
+            }
+        }
+    }
+    __device__ __forceinline__ void load(int step)
+    {
+        const uint8_t* p = base + (LONG ? (int64_t)step * BK * S : (int64_t)step * BK * pitch * S);
+        const int left = len - step * BK;   // terms from here on
+        const bool last = left < BK;
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+            uint32_t o = offset[q];
+            if (last) {
+                int row, term;
+                where(q, row, term);
+                // LONG: back to the row's last piece (which may lie before p); else to a term that there is
+                const int back = LONG ? (term > left - V ? term - (left - V) : 0) : term >= left ? term * pitch : 0;
+                o -= (uint32_t)back * (uint32_t)S;
+            }
+            piece[q] = load_raw<DT>(p + (int32_t)o, 0);
+        }
+    }
+    __device__ __forceinline__ void store(int step, uint8_t* lds) const
+    {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
+        const int left = len - step * BK;
+        const bool last = left < BK;
+#pragma unroll
+        for (int q = 0; q < N; ++q) {
+            raw16 w = piece[q];
+            int row, term;
+            where(q, row, term);
+            if (LONG && last) {
+                const int back = term > left - V ? term - (left - V) : 0;
+                w = drop_values<DT>(w, back < V ? back : V);
+            }
+            if (!LONG && edge) w = drop_values<DT>(w, moved[q]);
+            if (!LONG && last && term >= left) w = raw16{0u, 0u, 0u, 0u};
+            *reinterpret_cast<raw16*>(lds + (q * W + wave) * 1024 + lane * 16) = w;
+        }
+    }
+};
+
 // Reads of a wavefront's fragments: 32 rows, from row `first` of the tile of R rows, by 16 terms.
 template <bool LONG, int R, int BK, int N>
 struct Fragments {
@@ -410,13 +663,13 @@ struct Fragments {
             const int row = first + (lane & 31);   // first and the fragments are multiples of 32 apart: the same exchange
 #pragma unroll
             for (int h = 0; h < BK / 16; ++h)
-                place[h] = row * BK * 2 + (((2 * h + (lane >> 5)) ^ Feed<LONG, R, BK, 1>::swap_of_row(row)) * 16);
+                place[h] = row * BK * 2 + (((2 * h + (lane >> 5)) ^ swap_of_row<BK / 8>(row)) * 16);
         } else {
             const int within = (lane & 15) >> 2, term = 8 * (lane >> 5) + within;   // within: the term mod 4
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int piece = (first + 32 * i) / 8 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-                place[i] = term * R * 2 + ((piece ^ within << 2) * 16) + (lane & 1) * 8;
+                place[i] = term * R * 2 + ((piece ^ swap_of_term<DT_BF16, R>(term)) * 16) + (lane & 1) * 8;
             }
         }
     }
@@ -434,7 +687,8 @@ struct Fragments {
     }
 };
 
-typedef Config<256, 256, 32, 4, 2, 4, 2> FastConfig;
+typedef Config<256, 256, 32, 4, 2, 4, 2> LargeTile;
+typedef Config<128, 128, 32, 4, 2, 2, 2> SmallTile;   // where large ones are too few for the CUs
 
 // Asks the scheduler for READS reads of the LDS spread among the next PRODUCTS matrix products.
 template <int READS, int PRODUCTS, int M = 0>
@@ -448,28 +702,39 @@ __device__ __forceinline__ void spread_reads()
     }
 }
 
-template <int MODE, class C>
+template <int MODE, class C, bool EVEN>
 __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
 {
     constexpr bool ALONG = MODE != MODE_DW, BLONG = MODE == MODE_Y;
     constexpr int BM = C::BM, BN = C::BN, BK = C::BK, NB = C::NB;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[NB * C::BYTES];
-    Tile t;
-    if (!(MODE == MODE_DW ? find_weight_tile(A, t) : find_row_tile<BM>(A, t))) return;
+    TileOf<MODE> t;
+    if constexpr (MODE == MODE_DW) {
+        if (!find_weight_tile(A, t)) return;
+    } else {
+        if (!find_row_tile<BM>(A, t)) return;
+    }
     const int i0 = t.ti * BM, j0 = t.tj * BN;
     const int limit_i = MODE == MODE_DW ? A.ni - i0 : t.hi - t.lo - i0, limit_j = A.nj - j0;
     const int len = MODE == MODE_DW ? t.hi - t.lo : t.e < A.experts ? A.len : 0;
     const int steps = (len + BK - 1) / BK;
-    Feed<ALONG, BM, BK, C::W> fa;
-    Feed<BLONG, BN, BK, C::W> fb;
-    if constexpr (MODE == MODE_DW) {
-        fa.start(at<DT_BF16>(A.a, (int64_t)t.lo * A.ni + i0), (int64_t)A.ni * 2, len, len, (int64_t)i0 * 2);
-        fb.start(at<DT_BF16>(A.b, (int64_t)t.lo * A.nj + j0), (int64_t)A.nj * 2, len, len, (int64_t)j0 * 2);
-    } else {
-        const uint8_t* w = at<DT_BF16>(A.b, (int64_t)(t.e < A.experts ? t.e : 0) * A.len * A.nj);
-        fa.start(at<DT_BF16>(A.a, (int64_t)(t.lo + i0) * A.len), (int64_t)A.len * 2, limit_i, len, 0);
-        if constexpr (MODE == MODE_Y) fb.start(w + (int64_t)j0 * A.len * 2, (int64_t)A.len * 2, limit_j, len, 0);
-        else fb.start(w + (int64_t)j0 * 2, (int64_t)A.nj * 2, len, len, (int64_t)j0 * 2);
+    typename std::conditional<EVEN, Feed<ALONG, BM, BK, C::W>, StagedFeed<DT_BF16, ALONG, BM, BK, C::W>>::type fa;
+    typename std::conditional<EVEN, Feed<BLONG, BN, BK, C::W>, StagedFeed<DT_BF16, BLONG, BN, BK, C::W>>::type fb;
+    {
+        // the operands' first values: of this expert's rows and weights
+        const int64_t first_row = MODE == MODE_DW ? t.lo : t.lo + i0;
+        const int pitch_a = MODE == MODE_DW ? A.ni : A.len, pitch_b = MODE == MODE_Y ? A.len : A.nj;
+        const uint8_t* pa = at<DT_BF16>(A.a, first_row * pitch_a);
+        const uint8_t* pb = MODE == MODE_DW ? at<DT_BF16>(A.b, (int64_t)t.lo * A.nj)
+                                            : at<DT_BF16>(A.b, (int64_t)(t.e < A.experts ? t.e : 0) * A.len * A.nj);
+        if (MODE == MODE_Y) pb = at<DT_BF16>(pb, (int64_t)j0 * A.len);
+        if constexpr (EVEN) {
+            fa.start(MODE == MODE_DW ? pa + (int64_t)i0 * 2 : pa, (int64_t)pitch_a * 2, ALONG ? limit_i : len, len, (int64_t)i0 * 2);
+            fb.start(MODE == MODE_Y ? pb : pb + (int64_t)j0 * 2, (int64_t)pitch_b * 2, BLONG ? limit_j : len, len, (int64_t)j0 * 2);
+        } else {
+            fa.start(pa, pitch_a, ALONG ? 0 : i0, ALONG ? limit_i : A.ni, len);
+            fb.start(pb, pitch_b, BLONG ? 0 : j0, BLONG ? limit_j : A.nj, len);
+        }
     }
     const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
     const int wi = wave % C::WI * (BM / C::WI), wj = wave / C::WI * (BN / C::WJ);
@@ -485,9 +750,23 @@ __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
     constexpr int H = BK / 16;
+    constexpr int LEAD = EVEN ? NB - 1 : 2;   // steps from the one that is multiplied to the one on its way to the LDS
+    // the pieces of step s on their way to the LDS (EVEN); else step s's from the registers, and those of the next loaded
     auto issue = [&](int s, int buffer) {
-        fa.issue(s, steps, lds + buffer * C::BYTES);
-        fb.issue(s, steps, lds + buffer * C::BYTES + BM * BK * 2);
+        uint8_t* la = lds + buffer * C::BYTES;
+        if constexpr (EVEN) {
+            fa.issue(s, steps, la);
+            fb.issue(s, steps, la + BM * BK * 2);
+        } else {
+            if (s < steps) {
+                fa.store(s, la);
+                fb.store(s, la + BM * BK * 2);
+            }
+            if (s + 1 < steps) {
+                fa.load(s + 1);
+                fb.load(s + 1);
+            }
+        }
     };
     // fragments are read one product ahead, so that the LDS works while the matrix cores do
     mm_bf16x8 a[2][C::NI], b[2][C::NJ];
@@ -508,12 +787,16 @@ __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
     constexpr int READS = (ALONG ? 1 : 2) * C::NI + (BLONG ? 1 : 2) * C::NJ, PRODUCTS = C::NI * C::NJ;
     auto interleave = [&]() { spread_reads<READS, PRODUCTS>(); };
     if (steps > 0) {
+        if constexpr (!EVEN) {
+            fa.load(0);
+            fb.load(0);
+        }
 #pragma unroll
-        for (int s = 0; s < NB - 1; ++s) issue(s, s);
-        wait_loads<(NB - 2) * C::LOADS>();
+        for (int s = 0; s < LEAD; ++s) issue(s, s);
+        if constexpr (EVEN) wait_loads<(NB - 2) * C::LOADS>();
         __syncthreads();
         fetch(0, 0, 0);
-        int now = 0, next = 1, ahead = NB - 1;
+        int now = 0, next = 1, ahead = LEAD;
         for (int s = 0; s + 1 < steps; ++s) {
 #pragma unroll
             for (int h = 0; h + 1 < H; ++h) {
@@ -522,9 +805,9 @@ __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
                 interleave();
             }
             // the next step's pieces have arrived, everyone's after the barrier, and the step before has been read
-            wait_loads<(NB - 3) * C::LOADS>();
+            if constexpr (EVEN) wait_loads<(NB - 3) * C::LOADS>();
             __syncthreads();
-            issue(s + NB - 1, ahead);
+            issue(s + LEAD, ahead);
             fetch(0, next, 0);
             multiply((H - 1) & 1);
             interleave();
@@ -537,7 +820,25 @@ __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
             if (h + 1 < H) fetch((h + 1) & 1, now, h + 1);
             multiply(h & 1);
         }
-        wait_loads<0>();   // nothing is on its way to the LDS when the workgroup ends
+        if constexpr (EVEN) wait_loads<0>();   // nothing is on its way to the LDS when the workgroup ends
+    }
+    if constexpr (MODE == MODE_DW) {
+        if (A.splits > 1) {   // a part of the sums
+            float* to = part_of(A, t) + j0;
+#pragma unroll
+            for (int i = 0; i < C::NI; ++i) {
+                const int row = i0 + wi + 32 * i + (lane & 31);
+                if (row >= A.ni) continue;
+#pragma unroll
+                for (int j = 0; j < C::NJ; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float four[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                        store_like<DT_F32, 4>(to + (int64_t)row * A.nj, wj + 32 * j + 8 * q + 4 * (lane >> 5), limit_j, four);
+                    }
+            }
+            return;
+        }
     }
     // a lane has row lane mod 32 and, of each 8 columns, 4: the two halves exchange fours for whole 16 bytes
     uint8_t* out = MODE == MODE_DW ? at<DT_BF16>(A.c, ((int64_t)t.e * A.ni + i0) * A.nj + j0)
@@ -560,30 +861,198 @@ __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
                 const auto s0 = __builtin_amdgcn_permlane32_swap(x[0][0], x[1][0], false, false);
                 const auto s1 = __builtin_amdgcn_permlane32_swap(x[0][1], x[1][1], false, false);
                 const int c = wj + 32 * j + 8 * (q + half);
-                if (row < limit_i && c < limit_j)
-                    store_raw<DT_BF16>(out, (int64_t)row * A.nj + c, raw16{s0[0], s1[0], s0[1], s1[1]});
+                const raw16 eight = {s0[0], s1[0], s0[1], s1[1]};
+                const int64_t o = (int64_t)row * A.nj + c;
+                if (row >= limit_i || c >= limit_j) continue;
+                if (EVEN || c + 8 <= limit_j) {
+                    store_raw<DT_BF16>(out, o, eight);
+                } else {
+                    const uint32_t u[4] = {eight.x, eight.y, eight.z, eight.w};
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+                        if (c + r < limit_j) reinterpret_cast<uint16_t*>(out)[o + r] = (uint16_t)(u[r / 2] >> (16 * (r & 1)));
+                }
             }
         }
     }
 }
 
-// (named here: the host's compilation leaves out their launch functions otherwise)
-template __global__ void k_experts_fast<MODE_Y, FastConfig>(ExpertArgs);
-template __global__ void k_experts_fast<MODE_DX, FastConfig>(ExpertArgs);
-template __global__ void k_experts_fast<MODE_DW, FastConfig>(ExpertArgs);
+// (Named here: the host's compilation leaves out their launch functions otherwise.)
+#define ABH_EXPERTS_FAST(C)                                                        \
+    template __global__ void k_experts_fast<MODE_Y, C, true>(ExpertArgs);          \
+    template __global__ void k_experts_fast<MODE_Y, C, false>(ExpertArgs);         \
+    template __global__ void k_experts_fast<MODE_DX, C, true>(ExpertArgs);         \
+    template __global__ void k_experts_fast<MODE_DX, C, false>(ExpertArgs);        \
+    template __global__ void k_experts_fast<MODE_DW, C, true>(ExpertArgs);         \
+    template __global__ void k_experts_fast<MODE_DW, C, false>(ExpertArgs);
+ABH_EXPERTS_FAST(LargeTile)
+ABH_EXPERTS_FAST(SmallTile)
+#undef ABH_EXPERTS_FAST
+
+// ------------------------------------------------------------------------------------ FP32
+//
+// The same with FP32 matrix instructions (32 x 32 x 2, a sixteenth of BF16's rate, which bounds it): tiles of 128 x 128 or,
+// where those are few, 64 x 64, four wavefronts of a quarter each, 32 terms a step, two buffers.  A long operand is read
+// four terms a lane, and the instructions take the terms in that order from both.
+
+template <bool LONG, int R, int N>
+struct FragmentsF32 {
+    int row;
+    __device__ __forceinline__ void start(int first) { row = first + (threadIdx.x & 31); }
+    // 32 rows from row + 32 i, terms 8 h + 4 (lane / 32) ..
+    __device__ __forceinline__ mm_f32x4 read(const uint8_t* lds, int i, int h) const
+    {
+        const int half = (threadIdx.x & 63) >> 5, r = row + 32 * i;
+        if constexpr (LONG) {
+            return *reinterpret_cast<const mm_f32x4*>(lds + r * 128 + ((2 * h + half) ^ swap_of_row<8>(r)) * 16);
+        } else {
+            const float* f = reinterpret_cast<const float*>(lds);
+            mm_f32x4 x;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int term = 8 * h + 4 * half + q;
+                x[q] = f[term * R + ((r >> 2) ^ swap_of_term<DT_F32, R>(term)) * 4 + (r & 3)];
+            }
+            return x;
+        }
+    }
+};
+
+template <int MODE, int B>
+__global__ __launch_bounds__(256, 2) void k_experts_f32(ExpertArgs A)
+{
+    constexpr bool ALONG = MODE != MODE_DW, BLONG = MODE == MODE_Y;
+    constexpr int BK = 32, NI = B / 64, BYTES = B * BK * 4;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2][2 * BYTES];
+    TileOf<MODE> t;
+    if constexpr (MODE == MODE_DW) {
+        if (!find_weight_tile(A, t)) return;
+    } else {
+        if (!find_row_tile<B>(A, t)) return;
+    }
+    const int i0 = t.ti * B, j0 = t.tj * B;
+    const int limit_i = MODE == MODE_DW ? A.ni - i0 : t.hi - t.lo - i0, limit_j = A.nj - j0;
+    const int len = MODE == MODE_DW ? t.hi - t.lo : t.e < A.experts ? A.len : 0;
+    const int steps = (len + BK - 1) / BK;
+    StagedFeed<DT_F32, ALONG, B, BK, 4> fa;
+    StagedFeed<DT_F32, BLONG, B, BK, 4> fb;
+    {
+        const int64_t first_row = MODE == MODE_DW ? t.lo : t.lo + i0;
+        const int pitch_a = MODE == MODE_DW ? A.ni : A.len, pitch_b = MODE == MODE_Y ? A.len : A.nj;
+        const uint8_t* pa = at<DT_F32>(A.a, first_row * pitch_a);
+        const uint8_t* pb = MODE == MODE_DW ? at<DT_F32>(A.b, (int64_t)t.lo * A.nj)
+                                            : at<DT_F32>(A.b, (int64_t)(t.e < A.experts ? t.e : 0) * A.len * A.nj);
+        if (MODE == MODE_Y) pb = at<DT_F32>(pb, (int64_t)j0 * A.len);
+        fa.start(pa, pitch_a, ALONG ? 0 : i0, ALONG ? limit_i : A.ni, len);
+        fb.start(pb, pitch_b, BLONG ? 0 : j0, BLONG ? limit_j : A.nj, len);
+    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
+    const int wi = (wave & 1) * (B / 2), wj = (wave >> 1) * (B / 2);
+    FragmentsF32<ALONG, B, NI> ra;
+    FragmentsF32<BLONG, B, NI> rb;
+    ra.start(wi);
+    rb.start(wj);
+    mm_f32x16 acc[NI][NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+    if (steps > 0) {
+        fa.load(0);
+        fb.load(0);
+    }
+    for (int s = 0; s < steps; ++s) {
+        uint8_t* now = lds[s & 1];
+        fa.store(s, now);
+        fb.store(s, now + BYTES);
+        if (s + 1 < steps) {
+            fa.load(s + 1);
+            fb.load(s + 1);
+        }
+        __syncthreads();   // written; and whoever is here has read the buffer that the next step writes
+#pragma unroll
+        for (int h = 0; h < BK / 8; ++h) {
+            mm_f32x4 a[NI], b[NI];
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                a[i] = ra.read(now, i, h);
+                b[i] = rb.read(now + BYTES, i, h);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                for (int i = 0; i < NI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(b[j][q], a[i][q], acc[i][j], 0, 0, 0);
+        }
+    }
+    float* out;
+    if constexpr (MODE == MODE_DW) {
+        out = (A.splits > 1 ? part_of(A, t) : static_cast<float*>(A.c) + (int64_t)t.e * A.ni * A.nj) + (int64_t)i0 * A.nj + j0;
+    } else {
+        out = static_cast<float*>(A.c) + (int64_t)(t.lo + i0) * A.nj + j0;
+    }
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const int row = wi + 32 * i + (lane & 31);
+        if (row >= limit_i) continue;
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float four[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                store_like<DT_F32, 4>(out + (int64_t)row * A.nj, wj + 32 * j + 8 * q + 4 * (lane >> 5), limit_j, four);
+            }
+    }
+}
 
 // --------------------------------------------------------------------- launches
 
+constexpr int64_t kExpertSize = (int64_t)1 << 22, kExpertRows = (int64_t)1 << 30;
+
+// How a call is cut: which kernel, its tile, and the parts of the rows of a dW.
+struct Plan {
+    enum { FEW, ANY, LARGE, SMALL, F32_128, F32_64 } kernel;
+    int tile, splits;
+};
+
+static Plan plan_experts(int mode, int32_t dtype, int64_t rows, int64_t experts, int64_t n, int64_t k)
+{
+    const bool bf = dtype == ADAMBRIDGE_DT_BF16;
+    const int64_t used = std::min(rows, experts), ni = n, nj = mode == MODE_Y ? n : k;
+    if (mode == MODE_Y && rows <= std::max<int64_t>(64, 8 * experts)) return {Plan::FEW, 0, 1};
+    // rows of a piece or more, a tile of 256 of them within 32-bit offsets
+    const int64_t piece = bf ? 8 : 4;
+    if (n < piece || k < piece || n > kExpertSize / 4 || k > kExpertSize / 4) return {Plan::ANY, kTile, 1};
+    // tiles, if every expert's last one is half empty
+    auto tiles = [&](int64_t t) {
+        const int64_t j = (nj + t - 1) / t;
+        return mode == MODE_DW ? experts * ((ni + t - 1) / t) * j : (rows / t + (used + 1) / 2) * j;
+    };
+    Plan p = bf ? Plan{Plan::LARGE, 256, 1} : Plan{Plan::F32_128, 128, 1};
+    if (tiles(p.tile) < (bf ? 128 : 512)) p = bf ? Plan{Plan::SMALL, 128, 1} : Plan{Plan::F32_64, 64, 1};
+    if (mode == MODE_DW) {   // few tiles with many rows: parts of 256 rows or more, two workgroups a CU
+        const int64_t t = std::max<int64_t>(1, tiles(p.tile));
+        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / t, rows / experts / 256));
+    }
+    return p;
+}
+
 template <int MODE>
 static int experts_mm(const void* a, const void* b, const int32_t* ends, void* c, int32_t dtype, int64_t rows, int64_t experts,
-                      int64_t n, int64_t k)
+                      int64_t n, int64_t k, void* work)
 {
-    constexpr int64_t most = (int64_t)1 << 22;
-    if (rows < 0 || rows > (int64_t)1 << 30 || experts < 1 || experts > kExpertsMost || n < 1 || n > most || k < 1 || k > most)
+    if (rows < 0 || rows > kExpertRows || experts < 1 || experts > kExpertsMost || n < 1 || n > kExpertSize || k < 1 || k > kExpertSize)
         return ADAMBRIDGE_EBADN;
     if (dtype != ADAMBRIDGE_DT_F32 && dtype != ADAMBRIDGE_DT_BF16) return ADAMBRIDGE_EMVDTYPE;
     if (MODE != MODE_DW && rows == 0) return 0;
-    if ((!a && rows) || (!b && rows) || !ends || !c) return ADAMBRIDGE_ENULL;
+    const Plan p = plan_experts(MODE, dtype, rows, experts, n, k);
+    if ((!a && rows) || (!b && rows) || !ends || !c || (p.splits > 1 && !work)) return ADAMBRIDGE_ENULL;
+    if (p.splits > 1 && (uintptr_t)work % 4) return ADAMBRIDGE_EALIGN;
+    const bool bf = dtype == ADAMBRIDGE_DT_BF16;
+    const int64_t size = bf ? 2 : 4;
     ExpertArgs A;
     A.a = a;
     A.b = b;
@@ -594,21 +1063,44 @@ static int experts_mm(const void* a, const void* b, const int32_t* ends, void* c
     A.ni = (int32_t)n;
     A.nj = (int32_t)(MODE == MODE_Y ? n : k);
     A.len = (int32_t)(MODE == MODE_Y ? k : n);
-    // rows of whole 16-byte pieces, 256 of them within a buffer's offsets
-    const bool fast = dtype == ADAMBRIDGE_DT_BF16 && n % 8 == 0 && k % 8 == 0 && n <= (int64_t)1 << 21 && k <= (int64_t)1 << 21 &&
-                      ((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) % 16 == 0;
-    typedef FastConfig C;
-    const int tile_i = fast ? C::BM : kTile, tile_j = fast ? C::BN : kTile;
-    A.tiles_j = (A.nj + tile_j - 1) / tile_j;
-    A.tiles_i = (A.ni + tile_i - 1) / tile_i;
-    // every expert, and the rows that are no expert's, may have a partial tile
-    const int64_t tiles = MODE == MODE_DW ? experts * (((int64_t)A.tiles_i * A.tiles_j + kXcd - 1) / kXcd * kXcd)
-                                          : std::min(rows, rows / tile_i + experts + 1) * A.tiles_j;
-    if (tiles > ((int64_t)1 << 31) - 64) return ADAMBRIDGE_EBADN;
-    const dim3 grid((unsigned)((tiles + kXcd - 1) / kXcd * kXcd));
-    if (fast) hipLaunchKernelGGL((k_experts_fast<MODE, C>), grid, dim3(C::T), 0, t_stream, A);
-    else if (dtype == ADAMBRIDGE_DT_BF16) hipLaunchKernelGGL((k_experts_any<DT_BF16, MODE>), grid, dim3(kMmThreads2), 0, t_stream, A);
-    else hipLaunchKernelGGL((k_experts_any<DT_F32, MODE>), grid, dim3(kMmThreads2), 0, t_stream, A);
+    A.splits = p.splits;
+    A.part = static_cast<float*>(work);
+    if (p.kernel == Plan::FEW) {
+        A.tiles_j = (A.nj + kFewColumns - 1) / kFewColumns;
+        const bool even = k * size % 16 == 0 && ((uintptr_t)a | (uintptr_t)b) % 16 == 0 && std::max<int64_t>(rows, kFewColumns) * k * size < (int64_t)1 << 31;
+        const dim3 grid((unsigned)(std::min(rows, experts + 1) * A.tiles_j)), block(kFewWaves * kWave);   // experts that may have rows
+        if (bf && even) hipLaunchKernelGGL((k_experts_few<DT_BF16, true>), grid, block, 0, t_stream, A);
+        else if (bf) hipLaunchKernelGGL((k_experts_few<DT_BF16, false>), grid, block, 0, t_stream, A);
+        else if (even) hipLaunchKernelGGL((k_experts_few<DT_F32, true>), grid, block, 0, t_stream, A);
+        else hipLaunchKernelGGL((k_experts_few<DT_F32, false>), grid, block, 0, t_stream, A);
+    } else {
+        const bool even = n % 8 == 0 && k % 8 == 0 && ((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) % 16 == 0;
+        A.tiles_j = (A.nj + p.tile - 1) / p.tile;
+        A.tiles_i = (A.ni + p.tile - 1) / p.tile;
+        // every expert, and the rows that are no expert's, may have a partial tile
+        const int64_t tiles = MODE == MODE_DW ? experts * p.splits * (((int64_t)A.tiles_i * A.tiles_j + kXcd - 1) / kXcd * kXcd)
+                                              : std::min(rows, rows / p.tile + experts + 1) * A.tiles_j;
+        if (tiles > ((int64_t)1 << 31) - 64) return ADAMBRIDGE_EBADN;
+        const dim3 grid((unsigned)((tiles + kXcd - 1) / kXcd * kXcd));
+        if (p.kernel == Plan::LARGE && even)
+            hipLaunchKernelGGL((k_experts_fast<MODE, LargeTile, true>), grid, dim3(LargeTile::T), 0, t_stream, A);
+        else if (p.kernel == Plan::LARGE)
+            hipLaunchKernelGGL((k_experts_fast<MODE, LargeTile, false>), grid, dim3(LargeTile::T), 0, t_stream, A);
+        else if (p.kernel == Plan::SMALL && even)
+            hipLaunchKernelGGL((k_experts_fast<MODE, SmallTile, true>), grid, dim3(SmallTile::T), 0, t_stream, A);
+        else if (p.kernel == Plan::SMALL)
+            hipLaunchKernelGGL((k_experts_fast<MODE, SmallTile, false>), grid, dim3(SmallTile::T), 0, t_stream, A);
+        else if (p.kernel == Plan::F32_128) hipLaunchKernelGGL((k_experts_f32<MODE, 128>), grid, dim3(256), 0, t_stream, A);
+        else if (p.kernel == Plan::F32_64) hipLaunchKernelGGL((k_experts_f32<MODE, 64>), grid, dim3(256), 0, t_stream, A);
+        else if (bf) hipLaunchKernelGGL((k_experts_any<DT_BF16, MODE>), grid, dim3(kMmThreads2), 0, t_stream, A);
+        else hipLaunchKernelGGL((k_experts_any<DT_F32, MODE>), grid, dim3(kMmThreads2), 0, t_stream, A);
+    }
+    if (p.splits > 1) {
+        const int64_t values = experts * n * k;
+        const dim3 grid((unsigned)((values + 1023) / 1024));
+        if (bf) hipLaunchKernelGGL((k_experts_sum<DT_BF16>), grid, dim3(256), 0, t_stream, A.part, values, p.splits, c);
+        else hipLaunchKernelGGL((k_experts_sum<DT_F32>), grid, dim3(256), 0, t_stream, A.part, values, p.splits, c);
+    }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : hip_fail(e, "hipLaunchKernelGGL (expert product)");
 }
@@ -622,19 +1114,28 @@ extern "C" {
 ADAMBRIDGE_API int adambridge_expert_mm(const void* x, const void* weight, const int32_t* ends, void* y, int32_t dtype,
                                         int64_t rows, int64_t experts, int64_t n, int64_t k)
 {
-    return experts_mm<MODE_Y>(x, weight, ends, y, dtype, rows, experts, n, k);
+    return experts_mm<MODE_Y>(x, weight, ends, y, dtype, rows, experts, n, k, nullptr);
 }
 
 ADAMBRIDGE_API int adambridge_expert_mm_dx(const void* gout, const void* weight, const int32_t* ends, void* dx, int32_t dtype,
                                            int64_t rows, int64_t experts, int64_t n, int64_t k)
 {
-    return experts_mm<MODE_DX>(gout, weight, ends, dx, dtype, rows, experts, n, k);
+    return experts_mm<MODE_DX>(gout, weight, ends, dx, dtype, rows, experts, n, k, nullptr);
+}
+
+ADAMBRIDGE_API int64_t adambridge_expert_mm_dw_work(int32_t dtype, int64_t rows, int64_t experts, int64_t n, int64_t k)
+{
+    if (rows < 0 || rows > kExpertRows || experts < 1 || experts > kExpertsMost || n < 1 || n > kExpertSize || k < 1 || k > kExpertSize)
+        return ADAMBRIDGE_EBADN;
+    if (dtype != ADAMBRIDGE_DT_F32 && dtype != ADAMBRIDGE_DT_BF16) return ADAMBRIDGE_EMVDTYPE;
+    const Plan p = plan_experts(MODE_DW, dtype, rows, experts, n, k);
+    return p.splits > 1 ? p.splits * experts * n * k * 4 : 0;
 }
 
 ADAMBRIDGE_API int adambridge_expert_mm_dw(const void* gout, const void* x, const int32_t* ends, void* dw, int32_t dtype,
-                                           int64_t rows, int64_t experts, int64_t n, int64_t k)
+                                           int64_t rows, int64_t experts, int64_t n, int64_t k, void* work)
 {
-    return experts_mm<MODE_DW>(gout, x, ends, dw, dtype, rows, experts, n, k);
+    return experts_mm<MODE_DW>(gout, x, ends, dw, dtype, rows, experts, n, k, work);
 }
 
 }  // extern "C"

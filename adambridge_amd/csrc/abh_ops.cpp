@@ -53,6 +53,7 @@ struct Api {
     decltype(&adambridge_combine_backward) combine_backward;
     decltype(&adambridge_expert_mm) expert_mm;
     decltype(&adambridge_expert_mm_dx) expert_mm_dx;
+    decltype(&adambridge_expert_mm_dw_work) expert_mm_dw_work;
     decltype(&adambridge_expert_mm_dw) expert_mm_dw;
 };
 
@@ -443,7 +444,15 @@ struct ExpertMM : Function<ExpertMM> {
         const int64_t n = weight.size(1), k = weight.size(2);
         tensor_list out(3);
         if (want_x) out[0] = run_experts(api.expert_mm_dx, "adambridge_expert_mm_dx", g, weight, ends, {g.size(0), k}, n, k);
-        if (want_w) out[1] = run_experts(api.expert_mm_dw, "adambridge_expert_mm_dw", g, x, ends, weight.sizes(), n, k);
+        if (want_w) {
+            const int64_t bytes = api.expert_mm_dw_work(code(g.scalar_type()), g.size(0), ends.size(0), n, k);
+            check(bytes, "adambridge_expert_mm_dw_work");
+            Tensor work = scratch(bytes, g);
+            out[1] = fresh(weight.sizes(), g.scalar_type(), g);
+            const On on(g);
+            check(api.expert_mm_dw(address(g), address(x), ends.const_data_ptr<int32_t>(), place(out[1]), code(g.scalar_type()), g.size(0),
+                                   ends.size(0), n, k, place(work)), "adambridge_expert_mm_dw");
+        }
         return out;
     }
 };
@@ -485,7 +494,8 @@ PyObject* connect(PyObject*, PyObject* const* args, Py_ssize_t nargs)
         {&found.route, "adambridge_route"}, {&found.route_backward, "adambridge_route_backward"},
         {&found.dispatch, "adambridge_dispatch"}, {&found.combine, "adambridge_combine"},
         {&found.combine_backward, "adambridge_combine_backward"}, {&found.expert_mm, "adambridge_expert_mm"},
-        {&found.expert_mm_dx, "adambridge_expert_mm_dx"}, {&found.expert_mm_dw, "adambridge_expert_mm_dw"}};
+        {&found.expert_mm_dx, "adambridge_expert_mm_dx"}, {&found.expert_mm_dw_work, "adambridge_expert_mm_dw_work"},
+        {&found.expert_mm_dw, "adambridge_expert_mm_dw"}};
     for (const auto& e : entries) {
         PyObject* o = PyDict_GetItemString(args[0], e.name);
         void* const p = o ? PyLong_AsVoidPtr(o) : nullptr;

@@ -136,6 +136,33 @@ __device__ __forceinline__ raw16 load_vec_raw(const void* row, int64_t i, int64_
     return to_raw<DT>(x);   // exact
 }
 
+// 8 BF16 values moved d places down (0 .. 8), zeros after them.
+__device__ __forceinline__ raw16 drop_bf16(const raw16 w, int d)
+{
+    uint64_t lo = (uint64_t)w.y << 32 | w.x, hi = (uint64_t)w.w << 32 | w.z;
+    lo = d & 4 ? hi : lo;
+    hi = d & 4 ? 0u : hi;
+    const int bits = (d & 3) * 16;
+    lo = lo >> bits | (hi << 1) << (63 - bits);
+    hi >>= bits;
+    return d & 8 ? raw16{0u, 0u, 0u, 0u} : raw16{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+}
+
+// 4 FP32 values moved d places down (0 .. 4).
+__device__ __forceinline__ raw16 drop_f32(raw16 w, int d)
+{
+    if (d & 2) w = raw16{w.z, w.w, 0u, 0u};
+    if (d & 1) w = raw16{w.y, w.z, w.w, 0u};
+    return d & 4 ? raw16{0u, 0u, 0u, 0u} : w;
+}
+
+template <int DT>
+__device__ __forceinline__ raw16 drop_values(const raw16 w, int d)
+{
+    if constexpr (DT == DT_BF16) return drop_bf16(w, d);
+    else return drop_f32(w, d);
+}
+
 // N values of WT at i .. of a row of n (N a lane's values of another type), `none` without a row.
 template <int WT, int N>
 __device__ __forceinline__ void load_like(const void* row, int64_t i, int64_t n, float none, float* x)

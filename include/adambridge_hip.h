@@ -548,14 +548,15 @@ ADAMBRIDGE_API int adambridge_combine_backward(const void* gout, const void* row
 /* Products grouped by expert (1 .. 4096): rows (0 .. 2^30) sorted by expert, expert e's being ends[e - 1] .. ends[e] - 1 (ends
  * in device memory, none below the one before it; the first expert's start at 0); weight: experts x n x k (n and k 1 ..
  * 2^22).  y = x weight[e]^T (x: rows x k, y: rows x n); dx = gout weight[e] (gout: rows x n); dw[e] = gout^T x over e's
- * rows, zeros where there are none.  Rows from the last end on give zeros.  Ends that break the rule give
+ * rows, zeros where there are none (work: adambridge_expert_mm_dw_work bytes, NULL if 0).  Rows from the last end on give zeros.  Ends that break the rule give
  * unspecified values, and nothing outside the arrays is touched. */
 ADAMBRIDGE_API int adambridge_expert_mm(const void* x, const void* weight, const int32_t* ends, void* y, int32_t dtype,
                                         int64_t rows, int64_t experts, int64_t n, int64_t k);
 ADAMBRIDGE_API int adambridge_expert_mm_dx(const void* gout, const void* weight, const int32_t* ends, void* dx, int32_t dtype,
                                            int64_t rows, int64_t experts, int64_t n, int64_t k);
+ADAMBRIDGE_API int64_t adambridge_expert_mm_dw_work(int32_t dtype, int64_t rows, int64_t experts, int64_t n, int64_t k);
 ADAMBRIDGE_API int adambridge_expert_mm_dw(const void* gout, const void* x, const int32_t* ends, void* dw, int32_t dtype,
-                                           int64_t rows, int64_t experts, int64_t n, int64_t k);
+                                           int64_t rows, int64_t experts, int64_t n, int64_t k, void* work);
 
 #ifdef __cplusplus
 }
