@@ -125,7 +125,7 @@ EXPORTS = (
     "adambridge_layer_norm", "adambridge_layer_norm_work", "adambridge_layer_norm_backward", "adambridge_route_work",
     "adambridge_route", "adambridge_route_backward", "adambridge_dispatch", "adambridge_combine",
     "adambridge_combine_backward", "adambridge_expert_mm", "adambridge_expert_mm_dx",
-    "adambridge_expert_mm_dw_work", "adambridge_expert_mm_dw",
+    "adambridge_expert_mm_work", "adambridge_expert_mm_dw",
 )
 
 
@@ -182,9 +182,9 @@ def open_library(path: Path = LIB_PATH) -> ctypes.CDLL:
         "adambridge_dispatch": (ctypes.c_int, [vp, i32, vp, i64, i64, i64, vp]),
         "adambridge_combine": (ctypes.c_int, [vp, i32, vp, vp, i64, i64, i64, vp]),
         "adambridge_combine_backward": (ctypes.c_int, [vp, vp, i32, vp, vp, i64, i64, i64, vp, vp]),
-        "adambridge_expert_mm": (ctypes.c_int, [vp, vp, vp, vp, i32, i64, i64, i64, i64]),
-        "adambridge_expert_mm_dx": (ctypes.c_int, [vp, vp, vp, vp, i32, i64, i64, i64, i64]),
-        "adambridge_expert_mm_dw_work": (i64, [i32, i64, i64, i64, i64]),
+        "adambridge_expert_mm": (ctypes.c_int, [vp, vp, vp, vp, i32, i64, i64, i64, i64, vp]),
+        "adambridge_expert_mm_dx": (ctypes.c_int, [vp, vp, vp, vp, i32, i64, i64, i64, i64, vp]),
+        "adambridge_expert_mm_work": (i64, [i32, i32, i64, i64, i64, i64]),
         "adambridge_expert_mm_dw": (ctypes.c_int, [vp, vp, vp, vp, i32, i64, i64, i64, i64, vp]),
     }
     for name in EXPORTS:
@@ -609,18 +609,17 @@ class HipKernels:
                          experts, n, k)
         if wanted[1]:
             dw = torch.empty(experts, n, k, dtype=gout.dtype, device=gout.device)
-            work = self._work(gout.device, "adambridge_expert_mm_dw", _DTYPE_CODES[gout.dtype], rows, experts, n, k)
-            self._expert("adambridge_expert_mm_dw", ("gout", gout, (rows, n)), ("x", x, (rows, k)), ends, dw, experts, n, k,
-                         _address(work))
+            self._expert("adambridge_expert_mm_dw", ("gout", gout, (rows, n)), ("x", x, (rows, k)), ends, dw, experts, n, k)
         return dx, dw
 
-    def _expert(self, name: str, a: tuple, b: tuple, ends: torch.Tensor, out: torch.Tensor, experts: int, n: int, k: int,
-                *work) -> None:
+    def _expert(self, name: str, a: tuple, b: tuple, ends: torch.Tensor, out: torch.Tensor, experts: int, n: int, k: int) -> None:
         for what, t, shape in (a, b):
             self._operand(what, t, tuple(_DTYPE_CODES) if t is a[1] else (a[1].dtype,), shape, out.device)
         self._operand("ends", ends, (torch.int32,), (experts,), out.device)
+        product = ("adambridge_expert_mm", "adambridge_expert_mm_dx", "adambridge_expert_mm_dw").index(name)
+        work = self._work(out.device, "adambridge_expert_mm", product, _DTYPE_CODES[out.dtype], a[1].shape[0], experts, n, k)
         rc = self._on(out.device, getattr(self._lib, name), a[1].data_ptr(), b[1].data_ptr(), ends.data_ptr(), out.data_ptr(),
-                      _DTYPE_CODES[out.dtype], a[1].shape[0], experts, n, k, *work)
+                      _DTYPE_CODES[out.dtype], a[1].shape[0], experts, n, k, _address(work))
         self._check(rc, name)
 
     def fused_adamw(self, master: torch.Tensor, grad: torch.Tensor, m: torch.Tensor, v: torch.Tensor,

@@ -63,34 +63,32 @@ __device__ __forceinline__ void expert_rows(const ExpertArgs& A, int e, int& lo,
 
 struct Tile {
     int e, lo, hi, ti, tj;
+    int split, splits;   // which part of its sum, of how many
+    int rest;            // which of the split tiles
 };
 
 // The tile's numbers in scalar registers: divisions leave them, the same in all lanes, in vector ones, where the addresses made
 // of them cannot describe a buffer.
 __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// This workgroup's row tile of BM rows: consecutive tiles go to one XCD, whose L2 then holds an expert's weights for
-// the tiles of its rows.  Every wavefront finds it for itself.
+// The tiles of BM rows that all experts' rows make.  Every wavefront counts them for itself.
 template <int BM>
-__device__ __forceinline__ bool find_row_tile(const ExpertArgs& A, Tile& t)
+__device__ __forceinline__ int count_row_tiles(const ExpertArgs& A)
 {
-    const int lane = threadIdx.x & 63;
     int total = 0;
     for (int e0 = 0; e0 <= A.experts; e0 += kWave) {
         int lo, hi;
-        expert_rows(A, e0 + lane, lo, hi);
-        int n = (hi - lo + BM - 1) / BM;
-#pragma unroll
-        for (int d = 1; d < kWave; d *= 2) n += __shfl_xor(n, d);
-        total += n;
+        expert_rows(A, e0 + (int)(threadIdx.x & 63), lo, hi);
+        total += group_reduce<kWave>((hi - lo + BM - 1) / BM, [](int a, int b) { return a + b; });
     }
-    total = __builtin_amdgcn_readfirstlane(total);
-    const int tiles = total * A.tiles_j;
-    const int per = (tiles + kXcd - 1) / kXcd;
-    const int slot = (int)(blockIdx.x / kXcd);
-    int idx = (int)(blockIdx.x % kXcd) * per + slot;
-    if (slot >= per || idx >= tiles) return false;
-    const int q = idx / A.tiles_j;
+    return scalar(total) * A.tiles_j;
+}
+
+// Tile idx of them, expert by expert, kGroupTiles row tiles at a time down the columns.
+template <int BM>
+__device__ __forceinline__ bool locate_row_tile(const ExpertArgs& A, int idx, Tile& t)
+{
+    const int lane = threadIdx.x & 63, q = idx / A.tiles_j;
     int before = 0;
     for (int e0 = 0; e0 <= A.experts; e0 += kWave) {
         int lo, hi;
@@ -122,13 +120,64 @@ __device__ __forceinline__ bool find_row_tile(const ExpertArgs& A, Tile& t)
     return false;
 }
 
-// A tile of dW (and of one of the parts of its expert's rows).  The XCDs share every expert's tiles evenly, because
-// experts differ in rows and so in work.
-struct WeightTile : Tile {
-    int split;
+// This workgroup's row tile: consecutive tiles go to one XCD, whose L2 then holds an expert's weights for the tiles of its
+// rows.
+template <int BM>
+__device__ __forceinline__ bool find_row_tile(const ExpertArgs& A, Tile& t)
+{
+    const int tiles = count_row_tiles<BM>(A), per = (tiles + kXcd - 1) / kXcd;
+    const int slot = (int)(blockIdx.x / kXcd), idx = (int)(blockIdx.x % kXcd) * per + slot;
+    t.split = t.rest = 0;
+    t.splits = 1;
+    return slot < per && idx < tiles && locate_row_tile<BM>(A, idx, t);
+}
+
+// The same where a CU has one workgroup: whole rounds of kCus tiles, spread over the XCDs, and the rest of them over the XCDs
+// again.  A short rest would hold all CUs for a whole tile's time: it is cut along the sum into as many parts as fill
+// them (at the price of 512 KB of partial sums a part, written and added up by another kernel, about 30 us, which is 64 steps).
+constexpr int kCus = 256, kMostRest = 128, kMostParts = 16;
+
+struct Rounds {
+    int full, rest, splits;
 };
 
-__device__ __forceinline__ bool find_weight_tile(const ExpertArgs& A, WeightTile& t)
+template <int BM, int BK>
+__device__ __forceinline__ Rounds rounds_of(const ExpertArgs& A)
+{
+    const int tiles = count_row_tiles<BM>(A), steps = (A.len + BK - 1) / BK;
+    Rounds r{tiles / kCus * kCus, tiles % kCus, 1};
+    if (A.part && r.rest > 0 && r.rest <= kMostRest) {
+        const int fit = kCus / r.rest < kMostParts ? kCus / r.rest : kMostParts;
+        if (steps / fit * (fit - 1) >= 64) r.splits = fit;
+    }
+    return r;
+}
+
+template <int BM, int BK>
+__device__ __forceinline__ bool find_round_tile(const ExpertArgs& A, Tile& t)
+{
+    const Rounds r = rounds_of<BM, BK>(A);
+    const int b = (int)blockIdx.x;
+    int idx;
+    t.split = t.rest = 0;
+    t.splits = 1;
+    if (b < r.full) {
+        idx = b % kXcd * (r.full / kXcd) + b / kXcd;
+    } else {
+        const int items = r.rest * r.splits, per = (items + kXcd - 1) / kXcd, slot = (b - r.full) / kXcd;
+        const int item = (b - r.full) % kXcd * per + slot;
+        if (slot >= per || item >= items) return false;
+        t.rest = scalar(item / r.splits);
+        t.split = scalar(item - t.rest * r.splits);
+        t.splits = scalar(r.splits);
+        idx = r.full + t.rest;
+    }
+    return locate_row_tile<BM>(A, idx, t);
+}
+
+// A tile of dW (and of one of the parts of its expert's rows).  The XCDs share every expert's tiles evenly, because
+// experts differ in rows and so in work.
+__device__ __forceinline__ bool find_weight_tile(const ExpertArgs& A, Tile& t)
 {
     const int an = A.tiles_i * A.tiles_j, per = (an + kXcd - 1) / kXcd;
     const int slot = (int)(blockIdx.x / kXcd), turn = slot / per;
@@ -144,6 +193,7 @@ __device__ __forceinline__ bool find_weight_tile(const ExpertArgs& A, WeightTile
     t.tj = scalar(r / wide);
     t.e = scalar(t.e);
     t.split = scalar(t.split);
+    t.splits = A.splits;
     int lo, hi;
     expert_rows(A, t.e, lo, hi);
     lo = scalar(lo);
@@ -154,11 +204,8 @@ __device__ __forceinline__ bool find_weight_tile(const ExpertArgs& A, WeightTile
     return true;
 }
 
-template <int MODE>
-using TileOf = typename std::conditional<MODE == MODE_DW, WeightTile, Tile>::type;
-
 // Where this part's sums go: FP32, rows of nj.
-__device__ __forceinline__ float* part_of(const ExpertArgs& A, const WeightTile& t)
+__device__ __forceinline__ float* part_of(const ExpertArgs& A, const Tile& t)
 {
     return A.part + ((int64_t)t.split * A.experts + t.e) * A.ni * A.nj;
 }
@@ -265,7 +312,7 @@ __global__ __launch_bounds__(kMmThreads2, 2) void k_experts_any(ExpertArgs A)
 {
     constexpr bool ALONG = MODE != MODE_DW, BLONG = MODE == MODE_Y;
     __shared__ __attribute__((aligned(16))) Element<DT> la[kTile * kPitch<DT>], lb[kTile * kPitch<DT>];
-    TileOf<MODE> t;
+    Tile t;
     if constexpr (MODE == MODE_DW) {
         if (!find_weight_tile(A, t)) return;
     } else {
@@ -494,6 +541,7 @@ template <int BM_, int BN_, int BK_, int NB_, int WI_, int WJ_, int OCC_>
 struct Config {
     static constexpr int BM = BM_, BN = BN_, BK = BK_, NB = NB_, WI = WI_, WJ = WJ_, OCC = OCC_, W = WI * WJ, T = W * kWave;
     static constexpr int NI = BM / WI / 32, NJ = BN / WJ / 32;
+    static constexpr bool ROUNDS = NB * (BM + BN) * BK * 2 > 80 * 1024;   // a CU's LDS holds one workgroup's buffers
     static constexpr int LOADS = (BM + BN) * BK * 2 / 1024 / W;   // of a wavefront and step
     static constexpr int BYTES = (BM + BN) * BK * 2;
 };
@@ -524,18 +572,18 @@ struct Feed {
     static constexpr int N = R * BK * 2 / 1024 / W, CH = BK / 8;
     const uint8_t* base;   // the tile's first value
     uint32_t offset[N];    // of this lane's pieces
-    int64_t left;          // !LONG: bytes from base to the operand's end
+    int64_t left;          // bytes from base to the end of the tile's rows, or of the operand's terms
     int32_t pitch;         // bytes
     bool past;             // LONG: whether this lane's pieces are past the end in the last step
 
-    // rows: LONG: the tile's rows; else the operand's terms.  lead: !LONG: bytes before base in its first row.
+    // rows: LONG: the tile's rows; else the operand's terms.  lead: bytes before base in its first row.
     __device__ __forceinline__ void start(const uint8_t* p, int64_t pitch_bytes, int rows, int len, int64_t lead)
     {
         const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
         base = p;
         pitch = (int32_t)pitch_bytes;
         past = false;
-        left = LONG ? (int64_t)(rows < R ? rows : R) * pitch_bytes : (int64_t)rows * pitch_bytes - lead;
+        left = (int64_t)(LONG && rows > R ? R : rows) * pitch_bytes - lead;
 #pragma unroll
         for (int q = 0; q < N; ++q) {
             if constexpr (LONG) {
@@ -551,7 +599,7 @@ struct Feed {
     __device__ __forceinline__ void issue(int step, int steps, uint8_t* lds) const
     {
         const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
-        const int64_t skip = LONG ? 0 : (int64_t)step * BK * pitch;
+        const int64_t skip = LONG ? 0 : (int64_t)step * BK * pitch;   // LONG: the steps are offsets
         const int64_t bytes = left - skip;
         const int32_t range = step >= steps ? 0 : (int32_t)(bytes < 0x7fffffff ? bytes : 0x7fffffff);   // past the end: zeros
         const uint64_t first = (uint64_t)(base + skip);
@@ -708,15 +756,24 @@ __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
     constexpr bool ALONG = MODE != MODE_DW, BLONG = MODE == MODE_Y;
     constexpr int BM = C::BM, BN = C::BN, BK = C::BK, NB = C::NB;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[NB * C::BYTES];
-    TileOf<MODE> t;
+    Tile t;
     if constexpr (MODE == MODE_DW) {
         if (!find_weight_tile(A, t)) return;
+    } else if constexpr (C::ROUNDS) {
+        if (!find_round_tile<BM, BK>(A, t)) return;
     } else {
         if (!find_row_tile<BM>(A, t)) return;
     }
     const int i0 = t.ti * BM, j0 = t.tj * BN;
     const int limit_i = MODE == MODE_DW ? A.ni - i0 : t.hi - t.lo - i0, limit_j = A.nj - j0;
-    const int len = MODE == MODE_DW ? t.hi - t.lo : t.e < A.experts ? A.len : 0;
+    // the terms of this part, from the operands' term k0 on
+    int len = MODE == MODE_DW ? t.hi - t.lo : t.e < A.experts ? A.len : 0, k0 = 0;
+    if (MODE != MODE_DW && C::ROUNDS && t.splits > 1 && len > 0) {
+        const int all = (len + BK - 1) / BK;
+        k0 = all * t.split / t.splits * BK;
+        const int end = all * (t.split + 1) / t.splits * BK;
+        len = (end < len ? end : len) - k0;
+    }
     const int steps = (len + BK - 1) / BK;
     typename std::conditional<EVEN, Feed<ALONG, BM, BK, C::W>, StagedFeed<DT_BF16, ALONG, BM, BK, C::W>>::type fa;
     typename std::conditional<EVEN, Feed<BLONG, BN, BK, C::W>, StagedFeed<DT_BF16, BLONG, BN, BK, C::W>>::type fb;
@@ -728,16 +785,20 @@ __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
         const uint8_t* pb = MODE == MODE_DW ? at<DT_BF16>(A.b, (int64_t)t.lo * A.nj)
                                             : at<DT_BF16>(A.b, (int64_t)(t.e < A.experts ? t.e : 0) * A.len * A.nj);
         if (MODE == MODE_Y) pb = at<DT_BF16>(pb, (int64_t)j0 * A.len);
+        if (MODE != MODE_DW) {
+            pa = at<DT_BF16>(pa, k0);
+            pb = at<DT_BF16>(pb, MODE == MODE_Y ? (int64_t)k0 : (int64_t)k0 * A.nj);
+        }
         if constexpr (EVEN) {
-            fa.start(MODE == MODE_DW ? pa + (int64_t)i0 * 2 : pa, (int64_t)pitch_a * 2, ALONG ? limit_i : len, len, (int64_t)i0 * 2);
-            fb.start(MODE == MODE_Y ? pb : pb + (int64_t)j0 * 2, (int64_t)pitch_b * 2, BLONG ? limit_j : len, len, (int64_t)j0 * 2);
+            fa.start(MODE == MODE_DW ? pa + (int64_t)i0 * 2 : pa, (int64_t)pitch_a * 2, ALONG ? limit_i : len, len, (int64_t)(ALONG ? k0 : i0) * 2);
+            fb.start(MODE == MODE_Y ? pb : pb + (int64_t)j0 * 2, (int64_t)pitch_b * 2, BLONG ? limit_j : len, len, (int64_t)(BLONG ? k0 : j0) * 2);
         } else {
             fa.start(pa, pitch_a, ALONG ? 0 : i0, ALONG ? limit_i : A.ni, len);
             fb.start(pb, pitch_b, BLONG ? 0 : j0, BLONG ? limit_j : A.nj, len);
         }
     }
     const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
-    const int wi = wave % C::WI * (BM / C::WI), wj = wave / C::WI * (BN / C::WJ);
+    const int wi = wave / C::WJ * (BM / C::WI), wj = wave % C::WJ * (BN / C::WJ);   // a SIMD's two wavefronts: other rows each
     Fragments<ALONG, BM, BK, C::NI> ra;
     Fragments<BLONG, BN, BK, C::NJ> rb;
     ra.start(wi);
@@ -797,6 +858,21 @@ __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
         __syncthreads();
         fetch(0, 0, 0);
         int now = 0, next = 1, ahead = LEAD;
+        auto turn = [&]() {
+            now = next;
+            next = next + 1 == NB ? 0 : next + 1;
+            ahead = ahead + 1 == NB ? 0 : ahead + 1;
+        };
+        if (wi >= limit_i) {   // an expert's last rows: no row of this wavefront, which leaves its SIMD to the other one
+            for (int s = 0; s + 1 < steps; ++s) {
+                if constexpr (EVEN) wait_loads<(NB - 3) * C::LOADS>();
+                __syncthreads();
+                issue(s + LEAD, ahead);
+                turn();
+            }
+            if constexpr (EVEN) wait_loads<0>();
+            return;
+        }
         for (int s = 0; s + 1 < steps; ++s) {
 #pragma unroll
             for (int h = 0; h + 1 < H; ++h) {
@@ -811,9 +887,7 @@ __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
             fetch(0, next, 0);
             multiply((H - 1) & 1);
             interleave();
-            now = next;
-            next = next + 1 == NB ? 0 : next + 1;
-            ahead = ahead + 1 == NB ? 0 : ahead + 1;
+            turn();
         }
 #pragma unroll
         for (int h = 0; h < H; ++h) {
@@ -837,6 +911,20 @@ __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
                         store_like<DT_F32, 4>(to + (int64_t)row * A.nj, wj + 32 * j + 8 * q + 4 * (lane >> 5), limit_j, four);
                     }
             }
+            return;
+        }
+    }
+    if constexpr (MODE != MODE_DW && C::ROUNDS) {
+        if (t.splits > 1) {   // a part of the sums of a tile
+            float* to = A.part + ((int64_t)t.rest * t.splits + t.split) * BM * BN;
+#pragma unroll
+            for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+                for (int j = 0; j < C::NJ; ++j)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        *reinterpret_cast<mm_f32x4*>(to + (wi + 32 * i + (lane & 31)) * BN + wj + 32 * j + 8 * q + 4 * (lane >> 5)) =
+                            mm_f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
             return;
         }
     }
@@ -875,6 +963,33 @@ __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
             }
         }
     }
+}
+
+// C's tiles of the rest (find_round_tile) from their parts, in order: 16 rows of a tile a workgroup, 16 columns a lane.
+template <class C>
+__global__ __launch_bounds__(256) void k_experts_rest(ExpertArgs A)
+{
+    const Rounds r = rounds_of<C::BM, C::BK>(A);
+    const int rest = (int)blockIdx.x / (C::BM / 16);
+    Tile t;
+    if (r.splits < 2 || rest >= r.rest || !locate_row_tile<C::BM>(A, r.full + rest, t)) return;
+    const int row = (int)blockIdx.x % (C::BM / 16) * 16 + (int)threadIdx.x / 16, col = (int)threadIdx.x % 16 * (C::BN / 16);
+    const int i = t.ti * C::BM + row, j = t.tj * C::BN + col;
+    if (i >= t.hi - t.lo || j >= A.nj) return;
+    const float* part = A.part + (int64_t)rest * r.splits * C::BM * C::BN + row * C::BN + col;
+    float s[C::BN / 16];
+#pragma unroll
+    for (int k = 0; k < C::BN / 16; ++k) s[k] = 0.0f;
+    for (int p = 0; p < r.splits; ++p)
+#pragma unroll
+        for (int k = 0; k < C::BN / 16; k += 4) {
+            const mm_f32x4 x = *reinterpret_cast<const mm_f32x4*>(part + (int64_t)p * C::BM * C::BN + k);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) s[k + q] += x[q];
+        }
+    void* c = at<DT_BF16>(A.c, (int64_t)(t.lo + i) * A.nj);
+#pragma unroll
+    for (int k = 0; k < C::BN / 16; k += 8) store_like<DT_BF16, 8>(c, j + k, A.nj, s + k);
 }
 
 // (Named here: the host's compilation leaves out their launch functions otherwise.)
@@ -924,7 +1039,7 @@ __global__ __launch_bounds__(256, 2) void k_experts_f32(ExpertArgs A)
     constexpr bool ALONG = MODE != MODE_DW, BLONG = MODE == MODE_Y;
     constexpr int BK = 32, NI = B / 64, BYTES = B * BK * 4;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2][2 * BYTES];
-    TileOf<MODE> t;
+    Tile t;
     if constexpr (MODE == MODE_DW) {
         if (!find_weight_tile(A, t)) return;
     } else {
@@ -1016,27 +1131,31 @@ constexpr int64_t kExpertSize = (int64_t)1 << 22, kExpertRows = (int64_t)1 << 30
 struct Plan {
     enum { FEW, ANY, LARGE, SMALL, F32_128, F32_64 } kernel;
     int tile, splits;
+    bool rest;   // whether the tiles after the last whole round may be cut
+    int64_t work(int64_t values) const { return rest ? (int64_t)kCus * LargeTile::BM * LargeTile::BN * 4 : splits > 1 ? splits * values * 4 : 0; }
 };
 
 static Plan plan_experts(int mode, int32_t dtype, int64_t rows, int64_t experts, int64_t n, int64_t k)
 {
     const bool bf = dtype == ADAMBRIDGE_DT_BF16;
     const int64_t used = std::min(rows, experts), ni = n, nj = mode == MODE_Y ? n : k;
-    if (mode == MODE_Y && rows <= std::max<int64_t>(64, 8 * experts)) return {Plan::FEW, 0, 1};
+    if (mode == MODE_Y && rows <= std::max<int64_t>(64, 8 * experts)) return {Plan::FEW, 0, 1, false};
     // rows of a piece or more, a tile of 256 of them within 32-bit offsets
     const int64_t piece = bf ? 8 : 4;
-    if (n < piece || k < piece || n > kExpertSize / 4 || k > kExpertSize / 4) return {Plan::ANY, kTile, 1};
+    if (n < piece || k < piece || n > kExpertSize / 4 || k > kExpertSize / 4) return {Plan::ANY, kTile, 1, false};
     // tiles, if every expert's last one is half empty
     auto tiles = [&](int64_t t) {
         const int64_t j = (nj + t - 1) / t;
         return mode == MODE_DW ? experts * ((ni + t - 1) / t) * j : (rows / t + (used + 1) / 2) * j;
     };
-    Plan p = bf ? Plan{Plan::LARGE, 256, 1} : Plan{Plan::F32_128, 128, 1};
-    if (tiles(p.tile) < (bf ? 128 : 512)) p = bf ? Plan{Plan::SMALL, 128, 1} : Plan{Plan::F32_64, 64, 1};
+    Plan p = bf ? Plan{Plan::LARGE, 256, 1, false} : Plan{Plan::F32_128, 128, 1, false};
+    if (tiles(p.tile) < (bf ? 128 : 512)) p = bf ? Plan{Plan::SMALL, 128, 1, false} : Plan{Plan::F32_64, 64, 1, false};
     if (mode == MODE_DW) {   // few tiles with many rows: parts of 256 rows or more, two workgroups a CU
         const int64_t t = std::max<int64_t>(1, tiles(p.tile));
         p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / t, rows / experts / 256));
     }
+    // a long sum, and so few rounds that a cut rest may count
+    if (mode != MODE_DW && p.kernel == Plan::LARGE) p.rest = (mode == MODE_Y ? k : n) >= 128 * LargeTile::BK && tiles(256) <= 4 * kCus;
     return p;
 }
 
@@ -1049,8 +1168,8 @@ static int experts_mm(const void* a, const void* b, const int32_t* ends, void* c
     if (dtype != ADAMBRIDGE_DT_F32 && dtype != ADAMBRIDGE_DT_BF16) return ADAMBRIDGE_EMVDTYPE;
     if (MODE != MODE_DW && rows == 0) return 0;
     const Plan p = plan_experts(MODE, dtype, rows, experts, n, k);
-    if ((!a && rows) || (!b && rows) || !ends || !c || (p.splits > 1 && !work)) return ADAMBRIDGE_ENULL;
-    if (p.splits > 1 && (uintptr_t)work % 4) return ADAMBRIDGE_EALIGN;
+    if ((!a && rows) || (!b && rows) || !ends || !c || (p.work(1) && !work)) return ADAMBRIDGE_ENULL;
+    if (p.work(1) && (uintptr_t)work % 16) return ADAMBRIDGE_EALIGN;
     const bool bf = dtype == ADAMBRIDGE_DT_BF16;
     const int64_t size = bf ? 2 : 4;
     ExpertArgs A;
@@ -1064,7 +1183,7 @@ static int experts_mm(const void* a, const void* b, const int32_t* ends, void* c
     A.nj = (int32_t)(MODE == MODE_Y ? n : k);
     A.len = (int32_t)(MODE == MODE_Y ? k : n);
     A.splits = p.splits;
-    A.part = static_cast<float*>(work);
+    A.part = p.splits > 1 || p.rest ? static_cast<float*>(work) : nullptr;
     if (p.kernel == Plan::FEW) {
         A.tiles_j = (A.nj + kFewColumns - 1) / kFewColumns;
         const bool even = k * size % 16 == 0 && ((uintptr_t)a | (uintptr_t)b) % 16 == 0 && std::max<int64_t>(rows, kFewColumns) * k * size < (int64_t)1 << 31;
@@ -1080,8 +1199,8 @@ static int experts_mm(const void* a, const void* b, const int32_t* ends, void* c
         // every expert, and the rows that are no expert's, may have a partial tile
         const int64_t tiles = MODE == MODE_DW ? experts * p.splits * (((int64_t)A.tiles_i * A.tiles_j + kXcd - 1) / kXcd * kXcd)
                                               : std::min(rows, rows / p.tile + experts + 1) * A.tiles_j;
-        if (tiles > ((int64_t)1 << 31) - 64) return ADAMBRIDGE_EBADN;
-        const dim3 grid((unsigned)((tiles + kXcd - 1) / kXcd * kXcd));
+        if (tiles > ((int64_t)1 << 31) - 1024) return ADAMBRIDGE_EBADN;
+        const dim3 grid((unsigned)((tiles + kXcd - 1) / kXcd * kXcd + (p.rest ? kCus : 0)));
         if (p.kernel == Plan::LARGE && even)
             hipLaunchKernelGGL((k_experts_fast<MODE, LargeTile, true>), grid, dim3(LargeTile::T), 0, t_stream, A);
         else if (p.kernel == Plan::LARGE)
@@ -1095,6 +1214,8 @@ static int experts_mm(const void* a, const void* b, const int32_t* ends, void* c
         else if (bf) hipLaunchKernelGGL((k_experts_any<DT_BF16, MODE>), grid, dim3(kMmThreads2), 0, t_stream, A);
         else hipLaunchKernelGGL((k_experts_any<DT_F32, MODE>), grid, dim3(kMmThreads2), 0, t_stream, A);
     }
+    if (p.rest)
+        hipLaunchKernelGGL((k_experts_rest<LargeTile>), dim3(kMostRest * LargeTile::BM / 16), dim3(256), 0, t_stream, A);
     if (p.splits > 1) {
         const int64_t values = experts * n * k;
         const dim3 grid((unsigned)((values + 1023) / 1024));
@@ -1111,25 +1232,25 @@ using namespace abh;
 
 extern "C" {
 
-ADAMBRIDGE_API int adambridge_expert_mm(const void* x, const void* weight, const int32_t* ends, void* y, int32_t dtype,
-                                        int64_t rows, int64_t experts, int64_t n, int64_t k)
+ADAMBRIDGE_API int64_t adambridge_expert_mm_work(int32_t product, int32_t dtype, int64_t rows, int64_t experts, int64_t n, int64_t k)
 {
-    return experts_mm<MODE_Y>(x, weight, ends, y, dtype, rows, experts, n, k, nullptr);
+    if (product < MODE_Y || product > MODE_DW || rows < 0 || rows > kExpertRows || experts < 1 || experts > kExpertsMost || n < 1 ||
+        n > kExpertSize || k < 1 || k > kExpertSize)
+        return ADAMBRIDGE_EBADN;
+    if (dtype != ADAMBRIDGE_DT_F32 && dtype != ADAMBRIDGE_DT_BF16) return ADAMBRIDGE_EMVDTYPE;
+    return rows ? plan_experts(product, dtype, rows, experts, n, k).work(experts * n * k) : 0;
+}
+
+ADAMBRIDGE_API int adambridge_expert_mm(const void* x, const void* weight, const int32_t* ends, void* y, int32_t dtype,
+                                        int64_t rows, int64_t experts, int64_t n, int64_t k, void* work)
+{
+    return experts_mm<MODE_Y>(x, weight, ends, y, dtype, rows, experts, n, k, work);
 }
 
 ADAMBRIDGE_API int adambridge_expert_mm_dx(const void* gout, const void* weight, const int32_t* ends, void* dx, int32_t dtype,
-                                           int64_t rows, int64_t experts, int64_t n, int64_t k)
+                                           int64_t rows, int64_t experts, int64_t n, int64_t k, void* work)
 {
-    return experts_mm<MODE_DX>(gout, weight, ends, dx, dtype, rows, experts, n, k, nullptr);
-}
-
-ADAMBRIDGE_API int64_t adambridge_expert_mm_dw_work(int32_t dtype, int64_t rows, int64_t experts, int64_t n, int64_t k)
-{
-    if (rows < 0 || rows > kExpertRows || experts < 1 || experts > kExpertsMost || n < 1 || n > kExpertSize || k < 1 || k > kExpertSize)
-        return ADAMBRIDGE_EBADN;
-    if (dtype != ADAMBRIDGE_DT_F32 && dtype != ADAMBRIDGE_DT_BF16) return ADAMBRIDGE_EMVDTYPE;
-    const Plan p = plan_experts(MODE_DW, dtype, rows, experts, n, k);
-    return p.splits > 1 ? p.splits * experts * n * k * 4 : 0;
+    return experts_mm<MODE_DX>(gout, weight, ends, dx, dtype, rows, experts, n, k, work);
 }
 
 ADAMBRIDGE_API int adambridge_expert_mm_dw(const void* gout, const void* x, const int32_t* ends, void* dw, int32_t dtype,

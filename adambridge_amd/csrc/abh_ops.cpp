@@ -53,7 +53,7 @@ struct Api {
     decltype(&adambridge_combine_backward) combine_backward;
     decltype(&adambridge_expert_mm) expert_mm;
     decltype(&adambridge_expert_mm_dx) expert_mm_dx;
-    decltype(&adambridge_expert_mm_dw_work) expert_mm_dw_work;
+    decltype(&adambridge_expert_mm_work) expert_mm_work;
     decltype(&adambridge_expert_mm_dw) expert_mm_dw;
 };
 
@@ -414,12 +414,16 @@ PyObject* combine(PyObject*, PyObject* const* args, Py_ssize_t nargs)
 
 // ------------------------------------------------------------------------------- expert_mm
 
-Tensor run_experts(decltype(&adambridge_expert_mm) fn, const char* name, const Tensor& a, const Tensor& b, const Tensor& ends,
-                   at::IntArrayRef sizes, int64_t n, int64_t k)
+Tensor run_experts(int32_t product, const Tensor& a, const Tensor& b, const Tensor& ends, at::IntArrayRef sizes, int64_t n, int64_t k)
 {
-    Tensor out = fresh(sizes, a.scalar_type(), a);
+    const int64_t rows = a.size(0), experts = ends.size(0);
+    const int32_t type = code(a.scalar_type());
+    const int64_t bytes = api.expert_mm_work(product, type, rows, experts, n, k);
+    check(bytes, "adambridge_expert_mm_work");
+    Tensor out = fresh(sizes, a.scalar_type(), a), work = scratch(bytes, a);
     const On on(a);
-    check(fn(address(a), address(b), ends.const_data_ptr<int32_t>(), place(out), code(a.scalar_type()), a.size(0), ends.size(0), n, k), name);
+    const auto fn = product == ADAMBRIDGE_EXPERTS_Y ? api.expert_mm : product == ADAMBRIDGE_EXPERTS_DX ? api.expert_mm_dx : api.expert_mm_dw;
+    check(fn(address(a), address(b), ends.const_data_ptr<int32_t>(), place(out), type, rows, experts, n, k, place(work)), "adambridge_expert_mm");
     return out;
 }
 
@@ -428,7 +432,7 @@ struct ExpertMM : Function<ExpertMM> {
     {
         const at::AutoDispatchBelowADInplaceOrView below;
         ctx->save_for_backward({weight.requires_grad() ? x : Tensor(), weight, ends});
-        return run_experts(api.expert_mm, "adambridge_expert_mm", x, weight, ends, {x.size(0), weight.size(1)}, weight.size(1), weight.size(2));
+        return run_experts(ADAMBRIDGE_EXPERTS_Y, x, weight, ends, {x.size(0), weight.size(1)}, weight.size(1), weight.size(2));
     }
     static tensor_list backward(AutogradContext* ctx, const tensor_list& grads)
     {
@@ -443,16 +447,8 @@ struct ExpertMM : Function<ExpertMM> {
         const Tensor g = grads[0].contiguous();
         const int64_t n = weight.size(1), k = weight.size(2);
         tensor_list out(3);
-        if (want_x) out[0] = run_experts(api.expert_mm_dx, "adambridge_expert_mm_dx", g, weight, ends, {g.size(0), k}, n, k);
-        if (want_w) {
-            const int64_t bytes = api.expert_mm_dw_work(code(g.scalar_type()), g.size(0), ends.size(0), n, k);
-            check(bytes, "adambridge_expert_mm_dw_work");
-            Tensor work = scratch(bytes, g);
-            out[1] = fresh(weight.sizes(), g.scalar_type(), g);
-            const On on(g);
-            check(api.expert_mm_dw(address(g), address(x), ends.const_data_ptr<int32_t>(), place(out[1]), code(g.scalar_type()), g.size(0),
-                                   ends.size(0), n, k, place(work)), "adambridge_expert_mm_dw");
-        }
+        if (want_x) out[0] = run_experts(ADAMBRIDGE_EXPERTS_DX, g, weight, ends, {g.size(0), k}, n, k);
+        if (want_w) out[1] = run_experts(ADAMBRIDGE_EXPERTS_DW, g, x, ends, weight.sizes(), n, k);
         return out;
     }
 };
@@ -472,7 +468,7 @@ PyObject* expert_mm(PyObject*, PyObject* const* args, Py_ssize_t nargs)
         Py_RETURN_NONE;
     if (wants_grad({x, weight})) return THPVariable_Wrap(ExpertMM::apply(*x, *weight, *ends));
     const at::AutoDispatchBelowADInplaceOrView below;
-    return THPVariable_Wrap(run_experts(api.expert_mm, "adambridge_expert_mm", *x, *weight, *ends, {x->size(0), weight->size(1)},
+    return THPVariable_Wrap(run_experts(ADAMBRIDGE_EXPERTS_Y, *x, *weight, *ends, {x->size(0), weight->size(1)},
                                         weight->size(1), weight->size(2)));
     END_HANDLE_TH_ERRORS
 }
@@ -494,7 +490,7 @@ PyObject* connect(PyObject*, PyObject* const* args, Py_ssize_t nargs)
         {&found.route, "adambridge_route"}, {&found.route_backward, "adambridge_route_backward"},
         {&found.dispatch, "adambridge_dispatch"}, {&found.combine, "adambridge_combine"},
         {&found.combine_backward, "adambridge_combine_backward"}, {&found.expert_mm, "adambridge_expert_mm"},
-        {&found.expert_mm_dx, "adambridge_expert_mm_dx"}, {&found.expert_mm_dw_work, "adambridge_expert_mm_dw_work"},
+        {&found.expert_mm_dx, "adambridge_expert_mm_dx"}, {&found.expert_mm_work, "adambridge_expert_mm_work"},
         {&found.expert_mm_dw, "adambridge_expert_mm_dw"}};
     for (const auto& e : entries) {
         PyObject* o = PyDict_GetItemString(args[0], e.name);

@@ -506,7 +506,7 @@ ADAMBRIDGE_API int adambridge_cross_entropy_backward(const void* logits, int32_t
  * ADAMBRIDGE_DT_F32 or _BF16, row-major and contiguous, at any element's address; sums, statistics and weights are FP32
  * and each result is rounded once.  All on the calling thread's stream (asynchronous); results do not depend on
  * scheduling.  Return 0, ADAMBRIDGE_EBADN (a size out of its range), _EMVDTYPE, _ENULL, _EALIGN (work not at a
- * 4-byte boundary) or _EHIP; the _work functions the bytes of scratch a call takes, or ADAMBRIDGE_EBADN / _EMVDTYPE. */
+ * 4-byte boundary, or as said) or _EHIP; the _work functions the bytes of scratch a call takes, or ADAMBRIDGE_EBADN / _EMVDTYPE. */
 
 /* Layer norm over rows of cols values (each 1 .. 2^30): y = (x - mean) rstd weight + bias with rstd = 1 / sqrt(var + eps),
  * var the mean of squared deviations.  weight and bias: cols values of w_dtype, or NULL (1 and 0).  stats: NULL, or the
@@ -548,13 +548,17 @@ ADAMBRIDGE_API int adambridge_combine_backward(const void* gout, const void* row
 /* Products grouped by expert (1 .. 4096): rows (0 .. 2^30) sorted by expert, expert e's being ends[e - 1] .. ends[e] - 1 (ends
  * in device memory, none below the one before it; the first expert's start at 0); weight: experts x n x k (n and k 1 ..
  * 2^22).  y = x weight[e]^T (x: rows x k, y: rows x n); dx = gout weight[e] (gout: rows x n); dw[e] = gout^T x over e's
- * rows, zeros where there are none (work: adambridge_expert_mm_dw_work bytes, NULL if 0).  Rows from the last end on give zeros.  Ends that break the rule give
+ * rows, zeros where there are none.  work: adambridge_expert_mm_work bytes of the product (ADAMBRIDGE_EXPERTS_Y, _DX or
+ * _DW), 16-byte aligned, NULL if 0.  Rows from the last end on give zeros.  Ends that break the rule give
  * unspecified values, and nothing outside the arrays is touched. */
+#define ADAMBRIDGE_EXPERTS_Y 0
+#define ADAMBRIDGE_EXPERTS_DX 1
+#define ADAMBRIDGE_EXPERTS_DW 2
+ADAMBRIDGE_API int64_t adambridge_expert_mm_work(int32_t product, int32_t dtype, int64_t rows, int64_t experts, int64_t n, int64_t k);
 ADAMBRIDGE_API int adambridge_expert_mm(const void* x, const void* weight, const int32_t* ends, void* y, int32_t dtype,
-                                        int64_t rows, int64_t experts, int64_t n, int64_t k);
+                                        int64_t rows, int64_t experts, int64_t n, int64_t k, void* work);
 ADAMBRIDGE_API int adambridge_expert_mm_dx(const void* gout, const void* weight, const int32_t* ends, void* dx, int32_t dtype,
-                                           int64_t rows, int64_t experts, int64_t n, int64_t k);
-ADAMBRIDGE_API int64_t adambridge_expert_mm_dw_work(int32_t dtype, int64_t rows, int64_t experts, int64_t n, int64_t k);
+                                           int64_t rows, int64_t experts, int64_t n, int64_t k, void* work);
 ADAMBRIDGE_API int adambridge_expert_mm_dw(const void* gout, const void* x, const int32_t* ends, void* dw, int32_t dtype,
                                            int64_t rows, int64_t experts, int64_t n, int64_t k, void* work);
 

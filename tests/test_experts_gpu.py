@@ -222,6 +222,17 @@ def test_expert_mm_matches_the_definition(counts, extra, n, k, dtype):
     _check_mm(counts, extra, n, k, dtype, seed=n + k)
 
 
+# what the smaller sizes do not reach: whole rounds of large tiles and a rest that is cut along its sum (of y and of dx), a
+# last tile of few rows, a dW of few tiles in parts of its rows; each with and without rows of whole 16-byte pieces
+@pytest.mark.parametrize("counts,extra,n,k,dtype", [
+    ([2000, 0, 2040], 0, 4096, 2048, torch.bfloat16), ([2040, 2000], 7, 2041, 4099, torch.bfloat16),
+    ([3000, 1090], 0, 4099, 2043, torch.bfloat16), ([70, 300, 2500, 90, 5300], 0, 2048, 4224, torch.bfloat16),
+    ([9001, 0], 0, 264, 72, torch.bfloat16), ([4000, 3001], 9, 130, 67, torch.bfloat16), ([5003], 0, 66, 70, torch.float32),
+    ([1500, 2600, 900], 0, 512, 1028, torch.float32), ([64, 3, 0, 61] * 40, 0, 1024, 520, torch.bfloat16)])
+def test_expert_mm_of_many_rows_matches_the_definition(counts, extra, n, k, dtype):
+    _check_mm(counts, extra, n, k, dtype, seed=n + k)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_no_rows_at_all(dtype):
     x = torch.randn(0, 24, device="cuda").to(dtype).requires_grad_()

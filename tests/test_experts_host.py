@@ -117,13 +117,15 @@ def test_entry_points_check_sizes_types_and_addresses():
     assert lib.adambridge_combine_backward(p, None, f32, p, p, 8, 2, 8, p, p) == enull
     assert lib.adambridge_combine_backward(p, None, f32, p, p, 8, 2, 8, None, None) == 0
 
-    for fn, *work in ((lib.adambridge_expert_mm,), (lib.adambridge_expert_mm_dx,), (lib.adambridge_expert_mm_dw, p)):
+    size = lib.adambridge_expert_mm_work
+    for product, fn in enumerate((lib.adambridge_expert_mm, lib.adambridge_expert_mm_dx, lib.adambridge_expert_mm_dw)):
         for sizes in ((-1, 2, 8, 8), ((1 << 30) + 1, 2, 8, 8), (4, 0, 8, 8), (4, 4097, 8, 8), (4, 2, 0, 8), (4, 2, 8, (1 << 22) + 1)):
-            assert fn(p, p, p, p, f32, *sizes, *work) == ebadn
-        assert fn(p, p, p, p, _hip.DT_F24, 4, 2, 8, 8, *work) == edtype
-        assert fn(p, p, None, p, f32, 4, 2, 8, 8, *work) == enull and fn(p, None, p, p, f32, 4, 2, 8, 8, *work) == enull
-    assert lib.adambridge_expert_mm_dw_work(bf16, 4, 2, 8, 8) == 0 and lib.adambridge_expert_mm_dw_work(bf16, 9000, 1, 64, 64) > 0
-    assert lib.adambridge_expert_mm_dw_work(9, 4, 2, 8, 8) == edtype and lib.adambridge_expert_mm_dw_work(bf16, 4, 0, 8, 8) == ebadn
+            assert fn(p, p, p, p, f32, *sizes, p) == ebadn and size(product, f32, *sizes) == ebadn
+        assert fn(p, p, p, p, _hip.DT_F24, 4, 2, 8, 8, p) == edtype and size(product, _hip.DT_F24, 4, 2, 8, 8) == edtype
+        assert fn(p, p, None, p, f32, 4, 2, 8, 8, p) == enull and fn(p, None, p, p, f32, 4, 2, 8, 8, p) == enull
+        assert size(product, bf16, 4, 2, 8, 8) == 0
+    assert size(3, f32, 4, 2, 8, 8) == ebadn
+    assert size(2, bf16, 9000, 1, 64, 64) > 0 and size(1, bf16, 8192, 8, 8192, 2048) > 0
     assert lib.adambridge_expert_mm_dw(p, p, p, p, bf16, 9000, 1, 64, 64, None) == enull
-    assert lib.adambridge_expert_mm_dw(p, p, p, p, bf16, 9000, 1, 64, 64, ctypes.c_void_p(258)) == ealign
-    assert lib.adambridge_expert_mm(None, p, p, None, f32, 0, 2, 8, 8) == 0   # no rows: nothing to do
+    assert lib.adambridge_expert_mm_dw(p, p, p, p, bf16, 9000, 1, 64, 64, ctypes.c_void_p(264)) == ealign
+    assert lib.adambridge_expert_mm(None, p, p, None, f32, 0, 2, 8, 8, None) == 0   # no rows: nothing to do
