@@ -153,11 +153,10 @@ __device__ __forceinline__ Rounds rounds_of(const ExpertArgs& A)
     return r;
 }
 
-template <int BM, int BK>
-__device__ __forceinline__ bool find_round_tile(const ExpertArgs& A, Tile& t)
+// Item b of them: workgroup blockIdx.x takes blockIdx.x, and + kCus, ... where it goes on.
+template <int BM>
+__device__ __forceinline__ bool find_round_tile(const ExpertArgs& A, const Rounds& r, int b, Tile& t)
 {
-    const Rounds r = rounds_of<BM, BK>(A);
-    const int b = (int)blockIdx.x;
     int idx;
     t.split = t.rest = 0;
     t.splits = 1;
@@ -750,187 +749,72 @@ __device__ __forceinline__ void spread_reads()
     }
 }
 
-template <int MODE, class C, bool EVEN>
-__global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
-{
-    constexpr bool ALONG = MODE != MODE_DW, BLONG = MODE == MODE_Y;
-    constexpr int BM = C::BM, BN = C::BN, BK = C::BK, NB = C::NB;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[NB * C::BYTES];
+// A tile in numbers: C's rows and columns from i0, j0 and how many there are, the operands' terms from k0 on.
+struct Cut {
     Tile t;
-    if constexpr (MODE == MODE_DW) {
-        if (!find_weight_tile(A, t)) return;
-    } else if constexpr (C::ROUNDS) {
-        if (!find_round_tile<BM, BK>(A, t)) return;
-    } else {
-        if (!find_row_tile<BM>(A, t)) return;
+    int i0, j0, limit_i, limit_j, k0, len, steps;
+};
+
+template <int MODE, class C>
+__device__ __forceinline__ Cut cut_of(const ExpertArgs& A, const Tile& t)
+{
+    Cut u;
+    u.t = t;
+    u.i0 = t.ti * C::BM;
+    u.j0 = t.tj * C::BN;
+    u.limit_i = MODE == MODE_DW ? A.ni - u.i0 : t.hi - t.lo - u.i0;
+    u.limit_j = A.nj - u.j0;
+    u.len = MODE == MODE_DW ? t.hi - t.lo : t.e < A.experts ? A.len : 0;
+    u.k0 = 0;
+    if (MODE != MODE_DW && C::ROUNDS && t.splits > 1 && u.len > 0) {
+        const int all = (u.len + C::BK - 1) / C::BK;
+        u.k0 = scalar(all * t.split / t.splits * C::BK);
+        const int end = scalar(all * (t.split + 1) / t.splits * C::BK);
+        u.len = (end < u.len ? end : u.len) - u.k0;
     }
-    const int i0 = t.ti * BM, j0 = t.tj * BN;
-    const int limit_i = MODE == MODE_DW ? A.ni - i0 : t.hi - t.lo - i0, limit_j = A.nj - j0;
-    // the terms of this part, from the operands' term k0 on
-    int len = MODE == MODE_DW ? t.hi - t.lo : t.e < A.experts ? A.len : 0, k0 = 0;
-    if (MODE != MODE_DW && C::ROUNDS && t.splits > 1 && len > 0) {
-        const int all = (len + BK - 1) / BK;
-        k0 = all * t.split / t.splits * BK;
-        const int end = all * (t.split + 1) / t.splits * BK;
-        len = (end < len ? end : len) - k0;
-    }
-    const int steps = (len + BK - 1) / BK;
-    typename std::conditional<EVEN, Feed<ALONG, BM, BK, C::W>, StagedFeed<DT_BF16, ALONG, BM, BK, C::W>>::type fa;
-    typename std::conditional<EVEN, Feed<BLONG, BN, BK, C::W>, StagedFeed<DT_BF16, BLONG, BN, BK, C::W>>::type fb;
-    {
-        // the operands' first values: of this expert's rows and weights
-        const int64_t first_row = MODE == MODE_DW ? t.lo : t.lo + i0;
-        const int pitch_a = MODE == MODE_DW ? A.ni : A.len, pitch_b = MODE == MODE_Y ? A.len : A.nj;
-        const uint8_t* pa = at<DT_BF16>(A.a, first_row * pitch_a);
-        const uint8_t* pb = MODE == MODE_DW ? at<DT_BF16>(A.b, (int64_t)t.lo * A.nj)
-                                            : at<DT_BF16>(A.b, (int64_t)(t.e < A.experts ? t.e : 0) * A.len * A.nj);
-        if (MODE == MODE_Y) pb = at<DT_BF16>(pb, (int64_t)j0 * A.len);
-        if (MODE != MODE_DW) {
-            pa = at<DT_BF16>(pa, k0);
-            pb = at<DT_BF16>(pb, MODE == MODE_Y ? (int64_t)k0 : (int64_t)k0 * A.nj);
-        }
-        if constexpr (EVEN) {
-            fa.start(MODE == MODE_DW ? pa + (int64_t)i0 * 2 : pa, (int64_t)pitch_a * 2, ALONG ? limit_i : len, len, (int64_t)(ALONG ? k0 : i0) * 2);
-            fb.start(MODE == MODE_Y ? pb : pb + (int64_t)j0 * 2, (int64_t)pitch_b * 2, BLONG ? limit_j : len, len, (int64_t)(BLONG ? k0 : j0) * 2);
-        } else {
-            fa.start(pa, pitch_a, ALONG ? 0 : i0, ALONG ? limit_i : A.ni, len);
-            fb.start(pb, pitch_b, BLONG ? 0 : j0, BLONG ? limit_j : A.nj, len);
-        }
-    }
-    const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
-    const int wi = wave / C::WJ * (BM / C::WI), wj = wave % C::WJ * (BN / C::WJ);   // a SIMD's two wavefronts: other rows each
-    Fragments<ALONG, BM, BK, C::NI> ra;
-    Fragments<BLONG, BN, BK, C::NJ> rb;
-    ra.start(wi);
-    rb.start(wj);
-    mm_f32x16 acc[C::NI][C::NJ];
-#pragma unroll
-    for (int i = 0; i < C::NI; ++i)
-#pragma unroll
-        for (int j = 0; j < C::NJ; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-    constexpr int H = BK / 16;
-    constexpr int LEAD = EVEN ? NB - 1 : 2;   // steps from the one that is multiplied to the one on its way to the LDS
-    // the pieces of step s on their way to the LDS (EVEN); else step s's from the registers, and those of the next loaded
-    auto issue = [&](int s, int buffer) {
-        uint8_t* la = lds + buffer * C::BYTES;
-        if constexpr (EVEN) {
-            fa.issue(s, steps, la);
-            fb.issue(s, steps, la + BM * BK * 2);
-        } else {
-            if (s < steps) {
-                fa.store(s, la);
-                fb.store(s, la + BM * BK * 2);
-            }
-            if (s + 1 < steps) {
-                fa.load(s + 1);
-                fb.load(s + 1);
-            }
-        }
-    };
-    // fragments are read one product ahead, so that the LDS works while the matrix cores do
-    mm_bf16x8 a[2][C::NI], b[2][C::NJ];
-    auto fetch = [&](int set, int buffer, int h) {
-        const uint8_t* la = lds + buffer * C::BYTES;
-#pragma unroll
-        for (int i = 0; i < C::NI; ++i) a[set][i] = ra.read(la, i, h);
-#pragma unroll
-        for (int j = 0; j < C::NJ; ++j) b[set][j] = rb.read(la + BM * BK * 2, j, h);
-    };
-    auto multiply = [&](int set) {
-#pragma unroll
-        for (int i = 0; i < C::NI; ++i)
-#pragma unroll
-            for (int j = 0; j < C::NJ; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[set][j], a[set][i], acc[i][j], 0, 0, 0);
-    };
-    constexpr int READS = (ALONG ? 1 : 2) * C::NI + (BLONG ? 1 : 2) * C::NJ, PRODUCTS = C::NI * C::NJ;
-    auto interleave = [&]() { spread_reads<READS, PRODUCTS>(); };
-    if (steps > 0) {
-        if constexpr (!EVEN) {
-            fa.load(0);
-            fb.load(0);
-        }
-#pragma unroll
-        for (int s = 0; s < LEAD; ++s) issue(s, s);
-        if constexpr (EVEN) wait_loads<(NB - 2) * C::LOADS>();
-        __syncthreads();
-        fetch(0, 0, 0);
-        int now = 0, next = 1, ahead = LEAD;
-        auto turn = [&]() {
-            now = next;
-            next = next + 1 == NB ? 0 : next + 1;
-            ahead = ahead + 1 == NB ? 0 : ahead + 1;
-        };
-        if (wi >= limit_i) {   // an expert's last rows: no row of this wavefront, which leaves its SIMD to the other one
-            for (int s = 0; s + 1 < steps; ++s) {
-                if constexpr (EVEN) wait_loads<(NB - 3) * C::LOADS>();
-                __syncthreads();
-                issue(s + LEAD, ahead);
-                turn();
-            }
-            if constexpr (EVEN) wait_loads<0>();
-            return;
-        }
-        for (int s = 0; s + 1 < steps; ++s) {
-#pragma unroll
-            for (int h = 0; h + 1 < H; ++h) {
-                fetch((h + 1) & 1, now, h + 1);
-                multiply(h & 1);
-                interleave();
-            }
-            // the next step's pieces have arrived, everyone's after the barrier, and the step before has been read
-            if constexpr (EVEN) wait_loads<(NB - 3) * C::LOADS>();
-            __syncthreads();
-            issue(s + LEAD, ahead);
-            fetch(0, next, 0);
-            multiply((H - 1) & 1);
-            interleave();
-            turn();
-        }
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-            if (h + 1 < H) fetch((h + 1) & 1, now, h + 1);
-            multiply(h & 1);
-        }
-        if constexpr (EVEN) wait_loads<0>();   // nothing is on its way to the LDS when the workgroup ends
-    }
+    u.steps = (u.len + C::BK - 1) / C::BK;
+    return u;
+}
+
+// Where the results of a wavefront's products go.
+template <int MODE, class C, bool EVEN>
+__device__ __forceinline__ void store_tile(const ExpertArgs& A, const Cut& u, const mm_f32x16 (&acc)[C::NI][C::NJ], int wi, int wj)
+{
+    const int lane = threadIdx.x & 63;
     if constexpr (MODE == MODE_DW) {
         if (A.splits > 1) {   // a part of the sums
-            float* to = part_of(A, t) + j0;
+            float* to = part_of(A, u.t) + u.j0;
 #pragma unroll
             for (int i = 0; i < C::NI; ++i) {
-                const int row = i0 + wi + 32 * i + (lane & 31);
+                const int row = u.i0 + wi + 32 * i + (lane & 31);
                 if (row >= A.ni) continue;
 #pragma unroll
                 for (int j = 0; j < C::NJ; ++j)
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
                         const float four[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                        store_like<DT_F32, 4>(to + (int64_t)row * A.nj, wj + 32 * j + 8 * q + 4 * (lane >> 5), limit_j, four);
+                        store_like<DT_F32, 4>(to + (int64_t)row * A.nj, wj + 32 * j + 8 * q + 4 * (lane >> 5), u.limit_j, four);
                     }
             }
             return;
         }
-    }
-    if constexpr (MODE != MODE_DW && C::ROUNDS) {
-        if (t.splits > 1) {   // a part of the sums of a tile
-            float* to = A.part + ((int64_t)t.rest * t.splits + t.split) * BM * BN;
+    } else if constexpr (C::ROUNDS) {
+        if (u.t.splits > 1) {   // a part of the sums of a tile
+            float* to = A.part + ((int64_t)u.t.rest * u.t.splits + u.t.split) * C::BM * C::BN;
 #pragma unroll
             for (int i = 0; i < C::NI; ++i)
 #pragma unroll
                 for (int j = 0; j < C::NJ; ++j)
 #pragma unroll
                     for (int q = 0; q < 4; ++q)
-                        *reinterpret_cast<mm_f32x4*>(to + (wi + 32 * i + (lane & 31)) * BN + wj + 32 * j + 8 * q + 4 * (lane >> 5)) =
+                        *reinterpret_cast<mm_f32x4*>(to + (wi + 32 * i + (lane & 31)) * C::BN + wj + 32 * j + 8 * q + 4 * (lane >> 5)) =
                             mm_f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
             return;
         }
     }
     // a lane has row lane mod 32 and, of each 8 columns, 4: the two halves exchange fours for whole 16 bytes
-    uint8_t* out = MODE == MODE_DW ? at<DT_BF16>(A.c, ((int64_t)t.e * A.ni + i0) * A.nj + j0)
-                                   : at<DT_BF16>(A.c, (int64_t)(t.lo + i0) * A.nj + j0);
+    uint8_t* out = MODE == MODE_DW ? at<DT_BF16>(A.c, ((int64_t)u.t.e * A.ni + u.i0) * A.nj + u.j0)
+                                   : at<DT_BF16>(A.c, (int64_t)(u.t.lo + u.i0) * A.nj + u.j0);
     const int half = lane >> 5;
 #pragma unroll
     for (int i = 0; i < C::NI; ++i) {
@@ -951,17 +835,178 @@ __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
                 const int c = wj + 32 * j + 8 * (q + half);
                 const raw16 eight = {s0[0], s1[0], s0[1], s1[1]};
                 const int64_t o = (int64_t)row * A.nj + c;
-                if (row >= limit_i || c >= limit_j) continue;
-                if (EVEN || c + 8 <= limit_j) {
+                if (row >= u.limit_i || c >= u.limit_j) continue;
+                if (EVEN || c + 8 <= u.limit_j) {
                     store_raw<DT_BF16>(out, o, eight);
                 } else {
-                    const uint32_t u[4] = {eight.x, eight.y, eight.z, eight.w};
+                    const uint32_t v[4] = {eight.x, eight.y, eight.z, eight.w};
 #pragma unroll
                     for (int r = 0; r < 8; ++r)
-                        if (c + r < limit_j) reinterpret_cast<uint16_t*>(out)[o + r] = (uint16_t)(u[r / 2] >> (16 * (r & 1)));
+                        if (c + r < u.limit_j) reinterpret_cast<uint16_t*>(out)[o + r] = (uint16_t)(v[r / 2] >> (16 * (r & 1)));
                 }
             }
         }
+    }
+}
+
+// Where a CU has one workgroup, y and dx have kCus of them, each with a tile a round: the next tile's first steps are on
+// their way while this one's results are stored (y of 65536 rows, 64 experts 1536 x 2048: 448 -> 436 us).  (dW's tiles differ in work with their experts' rows; those are handed out
+// by the hardware.)
+template <int MODE, class C, bool EVEN>
+__global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
+{
+    constexpr bool ALONG = MODE != MODE_DW, BLONG = MODE == MODE_Y, ROUND = MODE != MODE_DW && C::ROUNDS;
+    constexpr bool MANY = ROUND && EVEN;   // through the registers: no registers for it
+    constexpr int BM = C::BM, BN = C::BN, BK = C::BK, NB = C::NB, H = BK / 16;
+    constexpr int LEAD = EVEN ? NB - 1 : 2;   // steps from the one that is multiplied to the one on its way to the LDS
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[NB * C::BYTES];
+    Tile t;
+    Rounds rounds{};
+    int item = (int)blockIdx.x;
+    if constexpr (MODE == MODE_DW) {
+        if (!find_weight_tile(A, t)) return;
+    } else if constexpr (ROUND) {
+        rounds = rounds_of<BM, BK>(A);
+        if (!find_round_tile<BM>(A, rounds, item, t)) return;
+    } else {
+        if (!find_row_tile<BM>(A, t)) return;
+    }
+    const int wave = threadIdx.x / kWave;
+    const int wi = wave / C::WJ * (BM / C::WI), wj = wave % C::WJ * (BN / C::WJ);   // a SIMD's two wavefronts: other rows each
+    Fragments<ALONG, BM, BK, C::NI> ra;
+    Fragments<BLONG, BN, BK, C::NJ> rb;
+    ra.start(wi);
+    rb.start(wj);
+    typename std::conditional<EVEN, Feed<ALONG, BM, BK, C::W>, StagedFeed<DT_BF16, ALONG, BM, BK, C::W>>::type fa;
+    typename std::conditional<EVEN, Feed<BLONG, BN, BK, C::W>, StagedFeed<DT_BF16, BLONG, BN, BK, C::W>>::type fb;
+    Cut u = cut_of<MODE, C>(A, t);
+    // the pieces of step s on their way to the LDS (EVEN); else step s's from the registers, and those of the next loaded
+    auto issue = [&](int s, int buffer) {
+        uint8_t* la = lds + buffer * C::BYTES;
+        if constexpr (EVEN) {
+            fa.issue(s, u.steps, la);
+            fb.issue(s, u.steps, la + BM * BK * 2);
+        } else {
+            if (s < u.steps) {
+                fa.store(s, la);
+                fb.store(s, la + BM * BK * 2);
+            }
+            if (s + 1 < u.steps) {
+                fa.load(s + 1);
+                fb.load(s + 1);
+            }
+        }
+    };
+    auto begin = [&]() {   // u's first LEAD steps
+        // the operands' first values: of this expert's rows and weights
+        const int64_t first_row = MODE == MODE_DW ? u.t.lo : u.t.lo + u.i0;
+        const int pitch_a = MODE == MODE_DW ? A.ni : A.len, pitch_b = MODE == MODE_Y ? A.len : A.nj;
+        const uint8_t* pa = at<DT_BF16>(A.a, first_row * pitch_a);
+        const uint8_t* pb = MODE == MODE_DW ? at<DT_BF16>(A.b, (int64_t)u.t.lo * A.nj)
+                                            : at<DT_BF16>(A.b, (int64_t)(u.t.e < A.experts ? u.t.e : 0) * A.len * A.nj);
+        if (MODE == MODE_Y) pb = at<DT_BF16>(pb, (int64_t)u.j0 * A.len);
+        if (MODE != MODE_DW) {
+            pa = at<DT_BF16>(pa, u.k0);
+            pb = at<DT_BF16>(pb, MODE == MODE_Y ? (int64_t)u.k0 : (int64_t)u.k0 * A.nj);
+        }
+        if constexpr (EVEN) {
+            fa.start(MODE == MODE_DW ? pa + (int64_t)u.i0 * 2 : pa, (int64_t)pitch_a * 2, ALONG ? u.limit_i : u.len, u.len,
+                     (int64_t)(ALONG ? u.k0 : u.i0) * 2);
+            fb.start(MODE == MODE_Y ? pb : pb + (int64_t)u.j0 * 2, (int64_t)pitch_b * 2, BLONG ? u.limit_j : u.len, u.len,
+                     (int64_t)(BLONG ? u.k0 : u.j0) * 2);
+        } else {
+            fa.start(pa, pitch_a, ALONG ? 0 : u.i0, ALONG ? u.limit_i : A.ni, u.len);
+            fb.start(pb, pitch_b, BLONG ? 0 : u.j0, BLONG ? u.limit_j : A.nj, u.len);
+            if (u.steps > 0) {
+                fa.load(0);
+                fb.load(0);
+            }
+        }
+        if (u.steps > 0)
+#pragma unroll
+            for (int s = 0; s < LEAD; ++s) issue(s, s);
+    };
+    begin();
+    for (;;) {
+        bool more = false;
+        if constexpr (MANY) {   // the next tile's place, while this one's first pieces are on their way
+            item += kCus;
+            more = find_round_tile<BM>(A, rounds, item, t);
+        }
+        mm_f32x16 acc[C::NI][C::NJ];
+#pragma unroll
+        for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+            for (int j = 0; j < C::NJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+        // fragments are read one product ahead, so that the LDS works while the matrix cores do
+        mm_bf16x8 a[2][C::NI], b[2][C::NJ];
+        auto fetch = [&](int set, int buffer, int h) {
+            const uint8_t* la = lds + buffer * C::BYTES;
+#pragma unroll
+            for (int i = 0; i < C::NI; ++i) a[set][i] = ra.read(la, i, h);
+#pragma unroll
+            for (int j = 0; j < C::NJ; ++j) b[set][j] = rb.read(la + BM * BK * 2, j, h);
+        };
+        auto multiply = [&](int set) {
+#pragma unroll
+            for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+                for (int j = 0; j < C::NJ; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[set][j], a[set][i], acc[i][j], 0, 0, 0);
+        };
+        constexpr int READS = (ALONG ? 1 : 2) * C::NI + (BLONG ? 1 : 2) * C::NJ, PRODUCTS = C::NI * C::NJ;
+        if (u.steps > 0) {
+            if constexpr (EVEN) wait_loads<(NB - 2) * C::LOADS>();
+            __syncthreads();
+            int now = 0, next = 1, ahead = LEAD;
+            auto turn = [&]() {
+                now = next;
+                next = next + 1 == NB ? 0 : next + 1;
+                ahead = ahead + 1 == NB ? 0 : ahead + 1;
+            };
+            if (wi >= u.limit_i) {   // an expert's last rows: no row of this wavefront, which leaves its SIMD to the other one
+                for (int s = 0; s + 1 < u.steps; ++s) {
+                    if constexpr (EVEN) wait_loads<(NB - 3) * C::LOADS>();
+                    __syncthreads();
+                    issue(s + LEAD, ahead);
+                    turn();
+                }
+            } else {
+                fetch(0, 0, 0);
+                for (int s = 0; s + 1 < u.steps; ++s) {
+#pragma unroll
+                    for (int h = 0; h + 1 < H; ++h) {
+                        fetch((h + 1) & 1, now, h + 1);
+                        multiply(h & 1);
+                        spread_reads<READS, PRODUCTS>();
+                    }
+                    // the next step's pieces have arrived, everyone's after the barrier, and the step before has been read
+                    if constexpr (EVEN) wait_loads<(NB - 3) * C::LOADS>();
+                    __syncthreads();
+                    issue(s + LEAD, ahead);
+                    fetch(0, next, 0);
+                    multiply((H - 1) & 1);
+                    spread_reads<READS, PRODUCTS>();
+                    turn();
+                }
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    if (h + 1 < H) fetch((h + 1) & 1, now, h + 1);
+                    multiply(h & 1);
+                }
+            }
+            if constexpr (EVEN) wait_loads<0>();   // nothing is on its way to the LDS when the workgroup ends or goes on
+        }
+        const Cut done = u;
+        if (more) {
+            __syncthreads();   // everyone has read this tile's last step
+            u = cut_of<MODE, C>(A, t);
+            begin();
+        }
+        store_tile<MODE, C, EVEN>(A, done, acc, wi, wj);
+        if (!more) break;
     }
 }
 
@@ -1201,10 +1246,11 @@ static int experts_mm(const void* a, const void* b, const int32_t* ends, void* c
                                               : std::min(rows, rows / p.tile + experts + 1) * A.tiles_j;
         if (tiles > ((int64_t)1 << 31) - 1024) return ADAMBRIDGE_EBADN;
         const dim3 grid((unsigned)((tiles + kXcd - 1) / kXcd * kXcd + (p.rest ? kCus : 0)));
+        const dim3 rounds(MODE == MODE_DW || !even ? grid.x : std::min(grid.x, (unsigned)kCus));
         if (p.kernel == Plan::LARGE && even)
-            hipLaunchKernelGGL((k_experts_fast<MODE, LargeTile, true>), grid, dim3(LargeTile::T), 0, t_stream, A);
+            hipLaunchKernelGGL((k_experts_fast<MODE, LargeTile, true>), rounds, dim3(LargeTile::T), 0, t_stream, A);
         else if (p.kernel == Plan::LARGE)
-            hipLaunchKernelGGL((k_experts_fast<MODE, LargeTile, false>), grid, dim3(LargeTile::T), 0, t_stream, A);
+            hipLaunchKernelGGL((k_experts_fast<MODE, LargeTile, false>), rounds, dim3(LargeTile::T), 0, t_stream, A);
         else if (p.kernel == Plan::SMALL && even)
             hipLaunchKernelGGL((k_experts_fast<MODE, SmallTile, true>), grid, dim3(SmallTile::T), 0, t_stream, A);
         else if (p.kernel == Plan::SMALL)

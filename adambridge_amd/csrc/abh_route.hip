@@ -373,7 +373,8 @@ __global__ __launch_bounds__(256) void k_combine(ShuffleArgs A, int vectors)
     }
 }
 
-// An assignment a wavefront: out[row] = w g[t], dw = <g[t], x[row]>.
+// An assignment a wavefront: out[row] = w g[t], dw = <g[t], x[row]>.  The rows, kept since the forward pass, are in no
+// cache and read once (streamed: 113 -> 100 us for 16384 x 4 of 2048; combine's own, just written, are in one).
 template <int DT>
 __global__ __launch_bounds__(256) void k_combine_back(ShuffleArgs A)
 {
@@ -394,7 +395,7 @@ __global__ __launch_bounds__(256) void k_combine_back(ShuffleArgs A)
                 const int64_t cu = c + u * kWave * K;
                 if (cu >= A.cols) continue;
                 g[u] = load_vec_raw<DT>(gt, cu, A.cols);
-                if (A.dw) v[u] = load_vec_raw<DT>(xr, cu, A.cols);
+                if (A.dw) v[u] = load_vec_raw<DT, true>(xr, cu, A.cols);
             }
 #pragma unroll
             for (int u = 0; u < U; ++u) {

@@ -126,11 +126,18 @@ __device__ __forceinline__ void stream_vec(void* row, int64_t i, int64_t n, cons
     }
 }
 
-// The same as they lie in memory.
+// 16 bytes that are read once: not kept in the caches.
 template <int DT>
+__device__ __forceinline__ raw16 once_raw(const void* base, int64_t i)
+{
+    return __builtin_nontemporal_load(reinterpret_cast<const typename Vec16<DT>::type*>(at<DT>(base, i)));
+}
+
+// The same as they lie in memory.
+template <int DT, bool ONCE = false>
 __device__ __forceinline__ raw16 load_vec_raw(const void* row, int64_t i, int64_t n)
 {
-    if (i + kLane<DT> <= n) return load_raw<DT>(row, i);
+    if (i + kLane<DT> <= n) return ONCE ? once_raw<DT>(row, i) : load_raw<DT>(row, i);
     float x[kLane<DT>];
     load_vec<DT>(row, i, n, x);
     return to_raw<DT>(x);   // exact
