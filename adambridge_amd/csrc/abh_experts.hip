@@ -229,6 +229,7 @@ __global__ __launch_bounds__(256) void k_experts_sum(const float* part, int64_t 
 
 // ------------------------------------------------------------- any sizes, any alignment
 //
+// For rows shorter than a piece of 16 bytes and sizes beyond 2^20; right for all of them.
 // Tiles of 128 x 128, four wavefronts of 64 x 64, 32 terms a step; the next step's values are loaded to registers while
 // the one before is multiplied.  LDS rows of 32 terms are padded by 16 bytes, so that the 16-byte reads of 16
 // rows fall on different banks.  A lane's values of k come 16 bytes at a time: the matrix instructions take
@@ -409,6 +410,10 @@ __global__ __launch_bounds__(kMmThreads2, 2) void k_experts_any(ExpertArgs A)
 // 16 columns of C a workgroup, whose four wavefronts split the sum and add their parts in order.  The rows are the
 // matrix instruction's other side, 16 at a time (whatever their number costs nothing beside the weights) and up to
 // 64 for one reading.  Any size and alignment; a workgroup finds the expert that is the blockIdx-th with rows.
+//
+// Measured on MI355X, 64 experts 1536 x 2048 in BF16 that are in no cache: 8 rows 10.8 us (4.65 TB/s of weights), 64 rows 40 us
+// (5.19), 256 rows 69 us (5.29); FP32, 256 rows 135 us (5.42).  Bound by the reads on their way: 16 of a wavefront instead of 8
+// take 12.1, eight wavefronts a workgroup 15.5 us for 8 rows.
 
 constexpr int kFewColumns = 16, kFewWaves = 4, kFewAhead = 8;
 constexpr uint32_t kOutside = 0x80000000u;   // an offset outside every buffer
@@ -522,8 +527,11 @@ __global__ __launch_bounds__(kFewWaves * kWave) void k_experts_few(ExpertArgs A)
 // outside an operand is out of its buffer's range and arrives as zeros.  A wavefront reads the fragments of its next
 // 8 matrix products of 32 x 32 x 16 while the matrix cores work on these.
 //
+// Rows that are not whole 16-byte pieces go through the registers (StagedFeed): 8192 rows of 8 experts 2047 x 1999, a training
+// pass 439 us, 2048 x 2000 308.
+//
 // Measured on MI355X, one expert, 8192^3: y 873 us (1259 TFLOP/s), dx 827 (1329), dW 821 (1339); the matrix cores are busy
-// 73% of the cycles, at 1.6 GHz of 2.4: power is the bound.  Slower: 64 terms a step with two buffers 891 (y),
+// 73% of the cycles, at 1.6 GHz of 2.4: power is the bound (the BLAS library's products: 1501, 1228, 1152).  Slower: 64 terms a step with two buffers 891 (y),
 // wavefronts of 128 x 128 (one a SIMD) 890, tiles of 128 x 256 with two workgroups a CU 1010, three buffers 989; five
 // buffers change nothing.
 //
@@ -600,7 +608,7 @@ struct Feed {
         const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
         const int64_t skip = LONG ? 0 : (int64_t)step * BK * pitch;   // LONG: the steps are offsets
         const int64_t bytes = left - skip;
-        const int32_t range = step >= steps ? 0 : (int32_t)(bytes < 0x7fffffff ? bytes : 0x7fffffff);   // past the end: zeros
+        const int32_t range = step >= steps || bytes < 0 ? 0 : (int32_t)(bytes < 0x7fffffff ? bytes : 0x7fffffff);   // past the end: zeros
         const uint64_t first = (uint64_t)(base + skip);
         const raw16 buffer = {(uint32_t)first, (uint32_t)(first >> 32) & 0xffffu, (uint32_t)range, 0x00020000u};
         const uint32_t along = LONG ? (uint32_t)step * BK * 2 : 0u;
@@ -735,7 +743,8 @@ struct Fragments {
 };
 
 typedef Config<256, 256, 32, 4, 2, 4, 2> LargeTile;
-typedef Config<128, 128, 32, 4, 2, 2, 2> SmallTile;   // where large ones are too few for the CUs
+typedef Config<128, 128, 32, 4, 2, 2, 2> SmallTile;
+static_assert(LargeTile::BM == 256 && LargeTile::BN == 256 && SmallTile::BM == 128 && SmallTile::BN == 128, "plan_experts counts these");   // where large ones are too few for the CUs
 
 // Asks the scheduler for READS reads of the LDS spread among the next PRODUCTS matrix products.
 template <int READS, int PRODUCTS, int M = 0>
@@ -1053,7 +1062,8 @@ ABH_EXPERTS_FAST(SmallTile)
 //
 // The same with FP32 matrix instructions (32 x 32 x 2, a sixteenth of BF16's rate, which bounds it): tiles of 128 x 128 or,
 // where those are few, 64 x 64, four wavefronts of a quarter each, 32 terms a step, two buffers.  A long operand is read
-// four terms a lane, and the instructions take the terms in that order from both.
+// four terms a lane, and the instructions take the terms in that order from both.  4096 x 4096 of 8192 rows: 128 / 124 / 127
+// TFLOP/s (y, dx, dW) of the 157 there are.
 
 template <bool LONG, int R, int N>
 struct FragmentsF32 {
@@ -1180,10 +1190,19 @@ struct Plan {
     int64_t work(int64_t values) const { return rest ? (int64_t)kCus * LargeTile::BM * LargeTile::BN * 4 : splits > 1 ? splits * values * 4 : 0; }
 };
 
+// Measured on MI355X, us, both sides of each line (experts of 1536 x 2048 unless said):
+//   few rows: y of 512 rows, 64 experts 85 streamed / 106 on tiles, 1024 rows 111 / 108; 64 rows of one expert 4096 x 4096 23 / 33,
+//     128 rows 42 / 42;
+//   large or small BF16 tiles: dx of 1024 rows, 8 experts 8192 x 2048 (64 large ones) 155 / 102, 2048 (104) 175 / 168, 4096 (160)
+//     188 / 229; dW of 16 experts 512 x 512 (64) 98 / 42; y of 4096 rows, 64 experts 122 / 102, 8192 (128 an expert) 124 / 126, 12288
+//     136 / 147;
+//   FP32 tiles of 128 or 64: 1237 rows, 5 experts 193 x 333, a training pass 142 / 48; 8192 rows, 8 experts 2048 x 2048 1984 on 128;
+//   parts of a dW: 13499 rows of one expert 704 x 65 382 whole / 30 in parts.
 static Plan plan_experts(int mode, int32_t dtype, int64_t rows, int64_t experts, int64_t n, int64_t k)
 {
     const bool bf = dtype == ADAMBRIDGE_DT_BF16;
     const int64_t used = std::min(rows, experts), ni = n, nj = mode == MODE_Y ? n : k;
+    // few rows an expert: the weights' bytes are all there is
     if (mode == MODE_Y && rows <= std::max<int64_t>(64, 8 * experts)) return {Plan::FEW, 0, 1, false};
     // rows of a piece or more, a tile of 256 of them within 32-bit offsets
     const int64_t piece = bf ? 8 : 4;
@@ -1193,14 +1212,16 @@ static Plan plan_experts(int mode, int32_t dtype, int64_t rows, int64_t experts,
         const int64_t j = (nj + t - 1) / t;
         return mode == MODE_DW ? experts * ((ni + t - 1) / t) * j : (rows / t + (used + 1) / 2) * j;
     };
-    Plan p = bf ? Plan{Plan::LARGE, 256, 1, false} : Plan{Plan::F32_128, 128, 1, false};
-    if (tiles(p.tile) < (bf ? 128 : 512)) p = bf ? Plan{Plan::SMALL, 128, 1, false} : Plan{Plan::F32_64, 64, 1, false};
+    Plan p = bf ? Plan{Plan::LARGE, LargeTile::BM, 1, false} : Plan{Plan::F32_128, 128, 1, false};
+    // tiles too few for the CUs, or large ones mostly without rows: smaller ones
+    if (tiles(p.tile) < (bf ? 128 : 512) || (bf && mode != MODE_DW && rows <= 128 * experts))
+        p = bf ? Plan{Plan::SMALL, SmallTile::BM, 1, false} : Plan{Plan::F32_64, 64, 1, false};
     if (mode == MODE_DW) {   // few tiles with many rows: parts of 256 rows or more, two workgroups a CU
         const int64_t t = std::max<int64_t>(1, tiles(p.tile));
         p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / t, rows / experts / 256));
     }
     // a long sum, and so few rounds that a cut rest may count
-    if (mode != MODE_DW && p.kernel == Plan::LARGE) p.rest = (mode == MODE_Y ? k : n) >= 128 * LargeTile::BK && tiles(256) <= 4 * kCus;
+    if (mode != MODE_DW && p.kernel == Plan::LARGE) p.rest = (mode == MODE_Y ? k : n) >= 128 * LargeTile::BK && tiles(LargeTile::BM) <= 4 * kCus;
     return p;
 }
 
