@@ -135,10 +135,13 @@ def _torch_dispatch(x, position):
 
 def _torch_gather_sum(rows, weights, position):
     wide = torch.promote_types(rows.dtype, torch.float32)
-    picked = rows.to(wide).index_select(0, position.reshape(-1).long()).view(*position.shape, rows.shape[1])
-    if weights is not None:
-        picked = picked * weights[:, :, None]   # never narrower than FP32
-    return picked.sum(1).to(rows.dtype)
+    total = None
+    for j in range(position.shape[1]):   # in order; no views, so that ``rows`` may be a batch
+        picked = rows.index_select(0, position[:, j].long()).to(wide)
+        if weights is not None:
+            picked = picked * weights[:, j:j + 1]   # never narrower than FP32
+        total = picked if total is None else total + picked
+    return total.to(rows.dtype)
 
 
 def _dispatch_backward(gout, position):
@@ -151,11 +154,12 @@ def _combine_backward(gout, rows, weights, position, want_rows, want_weights):
     drows = dweights = None
     if want_rows:
         flat = position.reshape(-1).long()
-        inverse = torch.empty_like(flat).scatter(0, flat, torch.arange(flat.numel(), device=flat.device))
-        drows = (weights[:, :, None] * g[:, None, :]).flatten(0, 1).index_select(0, inverse).to(gout.dtype)
+        assignment = torch.empty_like(flat).scatter(0, flat, torch.arange(flat.numel(), device=flat.device))
+        w = weights.reshape(-1).index_select(0, assignment)[:, None]
+        drows = (g.index_select(0, assignment // position.shape[1]) * w).to(gout.dtype)
     if want_weights:
-        picked = rows.float().index_select(0, position.reshape(-1).long()).view(*position.shape, rows.shape[1])
-        dweights = (picked * g[:, None, :]).sum(2)
+        dweights = torch.stack([(rows.index_select(0, position[:, j].long()).float() * g).sum(1)
+                                for j in range(position.shape[1])], 1)
     return drows, dweights, None
 
 
