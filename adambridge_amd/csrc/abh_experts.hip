@@ -485,17 +485,20 @@ __global__ __launch_bounds__(kFewWaves * kWave) void k_experts_few(ExpertArgs A)
                 raw16 xv[U];
 #pragma unroll
                 for (int u = 0; u < U; ++u) xv[u] = x.load(r0 + 16 * c + col, (s + u) * STEP + quarter * V, s + u < s1);
+                mm_f32x4 some = DT == DT_BF16 ? acc[c] : mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};   // FP32: short chains of sums
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     if constexpr (DT == DT_BF16) {
-                        acc[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mm_bf16x8, wv[u]),
-                                                                         __builtin_bit_cast(mm_bf16x8, xv[u]), acc[c], 0, 0, 0);
+                        some = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mm_bf16x8, wv[u]),
+                                                                       __builtin_bit_cast(mm_bf16x8, xv[u]), some, 0, 0, 0);
                     } else {
                         const mm_f32x4 wf = __builtin_bit_cast(mm_f32x4, wv[u]), xf = __builtin_bit_cast(mm_f32x4, xv[u]);
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[q], xf[q], acc[c], 0, 0, 0);
+                        for (int q = 0; q < 4; ++q) some = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[q], xf[q], some, 0, 0, 0);
                     }
                 }
+                if constexpr (DT == DT_BF16) acc[c] = some;
+                else acc[c] += some;
             }
         }
         if (r0 > 0) __syncthreads();   // the parts before have been read
@@ -1065,6 +1068,11 @@ ABH_EXPERTS_FAST(SmallTile)
 // four terms a lane, and the instructions take the terms in that order from both.  4096 x 4096 of 8192 rows: 128 / 124 / 127
 // TFLOP/s (y, dx, dW) of the 157 there are.
 
+// A long sum's rounding errors grow with the chain it is taken in: every kF32Chain steps (256 terms) the products' sums are
+// added to others (norm of the error over the result's, 4096 terms: 1.1e-6 in one chain, 2.3e-7 in chains of 128; those cost 3%
+// of the time, 256 terms half of it).
+constexpr int kF32Chain = 8;
+
 template <bool LONG, int R, int N>
 struct FragmentsF32 {
     int row;
@@ -1122,13 +1130,24 @@ __global__ __launch_bounds__(256, 2) void k_experts_f32(ExpertArgs A)
     FragmentsF32<BLONG, B, NI> rb;
     ra.start(wi);
     rb.start(wj);
-    mm_f32x16 acc[NI][NI];
+    mm_f32x16 acc[NI][NI], sum[NI][NI];
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
         for (int j = 0; j < NI; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = sum[i][j][r] = 0.0f;
+    auto gather = [&]() {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    sum[i][j][r] += acc[i][j][r];
+                    acc[i][j][r] = 0.0f;
+                }
+    };
     if (steps > 0) {
         fa.load(0);
         fb.load(0);
@@ -1157,7 +1176,9 @@ __global__ __launch_bounds__(256, 2) void k_experts_f32(ExpertArgs A)
 #pragma unroll
                     for (int j = 0; j < NI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(b[j][q], a[i][q], acc[i][j], 0, 0, 0);
         }
+        if (s % kF32Chain == kF32Chain - 1) gather();
     }
+    gather();
     float* out;
     if constexpr (MODE == MODE_DW) {
         out = (A.splits > 1 ? part_of(A, t) : static_cast<float*>(A.c) + (int64_t)t.e * A.ni * A.nj) + (int64_t)i0 * A.nj + j0;
@@ -1172,7 +1193,7 @@ __global__ __launch_bounds__(256, 2) void k_experts_f32(ExpertArgs A)
         for (int j = 0; j < NI; ++j)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const float four[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                const float four[4] = {sum[i][j][4 * q], sum[i][j][4 * q + 1], sum[i][j][4 * q + 2], sum[i][j][4 * q + 3]};
                 store_like<DT_F32, 4>(out + (int64_t)row * A.nj, wj + 32 * j + 8 * q + 4 * (lane >> 5), limit_j, four);
             }
     }
@@ -1202,16 +1223,18 @@ static Plan plan_experts(int mode, int32_t dtype, int64_t rows, int64_t experts,
 {
     const bool bf = dtype == ADAMBRIDGE_DT_BF16;
     const int64_t used = std::min(rows, experts), ni = n, nj = mode == MODE_Y ? n : k;
-    // few rows an expert: the weights' bytes are all there is
-    if (mode == MODE_Y && rows <= std::max<int64_t>(64, 8 * experts)) return {Plan::FEW, 0, 1, false};
     // rows of a piece or more, a tile of 256 of them within 32-bit offsets
     const int64_t piece = bf ? 8 : 4;
-    if (n < piece || k < piece || n > kExpertSize / 4 || k > kExpertSize / 4) return {Plan::ANY, kTile, 1, false};
+    const bool any = n < piece || k < piece || n > kExpertSize / 4 || k > kExpertSize / 4;
     // tiles, if every expert's last one is half empty
     auto tiles = [&](int64_t t) {
         const int64_t j = (nj + t - 1) / t;
         return mode == MODE_DW ? experts * ((ni + t - 1) / t) * j : (rows / t + (used + 1) / 2) * j;
     };
+    // few rows an expert: the weights' bytes are all there is; or more, read at once, that would make too few tiles
+    if (mode == MODE_Y && (rows <= std::max<int64_t>(64, 8 * experts) || (rows <= 64 * experts && tiles(64) < 256)))
+        return {Plan::FEW, 0, 1, false};
+    if (any) return {Plan::ANY, kTile, 1, false};
     Plan p = bf ? Plan{Plan::LARGE, LargeTile::BM, 1, false} : Plan{Plan::F32_128, 128, 1, false};
     // tiles too few for the CUs, or large ones mostly without rows: smaller ones
     if (tiles(p.tile) < (bf ? 128 : 512) || (bf && mode != MODE_DW && rows <= 128 * experts))

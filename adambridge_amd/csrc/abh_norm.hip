@@ -38,7 +38,7 @@ struct NormArgs {
     float eps;
 };
 
-// G lanes a row, NV vectors a lane: a wavefront a row (four rows a workgroup) or a workgroup.
+// G lanes a row, NV vectors a lane: part of a wavefront, a wavefront, or a workgroup.
 template <int G>
 constexpr int kNormThreads = G < 256 ? 256 : G;
 
@@ -49,7 +49,7 @@ __global__ __launch_bounds__(kNormThreads<G>) void k_norm(NormArgs A)
     __shared__ float part[2][2 * T / kWave];
     const int lane = threadIdx.x % G;
     const int64_t row = (int64_t)blockIdx.x * (T / G) + threadIdx.x / G;
-    if (G < T && row >= A.rows) return;   // whole wavefronts, and no barrier follows
+    if (G < T && row >= A.rows) return;   // whole groups of lanes that sum together, and no barrier follows
     const void* x = at<DT>(A.x, row * A.cols);
     raw16 v[NV];
     float sum = 0.0f, none = 0.0f;
@@ -148,8 +148,8 @@ __global__ __launch_bounds__(T) void k_norm_back(NormArgs A)
 {
     constexpr int K = kLane<DT>, R = T / G;
     constexpr bool AHEAD = T < 1024;
-    __shared__ float part[2][R][2 * G / kWave];
-    __shared__ float cross[R > 1 ? 2 * R * G * K : 1];
+    __shared__ float part[2][R][G > kWave ? 2 * G / kWave : 1];
+    __shared__ float cross[R > 1 ? R * G * K : 1];
     const int lane = threadIdx.x % G, sub = threadIdx.x / G;
     float w[NV][K], dw[NV][K], db[NV][K];
 #pragma unroll
@@ -216,23 +216,22 @@ __global__ __launch_bounds__(T) void k_norm_back(NormArgs A)
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int64_t c = (int64_t)(i * G + lane) * K;
-        if constexpr (R > 1) {   // the rows' sums, added in order
+#pragma unroll
+        for (int d = R / 2; d; d /= 2) {   // the rows' sums, a tree
             __syncthreads();
+            if (sub >= d && sub < 2 * d)
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                cross[(sub * 2 * K + k) * G + lane] = dw[i][k];
-                cross[(sub * 2 * K + K + k) * G + lane] = db[i][k];
-            }
+                for (int k = 0; k < K; ++k) {
+                    cross[((sub - d) * 2 * K + k) * G + lane] = dw[i][k];
+                    cross[((sub - d) * 2 * K + K + k) * G + lane] = db[i][k];
+                }
             __syncthreads();
-            if (sub == 0) {
+            if (sub < d)
 #pragma unroll
-                for (int r = 1; r < R; ++r)
-#pragma unroll
-                    for (int k = 0; k < K; ++k) {
-                        dw[i][k] += cross[(r * 2 * K + k) * G + lane];
-                        db[i][k] += cross[(r * 2 * K + K + k) * G + lane];
-                    }
-            }
+                for (int k = 0; k < K; ++k) {
+                    dw[i][k] += cross[(sub * 2 * K + k) * G + lane];
+                    db[i][k] += cross[(sub * 2 * K + K + k) * G + lane];
+                }
         }
         if (sub > 0 || c >= A.cols) continue;
         if (gridDim.x == 1) {   // the only workgroup: its sums are the gradients
@@ -362,6 +361,9 @@ struct Shape {
 // Few rows are spread over more lanes: what counts then is how long one row takes.
 static Shape norm_shape(int64_t rows, int64_t cols)
 {
+    if (cols <= 64) return {8, 8, 256};
+    if (cols <= 128) return {16, 8, 256};
+    if (cols <= 256) return {32, 8, 256};
     if (cols <= 512) return {64, 8, 256};
     if (cols <= 1024) return {64, 16, 256};
     if (rows < 1024) {
@@ -381,6 +383,9 @@ static Shape norm_shape(int64_t rows, int64_t cols)
 // Backward a lane holds five values a column and the next row's two: fewer columns a lane.
 static Shape norm_back_shape(int64_t cols)
 {
+    if (cols <= 64) return {8, 8, 512};
+    if (cols <= 128) return {16, 8, 512};
+    if (cols <= 256) return {32, 8, 512};
     if (cols <= 512) return {64, 8, 512};
     if (cols <= 1024) return {64, 16, 512};
     if (cols <= 2048) return {256, 8, 512};
@@ -411,7 +416,7 @@ static void launch_norm(const NormArgs& A, bool back, int parts)
                            t_stream, A);                                                                                \
         return;                                                                                                         \
     }
-    ABH_NORM(64, 8) ABH_NORM(64, 16) ABH_NORM(64, 32) ABH_NORM(64, 64) ABH_NORM(256, 8) ABH_NORM(256, 16) ABH_NORM(256, 32)
+    ABH_NORM(8, 8) ABH_NORM(16, 8) ABH_NORM(32, 8) ABH_NORM(64, 8) ABH_NORM(64, 16) ABH_NORM(64, 32) ABH_NORM(64, 64) ABH_NORM(256, 8) ABH_NORM(256, 16) ABH_NORM(256, 32)
     ABH_NORM(512, 16) ABH_NORM(512, 32) ABH_NORM(1024, 16)
 #undef ABH_NORM
 #define ABH_NORM_BACK(G, N, T)                                                                                          \
@@ -422,7 +427,7 @@ static void launch_norm(const NormArgs& A, bool back, int parts)
             hipLaunchKernelGGL((k_norm_back<DT, WT, G, N / K, T, false>), dim3(parts), dim3(T), 0, t_stream, A);         \
         return;                                                                                                         \
     }
-    ABH_NORM_BACK(64, 8, 512) ABH_NORM_BACK(64, 16, 512) ABH_NORM_BACK(256, 8, 512) ABH_NORM_BACK(256, 16, 512)
+    ABH_NORM_BACK(8, 8, 512) ABH_NORM_BACK(16, 8, 512) ABH_NORM_BACK(32, 8, 512) ABH_NORM_BACK(64, 8, 512) ABH_NORM_BACK(64, 16, 512) ABH_NORM_BACK(256, 8, 512) ABH_NORM_BACK(256, 16, 512)
     ABH_NORM_BACK(512, 16, 512) ABH_NORM_BACK(1024, 16, 1024)
 #undef ABH_NORM_BACK
     if (!back) {

@@ -244,12 +244,13 @@ __device__ __forceinline__ float wave_sum(float x) { return group_sum<kWave>(x);
 
 // Two sums over T lanes of a workgroup whose lanes all take part (in groups of T, this one's number `lane` in its own), for
 // each of them, in an order of its own whatever the schedule.  `part` is the group's 2 T / 64 floats of LDS, not
-// those of the call before: two that take turns need one barrier a call.  One wavefront uses none.
+// those of the call before: two that take turns need one barrier a call.  A wavefront or less (T 8, 16, 32) uses none.
 template <int T>
 __device__ __forceinline__ void block_sum2(float& a, float& b, float* part, int lane)
 {
-    a = wave_sum(a);
-    b = wave_sum(b);
+    constexpr int G = T < kWave ? T : kWave;
+    a = group_sum<G>(a);
+    b = group_sum<G>(b);
     if constexpr (T > kWave) {
         if (lane % kWave == 0) {
             part[lane / kWave] = a;
