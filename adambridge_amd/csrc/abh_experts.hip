@@ -153,10 +153,11 @@ __device__ __forceinline__ Rounds rounds_of(const ExpertArgs& A)
     return r;
 }
 
-// Item b of them: workgroup blockIdx.x takes blockIdx.x, and + kCus, ... where it goes on.
-template <int BM>
-__device__ __forceinline__ bool find_round_tile(const ExpertArgs& A, const Rounds& r, int b, Tile& t)
+template <int BM, int BK>
+__device__ __forceinline__ bool find_round_tile(const ExpertArgs& A, Tile& t)
 {
+    const Rounds r = rounds_of<BM, BK>(A);
+    const int b = (int)blockIdx.x;
     int idx;
     t.split = t.rest = 0;
     t.splits = 1;
@@ -534,7 +535,8 @@ __global__ __launch_bounds__(kFewWaves * kWave) void k_experts_few(ExpertArgs A)
 // pass 439 us, 2048 x 2000 308.
 //
 // Measured on MI355X, one expert, 8192^3: y 873 us (1259 TFLOP/s), dx 827 (1329), dW 821 (1339); the matrix cores are busy
-// 73% of the cycles, at 1.6 GHz of 2.4: power is the bound (the BLAS library's products: 1501, 1228, 1152).  Slower: 64 terms a step with two buffers 891 (y),
+// 73% of the cycles, at 1.6 GHz of 2.4: power is the bound, and what takes stalls away alone gives the clock back (workgroups that go
+// on to the next tile while the last one's results are stored, those stores beside the next loads: 0-3% slower). (The BLAS library's products: 1501, 1228, 1152.)  Slower: 64 terms a step with two buffers 891 (y),
 // wavefronts of 128 x 128 (one a SIMD) 890, tiles of 128 x 256 with two workgroups a CU 1010, three buffers 989; five
 // buffers change nothing.
 //
@@ -594,6 +596,7 @@ struct Feed {
         pitch = (int32_t)pitch_bytes;
         past = false;
         left = (int64_t)(LONG && rows > R ? R : rows) * pitch_bytes - lead;
+        left = left < 0 ? 0 : left;
 #pragma unroll
         for (int q = 0; q < N; ++q) {
             if constexpr (LONG) {
@@ -611,7 +614,7 @@ struct Feed {
         const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
         const int64_t skip = LONG ? 0 : (int64_t)step * BK * pitch;   // LONG: the steps are offsets
         const int64_t bytes = left - skip;
-        const int32_t range = step >= steps || bytes < 0 ? 0 : (int32_t)(bytes < 0x7fffffff ? bytes : 0x7fffffff);   // past the end: zeros
+        const int32_t range = step >= steps ? 0 : (int32_t)(bytes < 0x7fffffff ? bytes : 0x7fffffff);   // past the end: zeros
         const uint64_t first = (uint64_t)(base + skip);
         const raw16 buffer = {(uint32_t)first, (uint32_t)(first >> 32) & 0xffffu, (uint32_t)range, 0x00020000u};
         const uint32_t along = LONG ? (uint32_t)step * BK * 2 : 0u;
@@ -861,25 +864,18 @@ __device__ __forceinline__ void store_tile(const ExpertArgs& A, const Cut& u, co
     }
 }
 
-// Where a CU has one workgroup, y and dx have kCus of them, each with a tile a round: the next tile's first steps are on
-// their way while this one's results are stored (y of 65536 rows, 64 experts 1536 x 2048: 448 -> 436 us).  (dW's tiles differ in work with their experts' rows; those are handed out
-// by the hardware.)
 template <int MODE, class C, bool EVEN>
 __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
 {
     constexpr bool ALONG = MODE != MODE_DW, BLONG = MODE == MODE_Y, ROUND = MODE != MODE_DW && C::ROUNDS;
-    constexpr bool MANY = ROUND && EVEN;   // through the registers: no registers for it
     constexpr int BM = C::BM, BN = C::BN, BK = C::BK, NB = C::NB, H = BK / 16;
     constexpr int LEAD = EVEN ? NB - 1 : 2;   // steps from the one that is multiplied to the one on its way to the LDS
     __shared__ __attribute__((aligned(1024))) uint8_t lds[NB * C::BYTES];
     Tile t;
-    Rounds rounds{};
-    int item = (int)blockIdx.x;
     if constexpr (MODE == MODE_DW) {
         if (!find_weight_tile(A, t)) return;
     } else if constexpr (ROUND) {
-        rounds = rounds_of<BM, BK>(A);
-        if (!find_round_tile<BM>(A, rounds, item, t)) return;
+        if (!find_round_tile<BM, BK>(A, t)) return;
     } else {
         if (!find_row_tile<BM>(A, t)) return;
     }
@@ -891,7 +887,7 @@ __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
     rb.start(wj);
     typename std::conditional<EVEN, Feed<ALONG, BM, BK, C::W>, StagedFeed<DT_BF16, ALONG, BM, BK, C::W>>::type fa;
     typename std::conditional<EVEN, Feed<BLONG, BN, BK, C::W>, StagedFeed<DT_BF16, BLONG, BN, BK, C::W>>::type fb;
-    Cut u = cut_of<MODE, C>(A, t);
+    const Cut u = cut_of<MODE, C>(A, t);
     // the pieces of step s on their way to the LDS (EVEN); else step s's from the registers, and those of the next loaded
     auto issue = [&](int s, int buffer) {
         uint8_t* la = lds + buffer * C::BYTES;
@@ -909,7 +905,7 @@ __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
             }
         }
     };
-    auto begin = [&]() {   // u's first LEAD steps
+    {
         // the operands' first values: of this expert's rows and weights
         const int64_t first_row = MODE == MODE_DW ? u.t.lo : u.t.lo + u.i0;
         const int pitch_a = MODE == MODE_DW ? A.ni : A.len, pitch_b = MODE == MODE_Y ? A.len : A.nj;
@@ -937,89 +933,75 @@ __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
         if (u.steps > 0)
 #pragma unroll
             for (int s = 0; s < LEAD; ++s) issue(s, s);
+    }
+    mm_f32x16 acc[C::NI][C::NJ];
+#pragma unroll
+    for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+        for (int j = 0; j < C::NJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+    // fragments are read one product ahead, so that the LDS works while the matrix cores do
+    mm_bf16x8 a[2][C::NI], b[2][C::NJ];
+    auto fetch = [&](int set, int buffer, int h) {
+        const uint8_t* la = lds + buffer * C::BYTES;
+#pragma unroll
+        for (int i = 0; i < C::NI; ++i) a[set][i] = ra.read(la, i, h);
+#pragma unroll
+        for (int j = 0; j < C::NJ; ++j) b[set][j] = rb.read(la + BM * BK * 2, j, h);
     };
-    begin();
-    for (;;) {
-        bool more = false;
-        if constexpr (MANY) {   // the next tile's place, while this one's first pieces are on their way
-            item += kCus;
-            more = find_round_tile<BM>(A, rounds, item, t);
-        }
-        mm_f32x16 acc[C::NI][C::NJ];
+    auto multiply = [&](int set) {
 #pragma unroll
         for (int i = 0; i < C::NI; ++i)
 #pragma unroll
             for (int j = 0; j < C::NJ; ++j)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-        // fragments are read one product ahead, so that the LDS works while the matrix cores do
-        mm_bf16x8 a[2][C::NI], b[2][C::NJ];
-        auto fetch = [&](int set, int buffer, int h) {
-            const uint8_t* la = lds + buffer * C::BYTES;
-#pragma unroll
-            for (int i = 0; i < C::NI; ++i) a[set][i] = ra.read(la, i, h);
-#pragma unroll
-            for (int j = 0; j < C::NJ; ++j) b[set][j] = rb.read(la + BM * BK * 2, j, h);
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[set][j], a[set][i], acc[i][j], 0, 0, 0);
+    };
+    constexpr int READS = (ALONG ? 1 : 2) * C::NI + (BLONG ? 1 : 2) * C::NJ, PRODUCTS = C::NI * C::NJ;
+    if (u.steps > 0) {
+        if constexpr (EVEN) wait_loads<(NB - 2) * C::LOADS>();
+        __syncthreads();
+        int now = 0, next = 1, ahead = LEAD;
+        auto turn = [&]() {
+            now = next;
+            next = next + 1 == NB ? 0 : next + 1;
+            ahead = ahead + 1 == NB ? 0 : ahead + 1;
         };
-        auto multiply = [&](int set) {
-#pragma unroll
-            for (int i = 0; i < C::NI; ++i)
-#pragma unroll
-                for (int j = 0; j < C::NJ; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[set][j], a[set][i], acc[i][j], 0, 0, 0);
-        };
-        constexpr int READS = (ALONG ? 1 : 2) * C::NI + (BLONG ? 1 : 2) * C::NJ, PRODUCTS = C::NI * C::NJ;
-        if (u.steps > 0) {
-            if constexpr (EVEN) wait_loads<(NB - 2) * C::LOADS>();
-            __syncthreads();
-            int now = 0, next = 1, ahead = LEAD;
-            auto turn = [&]() {
-                now = next;
-                next = next + 1 == NB ? 0 : next + 1;
-                ahead = ahead + 1 == NB ? 0 : ahead + 1;
-            };
-            if (wi >= u.limit_i) {   // an expert's last rows: no row of this wavefront, which leaves its SIMD to the other one
-                for (int s = 0; s + 1 < u.steps; ++s) {
-                    if constexpr (EVEN) wait_loads<(NB - 3) * C::LOADS>();
-                    __syncthreads();
-                    issue(s + LEAD, ahead);
-                    turn();
-                }
-            } else {
-                fetch(0, 0, 0);
-                for (int s = 0; s + 1 < u.steps; ++s) {
-#pragma unroll
-                    for (int h = 0; h + 1 < H; ++h) {
-                        fetch((h + 1) & 1, now, h + 1);
-                        multiply(h & 1);
-                        spread_reads<READS, PRODUCTS>();
-                    }
-                    // the next step's pieces have arrived, everyone's after the barrier, and the step before has been read
-                    if constexpr (EVEN) wait_loads<(NB - 3) * C::LOADS>();
-                    __syncthreads();
-                    issue(s + LEAD, ahead);
-                    fetch(0, next, 0);
-                    multiply((H - 1) & 1);
-                    spread_reads<READS, PRODUCTS>();
-                    turn();
-                }
-#pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    if (h + 1 < H) fetch((h + 1) & 1, now, h + 1);
-                    multiply(h & 1);
-                }
+        fetch(0, 0, 0);
+        if (wi >= u.limit_i) {   // an expert's last rows: no row of this wavefront, which leaves its SIMD to the other one
+            for (int s = 0; s + 1 < u.steps; ++s) {
+                if constexpr (EVEN) wait_loads<(NB - 3) * C::LOADS>();
+                __syncthreads();
+                issue(s + LEAD, ahead);
+                turn();
             }
-            if constexpr (EVEN) wait_loads<0>();   // nothing is on its way to the LDS when the workgroup ends or goes on
+            if constexpr (EVEN) wait_loads<0>();
+            return;
         }
-        const Cut done = u;
-        if (more) {
-            __syncthreads();   // everyone has read this tile's last step
-            u = cut_of<MODE, C>(A, t);
-            begin();
+        for (int s = 0; s + 1 < u.steps; ++s) {
+#pragma unroll
+            for (int h = 0; h + 1 < H; ++h) {
+                fetch((h + 1) & 1, now, h + 1);
+                multiply(h & 1);
+                spread_reads<READS, PRODUCTS>();
+            }
+            // the next step's pieces have arrived, everyone's after the barrier, and the step before has been read
+            if constexpr (EVEN) wait_loads<(NB - 3) * C::LOADS>();
+            __syncthreads();
+            issue(s + LEAD, ahead);
+            fetch(0, next, 0);
+            multiply((H - 1) & 1);
+            spread_reads<READS, PRODUCTS>();
+            turn();
         }
-        store_tile<MODE, C, EVEN>(A, done, acc, wi, wj);
-        if (!more) break;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            if (h + 1 < H) fetch((h + 1) & 1, now, h + 1);
+            multiply(h & 1);
+        }
+        if constexpr (EVEN) wait_loads<0>();   // nothing is on its way to the LDS when the workgroup ends
     }
+    store_tile<MODE, C, EVEN>(A, u, acc, wi, wj);
 }
 
 // C's tiles of the rest (find_round_tile) from their parts, in order: 16 rows of a tile a workgroup, 16 columns a lane.
@@ -1290,11 +1272,10 @@ static int experts_mm(const void* a, const void* b, const int32_t* ends, void* c
                                               : std::min(rows, rows / p.tile + experts + 1) * A.tiles_j;
         if (tiles > ((int64_t)1 << 31) - 1024) return ADAMBRIDGE_EBADN;
         const dim3 grid((unsigned)((tiles + kXcd - 1) / kXcd * kXcd + (p.rest ? kCus : 0)));
-        const dim3 rounds(MODE == MODE_DW || !even ? grid.x : std::min(grid.x, (unsigned)kCus));
         if (p.kernel == Plan::LARGE && even)
-            hipLaunchKernelGGL((k_experts_fast<MODE, LargeTile, true>), rounds, dim3(LargeTile::T), 0, t_stream, A);
+            hipLaunchKernelGGL((k_experts_fast<MODE, LargeTile, true>), grid, dim3(LargeTile::T), 0, t_stream, A);
         else if (p.kernel == Plan::LARGE)
-            hipLaunchKernelGGL((k_experts_fast<MODE, LargeTile, false>), rounds, dim3(LargeTile::T), 0, t_stream, A);
+            hipLaunchKernelGGL((k_experts_fast<MODE, LargeTile, false>), grid, dim3(LargeTile::T), 0, t_stream, A);
         else if (p.kernel == Plan::SMALL && even)
             hipLaunchKernelGGL((k_experts_fast<MODE, SmallTile, true>), grid, dim3(SmallTile::T), 0, t_stream, A);
         else if (p.kernel == Plan::SMALL)
