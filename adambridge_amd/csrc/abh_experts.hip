@@ -582,21 +582,24 @@ __device__ __forceinline__ int swap_of_term(int term)
 template <bool LONG, int R, int BK, int W>
 struct Feed {
     static constexpr int N = R * BK * 2 / 1024 / W, CH = BK / 8;
-    const uint8_t* base;   // the tile's first value
+    const uint8_t* base;   // the next step's first value (LONG: the tile's)
     uint32_t offset[N];    // of this lane's pieces
-    int64_t left;          // bytes from base to the end of the tile's rows, or of the operand's terms
     int32_t pitch;         // bytes
+    int32_t left;          // terms from the next step's first one on
+    int32_t lead;          // !LONG: bytes before base in its row.  LONG: the range
+    int32_t along;         // LONG: bytes from base to the next step
     bool past;             // LONG: whether this lane's pieces are past the end in the last step
 
-    // rows: LONG: the tile's rows; else the operand's terms.  lead: bytes before base in its first row.
-    __device__ __forceinline__ void start(const uint8_t* p, int64_t pitch_bytes, int rows, int len, int64_t lead)
+    // rows: LONG: those of the tile.  before: bytes before base in its first row.
+    __device__ __forceinline__ void start(const uint8_t* p, int pitch_bytes, int rows, int len, int before)
     {
         const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
         base = p;
-        pitch = (int32_t)pitch_bytes;
+        pitch = pitch_bytes;
+        left = len;
+        along = 0;
+        lead = LONG ? (rows < R ? rows < 0 ? 0 : rows : R) * pitch_bytes - before : before;
         past = false;
-        left = (int64_t)(LONG && rows > R ? R : rows) * pitch_bytes - lead;
-        left = left < 0 ? 0 : left;
 #pragma unroll
         for (int q = 0; q < N; ++q) {
             if constexpr (LONG) {
@@ -609,24 +612,29 @@ struct Feed {
             }
         }
     }
-    __device__ __forceinline__ void issue(int step, int steps, uint8_t* lds) const
+    // The next step's pieces to the LDS; past the last step: zeros.
+    __device__ __forceinline__ void issue(uint8_t* lds)
     {
         const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
-        const int64_t skip = LONG ? 0 : (int64_t)step * BK * pitch;   // LONG: the steps are offsets
-        const int64_t bytes = left - skip;
-        const int32_t range = step >= steps ? 0 : (int32_t)(bytes < 0x7fffffff ? bytes : 0x7fffffff);   // past the end: zeros
-        const uint64_t first = (uint64_t)(base + skip);
+        // the range ends with the operand: pieces over the end of its last term, and terms past it, are outside
+        const int terms = left < BK + 1 ? left : BK + 1;
+        const int bytes = LONG ? lead : terms * pitch - lead;
+        const int range = left > 0 ? bytes : 0;
+        const uint64_t first = (uint64_t)base;
         const raw16 buffer = {(uint32_t)first, (uint32_t)(first >> 32) & 0xffffu, (uint32_t)range, 0x00020000u};
-        const uint32_t along = LONG ? (uint32_t)step * BK * 2 : 0u;
+        const bool last = left <= BK;
 #pragma unroll
         for (int q = 0; q < N; ++q) {
             // In assembly, so that the compiler does not wait for it before each transposed read: no register is written, and
             // the arrival is waited for by wait_loads.
             const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)(lds + (q * W + wave) * 1024);
-            const uint32_t from = LONG && step + 1 == steps && past ? kOutside : offset[q];
+            const uint32_t from = LONG && last && past ? kOutside : offset[q];
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                          :: "s"(to), "v"(from), "s"(buffer), "s"(along) : "memory");
         }
+        left -= BK;
+        if constexpr (LONG) along += BK * 2;
+        else base += BK * pitch;
     }
 };
 
@@ -892,8 +900,8 @@ __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
     auto issue = [&](int s, int buffer) {
         uint8_t* la = lds + buffer * C::BYTES;
         if constexpr (EVEN) {
-            fa.issue(s, u.steps, la);
-            fb.issue(s, u.steps, la + BM * BK * 2);
+            fa.issue(la);
+            fb.issue(la + BM * BK * 2);
         } else {
             if (s < u.steps) {
                 fa.store(s, la);
@@ -918,10 +926,8 @@ __global__ __launch_bounds__(C::T, C::OCC) void k_experts_fast(ExpertArgs A)
             pb = at<DT_BF16>(pb, MODE == MODE_Y ? (int64_t)u.k0 : (int64_t)u.k0 * A.nj);
         }
         if constexpr (EVEN) {
-            fa.start(MODE == MODE_DW ? pa + (int64_t)u.i0 * 2 : pa, (int64_t)pitch_a * 2, ALONG ? u.limit_i : u.len, u.len,
-                     (int64_t)(ALONG ? u.k0 : u.i0) * 2);
-            fb.start(MODE == MODE_Y ? pb : pb + (int64_t)u.j0 * 2, (int64_t)pitch_b * 2, BLONG ? u.limit_j : u.len, u.len,
-                     (int64_t)(BLONG ? u.k0 : u.j0) * 2);
+            fa.start(MODE == MODE_DW ? pa + (int64_t)u.i0 * 2 : pa, pitch_a * 2, u.limit_i, u.len, (ALONG ? u.k0 : u.i0) * 2);
+            fb.start(MODE == MODE_Y ? pb : pb + (int64_t)u.j0 * 2, pitch_b * 2, u.limit_j, u.len, (BLONG ? u.k0 : u.j0) * 2);
         } else {
             fa.start(pa, pitch_a, ALONG ? 0 : u.i0, ALONG ? u.limit_i : A.ni, u.len);
             fb.start(pb, pitch_b, BLONG ? 0 : u.j0, BLONG ? u.limit_j : A.nj, u.len);
