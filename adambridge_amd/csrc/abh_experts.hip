@@ -126,7 +126,7 @@ template <int BM>
 __device__ __forceinline__ bool find_row_tile(const ExpertArgs& A, Tile& t)
 {
     const int tiles = count_row_tiles<BM>(A), per = (tiles + kXcd - 1) / kXcd;
-    const int slot = (int)(blockIdx.x / kXcd), idx = (int)(blockIdx.x % kXcd) * per + slot;
+    const int block = (int)block_index(), slot = block / kXcd, idx = block % kXcd * per + slot;
     t.split = t.rest = 0;
     t.splits = 1;
     return slot < per && idx < tiles && locate_row_tile<BM>(A, idx, t);
@@ -157,7 +157,7 @@ template <int BM, int BK>
 __device__ __forceinline__ bool find_round_tile(const ExpertArgs& A, Tile& t)
 {
     const Rounds r = rounds_of<BM, BK>(A);
-    const int b = (int)blockIdx.x;
+    const int b = (int)block_index();
     int idx;
     t.split = t.rest = 0;
     t.splits = 1;
@@ -180,9 +180,9 @@ __device__ __forceinline__ bool find_round_tile(const ExpertArgs& A, Tile& t)
 __device__ __forceinline__ bool find_weight_tile(const ExpertArgs& A, Tile& t)
 {
     const int an = A.tiles_i * A.tiles_j, per = (an + kXcd - 1) / kXcd;
-    const int slot = (int)(blockIdx.x / kXcd), turn = slot / per;
+    const int block = (int)block_index(), slot = block / kXcd, turn = slot / per;
     if (turn >= A.experts * A.splits) return false;
-    const int local = (int)((blockIdx.x + turn) % kXcd) * per + slot - turn * per;   // the first XCD changes: an may be below 8
+    const int local = (block % kXcd + turn) % kXcd * per + slot - turn * per;   // the first XCD changes: an may be below 8
     if (local >= an) return false;
     t.e = turn / A.splits;
     t.split = turn - t.e * A.splits;
@@ -447,8 +447,8 @@ __global__ __launch_bounds__(kFewWaves * kWave) void k_experts_few(ExpertArgs A)
     __shared__ mm_f32x4 parts[W - 1][CH][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int col = lane & 15, quarter = lane >> 4;
-    const int tj = (int)blockIdx.x % A.tiles_j;
-    int skip = (int)blockIdx.x / A.tiles_j;
+    const int block = (int)block_index(), tj = block % A.tiles_j;
+    int skip = block / A.tiles_j;
     int e = -1, lo = 0, hi = 0;
     for (int e0 = 0; e0 <= A.experts; e0 += kWave) {
         int l, h;
@@ -1264,7 +1264,7 @@ static int experts_mm(const void* a, const void* b, const int32_t* ends, void* c
     if (p.kernel == Plan::FEW) {
         A.tiles_j = (A.nj + kFewColumns - 1) / kFewColumns;
         const bool even = k * size % 16 == 0 && ((uintptr_t)a | (uintptr_t)b) % 16 == 0 && std::max<int64_t>(rows, kFewColumns) * k * size < (int64_t)1 << 31;
-        const dim3 grid((unsigned)(std::min(rows, experts + 1) * A.tiles_j)), block(kFewWaves * kWave);   // experts that may have rows
+        const dim3 grid = block_grid(std::min(rows, experts + 1) * A.tiles_j), block(kFewWaves * kWave);   // experts that may have rows
         if (bf && even) hipLaunchKernelGGL((k_experts_few<DT_BF16, true>), grid, block, 0, t_stream, A);
         else if (bf) hipLaunchKernelGGL((k_experts_few<DT_BF16, false>), grid, block, 0, t_stream, A);
         else if (even) hipLaunchKernelGGL((k_experts_few<DT_F32, true>), grid, block, 0, t_stream, A);
@@ -1276,8 +1276,8 @@ static int experts_mm(const void* a, const void* b, const int32_t* ends, void* c
         // every expert, and the rows that are no expert's, may have a partial tile
         const int64_t tiles = MODE == MODE_DW ? experts * p.splits * (((int64_t)A.tiles_i * A.tiles_j + kXcd - 1) / kXcd * kXcd)
                                               : std::min(rows, rows / p.tile + experts + 1) * A.tiles_j;
-        if (tiles > ((int64_t)1 << 31) - 1024) return ADAMBRIDGE_EBADN;
-        const dim3 grid((unsigned)((tiles + kXcd - 1) / kXcd * kXcd + (p.rest ? kCus : 0)));
+        if (tiles > (int64_t)1 << 30) return ADAMBRIDGE_EBADN;   // tiles are counted in 32 bits
+        const dim3 grid = block_grid((tiles + kXcd - 1) / kXcd * kXcd + (p.rest ? kCus : 0));
         if (p.kernel == Plan::LARGE && even)
             hipLaunchKernelGGL((k_experts_fast<MODE, LargeTile, true>), grid, dim3(LargeTile::T), 0, t_stream, A);
         else if (p.kernel == Plan::LARGE)

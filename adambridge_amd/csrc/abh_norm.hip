@@ -48,8 +48,8 @@ __global__ __launch_bounds__(kNormThreads<G>) void k_norm(NormArgs A)
     constexpr int K = kLane<DT>, T = kNormThreads<G>;
     __shared__ float part[2][2 * T / kWave];
     const int lane = threadIdx.x % G;
-    const int64_t row = (int64_t)blockIdx.x * (T / G) + threadIdx.x / G;
-    if (G < T && row >= A.rows) return;   // whole groups of lanes that sum together, and no barrier follows
+    const int64_t row = block_index() * (T / G) + threadIdx.x / G;
+    if (row >= A.rows) return;   // whole groups of lanes that sum together, or the workgroup
     const void* x = at<DT>(A.x, row * A.cols);
     raw16 v[NV];
     float sum = 0.0f, none = 0.0f;
@@ -105,7 +105,8 @@ __global__ __launch_bounds__(1024) void k_norm_long(NormArgs A)
 {
     constexpr int K = kLane<DT>, T = 1024;
     __shared__ float part[2][2 * T / kWave];
-    const int64_t row = blockIdx.x;
+    const int64_t row = block_index();
+    if (row >= A.rows) return;
     const void* x = at<DT>(A.x, row * A.cols);
     float sum = 0.0f, sq = 0.0f, none = 0.0f, v[K];
     for (int64_t c = (int64_t)threadIdx.x * K; c < A.cols; c += T * K) {
@@ -251,7 +252,8 @@ __global__ __launch_bounds__(1024) void k_norm_back_long(NormArgs A)
 {
     constexpr int K = kLane<DT>, T = 1024;
     __shared__ float part[2][2 * T / kWave];
-    const int64_t row = blockIdx.x;
+    const int64_t row = block_index();
+    if (row >= A.rows) return;
     const void* xr = at<DT>(A.x, row * A.cols);
     const void* gr = at<DT>(A.g, row * A.cols);
     const float mean = A.stats[2 * row], rstd = A.stats[2 * row + 1];
@@ -412,8 +414,7 @@ static void launch_norm(const NormArgs& A, bool back, int parts)
 #define ABH_NORM(G, N)                                                                                                  \
     if (!back && s.lanes == G && s.values == N) {                                                                       \
         constexpr int R = kNormThreads<G> / G;                                                                          \
-        hipLaunchKernelGGL((k_norm<DT, WT, G, N / K>), dim3((unsigned)((A.rows + R - 1) / R)), dim3(kNormThreads<G>), 0, \
-                           t_stream, A);                                                                                \
+        hipLaunchKernelGGL((k_norm<DT, WT, G, N / K>), block_grid((A.rows + R - 1) / R), dim3(kNormThreads<G>), 0, t_stream, A); \
         return;                                                                                                         \
     }
     ABH_NORM(8, 8) ABH_NORM(16, 8) ABH_NORM(32, 8) ABH_NORM(64, 8) ABH_NORM(64, 16) ABH_NORM(64, 32) ABH_NORM(64, 64) ABH_NORM(256, 8) ABH_NORM(256, 16) ABH_NORM(256, 32)
@@ -431,10 +432,10 @@ static void launch_norm(const NormArgs& A, bool back, int parts)
     ABH_NORM_BACK(512, 16, 512) ABH_NORM_BACK(1024, 16, 1024)
 #undef ABH_NORM_BACK
     if (!back) {
-        hipLaunchKernelGGL((k_norm_long<DT, WT>), dim3((unsigned)A.rows), dim3(1024), 0, t_stream, A);
+        hipLaunchKernelGGL((k_norm_long<DT, WT>), block_grid(A.rows), dim3(1024), 0, t_stream, A);
         return;
     }
-    if (A.y) hipLaunchKernelGGL((k_norm_back_long<DT, WT>), dim3((unsigned)A.rows), dim3(1024), 0, t_stream, A);
+    if (A.y) hipLaunchKernelGGL((k_norm_back_long<DT, WT>), block_grid(A.rows), dim3(1024), 0, t_stream, A);
     if (A.dw || A.db)
         hipLaunchKernelGGL((k_norm_columns<DT>), dim3((unsigned)((A.cols + 256 * kLane<DT> - 1) / (256 * kLane<DT>)), (unsigned)parts),
                            dim3(256), 0, t_stream, A);

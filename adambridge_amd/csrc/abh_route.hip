@@ -95,7 +95,8 @@ __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs A)
     __shared__ int32_t base[kMostExperts];
     constexpr int kPass = kRouteThreads / G;   // tokens at a time
     const int lane = threadIdx.x % G, sub = threadIdx.x / G;
-    const int64_t t0 = (int64_t)blockIdx.x * kBlockTokens;
+    const int64_t block = block_index(), t0 = block * kBlockTokens;
+    if (block >= A.blocks) return;
     const int tokens = (int)(A.tokens - t0 < kBlockTokens ? A.tokens - t0 : kBlockTokens);
     for (int e = threadIdx.x; e < A.experts; e += kRouteThreads) mask[e] = 0;
     __syncthreads();
@@ -154,7 +155,7 @@ __global__ __launch_bounds__(kRouteThreads) void k_route(RouteArgs A)
     __syncthreads();
     if (A.blocks > 1) {
         for (int e = threadIdx.x; e < A.experts; e += kRouteThreads)
-            A.counts[(int64_t)e * A.blocks + blockIdx.x] = (uint8_t)__builtin_popcountll(mask[e]);
+            A.counts[(int64_t)e * A.blocks + block] = (uint8_t)__builtin_popcountll(mask[e]);
         return;
     }
     if (threadIdx.x < kWave) {   // one wavefront sums the experts' counts
@@ -226,14 +227,15 @@ __global__ __launch_bounds__(1024) void k_route_bases(RouteArgs A)
 __global__ __launch_bounds__(kRouteThreads) void k_route_places(RouteArgs A)
 {
     __shared__ uint64_t mask[kMostExperts];
-    const int64_t t0 = (int64_t)blockIdx.x * kBlockTokens;
+    const int64_t block = block_index(), t0 = block * kBlockTokens;
+    if (block >= A.blocks) return;
     const int tokens = (int)(A.tokens - t0 < kBlockTokens ? A.tokens - t0 : kBlockTokens);
     for (int e = threadIdx.x; e < A.experts; e += kRouteThreads) mask[e] = 0;
     __syncthreads();
     for (int i = threadIdx.x; i < tokens * A.top_k; i += kRouteThreads)
         atomicOr(reinterpret_cast<unsigned long long*>(&mask[A.chosen[t0 * A.top_k + i]]), 1ull << (i / A.top_k));
     __syncthreads();
-    place_block(A, mask, A.bases + blockIdx.x, A.blocks, t0, tokens);
+    place_block(A, mask, A.bases + block, A.blocks, t0, tokens);
 }
 
 // dlogits of the chosen's softmax, w_j (g_j - sum w g), or of all's, [e = chosen_j] w_j g_j - p_e sum w g.  A wavefront a
@@ -245,7 +247,7 @@ __global__ __launch_bounds__(256) void k_route_back(const float* weights, const 
 {
     __shared__ float spread[4][kMostExperts];
     const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
-    const int64_t t = (int64_t)blockIdx.x * 4 + wave;
+    const int64_t t = block_index() * 4 + wave;
     const bool real = t < tokens, picks = real && lane < top_k;
     const float w = picks ? weights[t * top_k + lane] : 0.0f;
     const float g = picks ? gout[t * top_k + lane] : 0.0f;
@@ -308,7 +310,7 @@ template <int DT>
 __device__ __forceinline__ bool place_of(const ShuffleArgs& A, int vectors, Place& p)
 {
     constexpr int64_t a_load = kWave * kLane<DT>;
-    p.t = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    p.t = block_index() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     p.c0 = (int64_t)blockIdx.y * vectors * a_load + (threadIdx.x & 63) * kLane<DT>;
     p.c1 = ((int64_t)blockIdx.y + 1) * vectors * a_load;
     p.c1 = p.c1 < A.cols ? p.c1 : A.cols;
@@ -380,7 +382,7 @@ __global__ __launch_bounds__(256) void k_combine_back(ShuffleArgs A)
 {
     constexpr int K = kLane<DT>, U = 4;
     const int lane = threadIdx.x & 63;
-    const int64_t a = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int64_t a = block_index() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if (a >= A.tokens * A.top_k) return;
     const int64_t t = a / A.top_k, r = A.position[a];
     float dot = 0.0f;
@@ -437,7 +439,7 @@ static void launch_route(const RouteArgs& A)
     // 16 lanes a token while its choices fit them and its logits their registers: four tokens share a wavefront
 #define ABH_ROUTE(G, NV)                                                                                        \
     if (A.experts <= G * NV && A.top_k <= G) {                                                                  \
-        hipLaunchKernelGGL((k_route<DT, G, NV>), dim3(A.blocks), dim3(kRouteThreads), 0, t_stream, A);           \
+        hipLaunchKernelGGL((k_route<DT, G, NV>), block_grid(A.blocks), dim3(kRouteThreads), 0, t_stream, A);     \
         return;                                                                                                 \
     }
     ABH_ROUTE(16, 1) ABH_ROUTE(16, 2) ABH_ROUTE(16, 4) ABH_ROUTE(16, 8) ABH_ROUTE(16, 16) ABH_ROUTE(64, 16)
@@ -466,7 +468,7 @@ constexpr int kDispatchVectors = 1 << 20, kCombineVectors = 8;
 static dim3 shuffle_grid(const ShuffleArgs& A, int32_t dtype, int vectors)
 {
     const int64_t a_wave = (int64_t)vectors * kWave * (dtype == ADAMBRIDGE_DT_BF16 ? kLane<DT_BF16> : kLane<DT_F32>);
-    return dim3((unsigned)((A.tokens + 3) / 4), (unsigned)((A.cols + a_wave - 1) / a_wave));
+    return block_grid((A.tokens + 3) / 4, (A.cols + a_wave - 1) / a_wave);
 }
 
 }  // namespace abh
@@ -498,7 +500,7 @@ ADAMBRIDGE_API int adambridge_route(const void* logits, int32_t dtype, int64_t t
     else launch_route<DT_F32>(A);
     if (blocks > 1) {
         hipLaunchKernelGGL(k_route_bases, dim3((unsigned)experts), dim3(1024), 0, t_stream, A);
-        hipLaunchKernelGGL(k_route_places, dim3((unsigned)blocks), dim3(kRouteThreads), 0, t_stream, A);
+        hipLaunchKernelGGL(k_route_places, block_grid(blocks), dim3(kRouteThreads), 0, t_stream, A);
     }
     return done("hipLaunchKernelGGL (route)");
 }
@@ -510,7 +512,7 @@ ADAMBRIDGE_API int adambridge_route_backward(const float* weights, const int32_t
     if (route_sizes(tokens, experts, top_k)) return ADAMBRIDGE_EBADN;
     if (!route_type_ok(dtype)) return ADAMBRIDGE_EMVDTYPE;
     if (!weights || !chosen || !gout || !grad || (!normalize && !logits)) return ADAMBRIDGE_ENULL;
-    const dim3 grid((unsigned)((tokens + 3) / 4));
+    const dim3 grid = block_grid((tokens + 3) / 4);
     if (dtype == ADAMBRIDGE_DT_BF16)
         hipLaunchKernelGGL((k_route_back<DT_BF16>), grid, dim3(256), 0, t_stream, weights, chosen, gout, logits, tokens,
                            (int32_t)experts, (int32_t)top_k, normalize, grad);
@@ -550,7 +552,7 @@ ADAMBRIDGE_API int adambridge_combine_backward(const void* gout, const void* row
     if (dweights && !rows) return ADAMBRIDGE_ENULL;
     if (!drows && !dweights) return 0;
     const ShuffleArgs A{rows, gout, weights, position, drows, dweights, tokens, cols, (int32_t)top_k};
-    const dim3 grid((unsigned)((tokens * top_k + 3) / 4));
+    const dim3 grid = block_grid((tokens * top_k + 3) / 4);
     if (dtype == ADAMBRIDGE_DT_BF16) hipLaunchKernelGGL((k_combine_back<DT_BF16>), grid, dim3(256), 0, t_stream, A);
     else hipLaunchKernelGGL((k_combine_back<DT_F32>), grid, dim3(256), 0, t_stream, A);
     return done("hipLaunchKernelGGL (combine's gradient)");

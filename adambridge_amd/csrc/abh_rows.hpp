@@ -266,6 +266,17 @@ __device__ __forceinline__ void block_sum2(float& a, float& b, float* part, int 
     }
 }
 
+// A launch has fewer than 2^32 lanes along x: workgroups from kGridX on (a multiple of the XCDs) go along z, where the last of
+// them may be more than there is work for.
+constexpr int64_t kGridX = 1 << 21;   // of 1024 lanes at most
+
+__device__ __forceinline__ int64_t block_index() { return (int64_t)blockIdx.z * kGridX + blockIdx.x; }
+
+inline dim3 block_grid(int64_t blocks, int64_t y = 1)
+{
+    return blocks <= kGridX ? dim3((unsigned)blocks, (unsigned)y) : dim3((unsigned)kGridX, (unsigned)y, (unsigned)((blocks + kGridX - 1) / kGridX));
+}
+
 // Keeps a value in its register as it is: what is computed from it again later is computed again, not kept.
 __device__ __forceinline__ void hold(raw16& w) { asm volatile("" : "+v"(w)); }
 
