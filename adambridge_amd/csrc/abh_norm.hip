@@ -311,10 +311,11 @@ __global__ __launch_bounds__(256) void k_norm_columns(NormArgs A)
         }
 }
 
-// The P partial sums of 64 columns a workgroup: L lanes of 4 columns each take every L-th, then their sums in order.
-template <int WT, int L>
-__global__ __launch_bounds__(16 * L) void k_norm_sums(NormArgs A, int32_t parts)
+// The P partial sums of 64 columns a workgroup: 64 lanes of 4 columns each take every 64th, then their sums in order.
+template <int WT>
+__global__ __launch_bounds__(1024) void k_norm_sums(NormArgs A, int32_t parts)
 {
+    constexpr int L = 64;
     __shared__ float sums[L][64 + 4];
     const int col = (threadIdx.x & 15) * 4, at_row = threadIdx.x >> 4;
     const int64_t c0 = (int64_t)blockIdx.x * 64;   // of 2 cols: dw's, then db's
@@ -331,21 +332,19 @@ __global__ __launch_bounds__(16 * L) void k_norm_sums(NormArgs A, int32_t parts)
 #pragma unroll
     for (int k = 0; k < 4; ++k) sums[at_row][col + k] = s[k];
     __syncthreads();
-    if constexpr (L > 16) {   // sixteen at a time first
-        float some = 0.0f;
-        const int g = threadIdx.x >> 6, cc = threadIdx.x & 63;
-        if (g < L / 16)
+    float some = 0.0f;   // sixteen at a time first
+    const int g = threadIdx.x >> 6, cc = threadIdx.x & 63;
+    if (g < L / 16)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) some += sums[16 * g + i][cc];
-        __syncthreads();
-        if (g < L / 16) sums[g][cc] = some;
-        __syncthreads();
-    }
+        for (int i = 0; i < 16; ++i) some += sums[16 * g + i][cc];
+    __syncthreads();
+    if (g < L / 16) sums[g][cc] = some;
+    __syncthreads();
     const int64_t c = c0 + threadIdx.x;
     if (threadIdx.x < 64 && c < 2 * A.cols) {
         float all = 0.0f;
 #pragma unroll
-        for (int i = 0; i < (L > 16 ? L / 16 : 16); ++i) all += sums[i][threadIdx.x];
+        for (int i = 0; i < L / 16; ++i) all += sums[i][threadIdx.x];
         void* out = c < A.cols ? A.dw : A.db;
         if (out) put<WT>(out, c < A.cols ? c : c - A.cols, all);
     }
@@ -360,7 +359,11 @@ struct Shape {
     int lanes, values, group;
 };
 
-// Few rows are spread over more lanes: what counts then is how long one row takes.
+// A row of up to 1024 columns is a part of a wavefront's or a wavefront's, a wider one a workgroup's.  Measured on MI355X in BF16,
+// us, beside one of fewer lanes with more values: 4096 columns, 256 lanes or 64: 64 rows 3.8 / 6.7, 2048 rows 8.5 / 10.5, 65536
+// rows 187 / 187; 2048 columns, 256 or 64: 512 rows 3.7 / 4.7, 1024 rows 4.6 / 5.0, 2048 rows 6.0 / 5.6, 65536 rows 115 / 92; 8192
+// columns, 512 or 256: 64 rows 4.2 / 4.9, 2048 rows 14.3 / 14.7, 16384 rows 99 / 96; 16384 columns, 1024 or 512: 64 rows 5.0 /
+// 5.6, 1024 rows 15.0 / 14.6, 8192 rows 106 / 100.
 static Shape norm_shape(int64_t rows, int64_t cols)
 {
     if (cols <= 64) return {8, 8, 256};
@@ -368,21 +371,16 @@ static Shape norm_shape(int64_t rows, int64_t cols)
     if (cols <= 256) return {32, 8, 256};
     if (cols <= 512) return {64, 8, 256};
     if (cols <= 1024) return {64, 16, 256};
-    if (rows < 1024) {
-        if (cols <= 2048) return {256, 8, 256};
-        if (cols <= 4096) return {256, 16, 256};
-        if (cols <= 8192) return {512, 16, 512};
-        if (cols <= 16384) return {1024, 16, 1024};
-        return {0, 0, 0};
-    }
-    if (cols <= 2048) return {64, 32, 256};
-    if (cols <= 4096) return {64, 64, 256};
-    if (cols <= 8192) return {256, 32, 256};
-    if (cols <= 16384) return {512, 32, 512};
+    const bool few = rows < 2048;
+    if (cols <= 2048) return few ? Shape{256, 8, 256} : Shape{64, 32, 256};
+    if (cols <= 4096) return {256, 16, 256};
+    if (cols <= 8192) return few ? Shape{512, 16, 512} : Shape{256, 32, 256};
+    if (cols <= 16384) return few ? Shape{1024, 16, 1024} : Shape{512, 32, 512};
     return {0, 0, 0};
 }
 
-// Backward a lane holds five values a column and the next row's two: fewer columns a lane.
+// Backward a lane holds five values a column and the next row's two: fewer columns a lane (2048 columns, 256 lanes or 64 with
+// four times the values: 512 rows 8.0 / 18.6 us, 65536 rows 145 / 217).
 static Shape norm_back_shape(int64_t cols)
 {
     if (cols <= 64) return {8, 8, 512};
@@ -398,12 +396,13 @@ static Shape norm_back_shape(int64_t cols)
 }
 
 // Workgroups of the backward pass, each with its partial sums: one a CU, of two turns at least (65536 x 4096 BF16: 287 us; 512
-// workgroups 294, 768 325 and 1024 350, as the partial sums grow and more rows compete).
+// workgroups 294, 768 325 and 1024 350, as the partial sums grow and more rows compete).  Of the long form 1024 in all, each of
+// 2048 columns or 1024, for the same reason (2048 x 40000 BF16: 199 us; 512 of them 231, 2048 203, 256 a strip of columns 239).
 static int norm_parts(int64_t rows, int64_t cols)
 {
     const Shape s = norm_back_shape(cols);
-    const int64_t at_a_time = s.lanes ? s.group / s.lanes : 1;
-    return (int)std::max<int64_t>(1, std::min<int64_t>(256, (rows + at_a_time * 2 - 1) / (at_a_time * 2)));
+    const int64_t at_a_time = s.lanes ? s.group / s.lanes : 1, most = s.lanes ? 256 : std::min<int64_t>(256, 1024 / ((cols + 2047) / 2048));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(most, (rows + at_a_time * 2 - 1) / (at_a_time * 2)));
 }
 
 template <int DT, int WT>
@@ -417,7 +416,7 @@ static void launch_norm(const NormArgs& A, bool back, int parts)
         hipLaunchKernelGGL((k_norm<DT, WT, G, N / K>), block_grid((A.rows + R - 1) / R), dim3(kNormThreads<G>), 0, t_stream, A); \
         return;                                                                                                         \
     }
-    ABH_NORM(8, 8) ABH_NORM(16, 8) ABH_NORM(32, 8) ABH_NORM(64, 8) ABH_NORM(64, 16) ABH_NORM(64, 32) ABH_NORM(64, 64) ABH_NORM(256, 8) ABH_NORM(256, 16) ABH_NORM(256, 32)
+    ABH_NORM(8, 8) ABH_NORM(16, 8) ABH_NORM(32, 8) ABH_NORM(64, 8) ABH_NORM(64, 16) ABH_NORM(64, 32) ABH_NORM(256, 8) ABH_NORM(256, 16) ABH_NORM(256, 32)
     ABH_NORM(512, 16) ABH_NORM(512, 32) ABH_NORM(1024, 16)
 #undef ABH_NORM
 #define ABH_NORM_BACK(G, N, T)                                                                                          \
@@ -492,11 +491,8 @@ ADAMBRIDGE_API int adambridge_layer_norm_backward(const void* gout, const void* 
     norm_by_type(A, dtype, w_dtype, true, parts);
     if (sums && (parts > 1 || !norm_back_shape(cols).lanes)) {
         const dim3 grid((unsigned)((2 * cols + 63) / 64));
-        const bool bf = w_dtype == ADAMBRIDGE_DT_BF16, few = parts <= 64;
-        if (bf && few) hipLaunchKernelGGL((k_norm_sums<DT_BF16, 16>), grid, dim3(256), 0, t_stream, A, parts);
-        else if (bf) hipLaunchKernelGGL((k_norm_sums<DT_BF16, 64>), grid, dim3(1024), 0, t_stream, A, parts);
-        else if (few) hipLaunchKernelGGL((k_norm_sums<DT_F32, 16>), grid, dim3(256), 0, t_stream, A, parts);
-        else hipLaunchKernelGGL((k_norm_sums<DT_F32, 64>), grid, dim3(1024), 0, t_stream, A, parts);
+                if (w_dtype == ADAMBRIDGE_DT_BF16) hipLaunchKernelGGL((k_norm_sums<DT_BF16>), grid, dim3(1024), 0, t_stream, A, parts);
+        else hipLaunchKernelGGL((k_norm_sums<DT_F32>), grid, dim3(1024), 0, t_stream, A, parts);
     }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : hip_fail(e, "hipLaunchKernelGGL (layer norm's gradient)");
