@@ -550,7 +550,8 @@ ADAMBRIDGE_API int adambridge_combine_backward(const void* gout, const void* row
  * 2^22).  y = x weight[e]^T (x: rows x k, y: rows x n); dx = gout weight[e] (gout: rows x n); dw[e] = gout^T x over e's
  * rows, zeros where there are none.  work: adambridge_expert_mm_work bytes of the product (ADAMBRIDGE_EXPERTS_Y, _DX or
  * _DW), 16-byte aligned, NULL if 0.  Rows from the last end on give zeros.  Ends that break the rule give
- * unspecified values, and nothing outside the arrays is touched. */
+ * unspecified values, and nothing outside the arrays is touched.  A result of more than 2^30 tiles of 64 x 64 or larger is
+ * ADAMBRIDGE_EBADN. */
 #define ADAMBRIDGE_EXPERTS_Y 0
 #define ADAMBRIDGE_EXPERTS_DX 1
 #define ADAMBRIDGE_EXPERTS_DW 2
