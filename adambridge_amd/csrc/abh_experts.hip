@@ -186,8 +186,10 @@ __device__ __forceinline__ bool find_weight_tile(const ExpertArgs& A, Tile& t)
     if (local >= an) return false;
     t.e = turn / A.splits;
     t.split = turn - t.e * A.splits;
-    const int g = local / (kGroupTiles * A.tiles_j), first = g * kGroupTiles;
-    const int wide = A.tiles_i - first < kGroupTiles ? A.tiles_i - first : kGroupTiles;
+    // an XCD's tiles near a square: 6 of them as 2 x 3 read 1.56 GB in all, as 6 x 1 1.94 (64 experts 1536 x 2048: 424 us, 437)
+    const int high = per < 4 ? 1 : per < 8 ? 2 : per < 32 ? 4 : kGroupTiles;
+    const int g = local / (high * A.tiles_j), first = g * high;
+    const int wide = A.tiles_i - first < high ? A.tiles_i - first : high;
     const int r = local - first * A.tiles_j;
     t.ti = scalar(first + r % wide);
     t.tj = scalar(r / wide);
@@ -534,11 +536,12 @@ __global__ __launch_bounds__(kFewWaves * kWave) void k_experts_few(ExpertArgs A)
 // Rows that are not whole 16-byte pieces go through the registers (StagedFeed): 8192 rows of 8 experts 2047 x 1999, a training
 // pass 439 us, 2048 x 2000 308.
 //
-// Measured on MI355X, one expert, 8192^3: y 873 us (1259 TFLOP/s), dx 827 (1329), dW 821 (1339); the matrix cores are busy
-// 73% of the cycles, at 1.6 GHz of 2.4: power is the bound, and what takes stalls away alone gives the clock back (workgroups that go
-// on to the next tile while the last one's results are stored, those stores beside the next loads: 0-3% slower). (The BLAS library's products: 1501, 1228, 1152.)  Slower: 64 terms a step with two buffers 891 (y),
-// wavefronts of 128 x 128 (one a SIMD) 890, tiles of 128 x 256 with two workgroups a CU 1010, three buffers 989; five
-// buffers change nothing.
+// Measured on MI355X, one expert, 8192^3: y 873 us (1259 TFLOP/s), dx 827 (1329), dW 821 (1339); the BLAS library's products
+// 1501, 1228, 1152 TFLOP/s.  The matrix cores are busy 73% of the cycles, at 1.6 GHz of 2.4 (y of zeros: 750 us): power is the bound, and
+// what takes stalls away alone gives the clock back (workgroups that go on to the next tile while the last one's
+// results are stored, those stores beside the next loads: 0-3% slower).  Slower too: 64 terms a step with two buffers 891 (y),
+// wavefronts of 128 x 128 (one a SIMD) 890, tiles of 128 x 256 with two workgroups a CU 1010, three buffers 989, a long operand's
+// steps loaded two at a time, as whole lines of 128 bytes, 1-6%; five buffers change nothing.
 //
 // A long operand's tile is its rows by 64 bytes, a row's 16-byte pieces exchanged by the row, so that the reads of
 // neighbouring rows meet different banks.  One across its rows is 32 terms by its rows, read transposed
