@@ -47,8 +47,8 @@ struct ExpertArgs {
     int32_t ni, nj;     // MODE_DW: C's rows (n); columns of C
     int32_t len;        // the sum's length, but for MODE_DW
     int32_t tiles_i, tiles_j;
-    int32_t splits;     // MODE_DW: parts of an expert's rows, each with its own sums ...
-    float* part;        // ... splits x experts x ni x nj
+    int32_t splits;     // parts of a sum (MODE_DW: of an expert's rows), each with a result of its own ...
+    float* part;        // ... splits x the result
 };
 
 // Rows lo .. hi of expert e (e = experts: the rows that are no expert's).  Ends outside 0 .. rows, or one below the
@@ -125,11 +125,13 @@ __device__ __forceinline__ bool locate_row_tile(const ExpertArgs& A, int idx, Ti
 template <int BM>
 __device__ __forceinline__ bool find_row_tile(const ExpertArgs& A, Tile& t)
 {
-    const int tiles = count_row_tiles<BM>(A), per = (tiles + kXcd - 1) / kXcd;
-    const int block = (int)block_index(), slot = block / kXcd, idx = block % kXcd * per + slot;
-    t.split = t.rest = 0;
-    t.splits = 1;
-    return slot < per && idx < tiles && locate_row_tile<BM>(A, idx, t);
+    const int items = count_row_tiles<BM>(A) * A.splits, per = (items + kXcd - 1) / kXcd;
+    const int block = (int)block_index(), slot = block / kXcd, item = block % kXcd * per + slot;
+    const int idx = scalar(item / A.splits);
+    t.split = scalar(item - idx * A.splits);
+    t.splits = A.splits;
+    t.rest = 0;
+    return slot < per && item < items && locate_row_tile<BM>(A, idx, t);
 }
 
 // The same where a CU has one workgroup: whole rounds of kCus tiles, spread over the XCDs, and the rest of them over the XCDs
@@ -206,10 +208,12 @@ __device__ __forceinline__ bool find_weight_tile(const ExpertArgs& A, Tile& t)
     return true;
 }
 
-// Where this part's sums go: FP32, rows of nj.
+// Where this part's sums go: FP32, rows of nj, those of the tile's expert.
+template <int MODE>
 __device__ __forceinline__ float* part_of(const ExpertArgs& A, const Tile& t)
 {
-    return A.part + ((int64_t)t.split * A.experts + t.e) * A.ni * A.nj;
+    const int64_t row = MODE == MODE_DW ? ((int64_t)t.split * A.experts + t.e) * A.ni : (int64_t)t.split * A.rows + t.lo;
+    return A.part + row * A.nj;
 }
 
 // c = the parts' sums, in order, rounded once.
@@ -792,7 +796,7 @@ __device__ __forceinline__ Cut cut_of(const ExpertArgs& A, const Tile& t)
     u.limit_j = A.nj - u.j0;
     u.len = MODE == MODE_DW ? t.hi - t.lo : t.e < A.experts ? A.len : 0;
     u.k0 = 0;
-    if (MODE != MODE_DW && C::ROUNDS && t.splits > 1 && u.len > 0) {
+    if (MODE != MODE_DW && t.splits > 1 && u.len > 0) {
         const int all = (u.len + C::BK - 1) / C::BK;
         u.k0 = scalar(all * t.split / t.splits * C::BK);
         const int end = scalar(all * (t.split + 1) / t.splits * C::BK);
@@ -807,13 +811,13 @@ template <int MODE, class C, bool EVEN>
 __device__ __forceinline__ void store_tile(const ExpertArgs& A, const Cut& u, const mm_f32x16 (&acc)[C::NI][C::NJ], int wi, int wj)
 {
     const int lane = threadIdx.x & 63;
-    if constexpr (MODE == MODE_DW) {
+    if constexpr (MODE == MODE_DW || !C::ROUNDS) {
         if (A.splits > 1) {   // a part of the sums
-            float* to = part_of(A, u.t) + u.j0;
+            float* to = part_of<MODE>(A, u.t) + u.j0;
 #pragma unroll
             for (int i = 0; i < C::NI; ++i) {
                 const int row = u.i0 + wi + 32 * i + (lane & 31);
-                if (row >= A.ni) continue;
+                if (row >= u.i0 + u.limit_i) continue;
 #pragma unroll
                 for (int j = 0; j < C::NJ; ++j)
 #pragma unroll
@@ -1172,7 +1176,7 @@ __global__ __launch_bounds__(256, 2) void k_experts_f32(ExpertArgs A)
     gather();
     float* out;
     if constexpr (MODE == MODE_DW) {
-        out = (A.splits > 1 ? part_of(A, t) : static_cast<float*>(A.c) + (int64_t)t.e * A.ni * A.nj) + (int64_t)i0 * A.nj + j0;
+        out = (A.splits > 1 ? part_of<MODE>(A, t) : static_cast<float*>(A.c) + (int64_t)t.e * A.ni * A.nj) + (int64_t)i0 * A.nj + j0;
     } else {
         out = static_cast<float*>(A.c) + (int64_t)(t.lo + i0) * A.nj + j0;
     }
@@ -1199,12 +1203,15 @@ struct Plan {
     enum { FEW, ANY, LARGE, SMALL, F32_128, F32_64 } kernel;
     int tile, splits;
     bool rest;   // whether the tiles after the last whole round may be cut
+    // bytes of scratch, of a result of so many values
     int64_t work(int64_t values) const { return rest ? (int64_t)kCus * LargeTile::BM * LargeTile::BN * 4 : splits > 1 ? splits * values * 4 : 0; }
 };
 
 // Measured on MI355X, us, both sides of each line (experts of 1536 x 2048 unless said):
-//   few rows: y of 512 rows, 64 experts 85 streamed / 106 on tiles, 1024 rows 111 / 108; 64 rows of one expert 4096 x 4096 23 / 33,
-//     128 rows 42 / 42;
+//   few rows: y of 512 rows, 64 experts 85 streamed / 106 on tiles, 1024 rows 111 / 108; 16 rows of one expert 4096 x 4096 14.0 /
+//     15.9, 24 rows 17.1 / 16.0, 64 rows 25.9 / 17.3; 64 rows of one expert 1024 x 1024 8.8 / 10.9, 2048 x 8192 43 / 19;
+//   cut sums of small tiles: one expert 4096 x 4096, y of 128 rows 35.5 whole / 18.2 cut, 512 rows 35.8 / 30.5; 600 rows of one
+//     512 x 1024 11.5 / 12.1; 300 rows of 2 experts 8192 x 2048 y 21.5 / 30 in two (192 tiles, so whole), dx 65 / 33;
 //   large or small BF16 tiles: dx of 1024 rows, 8 experts 8192 x 2048 (64 large ones) 155 / 102, 2048 (104) 175 / 168, 4096 (160)
 //     188 / 229; dW of 16 experts 512 x 512 (64) 98 / 42; y of 4096 rows, 64 experts 122 / 102, 8192 (128 an expert) 124 / 126, 12288
 //     136 / 147;
@@ -1222,8 +1229,8 @@ static Plan plan_experts(int mode, int32_t dtype, int64_t rows, int64_t experts,
         const int64_t j = (nj + t - 1) / t;
         return mode == MODE_DW ? experts * ((ni + t - 1) / t) * j : (rows / t + (used + 1) / 2) * j;
     };
-    // few rows an expert: the weights' bytes are all there is; or more, read at once, that would make too few tiles
-    if (mode == MODE_Y && (rows <= std::max<int64_t>(64, 8 * experts) || (rows <= 64 * experts && tiles(64) < 256)))
+    // few rows an expert: the weights' bytes are all there is; or more, read at once, of too few tiles whose sums are not cut
+    if (mode == MODE_Y && (rows <= std::max<int64_t>(bf ? 16 : 64, 8 * experts) || (rows <= 64 * experts && tiles(64) < 256 && (!bf || k <= 1024))))
         return {Plan::FEW, 0, 1, false};
     if (any) return {Plan::ANY, kTile, 1, false};
     Plan p = bf ? Plan{Plan::LARGE, LargeTile::BM, 1, false} : Plan{Plan::F32_128, 128, 1, false};
@@ -1234,9 +1241,17 @@ static Plan plan_experts(int mode, int32_t dtype, int64_t rows, int64_t experts,
         const int64_t t = std::max<int64_t>(1, tiles(p.tile));
         p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / t, rows / experts / 256));
     }
+    // few tiles with long sums: parts of 16 steps or more, about a workgroup a CU (the tiles are fewer than reckoned with)
+    if (mode != MODE_DW && p.kernel == Plan::SMALL)
+        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(320 / std::max<int64_t>(1, tiles(p.tile)), (mode == MODE_Y ? k : n) / (16 * SmallTile::BK)));
     // a long sum, and so few rounds that a cut rest may count
     if (mode != MODE_DW && p.kernel == Plan::LARGE) p.rest = (mode == MODE_Y ? k : n) >= 128 * LargeTile::BK && tiles(LargeTile::BM) <= 4 * kCus;
     return p;
+}
+
+static int64_t result_values(int mode, int64_t rows, int64_t experts, int64_t n, int64_t k)
+{
+    return mode == MODE_DW ? experts * n * k : rows * (mode == MODE_Y ? n : k);
 }
 
 template <int MODE>
@@ -1248,6 +1263,7 @@ static int experts_mm(const void* a, const void* b, const int32_t* ends, void* c
     if (dtype != ADAMBRIDGE_DT_F32 && dtype != ADAMBRIDGE_DT_BF16) return ADAMBRIDGE_EMVDTYPE;
     if (MODE != MODE_DW && rows == 0) return 0;
     const Plan p = plan_experts(MODE, dtype, rows, experts, n, k);
+    const int64_t values = result_values(MODE, rows, experts, n, k);
     if ((!a && rows) || (!b && rows) || !ends || !c || (p.work(1) && !work)) return ADAMBRIDGE_ENULL;
     if (p.work(1) && (uintptr_t)work % 16) return ADAMBRIDGE_EALIGN;
     const bool bf = dtype == ADAMBRIDGE_DT_BF16;
@@ -1278,7 +1294,7 @@ static int experts_mm(const void* a, const void* b, const int32_t* ends, void* c
         A.tiles_i = (A.ni + p.tile - 1) / p.tile;
         // every expert, and the rows that are no expert's, may have a partial tile
         const int64_t tiles = MODE == MODE_DW ? experts * p.splits * (((int64_t)A.tiles_i * A.tiles_j + kXcd - 1) / kXcd * kXcd)
-                                              : std::min(rows, rows / p.tile + experts + 1) * A.tiles_j;
+                                              : std::min(rows, rows / p.tile + experts + 1) * A.tiles_j * p.splits;
         if (tiles > (int64_t)1 << 30) return ADAMBRIDGE_EBADN;   // tiles are counted in 32 bits
         const dim3 grid = block_grid((tiles + kXcd - 1) / kXcd * kXcd + (p.rest ? kCus : 0));
         if (p.kernel == Plan::LARGE && even)
@@ -1297,7 +1313,6 @@ static int experts_mm(const void* a, const void* b, const int32_t* ends, void* c
     if (p.rest)
         hipLaunchKernelGGL((k_experts_rest<LargeTile>), dim3(kMostRest * LargeTile::BM / 16), dim3(256), 0, t_stream, A);
     if (p.splits > 1) {
-        const int64_t values = experts * n * k;
         const dim3 grid((unsigned)((values + 1023) / 1024));
         if (bf) hipLaunchKernelGGL((k_experts_sum<DT_BF16>), grid, dim3(256), 0, t_stream, A.part, values, p.splits, c);
         else hipLaunchKernelGGL((k_experts_sum<DT_F32>), grid, dim3(256), 0, t_stream, A.part, values, p.splits, c);
@@ -1318,7 +1333,7 @@ ADAMBRIDGE_API int64_t adambridge_expert_mm_work(int32_t product, int32_t dtype,
         n > kExpertSize || k < 1 || k > kExpertSize)
         return ADAMBRIDGE_EBADN;
     if (dtype != ADAMBRIDGE_DT_F32 && dtype != ADAMBRIDGE_DT_BF16) return ADAMBRIDGE_EMVDTYPE;
-    return rows ? plan_experts(product, dtype, rows, experts, n, k).work(experts * n * k) : 0;
+    return rows ? plan_experts(product, dtype, rows, experts, n, k).work(result_values(product, rows, experts, n, k)) : 0;
 }
 
 ADAMBRIDGE_API int adambridge_expert_mm(const void* x, const void* weight, const int32_t* ends, void* y, int32_t dtype,

@@ -233,6 +233,13 @@ def test_expert_mm_of_many_rows_matches_the_definition(counts, extra, n, k, dtyp
     _check_mm(counts, extra, n, k, dtype, seed=n + k)
 
 
+# few tiles, whose sums are cut into parts (of y over k, of dx over n), the last one short; rows that are no expert's
+@pytest.mark.parametrize("counts,extra,n,k", [([128], 0, 1024, 4096), ([100, 0, 90], 5, 1000, 2056), ([200], 3, 515, 2051),
+                                              ([40], 0, 1024, 8200), ([150], 0, 4096, 520), ([60, 70], 1, 2049, 129)])
+def test_expert_mm_of_few_tiles_matches_the_definition(counts, extra, n, k):
+    _check_mm(counts, extra, n, k, torch.bfloat16, seed=n + k)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_no_rows_at_all(dtype):
     x = torch.randn(0, 24, device="cuda").to(dtype).requires_grad_()
