@@ -123,11 +123,12 @@ bool wants_grad(std::initializer_list<const Tensor*> ts)
 }
 
 // Whether a backward pass may run the kernels: not one that is differentiated in turn or observed, nor one whose gradient
-// is a batch or holds no memory of its own.
+// is a batch, holds no memory of its own or carries a tangent (an operand after the operator may be a dual one; the
+// torch operations carry it on).
 bool plain_backward(const Tensor& g)
 {
     return !at::GradMode::is_enabled() && !observed() && g.layout() == at::kStrided && g.is_cuda() && g.has_storage() &&
-           !g._is_zerotensor() && !g.is_neg() && !g.key_set().has(c10::DispatchKey::Python);
+           !g._is_zerotensor() && !g.is_neg() && !g.key_set().has(c10::DispatchKey::Python) && !g._fw_grad(0).defined();
 }
 
 // A backward pass in torch operations, by the Python function of that name.

@@ -1,0 +1,61 @@
+"""Calls of the expert block's operators that are not the ordinary ones: what reaches a kernel, and what must not."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+import adambridge_amd as ab
+
+pytestmark = pytest.mark.gpu
+
+NAMES = ("layer_norm", "route", "route_all", "dispatch", "combine", "expert_mm")
+
+
+def _gen(seed):
+    return torch.Generator("cuda").manual_seed(seed)
+
+
+def _operator(name, dtype=torch.float32):
+    """The operator as a function of its differentiable operands, and those."""
+    gen = _gen(len(name))
+    leaf = lambda *shape: torch.randn(*shape, generator=gen, device="cuda").to(dtype).requires_grad_()
+    r = ab.route(torch.randn(24, 6, generator=gen, device="cuda"), 2)
+    if name == "layer_norm":
+        return ab.layer_norm, [leaf(24, 40), leaf(40), leaf(40)]
+    if name.startswith("route"):
+        return lambda x: ab.route(x, 3, normalize=name == "route").weights, [leaf(24, 16)]
+    if name == "dispatch":
+        return lambda x: ab.dispatch(x, r), [leaf(24, 40)]
+    if name == "combine":
+        return lambda y, w: ab.combine(y, r._replace(weights=w)), [leaf(48, 40), r.weights.detach().clone().requires_grad_()]
+    return lambda x, w: ab.expert_mm(x, w, r.ends), [leaf(48, 40), leaf(6, 24, 40)]
+
+
+def _gradients(name, dtype=torch.float32, seed=1):
+    fn, leaves = _operator(name, dtype)
+    out = fn(*leaves)
+    g = torch.randn(out.shape, generator=_gen(seed), device="cuda").to(out.dtype)
+    return torch.autograd.grad(out, leaves, g)
+
+
+def _near(got, want):
+    return torch.allclose(got, want, rtol=1e-4, atol=1e-5 * (1.0 + want.abs().max().item()))
+
+
+# ------------------------------------------------------------------------------- tangents
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_gradient_s_tangent_is_carried_on(name):
+    """Forward mode over a backward pass, the dual operand behind the operator: its gradient is linear in the one that
+    arrives, so the tangent of its gradient is the gradient of the tangent."""
+    fn, leaves = _operator(name)
+    out = fn(*leaves)
+    scale, tangent = (torch.randn(out.shape, generator=_gen(s), device="cuda") for s in (5, 6))
+    with forward_ad.dual_level():
+        grads = torch.autograd.grad((fn(*leaves) * forward_ad.make_dual(scale, tangent)).sum(), leaves)
+        got = [forward_ad.unpack_dual(t) for t in grads]
+        got = [(t.primal.clone(), None if t.tangent is None else t.tangent.clone()) for t in got]
+    want = zip(torch.autograd.grad(out, leaves, scale, retain_graph=True), torch.autograd.grad(out, leaves, tangent))
+    for (primal, moved), (want_primal, want_moved) in zip(got, want):
+        assert moved is not None
+        assert _near(primal, want_primal) and _near(moved, want_moved)
