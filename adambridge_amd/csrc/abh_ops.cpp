@@ -131,6 +131,23 @@ bool plain_backward(const Tensor& g)
            !g._is_zerotensor() && !g.is_neg() && !g.key_set().has(c10::DispatchKey::Python) && !g._fw_grad(0).defined();
 }
 
+// Whether a saved tensor is one that the kernels take, once it is contiguous: of this type, in memory of its own beside the
+// gradient.  A hook on saved tensors may give back any other.  One of other sizes is an error, also where torch operations
+// follow: they would index it on the device.  (Sizes without numbers, of a trace, are left to those.)
+bool restored(const Tensor& t, const Tensor& g, at::ScalarType type, at::IntArrayRef sizes)
+{
+    TORCH_CHECK(t.defined() && (t.unsafeGetTensorImpl()->has_symbolic_sizes_strides() || t.sizes() == sizes),
+                "a saved tensor came back as another: expected sizes ", sizes, ", got ", t.defined() ? t.sizes() : at::IntArrayRef());
+    return t.layout() == at::kStrided && t.device() == g.device() && t.scalar_type() == type && t.has_storage() && !t._is_zerotensor() &&
+           !t.is_neg() && !t.key_set().has(c10::DispatchKey::Python) && !t._fw_grad(0).defined();
+}
+
+// A gradient's sizes (none has no dimension); nothing where they are a trace's.
+at::IntArrayRef sizes_of(const Tensor& g)
+{
+    return g.unsafeGetTensorImpl()->has_symbolic_sizes_strides() ? at::IntArrayRef() : g.sizes();
+}
+
 // A backward pass in torch operations, by the Python function of that name.
 template <class Arguments>
 tensor_list in_torch(const char* name, const Arguments& arguments, size_t n)
@@ -182,26 +199,29 @@ struct LayerNorm : Function<LayerNorm> {
         // only given tensors count among a function's edges
         const bool want_x = ctx->needs_input_grad(0), want_w = (given & 1) && ctx->needs_input_grad(1),
                    want_b = (given & 2) && ctx->needs_input_grad(1 + (given & 1));
-        if (!plain_backward(grads[0]))
+        const at::IntArrayRef sizes = sizes_of(grads[0]);
+        const int64_t cols = sizes.empty() ? 0 : sizes.back(), rows = cols ? grads[0].numel() / cols : 0;
+        const bool whole = cols && restored(x, grads[0], grads[0].scalar_type(), sizes) & restored(stats, grads[0], at::kFloat, {rows, 2}) &
+                                       (!w.defined() || restored(w, grads[0], wt, {cols}));
+        if (!whole || !plain_backward(grads[0]))
             return in_torch("layer_norm", [&] {
                 return pybind11::make_tuple(grads[0], x, or_none(w), ctx->saved_data["eps"].toDouble(), want_x, want_w, want_b,
                                             pybind11::reinterpret_borrow<pybind11::object>((PyObject*)torch::getTHPDtype(wt)));
             }, 4);
         const at::AutoDispatchBelowADInplaceOrView below;
-        const Tensor g = grads[0].contiguous();
-        const int64_t cols = x.size(-1), rows = x.numel() / cols;
+        const Tensor g = grads[0].contiguous(), xc = x.contiguous(), wc = w.defined() ? w.contiguous() : w, sc = stats.contiguous();
         tensor_list out(4);
-        if (want_x) out[0] = fresh(x.sizes(), x.scalar_type(), x);
-        if (want_w) out[1] = fresh({cols}, wt, x);
-        if (want_b) out[2] = fresh({cols}, wt, x);
+        if (want_x) out[0] = fresh(sizes, g.scalar_type(), g);
+        if (want_w) out[1] = fresh({cols}, wt, g);
+        if (want_b) out[2] = fresh({cols}, wt, g);
         Tensor work;
         if (want_w || want_b) {
-            const int64_t bytes = api.layer_norm_work(rows, cols, code(x.scalar_type()));
+            const int64_t bytes = api.layer_norm_work(rows, cols, code(g.scalar_type()));
             check(bytes, "adambridge_layer_norm_work");
-            work = scratch(bytes, x);
+            work = scratch(bytes, g);
         }
-        const On on(x);
-        check(api.layer_norm_backward(address(g), address(x), code(x.scalar_type()), address(w), code(wt), stats.const_data_ptr<float>(),
+        const On on(g);
+        check(api.layer_norm_backward(address(g), address(xc), code(g.scalar_type()), address(wc), code(wt), sc.const_data_ptr<float>(),
                                       rows, cols, place(out[0]), place(out[1]), place(out[2]), place(work)),
               "adambridge_layer_norm_backward");
         return out;
@@ -266,17 +286,20 @@ struct Route : Function<Route> {
         const int64_t of = ctx->saved_data["of"].toInt(), experts = of >> 16;
         const bool normalize = of & 1;
         const at::ScalarType type = (at::ScalarType)(of >> 8 & 255);
-        if (!plain_backward(grads[0]))
+        const at::IntArrayRef sizes = sizes_of(grads[0]);
+        const bool whole = !sizes.empty() && restored(weights, grads[0], at::kFloat, sizes) & restored(chosen, grads[0], at::kInt, sizes) &
+                                                 (normalize || restored(logits, grads[0], type, {sizes[0], experts}));
+        if (!whole || !plain_backward(grads[0]))
             return in_torch("route", [&] {
                 return pybind11::make_tuple(grads[0], weights, chosen, or_none(logits), experts, normalize,
                                             pybind11::reinterpret_borrow<pybind11::object>((PyObject*)torch::getTHPDtype(type)));
             }, 3);
         const at::AutoDispatchBelowADInplaceOrView below;
-        const Tensor g = grads[0].contiguous();
-        const int64_t tokens = weights.size(0), top_k = weights.size(1);
-        out[0] = fresh({tokens, experts}, type, weights);
-        const On on(weights);
-        check(api.route_backward(weights.const_data_ptr<float>(), chosen.const_data_ptr<int32_t>(), g.const_data_ptr<float>(), address(logits),
+        const Tensor g = grads[0].contiguous(), w = weights.contiguous(), c = chosen.contiguous(), l = normalize ? Tensor() : logits.contiguous();
+        const int64_t tokens = sizes[0], top_k = sizes[1];
+        out[0] = fresh({tokens, experts}, type, g);
+        const On on(g);
+        check(api.route_backward(w.const_data_ptr<float>(), c.const_data_ptr<int32_t>(), g.const_data_ptr<float>(), address(l),
                                  code(type), tokens, experts, top_k, normalize, place(out[0])), "adambridge_route_backward");
         return out;
     }
@@ -342,15 +365,19 @@ struct Dispatch : Function<Dispatch> {
     {
         const at::AutoDispatchBelowADInplaceOrView below;
         ctx->save_for_backward({position});
+        ctx->saved_data["top_k"] = position.size(1);
         return run_dispatch(x, position);
     }
     static tensor_list backward(AutogradContext* ctx, const tensor_list& grads)
     {
         const tensor_list saved = ctx->get_saved_variables();
-        if (!plain_backward(grads[0]))
+        const int64_t top_k = ctx->saved_data["top_k"].toInt();
+        const at::IntArrayRef sizes = sizes_of(grads[0]);
+        const bool whole = !sizes.empty() && restored(saved[0], grads[0], at::kInt, {sizes[0] / top_k, top_k});
+        if (!whole || !plain_backward(grads[0]))
             return in_torch("dispatch", [&] { return pybind11::make_tuple(grads[0], saved[0]); }, 2);
         const at::AutoDispatchBelowADInplaceOrView below;
-        return {run_combine(grads[0].contiguous(), Tensor(), saved[0]), Tensor()};
+        return {run_combine(grads[0].contiguous(), Tensor(), saved[0].contiguous()), Tensor()};
     }
 };
 
@@ -359,6 +386,7 @@ struct Combine : Function<Combine> {
     {
         const at::AutoDispatchBelowADInplaceOrView below;
         ctx->save_for_backward({weights.requires_grad() ? rows : Tensor(), weights, position});
+        ctx->saved_data["top_k"] = position.size(1);
         return run_combine(rows, weights, position);
     }
     static tensor_list backward(AutogradContext* ctx, const tensor_list& grads)
@@ -366,19 +394,22 @@ struct Combine : Function<Combine> {
         const tensor_list saved = ctx->get_saved_variables();
         const Tensor &rows = saved[0], &weights = saved[1], &position = saved[2];
         const bool want_rows = ctx->needs_input_grad(0), want_weights = ctx->needs_input_grad(1);
-        if (!plain_backward(grads[0]))
+        const at::IntArrayRef sizes = sizes_of(grads[0]);
+        const int64_t tokens = sizes.empty() ? 0 : sizes[0], cols = sizes.empty() ? 0 : sizes[1], top_k = ctx->saved_data["top_k"].toInt();
+        const bool whole = tokens && restored(weights, grads[0], at::kFloat, {tokens, top_k}) & restored(position, grads[0], at::kInt, {tokens, top_k}) &
+                                         (!want_weights || restored(rows, grads[0], grads[0].scalar_type(), {tokens * top_k, cols}));
+        if (!whole || !plain_backward(grads[0]))
             return in_torch("combine", [&] {
                 return pybind11::make_tuple(grads[0], or_none(rows), weights, position, want_rows, want_weights);
             }, 3);
         const at::AutoDispatchBelowADInplaceOrView below;
-        const Tensor g = grads[0].contiguous();
-        const int64_t tokens = position.size(0), top_k = position.size(1), cols = g.size(1);
+        const Tensor g = grads[0].contiguous(), r = want_weights ? rows.contiguous() : Tensor(), w = weights.contiguous(), p = position.contiguous();
         tensor_list out(3);
         if (want_rows) out[0] = fresh({tokens * top_k, cols}, g.scalar_type(), g);
         if (want_weights) out[1] = fresh({tokens, top_k}, at::kFloat, g);
         const On on(g);
-        check(api.combine_backward(address(g), address(rows), code(g.scalar_type()), weights.const_data_ptr<float>(),
-                                   position.const_data_ptr<int32_t>(), tokens, top_k, cols, place(out[0]),
+        check(api.combine_backward(address(g), address(r), code(g.scalar_type()), w.const_data_ptr<float>(),
+                                   p.const_data_ptr<int32_t>(), tokens, top_k, cols, place(out[0]),
                                    out[1].defined() ? out[1].mutable_data_ptr<float>() : nullptr), "adambridge_combine_backward");
         return out;
     }
@@ -433,6 +464,7 @@ struct ExpertMM : Function<ExpertMM> {
     {
         const at::AutoDispatchBelowADInplaceOrView below;
         ctx->save_for_backward({weight.requires_grad() ? x : Tensor(), weight, ends});
+        ctx->saved_data["of"] = (int64_t)(weight.size(0) | weight.size(2) << 16);
         return run_experts(ADAMBRIDGE_EXPERTS_Y, x, weight, ends, {x.size(0), weight.size(1)}, weight.size(1), weight.size(2));
     }
     static tensor_list backward(AutogradContext* ctx, const tensor_list& grads)
@@ -440,16 +472,21 @@ struct ExpertMM : Function<ExpertMM> {
         const tensor_list saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &weight = saved[1], &ends = saved[2];
         const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
-        if (!plain_backward(grads[0]))
+        const at::IntArrayRef sizes = sizes_of(grads[0]);
+        const int64_t of = ctx->saved_data["of"].toInt(), experts = of & 0xffff, k = of >> 16;
+        const int64_t rows = sizes.empty() ? 0 : sizes[0], n = sizes.empty() ? 0 : sizes[1];
+        const at::ScalarType type = grads[0].scalar_type();
+        const bool whole = n && restored(weight, grads[0], type, {experts, n, k}) & restored(ends, grads[0], at::kInt, {experts}) &
+                                    (!want_w || restored(x, grads[0], type, {rows, k}));
+        if (!whole || !plain_backward(grads[0]))
             return in_torch("expert_mm", [&] {
                 return pybind11::make_tuple(grads[0], or_none(x), weight, ends, want_x, want_w);
             }, 3);
         const at::AutoDispatchBelowADInplaceOrView below;
-        const Tensor g = grads[0].contiguous();
-        const int64_t n = weight.size(1), k = weight.size(2);
+        const Tensor g = grads[0].contiguous(), e = ends.contiguous();
         tensor_list out(3);
-        if (want_x) out[0] = run_experts(ADAMBRIDGE_EXPERTS_DX, g, weight, ends, {g.size(0), k}, n, k);
-        if (want_w) out[1] = run_experts(ADAMBRIDGE_EXPERTS_DW, g, x, ends, weight.sizes(), n, k);
+        if (want_x) out[0] = run_experts(ADAMBRIDGE_EXPERTS_DX, g, weight.contiguous(), e, {rows, k}, n, k);
+        if (want_w) out[1] = run_experts(ADAMBRIDGE_EXPERTS_DW, g, x.contiguous(), e, {experts, n, k}, n, k);
         return out;
     }
 };

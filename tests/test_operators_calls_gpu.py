@@ -59,3 +59,65 @@ def test_a_gradient_s_tangent_is_carried_on(name):
     for (primal, moved), (want_primal, want_moved) in zip(got, want):
         assert moved is not None
         assert _near(primal, want_primal) and _near(moved, want_moved)
+
+
+# ------------------------------------------------------------------------- saved tensors
+
+def _strided(t):
+    """The same values in memory of another order."""
+    if t.dim() == 1:
+        return torch.stack((t, t), 1)[:, 0]
+    return t.transpose(-1, -2).contiguous().transpose(-1, -2)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("name", NAMES)
+def test_saved_tensors_that_come_back_strided(name, dtype):
+    want = _gradients(name, dtype)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, _strided):
+        got = _gradients(name, dtype)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_saved_tensors_that_come_back_expanded():
+    """Equal rows given back as one row of memory, expanded."""
+    r = ab.route(torch.randn(24, 6, generator=_gen(0), device="cuda"), 2)
+
+    def rows(*shape):
+        return torch.randn(shape[1:], generator=_gen(1), device="cuda").expand(shape).contiguous().requires_grad_()
+
+    cases = [(ab.layer_norm, [rows(24, 40), rows(1, 40)[0].detach().requires_grad_()]),
+             (lambda y, w: ab.combine(y, r._replace(weights=w)), [rows(48, 40), rows(24, 2)]),
+             (lambda x, w: ab.expert_mm(x, w, r.ends), [rows(48, 40), rows(6, 24, 40)])]
+    for fn, leaves in cases:
+        ordinary = fn(*leaves)
+        g = torch.randn(ordinary.shape, generator=_gen(2), device="cuda")
+        want = torch.autograd.grad(ordinary, leaves, g)
+        equal_rows = lambda t: t.dim() > 1 and t.is_floating_point() and bool((t == t[:1]).all())
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: (t[:1].clone(), t.shape) if equal_rows(t) else t,
+                                                      lambda p: p[0].expand(p[1]) if type(p) is tuple else p):
+            out = fn(*leaves)
+            got = torch.autograd.grad(out, leaves, g)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("name", ["layer_norm", "route_all", "combine"])
+def test_saved_tensors_that_come_back_of_another_type(name):
+    """Torch operations take them, in whatever type they are."""
+    want = _gradients(name)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.double() if t.is_floating_point() else t):
+        got = _gradients(name)
+    assert all(a.dtype == b.dtype and _near(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("back", [lambda t: t[:-1], lambda t: t[..., None], lambda t: t.cpu()],
+                         ids=["fewer", "another dimension", "the host's"])
+@pytest.mark.parametrize("name", NAMES)
+def test_saved_tensors_that_cannot_be_the_operand_s_are_refused(name, back):
+    """On the host, before any address of a smaller tensor reaches a kernel or an index a device."""
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back), pytest.raises(RuntimeError, match="came back|same device"):
+        _gradients(name)
+    fn, leaves = _operator(name)   # nor where torch operations follow
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back), pytest.raises(RuntimeError, match="came back|same device"):
+        out = fn(*leaves)
+        torch.autograd.grad(out, leaves, torch.ones_like(out), create_graph=True)
