@@ -720,8 +720,10 @@ def ops():
         except ImportError as exc:
             raise RuntimeError(f"adambridge_amd/_ops.so is not built or does not load ({exc}): "
                                "run `python -m adambridge_amd.build` (or __graft_entry__.build())") from exc
+        from torch.utils._device import DeviceContext
+
         from . import experts, norms
         _ops.connect({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in EXPORTS},
-                     {**norms.BACKWARD, **experts.BACKWARD})
+                     {**norms.BACKWARD, **experts.BACKWARD}, DeviceContext)
         _ops_module = _ops
     return _ops_module

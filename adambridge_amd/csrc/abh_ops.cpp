@@ -18,6 +18,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/PyInterpreter.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
@@ -60,6 +61,7 @@ struct Api {
 Api api;
 bool connected = false;
 PyObject* twice = nullptr;   // the backward passes in torch operations, by name
+PyObject* placing = nullptr; // the class of the modes that only place new tensors (a default device)
 
 // The tensor's device current and its current stream the library's, for the scope.
 struct On {
@@ -89,8 +91,10 @@ Tensor scratch(int64_t bytes, const Tensor& like) { return bytes ? fresh({(bytes
 
 bool observed()
 {
+    using Modes = at::impl::PythonTorchFunctionTLS;
+    for (int64_t i = 0, n = Modes::stack_len(); i < n; ++i)   // (also without the GIL: a type's address, no reference)
+        if ((PyObject*)Py_TYPE(Modes::get_stack_at(i)->ptr(getPyInterpreter())) != placing) return true;
     return torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::any_modes_set() ||
-           at::impl::PythonTorchFunctionTLS::stack_len() > 0 ||
            c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode);
 }
 
@@ -513,11 +517,11 @@ PyObject* expert_mm(PyObject*, PyObject* const* args, Py_ssize_t nargs)
 
 // --------------------------------------------------------------------------------- connect
 
-// connect(addresses by entry point, backward passes in torch operations by operator)
+// connect(addresses by entry point, backward passes in torch operations by operator, the class of default devices' modes)
 PyObject* connect(PyObject*, PyObject* const* args, Py_ssize_t nargs)
 {
-    if (nargs != 2 || !PyDict_CheckExact(args[0]) || !PyDict_CheckExact(args[1])) {
-        PyErr_SetString(PyExc_TypeError, "connect(addresses, backward passes)");
+    if (nargs != 3 || !PyDict_CheckExact(args[0]) || !PyDict_CheckExact(args[1]) || !PyType_Check(args[2])) {
+        PyErr_SetString(PyExc_TypeError, "connect(addresses, backward passes, class of default devices' modes)");
         return nullptr;
     }
     Api found;
@@ -541,6 +545,8 @@ PyObject* connect(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     }
     Py_INCREF(args[1]);
     Py_XSETREF(twice, args[1]);
+    Py_INCREF(args[2]);
+    Py_XSETREF(placing, args[2]);
     api = found;
     connected = true;
     Py_RETURN_NONE;

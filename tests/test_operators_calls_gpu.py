@@ -5,6 +5,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 import adambridge_amd as ab
+from adambridge_amd import experts, norms
 
 pytestmark = pytest.mark.gpu
 
@@ -121,3 +122,33 @@ def test_saved_tensors_that_cannot_be_the_operand_s_are_refused(name, back):
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t, back), pytest.raises(RuntimeError, match="came back|same device"):
         out = fn(*leaves)
         torch.autograd.grad(out, leaves, torch.ones_like(out), create_graph=True)
+
+
+# ----------------------------------------------------------------------- default devices
+
+def test_a_default_device_leaves_the_kernels_on(monkeypatch):
+    """A default device says where factory calls put their tensors; it observes no operation."""
+    want = [_gradients(name) for name in NAMES]
+    for module, name in ((experts, "_torch_route"), (experts, "_torch_dispatch"), (experts, "_torch_gather_sum"),
+                         (experts, "_torch_rows"), (norms, "_torch_layer_norm")):
+        monkeypatch.setattr(module, name, None)
+    for device in ("cuda", "cpu"):
+        with torch.device(device):
+            got = [_gradients(name) for name in NAMES]
+        assert all(torch.equal(a, b) for one, two in zip(got, want) for a, b in zip(one, two))
+
+
+def test_a_mode_that_observes_operations_sees_them():
+    class Count(torch.overrides.TorchFunctionMode):
+        def __init__(self):
+            self.seen = 0
+
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            self.seen += 1
+            return func(*args, **(kwargs or {}))
+
+    for name in NAMES:
+        fn, leaves = _operator(name)
+        with torch.device("cuda"), Count() as count:
+            fn(*leaves)
+        assert count.seen > 4, name
