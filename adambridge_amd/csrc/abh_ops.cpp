@@ -103,7 +103,8 @@ const Tensor* plain(PyObject* o)
 {
     if (Py_TYPE(o) != (PyTypeObject*)THPVariableClass && Py_TYPE(o) != (PyTypeObject*)ParameterClass) return nullptr;
     const Tensor& t = THPVariable_Unpack(o);
-    if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || !t.has_storage() || t.is_neg() || !t.is_contiguous())
+    if (!t.defined() || t.layout() != at::kStrided || !t.is_cuda() || !t.has_storage() || t._is_zerotensor() || t.is_neg() ||
+        !t.is_contiguous())
         return nullptr;
     return t._fw_grad(0).defined() ? nullptr : &t;
 }

@@ -152,3 +152,18 @@ def test_a_mode_that_observes_operations_sees_them():
         with torch.device("cuda"), Count() as count:
             fn(*leaves)
         assert count.seen > 4, name
+
+
+# -------------------------------------------------------------------------- zero tensors
+
+def test_tensors_without_memory_take_torch_operations():
+    """A tensor of zeros that holds no memory has no address to give to a kernel."""
+    zero = lambda *shape: torch._efficientzerotensor(shape, device="cuda")
+    some = lambda *shape: torch.randn(*shape, generator=_gen(3), device="cuda")
+    r = ab.route(some(12, 4), 2)
+    bias = some(16)
+    assert torch.equal(ab.layer_norm(zero(12, 16), some(16), bias), bias.expand(12, 16))
+    assert torch.equal(ab.route(zero(12, 4), 2).experts, torch.tensor([0, 1], device="cuda").int().expand(12, 2))
+    assert not ab.dispatch(zero(12, 16), r).any() and not ab.combine(zero(24, 16), r).any()
+    assert not ab.expert_mm(zero(24, 16), some(4, 8, 16), r.ends).any()
+    assert not ab.expert_mm(some(24, 16), zero(4, 8, 16), r.ends).any()
