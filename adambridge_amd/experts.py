@@ -213,7 +213,8 @@ def combine(rows: torch.Tensor, routing: Routing) -> torch.Tensor:
 def _bounds(rows: int, ends: torch.Tensor) -> list[tuple[int, int]]:
     """Each expert's rows; ends out of range or order pulled to the nearest that are not, as the kernels do."""
     out, lo = [], 0
-    for end in ends.tolist():
+    # under a function transform a copy to the host is a wrapped tensor, whose values come one by one
+    for end in [e.item() for e in ends.cpu()] if torch._C._are_functorch_transforms_active() else ends.tolist():
         lo = min(max(lo, 0), rows)
         out.append((lo, min(max(end, lo), rows)))
         lo = end

@@ -167,3 +167,24 @@ def test_tensors_without_memory_take_torch_operations():
     assert not ab.dispatch(zero(12, 16), r).any() and not ab.combine(zero(24, 16), r).any()
     assert not ab.expert_mm(zero(24, 16), some(4, 8, 16), r.ends).any()
     assert not ab.expert_mm(some(24, 16), zero(4, 8, 16), r.ends).any()
+
+
+# ---------------------------------------------------------------------------- transforms
+
+@pytest.mark.parametrize("name", NAMES)
+def test_function_transforms(name):
+    """torch.func's grad, jvp and vmap give the ordinary gradients, linear forms and rows."""
+    fn, leaves = _operator(name)
+    out = fn(*leaves)
+    g = torch.randn(out.shape, generator=_gen(1), device="cuda")
+    want = torch.autograd.grad(out, leaves, g)
+    free = [t.detach() for t in leaves]
+    got = torch.func.grad(lambda *ts: (fn(*ts) * g).sum(), argnums=tuple(range(len(free))))(*free)
+    assert all(_near(a, b) for a, b in zip(got, want))
+    moves = [torch.randn(t.shape, generator=_gen(8 + i), device="cuda") for i, t in enumerate(free)]
+    primal, moved = torch.func.jvp(fn, tuple(free), tuple(moves))
+    assert _near(primal, out.detach())
+    assert torch.allclose((moved * g).sum(), sum((a * b).sum() for a, b in zip(want, moves)), rtol=1e-3, atol=1e-2)
+    if name not in ("route", "route_all"):   # (a routing of a batch of logits has no one order)
+        twice = torch.func.vmap(fn, in_dims=(0,) + (None,) * (len(free) - 1))(torch.stack((free[0], 2 * free[0])), *free[1:])
+        assert _near(twice[0], out.detach()) and _near(twice[1], fn(2 * free[0], *free[1:]))
