@@ -51,14 +51,28 @@ struct ExpertArgs {
     float* part;        // ... splits x the result
 };
 
-// Rows lo .. hi of expert e (e = experts: the rows that are no expert's).  Ends outside 0 .. rows, or one below the
-// one before it, are pulled to the nearest that are not, so that no value of them leads out of the arrays.
-__device__ __forceinline__ void expert_rows(const ExpertArgs& A, int e, int& lo, int& hi)
+// Rows lo .. hi of expert e0 + the lane's number (expert `experts`: the rows that are no expert's), of 64 experts at a time
+// from 0 on; `before` (0 at first) is the last end before them.  An end outside 0 .. rows, or below one before it, is the
+// nearest that is not: whatever the ends are, no two experts share a row, and the experts' tiles are no more than
+// the launch reckons with.
+__device__ __forceinline__ void wave_rows(const ExpertArgs& A, int e0, int& before, int& lo, int& hi)
 {
+    const int lane = threadIdx.x & 63, e = e0 + lane;
     lo = e > 0 && e <= A.experts ? A.ends[e - 1] : e == 0 ? 0 : A.rows;
     hi = e < A.experts ? A.ends[e] : A.rows;
     lo = lo < 0 ? 0 : lo > A.rows ? A.rows : lo;
-    hi = hi < lo ? lo : hi > A.rows ? A.rows : hi;
+    hi = hi < 0 ? 0 : hi > A.rows ? A.rows : hi;
+    if (__builtin_amdgcn_ballot_w64(hi < lo || lo < before)) {   // the largest so far
+        hi = hi > before ? hi : before;
+#pragma unroll
+        for (int d = 1; d < kWave; d *= 2) {
+            const int y = __shfl_up(hi, d);
+            if (lane >= d && y > hi) hi = y;
+        }
+        lo = __shfl_up(hi, 1);
+        if (lane == 0) lo = before;
+    }
+    before = __builtin_amdgcn_readlane(hi, kWave - 1);
 }
 
 struct Tile {
@@ -75,10 +89,10 @@ __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirst
 template <int BM>
 __device__ __forceinline__ int count_row_tiles(const ExpertArgs& A)
 {
-    int total = 0;
+    int total = 0, last = 0;
     for (int e0 = 0; e0 <= A.experts; e0 += kWave) {
         int lo, hi;
-        expert_rows(A, e0 + (int)(threadIdx.x & 63), lo, hi);
+        wave_rows(A, e0, last, lo, hi);
         total += group_reduce<kWave>((hi - lo + BM - 1) / BM, [](int a, int b) { return a + b; });
     }
     return scalar(total) * A.tiles_j;
@@ -89,10 +103,10 @@ template <int BM>
 __device__ __forceinline__ bool locate_row_tile(const ExpertArgs& A, int idx, Tile& t)
 {
     const int lane = threadIdx.x & 63, q = idx / A.tiles_j;
-    int before = 0;
+    int before = 0, last = 0;
     for (int e0 = 0; e0 <= A.experts; e0 += kWave) {
         int lo, hi;
-        expert_rows(A, e0 + lane, lo, hi);
+        wave_rows(A, e0, last, lo, hi);
         const int n = (hi - lo + BM - 1) / BM;
         int s = n;
 #pragma unroll
@@ -198,10 +212,11 @@ __device__ __forceinline__ bool find_weight_tile(const ExpertArgs& A, Tile& t)
     t.e = scalar(t.e);
     t.split = scalar(t.split);
     t.splits = A.splits;
-    int lo, hi;
-    expert_rows(A, t.e, lo, hi);
-    lo = scalar(lo);
-    hi = scalar(hi);
+    int lo = 0, hi = A.ends[t.e];   // as wave_rows has them
+    for (int e = threadIdx.x & 63; e < t.e; e += kWave) lo = lo > A.ends[e] ? lo : A.ends[e];
+    lo = scalar(group_reduce<kWave>(lo, [](int a, int b) { return a > b ? a : b; }));
+    lo = lo < A.rows ? lo : A.rows;
+    hi = scalar(hi < lo ? lo : hi < A.rows ? hi : A.rows);
     const int chunk = ((hi - lo + A.splits - 1) / A.splits + 31) / 32 * 32;   // whole steps of 32 rows
     t.lo = scalar(chunk * t.split < hi - lo ? lo + chunk * t.split : hi);
     t.hi = scalar(t.lo + chunk < hi ? t.lo + chunk : hi);
@@ -455,10 +470,10 @@ __global__ __launch_bounds__(kFewWaves * kWave) void k_experts_few(ExpertArgs A)
     const int col = lane & 15, quarter = lane >> 4;
     const int block = (int)block_index(), tj = block % A.tiles_j;
     int skip = block / A.tiles_j;
-    int e = -1, lo = 0, hi = 0;
+    int e = -1, lo = 0, hi = 0, last = 0;
     for (int e0 = 0; e0 <= A.experts; e0 += kWave) {
         int l, h;
-        expert_rows(A, e0 + lane, l, h);
+        wave_rows(A, e0, last, l, h);
         const uint64_t with = __builtin_amdgcn_ballot_w64(h > l);
         const int count = __builtin_popcountll(with);
         if (skip < count) {

@@ -211,13 +211,12 @@ def combine(rows: torch.Tensor, routing: Routing) -> torch.Tensor:
 # ------------------------------------------------------------------- expert_mm
 
 def _bounds(rows: int, ends: torch.Tensor) -> list[tuple[int, int]]:
-    """Each expert's rows; ends out of range or order pulled to the nearest that are not, as the kernels do."""
+    """Each expert's rows; an end out of range, or below one before it, is the nearest that is not, as the kernels take it."""
     out, lo = [], 0
     # under a function transform a copy to the host is a wrapped tensor, whose values come one by one
     for end in [e.item() for e in ends.cpu()] if torch._C._are_functorch_transforms_active() else ends.tolist():
-        lo = min(max(lo, 0), rows)
         out.append((lo, min(max(end, lo), rows)))
-        lo = end
+        lo = out[-1][1]
     return out
 
 
@@ -247,7 +246,8 @@ BACKWARD = {"route": _route_backward, "dispatch": _dispatch_backward, "combine":
 def expert_mm(x: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
     """``x[r] @ weight[e].T`` for each row ``r`` of each expert ``e``: ``x`` ``[rows, in]`` sorted by expert, ``weight``
     ``[experts, out, in]`` (stacked Linear weights), expert ``e``'s rows ``ends[e - 1]`` to ``ends[e] - 1`` (``ends``: int32
-    ``[experts]``, not decreasing, on the device).  Rows from the last end on give zeros.
+    ``[experts]``, not decreasing, on the device; one that is below another before it counts as that, one beyond the rows as
+    their number).  Rows from the last end on give zeros.
 
     Sums are FP32, rounded once.  Differentiable in ``x`` and ``weight``; an expert without rows has zero gradients.
     Under autocast both operands are taken in autocast's type, as a Linear's are."""

@@ -549,9 +549,9 @@ ADAMBRIDGE_API int adambridge_combine_backward(const void* gout, const void* row
  * in device memory, none below the one before it; the first expert's start at 0); weight: experts x n x k (n and k 1 ..
  * 2^22).  y = x weight[e]^T (x: rows x k, y: rows x n); dx = gout weight[e] (gout: rows x n); dw[e] = gout^T x over e's
  * rows, zeros where there are none.  work: adambridge_expert_mm_work bytes of the product (ADAMBRIDGE_EXPERTS_Y, _DX or
- * _DW), 16-byte aligned, NULL if 0.  Rows from the last end on give zeros.  Ends that break the rule give
- * unspecified values, and nothing outside the arrays is touched.  A result of more than 2^30 tiles of 64 x 64 or larger is
- * ADAMBRIDGE_EBADN. */
+ * _DW), 16-byte aligned, NULL if 0.  Rows from the last end on give zeros.  An end outside 0 .. rows, or below one
+ * before it, counts as the nearest that is not: no two experts share a row and nothing outside the arrays is touched.  A
+ * result of more than 2^30 tiles of 64 x 64 or larger is ADAMBRIDGE_EBADN. */
 #define ADAMBRIDGE_EXPERTS_Y 0
 #define ADAMBRIDGE_EXPERTS_DX 1
 #define ADAMBRIDGE_EXPERTS_DW 2

@@ -1,0 +1,18 @@
+"""The expert block's operators in torch operations, on the CPU: operands at the edge of what they take."""
+
+import torch
+
+import adambridge_amd as ab
+
+
+def test_decreasing_ends_share_no_rows():
+    """An end below one before it counts as that: each row is one expert's, and the result has the rows of x."""
+    gen = torch.Generator().manual_seed(0)
+    x = torch.randn(9, 4, generator=gen, dtype=torch.float64, requires_grad=True)
+    w = torch.randn(5, 3, 4, generator=gen, dtype=torch.float64, requires_grad=True)
+    g = torch.randn(9, 3, generator=gen, dtype=torch.float64)
+    for ends, same in (([5, 3, 8, 2, 9], [5, 5, 8, 8, 9]), ([-2, 4, 1, 1, 6], [0, 4, 4, 4, 6]), ([12, 3, 3, 20, 1], [9] * 5)):
+        out, want = (ab.expert_mm(x, w, torch.tensor(e, dtype=torch.int32)) for e in (ends, same))
+        assert out.shape == (9, 3) and torch.equal(out, want)
+        for a, b in zip(torch.autograd.grad(out, (x, w), g), torch.autograd.grad(want, (x, w), g)):
+            assert torch.equal(a, b)
