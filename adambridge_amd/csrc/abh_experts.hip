@@ -260,6 +260,11 @@ __global__ __launch_bounds__(256) void k_experts_sum(const float* part, int64_t 
 
 constexpr int kTile = 128, kStep = 32, kMmThreads2 = 256;
 
+// A long FP32 sum's rounding errors grow with the chain it is taken in: every kF32Chain steps (256 terms) the products' sums are
+// added to others (norm of the error over the result's, 4096 terms on tiles: 1.1e-6 in one chain, 2.3e-7 in chains of 128; those
+// cost 3% of the time, 256 terms half of it; a gradient of 60000 rows of 3 values, below: 4.3e-6 in one chain, 3.9e-7).
+constexpr int kF32Chain = 8;
+
 template <int DT>
 constexpr int kPitch = kStep + 16 / kSize<DT>;
 template <int DT>
@@ -329,7 +334,9 @@ struct Stage {
     }
 };
 
-template <int DT, int MODE>
+// CHAINS: sums of more than kF32Chain steps in FP32.  (Two sets of sums leave two workgroups a CU of three: 65000 rows 3 -> 1000
+// 186 us with them, 168 without.)
+template <int DT, int MODE, bool CHAINS>
 __global__ __launch_bounds__(kMmThreads2, 2) void k_experts_any(ExpertArgs A)
 {
     constexpr bool ALONG = MODE != MODE_DW, BLONG = MODE == MODE_Y;
@@ -359,11 +366,12 @@ __global__ __launch_bounds__(kMmThreads2, 2) void k_experts_any(ExpertArgs A)
     }
     const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave, col = lane & 15, quarter = lane >> 4;
     const int wi = (wave & 1) * 64, wj = (wave >> 1) * 64;
-    mm_f32x4 acc[4][4];
+    const int live_i = scalar(limit_i - wi + 15) / 16, live_j = scalar(limit_j - wj + 15) / 16;   // FP32: the 16 x 16 that have results
+    mm_f32x4 acc[4][4], sum[4][4];   // sum: CHAINS'
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < 4; ++j) acc[i][j] = sum[i][j] = mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     Stage<DT, ALONG> sa;
     Stage<DT, BLONG> sb;
     if (len > 0) {
@@ -390,7 +398,7 @@ __global__ __launch_bounds__(kMmThreads2, 2) void k_experts_any(ExpertArgs A)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa[i], acc[i][j], 0, 0, 0);
         } else {
-#pragma unroll
+#pragma unroll 1
             for (int h = 0; h < kStep; h += 16) {
                 mm_f32x4 fa[4], fb[4];
 #pragma unroll
@@ -404,7 +412,17 @@ __global__ __launch_bounds__(kMmThreads2, 2) void k_experts_any(ExpertArgs A)
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[j][q], fa[i][q], acc[i][j], 0, 0, 0);
+                            if (i < live_i && j < live_j)
+                                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[j][q], fa[i][q], acc[i][j], 0, 0, 0);
+            }
+            if (CHAINS && (s / kStep % kF32Chain == kF32Chain - 1 || s + kStep >= len)) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        sum[i][j] += acc[i][j];
+                        acc[i][j] = mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    }
             }
         }
         __syncthreads();
@@ -421,7 +439,7 @@ __global__ __launch_bounds__(kMmThreads2, 2) void k_experts_any(ExpertArgs A)
             const int64_t o = (int64_t)row * A.nj + c;
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                if (c + r < limit_j) put<DT>(out, o + r, acc[i][j][r]);
+                if (c + r < limit_j) put<DT>(out, o + r, CHAINS ? sum[i][j][r] : acc[i][j][r]);
         }
     }
 }
@@ -1078,11 +1096,6 @@ ABH_EXPERTS_FAST(SmallTile)
 // four terms a lane, and the instructions take the terms in that order from both.  4096 x 4096 of 8192 rows: 128 / 124 / 127
 // TFLOP/s (y, dx, dW) of the 157 there are.
 
-// A long sum's rounding errors grow with the chain it is taken in: every kF32Chain steps (256 terms) the products' sums are
-// added to others (norm of the error over the result's, 4096 terms: 1.1e-6 in one chain, 2.3e-7 in chains of 128; those cost 3%
-// of the time, 256 terms half of it).
-constexpr int kF32Chain = 8;
-
 template <bool LONG, int R, int N>
 struct FragmentsF32 {
     int row;
@@ -1322,8 +1335,9 @@ static int experts_mm(const void* a, const void* b, const int32_t* ends, void* c
             hipLaunchKernelGGL((k_experts_fast<MODE, SmallTile, false>), grid, dim3(SmallTile::T), 0, t_stream, A);
         else if (p.kernel == Plan::F32_128) hipLaunchKernelGGL((k_experts_f32<MODE, 128>), grid, dim3(256), 0, t_stream, A);
         else if (p.kernel == Plan::F32_64) hipLaunchKernelGGL((k_experts_f32<MODE, 64>), grid, dim3(256), 0, t_stream, A);
-        else if (bf) hipLaunchKernelGGL((k_experts_any<DT_BF16, MODE>), grid, dim3(kMmThreads2), 0, t_stream, A);
-        else hipLaunchKernelGGL((k_experts_any<DT_F32, MODE>), grid, dim3(kMmThreads2), 0, t_stream, A);
+        else if (bf) hipLaunchKernelGGL((k_experts_any<DT_BF16, MODE, false>), grid, dim3(kMmThreads2), 0, t_stream, A);
+        else if (A.len > kF32Chain * kStep) hipLaunchKernelGGL((k_experts_any<DT_F32, MODE, true>), grid, dim3(kMmThreads2), 0, t_stream, A);
+        else hipLaunchKernelGGL((k_experts_any<DT_F32, MODE, MODE == MODE_DW>), grid, dim3(kMmThreads2), 0, t_stream, A);   // (dW's: the rows)
     }
     if (p.rest)
         hipLaunchKernelGGL((k_experts_rest<LargeTile>), dim3(kMostRest * LargeTile::BM / 16), dim3(256), 0, t_stream, A);
