@@ -250,7 +250,7 @@ def expert_mm(x: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) -> torc
     their number).  Rows from the last end on give zeros.
 
     Sums are FP32, rounded once.  Differentiable in ``x`` and ``weight``; an expert without rows has zero gradients.
-    Under autocast both operands are taken in autocast's type, as a Linear's are."""
+    Under autocast both operands are taken in autocast's type, as a Linear's are (not float64)."""
     if torch.compiler.is_compiling():
         return _uncompiled(expert_mm, x, weight, ends)
     if x.is_cuda:
@@ -267,7 +267,7 @@ def expert_mm(x: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) -> torc
         raise ValueError(f"x, weight and ends must be on one device, got {x.device}, {weight.device} and {ends.device}")
     if torch.is_autocast_enabled(x.device.type):
         cast = torch.get_autocast_dtype(x.device.type)
-        x, weight = x.to(cast), weight.to(cast)
+        x, weight = (t.to(cast) if t.is_floating_point() and t.dtype != torch.float64 else t for t in (x, weight))
     if x.dtype != weight.dtype or not x.is_floating_point():
         raise ValueError(f"x and weight must be of one floating-point type, got {x.dtype} and {weight.dtype}")
     experts, n, k = weight.shape

@@ -1,5 +1,6 @@
 """The expert block's operators in torch operations, on the CPU: operands at the edge of what they take."""
 
+import pytest
 import torch
 
 import adambridge_amd as ab
@@ -16,3 +17,16 @@ def test_decreasing_ends_share_no_rows():
         assert out.shape == (9, 3) and torch.equal(out, want)
         for a, b in zip(torch.autograd.grad(out, (x, w), g), torch.autograd.grad(want, (x, w), g)):
             assert torch.equal(a, b)
+
+
+def test_autocast_casts_what_a_linear_s_does():
+    """float32 and half types; float64 stays, whole numbers and a float64 beside a float32 are refused."""
+    x, w, ends = torch.randn(6, 4, dtype=torch.float64), torch.randn(2, 3, 4, dtype=torch.float64), torch.tensor([2, 6], dtype=torch.int32)
+    want = ab.expert_mm(x, w, ends)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        assert torch.equal(ab.expert_mm(x, w, ends), want)
+        assert ab.expert_mm(x.float(), w.float(), ends).dtype == torch.bfloat16
+        assert ab.expert_mm(x.half(), w.float(), ends).dtype == torch.bfloat16
+        for a, b in ((x.long(), w.float()), (x.long(), w.long()), (x.float(), w)):
+            with pytest.raises(ValueError, match="one floating-point type"):
+                ab.expert_mm(a, b, ends)
