@@ -126,18 +126,29 @@ def _fits(tokens: int, top_k: int, cols: int) -> bool:
     return tokens > 0 and top_k <= _MOST_CHOSEN and 0 < cols <= _MOST_SIZE and tokens * top_k <= _MOST_ASSIGNED
 
 
+def _assignments(position):
+    """The assignment that each row is, 0 where no position names it.  (Positions outside the rows go to one row more.)"""
+    flat, n = position.reshape(-1).long(), position.numel()
+    flat = torch.where((flat >= 0) & (flat < n), flat, n)
+    return flat.new_zeros(n + 1).scatter(0, flat, torch.arange(n, device=flat.device))[:n]
+
+
+def _picked(rows, position, j):
+    """Each token's row of its choice ``j``, zeros for a position outside the rows.  (No views: ``rows`` may be a batch.)"""
+    at, n = position[:, j].long(), position.numel()
+    inside = ((at >= 0) & (at < n))[:, None]
+    return torch.where(inside, rows.index_select(0, at.clamp(0, max(n - 1, 0))), 0.0)
+
+
 def _torch_dispatch(x, position):
-    token = torch.empty_like(position.reshape(-1), dtype=torch.int64)
-    at = torch.arange(position.numel(), device=x.device)
-    token = token.scatter(0, position.reshape(-1).long(), at // position.shape[1])
-    return x.index_select(0, token)
+    return x.index_select(0, _assignments(position) // position.shape[1])
 
 
 def _torch_gather_sum(rows, weights, position):
     wide = torch.promote_types(rows.dtype, torch.float32)
     total = None
-    for j in range(position.shape[1]):   # in order; no views, so that ``rows`` may be a batch
-        picked = rows.index_select(0, position[:, j].long()).to(wide)
+    for j in range(position.shape[1]):   # in order
+        picked = _picked(rows, position, j).to(wide)
         if weights is not None:
             picked = picked * weights[:, j:j + 1]   # never narrower than FP32
         total = picked if total is None else total + picked
@@ -153,13 +164,11 @@ def _combine_backward(gout, rows, weights, position, want_rows, want_weights):
     g = gout.float()
     drows = dweights = None
     if want_rows:
-        flat = position.reshape(-1).long()
-        assignment = torch.empty_like(flat).scatter(0, flat, torch.arange(flat.numel(), device=flat.device))
+        assignment = _assignments(position)
         w = weights.reshape(-1).index_select(0, assignment)[:, None]
         drows = (g.index_select(0, assignment // position.shape[1]) * w).to(gout.dtype)
     if want_weights:
-        dweights = torch.stack([(rows.index_select(0, position[:, j].long()).float() * g).sum(1)
-                                for j in range(position.shape[1])], 1)
+        dweights = torch.stack([(_picked(rows, position, j).float() * g).sum(1) for j in range(position.shape[1])], 1)
     return drows, dweights, None
 
 
@@ -185,7 +194,10 @@ def dispatch(x: torch.Tensor, routing: Routing) -> torch.Tensor:
 
 def combine(rows: torch.Tensor, routing: Routing) -> torch.Tensor:
     """Each token's sum of its ``rows`` (``[tokens * top_k, hidden]``, in the experts' order), weighted by the routing's
-    weights, summed in FP32 in the order of its choices and rounded once: ``[tokens, hidden]``."""
+    weights, summed in FP32 in the order of its choices and rounded once: ``[tokens, hidden]``.
+
+    A position outside the rows, which :func:`route` never gives, counts as a row of zeros.  A row that no position names
+    is unspecified in :func:`dispatch`'s result and in the gradient."""
     if torch.compiler.is_compiling():
         return _uncompiled(combine, rows, routing)
     if rows.is_cuda:

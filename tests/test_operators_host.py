@@ -30,3 +30,27 @@ def test_autocast_casts_what_a_linear_s_does():
         for a, b in ((x.long(), w.float()), (x.long(), w.long()), (x.float(), w)):
             with pytest.raises(ValueError, match="one floating-point type"):
                 ab.expert_mm(a, b, ends)
+
+
+def test_positions_outside_the_rows_count_as_zeros():
+    """As in the kernels: no error of an index, on whatever device."""
+    gen = torch.Generator().manual_seed(3)
+    r = ab.route(torch.randn(5, 4, generator=gen), 2)
+    position = r.position.clone()
+    position[1, 1], position[3, 0] = 10, -1
+    bad, keep = r._replace(position=position), torch.ones(5, 2)
+    keep[1, 1] = keep[3, 0] = 0.0
+    y = torch.randn(10, 6, generator=gen, requires_grad=True)
+    weights = r.weights.clone().requires_grad_()
+    out, want = ab.combine(y, bad._replace(weights=weights)), ab.combine(y, r._replace(weights=weights * keep))
+    assert torch.allclose(out, want)
+    g = torch.randn(5, 6, generator=gen)
+    for a, b in zip(torch.autograd.grad(out, (y, weights), g), torch.autograd.grad(want, (y, weights), g)):
+        assert torch.allclose(a, b)
+    x = torch.randn(5, 6, generator=gen, requires_grad=True)
+    rows = ab.dispatch(x, bad)
+    named = position[(position >= 0) & (position < 10)].long()
+    assert torch.equal(rows[named], ab.dispatch(x, r)[named])
+    g = torch.zeros(10, 6)
+    g[named] = 1.0
+    assert torch.equal(torch.autograd.grad(rows, x, g)[0], keep.sum(1, keepdim=True).expand(5, 6))
