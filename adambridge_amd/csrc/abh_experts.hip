@@ -669,8 +669,11 @@ struct Feed {
             // the arrival is waited for by wait_loads.
             const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)(lds + (q * W + wave) * 1024);
             const uint32_t from = LONG && last && past ? kOutside : offset[q];
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"   // m0 is never allocated ("reserved"), but the compiler reuses what it put there itself
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                         :: "s"(to), "v"(from), "s"(buffer), "s"(along) : "memory");
+                         :: "s"(to), "v"(from), "s"(buffer), "s"(along) : "m0", "memory");
+#pragma clang diagnostic pop
         }
         left -= BK;
         if constexpr (LONG) along += BK * 2;
