@@ -5,7 +5,7 @@
 A block is ``x + combine(down(gelu(up(dispatch(layer_norm(x))))))``: the package's layer norm, a router that
 chooses ``top_k`` of the experts for each token, the rows' way to them, their products, and the way back.  The
 loss is ``causal_lm_loss``, the optimizer ``AdamBridge`` (on the GPU; on the CPU, where its kernels do not
-run, torch's AdamW).  Nothing in a step waits for the device but the printing of the loss.
+run, torch's AdamW).  Nothing in a step waits for the device: the losses are read when the steps are done.
 """
 
 import argparse
@@ -54,6 +54,20 @@ class Model(torch.nn.Module):
         return ab.layer_norm(x, self.norm.weight, self.norm.bias, self.norm.eps)
 
 
+def fit(model: Model, opt: torch.optim.Optimizer, ids: torch.Tensor, steps: int, batch: int, seq: int) -> list[torch.Tensor]:
+    """``steps`` steps on windows of ``ids``; their losses, on the device."""
+    losses = []
+    for step in range(steps):
+        starts = torch.randint(0, 16, (batch,)).tolist()
+        x = torch.stack([ids[s:s + seq] for s in starts])
+        loss = ab.causal_lm_loss(model(x), model.head, x)
+        loss.backward()
+        opt.step()
+        opt.zero_grad()
+        losses.append(loss.detach())
+    return losses
+
+
 def train(steps: int, device: str, precision: str, batch: int = 8, seq: int = 64) -> tuple[list[float], Model, torch.Tensor]:
     """The losses of ``steps`` steps on a repeated sequence of tokens, the model, and the sequence."""
     torch.manual_seed(0)
@@ -63,17 +77,9 @@ def train(steps: int, device: str, precision: str, batch: int = 8, seq: int = 64
     else:
         opt = torch.optim.AdamW(model.parameters(), lr=3e-3)
     pattern = torch.randperm(512)[:16]   # no token twice: the tokens before say which comes next
-    ids = pattern.repeat(seq // 16 + 2)
-    losses = []
-    for step in range(steps):
-        starts = torch.randint(0, 16, (batch,)).tolist()
-        x = torch.stack([ids[s:s + seq] for s in starts]).to(device)
-        loss = ab.causal_lm_loss(model(x), model.head, x)
-        loss.backward()
-        opt.step()
-        opt.zero_grad()
-        losses.append(loss.item())
-    return losses, model, ids.to(device)
+    ids = pattern.repeat(seq // 16 + 2).to(device)
+    losses = fit(model, opt, ids, steps, batch, seq)
+    return [loss.item() for loss in losses], model, ids
 
 
 @torch.no_grad()
