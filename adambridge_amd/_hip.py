@@ -516,38 +516,6 @@ class HipKernels:
         self._check(rc, "adambridge_layer_norm_backward")
         return dx, dw, db
 
-    def route(self, logits: torch.Tensor, top_k: int, normalize: bool) -> tuple:
-        """Weights, chosen experts, ends, order and position of contiguous [tokens, experts] logits
-        (adambridge_route)."""
-        tokens, experts = logits.shape
-        self._operand("logits", logits, tuple(_DTYPE_CODES), (tokens, experts), logits.device)
-        work = self._work(logits.device, "adambridge_route", tokens, experts, top_k)
-        weights = torch.empty(tokens, top_k, dtype=torch.float32, device=logits.device)
-        ints = torch.empty(3 * tokens * top_k + experts, dtype=torch.int32, device=logits.device)
-        n = tokens * top_k
-        chosen, position = ints[:n].view(tokens, top_k), ints[n:2 * n].view(tokens, top_k)
-        order, ends = ints[2 * n:3 * n], ints[3 * n:]
-        rc = self._on(logits.device, self._lib.adambridge_route, logits.data_ptr(), _DTYPE_CODES[logits.dtype], tokens, experts,
-                      top_k, int(normalize), weights.data_ptr(), chosen.data_ptr(), ends.data_ptr(), order.data_ptr(),
-                      position.data_ptr(), _address(work))
-        self._check(rc, "adambridge_route")
-        return weights, chosen, ends, order, position
-
-    def route_backward(self, weights: torch.Tensor, chosen: torch.Tensor, gout: torch.Tensor, logits: torch.Tensor | None,
-                       dtype: torch.dtype, experts: int, normalize: bool) -> torch.Tensor:
-        """The logits' gradient (of ``dtype``) from the weights' (adambridge_route_backward)."""
-        tokens, top_k = weights.shape
-        self._operand("weights", weights, (torch.float32,), (tokens, top_k), weights.device)
-        self._operand("gout", gout, (torch.float32,), (tokens, top_k), weights.device)
-        self._operand("chosen", chosen, (torch.int32,), (tokens, top_k), weights.device)
-        if not normalize:
-            self._operand("logits", logits, (dtype,), (tokens, experts), weights.device)
-        grad = torch.empty(tokens, experts, dtype=dtype, device=weights.device)
-        rc = self._on(weights.device, self._lib.adambridge_route_backward, weights.data_ptr(), chosen.data_ptr(), gout.data_ptr(),
-                      _address(logits), _DTYPE_CODES[dtype], tokens, experts, top_k, int(normalize), grad.data_ptr())
-        self._check(rc, "adambridge_route_backward")
-        return grad
-
     def dispatch(self, x: torch.Tensor, position: torch.Tensor) -> torch.Tensor:
         """The rows ``position`` [tokens, top_k] gives each token of contiguous [tokens, cols] values
         (adambridge_dispatch)."""
@@ -559,19 +527,6 @@ class HipKernels:
                       top_k, cols, rows.data_ptr())
         self._check(rc, "adambridge_dispatch")
         return rows
-
-    def combine(self, rows: torch.Tensor, weights: torch.Tensor | None, position: torch.Tensor) -> torch.Tensor:
-        """Each token's weighted sum of its rows (adambridge_combine)."""
-        (tokens, top_k), cols = position.shape, rows.shape[1]
-        self._operand("rows", rows, tuple(_DTYPE_CODES), (tokens * top_k, cols), rows.device)
-        self._operand("position", position, (torch.int32,), (tokens, top_k), rows.device)
-        if weights is not None:
-            self._operand("weights", weights, (torch.float32,), (tokens, top_k), rows.device)
-        out = torch.empty(tokens, cols, dtype=rows.dtype, device=rows.device)
-        rc = self._on(rows.device, self._lib.adambridge_combine, rows.data_ptr(), _DTYPE_CODES[rows.dtype], _address(weights),
-                      position.data_ptr(), tokens, top_k, cols, out.data_ptr())
-        self._check(rc, "adambridge_combine")
-        return out
 
     def combine_backward(self, gout: torch.Tensor, rows: torch.Tensor | None, weights: torch.Tensor, position: torch.Tensor,
                          wanted: tuple) -> tuple:

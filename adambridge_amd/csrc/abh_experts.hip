@@ -19,7 +19,6 @@
 #include <algorithm>
 #include <type_traits>
 
-
 #include "../../include/adambridge_hip.h"
 #include "abh_device.hpp"
 #include "abh_host.hpp"
@@ -32,8 +31,6 @@ constexpr int kXcd = 8;
 constexpr int kGroupTiles = 8;   // row tiles that share their columns' weights while those are in the L2
 
 typedef float mm_f32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t mm_u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t mm_u32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 mm_bf16x8 __attribute__((ext_vector_type(8)));
 
 enum { MODE_Y = 0, MODE_DX = 1, MODE_DW = 2 };

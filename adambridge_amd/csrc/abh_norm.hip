@@ -491,7 +491,7 @@ ADAMBRIDGE_API int adambridge_layer_norm_backward(const void* gout, const void* 
     norm_by_type(A, dtype, w_dtype, true, parts);
     if (sums && (parts > 1 || !norm_back_shape(cols).lanes)) {
         const dim3 grid((unsigned)((2 * cols + 63) / 64));
-                if (w_dtype == ADAMBRIDGE_DT_BF16) hipLaunchKernelGGL((k_norm_sums<DT_BF16>), grid, dim3(1024), 0, t_stream, A, parts);
+        if (w_dtype == ADAMBRIDGE_DT_BF16) hipLaunchKernelGGL((k_norm_sums<DT_BF16>), grid, dim3(1024), 0, t_stream, A, parts);
         else hipLaunchKernelGGL((k_norm_sums<DT_F32>), grid, dim3(1024), 0, t_stream, A, parts);
     }
     const hipError_t e = hipGetLastError();

@@ -19,8 +19,6 @@
 
 #include <stdint.h>
 
-#include <algorithm>
-
 #include "../../include/adambridge_hip.h"
 #include "abh_device.hpp"
 #include "abh_host.hpp"
