@@ -1,11 +1,13 @@
 """Calls of the expert block's operators that are not the ordinary ones: what reaches a kernel, and what must not."""
 
+import threading
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
 import adambridge_amd as ab
-from adambridge_amd import experts, norms
+from adambridge_amd import _hip, experts, norms
 
 pytestmark = pytest.mark.gpu
 
@@ -188,3 +190,67 @@ def test_function_transforms(name):
     if name not in ("route", "route_all"):   # (a routing of a batch of logits has no one order)
         twice = torch.func.vmap(fn, in_dims=(0,) + (None,) * (len(free) - 1))(torch.stack((free[0], 2 * free[0])), *free[1:])
         assert _near(twice[0], out.detach()) and _near(twice[1], fn(2 * free[0], *free[1:]))
+
+
+# ----------------------------------------------------------------- threads and refusals
+
+def test_threads_have_a_stream_each():
+    want = [_gradients(name) for name in NAMES]
+    torch.cuda.synchronize()
+    got, errors = {}, []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got[i] = [_gradients(name) for name in NAMES]
+                torch.cuda.current_stream().synchronize()
+        except Exception as error:   # reported by the thread that asserts
+            errors.append(error)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors and len(got) == 3
+    for one in got.values():
+        assert all(torch.equal(a, b) for x, y in zip(one, want) for a, b in zip(x, y))
+
+
+def test_calls_that_are_not_ordinary_ones_are_left_to_python():
+    """The native calls answer None, before anything is done, to what their kernels do not take."""
+    o = _hip.ops()
+    x, w, b = (torch.randn(*s, device="cuda") for s in ((6, 16), (16,), (16,)))
+    for args in ((x.half(), w, b, 1e-5), (x.t(), w[:6], None, 1e-5), (x[:, ::2], None, None, 1e-5), (x, w[:8], None, 1e-5),
+                 (x, w, b.bfloat16(), 1e-5), (x, w.cpu(), None, 1e-5), (x.cpu(), None, None, 1e-5), (x, w.double(), None, 1e-5),
+                 (x, w, b, 1), (x[:0], w, b, 1e-5), (x[0, 0], None, None, 1e-5), (x, w, 3.0, 1e-5), (x, w, None)):
+        assert o.layer_norm(*args) is None
+    for args in ((x.half(), 2, True), (x, 17, True), (x, 0, True), (x, True, True), (x, 2, 1), (x, 1 << 70, True), (x.t(), 2, True),
+                 (x[0], 1, True), (x[:0], 2, True), (torch.randn(2, 1025, device="cuda"), 2, True),
+                 (torch.randn(2, 100, device="cuda"), 65, True)):
+        assert o.route(*args) is None
+    r = ab.route(torch.randn(6, 4, device="cuda"), 2)
+    y = torch.randn(12, 16, device="cuda")
+    for args in ((x, r.position.long()), (x, r.position[:5]), (x, r.position.t()), (x, r.position.cpu()), (x.double(), r.position),
+                 (x[0], r.position), (x, r.position[0]), (x, None)):
+        assert o.dispatch(*args) is None
+    for args in ((x, r.weights, r.position), (y, r.weights.double(), r.position), (y, r.weights[:, :1].contiguous(), r.position),
+                 (y, r.weights, r.position.long()), (y, r.weights.cpu(), r.position), (y.t(), r.weights, r.position), (y, None, r.position)):
+        assert o.combine(*args) is None
+    w = torch.randn(4, 8, 16, device="cuda")
+    for args in ((y, w.bfloat16(), r.ends), (y, w, r.ends.long()), (y, w, r.ends[:3]), (y, w[:, :, :8].contiguous(), r.ends),
+                 (y, w.transpose(1, 2), r.ends), (y.half(), w.half(), r.ends), (y, w[0], r.ends), (y, w, r.ends.cpu()),
+                 (y, w[:, :0], r.ends), (y[0], w, r.ends)):
+        assert o.expert_mm(*args) is None
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        assert o.expert_mm(y, w, r.ends) is None
+    with pytest.raises(ValueError, match="of one type"):
+        ab.layer_norm(x, torch.ones(16, device="cuda"), b.bfloat16())
+    with pytest.raises(ValueError, match="top_k must be an int"):
+        ab.route(x, 17)
+    with pytest.raises(ValueError, match="int32"):
+        ab.dispatch(x, r._replace(position=r.position.long()))
+    with pytest.raises(ValueError, match="weights must be float32"):
+        ab.combine(y, r._replace(weights=r.weights.double()))
+    with pytest.raises(ValueError, match="on one device"):
+        ab.expert_mm(y, w, r.ends.cpu())
+    assert ab.expert_mm(y.half(), w.half(), r.ends).dtype == torch.float16   # torch operations
