@@ -484,6 +484,7 @@ ADAMBRIDGE_API int adambridge_layer_norm_backward(const void* gout, const void* 
     if (!type_ok(dtype) || !type_ok(w_dtype)) return ADAMBRIDGE_EMVDTYPE;
     const bool sums = dweight || dbias;
     if (!gout || !x || !stats || (sums && !work)) return ADAMBRIDGE_ENULL;
+    if (sums && (uintptr_t)work % 4) return ADAMBRIDGE_EALIGN;
     if (!dx && !sums) return 0;
     const int parts = norm_parts(rows, cols);
     const NormArgs A{x, gout, weight, nullptr, dx, const_cast<float*>(stats), dweight, dbias, static_cast<float*>(work),

@@ -1,9 +1,12 @@
 """The expert block's operators in torch operations, on the CPU: operands at the edge of what they take."""
 
+import ctypes
+
 import pytest
 import torch
 
 import adambridge_amd as ab
+from adambridge_amd import _hip
 
 
 def test_decreasing_ends_share_no_rows():
@@ -54,3 +57,11 @@ def test_positions_outside_the_rows_count_as_zeros():
     g = torch.zeros(10, 6)
     g[named] = 1.0
     assert torch.equal(torch.autograd.grad(rows, x, g)[0], keep.sum(1, keepdim=True).expand(5, 6))
+
+
+def test_scratch_of_a_norm_s_gradient_is_at_a_word():
+    """Refused before anything is launched."""
+    lib, p = _hip.open_library(), ctypes.c_void_p(256)
+    for offset in (1, 2, 3):
+        rc = lib.adambridge_layer_norm_backward(p, p, _hip.DT_F32, None, _hip.DT_F32, p, 4, 4, p, p, p, ctypes.c_void_p(256 + offset))
+        assert rc == -14
