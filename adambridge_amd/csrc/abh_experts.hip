@@ -1257,7 +1257,9 @@ static Plan plan_experts(int mode, int32_t dtype, int64_t rows, int64_t experts,
         const int64_t j = (nj + t - 1) / t;
         return mode == MODE_DW ? experts * ((ni + t - 1) / t) * j : (rows / t + (used + 1) / 2) * j;
     };
-    // few rows an expert: the weights' bytes are all there is; or more, read at once, of too few tiles whose sums are not cut
+    // few rows an expert: the weights' bytes are all there is; or more, read at once, of too few tiles whose sums are not cut.  By
+    // the average, the host knows no other: rows that are all one expert's are slower so than on tiles (512 rows, us, spread
+    // evenly / all one expert's / that expert alone, on tiles: 64 experts 87 / 81 / 18, 8 experts 1024 x 1024 14 / 43 / 14)
     if (mode == MODE_Y && (rows <= std::max<int64_t>(bf ? 16 : 64, 8 * experts) || (rows <= 64 * experts && tiles(64) < 256 && (!bf || k <= 1024))))
         return {Plan::FEW, 0, 1, false};
     if (any) return {Plan::ANY, kTile, 1, false};
@@ -1269,7 +1271,8 @@ static Plan plan_experts(int mode, int32_t dtype, int64_t rows, int64_t experts,
         const int64_t t = std::max<int64_t>(1, tiles(p.tile));
         p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / t, rows / experts / 256));
     }
-    // few tiles with long sums: parts of 16 steps or more, about a workgroup a CU (the tiles are fewer than reckoned with)
+    // few tiles with long sums: parts of 16 steps or more, about a workgroup a CU (by the reckoned tiles: the experts' last ones make
+    // up to half a row tile an expert more or fewer)
     if (mode != MODE_DW && p.kernel == Plan::SMALL)
         p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(320 / std::max<int64_t>(1, tiles(p.tile)), (mode == MODE_Y ? k : n) / (16 * SmallTile::BK)));
     // a long sum, and so few rounds that a cut rest may count

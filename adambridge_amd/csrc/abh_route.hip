@@ -59,7 +59,9 @@ __device__ __forceinline__ float key_value(uint32_t key)
     return key == 0xffffffffu ? __builtin_nanf("") : bitsf(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-// exp(x - m) with m = -inf taken as 0, so that a row without any finite logit has weights 0 and not NaN.
+// exp(x - m) with m = -inf taken as 0, so that a row without any finite logit has weights 0 and not NaN.  x - m and its
+// product with log2 e are rounded to FP32: the largest weight's exponential is exact, one of e^-8 is off by at most 2^-20 of
+// itself, one near FP32's smallest, e^-87, by 2^-17.
 __device__ __forceinline__ float exp_below(float x, float m)
 {
     return __builtin_amdgcn_exp2f((x - (m == kRouteNegInf ? 0.0f : m)) * kRouteLog2e);
