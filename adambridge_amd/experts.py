@@ -63,9 +63,9 @@ def _torch_route(logits, top_k, normalize):
     weights = e / torch.where(total == 0.0, 1.0, total)
     flat = chosen.reshape(-1)
     order = torch.sort(flat, stable=True).indices
-    at = torch.arange(tokens * top_k, device=logits.device)
-    position = torch.empty_like(order).scatter_(0, order, at).view(tokens, top_k)
-    ends = torch.zeros(experts, dtype=torch.int64, device=logits.device).scatter_add_(0, flat, torch.ones_like(flat)).cumsum(0)
+    at = torch.arange(tokens * top_k, device=logits.device)   # nothing in place below: ``logits`` may be a batch
+    position = torch.zeros_like(order).scatter(0, order, at).view(tokens, top_k)
+    ends = torch.zeros(experts, dtype=torch.int64, device=logits.device).scatter_add(0, flat, torch.ones_like(flat)).cumsum(0)
     return Routing(weights, chosen.int(), ends.int(), order.int(), position.int())
 
 
@@ -261,7 +261,8 @@ def expert_mm(x: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) -> torc
     ``[experts]``, not decreasing, on the device; one that is below another before it counts as that, one beyond the rows as
     their number).  Rows from the last end on give zeros.
 
-    Sums are FP32, rounded once.  Differentiable in ``x`` and ``weight``; an expert without rows has zero gradients.
+    Sums are FP32, rounded once.  Differentiable in ``x`` and ``weight``; an expert without rows has zero gradients.  (Under
+    ``vmap`` the ends, which decide sizes, are one for all.)
     Under autocast both operands are taken in autocast's type, as a Linear's are (not float64)."""
     if torch.compiler.is_compiling():
         return _uncompiled(expert_mm, x, weight, ends)

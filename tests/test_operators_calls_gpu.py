@@ -187,9 +187,19 @@ def test_function_transforms(name):
     primal, moved = torch.func.jvp(fn, tuple(free), tuple(moves))
     assert _near(primal, out.detach())
     assert torch.allclose((moved * g).sum(), sum((a * b).sum() for a, b in zip(want, moves)), rtol=1e-3, atol=1e-2)
-    if name not in ("route", "route_all"):   # (a routing of a batch of logits has no one order)
+    if name not in ("route", "route_all"):   # (theirs: test_routings_of_a_batch)
         twice = torch.func.vmap(fn, in_dims=(0,) + (None,) * (len(free) - 1))(torch.stack((free[0], 2 * free[0])), *free[1:])
         assert _near(twice[0], out.detach()) and _near(twice[1], fn(2 * free[0], *free[1:]))
+
+
+def test_routings_of_a_batch():
+    logits = torch.randn(3, 70, 12, generator=_gen(4), device="cuda")
+    for normalize in (True, False):
+        one_by_one = [ab.route(t, 2, normalize) for t in logits]
+        at_once = torch.func.vmap(lambda t: tuple(ab.route(t, 2, normalize)))(logits)
+        assert _near(at_once[0], torch.stack([r.weights for r in one_by_one]))
+        for i in range(1, 5):
+            assert torch.equal(at_once[i], torch.stack([r[i] for r in one_by_one]))
 
 
 # ----------------------------------------------------------------- threads and refusals

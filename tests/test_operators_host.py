@@ -65,3 +65,19 @@ def test_scratch_of_a_norm_s_gradient_is_at_a_word():
     for offset in (1, 2, 3):
         rc = lib.adambridge_layer_norm_backward(p, p, _hip.DT_F32, None, _hip.DT_F32, p, 4, 4, p, p, p, ctypes.c_void_p(256 + offset))
         assert rc == -14
+
+
+def test_routings_of_a_batch():
+    """vmap over logits gives each one's routing, and what is dispatched and combined by it."""
+    gen = torch.Generator().manual_seed(5)
+    logits, x, y = (torch.randn(3, *s, generator=gen) for s in ((6, 4), (6, 5), (12, 5)))
+    for normalize in (True, False):
+        one_by_one = [ab.route(t, 2, normalize) for t in logits]
+        at_once = torch.func.vmap(lambda t: tuple(ab.route(t, 2, normalize)))(logits)
+        for i, got in enumerate(at_once):
+            assert torch.equal(got, torch.stack([r[i] for r in one_by_one]))
+    one_by_one = [ab.route(t, 2) for t in logits]
+    got = torch.func.vmap(lambda t, a: ab.dispatch(a, ab.route(t, 2)))(logits, x)
+    assert torch.equal(got, torch.stack([ab.dispatch(a, r) for a, r in zip(x, one_by_one)]))
+    got = torch.func.vmap(lambda t, a: ab.combine(a, ab.route(t, 2)))(logits, y)
+    assert torch.allclose(got, torch.stack([ab.combine(a, r) for a, r in zip(y, one_by_one)]))
