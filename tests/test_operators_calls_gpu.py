@@ -64,6 +64,28 @@ def test_a_gradient_s_tangent_is_carried_on(name):
         assert _near(primal, want_primal) and _near(moved, want_moved)
 
 
+@pytest.mark.parametrize("name", NAMES)
+def test_second_derivatives(name):
+    """The kernels' gradients, differentiated in turn: as torch operations differentiate the definition in 64 bits."""
+    _, leaves = _operator(name)
+    r = ab.route(torch.randn(24, 6, generator=_gen(9), device="cuda"), 2)
+    fns = {"layer_norm": lambda r: ab.layer_norm, "route": lambda r: lambda x: ab.route(x, 3).weights,
+           "route_all": lambda r: lambda x: ab.route(x, 3, normalize=False).weights, "dispatch": lambda r: lambda x: ab.dispatch(x, r),
+           "combine": lambda r: lambda y, w: ab.combine(y, r._replace(weights=w)), "expert_mm": lambda r: lambda x, w: ab.expert_mm(x, w, r.ends)}
+    results = []
+    for cast in (lambda t: t, lambda t: t.cpu().double() if t.is_floating_point() else t.cpu()):
+        here = [cast(t.detach()).requires_grad_() for t in leaves]
+        out = fns[name](ab.Routing(*map(cast, r)))(*here)
+        g, *moves = [cast(torch.randn(t.shape, generator=_gen(20 + i), device="cuda")) for i, t in enumerate((out, *here))]
+        g.requires_grad_()
+        first = torch.autograd.grad((out * out).sum() if name == "dispatch" else (out * g).sum(), here, create_graph=True)
+        second = torch.autograd.grad(sum((a * m).sum() for a, m in zip(first, moves)), [g, *here], allow_unused=True)
+        results.append([t if t is None else t.cpu().float() for t in second])
+    for got, want in zip(*results):
+        assert (got is None) == (want is None) and (got is None or _near(got, want) or torch.allclose(got, want, rtol=1e-3, atol=1e-3))
+    assert any(t is not None for t in results[0])
+
+
 # ------------------------------------------------------------------------- saved tensors
 
 def _strided(t):
