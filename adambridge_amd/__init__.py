@@ -13,6 +13,7 @@ from .losses import causal_lm_loss
 from .norms import layer_norm
 from .optimizer import AdamBridge, AutoTuneConfig, LionBridge, OptiComputeAdamW
 from .precision import bytes_per_param
+from .vocabulary import embed
 
 __version__ = "0.1.0"
 
@@ -30,6 +31,7 @@ __all__ = [
     "dispatch",
     "expert_mm",
     "combine",
+    "embed",
     "native",
     "precision",
     "__version__",

@@ -125,7 +125,8 @@ EXPORTS = (
     "adambridge_layer_norm", "adambridge_layer_norm_work", "adambridge_layer_norm_backward", "adambridge_route_work",
     "adambridge_route", "adambridge_route_backward", "adambridge_dispatch", "adambridge_combine",
     "adambridge_combine_backward", "adambridge_expert_mm", "adambridge_expert_mm_dx",
-    "adambridge_expert_mm_work", "adambridge_expert_mm_dw",
+    "adambridge_expert_mm_work", "adambridge_expert_mm_dw", "adambridge_embed", "adambridge_embed_work",
+    "adambridge_embed_backward",
 )
 
 
@@ -186,6 +187,9 @@ def open_library(path: Path = LIB_PATH) -> ctypes.CDLL:
         "adambridge_expert_mm_dx": (ctypes.c_int, [vp, vp, vp, vp, i32, i64, i64, i64, i64, vp]),
         "adambridge_expert_mm_work": (i64, [i32, i32, i64, i64, i64, i64]),
         "adambridge_expert_mm_dw": (ctypes.c_int, [vp, vp, vp, vp, i32, i64, i64, i64, i64, vp]),
+        "adambridge_embed": (ctypes.c_int, [vp, i32, i64, vp, i32, i64, i64, ctypes.c_float, vp]),
+        "adambridge_embed_work": (i64, [i64, i64, i64]),
+        "adambridge_embed_backward": (ctypes.c_int, [vp, i32, i64, vp, i32, i64, i64, ctypes.c_float, i64, vp, vp]),
     }
     for name in EXPORTS:
         fn = getattr(lib, name)
@@ -677,8 +681,8 @@ def ops():
                                "run `python -m adambridge_amd.build` (or __graft_entry__.build())") from exc
         from torch.utils._device import DeviceContext
 
-        from . import experts, norms
+        from . import experts, norms, vocabulary
         _ops.connect({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in EXPORTS},
-                     {**norms.BACKWARD, **experts.BACKWARD}, DeviceContext)
+                     {**norms.BACKWARD, **experts.BACKWARD, **vocabulary.BACKWARD}, DeviceContext)
         _ops_module = _ops
     return _ops_module

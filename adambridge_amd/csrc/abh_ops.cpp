@@ -1,9 +1,9 @@
-// abh_ops.cpp -- the host's side of an expert block's operators, natively (Python module _ops).
+// abh_ops.cpp -- the host's side of the operators of a model of expert blocks, natively (Python module _ops).
 //
 // A call of one token costs what its host work costs: through Python's autograd functions and ctypes a layer norm of
 // one row took 13 us, its training pass 100, for kernels of 4 and 8.  Here are the ordinary calls: plain contiguous
 // tensors of the kernels' types on one GPU, in no trace, transform or mode.  Every other call returns None, before
-// anything is done, and the Python functions (norms.py, experts.py) check it, lay it out or take torch
+// anything is done, and the Python functions (norms.py, experts.py, vocabulary.py) check it, lay it out or take torch
 // operations.  The backward passes are here too; one that is itself differentiated, batched or observed calls the
 // Python function of the same formula in torch operations that connect() was given.
 
@@ -27,6 +27,7 @@
 #include <cstdint>
 #include <cstring>
 #include <string>
+#include <vector>
 
 #include "../../include/adambridge_hip.h"
 
@@ -56,6 +57,9 @@ struct Api {
     decltype(&adambridge_expert_mm_dx) expert_mm_dx;
     decltype(&adambridge_expert_mm_work) expert_mm_work;
     decltype(&adambridge_expert_mm_dw) expert_mm_dw;
+    decltype(&adambridge_embed) embed;
+    decltype(&adambridge_embed_work) embed_work;
+    decltype(&adambridge_embed_backward) embed_backward;
 };
 
 Api api;
@@ -516,6 +520,80 @@ PyObject* expert_mm(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     END_HANDLE_TH_ERRORS
 }
 
+// ----------------------------------------------------------------------------------- embed
+
+Tensor embed_forward(const Tensor& ids, const Tensor& weight, double scale)
+{
+    std::vector<int64_t> sizes = ids.sizes().vec();
+    sizes.push_back(weight.size(1));
+    Tensor y = fresh(sizes, weight.scalar_type(), weight);
+    const On on(weight);
+    check(api.embed(address(ids), (int32_t)ids.element_size(), ids.numel(), address(weight), code(weight.scalar_type()), weight.size(0),
+                    weight.size(1), (float)scale, place(y)), "adambridge_embed");
+    return y;
+}
+
+struct Embed : Function<Embed> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& ids, const Tensor& weight, double scale, int64_t padding)
+    {
+        const at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({ids});
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["padding"] = padding;
+        ctx->saved_data["vocab"] = weight.size(0);
+        ctx->saved_data["type"] = (int64_t)ids.scalar_type();
+        return embed_forward(ids, weight, scale);
+    }
+    static tensor_list backward(AutogradContext* ctx, const tensor_list& grads)
+    {
+        const tensor_list saved = ctx->get_saved_variables();
+        const Tensor& ids = saved[0];
+        const double scale = ctx->saved_data["scale"].toDouble();
+        const int64_t padding = ctx->saved_data["padding"].toInt(), vocab = ctx->saved_data["vocab"].toInt();
+        const at::IntArrayRef sizes = sizes_of(grads[0]);
+        const bool whole = !sizes.empty() && restored(ids, grads[0], (at::ScalarType)ctx->saved_data["type"].toInt(), sizes.slice(0, sizes.size() - 1));
+        if (!whole || !plain_backward(grads[0]))
+            return in_torch("embed", [&] {
+                return pybind11::make_tuple(grads[0], ids, vocab, scale,
+                                            padding < 0 ? pybind11::object(pybind11::none()) : pybind11::object(pybind11::int_(padding)));
+            }, 4);
+        const at::AutoDispatchBelowADInplaceOrView below;
+        const Tensor g = grads[0].contiguous(), i = ids.contiguous();
+        const int64_t tokens = i.numel(), hidden = sizes.back();
+        const int64_t bytes = api.embed_work(tokens, vocab, hidden);
+        check(bytes, "adambridge_embed_work");
+        tensor_list out(4);
+        out[1] = fresh({vocab, hidden}, g.scalar_type(), g);
+        Tensor work = scratch(bytes, g);
+        const On on(g);
+        check(api.embed_backward(address(i), (int32_t)i.element_size(), tokens, address(g), code(g.scalar_type()), vocab, hidden, (float)scale,
+                                 padding, place(out[1]), place(work)), "adambridge_embed_backward");
+        return out;
+    }
+};
+
+// embed(ids, weight, scale, padding_idx or None)
+PyObject* embed(PyObject*, PyObject* const* args, Py_ssize_t nargs)
+{
+    HANDLE_TH_ERRORS
+    if (nargs != 4 || !connected || observed()) Py_RETURN_NONE;
+    const Tensor *ids = plain(args[0]), *weight = plain(args[1]);
+    if (!values(weight, 2) || !ids || ids->device() != weight->device() || !PyFloat_CheckExact(args[2])) Py_RETURN_NONE;
+    if ((ids->scalar_type() != at::kLong && ids->scalar_type() != at::kInt) || (args[3] != Py_None && !PyLong_CheckExact(args[3]))) Py_RETURN_NONE;
+    int64_t padding = -1;
+    if (args[3] != Py_None) {
+        padding = PyLong_AsLongLong(args[3]);
+        if (padding == -1 && PyErr_Occurred()) PyErr_Clear();
+        if (padding < 0 || padding >= weight->size(0)) Py_RETURN_NONE;
+    }
+    if (api.embed_work(ids->numel(), weight->size(0), weight->size(1)) < 0) Py_RETURN_NONE;   // sizes out of the kernels' range
+    const double scale = PyFloat_AS_DOUBLE(args[2]);
+    if (wants_grad({weight})) return THPVariable_Wrap(Embed::apply(*ids, *weight, scale, padding));
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return THPVariable_Wrap(embed_forward(*ids, *weight, scale));
+    END_HANDLE_TH_ERRORS
+}
+
 // --------------------------------------------------------------------------------- connect
 
 // connect(addresses by entry point, backward passes in torch operations by operator, the class of default devices' modes)
@@ -534,7 +612,8 @@ PyObject* connect(PyObject*, PyObject* const* args, Py_ssize_t nargs)
         {&found.dispatch, "adambridge_dispatch"}, {&found.combine, "adambridge_combine"},
         {&found.combine_backward, "adambridge_combine_backward"}, {&found.expert_mm, "adambridge_expert_mm"},
         {&found.expert_mm_dx, "adambridge_expert_mm_dx"}, {&found.expert_mm_work, "adambridge_expert_mm_work"},
-        {&found.expert_mm_dw, "adambridge_expert_mm_dw"}};
+        {&found.expert_mm_dw, "adambridge_expert_mm_dw"}, {&found.embed, "adambridge_embed"},
+        {&found.embed_work, "adambridge_embed_work"}, {&found.embed_backward, "adambridge_embed_backward"}};
     for (const auto& e : entries) {
         PyObject* o = PyDict_GetItemString(args[0], e.name);
         void* const p = o ? PyLong_AsVoidPtr(o) : nullptr;
@@ -561,6 +640,7 @@ PyMethodDef kMethods[] = {
     {"dispatch", ABH_FAST(dispatch), "dispatch(x, position); None if the call is not an ordinary one."},
     {"combine", ABH_FAST(combine), "combine(rows, weights, position); None if the call is not an ordinary one."},
     {"expert_mm", ABH_FAST(expert_mm), "expert_mm(x, weight, ends); None if the call is not an ordinary one."},
+    {"embed", ABH_FAST(embed), "embed(ids, weight, scale, padding_idx); None if the call is not an ordinary one."},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_ops", "The host's side of an expert block's operators.", -1, kMethods,

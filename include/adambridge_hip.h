@@ -563,6 +563,20 @@ ADAMBRIDGE_API int adambridge_expert_mm_dx(const void* gout, const void* weight,
 ADAMBRIDGE_API int adambridge_expert_mm_dw(const void* gout, const void* x, const int32_t* ends, void* dw, int32_t dtype,
                                            int64_t rows, int64_t experts, int64_t n, int64_t k, void* work);
 
+/* A language model's ends.  The reference has none of it but the loss above; types, addresses, sums, streams and codes as
+ * those of the expert block's operators. */
+
+/* embed: y[i] = scale weight[ids[i]] for tokens (1 .. 2^30) ids of id_bytes (4 or 8, whole numbers; else
+ * ADAMBRIDGE_EMVDTYPE), weight: vocab x hidden (1 .. 2^30, 1 .. 2^22); an id outside the vocabulary gives a row of NaN (nothing is read for
+ * it).  The backward call writes all of dweight, vocab x hidden: scale times the sum of the rows of gout, tokens x hidden,
+ * whose id is the word, zeros without any and for the word `padding` (-1: none); rows of ids outside the vocabulary are
+ * left out.  work: adambridge_embed_work bytes, 8-byte aligned. */
+ADAMBRIDGE_API int adambridge_embed(const void* ids, int32_t id_bytes, int64_t tokens, const void* weight, int32_t dtype,
+                                    int64_t vocab, int64_t hidden, float scale, void* y);
+ADAMBRIDGE_API int64_t adambridge_embed_work(int64_t tokens, int64_t vocab, int64_t hidden);
+ADAMBRIDGE_API int adambridge_embed_backward(const void* ids, int32_t id_bytes, int64_t tokens, const void* gout, int32_t dtype,
+                                             int64_t vocab, int64_t hidden, float scale, int64_t padding, void* dweight, void* work);
+
 #ifdef __cplusplus
 }
 #endif
