@@ -20,6 +20,7 @@
 #include <stdint.h>
 
 #include "../../include/adambridge_hip.h"
+#include "abh_choice.hpp"
 #include "abh_device.hpp"
 #include "abh_host.hpp"
 #include "abh_rows.hpp"
@@ -30,8 +31,6 @@ constexpr int kBlockTokens = 64;
 constexpr int kRouteThreads = 1024;   // so that a block of tokens is chosen from in few passes: blocks are few
 constexpr int kMostExperts = 1024;
 constexpr int kMostChosen = 64;
-constexpr float kRouteLog2e = 1.4426950408889634f;
-constexpr float kRouteNegInf = -__builtin_inff();
 
 struct RouteArgs {
     const void* logits;
@@ -45,33 +44,6 @@ struct RouteArgs {
     uint8_t* counts;     // experts x blocks
     int32_t* bases;      // experts x blocks
 };
-
-// A total order of floats as integers: -inf lowest but 0 (nothing), +0 and -0 equal, NaN above all.
-__device__ __forceinline__ uint32_t order_key(float x)
-{
-    if (x != x) return 0xffffffffu;
-    const uint32_t u = fbits(x + 0.0f);
-    return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-
-__device__ __forceinline__ float key_value(uint32_t key)
-{
-    return key == 0xffffffffu ? __builtin_nanf("") : bitsf(key & 0x80000000u ? key & 0x7fffffffu : ~key);
-}
-
-// exp(x - m) with m = -inf taken as 0, so that a row without any finite logit has weights 0 and not NaN.  x - m and its
-// product with log2 e are rounded to FP32: the largest weight's exponential is exact, one of e^-8 is off by at most 2^-20 of
-// itself, one near FP32's smallest, e^-87, by 2^-17.
-__device__ __forceinline__ float exp_below(float x, float m)
-{
-    return __builtin_amdgcn_exp2f((x - (m == kRouteNegInf ? 0.0f : m)) * kRouteLog2e);
-}
-
-template <int G>
-__device__ __forceinline__ uint32_t group_max(uint32_t x)
-{
-    return group_reduce<G>(x, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-}
 
 // Masks of a block's tokens by expert, and the rows of its assignments: base[e] + the bits below.
 __device__ __forceinline__ void place_block(const RouteArgs& A, const uint64_t* mask, const int32_t* base, int64_t base_stride,
