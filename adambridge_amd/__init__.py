@@ -8,12 +8,12 @@ of parameters per launch.  The public API mirrors the reference package
 
 from . import native, precision
 from .engine import StepStats
-from .experts import Routing, combine, dispatch, expert_mm, route
+from .experts import Routing, combine, dispatch, expert_mlp, expert_mm, route
 from .losses import causal_lm_loss
 from .norms import layer_norm
 from .optimizer import AdamBridge, AutoTuneConfig, LionBridge, OptiComputeAdamW
 from .precision import bytes_per_param
-from .vocabulary import embed
+from .vocabulary import embed, token_losses
 
 __version__ = "0.1.0"
 
@@ -31,7 +31,9 @@ __all__ = [
     "dispatch",
     "expert_mm",
     "combine",
+    "expert_mlp",
     "embed",
+    "token_losses",
     "native",
     "precision",
     "__version__",

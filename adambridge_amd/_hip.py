@@ -126,7 +126,9 @@ EXPORTS = (
     "adambridge_route", "adambridge_route_backward", "adambridge_dispatch", "adambridge_combine",
     "adambridge_combine_backward", "adambridge_expert_mm", "adambridge_expert_mm_dx",
     "adambridge_expert_mm_work", "adambridge_expert_mm_dw", "adambridge_embed", "adambridge_embed_work",
-    "adambridge_embed_backward",
+    "adambridge_embed_backward", "adambridge_token_losses", "adambridge_token_losses_work",
+    "adambridge_token_losses_backward", "adambridge_token_losses_backward_work", "adambridge_expert_mlp",
+    "adambridge_expert_mlp_work",
 )
 
 
@@ -190,6 +192,12 @@ def open_library(path: Path = LIB_PATH) -> ctypes.CDLL:
         "adambridge_embed": (ctypes.c_int, [vp, i32, i64, vp, i32, i64, i64, ctypes.c_float, vp]),
         "adambridge_embed_work": (i64, [i64, i64, i64]),
         "adambridge_embed_backward": (ctypes.c_int, [vp, i32, i64, vp, i32, i64, i64, ctypes.c_float, i64, vp, vp]),
+        "adambridge_token_losses": (ctypes.c_int, [vp, vp, i32, vp, i64, i64, i64, i64, vp, vp, vp]),
+        "adambridge_token_losses_work": (i64, [i32, i64, i64, i64]),
+        "adambridge_token_losses_backward": (ctypes.c_int, [vp, vp, vp, i32, vp, i64, i64, i64, i64, vp, vp, vp, vp]),
+        "adambridge_token_losses_backward_work": (i64, [i32, i64, i64, i64]),
+        "adambridge_expert_mlp": (ctypes.c_int, [vp, vp, i32, vp, vp, vp, i32, i64, i64, i64, i64, i64, i32, i32, vp, vp]),
+        "adambridge_expert_mlp_work": (i64, [i32, i64, i64, i64, i64, i64]),
     }
     for name in EXPORTS:
         fn = getattr(lib, name)

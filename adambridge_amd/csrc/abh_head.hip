@@ -1,0 +1,746 @@
+// abh_head.hip -- each row's cross-entropy over a vocabulary, from the rows before the head's product, and its gradients.
+//
+//   x[t, v]  = <h[t], W[v]>
+//   loss[t]  = log(sum over v of exp x[t, v]) - x[t, target[t]]
+//   G[t, v]  = gout[t] (exp(x[t, v]) / sum - [v = target[t]]),   dh = G W,   dW = G^T h
+//
+// No logit is kept.  Forward, a tile of the product ends in its rows' maxima and sums of exponentials, 8 bytes a row and
+// tile, which are merged in order; the logits are the products' FP32 sums, never rounded.  Backward, the vocabulary goes by
+// in pieces: a piece's logits are computed again and end as G (in the operands' type: its rounding is the only one between
+// the sums, and what a matrix product of that type takes), then the piece's rows of dW are G^T h, written once, and
+// dh's FP32 sums grow by G W.  So each piece of W is read once for all rows, where slices of rows would read W, and
+// add to dW, once a slice.
+//
+// Rows that are not scored cost nothing and reach nothing, whatever they hold: the scored ones are copied together first, and the
+// products end with them (how many they are is known on the device only).  The matrix products bound all of it (6 T H V operations forward
+// and backward and 2 T H V for the logits again); a few rows are the weights read once, which HBM bounds.
+
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "../../include/adambridge_hip.h"
+#include "abh_device.hpp"
+#include "abh_host.hpp"
+#include "abh_rows.hpp"
+#include "abh_tiles.hpp"
+
+namespace abh {
+
+constexpr float kHeadLog2e = 1.4426950408889634f;
+constexpr float kHeadNegInf = -__builtin_inff();
+constexpr int kHeadCus = 256;
+constexpr int kFewRows = 64;         // at most, for k_head_few
+constexpr int kFinishLanes = 1024;
+
+// A maximum and the sum of exp(x - m) over what was seen.  m = -inf: nothing above -inf yet.
+struct Sums {
+    float m, s;
+};
+
+__device__ __forceinline__ float exp_of(float x, float m) { return __builtin_amdgcn_exp2f((x - m) * kHeadLog2e); }
+// The subtrahend that stands for a maximum, so that exp(-inf + inf) is never taken.
+__device__ __forceinline__ float shift_for(float m) { return m == kHeadNegInf ? 0.0f : m; }
+
+__device__ __forceinline__ Sums merged(const Sums a, const Sums b)
+{
+    const float m = __builtin_fmaxf(a.m, b.m), t = shift_for(m);
+    return Sums{m, a.s * exp_of(a.m, t) + b.s * exp_of(b.m, t)};
+}
+
+struct HeadArgs {
+    const void* h;            // the scored rows, together: count x hidden
+    const void* w;            // vocab x hidden
+    const int64_t* targets;   // of all rows
+    const int32_t* index;     // a scored row's number among all
+    const int32_t* count;     // how many are scored
+    int32_t rows, hidden;     // rows: all
+    int64_t vocab, v0;        // the piece: words v0 .. v0 + width
+    int32_t width, pitch;     // pitch: a row of G
+    int32_t tiles_j;
+    Sums* part;               // column tiles x rows
+    float* picked;            // a scored row's logit of its target
+    const float* stats;       // of all rows: maximum, 1 / sum
+    const float* gout;        // of all rows
+    void* g;                  // count x pitch
+    float* dh;                // parts x count x hidden
+    void* dw;                 // vocab x hidden
+    int32_t fresh;            // dh's first piece
+};
+
+// ------------------------------------------------------------------------ the scored rows
+
+// index[i] = the i-th scored row, place[t] = its number or -1; losses of the others are 0.  One workgroup.
+__global__ __launch_bounds__(1024) void k_head_rows(const int64_t* targets, int64_t ignore, int32_t rows, int32_t* index, int32_t* place,
+                                                    int32_t* count, float* losses)
+{
+    __shared__ int32_t waves[2][16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
+    int32_t before = 0;
+    for (int32_t t0 = 0, turn = 0; t0 < rows; t0 += 1024, turn ^= 1) {
+        const int32_t t = t0 + (int32_t)threadIdx.x;
+        const bool scored = t < rows && targets[t] != ignore;
+        const uint64_t mask = __builtin_amdgcn_ballot_w64(scored);
+        if (lane == 0) waves[turn][wave] = __builtin_popcountll(mask);
+        __syncthreads();
+        int32_t at = before, all = 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            const int32_t n = waves[turn][w];
+            at += w < wave ? n : 0;
+            all += n;
+        }
+        before += all;
+        at += __builtin_popcountll(mask & (((uint64_t)1 << lane) - 1));
+        if (scored) index[at] = t;
+        if (t < rows) {
+            if (place) place[t] = scored ? at : -1;
+            if (losses && !scored) losses[t] = 0.0f;
+        }
+    }
+    if (threadIdx.x == 0) *count = before;
+}
+
+// The scored rows of h, together.
+template <int DT>
+__global__ __launch_bounds__(256) void k_head_gather(const void* h, const int32_t* index, const int32_t* count, int32_t hidden, void* out)
+{
+    constexpr int L = kLane<DT>;
+    const int64_t i = block_index();
+    if (i >= *count) return;
+    const void* from = at<DT>(h, (int64_t)index[i] * hidden);
+    void* to = at<DT>(out, i * hidden);
+    for (int32_t c = threadIdx.x * L; c < hidden; c += 256 * L) {
+        if (c + L <= hidden) {
+            store_raw<DT>(to, c, load_raw<DT>(from, c));
+        } else {
+            for (int32_t k = c; k < hidden; ++k) put<DT>(to, k, get<DT>(from, k));
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------ tiles
+
+struct HeadTile {
+    int ti, tj, split;
+};
+
+// This workgroup's of tiles_i x tiles_j tiles in `splits` parts: consecutive ones to one XCD, kGroupTiles row tiles at a time
+// down the columns.
+__device__ __forceinline__ bool head_tile(int tiles_i, int tiles_j, int splits, HeadTile& t)
+{
+    const int items = tiles_i * tiles_j * splits, per = (items + kXcd - 1) / kXcd;
+    const int block = (int)block_index(), slot = block / kXcd, item = block % kXcd * per + slot;
+    if (slot >= per || item >= items) return false;
+    const int idx = item / splits;
+    t.split = scalar(item - idx * splits);
+    const int g = idx / (kGroupTiles * tiles_j), first = g * kGroupTiles;
+    const int wide = tiles_i - first < kGroupTiles ? tiles_i - first : kGroupTiles;
+    const int r = idx - first * tiles_j;
+    t.ti = scalar(first + r % wide);
+    t.tj = scalar(r / wide);
+    return true;
+}
+
+// What a kernel's type and tile are.  BF16: abh_tiles.hpp's; FP32: B x B of four wavefronts.
+template <class C_, bool EVEN_>
+struct HeadBf16 {
+    typedef C_ C;
+    static constexpr int DT = DT_BF16, BM = C::BM, BN = C::BN, BK = C::BK, NI = C::NI, NJ = C::NJ, WJ = C::WJ, T = C::T, OCC = C::OCC;
+    static constexpr bool EVEN = EVEN_;
+    static constexpr int LDS = C::NB * C::BYTES;
+    static __device__ __forceinline__ int wi() { return (int)threadIdx.x / kWave / WJ * (BM / C::WI); }
+    static __device__ __forceinline__ int wj() { return (int)threadIdx.x / kWave % WJ * (BN / WJ); }
+};
+template <int B>
+struct HeadF32 {
+    static constexpr int DT = DT_F32, BM = B, BN = B, BK = 32, NI = B / 64, NJ = B / 64, WJ = 2, T = 256, OCC = 2;
+    static constexpr bool EVEN = false;
+    static constexpr int LDS = 2 * 2 * B * 32 * 4;
+    static __device__ __forceinline__ int wi() { return (int)(threadIdx.x / kWave & 1) * (B / 2); }
+    static __device__ __forceinline__ int wj() { return (int)(threadIdx.x / kWave >> 1) * (B / 2); }
+};
+
+// One operand of a tile.  LONG: p is its first row, `rows` of them are left; else p is the operand's first term, its rows have
+// `rows` values and the tile begins at `first`.  len: terms.
+struct Operand {
+    const uint8_t* p;
+    int pitch, first, rows, len;
+};
+
+// The tile's sums; false where the wavefront has no row.
+template <class H, bool ALONG, bool BLONG>
+__device__ __forceinline__ bool head_multiply(uint8_t* lds, const Operand& a, const Operand& b, bool live, mm_f32x16 (&acc)[H::NI][H::NJ])
+{
+    const int steps = ((a.len > b.len ? a.len : b.len) + H::BK - 1) / H::BK;
+    if constexpr (H::DT == DT_BF16) {
+        typedef typename H::C C;
+        TileFeed<ALONG, H::BM, H::BK, C::W, H::EVEN> fa;
+        TileFeed<BLONG, H::BN, H::BK, C::W, H::EVEN> fb;
+        if constexpr (H::EVEN) {
+            fa.start(ALONG ? a.p : a.p + (int64_t)a.first * 2, a.pitch * 2, a.rows, a.len, ALONG ? 0 : a.first * 2);
+            fb.start(BLONG ? b.p : b.p + (int64_t)b.first * 2, b.pitch * 2, b.rows, b.len, BLONG ? 0 : b.first * 2);
+        } else {
+            fa.start(a.p, a.pitch, ALONG ? 0 : a.first, a.rows, a.len);
+            fb.start(b.p, b.pitch, BLONG ? 0 : b.first, b.rows, b.len);
+        }
+        return multiply_tile<C, ALONG, BLONG, H::EVEN>(lds, fa, fb, steps, H::wi(), H::wj(), live, acc);
+    } else {
+        StagedFeed<DT_F32, ALONG, H::BM, 32, 4> fa;
+        StagedFeed<DT_F32, BLONG, H::BN, 32, 4> fb;
+        fa.start(a.p, a.pitch, ALONG ? 0 : a.first, a.rows, a.len);
+        fb.start(b.p, b.pitch, BLONG ? 0 : b.first, b.rows, b.len);
+        multiply_tile_f32<H::BM, ALONG, BLONG>(*reinterpret_cast<uint8_t(*)[2][2 * H::BM * 32 * 4]>(lds), fa, fb, steps, H::wi(), H::wj(), acc);
+        return true;
+    }
+}
+
+// Column of the tile that is a lane's value r of its columns j.
+__device__ __forceinline__ int column_of(int wj, int j, int r) { return wj + 32 * j + 8 * (r >> 2) + 4 * (int)((threadIdx.x & 63) >> 5) + (r & 3); }
+
+// ------------------------------------------------------------------------------ forward
+
+// Each row's maximum and sum over the tile's words, and the target's logit.
+template <class H>
+__global__ __launch_bounds__(H::T, H::OCC) void k_head_sums(HeadArgs A)
+{
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[H::LDS];
+    __shared__ Sums row_sums[H::WJ][H::BM];
+    const int count = scalar(*A.count);
+    HeadTile t;
+    if (!head_tile((count + H::BM - 1) / H::BM, A.tiles_j, 1, t)) return;
+    const int i0 = t.ti * H::BM, j0 = t.tj * H::BN, limit_i = count - i0, limit_j = A.width - j0;
+    const Operand a{at<H::DT>(A.h, (int64_t)i0 * A.hidden), A.hidden, 0, limit_i, A.hidden};
+    const Operand b{at<H::DT>(A.w, (A.v0 + j0) * A.hidden), A.hidden, 0, limit_j, A.hidden};
+    mm_f32x16 acc[H::NI][H::NJ];
+    const int wi = H::wi(), wj = H::wj(), lane = threadIdx.x & 63;
+    const bool live = head_multiply<H, true, true>(lds, a, b, wi < limit_i, acc);
+    if (live) {
+#pragma unroll
+        for (int i = 0; i < H::NI; ++i) {
+            const int row = wi + 32 * i + (lane & 31);
+            const int64_t target = row < limit_i ? A.targets[A.index[i0 + row]] - j0 : -1;
+            float m = kHeadNegInf;
+#pragma unroll
+            for (int j = 0; j < H::NJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int c = column_of(wj, j, r);
+                    if (c == target && c < limit_j) A.picked[i0 + row] = acc[i][j][r];
+                    if (c >= limit_j) acc[i][j][r] = kHeadNegInf;
+                    m = __builtin_fmaxf(m, acc[i][j][r]);
+                }
+            m = __builtin_fmaxf(m, __shfl_xor(m, 32));
+            const float shift = shift_for(m);
+            float s = 0.0f;
+#pragma unroll
+            for (int j = 0; j < H::NJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s += exp_of(acc[i][j][r], shift);
+            s += __shfl_xor(s, 32);
+            if (lane < 32) row_sums[wj / (H::BN / H::WJ)][row] = Sums{m, s};
+        }
+    }
+    __syncthreads();
+    for (int row = threadIdx.x; row < H::BM && row < limit_i; row += H::T) {
+        Sums all = row_sums[0][row];
+#pragma unroll
+        for (int w = 1; w < H::WJ; ++w) all = merged(all, row_sums[w][row]);
+        A.part[(int64_t)t.tj * A.rows + i0 + row] = all;
+    }
+}
+
+// The same of few rows: the weights are read once, 16 words a wavefront.  part: workgroups x rows.
+template <int DT, bool EVEN>
+__global__ __launch_bounds__(256) void k_head_few(HeadArgs A)
+{
+    constexpr int V = kLane<DT>, STEP = 4 * V, CH = kFewRows / 16, U = 8;
+    __shared__ Sums row_sums[4][kFewRows];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+    const int col = lane & 15, quarter = lane >> 4;
+    const int64_t j0 = (block_index() * 4 + wave) * 16;
+    const int words = j0 >= A.vocab ? 0 : (int)(A.vocab - j0 < 16 ? A.vocab - j0 : 16);
+    const int steps = (A.hidden + STEP - 1) / STEP;
+    const Pieces<DT, EVEN> w{at<DT>(A.w, (words ? j0 : 0) * A.hidden), (uint32_t)(words * A.hidden * kSize<DT>), A.hidden, words};
+    const Pieces<DT, EVEN> x{static_cast<const uint8_t*>(A.h), (uint32_t)(A.rows * A.hidden * kSize<DT>), A.hidden, A.rows};
+    mm_f32x4 acc[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c) acc[c] = mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (words)
+        for (int s = 0; s < steps; s += U) {
+            raw16 wv[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) wv[u] = w.load(col, (s + u) * STEP + quarter * V, s + u < steps);
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                if (16 * c >= A.rows) break;
+                raw16 xv[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) xv[u] = x.load(16 * c + col, (s + u) * STEP + quarter * V, s + u < steps);
+                mm_f32x4 some = DT == DT_BF16 ? acc[c] : mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};   // FP32: short chains of sums
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if constexpr (DT == DT_BF16) {
+                        some = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mm_bf16x8, wv[u]),
+                                                                       __builtin_bit_cast(mm_bf16x8, xv[u]), some, 0, 0, 0);
+                    } else {
+                        const mm_f32x4 wf = __builtin_bit_cast(mm_f32x4, wv[u]), xf = __builtin_bit_cast(mm_f32x4, xv[u]);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) some = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[q], xf[q], some, 0, 0, 0);
+                    }
+                }
+                if constexpr (DT == DT_BF16) acc[c] = some;
+                else acc[c] += some;
+            }
+        }
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+        if (16 * c >= A.rows) break;
+        const int row = 16 * c + col;
+        const int64_t target = row < A.rows ? A.targets[row] - j0 : -1;
+        Sums all{kHeadNegInf, 0.0f};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int word = 4 * quarter + r;
+            if (word >= words) acc[c][r] = kHeadNegInf;
+            else if (word == target) A.picked[row] = acc[c][r];
+            all.m = __builtin_fmaxf(all.m, acc[c][r]);
+        }
+        all.m = __builtin_fmaxf(all.m, __shfl_xor(all.m, 16));
+        all.m = __builtin_fmaxf(all.m, __shfl_xor(all.m, 32));
+        const float shift = shift_for(all.m);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) all.s += exp_of(acc[c][r], shift);
+        all.s += __shfl_xor(all.s, 16);
+        all.s += __shfl_xor(all.s, 32);
+        if (quarter == 0) row_sums[wave][row] = all;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < A.rows) {
+        Sums all = row_sums[0][threadIdx.x];
+#pragma unroll
+        for (int k = 1; k < 4; ++k) all = merged(all, row_sums[k][threadIdx.x]);
+        A.part[block_index() * A.rows + threadIdx.x] = all;
+    }
+}
+
+// The parts of R rows a workgroup, in an order of their own; losses, and what the gradient takes.  index: NULL where the parts'
+// rows are all rows.
+template <int R>
+__global__ __launch_bounds__(kFinishLanes) void k_head_finish(const Sums* part, int32_t parts, int32_t stride, const int32_t* index, const int32_t* count,
+                                                              const int64_t* targets, int64_t vocab, int64_t ignore, const float* picked, float* losses,
+                                                              float* stats)
+{
+    constexpr int S = kFinishLanes / R;
+    __shared__ Sums tree[S][R];
+    const int r = threadIdx.x % R, slice = threadIdx.x / R;
+    const int64_t row = block_index() * R + r, rows = index ? *count : stride;
+    if (block_index() * R >= rows) return;
+    Sums all{kHeadNegInf, 0.0f};
+    if (row < rows)
+        for (int32_t p = slice; p < parts; p += S) all = merged(all, part[(int64_t)p * stride + row]);
+    tree[slice][r] = all;
+    __syncthreads();
+#pragma unroll
+    for (int d = S / 2; d > 0; d >>= 1) {
+        if (slice < d) tree[slice][r] = merged(tree[slice][r], tree[slice + d][r]);
+        __syncthreads();
+    }
+    if (slice || row >= rows) return;
+    all = tree[0][r];
+    if (all.m == kHeadNegInf) all.s = __builtin_nanf("");   // every logit -inf: no distribution
+    const int64_t t = index ? index[row] : row, target = targets[t];
+    if (stats) {
+        stats[2 * t] = all.m;
+        stats[2 * t + 1] = 1.0f / all.s;
+    }
+    losses[t] = target == ignore ? 0.0f : target < 0 || target >= vocab ? __builtin_nanf("") : logf(all.s) - (picked[row] - all.m);
+}
+
+// ------------------------------------------------------------------------------ backward
+
+// A piece's gradient at the logits.
+template <class H>
+__global__ __launch_bounds__(H::T, H::OCC) void k_head_grad(HeadArgs A)
+{
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[H::LDS];
+    const int count = scalar(*A.count);
+    HeadTile t;
+    if (!head_tile((count + H::BM - 1) / H::BM, A.tiles_j, 1, t)) return;
+    const int i0 = t.ti * H::BM, j0 = t.tj * H::BN, limit_i = count - i0, limit_j = A.width - j0;
+    const Operand a{at<H::DT>(A.h, (int64_t)i0 * A.hidden), A.hidden, 0, limit_i, A.hidden};
+    const Operand b{at<H::DT>(A.w, (A.v0 + j0) * A.hidden), A.hidden, 0, limit_j, A.hidden};
+    mm_f32x16 acc[H::NI][H::NJ];
+    const int wi = H::wi(), wj = H::wj(), lane = threadIdx.x & 63;
+    if (!head_multiply<H, true, true>(lds, a, b, wi < limit_i, acc)) return;
+#pragma unroll
+    for (int i = 0; i < H::NI; ++i) {
+        const int row = wi + 32 * i + (lane & 31);
+        const bool real = row < limit_i;
+        const int64_t at_row = real ? A.index[i0 + row] : 0;
+        const int64_t target = A.targets[at_row];
+        const float m = A.stats[2 * at_row], g = target < 0 || target >= A.vocab ? __builtin_nanf("") : A.gout[at_row];
+        const float f = A.stats[2 * at_row + 1] * g;
+        const int64_t hot = target - A.v0 - j0;
+#pragma unroll
+        for (int j = 0; j < H::NJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int c = column_of(wj, j, r);
+                const float p = exp_of(acc[i][j][r], m) * f;
+                acc[i][j][r] = c >= limit_j ? 0.0f : c == hot ? p - g : p;
+            }
+    }
+    const int wide = (limit_j + 7) & ~7;   // whole pieces: zeros behind the vocabulary's last word
+    if constexpr (H::DT == DT_BF16) {
+        store_bf16<typename H::C, true>(at<DT_BF16>(A.g, (int64_t)i0 * A.pitch + j0), A.pitch, limit_i, wide, acc, wi, wj);
+    } else {
+#pragma unroll
+        for (int i = 0; i < H::NI; ++i) {
+            const int row = wi + 32 * i + (lane & 31);
+            if (row >= limit_i) continue;
+            float* out = static_cast<float*>(A.g) + (int64_t)(i0 + row) * A.pitch + j0;
+#pragma unroll
+            for (int j = 0; j < H::NJ; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int c = column_of(wj, j, 4 * q);
+                    if (c < wide) *reinterpret_cast<mm_f32x4*>(out + c) = mm_f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                }
+        }
+    }
+}
+
+// How many parts dh's sums are cut in: so that the tiles fill the CUs, of 16 steps or more.
+__device__ __host__ __forceinline__ int dh_splits(int64_t tiles, int width)
+{
+    const int64_t fit = kHeadCus / (tiles < 1 ? 1 : tiles), most = width / 512;
+    const int64_t n = fit < most ? fit : most;
+    return (int)(n < 1 ? 1 : n);
+}
+
+// dh (FP32) += G W of a piece.
+template <class H>
+__global__ __launch_bounds__(H::T, H::OCC) void k_head_dh(HeadArgs A)
+{
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[H::LDS];
+    const int count = scalar(*A.count), tiles_i = (count + H::BM - 1) / H::BM;
+    const int splits = dh_splits((int64_t)tiles_i * A.tiles_j, A.pitch);   // by the pitch: the same for every piece
+    HeadTile t;
+    if (!head_tile(tiles_i, A.tiles_j, splits, t)) return;
+    const int i0 = t.ti * H::BM, j0 = t.tj * H::BN, limit_i = count - i0, limit_j = A.hidden - j0;
+    const int steps = (A.width + H::BK - 1) / H::BK;
+    const int k0 = scalar(steps * t.split / splits * H::BK), k1 = scalar(steps * (t.split + 1) / splits * H::BK);
+    const int len = (k1 < A.width ? k1 : A.width) - k0;
+    if (len <= 0 && !A.fresh) return;
+    // G has zeros up to whole pieces, where W has ended
+    const Operand a{at<H::DT>(A.g, (int64_t)i0 * A.pitch + k0), A.pitch, 0, limit_i, (len + 7) & ~7};
+    const Operand b{at<H::DT>(A.w, (A.v0 + k0) * A.hidden), A.hidden, j0, A.hidden, len};
+    mm_f32x16 acc[H::NI][H::NJ];
+    const int wi = H::wi(), wj = H::wj(), lane = threadIdx.x & 63;
+    if (!head_multiply<H, true, false>(lds, a, b, wi < limit_i, acc)) return;
+    float* out = A.dh + ((int64_t)t.split * count + i0) * A.hidden + j0;
+#pragma unroll
+    for (int i = 0; i < H::NI; ++i) {
+        const int row = wi + 32 * i + (lane & 31);
+        if (row >= limit_i) continue;
+#pragma unroll
+        for (int j = 0; j < H::NJ; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int c = column_of(wj, j, 4 * q);
+                float four[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                if (!A.fresh) {
+                    float old[4];
+                    load_like<DT_F32, 4>(out + (int64_t)row * A.hidden, c, limit_j, 0.0f, old);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) four[k] += old[k];
+                }
+                store_like<DT_F32, 4>(out + (int64_t)row * A.hidden, c, limit_j, four);
+            }
+    }
+}
+
+// A piece's rows of dW.
+template <class H>
+__global__ __launch_bounds__(H::T, H::OCC) void k_head_dw(HeadArgs A)
+{
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[H::LDS];
+    const int count = scalar(*A.count);
+    HeadTile t;
+    if (!head_tile((A.width + H::BM - 1) / H::BM, A.tiles_j, 1, t)) return;
+    const int i0 = t.ti * H::BM, j0 = t.tj * H::BN, limit_i = A.width - i0, limit_j = A.hidden - j0;
+    const Operand a{static_cast<const uint8_t*>(A.g), A.pitch, i0, A.pitch, count};
+    const Operand b{static_cast<const uint8_t*>(A.h), A.hidden, j0, A.hidden, count};
+    mm_f32x16 acc[H::NI][H::NJ];
+    const int wi = H::wi(), wj = H::wj(), lane = threadIdx.x & 63;
+    if (!head_multiply<H, false, false>(lds, a, b, wi < limit_i, acc)) return;
+    uint8_t* out = at<H::DT>(A.dw, (A.v0 + i0) * A.hidden + j0);
+    if constexpr (H::DT == DT_BF16) {
+        store_bf16<typename H::C, H::EVEN>(out, A.hidden, limit_i, limit_j, acc, wi, wj);
+    } else {
+#pragma unroll
+        for (int i = 0; i < H::NI; ++i) {
+            const int row = wi + 32 * i + (lane & 31);
+            if (row >= limit_i) continue;
+#pragma unroll
+            for (int j = 0; j < H::NJ; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float four[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                    store_like<DT_F32, 4>(reinterpret_cast<float*>(out) + (int64_t)row * A.hidden, column_of(wj, j, 4 * q), limit_j, four);
+                }
+        }
+    }
+}
+
+// dh's rows at their places, the parts summed in order and rounded once; zeros for rows that are not scored.
+template <int DT>
+__global__ __launch_bounds__(256) void k_head_scatter(const float* sums, const int32_t* place, const int32_t* count, int32_t rows, int32_t hidden,
+                                                      int32_t tile, int32_t width, void* dh)
+{
+    constexpr int L = kLane<DT>;
+    const int64_t t = block_index();
+    if (t >= rows) return;
+    const int n = *count, p = place[t];
+    const int64_t tiles = (int64_t)((n + tile - 1) / tile) * ((hidden + tile - 1) / tile);
+    const int splits = dh_splits(tiles, width);
+    void* out = at<DT>(dh, t * hidden);
+    for (int32_t c = threadIdx.x * L; c < hidden; c += 256 * L) {
+        float x[L];
+#pragma unroll
+        for (int k = 0; k < L; ++k) x[k] = 0.0f;
+        if (p >= 0)
+            for (int s = 0; s < splits; ++s) {
+                float y[L];
+                load_like<DT_F32, L>(sums + ((int64_t)s * n + p) * hidden, c, hidden, 0.0f, y);
+#pragma unroll
+                for (int k = 0; k < L; ++k) x[k] += y[k];
+            }
+        stream_vec<DT>(out, c, hidden, x);
+    }
+}
+
+// ------------------------------------------------------------------------------ launches
+
+constexpr int64_t kHeadRows = (int64_t)1 << 23, kHeadVocab = (int64_t)1 << 22, kHeadHidden = (int64_t)1 << 20;
+constexpr int64_t kPieceValues = (int64_t)1 << 28, kLeastPiece = 4096;   // of G
+
+static int head_check(int32_t dtype, int64_t rows, int64_t vocab, int64_t hidden)
+{
+    if (dtype != ADAMBRIDGE_DT_F32 && dtype != ADAMBRIDGE_DT_BF16) return ADAMBRIDGE_EMVDTYPE;
+    const int piece = dtype == ADAMBRIDGE_DT_BF16 ? 8 : 4;
+    if (rows < 1 || rows > kHeadRows || vocab < 1 || vocab > kHeadVocab || hidden < piece || hidden > kHeadHidden) return ADAMBRIDGE_EBADN;
+    return 0;
+}
+
+static int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+// Scratch, handed out in whole 256 bytes.
+struct Scratch {
+    uint8_t* base;
+    int64_t used = 0;
+    template <class T>
+    T* take(int64_t n)
+    {
+        T* p = reinterpret_cast<T*>(base + used);
+        used += up(n * (int64_t)sizeof(T), 256);
+        return p;
+    }
+};
+
+// Sides of the FP32 tiles: as the expert products' rule, 64 where tiles of 128 are few.
+static int f32_tile(int64_t tiles_of_128) { return tiles_of_128 < 512 ? 64 : 128; }
+
+// The forward call's plan and scratch.
+struct HeadForward {
+    bool few;
+    int tile, parts;
+    int32_t *index, *count;
+    float* picked;
+    Sums* part;
+    void* h;
+    int64_t bytes;
+    HeadForward(void* work, int32_t dtype, int64_t rows, int64_t vocab, int64_t hidden)
+    {
+        few = rows <= kFewRows;
+        tile = dtype == ADAMBRIDGE_DT_BF16 ? LargeTile::BM : f32_tile((rows + 127) / 128 * ((vocab + 127) / 128));
+        parts = (int)(few ? (vocab + 63) / 64 : (vocab + tile - 1) / tile);
+        Scratch s{static_cast<uint8_t*>(work)};
+        picked = s.take<float>(rows);
+        part = s.take<Sums>(parts * rows);
+        index = few ? nullptr : s.take<int32_t>(rows);
+        count = few ? nullptr : s.take<int32_t>(1);
+        h = few ? nullptr : s.take<uint8_t>(rows * hidden * (dtype == ADAMBRIDGE_DT_BF16 ? 2 : 4));
+        bytes = s.used;
+    }
+};
+
+// The backward call's.
+struct HeadBackward {
+    int tile, dh_tile;
+    int32_t pitch;   // words of a piece
+    int32_t *index, *place, *count;
+    void *h, *g;
+    float* dh;
+    int64_t bytes;
+    HeadBackward(void* work, int32_t dtype, int64_t rows, int64_t vocab, int64_t hidden)
+    {
+        const bool bf = dtype == ADAMBRIDGE_DT_BF16;
+        const int64_t size = bf ? 2 : 4, most = std::max(kPieceValues / rows, kLeastPiece), pieces = (vocab + most - 1) / most;
+        pitch = (int32_t)up((vocab + pieces - 1) / pieces, 256);
+        tile = bf ? LargeTile::BM : f32_tile((rows + 127) / 128 * ((std::min<int64_t>(pitch, vocab) + 127) / 128));
+        dh_tile = bf ? LargeTile::BM : f32_tile((rows + 127) / 128 * ((hidden + 127) / 128));
+        Scratch s{static_cast<uint8_t*>(work)};
+        index = s.take<int32_t>(rows);
+        place = s.take<int32_t>(rows);
+        count = s.take<int32_t>(1);
+        h = s.take<uint8_t>(rows * hidden * size);
+        g = s.take<uint8_t>(rows * pitch * size);
+        // parts x rows x hidden: as many as fill the CUs with tiles, or one
+        dh = s.take<float>(std::max(rows * hidden, (int64_t)kHeadCus * dh_tile * dh_tile));
+        bytes = s.used;
+    }
+};
+
+static dim3 tile_grid(int64_t tiles) { return block_grid(up(tiles, kXcd)); }
+
+#define ABH_HEAD_LAUNCH(KERNEL, TILE, EVEN, GRID)                                                                             \
+    do {                                                                                                                      \
+        if (bf && (EVEN)) hipLaunchKernelGGL((KERNEL<HeadBf16<LargeTile, true>>), GRID, dim3(LargeTile::T), 0, t_stream, A);  \
+        else if (bf) hipLaunchKernelGGL((KERNEL<HeadBf16<LargeTile, false>>), GRID, dim3(LargeTile::T), 0, t_stream, A);      \
+        else if ((TILE) == 128) hipLaunchKernelGGL((KERNEL<HeadF32<128>>), GRID, dim3(256), 0, t_stream, A);                  \
+        else hipLaunchKernelGGL((KERNEL<HeadF32<64>>), GRID, dim3(256), 0, t_stream, A);                                      \
+    } while (0)
+
+static void launch_gather(bool bf, int64_t rows, const void* hidden_rows, const int32_t* index, const int32_t* count, int64_t hidden, void* out)
+{
+    if (bf) hipLaunchKernelGGL((k_head_gather<DT_BF16>), block_grid(rows), dim3(256), 0, t_stream, hidden_rows, index, count, (int32_t)hidden, out);
+    else hipLaunchKernelGGL((k_head_gather<DT_F32>), block_grid(rows), dim3(256), 0, t_stream, hidden_rows, index, count, (int32_t)hidden, out);
+}
+
+}  // namespace abh
+
+using namespace abh;
+
+extern "C" {
+
+ADAMBRIDGE_API int64_t adambridge_token_losses_work(int32_t dtype, int64_t rows, int64_t vocab, int64_t hidden)
+{
+    const int rc = head_check(dtype, rows, vocab, hidden);
+    return rc ? rc : HeadForward(nullptr, dtype, rows, vocab, hidden).bytes;
+}
+
+ADAMBRIDGE_API int adambridge_token_losses(const void* hidden, const void* weight, int32_t dtype, const int64_t* targets, int64_t rows,
+                                           int64_t vocab, int64_t size, int64_t ignore_index, float* losses, float* stats, void* work)
+{
+    const int rc = head_check(dtype, rows, vocab, size);
+    if (rc) return rc;
+    if (!hidden || !weight || !targets || !losses || !work) return ADAMBRIDGE_ENULL;
+    if ((uintptr_t)work % 16) return ADAMBRIDGE_EALIGN;
+    const bool bf = dtype == ADAMBRIDGE_DT_BF16;
+    const HeadForward p(work, dtype, rows, vocab, size);
+    HeadArgs A{};
+    A.w = weight;
+    A.targets = targets;
+    A.rows = (int32_t)rows;
+    A.hidden = (int32_t)size;
+    A.vocab = vocab;
+    A.part = p.part;
+    A.picked = p.picked;
+    if (p.few) {
+        A.h = hidden;
+        const int64_t bytes = size * (bf ? 2 : 4);
+        const bool even = bytes % 16 == 0 && ((uintptr_t)hidden | (uintptr_t)weight) % 16 == 0;
+        const dim3 grid = block_grid(p.parts), block(256);
+        if (bf && even) hipLaunchKernelGGL((k_head_few<DT_BF16, true>), grid, block, 0, t_stream, A);
+        else if (bf) hipLaunchKernelGGL((k_head_few<DT_BF16, false>), grid, block, 0, t_stream, A);
+        else if (even) hipLaunchKernelGGL((k_head_few<DT_F32, true>), grid, block, 0, t_stream, A);
+        else hipLaunchKernelGGL((k_head_few<DT_F32, false>), grid, block, 0, t_stream, A);
+        hipLaunchKernelGGL((k_head_finish<4>), dim3((unsigned)((rows + 3) / 4)), dim3(kFinishLanes), 0, t_stream, p.part, p.parts, A.rows, nullptr,
+                           nullptr, targets, vocab, ignore_index, p.picked, losses, stats);
+    } else {
+        hipLaunchKernelGGL(k_head_rows, dim3(1), dim3(1024), 0, t_stream, targets, ignore_index, A.rows, p.index, (int32_t*)nullptr, p.count, losses);
+        launch_gather(bf, rows, hidden, p.index, p.count, size, p.h);
+        A.h = p.h;
+        A.index = p.index;
+        A.count = p.count;
+        A.width = (int32_t)vocab;
+        A.tiles_j = p.parts;
+        const bool even = size % 8 == 0 && (uintptr_t)weight % 16 == 0;
+        const dim3 grid = tile_grid((rows + p.tile - 1) / p.tile * p.parts);
+        ABH_HEAD_LAUNCH(k_head_sums, p.tile, even, grid);
+        hipLaunchKernelGGL((k_head_finish<16>), block_grid((rows + 15) / 16), dim3(kFinishLanes), 0, t_stream, p.part, p.parts, A.rows, p.index,
+                           p.count, targets, vocab, ignore_index, p.picked, losses, stats);
+    }
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? 0 : hip_fail(e, "hipLaunchKernelGGL (token losses)");
+}
+
+ADAMBRIDGE_API int64_t adambridge_token_losses_backward_work(int32_t dtype, int64_t rows, int64_t vocab, int64_t hidden)
+{
+    const int rc = head_check(dtype, rows, vocab, hidden);
+    return rc ? rc : HeadBackward(nullptr, dtype, rows, vocab, hidden).bytes;
+}
+
+ADAMBRIDGE_API int adambridge_token_losses_backward(const float* gout, const void* hidden, const void* weight, int32_t dtype,
+                                                    const int64_t* targets, int64_t rows, int64_t vocab, int64_t size, int64_t ignore_index,
+                                                    const float* stats, void* dhidden, void* dweight, void* work)
+{
+    const int rc = head_check(dtype, rows, vocab, size);
+    if (rc) return rc;
+    if (!dhidden && !dweight) return 0;
+    if (!gout || !hidden || !weight || !targets || !stats || !work) return ADAMBRIDGE_ENULL;
+    if ((uintptr_t)work % 16) return ADAMBRIDGE_EALIGN;
+    const bool bf = dtype == ADAMBRIDGE_DT_BF16;
+    const HeadBackward p(work, dtype, rows, vocab, size);
+    hipLaunchKernelGGL(k_head_rows, dim3(1), dim3(1024), 0, t_stream, targets, ignore_index, (int32_t)rows, p.index, p.place, p.count, (float*)nullptr);
+    launch_gather(bf, rows, hidden, p.index, p.count, size, p.h);
+    HeadArgs A{};
+    A.h = p.h;
+    A.w = weight;
+    A.targets = targets;
+    A.index = p.index;
+    A.count = p.count;
+    A.rows = (int32_t)rows;
+    A.hidden = (int32_t)size;
+    A.vocab = vocab;
+    A.pitch = p.pitch;
+    A.stats = stats;
+    A.gout = gout;
+    A.g = p.g;
+    A.dh = p.dh;
+    A.dw = dweight;
+    A.fresh = 1;
+    const bool even = size % 8 == 0 && ((uintptr_t)weight | (uintptr_t)dweight) % 16 == 0;
+    for (int64_t v0 = 0; v0 < vocab; v0 += p.pitch) {
+        A.v0 = v0;
+        A.width = (int32_t)std::min<int64_t>(p.pitch, vocab - v0);
+        A.tiles_j = (A.width + p.tile - 1) / p.tile;
+        ABH_HEAD_LAUNCH(k_head_grad, p.tile, even, tile_grid((rows + p.tile - 1) / p.tile * A.tiles_j));
+        if (dweight) {
+            A.tiles_j = (int32_t)((size + p.tile - 1) / p.tile);
+            ABH_HEAD_LAUNCH(k_head_dw, p.tile, even, tile_grid((int64_t)(A.width + p.tile - 1) / p.tile * A.tiles_j));
+        }
+        if (dhidden) {
+            A.tiles_j = (int32_t)((size + p.dh_tile - 1) / p.dh_tile);
+            const int64_t tiles = (rows + p.dh_tile - 1) / p.dh_tile * A.tiles_j;
+            ABH_HEAD_LAUNCH(k_head_dh, p.dh_tile, even, tile_grid(std::max<int64_t>(tiles, kHeadCus)));
+        }
+        A.fresh = 0;
+    }
+    if (dhidden) {
+        if (bf)
+            hipLaunchKernelGGL((k_head_scatter<DT_BF16>), block_grid(rows), dim3(256), 0, t_stream, p.dh, p.place, p.count, A.rows, A.hidden, p.dh_tile,
+                               p.pitch, dhidden);
+        else
+            hipLaunchKernelGGL((k_head_scatter<DT_F32>), block_grid(rows), dim3(256), 0, t_stream, p.dh, p.place, p.count, A.rows, A.hidden, p.dh_tile,
+                               p.pitch, dhidden);
+    }
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? 0 : hip_fail(e, "hipLaunchKernelGGL (token losses backward)");
+}
+
+}  // extern "C"

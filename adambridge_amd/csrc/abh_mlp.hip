@@ -1,0 +1,349 @@
+// abh_mlp.hip -- a layer of expert MLPs for a few tokens, from the router's logits to the result, in two kernels.
+//
+//   out[t] = sum over the top_k experts e of token t, w[t, e] down[e] a(t, e)
+//   a(t, e) = act(up[e] x[t]),  or  act(gate[e] x[t]) * up[e] x[t]
+//
+// A few tokens' layer is the chosen experts' weights, read once from HBM, and what a
+// call costs beside: as route, dispatch, two or three products, an activation and combine it is seven launches, each with its
+// results through memory.  Here the first kernel chooses (every workgroup for itself: a few tokens' logits are a few KB), takes
+// its 16 rows of one chosen expert's up (and gate) times all tokens, and stores the activations; the second takes 16
+// rows of down of all chosen experts, weights and adds their products, and stores the result.
+//
+// The tokens, up to 16, are the other side of the matrix instructions, whatever their number: an expert's weights are read once
+// for all tokens that chose it.  Activations are rounded to the operands' type, which the instructions take; all other
+// sums are FP32, in an order of their own.
+
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "../../include/adambridge_hip.h"
+#include "abh_choice.hpp"
+#include "abh_device.hpp"
+#include "abh_host.hpp"
+#include "abh_rows.hpp"
+#include "abh_tiles.hpp"
+
+namespace abh {
+
+constexpr int kMlpTokens = 16, kMlpExperts = 1024, kMlpChosen = 64;
+constexpr int kMlpColumns = 16;   // of a workgroup
+constexpr int kUpWaves = 4, kDownWaves = 16;
+
+// A chosen expert: which tokens chose it, and their weights.
+struct Chosen {
+    int32_t expert;
+    uint32_t tokens;
+    float weight[kMlpTokens];
+};
+
+struct MlpArgs {
+    const void *x, *logits, *up, *gate, *down;
+    void* out;
+    Chosen* list;      // the chosen experts, in order of their number
+    int32_t* count;    // how many
+    void* a;           // chosen experts x 16 x inter
+    int32_t tokens, experts, top_k, inter, hidden;
+    int32_t logits_bf16, normalize, silu;
+    int32_t columns;   // workgroups of a chosen expert
+};
+
+// x Phi(x), and x / (1 + exp(-x)).
+__device__ __forceinline__ float activated(float x, bool silu)
+{
+    return silu ? x / (1.0f + expf(-x)) : 0.5f * x * (1.0f + erff(x * 0.70710678118654752f));
+}
+
+__device__ __forceinline__ float logit(const MlpArgs& A, int64_t i)
+{
+    return A.logits_bf16 ? get<DT_BF16>(A.logits, i) : get<DT_F32>(A.logits, i);
+}
+
+// The choice of all tokens, a wavefront a token, NV logits a lane (expert 64 v + lane).
+template <int NV>
+__device__ __forceinline__ void choose(const MlpArgs& A, uint32_t* mask, int32_t* expert, float* weight)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
+    for (int e = threadIdx.x; e < A.experts; e += kUpWaves * kWave) mask[e] = 0;
+    __syncthreads();
+    for (int t = wave; t < A.tokens; t += kUpWaves) {
+        float x[NV];
+        uint32_t key[NV];
+#pragma unroll
+        for (int v = 0; v < NV; ++v) x[v] = 64 * v + lane < A.experts ? logit(A, (int64_t)t * A.experts + 64 * v + lane) : 0.0f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v) key[v] = 64 * v + lane < A.experts ? order_key(x[v]) : 0u;
+        float top = 0.0f, sum = 0.0f, mine = 0.0f;
+        int my_expert = 0;
+        for (int j = 0; j < A.top_k; ++j) {
+            uint32_t most = key[0];
+#pragma unroll
+            for (int v = 1; v < NV; ++v) most = most > key[v] ? most : key[v];
+            most = group_max<kWave>(most);
+            int e = 0;   // the lowest index that has it
+#pragma unroll
+            for (int v = NV - 1; v >= 0; --v) {
+                const uint64_t with = __builtin_amdgcn_ballot_w64(key[v] == most);
+                e = with ? 64 * v + __builtin_ctzll(with) : e;
+            }
+#pragma unroll
+            for (int v = 0; v < NV; ++v) key[v] = 64 * v + lane == e ? 0u : key[v];
+            const float value = key_value(most);
+            if (j == 0) {
+                top = value;
+                if (!A.normalize) {   // the sum over all experts
+#pragma unroll
+                    for (int v = 0; v < NV; ++v) sum += 64 * v + lane < A.experts ? exp_below(x[v], top) : 0.0f;
+                    sum = wave_sum(sum);
+                }
+            }
+            const float w = exp_below(value, top);
+            if (A.normalize) sum += w;
+            if (lane == j) {
+                mine = w;
+                my_expert = e;
+            }
+        }
+        if (lane < A.top_k) {
+            weight[t * A.top_k + lane] = top == kRouteNegInf ? 0.0f : mine / sum;
+            expert[t * A.top_k + lane] = my_expert;
+            atomicOr(&mask[my_expert], 1u << t);
+        }
+    }
+    __syncthreads();
+}
+
+// 16 columns of up (and gate) of the blockIdx-th chosen expert: the wavefronts split the sum, the first adds their parts in order.
+template <int DT, bool EVEN, bool GATE, int NV>
+__global__ __launch_bounds__(kUpWaves * kWave) void k_mlp_up(MlpArgs A)
+{
+    constexpr int V = kLane<DT>, STEP = 4 * V, W = kUpWaves, M = GATE ? 2 : 1, U = GATE ? 4 : 8;
+    __shared__ uint32_t mask[kMlpExperts];
+    __shared__ int32_t expert[kMlpTokens * kMlpChosen];
+    __shared__ float weight[kMlpTokens * kMlpChosen];
+    __shared__ mm_f32x4 parts[W - 1][M][64];
+    choose<NV>(A, mask, expert, weight);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+    const int col = lane & 15, quarter = lane >> 4;
+    const int block = (int)block_index(), rank = block / A.columns, j0 = (block - rank * A.columns) * kMlpColumns;
+    int e = -1, skip = rank, before = 0;
+    for (int e0 = 0; e0 < A.experts; e0 += kWave) {
+        const uint64_t with = __builtin_amdgcn_ballot_w64(e0 + lane < A.experts && mask[e0 + lane < A.experts ? e0 + lane : 0] != 0);
+        const int n = __builtin_popcountll(with);
+        if (e < 0 && skip < n) {
+            uint64_t left = with;
+            for (int i = 0; i < skip; ++i) left &= left - 1;
+            e = e0 + __builtin_ctzll(left);
+        }
+        skip -= n;
+        before += n;
+    }
+    if (block == 0 && threadIdx.x == 0) *A.count = before;
+    if (e < 0) return;
+    const uint32_t tokens = mask[e];
+    if (j0 == 0 && threadIdx.x < kMlpTokens) {   // for the other kernel
+        Chosen* const c = A.list + rank;
+        float w = 0.0f;
+        if ((int)threadIdx.x < A.tokens)
+            for (int j = 0; j < A.top_k; ++j) w = expert[threadIdx.x * A.top_k + j] == e ? weight[threadIdx.x * A.top_k + j] : w;
+        c->weight[threadIdx.x] = w;
+        if (threadIdx.x == 0) {
+            c->expert = e;
+            c->tokens = tokens;
+        }
+    }
+    const int steps = (A.hidden + STEP - 1) / STEP, s0 = steps * wave / W, s1 = steps * (wave + 1) / W;
+    const int columns = A.inter - j0 < kMlpColumns ? A.inter - j0 : kMlpColumns;
+    const int64_t first = ((int64_t)e * A.inter + j0) * A.hidden;
+    const uint32_t bytes = (uint32_t)(columns * A.hidden * kSize<DT>);
+    const Pieces<DT, EVEN> w[2] = {{at<DT>(A.up, first), bytes, A.hidden, columns}, {at<DT>(GATE ? A.gate : A.up, first), bytes, A.hidden, columns}};
+    const Pieces<DT, EVEN> x{static_cast<const uint8_t*>(A.x), (uint32_t)(A.tokens * A.hidden * kSize<DT>), A.hidden, A.tokens};
+    mm_f32x4 acc[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) acc[m] = mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = s0; s < s1; s += U) {
+        raw16 wv[M][U], xv[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int m = 0; m < M; ++m) wv[m][u] = w[m].load(col, (s + u) * STEP + quarter * V, s + u < s1);
+#pragma unroll
+        for (int u = 0; u < U; ++u) xv[u] = x.load(col, (s + u) * STEP + quarter * V, s + u < s1);
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+            mm_f32x4 some = DT == DT_BF16 ? acc[m] : mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};   // FP32: short chains of sums
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if constexpr (DT == DT_BF16) {
+                    some = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mm_bf16x8, wv[m][u]), __builtin_bit_cast(mm_bf16x8, xv[u]), some,
+                                                                   0, 0, 0);
+                } else {
+                    const mm_f32x4 wf = __builtin_bit_cast(mm_f32x4, wv[m][u]), xf = __builtin_bit_cast(mm_f32x4, xv[u]);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) some = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[q], xf[q], some, 0, 0, 0);
+                }
+            }
+            if constexpr (DT == DT_BF16) acc[m] = some;
+            else acc[m] += some;
+        }
+    }
+    if (wave > 0)
+#pragma unroll
+        for (int m = 0; m < M; ++m) parts[wave - 1][m][lane] = acc[m];
+    __syncthreads();
+    if (wave > 0 || !(tokens >> col & 1)) return;
+#pragma unroll
+    for (int p = 0; p < W - 1; ++p)
+#pragma unroll
+        for (int m = 0; m < M; ++m) acc[m] += parts[p][m][lane];
+    void* row = at<DT>(A.a, ((int64_t)rank * kMlpTokens + col) * A.inter);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const float y = GATE ? activated(acc[M - 1][r], A.silu) * acc[0][r] : activated(acc[0][r], A.silu);
+        if (j0 + 4 * quarter + r < A.inter) put<DT>(row, j0 + 4 * quarter + r, y);
+    }
+}
+
+// 16 columns of the result: the wavefronts share the chosen experts' pieces of U steps, whose products are weighted and added in
+// the order of the experts, then the wavefronts' parts in theirs.
+template <int DT, bool EVEN>
+__global__ __launch_bounds__(kDownWaves * kWave) void k_mlp_down(MlpArgs A)
+{
+    constexpr int V = kLane<DT>, STEP = 4 * V, W = kDownWaves, U = 8;
+    __shared__ mm_f32x4 parts[W][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+    const int col = lane & 15, quarter = lane >> 4;
+    const int j0 = (int)block_index() * kMlpColumns, columns = A.hidden - j0 < kMlpColumns ? A.hidden - j0 : kMlpColumns;
+    const int pieces = (A.inter + U * STEP - 1) / (U * STEP), items = scalar(*A.count) * pieces;
+    mm_f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = wave; i < items; i += W) {
+        const int rank = i / pieces, k0 = (i - rank * pieces) * (U * STEP);
+        const Chosen* const c = A.list + rank;
+        const int e = scalar(c->expert);
+        const bool mine = c->tokens >> col & 1;
+        const Pieces<DT, EVEN> w{at<DT>(A.down, ((int64_t)e * A.hidden + j0) * A.inter), (uint32_t)(columns * A.inter * kSize<DT>), A.inter, columns};
+        const Pieces<DT, EVEN> a{at<DT>(A.a, (int64_t)rank * kMlpTokens * A.inter), (uint32_t)(kMlpTokens * A.inter * kSize<DT>), A.inter, kMlpTokens};
+        raw16 wv[U], av[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) wv[u] = w.load(col, k0 + u * STEP + quarter * V, true);
+#pragma unroll
+        for (int u = 0; u < U; ++u) av[u] = a.load(col, k0 + u * STEP + quarter * V, mine);   // another token's row: never written
+        mm_f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if constexpr (DT == DT_BF16) {
+                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mm_bf16x8, wv[u]), __builtin_bit_cast(mm_bf16x8, av[u]), acc, 0, 0, 0);
+            } else {
+                const mm_f32x4 wf = __builtin_bit_cast(mm_f32x4, wv[u]), af = __builtin_bit_cast(mm_f32x4, av[u]);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[q], af[q], acc, 0, 0, 0);
+            }
+        }
+        const float by = c->weight[col];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[r] = mine ? sum[r] + by * acc[r] : sum[r];   // what an expert holds stays with its tokens
+    }
+    parts[wave][lane] = sum;
+    __syncthreads();
+    if (threadIdx.x >= kMlpTokens * kMlpColumns) return;
+    const int token = threadIdx.x / kMlpColumns, j = threadIdx.x % kMlpColumns;
+    if (token >= A.tokens || j >= columns) return;
+    float y = 0.0f;
+#pragma unroll
+    for (int p = 0; p < W; ++p) y += parts[p][j / 4 * 16 + token][j % 4];
+    put<DT>(A.out, (int64_t)token * A.hidden + j0 + j, y);
+}
+
+// ------------------------------------------------------------------------------ launches
+
+constexpr int64_t kMlpSize = (int64_t)1 << 22;
+
+static int mlp_check(int32_t dtype, int64_t tokens, int64_t experts, int64_t top_k, int64_t inter, int64_t hidden)
+{
+    if (dtype != ADAMBRIDGE_DT_F32 && dtype != ADAMBRIDGE_DT_BF16) return ADAMBRIDGE_EMVDTYPE;
+    if (tokens < 1 || tokens > kMlpTokens || experts < 1 || experts > kMlpExperts || top_k < 1 || top_k > kMlpChosen || top_k > experts ||
+        inter < 1 || inter > kMlpSize || hidden < 1 || hidden > kMlpSize)
+        return ADAMBRIDGE_EBADN;
+    return 0;
+}
+
+// Scratch: how many experts are chosen, which, and their activations, at 256 bytes each.
+static int64_t list_bytes(int64_t used) { return (used * (int64_t)sizeof(Chosen) + 255) / 256 * 256; }
+
+template <int DT, bool EVEN, bool GATE>
+static void launch_up(const MlpArgs& A, const dim3 grid)
+{
+    const dim3 block(kUpWaves * kWave);
+    if (A.experts <= 64) hipLaunchKernelGGL((k_mlp_up<DT, EVEN, GATE, 1>), grid, block, 0, t_stream, A);
+    else if (A.experts <= 256) hipLaunchKernelGGL((k_mlp_up<DT, EVEN, GATE, 4>), grid, block, 0, t_stream, A);
+    else hipLaunchKernelGGL((k_mlp_up<DT, EVEN, GATE, 16>), grid, block, 0, t_stream, A);
+}
+
+template <int DT>
+static void launch_mlp(const MlpArgs& A, int64_t used)
+{
+    const bool up_even = A.hidden % kLane<DT> == 0 && ((uintptr_t)A.x | (uintptr_t)A.up | (uintptr_t)A.gate) % 16 == 0;
+    const bool down_even = A.inter % kLane<DT> == 0 && (uintptr_t)A.down % 16 == 0;
+    const dim3 grid = block_grid(used * A.columns);
+    if (up_even && A.gate) launch_up<DT, true, true>(A, grid);
+    else if (up_even) launch_up<DT, true, false>(A, grid);
+    else if (A.gate) launch_up<DT, false, true>(A, grid);
+    else launch_up<DT, false, false>(A, grid);
+    const dim3 columns = block_grid((A.hidden + kMlpColumns - 1) / kMlpColumns), block(kDownWaves * kWave);
+    if (down_even) hipLaunchKernelGGL((k_mlp_down<DT, true>), columns, block, 0, t_stream, A);
+    else hipLaunchKernelGGL((k_mlp_down<DT, false>), columns, block, 0, t_stream, A);
+}
+
+}  // namespace abh
+
+using namespace abh;
+
+extern "C" {
+
+ADAMBRIDGE_API int64_t adambridge_expert_mlp_work(int32_t dtype, int64_t tokens, int64_t experts, int64_t top_k, int64_t inter, int64_t hidden)
+{
+    const int rc = mlp_check(dtype, tokens, experts, top_k, inter, hidden);
+    if (rc) return rc;
+    const int64_t used = std::min(tokens * top_k, experts);
+    return 256 + list_bytes(used) + used * kMlpTokens * inter * (dtype == ADAMBRIDGE_DT_BF16 ? 2 : 4);
+}
+
+ADAMBRIDGE_API int adambridge_expert_mlp(const void* x, const void* logits, int32_t logits_dtype, const void* up, const void* gate, const void* down,
+                                         int32_t dtype, int64_t tokens, int64_t experts, int64_t top_k, int64_t inter, int64_t hidden,
+                                         int32_t activation, int32_t normalize, void* out, void* work)
+{
+    const int rc = mlp_check(dtype, tokens, experts, top_k, inter, hidden);
+    if (rc) return rc;
+    if (logits_dtype != ADAMBRIDGE_DT_F32 && logits_dtype != ADAMBRIDGE_DT_BF16) return ADAMBRIDGE_EMVDTYPE;
+    if (activation != ADAMBRIDGE_GELU && activation != ADAMBRIDGE_SILU) return ADAMBRIDGE_EMVDTYPE;
+    if (!x || !logits || !up || !down || !out || !work) return ADAMBRIDGE_ENULL;
+    if ((uintptr_t)work % 16) return ADAMBRIDGE_EALIGN;
+    const int64_t used = std::min(tokens * top_k, experts);
+    MlpArgs A{};
+    A.x = x;
+    A.logits = logits;
+    A.up = up;
+    A.gate = gate;
+    A.down = down;
+    A.out = out;
+    A.count = static_cast<int32_t*>(work);
+    A.list = reinterpret_cast<Chosen*>(static_cast<uint8_t*>(work) + 256);
+    A.a = static_cast<uint8_t*>(work) + 256 + list_bytes(used);
+    A.tokens = (int32_t)tokens;
+    A.experts = (int32_t)experts;
+    A.top_k = (int32_t)top_k;
+    A.inter = (int32_t)inter;
+    A.hidden = (int32_t)hidden;
+    A.logits_bf16 = logits_dtype == ADAMBRIDGE_DT_BF16;
+    A.normalize = normalize;
+    A.silu = activation == ADAMBRIDGE_SILU;
+    A.columns = (int32_t)((inter + kMlpColumns - 1) / kMlpColumns);
+    if (dtype == ADAMBRIDGE_DT_BF16) launch_mlp<DT_BF16>(A, used);
+    else launch_mlp<DT_F32>(A, used);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? 0 : hip_fail(e, "hipLaunchKernelGGL (expert MLP)");
+}
+
+}  // extern "C"

@@ -60,6 +60,12 @@ struct Api {
     decltype(&adambridge_embed) embed;
     decltype(&adambridge_embed_work) embed_work;
     decltype(&adambridge_embed_backward) embed_backward;
+    decltype(&adambridge_token_losses) token_losses;
+    decltype(&adambridge_token_losses_work) token_losses_work;
+    decltype(&adambridge_token_losses_backward) token_losses_backward;
+    decltype(&adambridge_token_losses_backward_work) token_losses_backward_work;
+    decltype(&adambridge_expert_mlp_work) expert_mlp_work;
+    decltype(&adambridge_expert_mlp) expert_mlp;
 };
 
 Api api;
@@ -520,6 +526,41 @@ PyObject* expert_mm(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------ expert_mlp
+
+// expert_mlp(x, logits, up, down, gate or None, top_k, silu, normalize), of a few tokens without gradients
+PyObject* expert_mlp(PyObject*, PyObject* const* args, Py_ssize_t nargs)
+{
+    HANDLE_TH_ERRORS
+    if (nargs != 8 || !connected || observed()) Py_RETURN_NONE;
+    const Tensor *x = plain(args[0]), *logits = plain(args[1]), *up = plain(args[2]), *down = plain(args[3]), *gate;
+    if (!plain_or_none(args[4], gate) || !values(x, 2) || !values(logits, 2) || logits->device() != x->device() || !values(up, 3)) Py_RETURN_NONE;
+    if (!beside(up, x, x->scalar_type()) || !beside(down, x, x->scalar_type()) || (gate && !beside(gate, x, x->scalar_type()))) Py_RETURN_NONE;
+    if (!PyLong_CheckExact(args[5]) || !PyBool_Check(args[6]) || !PyBool_Check(args[7]) || at::autocast::is_autocast_enabled(at::kCUDA)) Py_RETURN_NONE;
+    const int64_t tokens = x->size(0), hidden = x->size(1), experts = up->size(0), inter = up->size(1);
+    if (logits->size(0) != tokens || logits->size(1) != experts || up->size(2) != hidden || (gate && gate->sizes() != up->sizes()) ||
+        down->sizes() != at::IntArrayRef({experts, hidden, inter}) || wants_grad({x, logits, up, down, gate}))
+        Py_RETURN_NONE;
+    const int64_t top_k = PyLong_AsLongLong(args[5]);
+    if (top_k == -1 && PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    const int32_t type = code(x->scalar_type());
+    const int64_t bytes = api.expert_mlp_work(type, tokens, experts, top_k, inter, hidden);
+    if (bytes < 0) Py_RETURN_NONE;   // more than a few tokens, or sizes out of the kernels' range
+    const at::AutoDispatchBelowADInplaceOrView below;
+    Tensor out = fresh({tokens, hidden}, x->scalar_type(), *x), work = scratch(bytes, *x);
+    {
+        const On on(*x);
+        check(api.expert_mlp(address(*x), address(*logits), code(logits->scalar_type()), address(*up), gate ? address(*gate) : nullptr, address(*down),
+                             type, tokens, experts, top_k, inter, hidden, args[6] == Py_True ? ADAMBRIDGE_SILU : ADAMBRIDGE_GELU, args[7] == Py_True,
+                             place(out), place(work)), "adambridge_expert_mlp");
+    }
+    return THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
 // ----------------------------------------------------------------------------------- embed
 
 Tensor embed_forward(const Tensor& ids, const Tensor& weight, double scale)
@@ -594,6 +635,93 @@ PyObject* embed(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------- token losses
+
+Tensor losses_forward(const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t ignore, Tensor* stats)
+{
+    const int64_t rows = targets.numel(), vocab = weight.size(0), size = weight.size(1);
+    const int32_t type = code(hidden.scalar_type());
+    const int64_t bytes = api.token_losses_work(type, rows, vocab, size);
+    check(bytes, "adambridge_token_losses_work");
+    Tensor losses = fresh(targets.sizes(), at::kFloat, hidden), work = scratch(bytes, hidden);
+    if (stats) *stats = fresh({rows, 2}, at::kFloat, hidden);
+    const On on(hidden);
+    check(api.token_losses(address(hidden), address(weight), type, targets.const_data_ptr<int64_t>(), rows, vocab, size, ignore,
+                           losses.mutable_data_ptr<float>(), stats ? stats->mutable_data_ptr<float>() : nullptr, place(work)),
+          "adambridge_token_losses");
+    return losses;
+}
+
+struct TokenLosses : Function<TokenLosses> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& targets, int64_t ignore)
+    {
+        const at::AutoDispatchBelowADInplaceOrView below;
+        Tensor stats;
+        Tensor losses = losses_forward(hidden, weight, targets, ignore, &stats);
+        ctx->save_for_backward({hidden, weight, targets, stats});
+        ctx->saved_data["ignore"] = ignore;
+        ctx->saved_data["vocab"] = weight.size(0);
+        ctx->saved_data["size"] = weight.size(1);
+        ctx->saved_data["type"] = (int64_t)hidden.scalar_type();
+        return losses;
+    }
+    static tensor_list backward(AutogradContext* ctx, const tensor_list& grads)
+    {
+        const tensor_list saved = ctx->get_saved_variables();
+        const Tensor &hidden = saved[0], &weight = saved[1], &targets = saved[2], &stats = saved[3];
+        const int64_t ignore = ctx->saved_data["ignore"].toInt(), vocab = ctx->saved_data["vocab"].toInt(), size = ctx->saved_data["size"].toInt();
+        const at::ScalarType type = (at::ScalarType)ctx->saved_data["type"].toInt();
+        const bool want_h = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+        const bool numbers = !grads[0].unsafeGetTensorImpl()->has_symbolic_sizes_strides();
+        const at::IntArrayRef sizes = sizes_of(grads[0]);
+        const int64_t rows = numbers ? grads[0].numel() : 0;
+        std::vector<int64_t> with_size = sizes.vec();
+        with_size.push_back(size);
+        const bool whole = numbers && restored(hidden, grads[0], type, with_size) & restored(weight, grads[0], type, {vocab, size}) &
+                                          restored(targets, grads[0], at::kLong, sizes) & restored(stats, grads[0], at::kFloat, {rows, 2});
+        if (!whole || !plain_backward(grads[0]))
+            return in_torch("token_losses", [&] {
+                return pybind11::make_tuple(grads[0], hidden, weight, targets, ignore, want_h, want_w);
+            }, 4);
+        const at::AutoDispatchBelowADInplaceOrView below;
+        const Tensor g = grads[0].contiguous(), h = hidden.contiguous(), w = weight.contiguous(), t = targets.contiguous(), s = stats.contiguous();
+        const int64_t bytes = api.token_losses_backward_work(code(type), rows, vocab, size);
+        check(bytes, "adambridge_token_losses_backward_work");
+        tensor_list out(4);
+        if (want_h) out[0] = fresh(with_size, type, g);
+        if (want_w) out[1] = fresh({vocab, size}, type, g);
+        Tensor work = scratch(bytes, g);
+        const On on(g);
+        check(api.token_losses_backward(g.const_data_ptr<float>(), address(h), address(w), code(type), t.const_data_ptr<int64_t>(), rows, vocab,
+                                        size, ignore, s.const_data_ptr<float>(), place(out[0]), place(out[1]), place(work)),
+              "adambridge_token_losses_backward");
+        return out;
+    }
+};
+
+// token_losses(hidden, weight, targets, ignore_index)
+PyObject* token_losses(PyObject*, PyObject* const* args, Py_ssize_t nargs)
+{
+    HANDLE_TH_ERRORS
+    if (nargs != 4 || !connected || observed()) Py_RETURN_NONE;
+    const Tensor *hidden = plain(args[0]), *weight = plain(args[1]), *targets = plain(args[2]);
+    if (!values(weight, 2) || !hidden || hidden->dim() < 1 || !beside(hidden, weight, weight->scalar_type()) || !beside(targets, weight, at::kLong) ||
+        !PyLong_CheckExact(args[3]) || at::autocast::is_autocast_enabled(at::kCUDA))
+        Py_RETURN_NONE;
+    if (hidden->size(-1) != weight->size(1) || targets->sizes() != hidden->sizes().slice(0, hidden->dim() - 1)) Py_RETURN_NONE;
+    const int64_t ignore = PyLong_AsLongLong(args[3]);
+    if (ignore == -1 && PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    if (api.token_losses_work(code(weight->scalar_type()), targets->numel(), weight->size(0), weight->size(1)) < 0)
+        Py_RETURN_NONE;   // sizes out of the kernels' range
+    if (wants_grad({hidden, weight})) return THPVariable_Wrap(TokenLosses::apply(*hidden, *weight, *targets, ignore));
+    const at::AutoDispatchBelowADInplaceOrView below;
+    return THPVariable_Wrap(losses_forward(*hidden, *weight, *targets, ignore, nullptr));
+    END_HANDLE_TH_ERRORS
+}
+
 // --------------------------------------------------------------------------------- connect
 
 // connect(addresses by entry point, backward passes in torch operations by operator, the class of default devices' modes)
@@ -613,7 +741,11 @@ PyObject* connect(PyObject*, PyObject* const* args, Py_ssize_t nargs)
         {&found.combine_backward, "adambridge_combine_backward"}, {&found.expert_mm, "adambridge_expert_mm"},
         {&found.expert_mm_dx, "adambridge_expert_mm_dx"}, {&found.expert_mm_work, "adambridge_expert_mm_work"},
         {&found.expert_mm_dw, "adambridge_expert_mm_dw"}, {&found.embed, "adambridge_embed"},
-        {&found.embed_work, "adambridge_embed_work"}, {&found.embed_backward, "adambridge_embed_backward"}};
+        {&found.embed_work, "adambridge_embed_work"}, {&found.embed_backward, "adambridge_embed_backward"},
+        {&found.token_losses, "adambridge_token_losses"}, {&found.token_losses_work, "adambridge_token_losses_work"},
+        {&found.token_losses_backward, "adambridge_token_losses_backward"},
+        {&found.token_losses_backward_work, "adambridge_token_losses_backward_work"},
+        {&found.expert_mlp_work, "adambridge_expert_mlp_work"}, {&found.expert_mlp, "adambridge_expert_mlp"}};
     for (const auto& e : entries) {
         PyObject* o = PyDict_GetItemString(args[0], e.name);
         void* const p = o ? PyLong_AsVoidPtr(o) : nullptr;
@@ -640,7 +772,9 @@ PyMethodDef kMethods[] = {
     {"dispatch", ABH_FAST(dispatch), "dispatch(x, position); None if the call is not an ordinary one."},
     {"combine", ABH_FAST(combine), "combine(rows, weights, position); None if the call is not an ordinary one."},
     {"expert_mm", ABH_FAST(expert_mm), "expert_mm(x, weight, ends); None if the call is not an ordinary one."},
+    {"expert_mlp", ABH_FAST(expert_mlp), "expert_mlp(x, logits, up, down, gate, top_k, silu, normalize); None if the call is not an ordinary one."},
     {"embed", ABH_FAST(embed), "embed(ids, weight, scale, padding_idx); None if the call is not an ordinary one."},
+    {"token_losses", ABH_FAST(token_losses), "token_losses(hidden, weight, targets, ignore_index); None if the call is not an ordinary one."},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_ops", "The host's side of an expert block's operators.", -1, kMethods,

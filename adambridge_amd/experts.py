@@ -7,8 +7,10 @@ An expert MLP of ``top_k`` experts a token is::
     rows = expert_mm(F.gelu(expert_mm(rows, up, r.ends)), down, r.ends)
     y = combine(rows, r)                            # each token's weighted sum
 
+which is ``expert_mlp(x, x @ router.T, up, down, top_k)``, for a few tokens two kernels.
+
 Nothing of it waits for the device: how many rows an expert has is read there (``r.ends``).  On plain GPU
-tensors of float32 or bfloat16 the library's kernels compute it (csrc/abh_route.hip, csrc/abh_experts.hip, called by
+tensors of float32 or bfloat16 the library's kernels compute it (csrc/abh_route.hip, csrc/abh_experts.hip, csrc/abh_mlp.hip, called by
 csrc/abh_ops.cpp); elsewhere, and where an operation is traced, transformed or differentiated twice, torch operations do.
 """
 
@@ -17,15 +19,17 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+import torch.nn.functional as F
 
 from . import _hip
 from .losses import _observed
 from .norms import plain
 
-__all__ = ["Routing", "route", "dispatch", "expert_mm", "combine"]
+__all__ = ["Routing", "route", "dispatch", "expert_mm", "combine", "expert_mlp"]
 
 _MOST_EXPERTS, _MOST_CHOSEN, _MOST_ASSIGNED = 1024, 64, (1 << 31) - 1   # adambridge_route's
 _MOST_ROWS, _MOST_SIZE, _MOST_MM_EXPERTS = 1 << 30, 1 << 22, 4096       # adambridge_expert_mm's
+_FEW_TOKENS = 16                                                        # adambridge_expert_mlp's
 
 
 class Routing(NamedTuple):
@@ -290,3 +294,51 @@ def expert_mm(x: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) -> torc
     with torch.autocast("cuda", enabled=False):
         out = _hip.ops().expert_mm(x.contiguous(), weight.contiguous(), ends.contiguous())
     return _torch_rows(x, weight.transpose(1, 2), ends) if out is None else out
+
+
+# ------------------------------------------------------------------ expert_mlp
+
+_ACTIVATIONS = {"gelu": F.gelu, "silu": F.silu}
+
+
+def expert_mlp(x: torch.Tensor, logits: torch.Tensor, up: torch.Tensor, down: torch.Tensor, top_k: int,
+               gate: torch.Tensor | None = None, activation: str = "gelu", normalize: bool = True) -> torch.Tensor:
+    """A layer of expert MLPs: each token's sum, by the weights of ``route(logits, top_k, normalize)``, of
+    ``down[e] @ act(up[e] @ x)`` over its chosen experts, or with a ``gate`` of ``down[e] @ (act(gate[e] @ x) * (up[e] @ x))``:
+    ``x`` ``[tokens, hidden]``, ``logits`` ``[tokens, experts]``, ``up`` and ``gate`` ``[experts, inter, hidden]``, ``down``
+    ``[experts, hidden, inter]``; ``activation`` ``"gelu"`` or ``"silu"``.
+
+    Up to 16 tokens without gradients (a decoding step) take two kernels, which round the activations and the result only; more tokens,
+    and any that are trained, take :func:`route`, :func:`dispatch`, :func:`expert_mm` and :func:`combine`, whose results
+    are each rounded."""
+    if torch.compiler.is_compiling():
+        return _uncompiled(expert_mlp, x, logits, up, down, top_k, gate, activation, normalize)
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {activation!r}")
+    if x.is_cuda:
+        out = _hip.ops().expert_mlp(x, logits, up, down, gate, top_k, activation == "silu", bool(normalize))
+        if out is not None:
+            return out
+    if x.dim() != 2 or logits.dim() != 2 or up.dim() != 3 or x.shape[0] != logits.shape[0] or (logits.shape[1], x.shape[1]) != (up.shape[0], up.shape[2]):
+        raise ValueError(f"expert_mlp takes x [tokens, hidden], logits [tokens, experts] and up [experts, inter, hidden], got {tuple(x.shape)}, "
+                         f"{tuple(logits.shape)} and {tuple(up.shape)}")
+    if tuple(down.shape) != (up.shape[0], up.shape[2], up.shape[1]) or (gate is not None and gate.shape != up.shape):
+        raise ValueError(f"down must be [experts, hidden, inter] = {(up.shape[0], up.shape[2], up.shape[1])} and gate, if any, as up, got "
+                         f"{tuple(down.shape)} and {None if gate is None else tuple(gate.shape)}")
+    operands = (x, up, down) if gate is None else (x, up, down, gate)
+    if any(t.device != x.device for t in (logits, *operands)):
+        raise ValueError("x, logits, up, down and gate must be on one device")
+    if not torch.is_autocast_enabled(x.device.type) and any(t.dtype != x.dtype for t in operands):
+        raise ValueError(f"x, up, down and gate must be of one type, got {', '.join(str(t.dtype) for t in operands)}")
+    if plain(logits, *operands) and not all(t.is_contiguous() for t in (logits, *operands)) and x.shape[0] <= _FEW_TOKENS:
+        out = _hip.ops().expert_mlp(x.contiguous(), logits.contiguous(), up.contiguous(), down.contiguous(),
+                                    None if gate is None else gate.contiguous(), top_k, activation == "silu", bool(normalize))
+        if out is not None:
+            return out
+    r = route(logits, top_k, normalize)
+    rows, act = dispatch(x, r), _ACTIVATIONS[activation]
+    if gate is None:
+        rows = act(expert_mm(rows, up, r.ends))
+    else:
+        rows = act(expert_mm(rows, gate, r.ends)) * expert_mm(rows, up, r.ends)
+    return combine(expert_mm(rows, down, r.ends), r)

@@ -1,6 +1,6 @@
-"""A language model's ends: token ids to rows of an embedding.
+"""A language model's ends: token ids to rows of an embedding, and rows to their losses over the vocabulary.
 
-On plain GPU tensors of float32 or bfloat16 the library's kernels compute it (csrc/abh_embed.hip, called by
+On plain GPU tensors of float32 or bfloat16 the library's kernels compute it (csrc/abh_embed.hip, csrc/abh_head.hip, called by
 csrc/abh_ops.cpp); elsewhere, and where an operation is traced, transformed or differentiated twice, torch operations do.
 """
 
@@ -13,9 +13,11 @@ from .experts import _uncompiled
 from .losses import _observed
 from .norms import plain
 
-__all__ = ["embed"]
+__all__ = ["embed", "token_losses"]
 
 _MOST_TOKENS, _MOST_WORDS, _MOST_HIDDEN = 1 << 30, 1 << 30, 1 << 22   # adambridge_embed's
+_MOST_ROWS, _MOST_CLASSES, _MOST_SIZE = 1 << 23, 1 << 22, 1 << 20       # adambridge_token_losses's
+_LEAST_SIZE = {torch.bfloat16: 8, torch.float32: 4}
 
 
 # ----------------------------------------------------------------------- embed
@@ -74,5 +76,76 @@ def embed(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_i
     return _torch_embed(ids, weight, float(scale), padding_idx) if y is None else y
 
 
+# ---------------------------------------------------------------- token_losses
+
+def _scored(hidden, targets, vocab, ignore_index):
+    """The rows, zeros where they are not scored; which are; their targets, 0 for none."""
+    rows, flat = hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1)
+    scored = flat != ignore_index
+    rows = torch.where(scored[:, None], rows.to(torch.promote_types(rows.dtype, torch.float32)), 0.0)
+    inside = (flat >= 0) & (flat < vocab)
+    return rows, scored, inside, torch.where(inside, flat, 0)
+
+
+def _torch_token_losses(hidden, weight, targets, ignore_index):
+    """The definition in torch operations, which hold all logits."""
+    rows, scored, inside, at = _scored(hidden, targets, weight.shape[0], ignore_index)
+    logits = rows @ weight.to(rows.dtype).t()
+    loss = torch.logsumexp(logits, 1) - torch.gather(logits, 1, at[:, None].long())[:, 0]
+    return torch.where(scored, torch.where(inside, loss, torch.nan), 0.0).reshape(targets.shape)
+
+
+def _token_losses_backward(gout, hidden, weight, targets, ignore_index, want_hidden, want_weight):
+    """Both gradients in torch operations, differentiable in turn."""
+    with torch.autocast(gout.device.type, enabled=False):
+        vocab = weight.shape[0]
+        rows, scored, inside, at = _scored(hidden, targets, vocab, ignore_index)
+        wide = weight.to(rows.dtype)
+        seed = torch.where(scored, torch.where(inside, gout.reshape(-1), torch.nan), 0.0)[:, None]
+        hot = torch.arange(vocab, device=at.device) == at[:, None]
+        grad = ((rows @ wide.t()).softmax(1) - hot.to(rows.dtype)) * seed
+        return ((grad @ wide).to(hidden.dtype).reshape(hidden.shape) if want_hidden else None,
+                (grad.t() @ rows).to(weight.dtype) if want_weight else None, None, None)
+
+
+def token_losses(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
+    """Each row's cross-entropy of ``hidden @ weight.T`` against its target, without the logits: ``hidden`` ``[..., size]``,
+    ``weight`` ``[vocab, size]`` (a Linear head's), ``targets`` (int64 or int32) ``[...]``; float32 ``[...]`` (float64 from float64).
+
+    ``-token_losses(...)`` is the log-probability of each target.  Differentiable in ``hidden`` and ``weight``: the backward pass
+    goes through the vocabulary in pieces (its scratch beside copies of ``hidden``: half a GiB in BF16, or 4096 words for every
+    row) and computes each piece's logits again, from ``weight`` as it is then: as any saved operand, it must not be
+    written between the two passes.  Where a target is ``ignore_index`` the loss is 0 and its row reaches nothing and costs nothing,
+    whatever it holds; a target outside the vocabulary gives a loss and gradients of NaN.  ``hidden`` and ``weight`` are of
+    one type (under autocast, taken in its type, as a Linear's are).  Rows shorter than 16 bytes take torch operations."""
+    if torch.compiler.is_compiling():
+        return _uncompiled(token_losses, hidden, weight, targets, ignore_index)
+    if weight.is_cuda:
+        losses = _hip.ops().token_losses(hidden, weight, targets, ignore_index)
+        if losses is not None:
+            return losses
+    if hidden.dim() < 1 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or not weight.shape[0] or not weight.shape[1]:
+        raise ValueError(f"token_losses takes hidden [..., size] and weight [vocab, size], not empty, got {tuple(hidden.shape)} and "
+                         f"{tuple(weight.shape)}")
+    if targets.dtype not in (torch.int64, torch.int32) or targets.shape != hidden.shape[:-1]:
+        raise ValueError(f"targets must be int64 or int32 {tuple(hidden.shape[:-1])}, got {targets.dtype} {tuple(targets.shape)}")
+    if hidden.device != weight.device or targets.device != weight.device:
+        raise ValueError(f"hidden, weight and targets must be on one device, got {hidden.device}, {weight.device} and {targets.device}")
+    if isinstance(ignore_index, bool) or not isinstance(ignore_index, int):
+        raise ValueError(f"ignore_index must be an int, got {ignore_index!r}")
+    if torch.is_autocast_enabled(hidden.device.type):
+        cast = torch.get_autocast_dtype(hidden.device.type)
+        hidden, weight = (t.to(cast) if t.is_floating_point() and t.dtype != torch.float64 else t for t in (hidden, weight))
+    if hidden.dtype != weight.dtype or not hidden.is_floating_point():
+        raise ValueError(f"hidden and weight must be of one floating-point type, got {hidden.dtype} and {weight.dtype}")
+    with torch.autocast(hidden.device.type, enabled=False):
+        if (plain(hidden, weight) and type(targets) is torch.Tensor and 0 < targets.numel() <= _MOST_ROWS and weight.shape[0] <= _MOST_CLASSES
+                and _LEAST_SIZE[weight.dtype] <= weight.shape[1] <= _MOST_SIZE and not _observed()):
+            losses = _hip.ops().token_losses(hidden.contiguous(), weight.contiguous(), targets.long().contiguous(), ignore_index)
+            if losses is not None:
+                return losses
+        return _torch_token_losses(hidden, weight, targets, ignore_index)
+
+
 # for the backward passes that the kernels do not take
-BACKWARD = {"embed": _embed_backward}
+BACKWARD = {"embed": _embed_backward, "token_losses": _token_losses_backward}

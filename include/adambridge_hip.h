@@ -563,6 +563,18 @@ ADAMBRIDGE_API int adambridge_expert_mm_dx(const void* gout, const void* weight,
 ADAMBRIDGE_API int adambridge_expert_mm_dw(const void* gout, const void* x, const int32_t* ends, void* dw, int32_t dtype,
                                            int64_t rows, int64_t experts, int64_t n, int64_t k, void* work);
 
+/* The layer of a few tokens (1 .. 16) in one call: out = combine(down(a), r) of the routing r of logits (tokens x experts, of
+ * logits_dtype; experts 1 .. 1024, top_k 1 .. 64), a = act(up x), or with a gate act(gate x) up x; up and gate: experts x inter x
+ * hidden, down: experts x hidden x inter (inter and hidden 1 .. 2^22), gate NULL or not.  activation: ADAMBRIDGE_GELU (x Phi(x)) or
+ * _SILU (x / (1 + exp(-x))), else ADAMBRIDGE_EMVDTYPE.  The activations are rounded to the operands' type, nothing else but the
+ * result is.  work: adambridge_expert_mlp_work bytes, 16-byte aligned. */
+#define ADAMBRIDGE_GELU 0
+#define ADAMBRIDGE_SILU 1
+ADAMBRIDGE_API int64_t adambridge_expert_mlp_work(int32_t dtype, int64_t tokens, int64_t experts, int64_t top_k, int64_t inter, int64_t hidden);
+ADAMBRIDGE_API int adambridge_expert_mlp(const void* x, const void* logits, int32_t logits_dtype, const void* up, const void* gate, const void* down,
+                                         int32_t dtype, int64_t tokens, int64_t experts, int64_t top_k, int64_t inter, int64_t hidden,
+                                         int32_t activation, int32_t normalize, void* out, void* work);
+
 /* A language model's ends.  The reference has none of it but the loss above; types, addresses, sums, streams and codes as
  * those of the expert block's operators. */
 
@@ -576,6 +588,21 @@ ADAMBRIDGE_API int adambridge_embed(const void* ids, int32_t id_bytes, int64_t t
 ADAMBRIDGE_API int64_t adambridge_embed_work(int64_t tokens, int64_t vocab, int64_t hidden);
 ADAMBRIDGE_API int adambridge_embed_backward(const void* ids, int32_t id_bytes, int64_t tokens, const void* gout, int32_t dtype,
                                              int64_t vocab, int64_t hidden, float scale, int64_t padding, void* dweight, void* work);
+
+/* token_losses: losses[t] = log(sum over v of exp <hidden[t], weight[v]>) - <hidden[t], weight[targets[t]]> for rows (1 .. 2^23)
+ * of size values (a 16-byte piece of them, 8 BF16 or 4 FP32, to 2^20), weight: vocab x size (1 .. 2^22).  A row whose target is ignore_index
+ * has loss 0 and reaches nothing, whatever it holds; another target outside the vocabulary gives NaN (nothing is read for it).
+ * stats: NULL, or rows x 2 values that the gradient takes.  The backward call takes gout, a value a row, the gradient at the
+ * losses, and writes what is not NULL of dhidden (rows x size) and dweight (vocab x size), all of it, in the operands' type; the
+ * gradient at the logits is rounded to that type once on the way.  weight must hold what it held in the forward call.
+ * work: the _work functions' bytes, 16-byte aligned. */
+ADAMBRIDGE_API int64_t adambridge_token_losses_work(int32_t dtype, int64_t rows, int64_t vocab, int64_t hidden);
+ADAMBRIDGE_API int adambridge_token_losses(const void* hidden, const void* weight, int32_t dtype, const int64_t* targets, int64_t rows,
+                                           int64_t vocab, int64_t size, int64_t ignore_index, float* losses, float* stats, void* work);
+ADAMBRIDGE_API int64_t adambridge_token_losses_backward_work(int32_t dtype, int64_t rows, int64_t vocab, int64_t hidden);
+ADAMBRIDGE_API int adambridge_token_losses_backward(const float* gout, const void* hidden, const void* weight, int32_t dtype,
+                                                    const int64_t* targets, int64_t rows, int64_t vocab, int64_t size, int64_t ignore_index,
+                                                    const float* stats, void* dhidden, void* dweight, void* work);
 
 #ifdef __cplusplus
 }
