@@ -7,12 +7,11 @@
 //
 // The gradient's sums run over the tokens sorted by id, then by position, so that they have an order of their own and
 // dW is written once, by the words' rows, without atomics on values or a pass that clears it.  Text has a few words
-// very often: the tokens in their order are cut into chunks, and a word of more tokens than a chunk has is summed chunk
-// by chunk by as many workgroups, whose parts another kernel adds in order; any other word is one wavefront's.
+// very often: the sorted tokens are cut into chunks, and a word that has all tokens of a chunk is summed chunk by chunk by as
+// many workgroups, whose parts the word's wavefront adds in order; any other word's rows are its wavefront's.
 //
-// The sort: runs of 2048 (id, position) in a workgroup's LDS, then up to 32 runs at a time become one, each pair's
-// place being its own in its run plus how many of every other run are below it (a binary search each: all searches of a
-// lane are on their way at once).  Pairs differ, so the order is a total one.
+// The sort: runs of 4096 tokens by counting, then up to 32 runs at a time become one, each token's place being its own in its
+// run plus how many of every other run are below it.  (Id, position) pairs differ, so the order is a total one.
 
 #include <hip/hip_runtime.h>
 
@@ -24,11 +23,12 @@
 #include "abh_device.hpp"
 #include "abh_host.hpp"
 #include "abh_rows.hpp"
+#include "abh_tiles.hpp"
 
 namespace abh {
 
-constexpr int kRun = 2048, kSortThreads = 1024, kMergeRuns = 32;
-constexpr int kWords = 16;        // of a workgroup of k_embed_rows
+constexpr int kRun = 4096, kSortThreads = 1024;
+constexpr int kMostWords = 16;    // of a wavefront; fewer than its lanes
 constexpr int kLeastChunk = 64;   // tokens
 
 __device__ __forceinline__ int64_t id_at(const void* ids, int32_t id_bytes, int64_t i)
@@ -80,38 +80,48 @@ __global__ __launch_bounds__(256) void k_embed(EmbedArgs A)
 
 // ------------------------------------------------------------------------------- the sort
 
-// (id, position) in one word; an id outside the vocabulary is the vocabulary's size, behind all words.
+// Runs of kRun (id, position) in one word each; an id outside the vocabulary is the vocabulary's size, behind all words.  A token's place in
+// its run is counted: the tokens before it whose id is no larger, and those behind it whose id is smaller.  I tokens a workgroup,
+// each compared with the run's 4096 ids in the LDS by 1024 / I lanes.  (4096 tokens 4.5 us, where a sorting network in one
+// workgroup's LDS took 20; a run twice as long costs twice the comparisons and saves a step of the merge.)
+template <int I>
 __global__ __launch_bounds__(kSortThreads) void k_embed_sort(const void* ids, int32_t id_bytes, int64_t tokens, int64_t vocab, uint64_t* out)
 {
-    __shared__ uint64_t item[kRun];
-    const int64_t t0 = block_index() * kRun;
-    if (t0 >= tokens) return;
+    constexpr int S = kSortThreads / I, N = kRun / S, PAD = 4;   // S slices of N ids, 16 bytes apart: other banks
+    __shared__ __attribute__((aligned(16))) uint32_t key[S * (N + PAD)];
+    __shared__ uint32_t rank[I];
+    const int64_t i0 = block_index() * I, t0 = i0 / kRun * kRun;
+    if (i0 >= tokens) return;
     const int n = (int)(tokens - t0 < kRun ? tokens - t0 : kRun);
-    int size = 2;   // what is sorted: the next power of two
-    while (size < n) size *= 2;
-    for (int i = threadIdx.x; i < size; i += kSortThreads) {
-        uint64_t x = ~(uint64_t)0;
+    for (int i = threadIdx.x; i < kRun; i += kSortThreads) {
+        uint32_t x = ~0u;   // none
         if (i < n) {
             const int64_t id = id_at(ids, id_bytes, t0 + i);
-            x = (uint64_t)(id >= 0 && id < vocab ? id : vocab) << 32 | (uint32_t)(t0 + i);
+            x = (uint32_t)(id >= 0 && id < vocab ? id : vocab);
         }
-        item[i] = x;
+        key[i / N * (N + PAD) + i % N] = x;
+    }
+    if (threadIdx.x < I) rank[threadIdx.x] = 0;
+    __syncthreads();
+    const int item = (int)(i0 - t0) + (int)threadIdx.x % I, slice = threadIdx.x / I;
+    const uint32_t mine = key[item / N * (N + PAD) + item % N];
+    const uint32_t* const ids_of = key + slice * (N + PAD);
+    uint32_t below = 0;
+    if (slice * N < n) {
+        if (item / N != slice) {
+            const uint32_t limit = mine + (slice * N < item);
+#pragma unroll 4
+            for (int j = 0; j < N; j += 4) {
+                const raw16 k = *reinterpret_cast<const raw16*>(ids_of + j);
+                below += (k.x < limit) + (k.y < limit) + (k.z < limit) + (k.w < limit);
+            }
+        } else {
+            for (int j = 0; j < N; ++j) below += ids_of[j] < mine + (slice * N + j < item);
+        }
+        atomicAdd(&rank[threadIdx.x % I], below);
     }
     __syncthreads();
-    for (int k = 2; k <= size; k *= 2)
-        for (int j = k / 2; j > 0; j /= 2) {
-            const int i = threadIdx.x;
-            if (i < size / 2) {
-                const int a = (i & ~(j - 1)) << 1 | (i & (j - 1)), b = a | j;
-                const uint64_t x = item[a], y = item[b];
-                if ((x > y) == ((a & k) == 0)) {
-                    item[a] = y;
-                    item[b] = x;
-                }
-            }
-            __syncthreads();
-        }
-    for (int i = threadIdx.x; i < n; i += kSortThreads) out[t0 + i] = item[i];
+    if ((int)threadIdx.x < I && item < n) out[t0 + rank[threadIdx.x]] = (uint64_t)mine << 32 | (uint32_t)(t0 + item);
 }
 
 // How many of in[0 .. n) are below x.
@@ -126,29 +136,30 @@ __device__ __forceinline__ int64_t below(const uint64_t* in, int64_t n, uint64_t
     return lo;
 }
 
-// Runs of `run` sorted items, kMergeRuns of them at a time: one item a lane.
-__global__ __launch_bounds__(256) void k_embed_merge(const uint64_t* in, int64_t tokens, int64_t run, uint64_t* out)
+// Runs of `run` sorted items, R of them at a time: one item a lane, all runs' searches step by step together, every read taken
+// whether it counts or not, so that a step's reads overlap (65536 tokens 74 us with reads that wait for one another, 14 so).
+template <int R>
+__global__ __launch_bounds__(256) void k_embed_merge(const uint64_t* in, int64_t tokens, uint32_t run, uint64_t* out)
 {
     const int64_t i = block_index() * 256 + threadIdx.x;
     if (i >= tokens) return;
     const uint64_t x = in[i];
-    const int64_t mine = i / run, first = mine / kMergeRuns * kMergeRuns;
-    int64_t place = first * run + (i - mine * run);
-    // all runs' searches step by step together, so that their reads overlap
-    int32_t lo[kMergeRuns];
+    const uint32_t n = (uint32_t)tokens, mine = (uint32_t)i / run, first = mine / R * R;   // places below 2^31 + run
+    uint32_t place = first * run + ((uint32_t)i - mine * run), lo[R];
 #pragma unroll
-    for (int r = 0; r < kMergeRuns; ++r) lo[r] = 0;
-    int64_t step = 1;
-    while (step * 2 <= run) step *= 2;
-    for (; step > 0; step >>= 1) {
+    for (int r = 0; r < R; ++r) lo[r] = 0;
+    for (uint32_t step = run; step > 0; step >>= 1) {   // runs are powers of two
+        uint64_t y[R];
 #pragma unroll
-        for (int r = 0; r < kMergeRuns; ++r) {
-            const int64_t at = (first + r) * run + lo[r] + step - 1;   // below it: this and all before it are
-            if (lo[r] + step <= run && at < tokens && in[at] < x) lo[r] += (int32_t)step;
+        for (int r = 0; r < R; ++r) {
+            const uint32_t at = (first + r) * run + lo[r] + step - 1;   // below it: this and all before it are
+            y[r] = in[at < n ? at : n - 1];
         }
+#pragma unroll
+        for (int r = 0; r < R; ++r) lo[r] += lo[r] + step <= run && (first + r) * run + lo[r] + step <= n && y[r] < x ? step : 0u;
     }
 #pragma unroll
-    for (int r = 0; r < kMergeRuns; ++r) place += first + r == mine ? 0 : lo[r];
+    for (int r = 0; r < R; ++r) place += first + r == mine ? 0u : lo[r];
     out[place] = x;
 }
 
@@ -159,142 +170,188 @@ struct EmbedBackArgs {
     const void* gout;
     void* dweight;
     float* part;          // chunks x 2 x hidden
-    int64_t tokens, vocab, padding;
-    int32_t hidden, chunk;
+    int32_t* starts;      // vocab + 1
+    int64_t tokens, vocab, padding, part_blocks;
+    int32_t hidden, chunk, part_columns, words, pieces;   // words, pieces: of a wavefront of k_embed_rows, of a row
     float scale;
 };
 
 __device__ __forceinline__ uint32_t word_of(uint64_t item) { return (uint32_t)(item >> 32); }
 
-// Where a word's tokens begin and end, in lo .. hi.
-__device__ __forceinline__ int64_t first_of(const uint64_t* sorted, int64_t lo, int64_t hi, uint64_t word)
-{
-    return lo + below(sorted + lo, hi - lo, word << 32);
-}
-
-// Whether the word of the token at place p has more tokens than a chunk.
-__device__ __forceinline__ bool is_long(const EmbedBackArgs& A, int64_t p, uint32_t word)
-{
-    const int64_t lo = p > A.chunk ? p - A.chunk : 0, hi = p + A.chunk < A.tokens ? p + A.chunk + 1 : A.tokens;
-    return first_of(A.sorted, p, hi, (uint64_t)word + 1) - first_of(A.sorted, lo, p, word) > A.chunk;
-}
-
-// acc += the rows of g at the sorted places from .. to.
-template <int DT, int U>
-__device__ __forceinline__ void add_rows(const EmbedBackArgs& A, int64_t from, int64_t to, int32_t column, int32_t stride, float (&acc)[U][kLane<DT>])
-{
-    constexpr int L = kLane<DT>, AHEAD = 8 / U;
-    for (int64_t p = from; p < to; p += AHEAD) {
-        raw16 w[AHEAD][U];
-#pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
-            const int64_t place = p + a < to ? p + a : to - 1;
-            const void* row = at<DT>(A.gout, (int64_t)(uint32_t)A.sorted[place] * A.hidden);
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if (column + u * stride < A.hidden) w[a][u] = load_vec_raw<DT>(row, column + u * stride, A.hidden);
-        }
-#pragma unroll
-        for (int a = 0; a < AHEAD; ++a) {
-            if (p + a >= to) break;
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if (column + u * stride >= A.hidden) continue;
-                float x[L];
-                to_floats<DT>(w[a][u], x);
-#pragma unroll
-                for (int k = 0; k < L; ++k) acc[u][k] += x[k];
-            }
-        }
+// A lane's vector of a row.  One over the end of the row is the row's last whole one instead (then two lanes have the same
+// values, and store them); SHORT: rows of less than a vector.
+template <int DT, bool SHORT>
+struct Columns {
+    static constexpr int L = kLane<DT>;
+    int32_t first;
+    bool real;
+    __device__ __forceinline__ Columns(int32_t column, int32_t hidden) : first(SHORT || column + L <= hidden ? column : hidden - L), real(column < hidden) {}
+    __device__ __forceinline__ raw16 load(const void* row, int32_t hidden) const
+    {
+        if constexpr (SHORT) return real ? load_vec_raw<DT>(row, first, hidden) : raw16{0u, 0u, 0u, 0u};
+        else return load_raw<DT>(row, first);
     }
-}
-
-// A chunk's parts of the words that have more tokens than it: one that its first token belongs to, one that its last does.
-template <int DT>
-__global__ __launch_bounds__(256) void k_embed_parts(EmbedBackArgs A)
-{
-    constexpr int L = kLane<DT>;
-    const int64_t c = block_index(), p0 = c * A.chunk;
-    if (p0 >= A.tokens) return;
-    const int64_t p1 = p0 + A.chunk < A.tokens ? p0 + A.chunk : A.tokens;
-    const uint32_t first = word_of(A.sorted[p0]), last = word_of(A.sorted[p1 - 1]);
-    const int32_t column = (int32_t)(blockIdx.y * 256 + threadIdx.x) * L;
-    if (column >= A.hidden) return;
-#pragma unroll 1
-    for (int s = 0; s < 2; ++s) {
-        const uint32_t word = s ? last : first;
-        if ((s && last == first) || word >= A.vocab || word == A.padding || !is_long(A, s ? p1 - 1 : p0, word)) continue;
-        const int64_t from = s ? first_of(A.sorted, p0, p1, word) : p0, to = s ? p1 : first_of(A.sorted, p0, p1, (uint64_t)word + 1);
-        float acc[1][L];
-#pragma unroll
-        for (int k = 0; k < L; ++k) acc[0][k] = 0.0f;
-        add_rows<DT, 1>(A, from, to, column, 0, acc);
-        store_like<DT_F32, L>(A.part + (c * 2 + s) * A.hidden, column, A.hidden, acc[0]);
-    }
-}
-
-// The rows of the words of more tokens than a chunk, by the chunk they begin in (no two do in one).
-template <int DT>
-__global__ __launch_bounds__(256) void k_embed_long(EmbedBackArgs A)
-{
-    constexpr int L = kLane<DT>;
-    const int64_t c = block_index(), p0 = c * A.chunk;
-    if (p0 + A.chunk >= A.tokens) return;   // fewer tokens than a chunk's from here on
-    const int64_t p1 = p0 + A.chunk;
-    const uint32_t word = word_of(A.sorted[p1 - 1]);
-    if (word >= A.vocab || word == A.padding || (c > 0 && word_of(A.sorted[p0 - 1]) == word) || !is_long(A, p1 - 1, word)) return;
-    const int64_t from = first_of(A.sorted, p0, p1, word), to = first_of(A.sorted, p1, A.tokens, (uint64_t)word + 1);
-    const int32_t column = (int32_t)(blockIdx.y * 256 + threadIdx.x) * L;
-    if (column >= A.hidden) return;
-    float acc[L];
-#pragma unroll
-    for (int k = 0; k < L; ++k) acc[k] = 0.0f;
-    const int64_t end = (to - 1) / A.chunk;
-    const int s = from > p0;   // the other chunks begin with the word
-    for (int64_t q = c; q <= end; ++q) {
+    __device__ __forceinline__ void add(const raw16 w, float (&acc)[L]) const
+    {
         float x[L];
-        load_like<DT_F32, L>(A.part + (q * 2 + (q == c ? s : 0)) * A.hidden, column, A.hidden, 0.0f, x);
+        to_floats<DT>(w, x);
 #pragma unroll
         for (int k = 0; k < L; ++k) acc[k] += x[k];
     }
+    __device__ __forceinline__ void load_part(const float* part, int32_t hidden, float (&x)[L]) const
+    {
+        if constexpr (SHORT) {
+            load_like<DT_F32, L>(part, real ? first : 0, real ? hidden : 0, 0.0f, x);
+        } else {
 #pragma unroll
-    for (int k = 0; k < L; ++k) acc[k] *= A.scale;
-    stream_vec<DT>(at<DT>(A.dweight, (int64_t)word * A.hidden), column, A.hidden, acc);
+            for (int k = 0; k < L; k += 4) to_floats<DT_F32>(load_raw<DT_F32>(part, first + k), x + k);
+        }
+    }
+    __device__ __forceinline__ void store_part(float* part, int32_t hidden, const float (&x)[L]) const
+    {
+        if (!real) return;
+        if constexpr (SHORT) {
+            store_like<DT_F32, L>(part, first, hidden, x);
+        } else {
+#pragma unroll
+            for (int k = 0; k < L; k += 4) store_raw<DT_F32>(part, first + k, to_raw<DT_F32>(x + k));
+        }
+    }
+    __device__ __forceinline__ void stream(void* row, int32_t hidden, const float (&x)[L]) const
+    {
+        if (!real) return;
+        if constexpr (SHORT) stream_vec<DT>(row, first, hidden, x);
+        else stream_raw<DT>(row, first, to_raw<DT>(x));
+    }
+};
+
+// A word is long that all tokens of some chunk belong to.
+__device__ __forceinline__ bool is_long(const EmbedBackArgs& A, int from, int to)
+{
+    return (from + A.chunk - 1) / A.chunk * A.chunk + A.chunk <= to;
 }
 
-// All other rows, kWords words a workgroup, pieces of 64 x U vectors a wavefront.
-template <int DT, int U>
+// Two things at once.  The first workgroups: a chunk's parts of long words, of the one its first token belongs to and of the one its
+// last does.  The others: where each word's tokens begin, 256 words a workgroup.
+template <int DT, bool SHORT>
+__global__ __launch_bounds__(256) void k_embed_parts(EmbedBackArgs A)
+{
+    constexpr int L = kLane<DT>, AHEAD = 16;
+    const int64_t block = block_index();
+    if (block >= A.part_blocks) {
+        const int64_t v = (block - A.part_blocks) * 256 + threadIdx.x;
+        if (v <= A.vocab) A.starts[v] = (int32_t)below(A.sorted, A.tokens, (uint64_t)v << 32);
+        return;
+    }
+    const int64_t c = block / A.part_columns, p0 = c * A.chunk;
+    const int64_t p1 = p0 + A.chunk < A.tokens ? p0 + A.chunk : A.tokens, p2 = p1 + A.chunk;
+    const uint32_t first = word_of(A.sorted[p0]), last = word_of(A.sorted[p1 - 1]);
+    const uint32_t before = word_of(A.sorted[p0 >= A.chunk ? p0 - A.chunk : 0]), after = word_of(A.sorted[p2 <= A.tokens ? p2 - 1 : A.tokens - 1]);
+    const Columns<DT, SHORT> columns((int32_t)((block - c * A.part_columns) * 256 + threadIdx.x) * L, A.hidden);
+    const int lane = threadIdx.x & 63;
+#pragma unroll 1
+    for (int s = 0; s < 2; ++s) {
+        const uint32_t word = s ? last : first;
+        // the word has all of this chunk; of the one before, if it does not begin here; or of the next, if it begins here
+        const bool whole = first == last && p1 - p0 == A.chunk;
+        if (s ? first == last || p2 > A.tokens || after != word : !whole && (p0 < A.chunk || before != word)) continue;
+        if (word >= A.vocab || word == A.padding) continue;
+        int from = scalar((int)p0), to = scalar((int)p1);
+        if (first != last) {
+            const int edge = scalar((int)(p0 + below(A.sorted + p0, p1 - p0, (uint64_t)(s ? word : word + 1) << 32)));
+            from = s ? edge : from;
+            to = s ? to : edge;
+        }
+        float acc[L];
+#pragma unroll
+        for (int k = 0; k < L; ++k) acc[k] = 0.0f;
+        for (int p = from; p < to; p += kWave) {
+            const int n = to - p < kWave ? to - p : kWave;
+            const uint32_t position = (uint32_t)A.sorted[p + (lane < n ? lane : n - 1)];   // a lane reads one for its wavefront
+            for (int i = 0; i < n; i += AHEAD) {
+                raw16 w[AHEAD];
+#pragma unroll
+                for (int a = 0; a < AHEAD; ++a)
+                    w[a] = columns.load(at<DT>(A.gout, (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)position, i + a < n ? i + a : n - 1) * A.hidden), A.hidden);
+#pragma unroll
+                for (int a = 0; a < AHEAD; ++a)
+                    if (i + a < n) columns.add(w[a], acc);
+            }
+        }
+        columns.store_part(A.part + (c * 2 + s) * A.hidden, A.hidden, acc);
+    }
+}
+
+// dW: a wavefront has a piece of 64 vectors of A.words words' rows.  Their tokens lie together in the sorted order, and their rows are
+// loaded one after the other whichever word they belong to; a word is stored when its last one has been added.
+template <int DT, bool SHORT>
 __global__ __launch_bounds__(256) void k_embed_rows(EmbedBackArgs A)
 {
-    constexpr int L = kLane<DT>;
-    __shared__ int64_t bound[kWords + 1];
-    const int64_t v0 = block_index() * kWords;
+    constexpr int L = kLane<DT>, AHEAD = 8, N = 4;
+    const int lane = threadIdx.x & 63;
+    const int64_t item = block_index() * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+    const int64_t group = item / A.pieces, v0 = group * A.words;
     if (v0 >= A.vocab) return;
-    if (threadIdx.x <= kWords) bound[threadIdx.x] = first_of(A.sorted, 0, A.tokens, (uint64_t)v0 + threadIdx.x);
-    __syncthreads();
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
-    const int words = (int)(A.vocab - v0 < kWords ? A.vocab - v0 : kWords);
-    const int pieces = (A.hidden + 64 * U * L - 1) / (64 * U * L);
-    for (int i = wave; i < words * pieces; i += 4) {
-        const int w = i / pieces;
-        const int64_t from = bound[w], to = v0 + w == A.padding ? from : bound[w + 1];
-        if (to - from > A.chunk) continue;   // k_embed_long's
-        const int32_t column = (i - w * pieces) * (64 * U * L) + lane * L;
-        if (column >= A.hidden) continue;
-        float acc[U][L];
+    const int words = (int)(A.vocab - v0 < A.words ? A.vocab - v0 : A.words);
+    const Columns<DT, SHORT> columns((int32_t)(item - group * A.pieces) * (64 * L) + lane * L, A.hidden);
+    const int start = A.starts[v0 + (lane < words ? lane : words)], next = __shfl_down(start, 1);
+    // words that are not sums of their rows: the padding, and long ones
+    uint64_t apart = __builtin_amdgcn_ballot_w64(lane < words && (v0 + lane == A.padding || is_long(A, start, next)));
+    float acc[L];
+    auto clear = [&]() {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int k = 0; k < L; ++k) acc[k] = 0.0f;
+    };
+    auto flush = [&](int w) {
 #pragma unroll
-            for (int k = 0; k < L; ++k) acc[u][k] = 0.0f;
-        add_rows<DT, U>(A, from, to, column, 64 * L, acc);
-        void* out = at<DT>(A.dweight, (v0 + w) * A.hidden);
+        for (int k = 0; k < L; ++k) acc[k] *= A.scale;
+        columns.stream(at<DT>(A.dweight, (v0 + w) * A.hidden), A.hidden, acc);
+        clear();
+    };
+    clear();
+    for (int w = 0; w < words;) {
+        const int stop = apart ? __builtin_ctzll(apart) : words;   // words w .. stop are sums of their rows
+        const int to = __builtin_amdgcn_readlane(start, stop);
+        int end = __builtin_amdgcn_readlane(start, w + 1);
+        for (int p = __builtin_amdgcn_readlane(start, w); p < to; p += kWave) {
+            const int n = to - p < kWave ? to - p : kWave;
+            const uint32_t position = (uint32_t)A.sorted[p + (lane < n ? lane : n - 1)];
+            for (int i = 0; i < n; i += AHEAD) {
+                raw16 row[AHEAD];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (column + u * 64 * L >= A.hidden) continue;
+                for (int a = 0; a < AHEAD; ++a)
+                    row[a] = columns.load(at<DT>(A.gout, (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)position, i + a < n ? i + a : n - 1) * A.hidden), A.hidden);
 #pragma unroll
-            for (int k = 0; k < L; ++k) acc[u][k] *= A.scale;
-            stream_vec<DT>(out, column + u * 64 * L, A.hidden, acc[u]);
+                for (int a = 0; a < AHEAD; ++a)
+                    if (i + a < n) {
+                        while (p + i + a >= end) {
+                            flush(w);
+                            end = __builtin_amdgcn_readlane(start, ++w + 1);
+                        }
+                        columns.add(row[a], acc);
+                    }
+            }
         }
+        for (; w < stop; ++w) flush(w);
+        if (!apart) continue;
+        apart &= apart - 1;
+        if (v0 + w != A.padding) {   // its chunks' parts, in order: the other word's in the first chunk, unless it begins with it
+            const int from = __builtin_amdgcn_readlane(start, w), q0 = from / A.chunk, q1 = (__builtin_amdgcn_readlane(start, w + 1) - 1) / A.chunk;
+            for (int q = q0; q <= q1; q += N) {
+                float x[N][L];
+#pragma unroll
+                for (int a = 0; a < N; ++a) {
+                    const int qa = q + a <= q1 ? q + a : q1;
+                    columns.load_part(A.part + ((int64_t)qa * 2 + (qa == q0 && from % A.chunk != 0)) * A.hidden, A.hidden, x[a]);
+                }
+#pragma unroll
+                for (int a = 0; a < N; ++a)
+                    if (q + a <= q1)
+#pragma unroll
+                        for (int k = 0; k < L; ++k) acc[k] += x[a][k];
+            }
+        }
+        flush(w++);
     }
 }
 
@@ -312,13 +369,13 @@ static int embed_check(int32_t id_bytes, int64_t tokens, int32_t dtype, int64_t 
 // Tokens of a chunk: so many that there are at most 1024 chunks, whose parts are at most 8 KB times the row's values.
 static int64_t chunk_of(int64_t tokens)
 {
-    return std::max<int64_t>(kLeastChunk, (tokens + 1023) / 1024);
+    return std::max<int64_t>(kLeastChunk, ((tokens + 1023) / 1024 + 63) / 64 * 64);
 }
 
 static int64_t part_bytes(int64_t tokens, int64_t hidden)
 {
     const int64_t chunk = chunk_of(tokens);
-    return tokens > chunk ? (tokens + chunk - 1) / chunk * 2 * hidden * 4 : 0;   // else no word is longer than a chunk
+    return tokens >= chunk ? (tokens + chunk - 1) / chunk * 2 * hidden * 4 : 0;   // else no word has a whole chunk
 }
 
 template <int DT>
@@ -338,17 +395,22 @@ static void launch_embed(EmbedArgs& A)
 }
 
 template <int DT>
-static void launch_embed_back(const EmbedBackArgs& A)
+static void launch_embed_back(EmbedBackArgs& A)
 {
     const int vectors = (A.hidden + kLane<DT> - 1) / kLane<DT>;
-    if (A.tokens > A.chunk) {
-        const dim3 grid = block_grid((A.tokens + A.chunk - 1) / A.chunk, (vectors + 255) / 256);
-        hipLaunchKernelGGL((k_embed_parts<DT>), grid, dim3(256), 0, t_stream, A);
-        hipLaunchKernelGGL((k_embed_long<DT>), grid, dim3(256), 0, t_stream, A);
-    }
-    const dim3 grid = block_grid((A.vocab + kWords - 1) / kWords);
-    if (vectors <= 64) hipLaunchKernelGGL((k_embed_rows<DT, 1>), grid, dim3(256), 0, t_stream, A);
-    else hipLaunchKernelGGL((k_embed_rows<DT, 2>), grid, dim3(256), 0, t_stream, A);
+    A.part_columns = (vectors + 255) / 256;
+    A.part_blocks = A.tokens >= A.chunk ? (A.tokens + A.chunk - 1) / A.chunk * A.part_columns : 0;
+    const bool tiny = A.hidden < kLane<DT>;
+    const dim3 parts = block_grid(A.part_blocks + (A.vocab + 256) / 256);
+    if (tiny) hipLaunchKernelGGL((k_embed_parts<DT, true>), parts, dim3(256), 0, t_stream, A);
+    else hipLaunchKernelGGL((k_embed_parts<DT, false>), parts, dim3(256), 0, t_stream, A);
+    A.pieces = (vectors + 63) / 64;
+    // 16 words a wavefront, or fewer where that leaves wavefronts too few
+    A.words = kMostWords;
+    while (A.words > 2 && (A.vocab + A.words - 1) / A.words * A.pieces < 4096) A.words /= 2;
+    const dim3 grid = block_grid(((A.vocab + A.words - 1) / A.words * A.pieces + 3) / 4);
+    if (tiny) hipLaunchKernelGGL((k_embed_rows<DT, true>), grid, dim3(256), 0, t_stream, A);
+    else hipLaunchKernelGGL((k_embed_rows<DT, false>), grid, dim3(256), 0, t_stream, A);
 }
 
 }  // namespace abh
@@ -373,7 +435,7 @@ ADAMBRIDGE_API int adambridge_embed(const void* ids, int32_t id_bytes, int64_t t
 ADAMBRIDGE_API int64_t adambridge_embed_work(int64_t tokens, int64_t vocab, int64_t hidden)
 {
     const int rc = embed_check(8, tokens, ADAMBRIDGE_DT_F32, vocab, hidden);
-    return rc ? rc : (tokens > kRun ? 2 : 1) * tokens * 8 + part_bytes(tokens, hidden);
+    return rc ? rc : (tokens > kRun ? 2 : 1) * tokens * 8 + part_bytes(tokens, hidden) + (vocab + 1) * 4;
 }
 
 ADAMBRIDGE_API int adambridge_embed_backward(const void* ids, int32_t id_bytes, int64_t tokens, const void* gout, int32_t dtype,
@@ -385,13 +447,32 @@ ADAMBRIDGE_API int adambridge_embed_backward(const void* ids, int32_t id_bytes, 
     if ((uintptr_t)work % 8) return ADAMBRIDGE_EALIGN;
     uint64_t* sorted = static_cast<uint64_t*>(work);
     uint64_t* other = tokens > kRun ? sorted + tokens : nullptr;
-    hipLaunchKernelGGL(k_embed_sort, block_grid((tokens + kRun - 1) / kRun), dim3(kSortThreads), 0, t_stream, ids, id_bytes, tokens, vocab, sorted);
+    // few tokens over many CUs; many read their run's ids a quarter as often
+    if (tokens <= 4 * kRun) hipLaunchKernelGGL((k_embed_sort<16>), block_grid((tokens + 15) / 16), dim3(kSortThreads), 0, t_stream, ids, id_bytes, tokens, vocab, sorted);
+    else hipLaunchKernelGGL((k_embed_sort<64>), block_grid((tokens + 63) / 64), dim3(kSortThreads), 0, t_stream, ids, id_bytes, tokens, vocab, sorted);
     float* const part = reinterpret_cast<float*>(sorted + (tokens > kRun ? 2 : 1) * tokens);
-    for (int64_t run = kRun; run < tokens; run *= kMergeRuns) {
-        hipLaunchKernelGGL(k_embed_merge, block_grid((tokens + 255) / 256), dim3(256), 0, t_stream, sorted, tokens, run, other);
+    for (int64_t run = kRun; run < tokens;) {
+        const dim3 grid = block_grid((tokens + 255) / 256);
+        const int64_t runs = (tokens + run - 1) / run;
+        if (runs <= 4) hipLaunchKernelGGL((k_embed_merge<4>), grid, dim3(256), 0, t_stream, sorted, tokens, (uint32_t)run, other);
+        else if (runs <= 8) hipLaunchKernelGGL((k_embed_merge<8>), grid, dim3(256), 0, t_stream, sorted, tokens, (uint32_t)run, other);
+        else if (runs <= 16) hipLaunchKernelGGL((k_embed_merge<16>), grid, dim3(256), 0, t_stream, sorted, tokens, (uint32_t)run, other);
+        else hipLaunchKernelGGL((k_embed_merge<32>), grid, dim3(256), 0, t_stream, sorted, tokens, (uint32_t)run, other);
+        run *= runs <= 4 ? 4 : runs <= 8 ? 8 : runs <= 16 ? 16 : 32;
         std::swap(sorted, other);
     }
-    const EmbedBackArgs A{sorted, gout, dweight, part, tokens, vocab, padding, (int32_t)hidden, (int32_t)chunk_of(tokens), scale};
+    EmbedBackArgs A{};
+    A.sorted = sorted;
+    A.gout = gout;
+    A.dweight = dweight;
+    A.part = part;
+    A.starts = reinterpret_cast<int32_t*>(reinterpret_cast<uint8_t*>(part) + part_bytes(tokens, hidden));
+    A.tokens = tokens;
+    A.vocab = vocab;
+    A.padding = padding;
+    A.hidden = (int32_t)hidden;
+    A.chunk = (int32_t)chunk_of(tokens);
+    A.scale = scale;
     if (dtype == ADAMBRIDGE_DT_BF16) launch_embed_back<DT_BF16>(A);
     else launch_embed_back<DT_F32>(A);
     const hipError_t e = hipGetLastError();

@@ -32,7 +32,7 @@ namespace abh {
 constexpr float kHeadLog2e = 1.4426950408889634f;
 constexpr float kHeadNegInf = -__builtin_inff();
 constexpr int kHeadCus = 256;
-constexpr int kFewRows = 64;         // at most, for k_head_few
+constexpr int kFewRows = 64, kFewGroups = 2;   // k_head_few's rows at most, and words by 16 of a wavefront
 constexpr int kFinishLanes = 1024;
 
 // A maximum and the sum of exp(x - m) over what was seen.  m = -inf: nothing above -inf yet.
@@ -252,49 +252,70 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_sums(HeadArgs A)
     }
 }
 
-// The same of few rows: the weights are read once, 16 words a wavefront.  part: workgroups x rows.
+// The same of few rows: the weights are read once, NG times 16 words a wavefront, which share the rows' loads.  part: workgroups x
+// rows.
 template <int DT, bool EVEN>
 __global__ __launch_bounds__(256) void k_head_few(HeadArgs A)
 {
-    constexpr int V = kLane<DT>, STEP = 4 * V, CH = kFewRows / 16, U = 8;
+    constexpr int V = kLane<DT>, STEP = 4 * V, CH = kFewRows / 16, NG = kFewGroups, U = 4;
     __shared__ Sums row_sums[4][kFewRows];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int col = lane & 15, quarter = lane >> 4;
-    const int64_t j0 = (block_index() * 4 + wave) * 16;
-    const int words = j0 >= A.vocab ? 0 : (int)(A.vocab - j0 < 16 ? A.vocab - j0 : 16);
-    const int steps = (A.hidden + STEP - 1) / STEP;
+    const int64_t j0 = (block_index() * 4 + wave) * (16 * NG);
+    const int words = j0 >= A.vocab ? 0 : (int)(A.vocab - j0 < 16 * NG ? A.vocab - j0 : 16 * NG);
+    const int steps = words ? (A.hidden + STEP - 1) / STEP : 0;
     const Pieces<DT, EVEN> w{at<DT>(A.w, (words ? j0 : 0) * A.hidden), (uint32_t)(words * A.hidden * kSize<DT>), A.hidden, words};
     const Pieces<DT, EVEN> x{static_cast<const uint8_t*>(A.h), (uint32_t)(A.rows * A.hidden * kSize<DT>), A.hidden, A.rows};
-    mm_f32x4 acc[CH];
+    mm_f32x4 acc[CH][NG];
 #pragma unroll
-    for (int c = 0; c < CH; ++c) acc[c] = mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (words)
-        for (int s = 0; s < steps; s += U) {
-            raw16 wv[U];
+    for (int c = 0; c < CH; ++c)
 #pragma unroll
-            for (int u = 0; u < U; ++u) wv[u] = w.load(col, (s + u) * STEP + quarter * V, s + u < steps);
+        for (int n = 0; n < NG; ++n) acc[c][n] = mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    raw16 even[NG][U], odd[NG][U];
+    auto load = [&](int s, raw16 (&to)[NG][U]) {
 #pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                if (16 * c >= A.rows) break;
-                raw16 xv[U];
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int u = 0; u < U; ++u) xv[u] = x.load(16 * c + col, (s + u) * STEP + quarter * V, s + u < steps);
-                mm_f32x4 some = DT == DT_BF16 ? acc[c] : mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};   // FP32: short chains of sums
+            for (int n = 0; n < NG; ++n) to[n][u] = w.load(16 * n + col, (s + u) * STEP + quarter * V, s + u < steps);
+    };
+    // loads arrive in their order: a step's rows are asked for before the next one's weights, which are then on their way while
+    // this one is multiplied
+    auto turn = [&](int s, const raw16 (&now)[NG][U], raw16 (&next)[NG][U]) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            if (16 * c >= A.rows) break;
+            raw16 xv[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) xv[u] = x.load(16 * c + col, (s + u) * STEP + quarter * V, s + u < steps);
+            if (c == 0) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (s + U < steps) load(s + U, next);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int n = 0; n < NG; ++n) {
+                mm_f32x4 some = DT == DT_BF16 ? acc[c][n] : mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};   // FP32: short chains of sums
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     if constexpr (DT == DT_BF16) {
-                        some = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mm_bf16x8, wv[u]),
+                        some = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mm_bf16x8, now[n][u]),
                                                                        __builtin_bit_cast(mm_bf16x8, xv[u]), some, 0, 0, 0);
                     } else {
-                        const mm_f32x4 wf = __builtin_bit_cast(mm_f32x4, wv[u]), xf = __builtin_bit_cast(mm_f32x4, xv[u]);
+                        const mm_f32x4 wf = __builtin_bit_cast(mm_f32x4, now[n][u]), xf = __builtin_bit_cast(mm_f32x4, xv[u]);
 #pragma unroll
                         for (int q = 0; q < 4; ++q) some = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[q], xf[q], some, 0, 0, 0);
                     }
                 }
-                if constexpr (DT == DT_BF16) acc[c] = some;
-                else acc[c] += some;
+                if constexpr (DT == DT_BF16) acc[c][n] = some;
+                else acc[c][n] += some;
             }
         }
+    };
+    if (steps) load(0, even);
+    for (int s = 0; s < steps; s += 2 * U) {
+        turn(s, even, odd);
+        if (s + U < steps) turn(s + U, odd, even);
+    }
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         if (16 * c >= A.rows) break;
@@ -302,17 +323,21 @@ __global__ __launch_bounds__(256) void k_head_few(HeadArgs A)
         const int64_t target = row < A.rows ? A.targets[row] - j0 : -1;
         Sums all{kHeadNegInf, 0.0f};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int word = 4 * quarter + r;
-            if (word >= words) acc[c][r] = kHeadNegInf;
-            else if (word == target) A.picked[row] = acc[c][r];
-            all.m = __builtin_fmaxf(all.m, acc[c][r]);
-        }
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int word = 16 * n + 4 * quarter + r;
+                if (word >= words) acc[c][n][r] = kHeadNegInf;
+                else if (word == target) A.picked[row] = acc[c][n][r];
+                all.m = __builtin_fmaxf(all.m, acc[c][n][r]);
+            }
         all.m = __builtin_fmaxf(all.m, __shfl_xor(all.m, 16));
         all.m = __builtin_fmaxf(all.m, __shfl_xor(all.m, 32));
         const float shift = shift_for(all.m);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) all.s += exp_of(acc[c][r], shift);
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) all.s += exp_of(acc[c][n][r], shift);
         all.s += __shfl_xor(all.s, 16);
         all.s += __shfl_xor(all.s, 32);
         if (quarter == 0) row_sums[wave][row] = all;
@@ -567,7 +592,7 @@ struct HeadForward {
     {
         few = rows <= kFewRows;
         tile = dtype == ADAMBRIDGE_DT_BF16 ? LargeTile::BM : f32_tile((rows + 127) / 128 * ((vocab + 127) / 128));
-        parts = (int)(few ? (vocab + 63) / 64 : (vocab + tile - 1) / tile);
+        parts = (int)(few ? (vocab + 64 * kFewGroups - 1) / (64 * kFewGroups) : (vocab + tile - 1) / tile);
         Scratch s{static_cast<uint8_t*>(work)};
         picked = s.take<float>(rows);
         part = s.take<Sums>(parts * rows);

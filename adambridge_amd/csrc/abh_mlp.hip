@@ -29,7 +29,7 @@
 namespace abh {
 
 constexpr int kMlpTokens = 16, kMlpExperts = 1024, kMlpChosen = 64;
-constexpr int kMlpColumns = 16;   // of a workgroup
+constexpr int kMlpColumns = 16;   // a matrix instruction's
 constexpr int kUpWaves = 4, kDownWaves = 16;
 
 // A chosen expert: which tokens chose it, and their weights.
@@ -115,11 +115,11 @@ __device__ __forceinline__ void choose(const MlpArgs& A, uint32_t* mask, int32_t
     __syncthreads();
 }
 
-// 16 columns of up (and gate) of the blockIdx-th chosen expert: the wavefronts split the sum, the first adds their parts in order.
-template <int DT, bool EVEN, bool GATE, int NV>
+// 16 NG columns of up (and gate) of the blockIdx-th chosen expert: the wavefronts split the sum, the first adds their parts in order.
+template <int DT, bool EVEN, bool GATE, int NG, int NV>
 __global__ __launch_bounds__(kUpWaves * kWave) void k_mlp_up(MlpArgs A)
 {
-    constexpr int V = kLane<DT>, STEP = 4 * V, W = kUpWaves, M = GATE ? 2 : 1, U = GATE ? 4 : 8;
+    constexpr int V = kLane<DT>, STEP = 4 * V, W = kUpWaves, M = (GATE ? 2 : 1) * NG, U = 8 / M, COLS = kMlpColumns * NG;   // M: up's columns, then gate's
     __shared__ uint32_t mask[kMlpExperts];
     __shared__ int32_t expert[kMlpTokens * kMlpChosen];
     __shared__ float weight[kMlpTokens * kMlpChosen];
@@ -127,7 +127,7 @@ __global__ __launch_bounds__(kUpWaves * kWave) void k_mlp_up(MlpArgs A)
     choose<NV>(A, mask, expert, weight);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int col = lane & 15, quarter = lane >> 4;
-    const int block = (int)block_index(), rank = block / A.columns, j0 = (block - rank * A.columns) * kMlpColumns;
+    const int block = (int)block_index(), rank = block / A.columns, j0 = (block - rank * A.columns) * COLS;
     int e = -1, skip = rank, before = 0;
     for (int e0 = 0; e0 < A.experts; e0 += kWave) {
         const uint64_t with = __builtin_amdgcn_ballot_w64(e0 + lane < A.experts && mask[e0 + lane < A.experts ? e0 + lane : 0] != 0);
@@ -155,32 +155,40 @@ __global__ __launch_bounds__(kUpWaves * kWave) void k_mlp_up(MlpArgs A)
         }
     }
     const int steps = (A.hidden + STEP - 1) / STEP, s0 = steps * wave / W, s1 = steps * (wave + 1) / W;
-    const int columns = A.inter - j0 < kMlpColumns ? A.inter - j0 : kMlpColumns;
-    const int64_t first = ((int64_t)e * A.inter + j0) * A.hidden;
-    const uint32_t bytes = (uint32_t)(columns * A.hidden * kSize<DT>);
-    const Pieces<DT, EVEN> w[2] = {{at<DT>(A.up, first), bytes, A.hidden, columns}, {at<DT>(GATE ? A.gate : A.up, first), bytes, A.hidden, columns}};
+    Pieces<DT, EVEN> w[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        const int j = j0 + m % NG * kMlpColumns, columns = A.inter - j < kMlpColumns ? A.inter - j < 0 ? 0 : A.inter - j : kMlpColumns;
+        w[m] = {at<DT>(m < NG ? A.up : A.gate, ((int64_t)e * A.inter + (columns ? j : 0)) * A.hidden), (uint32_t)(columns * A.hidden * kSize<DT>), A.hidden, columns};
+    }
     const Pieces<DT, EVEN> x{static_cast<const uint8_t*>(A.x), (uint32_t)(A.tokens * A.hidden * kSize<DT>), A.hidden, A.tokens};
     mm_f32x4 acc[M];
 #pragma unroll
     for (int m = 0; m < M; ++m) acc[m] = mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = s0; s < s1; s += U) {
-        raw16 wv[M][U], xv[U];
+    raw16 even[M][U], odd[M][U];
+    auto load = [&](int s, raw16 (&to)[M][U]) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int m = 0; m < M; ++m) wv[m][u] = w[m].load(col, (s + u) * STEP + quarter * V, s + u < s1);
+            for (int m = 0; m < M; ++m) to[m][u] = w[m].load(col, (s + u) * STEP + quarter * V, s + u < s1);
+    };
+    auto turn = [&](int s, const raw16 (&now)[M][U], raw16 (&next)[M][U]) {   // as k_mlp_down's
+        raw16 xv[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) xv[u] = x.load(col, (s + u) * STEP + quarter * V, s + u < s1);
+        __builtin_amdgcn_sched_barrier(0);
+        if (s + U < s1) load(s + U, next);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int m = 0; m < M; ++m) {
             mm_f32x4 some = DT == DT_BF16 ? acc[m] : mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};   // FP32: short chains of sums
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 if constexpr (DT == DT_BF16) {
-                    some = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mm_bf16x8, wv[m][u]), __builtin_bit_cast(mm_bf16x8, xv[u]), some,
+                    some = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mm_bf16x8, now[m][u]), __builtin_bit_cast(mm_bf16x8, xv[u]), some,
                                                                    0, 0, 0);
                 } else {
-                    const mm_f32x4 wf = __builtin_bit_cast(mm_f32x4, wv[m][u]), xf = __builtin_bit_cast(mm_f32x4, xv[u]);
+                    const mm_f32x4 wf = __builtin_bit_cast(mm_f32x4, now[m][u]), xf = __builtin_bit_cast(mm_f32x4, xv[u]);
 #pragma unroll
                     for (int q = 0; q < 4; ++q) some = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[q], xf[q], some, 0, 0, 0);
                 }
@@ -188,6 +196,11 @@ __global__ __launch_bounds__(kUpWaves * kWave) void k_mlp_up(MlpArgs A)
             if constexpr (DT == DT_BF16) acc[m] = some;
             else acc[m] += some;
         }
+    };
+    if (s0 < s1) load(s0, even);
+    for (int s = s0; s < s1; s += 2 * U) {
+        turn(s, even, odd);
+        if (s + U < s1) turn(s + U, odd, even);
     }
     if (wave > 0)
 #pragma unroll
@@ -200,59 +213,89 @@ __global__ __launch_bounds__(kUpWaves * kWave) void k_mlp_up(MlpArgs A)
         for (int m = 0; m < M; ++m) acc[m] += parts[p][m][lane];
     void* row = at<DT>(A.a, ((int64_t)rank * kMlpTokens + col) * A.inter);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const float y = GATE ? activated(acc[M - 1][r], A.silu) * acc[0][r] : activated(acc[0][r], A.silu);
-        if (j0 + 4 * quarter + r < A.inter) put<DT>(row, j0 + 4 * quarter + r, y);
-    }
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int j = j0 + n * kMlpColumns + 4 * quarter + r;
+            const float y = GATE ? activated(acc[M - NG + n][r], A.silu) * acc[n][r] : activated(acc[n][r], A.silu);
+            if (j < A.inter) put<DT>(row, j, y);
+        }
 }
 
-// 16 columns of the result: the wavefronts share the chosen experts' pieces of U steps, whose products are weighted and added in
-// the order of the experts, then the wavefronts' parts in theirs.
-template <int DT, bool EVEN>
+// COLS columns of the result: the wavefronts share the chosen experts' pieces of U loads, whose products are weighted and added in
+// the order of the experts, then the wavefronts' parts in theirs.  Fewer than 16 columns leave rows of the matrix instruction for
+// other terms of the same columns (G slices of 4 lanes' vectors each, multiplied one slice at a time; a product's other rows are not
+// looked at): 2048 columns are 256 workgroups of 8, a CU each, where 128 of 16 reach 3.0 TB/s.
+template <int DT, bool EVEN, int COLS>
 __global__ __launch_bounds__(kDownWaves * kWave) void k_mlp_down(MlpArgs A)
 {
-    constexpr int V = kLane<DT>, STEP = 4 * V, W = kDownWaves, U = 8;
+    constexpr int V = kLane<DT>, STEP = 4 * V, W = kDownWaves, G = 16 / COLS, U = 4, PIECE = U * G * STEP;
     __shared__ mm_f32x4 parts[W][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int col = lane & 15, quarter = lane >> 4;
-    const int j0 = (int)block_index() * kMlpColumns, columns = A.hidden - j0 < kMlpColumns ? A.hidden - j0 : kMlpColumns;
-    const int pieces = (A.inter + U * STEP - 1) / (U * STEP), items = scalar(*A.count) * pieces;
+    const int j0 = (int)block_index() * COLS, columns = A.hidden - j0 < COLS ? A.hidden - j0 : COLS;
+    const int pieces = (A.inter + PIECE - 1) / PIECE, items = scalar(*A.count) * pieces;
     mm_f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int i = wave; i < items; i += W) {
-        const int rank = i / pieces, k0 = (i - rank * pieces) * (U * STEP);
-        const Chosen* const c = A.list + rank;
-        const int e = scalar(c->expert);
-        const bool mine = c->tokens >> col & 1;
+    raw16 even[U], odd[U];
+    auto load = [&](int i, raw16 (&to)[U]) {
+        const int rank = i / pieces, k0 = (i - rank * pieces) * PIECE + (col / COLS * 4 + quarter) * V;
+        const int e = scalar(A.list[rank].expert);
         const Pieces<DT, EVEN> w{at<DT>(A.down, ((int64_t)e * A.hidden + j0) * A.inter), (uint32_t)(columns * A.inter * kSize<DT>), A.inter, columns};
-        const Pieces<DT, EVEN> a{at<DT>(A.a, (int64_t)rank * kMlpTokens * A.inter), (uint32_t)(kMlpTokens * A.inter * kSize<DT>), A.inter, kMlpTokens};
-        raw16 wv[U], av[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) wv[u] = w.load(col, k0 + u * STEP + quarter * V, true);
-#pragma unroll
-        for (int u = 0; u < U; ++u) av[u] = a.load(col, k0 + u * STEP + quarter * V, mine);   // another token's row: never written
-        mm_f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if constexpr (DT == DT_BF16) {
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mm_bf16x8, wv[u]), __builtin_bit_cast(mm_bf16x8, av[u]), acc, 0, 0, 0);
-            } else {
-                const mm_f32x4 wf = __builtin_bit_cast(mm_f32x4, wv[u]), af = __builtin_bit_cast(mm_f32x4, av[u]);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[q], af[q], acc, 0, 0, 0);
-            }
-        }
+        for (int u = 0; u < U; ++u) to[u] = w.load(col % COLS, k0 + u * G * STEP, true);
+    };
+    // loads arrive in their order: this piece's activations are asked for before the next piece's weights, which are then on their
+    // way while this one is multiplied
+    auto turn = [&](int i, const raw16 (&now)[U], raw16 (&next)[U]) {
+        const int rank = i / pieces, k0 = (i - rank * pieces) * PIECE + quarter * V;
+        const Chosen* const c = A.list + rank;
+        const bool mine = c->tokens >> col & 1;
         const float by = c->weight[col];
+        const Pieces<DT, EVEN> a{at<DT>(A.a, (int64_t)rank * kMlpTokens * A.inter), (uint32_t)(kMlpTokens * A.inter * kSize<DT>), A.inter, kMlpTokens};
+        raw16 av[G][U];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) sum[r] = mine ? sum[r] + by * acc[r] : sum[r];   // what an expert holds stays with its tokens
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int u = 0; u < U; ++u) av[g][u] = a.load(col, k0 + (u * G + g) * STEP, mine);   // another token's row: never written
+        __builtin_amdgcn_sched_barrier(0);
+        if (i + W < items) load(i + W, next);
+        __builtin_amdgcn_sched_barrier(0);
+        mm_f32x4 product{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            mm_f32x4 acc{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                if constexpr (DT == DT_BF16) {
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mm_bf16x8, now[u]), __builtin_bit_cast(mm_bf16x8, av[g][u]), acc, 0, 0, 0);
+                } else {
+                    const mm_f32x4 wf = __builtin_bit_cast(mm_f32x4, now[u]), af = __builtin_bit_cast(mm_f32x4, av[g][u]);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[q], af[q], acc, 0, 0, 0);
+                }
+            }
+            const bool slice = 4 * quarter / COLS == g;   // whose rows this lane holds
+#pragma unroll
+            for (int r = 0; r < 4; ++r) product[r] = slice ? acc[r] : product[r];
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[r] = mine ? sum[r] + by * product[r] : sum[r];   // what an expert holds stays with its tokens
+    };
+    if (wave < items) load(wave, even);
+    for (int i = wave; i < items; i += 2 * W) {
+        turn(i, even, odd);
+        if (i + W < items) turn(i + W, odd, even);
     }
     parts[wave][lane] = sum;
     __syncthreads();
-    if (threadIdx.x >= kMlpTokens * kMlpColumns) return;
-    const int token = threadIdx.x / kMlpColumns, j = threadIdx.x % kMlpColumns;
+    if (threadIdx.x >= kMlpTokens * COLS) return;
+    const int token = threadIdx.x / COLS, j = threadIdx.x % COLS;
     if (token >= A.tokens || j >= columns) return;
     float y = 0.0f;
 #pragma unroll
-    for (int p = 0; p < W; ++p) y += parts[p][j / 4 * 16 + token][j % 4];
+    for (int p = 0; p < W; ++p)
+#pragma unroll
+        for (int g = 0; g < G; ++g) y += parts[p][(g * COLS + j) / 4 * 16 + token][(g * COLS + j) % 4];
     put<DT>(A.out, (int64_t)token * A.hidden + j0 + j, y);
 }
 
@@ -272,28 +315,45 @@ static int mlp_check(int32_t dtype, int64_t tokens, int64_t experts, int64_t top
 // Scratch: how many experts are chosen, which, and their activations, at 256 bytes each.
 static int64_t list_bytes(int64_t used) { return (used * (int64_t)sizeof(Chosen) + 255) / 256 * 256; }
 
-template <int DT, bool EVEN, bool GATE>
+template <int DT, bool EVEN, bool GATE, int NG>
 static void launch_up(const MlpArgs& A, const dim3 grid)
 {
     const dim3 block(kUpWaves * kWave);
-    if (A.experts <= 64) hipLaunchKernelGGL((k_mlp_up<DT, EVEN, GATE, 1>), grid, block, 0, t_stream, A);
-    else if (A.experts <= 256) hipLaunchKernelGGL((k_mlp_up<DT, EVEN, GATE, 4>), grid, block, 0, t_stream, A);
-    else hipLaunchKernelGGL((k_mlp_up<DT, EVEN, GATE, 16>), grid, block, 0, t_stream, A);
+    if (A.experts <= 64) hipLaunchKernelGGL((k_mlp_up<DT, EVEN, GATE, NG, 1>), grid, block, 0, t_stream, A);
+    else if (A.experts <= 256) hipLaunchKernelGGL((k_mlp_up<DT, EVEN, GATE, NG, 4>), grid, block, 0, t_stream, A);
+    else hipLaunchKernelGGL((k_mlp_up<DT, EVEN, GATE, NG, 16>), grid, block, 0, t_stream, A);
+}
+
+template <int DT, bool EVEN>
+static void launch_up(const MlpArgs& A, const dim3 grid, int groups)
+{
+    if (A.gate) groups == 2 ? launch_up<DT, EVEN, true, 2>(A, grid) : launch_up<DT, EVEN, true, 1>(A, grid);
+    else groups == 2 ? launch_up<DT, EVEN, false, 2>(A, grid) : launch_up<DT, EVEN, false, 1>(A, grid);
+}
+
+template <int DT, bool EVEN>
+static void launch_down(const MlpArgs& A)
+{
+    // columns of a workgroup: so many that there are 256 of them, if there can be
+    const dim3 block(kDownWaves * kWave);
+    if (A.hidden >= 4096) hipLaunchKernelGGL((k_mlp_down<DT, EVEN, 16>), block_grid((A.hidden + 15) / 16), block, 0, t_stream, A);
+    else if (A.hidden >= 2048) hipLaunchKernelGGL((k_mlp_down<DT, EVEN, 8>), block_grid((A.hidden + 7) / 8), block, 0, t_stream, A);
+    else hipLaunchKernelGGL((k_mlp_down<DT, EVEN, 4>), block_grid((A.hidden + 3) / 4), block, 0, t_stream, A);
 }
 
 template <int DT>
-static void launch_mlp(const MlpArgs& A, int64_t used)
+static void launch_mlp(MlpArgs& A, int64_t used)
 {
     const bool up_even = A.hidden % kLane<DT> == 0 && ((uintptr_t)A.x | (uintptr_t)A.up | (uintptr_t)A.gate) % 16 == 0;
     const bool down_even = A.inter % kLane<DT> == 0 && (uintptr_t)A.down % 16 == 0;
+    // two groups of columns share the tokens' rows and the choice, where that leaves a CU four workgroups
+    const int groups = used * ((A.inter + 31) / 32) >= 4 * 256 ? 2 : 1;
+    A.columns = (A.inter + groups * kMlpColumns - 1) / (groups * kMlpColumns);
     const dim3 grid = block_grid(used * A.columns);
-    if (up_even && A.gate) launch_up<DT, true, true>(A, grid);
-    else if (up_even) launch_up<DT, true, false>(A, grid);
-    else if (A.gate) launch_up<DT, false, true>(A, grid);
-    else launch_up<DT, false, false>(A, grid);
-    const dim3 columns = block_grid((A.hidden + kMlpColumns - 1) / kMlpColumns), block(kDownWaves * kWave);
-    if (down_even) hipLaunchKernelGGL((k_mlp_down<DT, true>), columns, block, 0, t_stream, A);
-    else hipLaunchKernelGGL((k_mlp_down<DT, false>), columns, block, 0, t_stream, A);
+    if (up_even) launch_up<DT, true>(A, grid, groups);
+    else launch_up<DT, false>(A, grid, groups);
+    if (down_even) launch_down<DT, true>(A);
+    else launch_down<DT, false>(A);
 }
 
 }  // namespace abh
@@ -339,7 +399,6 @@ ADAMBRIDGE_API int adambridge_expert_mlp(const void* x, const void* logits, int3
     A.logits_bf16 = logits_dtype == ADAMBRIDGE_DT_BF16;
     A.normalize = normalize;
     A.silu = activation == ADAMBRIDGE_SILU;
-    A.columns = (int32_t)((inter + kMlpColumns - 1) / kMlpColumns);
     if (dtype == ADAMBRIDGE_DT_BF16) launch_mlp<DT_BF16>(A, used);
     else launch_mlp<DT_F32>(A, used);
     const hipError_t e = hipGetLastError();

@@ -88,7 +88,8 @@ def test_embed_entry_points():
         args[i] = None
         assert lib.adambridge_embed_backward(*args) == ENULL
     assert lib.adambridge_embed_backward(P, 8, 4, P, f32, 4, 4, 1.0, -1, P, ctypes.c_void_p(260)) == EALIGN
-    assert lib.adambridge_embed_work(64, 4, 4) == 64 * 8 and lib.adambridge_embed_work(65, 4, 4) == 65 * 8 + 2 * 2 * 4 * 4
+    # the sorted tokens twice, two parts for each of at most 1024 chunks, a place a word
+    assert 0 < lib.adambridge_embed_work(1 << 20, 1000, 64) <= (1 << 20) * 16 + 1024 * 2 * 64 * 4 + 1001 * 4
 
 
 # ---------------------------------------------------------------- token_losses
