@@ -28,8 +28,8 @@
 namespace abh {
 
 constexpr int kRun = 4096, kSortThreads = 1024;
-constexpr int kMostWords = 16;    // of a wavefront; fewer than its lanes
-constexpr int kLeastChunk = 64;   // tokens
+constexpr int kMostWords = 8;     // of a wavefront; fewer than its lanes.  (65536 tokens, 32000 x 4096: 8 words 108 us, 16 112, 4 105)
+constexpr int kLeastChunk = 32;   // tokens.  (the words' rows and the parts: 146 us with 32, 149 with 64)
 
 __device__ __forceinline__ int64_t id_at(const void* ids, int32_t id_bytes, int64_t i)
 {
@@ -366,10 +366,10 @@ static int embed_check(int32_t id_bytes, int64_t tokens, int32_t dtype, int64_t 
     return 0;
 }
 
-// Tokens of a chunk: so many that there are at most 1024 chunks, whose parts are at most 8 KB times the row's values.
+// Tokens of a chunk: so many that there are at most 2048 chunks, whose parts are at most 16 KB times the row's values.
 static int64_t chunk_of(int64_t tokens)
 {
-    return std::max<int64_t>(kLeastChunk, ((tokens + 1023) / 1024 + 63) / 64 * 64);
+    return std::max<int64_t>(kLeastChunk, ((tokens + 2047) / 2048 + 31) / 32 * 32);
 }
 
 static int64_t part_bytes(int64_t tokens, int64_t hidden)
@@ -405,7 +405,7 @@ static void launch_embed_back(EmbedBackArgs& A)
     if (tiny) hipLaunchKernelGGL((k_embed_parts<DT, true>), parts, dim3(256), 0, t_stream, A);
     else hipLaunchKernelGGL((k_embed_parts<DT, false>), parts, dim3(256), 0, t_stream, A);
     A.pieces = (vectors + 63) / 64;
-    // 16 words a wavefront, or fewer where that leaves wavefronts too few
+    // fewer words a wavefront where there would be too few wavefronts (5003 words of 897 FP32 values: 2 words 7 us, 16 19)
     A.words = kMostWords;
     while (A.words > 2 && (A.vocab + A.words - 1) / A.words * A.pieces < 4096) A.words /= 2;
     const dim3 grid = block_grid(((A.vocab + A.words - 1) / A.words * A.pieces + 3) / 4);

@@ -32,7 +32,7 @@ namespace abh {
 constexpr float kHeadLog2e = 1.4426950408889634f;
 constexpr float kHeadNegInf = -__builtin_inff();
 constexpr int kHeadCus = 256;
-constexpr int kFewRows = 64, kFewGroups = 2;   // k_head_few's rows at most, and words by 16 of a wavefront
+constexpr int kFewGroups = 2;        // words, by 16, of a wavefront of k_head_few
 constexpr int kFinishLanes = 1024;
 
 // A maximum and the sum of exp(x - m) over what was seen.  m = -inf: nothing above -inf yet.
@@ -68,6 +68,7 @@ struct HeadArgs {
     float* dh;                // parts x count x hidden
     void* dw;                 // vocab x hidden
     int32_t fresh;            // dh's first piece
+    int32_t places;           // tiles that the CUs hold at a time
 };
 
 // ------------------------------------------------------------------------ the scored rows
@@ -200,6 +201,22 @@ __device__ __forceinline__ bool head_multiply(uint8_t* lds, const Operand& a, co
 // Column of the tile that is a lane's value r of its columns j.
 __device__ __forceinline__ int column_of(int wj, int j, int r) { return wj + 32 * j + 8 * (r >> 2) + 4 * (int)((threadIdx.x & 63) >> 5) + (r & 3); }
 
+// A target's column in the tile, from its distance to the tile's first word; one outside the tile.
+__device__ __forceinline__ int hot_column(int64_t distance, int limit) { return distance >= 0 && distance < limit ? (int)distance : -1; }
+
+// What lies behind the vocabulary's last word.
+template <class H>
+__device__ __forceinline__ void mask_columns(mm_f32x16 (&acc)[H::NI][H::NJ], int wj, int limit, float to)
+{
+#pragma unroll
+    for (int i = 0; i < H::NI; ++i)
+#pragma unroll
+        for (int j = 0; j < H::NJ; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (column_of(wj, j, r) >= limit) acc[i][j][r] = to;
+}
+
 // ------------------------------------------------------------------------------ forward
 
 // Each row's maximum and sum over the tile's words, and the target's logit.
@@ -216,22 +233,30 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_sums(HeadArgs A)
     const Operand b{at<H::DT>(A.w, (A.v0 + j0) * A.hidden), A.hidden, 0, limit_j, A.hidden};
     mm_f32x16 acc[H::NI][H::NJ];
     const int wi = H::wi(), wj = H::wj(), lane = threadIdx.x & 63;
+    int hot[H::NI];   // the target's column in the tile, or one outside it
+#pragma unroll
+    for (int i = 0; i < H::NI; ++i) {
+        const int row = wi + 32 * i + (lane & 31);
+        hot[i] = row < limit_i ? hot_column(A.targets[A.index[i0 + row]] - j0, limit_j) : -1;
+    }
     const bool live = head_multiply<H, true, true>(lds, a, b, wi < limit_i, acc);
     if (live) {
+        if (limit_j < H::BN) mask_columns<H>(acc, wj, limit_j, kHeadNegInf);
 #pragma unroll
         for (int i = 0; i < H::NI; ++i) {
             const int row = wi + 32 * i + (lane & 31);
-            const int64_t target = row < limit_i ? A.targets[A.index[i0 + row]] - j0 : -1;
+            if (__builtin_amdgcn_ballot_w64(hot[i] >= wj && hot[i] < wj + H::BN / H::WJ)) {
+#pragma unroll
+                for (int j = 0; j < H::NJ; ++j)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (column_of(wj, j, r) == hot[i]) A.picked[i0 + row] = acc[i][j][r];
+            }
             float m = kHeadNegInf;
 #pragma unroll
             for (int j = 0; j < H::NJ; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int c = column_of(wj, j, r);
-                    if (c == target && c < limit_j) A.picked[i0 + row] = acc[i][j][r];
-                    if (c >= limit_j) acc[i][j][r] = kHeadNegInf;
-                    m = __builtin_fmaxf(m, acc[i][j][r]);
-                }
+                for (int r = 0; r < 16; ++r) m = __builtin_fmaxf(m, acc[i][j][r]);
             m = __builtin_fmaxf(m, __shfl_xor(m, 32));
             const float shift = shift_for(m);
             float s = 0.0f;
@@ -253,12 +278,12 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_sums(HeadArgs A)
 }
 
 // The same of few rows: the weights are read once, NG times 16 words a wavefront, which share the rows' loads.  part: workgroups x
-// rows.
-template <int DT, bool EVEN>
+// rows.  CH: 16 rows each.
+template <int DT, bool EVEN, int CH>
 __global__ __launch_bounds__(256) void k_head_few(HeadArgs A)
 {
-    constexpr int V = kLane<DT>, STEP = 4 * V, CH = kFewRows / 16, NG = kFewGroups, U = 4;
-    __shared__ Sums row_sums[4][kFewRows];
+    constexpr int V = kLane<DT>, STEP = 4 * V, NG = kFewGroups, U = 4;
+    __shared__ Sums row_sums[4][16 * CH];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int col = lane & 15, quarter = lane >> 4;
     const int64_t j0 = (block_index() * 4 + wave) * (16 * NG);
@@ -399,25 +424,33 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_grad(HeadArgs A)
     const Operand b{at<H::DT>(A.w, (A.v0 + j0) * A.hidden), A.hidden, 0, limit_j, A.hidden};
     mm_f32x16 acc[H::NI][H::NJ];
     const int wi = H::wi(), wj = H::wj(), lane = threadIdx.x & 63;
-    if (!head_multiply<H, true, true>(lds, a, b, wi < limit_i, acc)) return;
+    // a row's numbers, asked for before the product
+    int hot[H::NI];
+    float top[H::NI], scale[H::NI], seed[H::NI];
 #pragma unroll
     for (int i = 0; i < H::NI; ++i) {
         const int row = wi + 32 * i + (lane & 31);
-        const bool real = row < limit_i;
-        const int64_t at_row = real ? A.index[i0 + row] : 0;
-        const int64_t target = A.targets[at_row];
-        const float m = A.stats[2 * at_row], g = target < 0 || target >= A.vocab ? __builtin_nanf("") : A.gout[at_row];
-        const float f = A.stats[2 * at_row + 1] * g;
-        const int64_t hot = target - A.v0 - j0;
+        const int64_t at_row = row < limit_i ? A.index[i0 + row] : 0, target = A.targets[at_row];
+        hot[i] = hot_column(target - A.v0 - j0, limit_j);
+        seed[i] = target < 0 || target >= A.vocab ? __builtin_nanf("") : A.gout[at_row];
+        top[i] = A.stats[2 * at_row];
+        scale[i] = A.stats[2 * at_row + 1] * seed[i];
+    }
+    if (!head_multiply<H, true, true>(lds, a, b, wi < limit_i, acc)) return;
+#pragma unroll
+    for (int i = 0; i < H::NI; ++i) {
 #pragma unroll
         for (int j = 0; j < H::NJ; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int c = column_of(wj, j, r);
-                const float p = exp_of(acc[i][j][r], m) * f;
-                acc[i][j][r] = c >= limit_j ? 0.0f : c == hot ? p - g : p;
-            }
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = exp_of(acc[i][j][r], top[i]) * scale[i];
+        if (__builtin_amdgcn_ballot_w64(hot[i] >= wj && hot[i] < wj + H::BN / H::WJ)) {
+#pragma unroll
+            for (int j = 0; j < H::NJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] -= column_of(wj, j, r) == hot[i] ? seed[i] : 0.0f;
+        }
     }
+    if (limit_j < H::BN) mask_columns<H>(acc, wj, limit_j, 0.0f);
     const int wide = (limit_j + 7) & ~7;   // whole pieces: zeros behind the vocabulary's last word
     if constexpr (H::DT == DT_BF16) {
         store_bf16<typename H::C, true>(at<DT_BF16>(A.g, (int64_t)i0 * A.pitch + j0), A.pitch, limit_i, wide, acc, wi, wj);
@@ -438,10 +471,10 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_grad(HeadArgs A)
     }
 }
 
-// How many parts dh's sums are cut in: so that the tiles fill the CUs, of 16 steps or more.
-__device__ __host__ __forceinline__ int dh_splits(int64_t tiles, int width)
+// How many parts dh's sums are cut in: so that the tiles fill the CUs' places, of 16 steps or more.
+__device__ __host__ __forceinline__ int dh_splits(int64_t tiles, int places, int width)
 {
-    const int64_t fit = kHeadCus / (tiles < 1 ? 1 : tiles), most = width / 512;
+    const int64_t fit = places / (tiles < 1 ? 1 : tiles), most = width / 512;
     const int64_t n = fit < most ? fit : most;
     return (int)(n < 1 ? 1 : n);
 }
@@ -452,7 +485,7 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_dh(HeadArgs A)
 {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[H::LDS];
     const int count = scalar(*A.count), tiles_i = (count + H::BM - 1) / H::BM;
-    const int splits = dh_splits((int64_t)tiles_i * A.tiles_j, A.pitch);   // by the pitch: the same for every piece
+    const int splits = dh_splits((int64_t)tiles_i * A.tiles_j, A.places, A.pitch);   // by the pitch: the same for every piece
     HeadTile t;
     if (!head_tile(tiles_i, A.tiles_j, splits, t)) return;
     const int i0 = t.ti * H::BM, j0 = t.tj * H::BN, limit_i = count - i0, limit_j = A.hidden - j0;
@@ -524,14 +557,13 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_dw(HeadArgs A)
 // dh's rows at their places, the parts summed in order and rounded once; zeros for rows that are not scored.
 template <int DT>
 __global__ __launch_bounds__(256) void k_head_scatter(const float* sums, const int32_t* place, const int32_t* count, int32_t rows, int32_t hidden,
-                                                      int32_t tile, int32_t width, void* dh)
+                                                      int32_t tile_m, int32_t tile_n, int32_t places, int32_t width, void* dh)
 {
     constexpr int L = kLane<DT>;
     const int64_t t = block_index();
     if (t >= rows) return;
     const int n = *count, p = place[t];
-    const int64_t tiles = (int64_t)((n + tile - 1) / tile) * ((hidden + tile - 1) / tile);
-    const int splits = dh_splits(tiles, width);
+    const int splits = dh_splits((int64_t)((n + tile_m - 1) / tile_m) * ((hidden + tile_n - 1) / tile_n), places, width);
     void* out = at<DT>(dh, t * hidden);
     for (int32_t c = threadIdx.x * L; c < hidden; c += 256 * L) {
         float x[L];
@@ -576,13 +608,30 @@ struct Scratch {
     }
 };
 
-// Sides of the FP32 tiles: as the expert products' rule, 64 where tiles of 128 are few.
-static int f32_tile(int64_t tiles_of_128) { return tiles_of_128 < 512 ? 64 : 128; }
+// A kernel's tile.
+enum Kind { LARGE, HALF, F32_128, F32_64 };
+static int tile_m(Kind k) { return k == LARGE || k == HALF ? 256 : k == F32_64 ? 64 : 128; }
+static int tile_n(Kind k) { return k == LARGE ? 256 : k == F32_64 ? 64 : 128; }
+static int places_of(Kind k) { return (k == LARGE ? 1 : k == F32_64 ? 4 : 2) * kHeadCus; }
+static int64_t tiles_of(Kind k, int64_t m, int64_t n) { return (m + tile_m(k) - 1) / tile_m(k) * ((n + tile_n(k) - 1) / tile_n(k)); }
+static_assert(HalfTile::BM == 256 && HalfTile::BN == 128, "tile_m, tile_n");
+
+// The tile for m x n sums.  FP32: as the expert products' rule, 64 where tiles of 128 are few.  BF16: 256 x 256; dW's 256 x 128, two
+// workgroups a CU, where their columns end closer behind the last one (us, 256 / 128 columns: dW of 2703 rows and 50688 words of 896
+// values 286 / 240, of 16384 rows and 16128 words of 4096 1649 / 1732; the other kernels are 8-18% slower on half tiles).
+enum Product { SUMS, WEIGHTS, ROWS };   // the logits, dW, dh
+static Kind kind_of(int32_t dtype, int64_t m, int64_t n, Product product)
+{
+    if (dtype != ADAMBRIDGE_DT_BF16) return tiles_of(F32_128, m, n) < 512 ? F32_64 : F32_128;
+    if (product == WEIGHTS) return tiles_of(HALF, m, n) * 21 < tiles_of(LARGE, m, n) * 40 ? HALF : LARGE;   // 1.05 times the values
+    return product == SUMS && tiles_of(LARGE, m, n) <= kHeadCus / 2 ? HALF : LARGE;
+}
 
 // The forward call's plan and scratch.
 struct HeadForward {
     bool few;
-    int tile, parts;
+    Kind kind;
+    int parts;
     int32_t *index, *count;
     float* picked;
     Sums* part;
@@ -590,9 +639,11 @@ struct HeadForward {
     int64_t bytes;
     HeadForward(void* work, int32_t dtype, int64_t rows, int64_t vocab, int64_t hidden)
     {
-        few = rows <= kFewRows;
-        tile = dtype == ADAMBRIDGE_DT_BF16 ? LargeTile::BM : f32_tile((rows + 127) / 128 * ((vocab + 127) / 128));
-        parts = (int)(few ? (vocab + 64 * kFewGroups - 1) / (64 * kFewGroups) : (vocab + tile - 1) / tile);
+        // rows that stream the weights, or go on tiles (us, 151936 x 896 and 32000 x 4096: BF16, 32 rows 72 and 75 streamed; 65 on
+        // tiles 72 and 76; FP32, 64 streamed 256 and 294, 65 on tiles 329 and 355)
+        few = rows <= (dtype == ADAMBRIDGE_DT_BF16 ? 16 : 64);
+        kind = kind_of(dtype, rows, vocab, SUMS);
+        parts = (int)(few ? (vocab + 64 * kFewGroups - 1) / (64 * kFewGroups) : (vocab + tile_n(kind) - 1) / tile_n(kind));
         Scratch s{static_cast<uint8_t*>(work)};
         picked = s.take<float>(rows);
         part = s.take<Sums>(parts * rows);
@@ -605,7 +656,7 @@ struct HeadForward {
 
 // The backward call's.
 struct HeadBackward {
-    int tile, dh_tile;
+    Kind grad, dw, dh_kind;
     int32_t pitch;   // words of a piece
     int32_t *index, *place, *count;
     void *h, *g;
@@ -613,11 +664,13 @@ struct HeadBackward {
     int64_t bytes;
     HeadBackward(void* work, int32_t dtype, int64_t rows, int64_t vocab, int64_t hidden)
     {
-        const bool bf = dtype == ADAMBRIDGE_DT_BF16;
-        const int64_t size = bf ? 2 : 4, most = std::max(kPieceValues / rows, kLeastPiece), pieces = (vocab + most - 1) / most;
+        const int64_t size = dtype == ADAMBRIDGE_DT_BF16 ? 2 : 4;
+        const int64_t most = std::max(kPieceValues / rows, kLeastPiece), pieces = (vocab + most - 1) / most;
         pitch = (int32_t)up((vocab + pieces - 1) / pieces, 256);
-        tile = bf ? LargeTile::BM : f32_tile((rows + 127) / 128 * ((std::min<int64_t>(pitch, vocab) + 127) / 128));
-        dh_tile = bf ? LargeTile::BM : f32_tile((rows + 127) / 128 * ((hidden + 127) / 128));
+        const int64_t width = std::min<int64_t>(pitch, vocab);
+        grad = kind_of(dtype, rows, width, SUMS);
+        dw = kind_of(dtype, width, hidden, WEIGHTS);
+        dh_kind = kind_of(dtype, rows, hidden, ROWS);
         Scratch s{static_cast<uint8_t*>(work)};
         index = s.take<int32_t>(rows);
         place = s.take<int32_t>(rows);
@@ -625,19 +678,24 @@ struct HeadBackward {
         h = s.take<uint8_t>(rows * hidden * size);
         g = s.take<uint8_t>(rows * pitch * size);
         // parts x rows x hidden: as many as fill the CUs with tiles, or one
-        dh = s.take<float>(std::max(rows * hidden, (int64_t)kHeadCus * dh_tile * dh_tile));
+        dh = s.take<float>(std::max(rows * hidden, (int64_t)places_of(dh_kind) * tile_m(dh_kind) * tile_n(dh_kind)));
         bytes = s.used;
     }
 };
 
 static dim3 tile_grid(int64_t tiles) { return block_grid(up(tiles, kXcd)); }
 
-#define ABH_HEAD_LAUNCH(KERNEL, TILE, EVEN, GRID)                                                                             \
-    do {                                                                                                                      \
-        if (bf && (EVEN)) hipLaunchKernelGGL((KERNEL<HeadBf16<LargeTile, true>>), GRID, dim3(LargeTile::T), 0, t_stream, A);  \
-        else if (bf) hipLaunchKernelGGL((KERNEL<HeadBf16<LargeTile, false>>), GRID, dim3(LargeTile::T), 0, t_stream, A);      \
-        else if ((TILE) == 128) hipLaunchKernelGGL((KERNEL<HeadF32<128>>), GRID, dim3(256), 0, t_stream, A);                  \
-        else hipLaunchKernelGGL((KERNEL<HeadF32<64>>), GRID, dim3(256), 0, t_stream, A);                                      \
+#define ABH_HEAD_BF16(KERNEL, TILE, EVEN, GRID)                                                                    \
+    do {                                                                                                           \
+        if (EVEN) hipLaunchKernelGGL((KERNEL<HeadBf16<TILE, true>>), GRID, dim3(TILE::T), 0, t_stream, A);         \
+        else hipLaunchKernelGGL((KERNEL<HeadBf16<TILE, false>>), GRID, dim3(TILE::T), 0, t_stream, A);             \
+    } while (0)
+#define ABH_HEAD_LAUNCH(KERNEL, KIND, EVEN, GRID)                                                                  \
+    do {                                                                                                           \
+        if ((KIND) == LARGE) ABH_HEAD_BF16(KERNEL, LargeTile, EVEN, GRID);                                         \
+        else if ((KIND) == HALF) ABH_HEAD_BF16(KERNEL, HalfTile, EVEN, GRID);                                      \
+        else if ((KIND) == F32_128) hipLaunchKernelGGL((KERNEL<HeadF32<128>>), GRID, dim3(256), 0, t_stream, A);   \
+        else hipLaunchKernelGGL((KERNEL<HeadF32<64>>), GRID, dim3(256), 0, t_stream, A);                           \
     } while (0)
 
 static void launch_gather(bool bf, int64_t rows, const void* hidden_rows, const int32_t* index, const int32_t* count, int64_t hidden, void* out)
@@ -680,10 +738,12 @@ ADAMBRIDGE_API int adambridge_token_losses(const void* hidden, const void* weigh
         const int64_t bytes = size * (bf ? 2 : 4);
         const bool even = bytes % 16 == 0 && ((uintptr_t)hidden | (uintptr_t)weight) % 16 == 0;
         const dim3 grid = block_grid(p.parts), block(256);
-        if (bf && even) hipLaunchKernelGGL((k_head_few<DT_BF16, true>), grid, block, 0, t_stream, A);
-        else if (bf) hipLaunchKernelGGL((k_head_few<DT_BF16, false>), grid, block, 0, t_stream, A);
-        else if (even) hipLaunchKernelGGL((k_head_few<DT_F32, true>), grid, block, 0, t_stream, A);
-        else hipLaunchKernelGGL((k_head_few<DT_F32, false>), grid, block, 0, t_stream, A);
+        if (bf && even) hipLaunchKernelGGL((k_head_few<DT_BF16, true, 1>), grid, block, 0, t_stream, A);
+        else if (bf) hipLaunchKernelGGL((k_head_few<DT_BF16, false, 1>), grid, block, 0, t_stream, A);
+        else if (even && rows <= 16) hipLaunchKernelGGL((k_head_few<DT_F32, true, 1>), grid, block, 0, t_stream, A);
+        else if (even) hipLaunchKernelGGL((k_head_few<DT_F32, true, 4>), grid, block, 0, t_stream, A);
+        else if (rows <= 16) hipLaunchKernelGGL((k_head_few<DT_F32, false, 1>), grid, block, 0, t_stream, A);
+        else hipLaunchKernelGGL((k_head_few<DT_F32, false, 4>), grid, block, 0, t_stream, A);
         hipLaunchKernelGGL((k_head_finish<4>), dim3((unsigned)((rows + 3) / 4)), dim3(kFinishLanes), 0, t_stream, p.part, p.parts, A.rows, nullptr,
                            nullptr, targets, vocab, ignore_index, p.picked, losses, stats);
     } else {
@@ -695,8 +755,7 @@ ADAMBRIDGE_API int adambridge_token_losses(const void* hidden, const void* weigh
         A.width = (int32_t)vocab;
         A.tiles_j = p.parts;
         const bool even = size % 8 == 0 && (uintptr_t)weight % 16 == 0;
-        const dim3 grid = tile_grid((rows + p.tile - 1) / p.tile * p.parts);
-        ABH_HEAD_LAUNCH(k_head_sums, p.tile, even, grid);
+        ABH_HEAD_LAUNCH(k_head_sums, p.kind, even, tile_grid(tiles_of(p.kind, rows, vocab)));
         hipLaunchKernelGGL((k_head_finish<16>), block_grid((rows + 15) / 16), dim3(kFinishLanes), 0, t_stream, p.part, p.parts, A.rows, p.index,
                            p.count, targets, vocab, ignore_index, p.picked, losses, stats);
     }
@@ -743,26 +802,26 @@ ADAMBRIDGE_API int adambridge_token_losses_backward(const float* gout, const voi
     for (int64_t v0 = 0; v0 < vocab; v0 += p.pitch) {
         A.v0 = v0;
         A.width = (int32_t)std::min<int64_t>(p.pitch, vocab - v0);
-        A.tiles_j = (A.width + p.tile - 1) / p.tile;
-        ABH_HEAD_LAUNCH(k_head_grad, p.tile, even, tile_grid((rows + p.tile - 1) / p.tile * A.tiles_j));
+        A.tiles_j = (A.width + tile_n(p.grad) - 1) / tile_n(p.grad);
+        ABH_HEAD_LAUNCH(k_head_grad, p.grad, even, tile_grid(tiles_of(p.grad, rows, A.width)));
         if (dweight) {
-            A.tiles_j = (int32_t)((size + p.tile - 1) / p.tile);
-            ABH_HEAD_LAUNCH(k_head_dw, p.tile, even, tile_grid((int64_t)(A.width + p.tile - 1) / p.tile * A.tiles_j));
+            A.tiles_j = (int32_t)((size + tile_n(p.dw) - 1) / tile_n(p.dw));
+            ABH_HEAD_LAUNCH(k_head_dw, p.dw, even, tile_grid(tiles_of(p.dw, A.width, size)));
         }
         if (dhidden) {
-            A.tiles_j = (int32_t)((size + p.dh_tile - 1) / p.dh_tile);
-            const int64_t tiles = (rows + p.dh_tile - 1) / p.dh_tile * A.tiles_j;
-            ABH_HEAD_LAUNCH(k_head_dh, p.dh_tile, even, tile_grid(std::max<int64_t>(tiles, kHeadCus)));
+            A.tiles_j = (int32_t)((size + tile_n(p.dh_kind) - 1) / tile_n(p.dh_kind));
+            A.places = places_of(p.dh_kind);
+            ABH_HEAD_LAUNCH(k_head_dh, p.dh_kind, even, tile_grid(std::max<int64_t>(tiles_of(p.dh_kind, rows, size), A.places)));
         }
         A.fresh = 0;
     }
     if (dhidden) {
         if (bf)
-            hipLaunchKernelGGL((k_head_scatter<DT_BF16>), block_grid(rows), dim3(256), 0, t_stream, p.dh, p.place, p.count, A.rows, A.hidden, p.dh_tile,
-                               p.pitch, dhidden);
+            hipLaunchKernelGGL((k_head_scatter<DT_BF16>), block_grid(rows), dim3(256), 0, t_stream, p.dh, p.place, p.count, A.rows, A.hidden,
+                               tile_m(p.dh_kind), tile_n(p.dh_kind), A.places, p.pitch, dhidden);
         else
-            hipLaunchKernelGGL((k_head_scatter<DT_F32>), block_grid(rows), dim3(256), 0, t_stream, p.dh, p.place, p.count, A.rows, A.hidden, p.dh_tile,
-                               p.pitch, dhidden);
+            hipLaunchKernelGGL((k_head_scatter<DT_F32>), block_grid(rows), dim3(256), 0, t_stream, p.dh, p.place, p.count, A.rows, A.hidden,
+                               tile_m(p.dh_kind), tile_n(p.dh_kind), A.places, p.pitch, dhidden);
     }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : hip_fail(e, "hipLaunchKernelGGL (token losses backward)");

@@ -46,6 +46,7 @@ struct MlpArgs {
     int32_t* count;    // how many
     void* a;           // chosen experts x 16 x inter
     int32_t tokens, experts, top_k, inter, hidden;
+    int32_t used;      // the most experts that can be chosen
     int32_t logits_bf16, normalize, silu;
     int32_t columns;   // workgroups of a chosen expert
 };
@@ -68,11 +69,19 @@ __device__ __forceinline__ void choose(const MlpArgs& A, uint32_t* mask, int32_t
     const int lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
     for (int e = threadIdx.x; e < A.experts; e += kUpWaves * kWave) mask[e] = 0;
     __syncthreads();
-    for (int t = wave; t < A.tokens; t += kUpWaves) {
-        float x[NV];
-        uint32_t key[NV];
+    constexpr int TOKENS = kMlpTokens / kUpWaves;   // of a wavefront; their logits are asked for at once
+    float logits[TOKENS][NV];
 #pragma unroll
-        for (int v = 0; v < NV; ++v) x[v] = 64 * v + lane < A.experts ? logit(A, (int64_t)t * A.experts + 64 * v + lane) : 0.0f;
+    for (int i = 0; i < TOKENS; ++i)
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+            logits[i][v] = wave + i * kUpWaves < A.tokens && 64 * v + lane < A.experts ? logit(A, (int64_t)(wave + i * kUpWaves) * A.experts + 64 * v + lane) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < TOKENS; ++i) {
+        const int t = wave + i * kUpWaves;
+        if (t >= A.tokens) break;
+        float(&x)[NV] = logits[i];
+        uint32_t key[NV];
 #pragma unroll
         for (int v = 0; v < NV; ++v) key[v] = 64 * v + lane < A.experts ? order_key(x[v]) : 0u;
         float top = 0.0f, sum = 0.0f, mine = 0.0f;
@@ -115,111 +124,117 @@ __device__ __forceinline__ void choose(const MlpArgs& A, uint32_t* mask, int32_t
     __syncthreads();
 }
 
-// 16 NG columns of up (and gate) of the blockIdx-th chosen expert: the wavefronts split the sum, the first adds their parts in order.
+// 16 NG columns of up (and gate) of a chosen expert at a time: the wavefronts split the sum, the first adds their parts in order, while
+// the next columns' first weights are on their way.
 template <int DT, bool EVEN, bool GATE, int NG, int NV>
-__global__ __launch_bounds__(kUpWaves * kWave) void k_mlp_up(MlpArgs A)
+__global__ __launch_bounds__(kUpWaves * kWave, EVEN ? 4 : 2) void k_mlp_up(MlpArgs A)
 {
-    constexpr int V = kLane<DT>, STEP = 4 * V, W = kUpWaves, M = (GATE ? 2 : 1) * NG, U = 8 / M, COLS = kMlpColumns * NG;   // M: up's columns, then gate's
+    constexpr int V = kLane<DT>, STEP = 4 * V, W = kUpWaves, M = (GATE ? 2 : 1) * NG, U = M == 4 ? 2 : 4, COLS = kMlpColumns * NG;   // M: up's columns, then gate's
     __shared__ uint32_t mask[kMlpExperts];
     __shared__ int32_t expert[kMlpTokens * kMlpChosen];
     __shared__ float weight[kMlpTokens * kMlpChosen];
-    __shared__ mm_f32x4 parts[W - 1][M][64];
+    __shared__ uint16_t list[kMlpExperts];
+    __shared__ mm_f32x4 parts[2][W - 1][M][64];
     choose<NV>(A, mask, expert, weight);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int col = lane & 15, quarter = lane >> 4;
-    const int block = (int)block_index(), rank = block / A.columns, j0 = (block - rank * A.columns) * COLS;
-    int e = -1, skip = rank, before = 0;
+    int count = 0;   // the chosen experts, in order of their number
     for (int e0 = 0; e0 < A.experts; e0 += kWave) {
-        const uint64_t with = __builtin_amdgcn_ballot_w64(e0 + lane < A.experts && mask[e0 + lane < A.experts ? e0 + lane : 0] != 0);
-        const int n = __builtin_popcountll(with);
-        if (e < 0 && skip < n) {
-            uint64_t left = with;
-            for (int i = 0; i < skip; ++i) left &= left - 1;
-            e = e0 + __builtin_ctzll(left);
-        }
-        skip -= n;
-        before += n;
+        const bool chosen = e0 + lane < A.experts && mask[e0 + lane < A.experts ? e0 + lane : 0] != 0;
+        const uint64_t with = __builtin_amdgcn_ballot_w64(chosen);
+        if (chosen && wave == 0) list[count + __builtin_popcountll(with & (((uint64_t)1 << lane) - 1))] = (uint16_t)(e0 + lane);
+        count += __builtin_popcountll(with);
     }
-    if (block == 0 && threadIdx.x == 0) *A.count = before;
-    if (e < 0) return;
-    const uint32_t tokens = mask[e];
-    if (j0 == 0 && threadIdx.x < kMlpTokens) {   // for the other kernel
-        Chosen* const c = A.list + rank;
-        float w = 0.0f;
-        if ((int)threadIdx.x < A.tokens)
-            for (int j = 0; j < A.top_k; ++j) w = expert[threadIdx.x * A.top_k + j] == e ? weight[threadIdx.x * A.top_k + j] : w;
-        c->weight[threadIdx.x] = w;
-        if (threadIdx.x == 0) {
-            c->expert = e;
-            c->tokens = tokens;
-        }
-    }
+    __syncthreads();
+    if (blockIdx.x == 0 && threadIdx.x == 0) *A.count = count;
     const int steps = (A.hidden + STEP - 1) / STEP, s0 = steps * wave / W, s1 = steps * (wave + 1) / W;
-    Pieces<DT, EVEN> w[M];
-#pragma unroll
-    for (int m = 0; m < M; ++m) {
-        const int j = j0 + m % NG * kMlpColumns, columns = A.inter - j < kMlpColumns ? A.inter - j < 0 ? 0 : A.inter - j : kMlpColumns;
-        w[m] = {at<DT>(m < NG ? A.up : A.gate, ((int64_t)e * A.inter + (columns ? j : 0)) * A.hidden), (uint32_t)(columns * A.hidden * kSize<DT>), A.hidden, columns};
-    }
+    const int turns = ((steps + W - 1) / W + U - 1) / U;   // of every wavefront; by twos, the odd one out without anything to load
     const Pieces<DT, EVEN> x{static_cast<const uint8_t*>(A.x), (uint32_t)(A.tokens * A.hidden * kSize<DT>), A.hidden, A.tokens};
-    mm_f32x4 acc[M];
-#pragma unroll
-    for (int m = 0; m < M; ++m) acc[m] = mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     raw16 even[M][U], odd[M][U];
-    auto load = [&](int s, raw16 (&to)[M][U]) {
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int m = 0; m < M; ++m) to[m][u] = w[m].load(col, (s + u) * STEP + quarter * V, s + u < s1);
-    };
-    auto turn = [&](int s, const raw16 (&now)[M][U], raw16 (&next)[M][U]) {   // as k_mlp_down's
-        raw16 xv[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) xv[u] = x.load(col, (s + u) * STEP + quarter * V, s + u < s1);
-        __builtin_amdgcn_sched_barrier(0);
-        if (s + U < s1) load(s + U, next);
-        __builtin_amdgcn_sched_barrier(0);
+    auto load = [&](int item, int s, raw16 (&to)[M][U]) {
+        const int rank = item / A.columns, j0 = (item - rank * A.columns) * COLS;
+        const int e = scalar(list[rank]);
 #pragma unroll
         for (int m = 0; m < M; ++m) {
-            mm_f32x4 some = DT == DT_BF16 ? acc[m] : mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};   // FP32: short chains of sums
+            const int j = j0 + m % NG * kMlpColumns, columns = A.inter - j < kMlpColumns ? A.inter - j < 0 ? 0 : A.inter - j : kMlpColumns;
+            const Pieces<DT, EVEN> w{at<DT>(m < NG ? A.up : A.gate, ((int64_t)e * A.inter + (columns ? j : 0)) * A.hidden),
+                                     (uint32_t)(columns * A.hidden * kSize<DT>), A.hidden, columns};
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                if constexpr (DT == DT_BF16) {
-                    some = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mm_bf16x8, now[m][u]), __builtin_bit_cast(mm_bf16x8, xv[u]), some,
-                                                                   0, 0, 0);
-                } else {
-                    const mm_f32x4 wf = __builtin_bit_cast(mm_f32x4, now[m][u]), xf = __builtin_bit_cast(mm_f32x4, xv[u]);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) some = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[q], xf[q], some, 0, 0, 0);
-                }
-            }
-            if constexpr (DT == DT_BF16) acc[m] = some;
-            else acc[m] += some;
+            for (int u = 0; u < U; ++u) to[m][u] = w.load(col, (s + u) * STEP + quarter * V, s + u < s1);
         }
     };
-    if (s0 < s1) load(s0, even);
-    for (int s = s0; s < s1; s += 2 * U) {
-        turn(s, even, odd);
-        if (s + U < s1) turn(s + U, odd, even);
-    }
-    if (wave > 0)
+    const int items = count * A.columns;
+    int item = (int)blockIdx.x, buffer = 0;
+    if (item < items) load(item, s0, even);
+    for (; item < items; item += (int)gridDim.x, buffer ^= 1) {
+        mm_f32x4 acc[M];
 #pragma unroll
-        for (int m = 0; m < M; ++m) parts[wave - 1][m][lane] = acc[m];
-    __syncthreads();
-    if (wave > 0 || !(tokens >> col & 1)) return;
+        for (int m = 0; m < M; ++m) acc[m] = mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        auto turn = [&](int t, const raw16 (&now)[M][U], raw16 (&next)[M][U]) {   // as k_mlp_down's
+            const int s = s0 + t * U;
+            raw16 xv[U];
 #pragma unroll
-    for (int p = 0; p < W - 1; ++p)
+            for (int u = 0; u < U; ++u) xv[u] = x.load(col, (s + u) * STEP + quarter * V, s + u < s1);
+            __builtin_amdgcn_sched_barrier(0);
+            const bool last = t + 1 >= turns && (t & 1);   // the next columns' first
+            const int ahead = last ? item + (int)gridDim.x : item;
+            if (ahead < items) load(ahead, last ? s0 : s + U, next);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int m = 0; m < M; ++m) acc[m] += parts[p][m][lane];
-    void* row = at<DT>(A.a, ((int64_t)rank * kMlpTokens + col) * A.inter);
+            for (int m = 0; m < M; ++m) {
+                mm_f32x4 some = DT == DT_BF16 ? acc[m] : mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};   // FP32: short chains of sums
 #pragma unroll
-    for (int n = 0; n < NG; ++n)
+                for (int u = 0; u < U; ++u) {
+                    if constexpr (DT == DT_BF16) {
+                        some = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mm_bf16x8, now[m][u]), __builtin_bit_cast(mm_bf16x8, xv[u]),
+                                                                       some, 0, 0, 0);
+                    } else {
+                        const mm_f32x4 wf = __builtin_bit_cast(mm_f32x4, now[m][u]), xf = __builtin_bit_cast(mm_f32x4, xv[u]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int j = j0 + n * kMlpColumns + 4 * quarter + r;
-            const float y = GATE ? activated(acc[M - NG + n][r], A.silu) * acc[n][r] : activated(acc[n][r], A.silu);
-            if (j < A.inter) put<DT>(row, j, y);
+                        for (int q = 0; q < 4; ++q) some = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[q], xf[q], some, 0, 0, 0);
+                    }
+                }
+                if constexpr (DT == DT_BF16) acc[m] = some;
+                else acc[m] += some;
+            }
+        };
+        for (int t = 0; t < turns; t += 2) {
+            turn(t, even, odd);
+            turn(t + 1, odd, even);
         }
+        if (wave > 0)
+#pragma unroll
+            for (int m = 0; m < M; ++m) parts[buffer][wave - 1][m][lane] = acc[m];
+        __syncthreads();   // and the first wavefront has read the other buffer
+        if (wave > 0) continue;
+        const int rank = item / A.columns, j0 = (item - rank * A.columns) * COLS, e = list[rank];
+        const uint32_t tokens = mask[e];
+        if (j0 == 0 && lane < kMlpTokens) {   // for the other kernel
+            Chosen* const c = A.list + rank;
+            float w = 0.0f;
+            if (lane < A.tokens)
+                for (int j = 0; j < A.top_k; ++j) w = expert[lane * A.top_k + j] == e ? weight[lane * A.top_k + j] : w;
+            c->weight[lane] = w;
+            if (lane == 0) {
+                c->expert = e;
+                c->tokens = tokens;
+            }
+        }
+        if (!(tokens >> col & 1)) continue;
+#pragma unroll
+        for (int p = 0; p < W - 1; ++p)
+#pragma unroll
+            for (int m = 0; m < M; ++m) acc[m] += parts[buffer][p][m][lane];
+        void* row = at<DT>(A.a, ((int64_t)rank * kMlpTokens + col) * A.inter);
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int j = j0 + n * kMlpColumns + 4 * quarter + r;
+                const float y = GATE ? activated(acc[M - NG + n][r], A.silu) * acc[n][r] : activated(acc[n][r], A.silu);
+                if (j < A.inter) put<DT>(row, j, y);
+            }
+    }
 }
 
 // COLS columns of the result: the wavefronts share the chosen experts' pieces of U loads, whose products are weighted and added in
@@ -229,24 +244,25 @@ __global__ __launch_bounds__(kUpWaves * kWave) void k_mlp_up(MlpArgs A)
 template <int DT, bool EVEN, int COLS>
 __global__ __launch_bounds__(kDownWaves * kWave) void k_mlp_down(MlpArgs A)
 {
-    constexpr int V = kLane<DT>, STEP = 4 * V, W = kDownWaves, G = 16 / COLS, U = 4, PIECE = U * G * STEP;
+    constexpr int V = kLane<DT>, STEP = 4 * V, W = kDownWaves, G = 16 / COLS, U = COLS == 4 ? 2 : 4, PIECE = U * G * STEP;
     __shared__ mm_f32x4 parts[W][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int col = lane & 15, quarter = lane >> 4;
     const int j0 = (int)block_index() * COLS, columns = A.hidden - j0 < COLS ? A.hidden - j0 : COLS;
-    const int pieces = (A.inter + PIECE - 1) / PIECE, items = scalar(*A.count) * pieces;
+    const int pieces = (A.inter + PIECE - 1) / PIECE, rank0 = wave / pieces;
+    const int first = scalar(A.list[rank0 < A.used ? rank0 : 0].expert);   // asked for beside the count; not looked at behind it
+    const int items = scalar(*A.count) * pieces;
     mm_f32x4 sum{0.0f, 0.0f, 0.0f, 0.0f};
-    raw16 even[U], odd[U];
-    auto load = [&](int i, raw16 (&to)[U]) {
+    raw16 pieces_of[3][U];   // two ahead of the one that is multiplied
+    auto load = [&](int i, int e, raw16 (&to)[U]) {
         const int rank = i / pieces, k0 = (i - rank * pieces) * PIECE + (col / COLS * 4 + quarter) * V;
-        const int e = scalar(A.list[rank].expert);
         const Pieces<DT, EVEN> w{at<DT>(A.down, ((int64_t)e * A.hidden + j0) * A.inter), (uint32_t)(columns * A.inter * kSize<DT>), A.inter, columns};
 #pragma unroll
         for (int u = 0; u < U; ++u) to[u] = w.load(col % COLS, k0 + u * G * STEP, true);
     };
-    // loads arrive in their order: this piece's activations are asked for before the next piece's weights, which are then on their
+    // loads arrive in their order: this piece's activations are asked for before a later piece's weights, which are then on their
     // way while this one is multiplied
-    auto turn = [&](int i, const raw16 (&now)[U], raw16 (&next)[U]) {
+    auto turn = [&](int i, const raw16 (&now)[U], raw16 (&ahead)[U]) {
         const int rank = i / pieces, k0 = (i - rank * pieces) * PIECE + quarter * V;
         const Chosen* const c = A.list + rank;
         const bool mine = c->tokens >> col & 1;
@@ -258,7 +274,7 @@ __global__ __launch_bounds__(kDownWaves * kWave) void k_mlp_down(MlpArgs A)
 #pragma unroll
             for (int u = 0; u < U; ++u) av[g][u] = a.load(col, k0 + (u * G + g) * STEP, mine);   // another token's row: never written
         __builtin_amdgcn_sched_barrier(0);
-        if (i + W < items) load(i + W, next);
+        if (i + 2 * W < items) load(i + 2 * W, scalar(A.list[(i + 2 * W) / pieces].expert), ahead);
         __builtin_amdgcn_sched_barrier(0);
         mm_f32x4 product{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -281,10 +297,12 @@ __global__ __launch_bounds__(kDownWaves * kWave) void k_mlp_down(MlpArgs A)
 #pragma unroll
         for (int r = 0; r < 4; ++r) sum[r] = mine ? sum[r] + by * product[r] : sum[r];   // what an expert holds stays with its tokens
     };
-    if (wave < items) load(wave, even);
-    for (int i = wave; i < items; i += 2 * W) {
-        turn(i, even, odd);
-        if (i + W < items) turn(i + W, odd, even);
+    if (wave < items) load(wave, first, pieces_of[0]);
+    if (wave + W < items) load(wave + W, scalar(A.list[(wave + W) / pieces].expert), pieces_of[1]);
+    for (int i = wave; i < items; i += 3 * W) {
+        turn(i, pieces_of[0], pieces_of[2]);
+        if (i + W < items) turn(i + W, pieces_of[1], pieces_of[0]);
+        if (i + 2 * W < items) turn(i + 2 * W, pieces_of[2], pieces_of[1]);
     }
     parts[wave][lane] = sum;
     __syncthreads();
@@ -342,14 +360,14 @@ static void launch_down(const MlpArgs& A)
 }
 
 template <int DT>
-static void launch_mlp(MlpArgs& A, int64_t used)
+static void launch_mlp(MlpArgs& A)
 {
     const bool up_even = A.hidden % kLane<DT> == 0 && ((uintptr_t)A.x | (uintptr_t)A.up | (uintptr_t)A.gate) % 16 == 0;
     const bool down_even = A.inter % kLane<DT> == 0 && (uintptr_t)A.down % 16 == 0;
     // two groups of columns share the tokens' rows and the choice, where that leaves a CU four workgroups
-    const int groups = used * ((A.inter + 31) / 32) >= 4 * 256 ? 2 : 1;
+    const int groups = (int64_t)A.used * ((A.inter + 31) / 32) >= 4 * 256 ? 2 : 1;
     A.columns = (A.inter + groups * kMlpColumns - 1) / (groups * kMlpColumns);
-    const dim3 grid = block_grid(used * A.columns);
+    const dim3 grid((unsigned)std::min<int64_t>((int64_t)A.used * A.columns, 4 * 256));   // as many as the CUs hold
     if (up_even) launch_up<DT, true>(A, grid, groups);
     else launch_up<DT, false>(A, grid, groups);
     if (down_even) launch_down<DT, true>(A);
@@ -392,6 +410,7 @@ ADAMBRIDGE_API int adambridge_expert_mlp(const void* x, const void* logits, int3
     A.list = reinterpret_cast<Chosen*>(static_cast<uint8_t*>(work) + 256);
     A.a = static_cast<uint8_t*>(work) + 256 + list_bytes(used);
     A.tokens = (int32_t)tokens;
+    A.used = (int32_t)used;
     A.experts = (int32_t)experts;
     A.top_k = (int32_t)top_k;
     A.inter = (int32_t)inter;
@@ -399,8 +418,8 @@ ADAMBRIDGE_API int adambridge_expert_mlp(const void* x, const void* logits, int3
     A.logits_bf16 = logits_dtype == ADAMBRIDGE_DT_BF16;
     A.normalize = normalize;
     A.silu = activation == ADAMBRIDGE_SILU;
-    if (dtype == ADAMBRIDGE_DT_BF16) launch_mlp<DT_BF16>(A, used);
-    else launch_mlp<DT_F32>(A, used);
+    if (dtype == ADAMBRIDGE_DT_BF16) launch_mlp<DT_BF16>(A);
+    else launch_mlp<DT_F32>(A);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : hip_fail(e, "hipLaunchKernelGGL (expert MLP)");
 }

@@ -270,6 +270,7 @@ struct Fragments {
 
 typedef Config<256, 256, 32, 4, 2, 4, 2> LargeTile;
 typedef Config<128, 128, 32, 4, 2, 2, 2> SmallTile;   // where large ones are too few for the CUs
+typedef Config<256, 128, 32, 3, 2, 2, 2> HalfTile;    // two workgroups a CU: one's products beside the other's results
 
 // Asks the scheduler for READS reads of the LDS spread among the next PRODUCTS matrix products.
 template <int READS, int PRODUCTS, int M = 0>

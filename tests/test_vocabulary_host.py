@@ -88,8 +88,8 @@ def test_embed_entry_points():
         args[i] = None
         assert lib.adambridge_embed_backward(*args) == ENULL
     assert lib.adambridge_embed_backward(P, 8, 4, P, f32, 4, 4, 1.0, -1, P, ctypes.c_void_p(260)) == EALIGN
-    # the sorted tokens twice, two parts for each of at most 1024 chunks, a place a word
-    assert 0 < lib.adambridge_embed_work(1 << 20, 1000, 64) <= (1 << 20) * 16 + 1024 * 2 * 64 * 4 + 1001 * 4
+    # the sorted tokens twice, two parts for each of at most 2048 chunks, a place a word
+    assert 0 < lib.adambridge_embed_work(1 << 20, 1000, 64) <= (1 << 20) * 16 + 2048 * 2 * 64 * 4 + 1001 * 4
 
 
 # ---------------------------------------------------------------- token_losses
