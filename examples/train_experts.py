@@ -3,15 +3,16 @@
     python -m examples.train_experts [--steps 60] [--device cuda|cpu] [--precision fp32|bf16|fp8]
 
 A block is ``x + combine(down(gelu(up(dispatch(layer_norm(x))))))``: the package's layer norm, a router that
-chooses ``top_k`` of the experts for each token, the rows' way to them, their products, and the way back.  The
-loss is ``causal_lm_loss``, the optimizer ``AdamBridge`` (on the GPU; on the CPU, where its kernels do not
-run, torch's AdamW).  Nothing in a step waits for the device: the losses are read when the steps are done.
+chooses ``top_k`` of the experts for each token, the rows' way to them, their products, and the way back, all but the
+norm in ``expert_mlp``.  Tokens come in by ``embed``; the loss is ``causal_lm_loss``, the optimizer ``AdamBridge`` (on the GPU;
+on the CPU, where its kernels do not run, torch's AdamW).  Nothing in a step waits for the device: the losses are read
+when the steps are done.  A decoded token takes one row through the model, with the sums over the tokens before kept
+from step to step; ``token_losses`` says afterwards how likely the model held each token.
 """
 
 import argparse
 
 import torch
-import torch.nn.functional as F
 
 import adambridge_amd as ab
 
@@ -30,9 +31,7 @@ class ExpertBlock(torch.nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         flat = x.reshape(-1, x.shape[-1])
         h = ab.layer_norm(flat, self.norm.weight, self.norm.bias, self.norm.eps)
-        r = ab.route(self.router(h), self.top_k)
-        rows = F.gelu(ab.expert_mm(ab.dispatch(h, r), self.up, r.ends))
-        return (flat + ab.combine(ab.expert_mm(rows, self.down, r.ends), r)).view(x.shape)
+        return (flat + ab.expert_mlp(h, self.router(h), self.up, self.down, self.top_k)).view(x.shape)
 
 
 class Model(torch.nn.Module):
@@ -47,10 +46,19 @@ class Model(torch.nn.Module):
 
     def forward(self, ids: torch.Tensor) -> torch.Tensor:
         """Hidden states of ``ids`` [batch, seq], ready for the head."""
-        x = self.embed(ids)
+        x = ab.embed(ids, self.embed.weight)
         count = torch.arange(1, ids.shape[1] + 1, device=ids.device)[:, None]
         for block in self.blocks:
             x = block(x + (x.float().cumsum(1) / count).to(x.dtype))
+        return ab.layer_norm(x, self.norm.weight, self.norm.bias, self.norm.eps)
+
+    def step(self, ids: torch.Tensor, sums: list[torch.Tensor], count: int) -> torch.Tensor:
+        """Hidden states of the next token ``ids`` [batch] of each sequence, the ``count``-th; ``sums``, [batch, hidden] FP32 for each
+        block, hold the tokens before and take this one."""
+        x = ab.embed(ids, self.embed.weight)
+        for block, total in zip(self.blocks, sums):
+            total += x.float()
+            x = block(x + (total / count).to(x.dtype))
         return ab.layer_norm(x, self.norm.weight, self.norm.bias, self.norm.eps)
 
 
@@ -85,10 +93,19 @@ def train(steps: int, device: str, precision: str, batch: int = 8, seq: int = 64
 @torch.no_grad()
 def decode(model: Model, prompt: torch.Tensor, tokens: int) -> torch.Tensor:
     """``tokens`` greedy tokens after ``prompt`` [seq], one at a time."""
-    ids = prompt[None]
-    for _ in range(tokens):
-        ids = torch.cat((ids, model.head(model(ids)[:, -1]).argmax(-1, keepdim=True)), 1)
-    return ids[0, len(prompt):]
+    sums = [torch.zeros(1, model.norm.normalized_shape[0], device=prompt.device) for _ in model.blocks]
+    ids = list(prompt[:, None])
+    for i in range(len(prompt) + tokens - 1):
+        hidden = model.step(ids[i], sums, i + 1)
+        if i + 1 == len(ids):
+            ids.append(model.head(hidden).argmax(-1))
+    return torch.cat(ids[len(prompt):])
+
+
+@torch.no_grad()
+def score(model: Model, ids: torch.Tensor) -> torch.Tensor:
+    """The log-probability of each token of ``ids`` [seq] after the first, given those before it."""
+    return -ab.token_losses(model(ids[None])[0, :-1], model.head.weight, ids[1:])
 
 
 def main() -> None:
@@ -102,6 +119,7 @@ def main() -> None:
         print(f"step {step:4d}  loss {losses[step]:.4f}")
     got = decode(model, ids[:24], 16)
     print("decoded", got.tolist(), "of", ids[24:40].tolist())
+    print(f"lowest probability of them {score(model, torch.cat((ids[:24], got)))[-16:].exp().min().item():.3f}")
 
 
 if __name__ == "__main__":
