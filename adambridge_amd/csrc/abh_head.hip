@@ -50,11 +50,17 @@ __device__ __forceinline__ Sums merged(const Sums a, const Sums b)
     return Sums{m, a.s * exp_of(a.m, t) + b.s * exp_of(b.m, t)};
 }
 
+// A scored row's target (-1: none of the vocabulary's), and what its gradient takes.
+struct HeadRow {
+    int32_t word;
+    float top, scale, seed;   // the logits' maximum, gout / sum, gout
+};
+
 struct HeadArgs {
     const void* h;            // the scored rows, together: count x hidden
     const void* w;            // vocab x hidden
     const int64_t* targets;   // of all rows
-    const int32_t* index;     // a scored row's number among all
+    const HeadRow* facts;     // of the scored rows
     const int32_t* count;     // how many are scored
     int32_t rows, hidden;     // rows: all
     int64_t vocab, v0;        // the piece: words v0 .. v0 + width
@@ -62,8 +68,6 @@ struct HeadArgs {
     int32_t tiles_j;
     Sums* part;               // column tiles x rows
     float* picked;            // a scored row's logit of its target
-    const float* stats;       // of all rows: maximum, 1 / sum
-    const float* gout;        // of all rows
     void* g;                  // count x pitch
     float* dh;                // parts x count x hidden
     void* dw;                 // vocab x hidden
@@ -104,20 +108,61 @@ __global__ __launch_bounds__(1024) void k_head_rows(const int64_t* targets, int6
     if (threadIdx.x == 0) *count = before;
 }
 
-// The scored rows of h, together.
-template <int DT>
-__global__ __launch_bounds__(256) void k_head_gather(const void* h, const int32_t* index, const int32_t* count, int32_t hidden, void* out)
+// What the gather kernel takes for the rows' facts.  gout, stats: of all rows (maximum, 1 / sum); NULL in the forward call.
+struct HeadFacts {
+    HeadRow* out;
+    int64_t vocab;
+    const float *stats, *gout;
+    __device__ __forceinline__ void put(int64_t to, int64_t from, int64_t target) const
+    {
+        HeadRow row{target < 0 || target >= vocab ? -1 : (int32_t)target, 0.0f, 0.0f, 0.0f};
+        if (gout) {
+            row.seed = row.word < 0 ? __builtin_nanf("") : gout[from];
+            row.top = stats[2 * from];
+            row.scale = stats[2 * from + 1] * row.seed;
+        }
+        out[to] = row;
+    }
+};
+
+// The scored rows of h, together: a row a workgroup.  FIND: a row counts the scored ones before it for itself, which for a few
+// thousand rows is less than another launch (the row's place is one of T; what k_head_rows writes is written here).
+template <int DT, bool FIND>
+__global__ __launch_bounds__(256) void k_head_gather(const void* h, const int64_t* targets, int64_t ignore, int32_t rows, int32_t* index, int32_t* place,
+                                                     int32_t* count, float* losses, HeadFacts facts, int32_t hidden, void* out)
 {
     constexpr int L = kLane<DT>;
-    const int64_t i = block_index();
-    if (i >= *count) return;
-    const void* from = at<DT>(h, (int64_t)index[i] * hidden);
-    void* to = at<DT>(out, i * hidden);
+    int64_t to = block_index(), from;
+    if constexpr (FIND) {
+        __shared__ int32_t part[4];
+        from = to;
+        const bool scored = targets[from] != ignore;
+        int32_t n = 0;
+        for (int64_t t = threadIdx.x; t < from; t += 256) n += targets[t] != ignore;
+        n = group_reduce<kWave>(n, [](int32_t a, int32_t b) { return a + b; });
+        if (threadIdx.x % kWave == 0) part[threadIdx.x / kWave] = n;
+        __syncthreads();
+        n = part[0] + part[1] + part[2] + part[3];
+        if (threadIdx.x == 0) {
+            if (scored) index[n] = (int32_t)from;
+            if (place) place[from] = scored ? n : -1;
+            if (losses && !scored) losses[from] = 0.0f;
+            if (from == rows - 1) *count = n + scored;
+        }
+        if (!scored) return;
+        to = n;
+    } else {
+        if (to >= *count) return;
+        from = index[to];
+    }
+    if (threadIdx.x == 0) facts.put(to, from, targets[from]);
+    const void* row = at<DT>(h, from * hidden);
+    void* copy = at<DT>(out, to * hidden);
     for (int32_t c = threadIdx.x * L; c < hidden; c += 256 * L) {
         if (c + L <= hidden) {
-            store_raw<DT>(to, c, load_raw<DT>(from, c));
+            store_raw<DT>(copy, c, load_raw<DT>(row, c));
         } else {
-            for (int32_t k = c; k < hidden; ++k) put<DT>(to, k, get<DT>(from, k));
+            for (int32_t k = c; k < hidden; ++k) put<DT>(copy, k, get<DT>(row, k));
         }
     }
 }
@@ -149,7 +194,9 @@ __device__ __forceinline__ bool head_tile(int tiles_i, int tiles_j, int splits, 
 template <class C_, bool EVEN_>
 struct HeadBf16 {
     typedef C_ C;
-    static constexpr int DT = DT_BF16, BM = C::BM, BN = C::BN, BK = C::BK, NI = C::NI, NJ = C::NJ, WJ = C::WJ, T = C::T, OCC = C::OCC;
+    static constexpr int DT = DT_BF16, BM = C::BM, BN = C::BN, BK = C::BK, WJ = C::WJ, T = C::T, OCC = C::OCC;
+    static constexpr int NI = BM / C::WI / 16, NJ = BN / WJ / 16, R = 4, SIDE = 16;   // sums of 16 x 16, four a lane
+    typedef mm_f32x4 Sum;
     static constexpr bool EVEN = EVEN_;
     static constexpr int LDS = C::NB * C::BYTES;
     static __device__ __forceinline__ int wi() { return (int)threadIdx.x / kWave / WJ * (BM / C::WI); }
@@ -157,7 +204,8 @@ struct HeadBf16 {
 };
 template <int B>
 struct HeadF32 {
-    static constexpr int DT = DT_F32, BM = B, BN = B, BK = 32, NI = B / 64, NJ = B / 64, WJ = 2, T = 256, OCC = 2;
+    static constexpr int DT = DT_F32, BM = B, BN = B, BK = 32, NI = B / 64, NJ = B / 64, WJ = 2, T = 256, OCC = 2, R = 16, SIDE = 32;
+    typedef mm_f32x16 Sum;
     static constexpr bool EVEN = false;
     static constexpr int LDS = 2 * 2 * B * 32 * 4;
     static __device__ __forceinline__ int wi() { return (int)(threadIdx.x / kWave & 1) * (B / 2); }
@@ -173,21 +221,26 @@ struct Operand {
 
 // The tile's sums; false where the wavefront has no row.
 template <class H, bool ALONG, bool BLONG>
-__device__ __forceinline__ bool head_multiply(uint8_t* lds, const Operand& a, const Operand& b, bool live, mm_f32x16 (&acc)[H::NI][H::NJ])
+__device__ __forceinline__ bool head_multiply(uint8_t* lds, const Operand& a, const Operand& b, bool live, typename H::Sum (&acc)[H::NI][H::NJ])
 {
     const int steps = ((a.len > b.len ? a.len : b.len) + H::BK - 1) / H::BK;
     if constexpr (H::DT == DT_BF16) {
         typedef typename H::C C;
         TileFeed<ALONG, H::BM, H::BK, C::W, H::EVEN> fa;
         TileFeed<BLONG, H::BN, H::BK, C::W, H::EVEN> fb;
-        if constexpr (H::EVEN) {
+        if constexpr (H::EVEN) {   // (rows past the operand's last: zeros)
             fa.start(ALONG ? a.p : a.p + (int64_t)a.first * 2, a.pitch * 2, a.rows, a.len, ALONG ? 0 : a.first * 2);
             fb.start(BLONG ? b.p : b.p + (int64_t)b.first * 2, b.pitch * 2, b.rows, b.len, BLONG ? 0 : b.first * 2);
         } else {
             fa.start(a.p, a.pitch, ALONG ? 0 : a.first, a.rows, a.len);
             fb.start(b.p, b.pitch, BLONG ? 0 : b.first, b.rows, b.len);
         }
-        return multiply_tile<C, ALONG, BLONG, H::EVEN>(lds, fa, fb, steps, H::wi(), H::wj(), live, acc);
+        if constexpr (std::is_same<C, WideTile>::value) {
+            multiply_wide<C, ALONG, BLONG>(lds, fa, fb, steps, H::wi(), H::wj(), acc);
+            return true;
+        } else {
+            return multiply_tile16<C, ALONG, BLONG, H::EVEN>(lds, fa, fb, steps, H::wi(), H::wj(), live, acc);
+        }
     } else {
         StagedFeed<DT_F32, ALONG, H::BM, 32, 4> fa;
         StagedFeed<DT_F32, BLONG, H::BN, 32, 4> fb;
@@ -198,23 +251,39 @@ __device__ __forceinline__ bool head_multiply(uint8_t* lds, const Operand& a, co
     }
 }
 
-// Column of the tile that is a lane's value r of its columns j.
-__device__ __forceinline__ int column_of(int wj, int j, int r) { return wj + 32 * j + 8 * (r >> 2) + 4 * (int)((threadIdx.x & 63) >> 5) + (r & 3); }
+// Column of the tile that is a lane's value r of its columns j, and its row of the rows i.
+template <class H>
+__device__ __forceinline__ int column_of(int wj, int j, int r)
+{
+    const int lane = threadIdx.x & 63;
+    if constexpr (H::SIDE == 16) return wj + 16 * j + 4 * (lane >> 4) + r;
+    else return wj + 32 * j + 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+}
+template <class H>
+__device__ __forceinline__ int row_of(int wi, int i) { return wi + H::SIDE * i + (int)(threadIdx.x & (H::SIDE - 1)); }
 
-// A target's column in the tile, from its distance to the tile's first word; one outside the tile.
-__device__ __forceinline__ int hot_column(int64_t distance, int limit) { return distance >= 0 && distance < limit ? (int)distance : -1; }
+// op over the lanes that have a row's values.
+template <class H, class Op>
+__device__ __forceinline__ float over_row(float x, Op op)
+{
+    if constexpr (H::SIDE == 16) x = op(x, __shfl_xor(x, 16));
+    return op(x, __shfl_xor(x, 32));
+}
+
+// A target's column in the tile that begins at word `first`; -1 outside the tile.
+__device__ __forceinline__ int hot_column(int word, int64_t first, int limit) { return word >= first && word < first + limit ? (int)(word - first) : -1; }
 
 // What lies behind the vocabulary's last word.
 template <class H>
-__device__ __forceinline__ void mask_columns(mm_f32x16 (&acc)[H::NI][H::NJ], int wj, int limit, float to)
+__device__ __forceinline__ void mask_columns(typename H::Sum (&acc)[H::NI][H::NJ], int wj, int limit, float to)
 {
 #pragma unroll
     for (int i = 0; i < H::NI; ++i)
 #pragma unroll
         for (int j = 0; j < H::NJ; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (column_of(wj, j, r) >= limit) acc[i][j][r] = to;
+            for (int r = 0; r < H::R; ++r)
+                if (column_of<H>(wj, j, r) >= limit) acc[i][j][r] = to;
 }
 
 // ------------------------------------------------------------------------------ forward
@@ -231,41 +300,41 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_sums(HeadArgs A)
     const int i0 = t.ti * H::BM, j0 = t.tj * H::BN, limit_i = count - i0, limit_j = A.width - j0;
     const Operand a{at<H::DT>(A.h, (int64_t)i0 * A.hidden), A.hidden, 0, limit_i, A.hidden};
     const Operand b{at<H::DT>(A.w, (A.v0 + j0) * A.hidden), A.hidden, 0, limit_j, A.hidden};
-    mm_f32x16 acc[H::NI][H::NJ];
+    typename H::Sum acc[H::NI][H::NJ];
     const int wi = H::wi(), wj = H::wj(), lane = threadIdx.x & 63;
-    int hot[H::NI];   // the target's column in the tile, or one outside it
+    int word[H::NI];   // the rows' targets, asked for before the product, with no condition: eight loads on their way at once
 #pragma unroll
     for (int i = 0; i < H::NI; ++i) {
-        const int row = wi + 32 * i + (lane & 31);
-        hot[i] = row < limit_i ? hot_column(A.targets[A.index[i0 + row]] - j0, limit_j) : -1;
+        const int row = row_of<H>(wi, i);
+        word[i] = A.facts[i0 + (row < limit_i ? row : 0)].word;
     }
     const bool live = head_multiply<H, true, true>(lds, a, b, wi < limit_i, acc);
     if (live) {
         if (limit_j < H::BN) mask_columns<H>(acc, wj, limit_j, kHeadNegInf);
 #pragma unroll
         for (int i = 0; i < H::NI; ++i) {
-            const int row = wi + 32 * i + (lane & 31);
-            if (__builtin_amdgcn_ballot_w64(hot[i] >= wj && hot[i] < wj + H::BN / H::WJ)) {
+            const int row = row_of<H>(wi, i), hot = row < limit_i ? hot_column(word[i], j0, limit_j) : -1;
+            if (__builtin_amdgcn_ballot_w64(hot >= wj && hot < wj + H::BN / H::WJ)) {
 #pragma unroll
                 for (int j = 0; j < H::NJ; ++j)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (column_of(wj, j, r) == hot[i]) A.picked[i0 + row] = acc[i][j][r];
+                    for (int r = 0; r < H::R; ++r)
+                        if (column_of<H>(wj, j, r) == hot) A.picked[i0 + row] = acc[i][j][r];
             }
             float m = kHeadNegInf;
 #pragma unroll
             for (int j = 0; j < H::NJ; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) m = __builtin_fmaxf(m, acc[i][j][r]);
-            m = __builtin_fmaxf(m, __shfl_xor(m, 32));
+                for (int r = 0; r < H::R; ++r) m = __builtin_fmaxf(m, acc[i][j][r]);
+            m = over_row<H>(m, [](float a, float b) { return __builtin_fmaxf(a, b); });
             const float shift = shift_for(m);
             float s = 0.0f;
 #pragma unroll
             for (int j = 0; j < H::NJ; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s += exp_of(acc[i][j][r], shift);
-            s += __shfl_xor(s, 32);
-            if (lane < 32) row_sums[wj / (H::BN / H::WJ)][row] = Sums{m, s};
+                for (int r = 0; r < H::R; ++r) s += exp_of(acc[i][j][r], shift);
+            s = over_row<H>(s, [](float a, float b) { return a + b; });
+            if (lane < H::SIDE) row_sums[wj / (H::BN / H::WJ)][row] = Sums{m, s};
         }
     }
     __syncthreads();
@@ -390,7 +459,14 @@ __global__ __launch_bounds__(kFinishLanes) void k_head_finish(const Sums* part, 
     if (block_index() * R >= rows) return;
     Sums all{kHeadNegInf, 0.0f};
     if (row < rows)
-        for (int32_t p = slice; p < parts; p += S) all = merged(all, part[(int64_t)p * stride + row]);
+        for (int32_t p = slice; p < parts; p += 4 * S) {   // four reads on their way
+            Sums next[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) next[k] = part[(int64_t)(p + k * S < parts ? p + k * S : p) * stride + row];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (p + k * S < parts) all = merged(all, next[k]);
+        }
     tree[slice][r] = all;
     __syncthreads();
 #pragma unroll
@@ -422,32 +498,28 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_grad(HeadArgs A)
     const int i0 = t.ti * H::BM, j0 = t.tj * H::BN, limit_i = count - i0, limit_j = A.width - j0;
     const Operand a{at<H::DT>(A.h, (int64_t)i0 * A.hidden), A.hidden, 0, limit_i, A.hidden};
     const Operand b{at<H::DT>(A.w, (A.v0 + j0) * A.hidden), A.hidden, 0, limit_j, A.hidden};
-    mm_f32x16 acc[H::NI][H::NJ];
+    typename H::Sum acc[H::NI][H::NJ];
     const int wi = H::wi(), wj = H::wj(), lane = threadIdx.x & 63;
-    // a row's numbers, asked for before the product
-    int hot[H::NI];
-    float top[H::NI], scale[H::NI], seed[H::NI];
+    // the rows' numbers, asked for before the product, with no condition
+    HeadRow facts[H::NI];
 #pragma unroll
     for (int i = 0; i < H::NI; ++i) {
-        const int row = wi + 32 * i + (lane & 31);
-        const int64_t at_row = row < limit_i ? A.index[i0 + row] : 0, target = A.targets[at_row];
-        hot[i] = hot_column(target - A.v0 - j0, limit_j);
-        seed[i] = target < 0 || target >= A.vocab ? __builtin_nanf("") : A.gout[at_row];
-        top[i] = A.stats[2 * at_row];
-        scale[i] = A.stats[2 * at_row + 1] * seed[i];
+        const int row = row_of<H>(wi, i);
+        facts[i] = A.facts[i0 + (row < limit_i ? row : 0)];
     }
     if (!head_multiply<H, true, true>(lds, a, b, wi < limit_i, acc)) return;
 #pragma unroll
     for (int i = 0; i < H::NI; ++i) {
+        const int hot = hot_column(facts[i].word, A.v0 + j0, limit_j);
 #pragma unroll
         for (int j = 0; j < H::NJ; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = exp_of(acc[i][j][r], top[i]) * scale[i];
-        if (__builtin_amdgcn_ballot_w64(hot[i] >= wj && hot[i] < wj + H::BN / H::WJ)) {
+            for (int r = 0; r < H::R; ++r) acc[i][j][r] = exp_of(acc[i][j][r], facts[i].top) * facts[i].scale;
+        if (__builtin_amdgcn_ballot_w64(hot >= wj && hot < wj + H::BN / H::WJ)) {
 #pragma unroll
             for (int j = 0; j < H::NJ; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) acc[i][j][r] -= column_of(wj, j, r) == hot[i] ? seed[i] : 0.0f;
+                for (int r = 0; r < H::R; ++r) acc[i][j][r] -= column_of<H>(wj, j, r) == hot ? facts[i].seed : 0.0f;
         }
     }
     if (limit_j < H::BN) mask_columns<H>(acc, wj, limit_j, 0.0f);
@@ -457,14 +529,14 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_grad(HeadArgs A)
     } else {
 #pragma unroll
         for (int i = 0; i < H::NI; ++i) {
-            const int row = wi + 32 * i + (lane & 31);
+            const int row = row_of<H>(wi, i);
             if (row >= limit_i) continue;
             float* out = static_cast<float*>(A.g) + (int64_t)(i0 + row) * A.pitch + j0;
 #pragma unroll
             for (int j = 0; j < H::NJ; ++j)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const int c = column_of(wj, j, 4 * q);
+                    const int c = column_of<H>(wj, j, 4 * q);
                     if (c < wide) *reinterpret_cast<mm_f32x4*>(out + c) = mm_f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
                 }
         }
@@ -496,19 +568,19 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_dh(HeadArgs A)
     // G has zeros up to whole pieces, where W has ended
     const Operand a{at<H::DT>(A.g, (int64_t)i0 * A.pitch + k0), A.pitch, 0, limit_i, (len + 7) & ~7};
     const Operand b{at<H::DT>(A.w, (A.v0 + k0) * A.hidden), A.hidden, j0, A.hidden, len};
-    mm_f32x16 acc[H::NI][H::NJ];
+    typename H::Sum acc[H::NI][H::NJ];
     const int wi = H::wi(), wj = H::wj(), lane = threadIdx.x & 63;
     if (!head_multiply<H, true, false>(lds, a, b, wi < limit_i, acc)) return;
     float* out = A.dh + ((int64_t)t.split * count + i0) * A.hidden + j0;
 #pragma unroll
     for (int i = 0; i < H::NI; ++i) {
-        const int row = wi + 32 * i + (lane & 31);
+        const int row = row_of<H>(wi, i);
         if (row >= limit_i) continue;
 #pragma unroll
         for (int j = 0; j < H::NJ; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int c = column_of(wj, j, 4 * q);
+            for (int q = 0; q < H::R / 4; ++q) {
+                const int c = column_of<H>(wj, j, 4 * q);
                 float four[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
                 if (!A.fresh) {
                     float old[4];
@@ -532,7 +604,7 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_dw(HeadArgs A)
     const int i0 = t.ti * H::BM, j0 = t.tj * H::BN, limit_i = A.width - i0, limit_j = A.hidden - j0;
     const Operand a{static_cast<const uint8_t*>(A.g), A.pitch, i0, A.pitch, count};
     const Operand b{static_cast<const uint8_t*>(A.h), A.hidden, j0, A.hidden, count};
-    mm_f32x16 acc[H::NI][H::NJ];
+    typename H::Sum acc[H::NI][H::NJ];
     const int wi = H::wi(), wj = H::wj(), lane = threadIdx.x & 63;
     if (!head_multiply<H, false, false>(lds, a, b, wi < limit_i, acc)) return;
     uint8_t* out = at<H::DT>(A.dw, (A.v0 + i0) * A.hidden + j0);
@@ -541,14 +613,14 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_dw(HeadArgs A)
     } else {
 #pragma unroll
         for (int i = 0; i < H::NI; ++i) {
-            const int row = wi + 32 * i + (lane & 31);
+            const int row = row_of<H>(wi, i);
             if (row >= limit_i) continue;
 #pragma unroll
             for (int j = 0; j < H::NJ; ++j)
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const float four[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                    store_like<DT_F32, 4>(reinterpret_cast<float*>(out) + (int64_t)row * A.hidden, column_of(wj, j, 4 * q), limit_j, four);
+                    store_like<DT_F32, 4>(reinterpret_cast<float*>(out) + (int64_t)row * A.hidden, column_of<H>(wj, j, 4 * q), limit_j, four);
                 }
         }
     }
@@ -608,23 +680,27 @@ struct Scratch {
     }
 };
 
-// A kernel's tile.
-enum Kind { LARGE, HALF, F32_128, F32_64 };
-static int tile_m(Kind k) { return k == LARGE || k == HALF ? 256 : k == F32_64 ? 64 : 128; }
-static int tile_n(Kind k) { return k == LARGE ? 256 : k == F32_64 ? 64 : 128; }
-static int places_of(Kind k) { return (k == LARGE ? 1 : k == F32_64 ? 4 : 2) * kHeadCus; }
+// A kernel's tile.  WIDE and LARGE have the same one: rows of whole pieces, and of any length.
+enum Kind { WIDE, LARGE, HALF, F32_128, F32_64 };
+static int tile_m(Kind k) { return k == F32_64 ? 64 : k == F32_128 ? 128 : 256; }
+static int tile_n(Kind k) { return k == WIDE || k == LARGE ? 256 : k == F32_64 ? 64 : 128; }
+static int places_of(Kind k) { return (k == WIDE || k == LARGE ? 1 : k == F32_64 ? 4 : 2) * kHeadCus; }
 static int64_t tiles_of(Kind k, int64_t m, int64_t n) { return (m + tile_m(k) - 1) / tile_m(k) * ((n + tile_n(k) - 1) / tile_n(k)); }
-static_assert(HalfTile::BM == 256 && HalfTile::BN == 128, "tile_m, tile_n");
+static_assert(HalfTile::BM == 256 && HalfTile::BN == 128 && WideTile::BM == LargeTile::BM && WideTile::BN == LargeTile::BN, "tile_m, tile_n");
 
-// The tile for m x n sums.  FP32: as the expert products' rule, 64 where tiles of 128 are few.  BF16: 256 x 256; dW's 256 x 128, two
-// workgroups a CU, where their columns end closer behind the last one (us, 256 / 128 columns: dW of 2703 rows and 50688 words of 896
-// values 286 / 240, of 16384 rows and 16128 words of 4096 1649 / 1732; the other kernels are 8-18% slower on half tiles).
+// The tile for m x n sums of so many terms.  FP32: as the expert products' rule, 64 where tiles of 128 are few.  BF16: 256 x 256;
+// dW's 256 x 128, two workgroups a CU, where their columns end closer behind the last one (us, 256 / 128 columns: dW of 2703 rows
+// and 50688 words of 896 values 286 / 240, of 16384 rows and 16128 words of 4096 1649 / 1732; the other kernels are 8-18% slower on
+// half tiles).  Four wavefronts a workgroup where the sums are long, else eight, whose epilogues hide one another's waits (us, four
+// / eight: 4096 rows of 32768 words of 1024 values 321 / 303, 2048 487 / 486, 4096 853 / 901, 8192 1599 / 1705).
 enum Product { SUMS, WEIGHTS, ROWS };   // the logits, dW, dh
-static Kind kind_of(int32_t dtype, int64_t m, int64_t n, Product product)
+static Kind kind_of(int32_t dtype, int64_t m, int64_t n, int64_t terms, Product product)
 {
     if (dtype != ADAMBRIDGE_DT_BF16) return tiles_of(F32_128, m, n) < 512 ? F32_64 : F32_128;
-    if (product == WEIGHTS) return tiles_of(HALF, m, n) * 21 < tiles_of(LARGE, m, n) * 40 ? HALF : LARGE;   // 1.05 times the values
-    return product == SUMS && tiles_of(LARGE, m, n) <= kHeadCus / 2 ? HALF : LARGE;
+    if (product == WEIGHTS && tiles_of(HALF, m, n) * 21 < tiles_of(LARGE, m, n) * 40) return HALF;   // 1.05 times the values
+    if (product == SUMS && tiles_of(LARGE, m, n) <= kHeadCus / 2) return HALF;
+    if (product == ROWS) terms /= dh_splits(tiles_of(LARGE, m, n), places_of(LARGE), (int)terms);
+    return terms >= 2048 ? WIDE : LARGE;
 }
 
 // The forward call's plan and scratch.
@@ -633,6 +709,7 @@ struct HeadForward {
     Kind kind;
     int parts;
     int32_t *index, *count;
+    HeadRow* facts;
     float* picked;
     Sums* part;
     void* h;
@@ -642,12 +719,13 @@ struct HeadForward {
         // rows that stream the weights, or go on tiles (us, 151936 x 896 and 32000 x 4096: BF16, 32 rows 72 and 75 streamed; 65 on
         // tiles 72 and 76; FP32, 64 streamed 256 and 294, 65 on tiles 329 and 355)
         few = rows <= (dtype == ADAMBRIDGE_DT_BF16 ? 16 : 64);
-        kind = kind_of(dtype, rows, vocab, SUMS);
+        kind = kind_of(dtype, rows, vocab, hidden, SUMS);
         parts = (int)(few ? (vocab + 64 * kFewGroups - 1) / (64 * kFewGroups) : (vocab + tile_n(kind) - 1) / tile_n(kind));
         Scratch s{static_cast<uint8_t*>(work)};
         picked = s.take<float>(rows);
         part = s.take<Sums>(parts * rows);
         index = few ? nullptr : s.take<int32_t>(rows);
+        facts = few ? nullptr : s.take<HeadRow>(rows);
         count = few ? nullptr : s.take<int32_t>(1);
         h = few ? nullptr : s.take<uint8_t>(rows * hidden * (dtype == ADAMBRIDGE_DT_BF16 ? 2 : 4));
         bytes = s.used;
@@ -659,6 +737,7 @@ struct HeadBackward {
     Kind grad, dw, dh_kind;
     int32_t pitch;   // words of a piece
     int32_t *index, *place, *count;
+    HeadRow* facts;
     void *h, *g;
     float* dh;
     int64_t bytes;
@@ -668,11 +747,12 @@ struct HeadBackward {
         const int64_t most = std::max(kPieceValues / rows, kLeastPiece), pieces = (vocab + most - 1) / most;
         pitch = (int32_t)up((vocab + pieces - 1) / pieces, 256);
         const int64_t width = std::min<int64_t>(pitch, vocab);
-        grad = kind_of(dtype, rows, width, SUMS);
-        dw = kind_of(dtype, width, hidden, WEIGHTS);
-        dh_kind = kind_of(dtype, rows, hidden, ROWS);
+        grad = kind_of(dtype, rows, width, hidden, SUMS);
+        dw = kind_of(dtype, width, hidden, rows, WEIGHTS);
+        dh_kind = kind_of(dtype, rows, hidden, pitch, ROWS);
         Scratch s{static_cast<uint8_t*>(work)};
         index = s.take<int32_t>(rows);
+        facts = s.take<HeadRow>(rows);
         place = s.take<int32_t>(rows);
         count = s.take<int32_t>(1);
         h = s.take<uint8_t>(rows * hidden * size);
@@ -692,16 +772,31 @@ static dim3 tile_grid(int64_t tiles) { return block_grid(up(tiles, kXcd)); }
     } while (0)
 #define ABH_HEAD_LAUNCH(KERNEL, KIND, EVEN, GRID)                                                                  \
     do {                                                                                                           \
-        if ((KIND) == LARGE) ABH_HEAD_BF16(KERNEL, LargeTile, EVEN, GRID);                                         \
+        if ((KIND) == WIDE && (EVEN)) hipLaunchKernelGGL((KERNEL<HeadBf16<WideTile, true>>), GRID, dim3(WideTile::T), 0, t_stream, A); \
+        else if ((KIND) == WIDE || (KIND) == LARGE) ABH_HEAD_BF16(KERNEL, LargeTile, EVEN, GRID);                  \
         else if ((KIND) == HALF) ABH_HEAD_BF16(KERNEL, HalfTile, EVEN, GRID);                                      \
         else if ((KIND) == F32_128) hipLaunchKernelGGL((KERNEL<HeadF32<128>>), GRID, dim3(256), 0, t_stream, A);   \
         else hipLaunchKernelGGL((KERNEL<HeadF32<64>>), GRID, dim3(256), 0, t_stream, A);                           \
     } while (0)
 
-static void launch_gather(bool bf, int64_t rows, const void* hidden_rows, const int32_t* index, const int32_t* count, int64_t hidden, void* out)
+// The scored rows: their numbers, how many, and copies of them.  One launch for a few thousand rows, whose counts grow with the
+// square of them, else two (us, one / two: the forward call of 100 rows of 151936 x 896 71.1 / 73.5; the kernels alone at 4096 rows
+// 10.8 / 11.3, at 16384 the first of two 17).
+constexpr int64_t kFindRows = 2048;
+
+static void launch_rows(bool bf, const void* h, const int64_t* targets, int64_t ignore, int64_t rows, int32_t* index, int32_t* place, int32_t* count,
+                        float* losses, const HeadFacts& facts, int64_t hidden, void* out)
 {
-    if (bf) hipLaunchKernelGGL((k_head_gather<DT_BF16>), block_grid(rows), dim3(256), 0, t_stream, hidden_rows, index, count, (int32_t)hidden, out);
-    else hipLaunchKernelGGL((k_head_gather<DT_F32>), block_grid(rows), dim3(256), 0, t_stream, hidden_rows, index, count, (int32_t)hidden, out);
+    const dim3 grid = block_grid(rows), block(256);
+    const int32_t n = (int32_t)rows, size = (int32_t)hidden;
+    if (rows <= kFindRows) {
+        if (bf) hipLaunchKernelGGL((k_head_gather<DT_BF16, true>), grid, block, 0, t_stream, h, targets, ignore, n, index, place, count, losses, facts, size, out);
+        else hipLaunchKernelGGL((k_head_gather<DT_F32, true>), grid, block, 0, t_stream, h, targets, ignore, n, index, place, count, losses, facts, size, out);
+        return;
+    }
+    hipLaunchKernelGGL(k_head_rows, dim3(1), dim3(1024), 0, t_stream, targets, ignore, n, index, place, count, losses);
+    if (bf) hipLaunchKernelGGL((k_head_gather<DT_BF16, false>), grid, block, 0, t_stream, h, targets, ignore, n, index, place, count, losses, facts, size, out);
+    else hipLaunchKernelGGL((k_head_gather<DT_F32, false>), grid, block, 0, t_stream, h, targets, ignore, n, index, place, count, losses, facts, size, out);
 }
 
 }  // namespace abh
@@ -747,10 +842,9 @@ ADAMBRIDGE_API int adambridge_token_losses(const void* hidden, const void* weigh
         hipLaunchKernelGGL((k_head_finish<4>), dim3((unsigned)((rows + 3) / 4)), dim3(kFinishLanes), 0, t_stream, p.part, p.parts, A.rows, nullptr,
                            nullptr, targets, vocab, ignore_index, p.picked, losses, stats);
     } else {
-        hipLaunchKernelGGL(k_head_rows, dim3(1), dim3(1024), 0, t_stream, targets, ignore_index, A.rows, p.index, (int32_t*)nullptr, p.count, losses);
-        launch_gather(bf, rows, hidden, p.index, p.count, size, p.h);
+        launch_rows(bf, hidden, targets, ignore_index, rows, p.index, nullptr, p.count, losses, HeadFacts{p.facts, vocab, nullptr, nullptr}, size, p.h);
         A.h = p.h;
-        A.index = p.index;
+        A.facts = p.facts;
         A.count = p.count;
         A.width = (int32_t)vocab;
         A.tiles_j = p.parts;
@@ -780,20 +874,16 @@ ADAMBRIDGE_API int adambridge_token_losses_backward(const float* gout, const voi
     if ((uintptr_t)work % 16) return ADAMBRIDGE_EALIGN;
     const bool bf = dtype == ADAMBRIDGE_DT_BF16;
     const HeadBackward p(work, dtype, rows, vocab, size);
-    hipLaunchKernelGGL(k_head_rows, dim3(1), dim3(1024), 0, t_stream, targets, ignore_index, (int32_t)rows, p.index, p.place, p.count, (float*)nullptr);
-    launch_gather(bf, rows, hidden, p.index, p.count, size, p.h);
+    launch_rows(bf, hidden, targets, ignore_index, rows, p.index, p.place, p.count, nullptr, HeadFacts{p.facts, vocab, stats, gout}, size, p.h);
     HeadArgs A{};
     A.h = p.h;
     A.w = weight;
-    A.targets = targets;
-    A.index = p.index;
+    A.facts = p.facts;
     A.count = p.count;
     A.rows = (int32_t)rows;
     A.hidden = (int32_t)size;
     A.vocab = vocab;
     A.pitch = p.pitch;
-    A.stats = stats;
-    A.gout = gout;
     A.g = p.g;
     A.dh = p.dh;
     A.dw = dweight;

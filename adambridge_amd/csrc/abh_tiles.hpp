@@ -121,32 +121,41 @@ struct Feed {
             }
         }
     }
-    // The next step's pieces to the LDS; past the last step: zeros.
-    __device__ __forceinline__ void issue(uint8_t* lds)
+    // The next step's pieces to the LDS; past the last step: zeros.  Piece by piece: where from, a piece, the step after.
+    __device__ __forceinline__ raw16 source() const
     {
-        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
         // the range ends with the operand: pieces over the end of its last term, and terms past it, are outside
         const int terms = left < BK + 1 ? left : BK + 1;
         const int bytes = LONG ? lead : terms * pitch - lead;
         const int range = left > 0 ? bytes : 0;
         const uint64_t first = (uint64_t)base;
-        const raw16 buffer = {(uint32_t)first, (uint32_t)(first >> 32) & 0xffffu, (uint32_t)range, 0x00020000u};
-        const bool last = left <= BK;
-#pragma unroll
-        for (int q = 0; q < N; ++q) {
-            // In assembly, so that the compiler does not wait for it before each transposed read: no register is written, and
-            // the arrival is waited for by wait_loads.
-            const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)(lds + (q * W + wave) * 1024);
-            const uint32_t from = LONG && last && past ? kOutside : offset[q];
+        return raw16{(uint32_t)first, (uint32_t)(first >> 32) & 0xffffu, (uint32_t)range, 0x00020000u};
+    }
+    __device__ __forceinline__ void issue_piece(int q, const raw16 buffer, uint8_t* lds) const
+    {
+        const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+        // In assembly, so that the compiler does not wait for it before each transposed read: no register is written, and
+        // the arrival is waited for by wait_loads.
+        const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)(lds + (q * W + wave) * 1024);
+        const uint32_t from = LONG && left <= BK && past ? kOutside : offset[q];
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"   // m0 is never allocated ("reserved"), but the compiler reuses what it put there itself
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
-                         :: "s"(to), "v"(from), "s"(buffer), "s"(along) : "m0", "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                     :: "s"(to), "v"(from), "s"(buffer), "s"(along) : "m0", "memory");
 #pragma clang diagnostic pop
-        }
+    }
+    __device__ __forceinline__ void advance()
+    {
         left -= BK;
         if constexpr (LONG) along += BK * 2;
         else base += BK * pitch;
+    }
+    __device__ __forceinline__ void issue(uint8_t* lds)
+    {
+        const raw16 buffer = source();
+#pragma unroll
+        for (int q = 0; q < N; ++q) issue_piece(q, buffer, lds);
+        advance();
     }
 };
 
@@ -270,6 +279,7 @@ struct Fragments {
 
 typedef Config<256, 256, 32, 4, 2, 4, 2> LargeTile;
 typedef Config<128, 128, 32, 4, 2, 2, 2> SmallTile;   // where large ones are too few for the CUs
+typedef Config<256, 256, 64, 2, 2, 2, 1> WideTile;    // four wavefronts of 128 x 128: multiply_wide
 typedef Config<256, 128, 32, 3, 2, 2, 2> HalfTile;    // two workgroups a CU: one's products beside the other's results
 
 // Asks the scheduler for READS reads of the LDS spread among the next PRODUCTS matrix products.
@@ -391,6 +401,279 @@ __device__ __forceinline__ bool multiply_tile(uint8_t* lds, TileFeed<ALONG, C::B
         if constexpr (EVEN) wait_loads<0>();   // nothing is on its way to the LDS when the workgroup ends
     }
     return true;
+}
+
+// ------------------------------------------------------------------- 16 x 16 x 32
+//
+// The same tiles by matrix instructions of 16 x 16 x 32, a step's 32 terms at once: a wavefront's 128 x 64 are 8 x 4 of them.
+
+// Reads of a wavefront's fragments: 16 rows, from row `first` of the tile of R rows, by 32 terms: the h-th of the step's.
+template <bool LONG, int R, int BK, int N>
+struct Fragments16 {
+    uint32_t place[LONG ? BK / 32 : N];
+    __device__ __forceinline__ void start(int first)
+    {
+        const int lane = threadIdx.x & 63, quarter = lane >> 4;
+        if constexpr (LONG) {
+            const int row = first + (lane & 15);   // the fragments are multiples of 16 apart: the same exchange
+#pragma unroll
+            for (int h = 0; h < BK / 32; ++h) place[h] = row * BK * 2 + (((4 * h + quarter) ^ swap_of_row<BK / 8>(row)) * 16);
+        } else {
+            const int within = (lane & 15) >> 2, term = 8 * quarter + within;   // within: the term mod 4
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int piece = (first + 16 * i) / 8 + ((lane & 3) >> 1);
+                place[i] = term * R * 2 + ((piece ^ swap_of_term<DT_BF16, R>(term)) * 16) + (lane & 1) * 8;
+            }
+        }
+    }
+    __device__ __forceinline__ mm_bf16x8 read(const uint8_t* lds, int i, int h) const
+    {
+        if constexpr (LONG) {
+            return __builtin_bit_cast(mm_bf16x8, *reinterpret_cast<const raw16*>(lds + place[h] + i * 16 * BK * 2));
+        } else {
+            typedef __attribute__((address_space(3))) mm_bf16x4* Local;
+            const uint8_t* p = lds + place[i] + h * 32 * R * 2;
+            const mm_bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Local)(p));
+            const mm_bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((Local)(p + 4 * R * 2));
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    }
+};
+
+// multiply_tile with them (us, 32 x 32 x 16 / 16 x 16 x 32: dW of 2703 rows and 50688 words of 896 values 244 / 232, 4096 x 32000
+// sums of 4096 terms 909 / 900).  A step is two halves of A's fragments: while the matrix cores work on one, the other's are read, or the
+// next step's first ones.
+template <class C, bool ALONG, bool BLONG, bool EVEN>
+__device__ __forceinline__ bool multiply_tile16(uint8_t* lds, TileFeed<ALONG, C::BM, C::BK, C::W, EVEN>& fa, TileFeed<BLONG, C::BN, C::BK, C::W, EVEN>& fb,
+                                                int steps, int wi, int wj, bool live, mm_f32x4 (&acc)[C::BM / C::WI / 16][C::BN / C::WJ / 16])
+{
+    constexpr int BM = C::BM, BN = C::BN, BK = C::BK, NB = C::NB, NI = BM / C::WI / 16, NJ = BN / C::WJ / 16, HI = NI / 2;
+    static_assert(BK == 32, "a step is one instruction deep");
+    constexpr int LEAD = EVEN ? NB - 1 : 2;
+    Fragments16<ALONG, BM, BK, NI> ra;
+    Fragments16<BLONG, BN, BK, NJ> rb;
+    ra.start(wi);
+    rb.start(wj);
+    auto issue = [&](int s, int buffer) {
+        uint8_t* la = lds + buffer * C::BYTES;
+        if constexpr (EVEN) {
+            fa.issue(la);
+            fb.issue(la + BM * BK * 2);
+        } else {
+            if (s < steps) {
+                fa.store(s, la);
+                fb.store(s, la + BM * BK * 2);
+            }
+            if (s + 1 < steps) {
+                fa.load(s + 1);
+                fb.load(s + 1);
+            }
+        }
+    };
+    if (steps > 0) {
+        if constexpr (!EVEN) {
+            fa.load(0);
+            fb.load(0);
+        }
+#pragma unroll
+        for (int s = 0; s < LEAD; ++s) issue(s, s);
+    }
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    mm_bf16x8 a[2][HI], b[NJ];
+    auto fetch_a = [&](int half, int buffer) {
+#pragma unroll
+        for (int i = 0; i < HI; ++i) a[half][i] = ra.read(lds + buffer * C::BYTES, half * HI + i, 0);
+    };
+    auto fetch_b = [&](int j, int buffer) { b[j] = rb.read(lds + buffer * C::BYTES + BM * BK * 2, j, 0); };
+    auto multiply = [&](int half, int j) {
+#pragma unroll
+        for (int i = 0; i < HI; ++i)
+            acc[half * HI + i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j], a[half][i], acc[half * HI + i][j], 0, 0, 0);
+    };
+    constexpr int RA = ALONG ? 1 : 2, RB = BLONG ? 1 : 2;   // reads of a fragment
+    if (steps > 0) {
+        if constexpr (EVEN) wait_loads<(NB - 2) * C::LOADS>();
+        __syncthreads();
+        int now = 0, next = 1, ahead = LEAD;
+        auto turn = [&]() {
+            now = next;
+            next = next + 1 == NB ? 0 : next + 1;
+            ahead = ahead + 1 == NB ? 0 : ahead + 1;
+        };
+        if (!live) {
+            for (int s = 0; s + 1 < steps; ++s) {
+                if constexpr (EVEN) wait_loads<(NB - 3) * C::LOADS>();
+                __syncthreads();
+                issue(s + LEAD, ahead);
+                turn();
+            }
+            if constexpr (EVEN) wait_loads<0>();
+            return false;
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) fetch_b(j, 0);
+        fetch_a(0, 0);
+        for (int s = 0; s + 1 < steps; ++s) {
+            fetch_a(1, now);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) multiply(0, j);
+            spread_reads<RA * HI, HI * NJ / 2>();   // early: the barrier waits for them
+            __builtin_amdgcn_sched_group_barrier(0x008, HI * NJ / 2, 0);
+            // the next step's pieces have arrived, everyone's after the barrier, and the step before has been read
+            if constexpr (EVEN) wait_loads<(NB - 3) * C::LOADS>();
+            __syncthreads();
+            issue(s + LEAD, ahead);
+            fetch_a(0, next);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                multiply(1, j);
+                fetch_b(j, next);   // in place of the one that these were the last products of
+            }
+            __builtin_amdgcn_sched_group_barrier(0x100, RA * HI / NJ, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, HI, 0);
+#pragma unroll
+            for (int j = 1; j < NJ; ++j) {
+                __builtin_amdgcn_sched_group_barrier(0x100, RA * HI / NJ + RB, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, HI, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x100, RB, 0);
+            turn();
+        }
+        fetch_a(1, now);
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) multiply(half, j);
+        if constexpr (EVEN) wait_loads<0>();   // nothing is on its way to the LDS when the workgroup ends
+    }
+    return true;
+}
+
+// The same by four wavefronts of 128 x 128, one a SIMD (rows of whole pieces).  They read two thirds of the LDS's bytes that eight
+// of 128 x 64 do.  A step is 64 terms, two instructions deep: a row's piece is then a whole line of 128 bytes, which steps of 32
+// terms ask the L2 for twice (4096 x 32000 sums of 4096 terms and a softmax's statistics: 127 million requests and 889 us by 32
+// terms, 843 by 64; eight wavefronts 886).  A half's fragments are in registers before its products begin.  In turns of 8 products
+// the other half's, or the next step's, are read beside them, B's early, A's each in the place of the one just used, and the step
+// after is sent on its way, two pieces a turn: what a CU takes from the L2.  The barrier stands where no read is pending.
+template <class C, bool ALONG, bool BLONG>
+__device__ __forceinline__ void multiply_wide(uint8_t* lds, Feed<ALONG, C::BM, C::BK, C::W>& fa, Feed<BLONG, C::BN, C::BK, C::W>& fb, int steps, int wi, int wj,
+                                              mm_f32x4 (&acc)[C::BM / C::WI / 16][C::BN / C::WJ / 16])
+{
+    constexpr int BM = C::BM, BN = C::BN, BK = C::BK, NB = C::NB, NI = BM / C::WI / 16, NJ = BN / C::WJ / 16;
+    typedef Feed<ALONG, C::BM, C::BK, C::W> FeedA;
+    typedef Feed<BLONG, C::BN, C::BK, C::W> FeedB;
+    static_assert(BK == 64 && NB == 2 && NI == 8 && NJ == 8 && FeedA::N == 8 && FeedB::N == 8, "the turns");
+    Fragments16<ALONG, BM, BK, NI> ra;
+    Fragments16<BLONG, BN, BK, NJ> rb;
+    ra.start(wi);
+    rb.start(wj);
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            acc[i][j] = mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            asm("" : "+a"(acc[i][j]));   // the sums live in the accumulation registers: the others are the fragments'
+        }
+    if (steps <= 0) return;
+    uint8_t *here = lds, *next = lds + C::BYTES;
+    auto issue = [&](const raw16 from_a, const raw16 from_b, int q, uint8_t* to) {
+        if (q < FeedA::N) fa.issue_piece(q, from_a, to);
+        else fb.issue_piece(q - FeedA::N, from_b, to + BM * BK * 2);
+    };
+    fa.issue(here);
+    fb.issue(here + BM * BK * 2);
+    fa.issue(next);
+    fb.issue(next + BM * BK * 2);
+    mm_bf16x8 a[NI], b[2][NJ];
+    wait_loads<C::LOADS>();
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) b[0][j] = rb.read(here + BM * BK * 2, j, 0);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) a[i] = ra.read(here, i, 0);
+    auto products = [&](int set, int i) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[set][j], a[i], acc[i][j], 0, 0, 0);
+    };
+    raw16 from_a = fa.source(), from_b = fb.source();
+    for (int s = 0; s < steps; ++s) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {   // the first half of the terms
+            if (s && i < 2) {
+                issue(from_a, from_b, 12 + 2 * i, next);
+                issue(from_a, from_b, 13 + 2 * i, next);
+            }
+            if (i == 1 && s) {
+                fa.advance();
+                fb.advance();
+            }
+            if (i < 4) {
+                b[1][2 * i] = rb.read(here + BM * BK * 2, 2 * i, 1);
+                b[1][2 * i + 1] = rb.read(here + BM * BK * 2, 2 * i + 1, 1);
+            }
+            products(0, i);
+            a[i] = ra.read(here, i, 1);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        from_a = fa.source();
+        from_b = fb.source();
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            if (i == 2) {
+                wait_loads<0>();   // the next step's pieces
+                __syncthreads();   // everyone's; and everyone has read this step's
+            }
+            if (i >= 2) {
+                issue(from_a, from_b, 2 * i - 4, here);
+                issue(from_a, from_b, 2 * i - 3, here);
+            }
+            if (i >= 2 && i < 6) {
+                b[0][2 * i - 4] = rb.read(next + BM * BK * 2, 2 * i - 4, 0);
+                b[0][2 * i - 3] = rb.read(next + BM * BK * 2, 2 * i - 3, 0);
+                if (i < 4) a[i - 2] = ra.read(next, i - 2, 0);
+            }
+            products(1, i);
+            if (i >= 2) a[i] = ra.read(next, i, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        uint8_t* const now = next;
+        next = here;
+        here = now;
+    }
+    wait_loads<0>();   // nothing is on its way to the LDS when the workgroup ends
+}
+
+// store_bf16 of such sums: a lane has row lane mod 16 and, of each 16 columns, four; neighbouring sixteens exchange fours.
+template <class C, bool EVEN, int NI, int NJ>
+__device__ __forceinline__ void store_bf16(uint8_t* out, int pitch, int limit_i, int limit_j, const mm_f32x4 (&acc)[NI][NJ], int wi, int wj)
+{
+    const int lane = threadIdx.x & 63, quarter = lane >> 4;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        const int row = wi + 16 * i + (lane & 15);
+#pragma unroll
+        for (int j = 0; j < NJ; j += 2) {
+            // sixteens 0 and 2 take the first 16 columns' eights, 1 and 3 the second's
+            const auto s0 = __builtin_amdgcn_permlane16_swap(bf16x2_rne(acc[i][j][0], acc[i][j][1]), bf16x2_rne(acc[i][j + 1][0], acc[i][j + 1][1]), false, false);
+            const auto s1 = __builtin_amdgcn_permlane16_swap(bf16x2_rne(acc[i][j][2], acc[i][j][3]), bf16x2_rne(acc[i][j + 1][2], acc[i][j + 1][3]), false, false);
+            const int c = wj + 16 * (j + (quarter & 1)) + 8 * (quarter >> 1);
+            const raw16 eight = {s0[0], s1[0], s0[1], s1[1]};
+            const int64_t o = (int64_t)row * pitch + c;
+            if (row >= limit_i || c >= limit_j) continue;
+            if (EVEN || c + 8 <= limit_j) {
+                store_raw<DT_BF16>(out, o, eight);
+            } else {
+                const uint32_t v[4] = {eight.x, eight.y, eight.z, eight.w};
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (c + r < limit_j) reinterpret_cast<uint16_t*>(out)[o + r] = (uint16_t)(v[r / 2] >> (16 * (r & 1)));
+            }
+        }
+    }
 }
 
 // A tile's results in BF16: rows of `pitch` values from out on, limit_i of them by limit_j.  EVEN: whole 16-byte pieces.
