@@ -65,7 +65,8 @@ struct HeadArgs {
     int32_t rows, hidden;     // rows: all
     int64_t vocab, v0;        // the piece: words v0 .. v0 + width
     int32_t width, pitch;     // pitch: a row of G
-    int32_t tiles_j;
+    int32_t tiles_j, splits;  // splits: of the logits' or dW's terms
+    float* parts;             // of split sums: splits x rows x pitch, or splits x width x hidden
     Sums* part;               // column tiles x rows
     float* picked;            // a scored row's logit of its target
     void* g;                  // count x pitch
@@ -190,6 +191,27 @@ __device__ __forceinline__ bool head_tile(int tiles_i, int tiles_j, int splits, 
     return true;
 }
 
+// How many parts sums are cut in whose tiles are few: so that they fill the CUs' places, of 512 terms or more.
+__device__ __host__ __forceinline__ int splits_of(int64_t tiles, int places, int64_t terms)
+{
+    const int64_t fit = places / (tiles < 1 ? 1 : tiles), most = terms / 512;
+    const int64_t n = fit < most ? fit : most;
+    return (int)(n < 1 ? 1 : n);
+}
+
+// A part's terms: whole steps.
+struct HeadTerms {
+    int first, len;
+};
+template <class H>
+__device__ __forceinline__ HeadTerms terms_of(int terms, int split, int splits)
+{
+    const int steps = (terms + H::BK - 1) / H::BK;
+    const int k0 = scalar(steps * split / splits * H::BK), k1 = scalar(steps * (split + 1) / splits * H::BK);
+    const int len = (k1 < terms ? k1 : terms) - k0;
+    return HeadTerms{k0, len < 0 ? 0 : len};
+}
+
 // What a kernel's type and tile are.  BF16: abh_tiles.hpp's; FP32: B x B of four wavefronts.
 template <class C_, bool EVEN_>
 struct HeadBf16 {
@@ -286,6 +308,128 @@ __device__ __forceinline__ void mask_columns(typename H::Sum (&acc)[H::NI][H::NJ
                 if (column_of<H>(wj, j, r) >= limit) acc[i][j][r] = to;
 }
 
+// The tile's sums in FP32.
+template <class H>
+__device__ __forceinline__ void store_sums(float* out, int64_t pitch, int limit_i, int limit_j, const typename H::Sum (&acc)[H::NI][H::NJ], int wi, int wj)
+{
+#pragma unroll
+    for (int i = 0; i < H::NI; ++i) {
+        const int row = row_of<H>(wi, i);
+        if (row >= limit_i) continue;
+#pragma unroll
+        for (int j = 0; j < H::NJ; ++j)
+#pragma unroll
+            for (int q = 0; q < H::R / 4; ++q) {
+                const float four[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                store_like<DT_F32, 4>(out + row * pitch, column_of<H>(wj, j, 4 * q), limit_j, four);
+            }
+    }
+}
+
+// --------------------------------------------------------------- few tiles: logits in parts
+//
+// Where the logits' tiles are too few for the CUs, their sums are cut along the terms: parts in FP32, which a workgroup a row adds
+// in order on its way over the row.
+
+template <class H>
+__global__ __launch_bounds__(H::T, H::OCC) void k_head_logits(HeadArgs A)
+{
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[H::LDS];
+    const int count = scalar(*A.count);
+    HeadTile t;
+    if (!head_tile((count + H::BM - 1) / H::BM, A.tiles_j, A.splits, t)) return;
+    const int i0 = t.ti * H::BM, j0 = t.tj * H::BN, limit_i = count - i0, limit_j = A.width - j0;
+    const HeadTerms k = terms_of<H>(A.hidden, t.split, A.splits);
+    const Operand a{at<H::DT>(A.h, (int64_t)i0 * A.hidden + k.first), A.hidden, 0, limit_i, k.len};
+    const Operand b{at<H::DT>(A.w, (A.v0 + j0) * A.hidden + k.first), A.hidden, 0, limit_j, k.len};
+    typename H::Sum acc[H::NI][H::NJ];
+    const int wi = H::wi(), wj = H::wj();
+    if (!head_multiply<H, true, true>(lds, a, b, wi < limit_i, acc)) return;
+    store_sums<H>(A.parts + ((int64_t)t.split * A.rows + i0) * A.pitch + j0, A.pitch, limit_i, limit_j, acc, wi, wj);
+}
+
+// Four logits of a row, from word v of the piece; to: what stands behind the last word.
+__device__ __forceinline__ void joined(const HeadArgs& A, int64_t row, int v, float to, float (&x)[4])
+{
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = 0.0f;
+    for (int s = 0; s < A.splits; ++s) {
+        float y[4];
+        to_floats<DT_F32>(load_raw<DT_F32>(A.parts + ((int64_t)s * A.rows + row) * A.pitch, v), y);   // a row has whole pieces
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] += y[k];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (v + k >= A.width) x[k] = to;
+}
+
+// A row's loss, and what the gradient takes.
+__device__ __forceinline__ void finish_row(Sums all, float picked, int64_t t, int64_t target, int64_t vocab, int64_t ignore, float* losses, float* stats)
+{
+    if (all.m == kHeadNegInf) all.s = __builtin_nanf("");   // every logit -inf: no distribution
+    if (stats) {
+        stats[2 * t] = all.m;
+        stats[2 * t + 1] = 1.0f / all.s;
+    }
+    losses[t] = target == ignore ? 0.0f : target < 0 || target >= vocab ? __builtin_nanf("") : logf(all.s) - (picked - all.m);
+}
+
+// The losses, LANES a row: the whole vocabulary is one piece here.
+template <int LANES>
+__global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void k_head_join(HeadArgs A, const int32_t* index, const int64_t* targets, int64_t ignore,
+                                                                        float* losses, float* stats)
+{
+    constexpr int ROWS = LANES < 256 ? 256 / LANES : 1, WAVES = LANES / kWave;
+    __shared__ Sums waves[ROWS][WAVES];
+    __shared__ float picked[ROWS];
+    const int slot = threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    const int64_t row = block_index() * ROWS + slot;
+    const bool real = row < *A.count;
+    const int word = real ? A.facts[row].word : -1;
+    Sums all{kHeadNegInf, 0.0f};
+    if (real)
+        for (int v = lane * 4; v < A.width; v += LANES * 4) {
+            float x[4];
+            joined(A, row, v, kHeadNegInf, x);
+            const float m = __builtin_fmaxf(__builtin_fmaxf(all.m, x[0]), __builtin_fmaxf(__builtin_fmaxf(x[1], x[2]), x[3])), shift = shift_for(m);
+            float s = all.s * exp_of(all.m, shift);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                s += exp_of(x[k], shift);
+                if (v + k == word) picked[slot] = x[k];
+            }
+            all = Sums{m, s};
+        }
+#pragma unroll
+    for (int d = 1; d < kWave; d <<= 1) all = merged(all, Sums{__shfl_xor(all.m, d), __shfl_xor(all.s, d)});
+    if (lane % kWave == 0) waves[slot][lane / kWave] = all;
+    __syncthreads();
+    if (lane || !real) return;
+    all = waves[slot][0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) all = merged(all, waves[slot][w]);
+    const int64_t t = index[row];
+    finish_row(all, picked[slot], t, targets[t], A.vocab, ignore, losses, stats);
+}
+
+// A piece's gradient at the logits: 4 words a lane, zeros behind the last one up to whole pieces.
+template <int DT>
+__global__ __launch_bounds__(256) void k_head_join_grad(HeadArgs A, int32_t columns)
+{
+    const int64_t row = block_index() / columns;
+    if (row >= *A.count) return;
+    const int v = ((int)(block_index() - row * columns) * 256 + (int)threadIdx.x) * 4;
+    if (v >= ((A.width + 7) & ~7)) return;
+    const HeadRow facts = A.facts[row];
+    float x[4];
+    joined(A, row, v, 0.0f, x);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        x[k] = v + k < A.width ? exp_of(x[k], facts.top) * facts.scale - (A.v0 + v + k == facts.word ? facts.seed : 0.0f) : 0.0f;
+    store_like<DT, 4>(at<DT>(A.g, row * A.pitch), v, A.pitch, x);
+}
+
 // ------------------------------------------------------------------------------ forward
 
 // Each row's maximum and sum over the tile's words, and the target's logit.
@@ -346,13 +490,13 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_sums(HeadArgs A)
     }
 }
 
-// The same of few rows: the weights are read once, NG times 16 words a wavefront, which share the rows' loads.  part: workgroups x
-// rows.  CH: 16 rows each.
-template <int DT, bool EVEN, int CH>
+// The same of 16 rows or fewer: the weights are read once, NG times 16 words a wavefront, which share the rows' loads.  part:
+// workgroups x rows.
+template <int DT, bool EVEN>
 __global__ __launch_bounds__(256) void k_head_few(HeadArgs A)
 {
     constexpr int V = kLane<DT>, STEP = 4 * V, NG = kFewGroups, U = 4;
-    __shared__ Sums row_sums[4][16 * CH];
+    __shared__ Sums row_sums[4][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int col = lane & 15, quarter = lane >> 4;
     const int64_t j0 = (block_index() * 4 + wave) * (16 * NG);
@@ -360,11 +504,9 @@ __global__ __launch_bounds__(256) void k_head_few(HeadArgs A)
     const int steps = words ? (A.hidden + STEP - 1) / STEP : 0;
     const Pieces<DT, EVEN> w{at<DT>(A.w, (words ? j0 : 0) * A.hidden), (uint32_t)(words * A.hidden * kSize<DT>), A.hidden, words};
     const Pieces<DT, EVEN> x{static_cast<const uint8_t*>(A.h), (uint32_t)(A.rows * A.hidden * kSize<DT>), A.hidden, A.rows};
-    mm_f32x4 acc[CH][NG];
+    mm_f32x4 acc[NG];
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-        for (int n = 0; n < NG; ++n) acc[c][n] = mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int n = 0; n < NG; ++n) acc[n] = mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     raw16 even[NG][U], odd[NG][U];
     auto load = [&](int s, raw16 (&to)[NG][U]) {
 #pragma unroll
@@ -375,34 +517,27 @@ __global__ __launch_bounds__(256) void k_head_few(HeadArgs A)
     // loads arrive in their order: a step's rows are asked for before the next one's weights, which are then on their way while
     // this one is multiplied
     auto turn = [&](int s, const raw16 (&now)[NG][U], raw16 (&next)[NG][U]) {
+        raw16 xv[U];
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            if (16 * c >= A.rows) break;
-            raw16 xv[U];
+        for (int u = 0; u < U; ++u) xv[u] = x.load(col, (s + u) * STEP + quarter * V, s + u < steps);
+        __builtin_amdgcn_sched_barrier(0);
+        if (s + U < steps) load(s + U, next);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int u = 0; u < U; ++u) xv[u] = x.load(16 * c + col, (s + u) * STEP + quarter * V, s + u < steps);
-            if (c == 0) {
-                __builtin_amdgcn_sched_barrier(0);
-                if (s + U < steps) load(s + U, next);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+        for (int n = 0; n < NG; ++n) {
+            mm_f32x4 some = DT == DT_BF16 ? acc[n] : mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};   // FP32: short chains of sums
 #pragma unroll
-            for (int n = 0; n < NG; ++n) {
-                mm_f32x4 some = DT == DT_BF16 ? acc[c][n] : mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};   // FP32: short chains of sums
+            for (int u = 0; u < U; ++u) {
+                if constexpr (DT == DT_BF16) {
+                    some = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mm_bf16x8, now[n][u]), __builtin_bit_cast(mm_bf16x8, xv[u]), some, 0, 0, 0);
+                } else {
+                    const mm_f32x4 wf = __builtin_bit_cast(mm_f32x4, now[n][u]), xf = __builtin_bit_cast(mm_f32x4, xv[u]);
 #pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    if constexpr (DT == DT_BF16) {
-                        some = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mm_bf16x8, now[n][u]),
-                                                                       __builtin_bit_cast(mm_bf16x8, xv[u]), some, 0, 0, 0);
-                    } else {
-                        const mm_f32x4 wf = __builtin_bit_cast(mm_f32x4, now[n][u]), xf = __builtin_bit_cast(mm_f32x4, xv[u]);
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) some = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[q], xf[q], some, 0, 0, 0);
-                    }
+                    for (int q = 0; q < 4; ++q) some = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[q], xf[q], some, 0, 0, 0);
                 }
-                if constexpr (DT == DT_BF16) acc[c][n] = some;
-                else acc[c][n] += some;
             }
+            if constexpr (DT == DT_BF16) acc[n] = some;
+            else acc[n] += some;
         }
     };
     if (steps) load(0, even);
@@ -410,38 +545,33 @@ __global__ __launch_bounds__(256) void k_head_few(HeadArgs A)
         turn(s, even, odd);
         if (s + U < steps) turn(s + U, odd, even);
     }
+    const int64_t target = col < A.rows ? A.targets[col] - j0 : -1;
+    Sums all{kHeadNegInf, 0.0f};
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-        if (16 * c >= A.rows) break;
-        const int row = 16 * c + col;
-        const int64_t target = row < A.rows ? A.targets[row] - j0 : -1;
-        Sums all{kHeadNegInf, 0.0f};
+    for (int n = 0; n < NG; ++n)
 #pragma unroll
-        for (int n = 0; n < NG; ++n)
+        for (int r = 0; r < 4; ++r) {
+            const int word = 16 * n + 4 * quarter + r;
+            if (word >= words) acc[n][r] = kHeadNegInf;
+            else if (word == target) A.picked[col] = acc[n][r];
+            all.m = __builtin_fmaxf(all.m, acc[n][r]);
+        }
+    all.m = __builtin_fmaxf(all.m, __shfl_xor(all.m, 16));
+    all.m = __builtin_fmaxf(all.m, __shfl_xor(all.m, 32));
+    const float shift = shift_for(all.m);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int word = 16 * n + 4 * quarter + r;
-                if (word >= words) acc[c][n][r] = kHeadNegInf;
-                else if (word == target) A.picked[row] = acc[c][n][r];
-                all.m = __builtin_fmaxf(all.m, acc[c][n][r]);
-            }
-        all.m = __builtin_fmaxf(all.m, __shfl_xor(all.m, 16));
-        all.m = __builtin_fmaxf(all.m, __shfl_xor(all.m, 32));
-        const float shift = shift_for(all.m);
+    for (int n = 0; n < NG; ++n)
 #pragma unroll
-        for (int n = 0; n < NG; ++n)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) all.s += exp_of(acc[c][n][r], shift);
-        all.s += __shfl_xor(all.s, 16);
-        all.s += __shfl_xor(all.s, 32);
-        if (quarter == 0) row_sums[wave][row] = all;
-    }
+        for (int r = 0; r < 4; ++r) all.s += exp_of(acc[n][r], shift);
+    all.s += __shfl_xor(all.s, 16);
+    all.s += __shfl_xor(all.s, 32);
+    if (quarter == 0) row_sums[wave][col] = all;
     __syncthreads();
     if ((int)threadIdx.x < A.rows) {
-        Sums all = row_sums[0][threadIdx.x];
+        Sums sums = row_sums[0][threadIdx.x];
 #pragma unroll
-        for (int k = 1; k < 4; ++k) all = merged(all, row_sums[k][threadIdx.x]);
-        A.part[block_index() * A.rows + threadIdx.x] = all;
+        for (int k = 1; k < 4; ++k) sums = merged(sums, row_sums[k][threadIdx.x]);
+        A.part[block_index() * A.rows + threadIdx.x] = sums;
     }
 }
 
@@ -475,14 +605,8 @@ __global__ __launch_bounds__(kFinishLanes) void k_head_finish(const Sums* part, 
         __syncthreads();
     }
     if (slice || row >= rows) return;
-    all = tree[0][r];
-    if (all.m == kHeadNegInf) all.s = __builtin_nanf("");   // every logit -inf: no distribution
-    const int64_t t = index ? index[row] : row, target = targets[t];
-    if (stats) {
-        stats[2 * t] = all.m;
-        stats[2 * t + 1] = 1.0f / all.s;
-    }
-    losses[t] = target == ignore ? 0.0f : target < 0 || target >= vocab ? __builtin_nanf("") : logf(all.s) - (picked[row] - all.m);
+    const int64_t t = index ? index[row] : row;
+    finish_row(tree[0][r], picked[row], t, targets[t], vocab, ignore, losses, stats);
 }
 
 // ------------------------------------------------------------------------------ backward
@@ -543,31 +667,21 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_grad(HeadArgs A)
     }
 }
 
-// How many parts dh's sums are cut in: so that the tiles fill the CUs' places, of 16 steps or more.
-__device__ __host__ __forceinline__ int dh_splits(int64_t tiles, int places, int width)
-{
-    const int64_t fit = places / (tiles < 1 ? 1 : tiles), most = width / 512;
-    const int64_t n = fit < most ? fit : most;
-    return (int)(n < 1 ? 1 : n);
-}
-
 // dh (FP32) += G W of a piece.
 template <class H>
 __global__ __launch_bounds__(H::T, H::OCC) void k_head_dh(HeadArgs A)
 {
     __shared__ __attribute__((aligned(1024))) uint8_t lds[H::LDS];
     const int count = scalar(*A.count), tiles_i = (count + H::BM - 1) / H::BM;
-    const int splits = dh_splits((int64_t)tiles_i * A.tiles_j, A.places, A.pitch);   // by the pitch: the same for every piece
+    const int splits = splits_of((int64_t)tiles_i * A.tiles_j, A.places, A.pitch);   // by the pitch: the same for every piece
     HeadTile t;
     if (!head_tile(tiles_i, A.tiles_j, splits, t)) return;
     const int i0 = t.ti * H::BM, j0 = t.tj * H::BN, limit_i = count - i0, limit_j = A.hidden - j0;
-    const int steps = (A.width + H::BK - 1) / H::BK;
-    const int k0 = scalar(steps * t.split / splits * H::BK), k1 = scalar(steps * (t.split + 1) / splits * H::BK);
-    const int len = (k1 < A.width ? k1 : A.width) - k0;
-    if (len <= 0 && !A.fresh) return;
+    const HeadTerms k = terms_of<H>(A.width, t.split, splits);
+    if (k.len == 0 && !A.fresh) return;
     // G has zeros up to whole pieces, where W has ended
-    const Operand a{at<H::DT>(A.g, (int64_t)i0 * A.pitch + k0), A.pitch, 0, limit_i, (len + 7) & ~7};
-    const Operand b{at<H::DT>(A.w, (A.v0 + k0) * A.hidden), A.hidden, j0, A.hidden, len};
+    const Operand a{at<H::DT>(A.g, (int64_t)i0 * A.pitch + k.first), A.pitch, 0, limit_i, (k.len + 7) & ~7};
+    const Operand b{at<H::DT>(A.w, (A.v0 + k.first) * A.hidden), A.hidden, j0, A.hidden, k.len};
     typename H::Sum acc[H::NI][H::NJ];
     const int wi = H::wi(), wj = H::wj(), lane = threadIdx.x & 63;
     if (!head_multiply<H, true, false>(lds, a, b, wi < limit_i, acc)) return;
@@ -600,29 +714,42 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_dw(HeadArgs A)
     __shared__ __attribute__((aligned(1024))) uint8_t lds[H::LDS];
     const int count = scalar(*A.count);
     HeadTile t;
-    if (!head_tile((A.width + H::BM - 1) / H::BM, A.tiles_j, 1, t)) return;
+    if (!head_tile((A.width + H::BM - 1) / H::BM, A.tiles_j, A.splits, t)) return;
     const int i0 = t.ti * H::BM, j0 = t.tj * H::BN, limit_i = A.width - i0, limit_j = A.hidden - j0;
-    const Operand a{static_cast<const uint8_t*>(A.g), A.pitch, i0, A.pitch, count};
-    const Operand b{static_cast<const uint8_t*>(A.h), A.hidden, j0, A.hidden, count};
+    const HeadTerms k = terms_of<H>(count, t.split, A.splits);
+    const Operand a{at<H::DT>(A.g, (int64_t)k.first * A.pitch), A.pitch, i0, A.pitch, k.len};
+    const Operand b{at<H::DT>(A.h, (int64_t)k.first * A.hidden), A.hidden, j0, A.hidden, k.len};
     typename H::Sum acc[H::NI][H::NJ];
     const int wi = H::wi(), wj = H::wj(), lane = threadIdx.x & 63;
     if (!head_multiply<H, false, false>(lds, a, b, wi < limit_i, acc)) return;
+    if (A.splits > 1) {
+        store_sums<H>(A.parts + ((int64_t)t.split * A.width + i0) * A.hidden + j0, A.hidden, limit_i, limit_j, acc, wi, wj);
+        return;
+    }
     uint8_t* out = at<H::DT>(A.dw, (A.v0 + i0) * A.hidden + j0);
-    if constexpr (H::DT == DT_BF16) {
-        store_bf16<typename H::C, H::EVEN>(out, A.hidden, limit_i, limit_j, acc, wi, wj);
-    } else {
+    if constexpr (H::DT == DT_BF16) store_bf16<typename H::C, H::EVEN>(out, A.hidden, limit_i, limit_j, acc, wi, wj);
+    else store_sums<H>(reinterpret_cast<float*>(out), A.hidden, limit_i, limit_j, acc, wi, wj);
+}
+
+// A row of dW a workgroup: its parts, in order.
+template <int DT>
+__global__ __launch_bounds__(256) void k_head_join_dw(HeadArgs A)
+{
+    constexpr int L = kLane<DT>;
+    const int64_t v = block_index();
+    if (v >= A.width) return;
+    void* out = at<DT>(A.dw, (A.v0 + v) * A.hidden);
+    for (int32_t c = threadIdx.x * L; c < A.hidden; c += 256 * L) {
+        float x[L];
 #pragma unroll
-        for (int i = 0; i < H::NI; ++i) {
-            const int row = row_of<H>(wi, i);
-            if (row >= limit_i) continue;
+        for (int k = 0; k < L; ++k) x[k] = 0.0f;
+        for (int s = 0; s < A.splits; ++s) {
+            float y[L];
+            load_like<DT_F32, L>(A.parts + ((int64_t)s * A.width + v) * A.hidden, c, A.hidden, 0.0f, y);
 #pragma unroll
-            for (int j = 0; j < H::NJ; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float four[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                    store_like<DT_F32, 4>(reinterpret_cast<float*>(out) + (int64_t)row * A.hidden, column_of<H>(wj, j, 4 * q), limit_j, four);
-                }
+            for (int k = 0; k < L; ++k) x[k] += y[k];
         }
+        stream_vec<DT>(out, c, A.hidden, x);
     }
 }
 
@@ -635,7 +762,7 @@ __global__ __launch_bounds__(256) void k_head_scatter(const float* sums, const i
     const int64_t t = block_index();
     if (t >= rows) return;
     const int n = *count, p = place[t];
-    const int splits = dh_splits((int64_t)((n + tile_m - 1) / tile_m) * ((hidden + tile_n - 1) / tile_n), places, width);
+    const int splits = splits_of((int64_t)((n + tile_m - 1) / tile_m) * ((hidden + tile_n - 1) / tile_n), places, width);
     void* out = at<DT>(dh, t * hidden);
     for (int32_t c = threadIdx.x * L; c < hidden; c += 256 * L) {
         float x[L];
@@ -699,7 +826,7 @@ static Kind kind_of(int32_t dtype, int64_t m, int64_t n, int64_t terms, Product 
     if (dtype != ADAMBRIDGE_DT_BF16) return tiles_of(F32_128, m, n) < 512 ? F32_64 : F32_128;
     if (product == WEIGHTS && tiles_of(HALF, m, n) * 21 < tiles_of(LARGE, m, n) * 40) return HALF;   // 1.05 times the values
     if (product == SUMS && tiles_of(LARGE, m, n) <= kHeadCus / 2) return HALF;
-    if (product == ROWS) terms /= dh_splits(tiles_of(LARGE, m, n), places_of(LARGE), (int)terms);
+    if (product != SUMS) terms /= splits_of(tiles_of(LARGE, m, n), places_of(LARGE), terms);
     return terms >= 2048 ? WIDE : LARGE;
 }
 
@@ -707,23 +834,30 @@ static Kind kind_of(int32_t dtype, int64_t m, int64_t n, int64_t terms, Product 
 struct HeadForward {
     bool few;
     Kind kind;
-    int parts;
+    int parts, splits;
     int32_t *index, *count;
     HeadRow* facts;
-    float* picked;
+    float *picked, *logits;
     Sums* part;
     void* h;
     int64_t bytes;
     HeadForward(void* work, int32_t dtype, int64_t rows, int64_t vocab, int64_t hidden)
     {
-        // rows that stream the weights, or go on tiles (us, 151936 x 896 and 32000 x 4096: BF16, 32 rows 72 and 75 streamed; 65 on
-        // tiles 72 and 76; FP32, 64 streamed 256 and 294, 65 on tiles 329 and 355)
-        few = rows <= (dtype == ADAMBRIDGE_DT_BF16 ? 16 : 64);
+        // Rows that stream the weights, or go on tiles: a wavefront streams its words' whole rows, which takes as long as they are
+        // unless there are words enough for all CUs.  (us, streamed / tiles, 16 rows, BF16 and FP32: 8000 words of 512 values
+        // 11 / 18 and 17 / 21, of 2048 27 / 20 and 49 / 35, 16000 of 2048 27 / 27 and 49 / 55, 38000 of 2048 49 / 54 and 100 / 132,
+        // 8000 of 8192 89 / 39 and 173 / 96.  32 rows of 151936 x 896 BF16 72 streamed, 69 on tiles.)
+        few = rows <= 16 && (hidden <= 1024 || vocab >= 16000);
         kind = kind_of(dtype, rows, vocab, hidden, SUMS);
         parts = (int)(few ? (vocab + 64 * kFewGroups - 1) / (64 * kFewGroups) : (vocab + tile_n(kind) - 1) / tile_n(kind));
+        // parts of the terms only where they are three or more (us, whole / two parts: 200 rows of 32000 x 4096 92 / 97; three or more:
+        // 121 rows of 10197 x 4608 78 / 49)
+        splits = splits_of(tiles_of(kind, rows, vocab), places_of(kind), hidden);
+        if (few || tiles_of(kind, rows, vocab) * 3 > places_of(kind)) splits = 1;
         Scratch s{static_cast<uint8_t*>(work)};
         picked = s.take<float>(rows);
-        part = s.take<Sums>(parts * rows);
+        part = s.take<Sums>(splits > 1 ? 0 : parts * rows);
+        logits = s.take<float>(splits > 1 ? splits * rows * up(vocab, 4) : 0);
         index = few ? nullptr : s.take<int32_t>(rows);
         facts = few ? nullptr : s.take<HeadRow>(rows);
         count = few ? nullptr : s.take<int32_t>(1);
@@ -736,10 +870,11 @@ struct HeadForward {
 struct HeadBackward {
     Kind grad, dw, dh_kind;
     int32_t pitch;   // words of a piece
+    int grad_splits, dw_splits;
     int32_t *index, *place, *count;
     HeadRow* facts;
     void *h, *g;
-    float* dh;
+    float *dh, *parts;
     int64_t bytes;
     HeadBackward(void* work, int32_t dtype, int64_t rows, int64_t vocab, int64_t hidden)
     {
@@ -759,6 +894,9 @@ struct HeadBackward {
         g = s.take<uint8_t>(rows * pitch * size);
         // parts x rows x hidden: as many as fill the CUs with tiles, or one
         dh = s.take<float>(std::max(rows * hidden, (int64_t)places_of(dh_kind) * tile_m(dh_kind) * tile_n(dh_kind)));
+        grad_splits = splits_of(tiles_of(grad, rows, width), places_of(grad), hidden);
+        dw_splits = splits_of(tiles_of(dw, width, hidden), places_of(dw), rows);
+        parts = s.take<float>(std::max(grad_splits > 1 ? grad_splits * rows * pitch : 0, dw_splits > 1 ? dw_splits * width * hidden : 0));
         bytes = s.used;
     }
 };
@@ -778,6 +916,13 @@ static dim3 tile_grid(int64_t tiles) { return block_grid(up(tiles, kXcd)); }
         else if ((KIND) == F32_128) hipLaunchKernelGGL((KERNEL<HeadF32<128>>), GRID, dim3(256), 0, t_stream, A);   \
         else hipLaunchKernelGGL((KERNEL<HeadF32<64>>), GRID, dim3(256), 0, t_stream, A);                           \
     } while (0)
+
+// Split logits' tiles are the smaller ones: the larger are taken where there are enough.
+static void launch_logits(const HeadArgs& A, bool bf, bool even, dim3 grid)
+{
+    if (bf) ABH_HEAD_BF16(k_head_logits, HalfTile, even, grid);
+    else hipLaunchKernelGGL((k_head_logits<HeadF32<64>>), grid, dim3(256), 0, t_stream, A);
+}
 
 // The scored rows: their numbers, how many, and copies of them.  One launch for a few thousand rows, whose counts grow with the
 // square of them, else two (us, one / two: the forward call of 100 rows of 151936 x 896 71.1 / 73.5; the kernels alone at 4096 rows
@@ -833,12 +978,10 @@ ADAMBRIDGE_API int adambridge_token_losses(const void* hidden, const void* weigh
         const int64_t bytes = size * (bf ? 2 : 4);
         const bool even = bytes % 16 == 0 && ((uintptr_t)hidden | (uintptr_t)weight) % 16 == 0;
         const dim3 grid = block_grid(p.parts), block(256);
-        if (bf && even) hipLaunchKernelGGL((k_head_few<DT_BF16, true, 1>), grid, block, 0, t_stream, A);
-        else if (bf) hipLaunchKernelGGL((k_head_few<DT_BF16, false, 1>), grid, block, 0, t_stream, A);
-        else if (even && rows <= 16) hipLaunchKernelGGL((k_head_few<DT_F32, true, 1>), grid, block, 0, t_stream, A);
-        else if (even) hipLaunchKernelGGL((k_head_few<DT_F32, true, 4>), grid, block, 0, t_stream, A);
-        else if (rows <= 16) hipLaunchKernelGGL((k_head_few<DT_F32, false, 1>), grid, block, 0, t_stream, A);
-        else hipLaunchKernelGGL((k_head_few<DT_F32, false, 4>), grid, block, 0, t_stream, A);
+        if (bf && even) hipLaunchKernelGGL((k_head_few<DT_BF16, true>), grid, block, 0, t_stream, A);
+        else if (bf) hipLaunchKernelGGL((k_head_few<DT_BF16, false>), grid, block, 0, t_stream, A);
+        else if (even) hipLaunchKernelGGL((k_head_few<DT_F32, true>), grid, block, 0, t_stream, A);
+        else hipLaunchKernelGGL((k_head_few<DT_F32, false>), grid, block, 0, t_stream, A);
         hipLaunchKernelGGL((k_head_finish<4>), dim3((unsigned)((rows + 3) / 4)), dim3(kFinishLanes), 0, t_stream, p.part, p.parts, A.rows, nullptr,
                            nullptr, targets, vocab, ignore_index, p.picked, losses, stats);
     } else {
@@ -849,9 +992,19 @@ ADAMBRIDGE_API int adambridge_token_losses(const void* hidden, const void* weigh
         A.width = (int32_t)vocab;
         A.tiles_j = p.parts;
         const bool even = size % 8 == 0 && (uintptr_t)weight % 16 == 0;
-        ABH_HEAD_LAUNCH(k_head_sums, p.kind, even, tile_grid(tiles_of(p.kind, rows, vocab)));
-        hipLaunchKernelGGL((k_head_finish<16>), block_grid((rows + 15) / 16), dim3(kFinishLanes), 0, t_stream, p.part, p.parts, A.rows, p.index,
-                           p.count, targets, vocab, ignore_index, p.picked, losses, stats);
+        if (p.splits > 1) {
+            A.pitch = (int32_t)up(vocab, 4);
+            A.splits = p.splits;
+            A.parts = p.logits;
+            launch_logits(A, bf, even, tile_grid(tiles_of(p.kind, rows, vocab) * p.splits));
+            // a wavefront a row, or a workgroup (8270 rows of 59 words: 1024 lanes 80 us)
+            if (vocab <= 1024) hipLaunchKernelGGL((k_head_join<64>), block_grid((rows + 3) / 4), dim3(256), 0, t_stream, A, p.index, targets, ignore_index, losses, stats);
+            else hipLaunchKernelGGL((k_head_join<1024>), block_grid(rows), dim3(1024), 0, t_stream, A, p.index, targets, ignore_index, losses, stats);
+        } else {
+            ABH_HEAD_LAUNCH(k_head_sums, p.kind, even, tile_grid(tiles_of(p.kind, rows, vocab)));
+            hipLaunchKernelGGL((k_head_finish<16>), block_grid((rows + 15) / 16), dim3(kFinishLanes), 0, t_stream, p.part, p.parts, A.rows, p.index,
+                               p.count, targets, vocab, ignore_index, p.picked, losses, stats);
+        }
     }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess ? 0 : hip_fail(e, "hipLaunchKernelGGL (token losses)");
@@ -888,15 +1041,27 @@ ADAMBRIDGE_API int adambridge_token_losses_backward(const float* gout, const voi
     A.dh = p.dh;
     A.dw = dweight;
     A.fresh = 1;
+    A.parts = p.parts;
     const bool even = size % 8 == 0 && ((uintptr_t)weight | (uintptr_t)dweight) % 16 == 0;
     for (int64_t v0 = 0; v0 < vocab; v0 += p.pitch) {
         A.v0 = v0;
         A.width = (int32_t)std::min<int64_t>(p.pitch, vocab - v0);
         A.tiles_j = (A.width + tile_n(p.grad) - 1) / tile_n(p.grad);
-        ABH_HEAD_LAUNCH(k_head_grad, p.grad, even, tile_grid(tiles_of(p.grad, rows, A.width)));
+        A.splits = p.grad_splits;
+        if (p.grad_splits > 1) {
+            launch_logits(A, bf, even, tile_grid(tiles_of(p.grad, rows, A.width) * p.grad_splits));
+            const int32_t columns = (A.width + 1023) / 1024;
+            if (bf) hipLaunchKernelGGL((k_head_join_grad<DT_BF16>), block_grid(rows * columns), dim3(256), 0, t_stream, A, columns);
+            else hipLaunchKernelGGL((k_head_join_grad<DT_F32>), block_grid(rows * columns), dim3(256), 0, t_stream, A, columns);
+        } else {
+            ABH_HEAD_LAUNCH(k_head_grad, p.grad, even, tile_grid(tiles_of(p.grad, rows, A.width)));
+        }
         if (dweight) {
             A.tiles_j = (int32_t)((size + tile_n(p.dw) - 1) / tile_n(p.dw));
-            ABH_HEAD_LAUNCH(k_head_dw, p.dw, even, tile_grid(tiles_of(p.dw, A.width, size)));
+            A.splits = p.dw_splits;
+            ABH_HEAD_LAUNCH(k_head_dw, p.dw, even, tile_grid(tiles_of(p.dw, A.width, size) * p.dw_splits));
+            if (p.dw_splits > 1 && bf) hipLaunchKernelGGL((k_head_join_dw<DT_BF16>), block_grid(A.width), dim3(256), 0, t_stream, A);
+            else if (p.dw_splits > 1) hipLaunchKernelGGL((k_head_join_dw<DT_F32>), block_grid(A.width), dim3(256), 0, t_stream, A);
         }
         if (dhidden) {
             A.tiles_j = (int32_t)((size + tile_n(p.dh_kind) - 1) / tile_n(p.dh_kind));
