@@ -29,6 +29,7 @@ namespace abh {
 
 constexpr int kRun = 4096, kSortThreads = 1024;
 constexpr int kMostWords = 8;     // of a wavefront; fewer than its lanes.  (65536 tokens, 32000 x 4096: 8 words 108 us, 16 112, 4 105)
+constexpr int kFewIds = 256;      // tokens whose ids every wavefront reads for itself
 constexpr int kLeastChunk = 32;   // tokens.  (the words' rows and the parts: 146 us with 32, 149 with 64)
 
 __device__ __forceinline__ int64_t id_at(const void* ids, int32_t id_bytes, int64_t i)
@@ -166,13 +167,14 @@ __global__ __launch_bounds__(256) void k_embed_merge(const uint64_t* in, int64_t
 // ------------------------------------------------------------------------------- the gradient
 
 struct EmbedBackArgs {
+    const void* ids;
     const uint64_t* sorted;
     const void* gout;
     void* dweight;
     float* part;          // chunks x 2 x hidden
     int32_t* starts;      // vocab + 1
     int64_t tokens, vocab, padding, part_blocks;
-    int32_t hidden, chunk, part_columns, words, pieces;   // words, pieces: of a wavefront of k_embed_rows, of a row
+    int32_t id_bytes, hidden, chunk, part_columns, words, pieces;   // words, pieces: of a wavefront of k_embed_rows, of a row
     float scale;
 };
 
@@ -355,6 +357,56 @@ __global__ __launch_bounds__(256) void k_embed_rows(EmbedBackArgs A)
     }
 }
 
+// The same of a few tokens in one launch: a wavefront has all ids, four a lane, and a word's tokens are the bits of four ballots, in
+// order.  (us of a forward and backward pass, 256 tokens so / 257 sorted: 5003 words of 897 BF16 values 47 / 51, 32000 of 4096 53 / 60;
+// one word's 256 rows of 4096, which are then one wavefront's, 63 / 60.)
+template <int DT, bool SHORT>
+__global__ __launch_bounds__(256) void k_embed_few(EmbedBackArgs A)
+{
+    constexpr int L = kLane<DT>, AHEAD = 8, B = kFewIds / kWave;
+    const int lane = threadIdx.x & 63;
+    const int64_t item = block_index() * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+    const int64_t group = item / A.pieces, v0 = group * A.words;
+    if (v0 >= A.vocab) return;
+    const int words = (int)(A.vocab - v0 < A.words ? A.vocab - v0 : A.words), tokens = (int)A.tokens;
+    const Columns<DT, SHORT> columns((int32_t)(item - group * A.pieces) * (64 * L) + lane * L, A.hidden);
+    int64_t id[B];
+#pragma unroll
+    for (int b = 0; b < B; ++b) {
+        const int i = b * kWave + lane;
+        id[b] = id_at(A.ids, A.id_bytes, i < tokens ? i : tokens - 1);
+        if (i >= tokens) id[b] = -1;
+    }
+    for (int w = 0; w < words; ++w) {
+        float acc[L];
+#pragma unroll
+        for (int k = 0; k < L; ++k) acc[k] = 0.0f;
+        if (v0 + w != A.padding) {
+#pragma unroll
+            for (int b = 0; b < B; ++b) {
+                uint64_t mine = __builtin_amdgcn_ballot_w64(id[b] == v0 + w);
+                while (mine) {
+                    raw16 row[AHEAD];
+                    int n = 0, from = 0;
+#pragma unroll
+                    for (int a = 0; a < AHEAD; ++a) {   // past the last one: it again, not added
+                        from = mine ? b * kWave + __builtin_ctzll(mine) : from;
+                        n += mine != 0;
+                        mine &= mine - 1;
+                        row[a] = columns.load(at<DT>(A.gout, (int64_t)from * A.hidden), A.hidden);
+                    }
+#pragma unroll
+                    for (int a = 0; a < AHEAD; ++a)
+                        if (a < n) columns.add(row[a], acc);
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < L; ++k) acc[k] *= A.scale;
+        columns.stream(at<DT>(A.dweight, (v0 + w) * A.hidden), A.hidden, acc);
+    }
+}
+
 // ------------------------------------------------------------------------------- launches
 
 constexpr int64_t kEmbedTokens = (int64_t)1 << 30, kEmbedVocab = (int64_t)1 << 30, kEmbedHidden = (int64_t)1 << 22;
@@ -398,18 +450,22 @@ template <int DT>
 static void launch_embed_back(EmbedBackArgs& A)
 {
     const int vectors = (A.hidden + kLane<DT> - 1) / kLane<DT>;
-    A.part_columns = (vectors + 255) / 256;
-    A.part_blocks = A.tokens >= A.chunk ? (A.tokens + A.chunk - 1) / A.chunk * A.part_columns : 0;
-    const bool tiny = A.hidden < kLane<DT>;
-    const dim3 parts = block_grid(A.part_blocks + (A.vocab + 256) / 256);
-    if (tiny) hipLaunchKernelGGL((k_embed_parts<DT, true>), parts, dim3(256), 0, t_stream, A);
-    else hipLaunchKernelGGL((k_embed_parts<DT, false>), parts, dim3(256), 0, t_stream, A);
+    const bool few = A.tokens <= kFewIds, tiny = A.hidden < kLane<DT>;
+    if (!few) {
+        A.part_columns = (vectors + 255) / 256;
+        A.part_blocks = A.tokens >= A.chunk ? (A.tokens + A.chunk - 1) / A.chunk * A.part_columns : 0;
+        const dim3 parts = block_grid(A.part_blocks + (A.vocab + 256) / 256);
+        if (tiny) hipLaunchKernelGGL((k_embed_parts<DT, true>), parts, dim3(256), 0, t_stream, A);
+        else hipLaunchKernelGGL((k_embed_parts<DT, false>), parts, dim3(256), 0, t_stream, A);
+    }
     A.pieces = (vectors + 63) / 64;
     // fewer words a wavefront where there would be too few wavefronts (5003 words of 897 FP32 values: 2 words 7 us, 16 19)
     A.words = kMostWords;
     while (A.words > 2 && (A.vocab + A.words - 1) / A.words * A.pieces < 4096) A.words /= 2;
     const dim3 grid = block_grid(((A.vocab + A.words - 1) / A.words * A.pieces + 3) / 4);
-    if (tiny) hipLaunchKernelGGL((k_embed_rows<DT, true>), grid, dim3(256), 0, t_stream, A);
+    if (few && tiny) hipLaunchKernelGGL((k_embed_few<DT, true>), grid, dim3(256), 0, t_stream, A);
+    else if (few) hipLaunchKernelGGL((k_embed_few<DT, false>), grid, dim3(256), 0, t_stream, A);
+    else if (tiny) hipLaunchKernelGGL((k_embed_rows<DT, true>), grid, dim3(256), 0, t_stream, A);
     else hipLaunchKernelGGL((k_embed_rows<DT, false>), grid, dim3(256), 0, t_stream, A);
 }
 
@@ -447,9 +503,9 @@ ADAMBRIDGE_API int adambridge_embed_backward(const void* ids, int32_t id_bytes, 
     if ((uintptr_t)work % 8) return ADAMBRIDGE_EALIGN;
     uint64_t* sorted = static_cast<uint64_t*>(work);
     uint64_t* other = tokens > kRun ? sorted + tokens : nullptr;
-    // few tokens over many CUs; many read their run's ids a quarter as often
-    if (tokens <= 4 * kRun) hipLaunchKernelGGL((k_embed_sort<16>), block_grid((tokens + 15) / 16), dim3(kSortThreads), 0, t_stream, ids, id_bytes, tokens, vocab, sorted);
-    else hipLaunchKernelGGL((k_embed_sort<64>), block_grid((tokens + 63) / 64), dim3(kSortThreads), 0, t_stream, ids, id_bytes, tokens, vocab, sorted);
+    // no order of a few; a few thousand over many CUs; many read their run's ids a quarter as often
+    if (tokens > kFewIds && tokens <= 4 * kRun) hipLaunchKernelGGL((k_embed_sort<16>), block_grid((tokens + 15) / 16), dim3(kSortThreads), 0, t_stream, ids, id_bytes, tokens, vocab, sorted);
+    else if (tokens > kFewIds) hipLaunchKernelGGL((k_embed_sort<64>), block_grid((tokens + 63) / 64), dim3(kSortThreads), 0, t_stream, ids, id_bytes, tokens, vocab, sorted);
     float* const part = reinterpret_cast<float*>(sorted + (tokens > kRun ? 2 : 1) * tokens);
     for (int64_t run = kRun; run < tokens;) {
         const dim3 grid = block_grid((tokens + 255) / 256);
@@ -462,6 +518,8 @@ ADAMBRIDGE_API int adambridge_embed_backward(const void* ids, int32_t id_bytes, 
         std::swap(sorted, other);
     }
     EmbedBackArgs A{};
+    A.ids = ids;
+    A.id_bytes = id_bytes;
     A.sorted = sorted;
     A.gout = gout;
     A.dweight = dweight;

@@ -85,3 +85,14 @@ def test_no_tokens():
         y = ab.embed(torch.empty(shape, dtype=torch.int64, device="cuda"), weight)
         assert y.shape == (*shape, 20)
         assert not torch.autograd.grad(y.sum(), weight)[0].any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("kind", ["words", "same", "outside"])
+@pytest.mark.parametrize("tokens,vocab,hidden", [(255, 3, 136), (256, 700, 136), (257, 700, 136), (256, 1, 2), (200, 40000, 9)])
+def test_about_the_fewest_tokens(tokens, vocab, hidden, kind, dtype):
+    """Tokens that are not sorted, and the first that are."""
+    gen = torch.Generator("cuda").manual_seed(tokens + vocab)
+    ids = _ids(kind, tokens, vocab, gen)
+    _check(ids, vocab, hidden, dtype, 1.0, None, gen)
+    _check(ids.int(), vocab, hidden, dtype, 1.7, vocab - 1, gen)

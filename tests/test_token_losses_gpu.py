@@ -166,3 +166,40 @@ def test_shapes_types_and_orders():
     assert torch.allclose(ab.token_losses(*tiny), torch.nn.functional.cross_entropy(tiny[0] @ tiny[1].t(), tiny[2], reduction="none"))
     with torch.autocast("cuda", dtype=BF16):
         assert torch.equal(ab.token_losses(h.float(), w.float(), t), want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("rows,vocab,size,ignored", [
+    (51, 74, 7540, 0.2), (1, 20, 8203, 0.0), (16, 1100, 2056, 0.2), (21, 1247, 2051, 0.2), (64, 37, 1030, 0.0), (1029, 342, 2053, 0.5),
+    (3001, 185, 130, 0.2), (5000, 259, 1024, 0.9), (2049, 3, 1544, 0.97), (130, 5000, 1536, 0.2)])
+def test_sums_of_few_tiles(rows, vocab, size, ignored, dtype):
+    """Few tiles of long sums: the logits', dW's and dh's are cut along their terms, which may be fewer than the parts."""
+    gen = torch.Generator("cuda").manual_seed(rows + vocab + size)
+    _check(*_inputs(rows, vocab, size, dtype, gen, ignored))
+
+
+@pytest.mark.parametrize("rows,vocab,size", [(2300, 4099, 2056), (4203, 4197, 2552), (4096, 4352, 2304)])
+def test_sums_of_many_tiles(rows, vocab, size):
+    """Many tiles of long sums, whose last step may be a part of one."""
+    gen = torch.Generator("cuda").manual_seed(rows + vocab + size)
+    _check(*_inputs(rows, vocab, size, BF16, gen))
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+def test_targets_and_logits_of_few_tiles(dtype):
+    """Infinities, NaN and targets outside the vocabulary where the logits come in parts, as where they do not."""
+    gen = torch.Generator("cuda").manual_seed(5)
+    h, w, t, gout = _inputs(40, 70, 2048, dtype, gen, 0.0)
+    t[0], t[1] = 70, -3
+    h[2] = torch.nan
+    w[:, 0] = 1.0
+    h[3], h[4] = 0.0, 0.0
+    h[3, 0], h[4, 0] = torch.inf, -torch.inf   # every logit inf, and -inf
+    h, w = h.requires_grad_(), w.requires_grad_()
+    loss = ab.token_losses(h, w, t)
+    dh, dw = torch.autograd.grad(loss, (h, w), gout)
+    assert loss[:5].isnan().all() and dh[:5].isnan().all() and dw.isnan().all()
+    rest = slice(5, None)
+    want, bound, dh_want, dh_bound, _, _ = _definition(h.detach()[rest], w.detach(), t[rest], gout[rest], -100)
+    assert ((loss.detach()[rest].double() - want).abs() <= bound).all()
+    assert ((dh[rest].double() - dh_want).abs() <= dh_bound).all()
