@@ -910,13 +910,17 @@ static dim3 tile_grid(int64_t tiles) { return block_grid(up(tiles, kXcd)); }
         if (EVEN) hipLaunchKernelGGL((KERNEL<HeadBf16<TILE, true>>), GRID, dim3(TILE::T), 0, t_stream, A);         \
         else hipLaunchKernelGGL((KERNEL<HeadBf16<TILE, false>>), GRID, dim3(TILE::T), 0, t_stream, A);             \
     } while (0)
-#define ABH_HEAD_LAUNCH(KERNEL, KIND, EVEN, GRID)                                                                  \
+#define ABH_HEAD_WHOLE(KERNEL, KIND, EVEN, GRID)   /* (dh's tiles are never halves) */                              \
     do {                                                                                                           \
         if ((KIND) == WIDE && (EVEN)) hipLaunchKernelGGL((KERNEL<HeadBf16<WideTile, true>>), GRID, dim3(WideTile::T), 0, t_stream, A); \
         else if ((KIND) == WIDE || (KIND) == LARGE) ABH_HEAD_BF16(KERNEL, LargeTile, EVEN, GRID);                  \
-        else if ((KIND) == HALF) ABH_HEAD_BF16(KERNEL, HalfTile, EVEN, GRID);                                      \
         else if ((KIND) == F32_128) hipLaunchKernelGGL((KERNEL<HeadF32<128>>), GRID, dim3(256), 0, t_stream, A);   \
         else hipLaunchKernelGGL((KERNEL<HeadF32<64>>), GRID, dim3(256), 0, t_stream, A);                           \
+    } while (0)
+#define ABH_HEAD_LAUNCH(KERNEL, KIND, EVEN, GRID)                                                                  \
+    do {                                                                                                           \
+        if ((KIND) == HALF) ABH_HEAD_BF16(KERNEL, HalfTile, EVEN, GRID);                                           \
+        else ABH_HEAD_WHOLE(KERNEL, KIND, EVEN, GRID);                                                             \
     } while (0)
 
 // Split logits' tiles are the smaller ones: the larger are taken where there are enough.
@@ -1068,7 +1072,7 @@ ADAMBRIDGE_API int adambridge_token_losses_backward(const float* gout, const voi
         if (dhidden) {
             A.tiles_j = (int32_t)((size + tile_n(p.dh_kind) - 1) / tile_n(p.dh_kind));
             A.places = places_of(p.dh_kind);
-            ABH_HEAD_LAUNCH(k_head_dh, p.dh_kind, even, tile_grid(std::max<int64_t>(tiles_of(p.dh_kind, rows, size), A.places)));
+            ABH_HEAD_WHOLE(k_head_dh, p.dh_kind, even, tile_grid(std::max<int64_t>(tiles_of(p.dh_kind, rows, size), A.places)));
         }
         A.fresh = 0;
     }

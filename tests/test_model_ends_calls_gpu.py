@@ -387,3 +387,36 @@ def test_a_decoding_step_is_the_whole_sequence_s_last_row():
     whole = _losses(p, ids, ids.roll(-1, 1))
     for t in range(12):
         assert torch.allclose(_losses(p, ids[:, t], ids.roll(-1, 1)[:, t]), whole[:, t], rtol=1e-4, atol=1e-4)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab,size", [(51, 74, 2056), (700, 300, 1030), (16, 500, 1544), (1100, 4099, 2056)])
+def test_sums_in_parts_captured_in_a_graph(rows, vocab, size, dtype):
+    """Few tiles, whose sums are cut and joined: replayed with other targets, after scratch of NaN, as the eager calls."""
+    gen = _gen(rows)
+    h = torch.randn(rows, size, generator=gen, device="cuda").to(dtype).requires_grad_()
+    w = (torch.randn(vocab, size, generator=gen, device="cuda") * size ** -0.5).to(dtype).requires_grad_()
+    t = torch.randint(0, vocab, (rows,), generator=gen, device="cuda")
+    seed = torch.rand(rows, generator=gen, device="cuda")
+
+    def once():
+        y = ab.token_losses(h, w, t)
+        table = ab.embed(t[:200], w)
+        return (y.detach(), *torch.autograd.grad(y, (h, w), seed), *torch.autograd.grad(table, w, h[:200].detach()))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        once()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = once()
+    for i in range(4):
+        t.copy_(torch.where(torch.rand(rows, generator=gen, device="cuda") < 0.3 * i, -100, torch.randint(0, vocab, (rows,), generator=gen, device="cuda")))
+        graph.replay()
+        torch.cuda.synchronize()
+        torch.full((1 << 26,), torch.nan, device="cuda")
+        eager = once()
+        assert all(torch.equal(a, b) for a, b in zip(captured, eager)), i
+        assert not any(x.isnan().any() for x in eager)
