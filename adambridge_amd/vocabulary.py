@@ -92,7 +92,9 @@ def _torch_token_losses(hidden, weight, targets, ignore_index):
     rows, scored, inside, at = _scored(hidden, targets, weight.shape[0], ignore_index)
     logits = rows @ weight.to(rows.dtype).t()
     loss = torch.logsumexp(logits, 1) - torch.gather(logits, 1, at[:, None].long())[:, 0]
-    return torch.where(scored, torch.where(inside, loss, torch.nan), 0.0).reshape(targets.shape)
+    # a factor, so that a target outside the vocabulary makes its row's gradients NaN too
+    loss = loss * torch.where(inside | ~scored, 1.0, torch.nan).to(loss.dtype)
+    return torch.where(scored, loss, 0.0).reshape(targets.shape)
 
 
 def _token_losses_backward(gout, hidden, weight, targets, ignore_index, want_hidden, want_weight):

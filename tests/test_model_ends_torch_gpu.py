@@ -1,0 +1,29 @@
+"""embed and token_losses where GPU tensors take torch operations: types, sizes and transforms that the kernels do not take, beside
+the kernels' own values."""
+
+import pytest
+import torch
+
+import adambridge_amd as ab
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 40), (torch.float32, 3), (torch.float32, 40), (torch.bfloat16, 7), (torch.float64, 9)])
+def test_a_target_outside_the_vocabulary_has_gradients_of_nan(dtype, size, rows):
+    """By the kernels (rows of 40 FP32 values) and by torch operations (the others) alike."""
+    gen = torch.Generator("cuda").manual_seed(size)
+    h, w = (torch.randn(*s, generator=gen, device="cuda").to(dtype).requires_grad_() for s in ((rows, size), (10, size)))
+    t = torch.randint(0, 10, (rows,), generator=gen, device="cuda")
+    t[1], t[2], t[3] = 99, -100, -1
+    loss = ab.token_losses(h, w, t)
+    dh, dw = torch.autograd.grad(loss.sum(), (h, w))
+    bad = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    bad[[1, 3]] = True
+    assert torch.equal(loss.isnan(), bad) and loss[2] == 0
+    assert torch.equal(dh.isnan().all(1), bad) and torch.equal(dh.isnan().any(1), bad) and not dh[2].any() and dw.isnan().all()
+    if dtype == torch.float32:
+        got = torch.func.grad(lambda a, b: ab.token_losses(a, b, t).sum(), argnums=(0, 1))(h.detach(), w.detach())
+        assert torch.equal(got[0].isnan(), dh.isnan()) and got[1].isnan().all()
+        assert torch.allclose(got[0][~bad], dh[~bad], rtol=1e-4, atol=1e-5)

@@ -1,0 +1,31 @@
+"""embed, token_losses and expert_mlp in torch operations: values, gradients and refusals where they differ from the kernels' most easily."""
+
+import pytest
+import torch
+
+import adambridge_amd as ab
+from adambridge_amd.vocabulary import BACKWARD
+
+
+def _same(got, want):
+    """NaN at the same places, the others alike (FP32 sums of a few terms, in another order)."""
+    return torch.equal(got.isnan(), want.isnan()) and torch.allclose(got.nan_to_num(), want.nan_to_num(), rtol=1e-5, atol=1e-6)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64, torch.float16, torch.bfloat16])
+def test_a_target_outside_the_vocabulary_has_gradients_of_nan(dtype):
+    gen = torch.Generator().manual_seed(0)
+    h, w = (torch.randn(*s, generator=gen).to(dtype).requires_grad_() for s in ((5, 6), (10, 6)))
+    t, g = torch.tensor([1, 99, -100, -1, 4]), torch.rand(5, generator=gen)
+    loss = ab.token_losses(h, w, t)
+    dh, dw = torch.autograd.grad(loss, (h, w), g.to(loss.dtype))
+    bad = torch.tensor([False, True, False, True, False])
+    assert torch.equal(loss.isnan(), bad) and loss[2] == 0
+    assert torch.equal(dh.isnan().all(1), bad) and torch.equal(dh.isnan().any(1), bad) and not dh[2].any() and dw.isnan().all()
+    alone = torch.autograd.grad(ab.token_losses(h, w, torch.where(bad, -100, t)), h, g.to(loss.dtype))[0]
+    assert torch.equal(dh[~bad], alone[~bad])
+    if dtype == torch.float32:
+        want = BACKWARD["token_losses"](g, h.detach(), w.detach(), t, -100, True, True)
+        assert _same(dh, want[0]) and _same(dw, want[1])
+        got = torch.func.grad(lambda a, b: (ab.token_losses(a, b, t) * g).sum(), argnums=(0, 1))(h.detach(), w.detach())
+        assert _same(got[0], dh) and _same(got[1], dw)
