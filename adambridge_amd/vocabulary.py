@@ -91,7 +91,7 @@ def _torch_token_losses(hidden, weight, targets, ignore_index):
     """The definition in torch operations, which hold all logits."""
     rows, scored, inside, at = _scored(hidden, targets, weight.shape[0], ignore_index)
     logits = rows @ weight.to(rows.dtype).t()
-    loss = torch.logsumexp(logits, 1) - torch.gather(logits, 1, at[:, None].long())[:, 0]
+    loss = -torch.gather(logits.log_softmax(1), 1, at[:, None].long())[:, 0]   # NaN where a logit is inf, as the kernels'
     # a factor, so that a target outside the vocabulary makes its row's gradients NaN too
     loss = loss * torch.where(inside | ~scored, 1.0, torch.nan).to(loss.dtype)
     return torch.where(scored, loss, 0.0).reshape(targets.shape)

@@ -29,3 +29,21 @@ def test_a_target_outside_the_vocabulary_has_gradients_of_nan(dtype):
         assert _same(dh, want[0]) and _same(dw, want[1])
         got = torch.func.grad(lambda a, b: (ab.token_losses(a, b, t) * g).sum(), argnums=(0, 1))(h.detach(), w.detach())
         assert _same(got[0], dh) and _same(got[1], dw)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_a_logit_of_inf_leaves_no_distribution(dtype):
+    """Losses and gradients of NaN, whether or not it is the target's; a word that no row can reach (-inf) leaves the others' losses."""
+    h, w = torch.ones(4, 6, dtype=dtype), torch.randn(10, 6, generator=torch.Generator().manual_seed(1)).to(dtype)
+    t = torch.tensor([1, 3, 2, -100])
+    w[3, 0] = torch.inf
+    h, w = h.requires_grad_(), w.requires_grad_()
+    loss = ab.token_losses(h, w, t)
+    assert torch.equal(loss.isnan(), t != -100)
+    assert torch.equal(torch.autograd.grad(loss.sum(), h)[0].isnan().any(1), t != -100)
+    with torch.no_grad():
+        w[3, 0] = -torch.inf
+    loss = ab.token_losses(h, w, t)
+    want = ab.token_losses(h[0], torch.cat((w[:3], w[4:])), torch.tensor(1))
+    assert torch.allclose(loss[0], want) and loss[1] == torch.inf and loss[3] == 0
+    assert ab.token_losses(h, torch.full_like(w, -torch.inf), t)[:3].isnan().all()
