@@ -90,7 +90,7 @@ def _scored(hidden, targets, vocab, ignore_index):
 def _torch_token_losses(hidden, weight, targets, ignore_index):
     """The definition in torch operations, which hold all logits."""
     rows, scored, inside, at = _scored(hidden, targets, weight.shape[0], ignore_index)
-    logits = rows @ weight.to(rows.dtype).t()
+    logits = torch.where(scored[:, None], rows @ weight.to(rows.dtype).t(), 0.0)   # (zeros times an infinite weight are NaN)
     loss = -torch.gather(logits.log_softmax(1), 1, at[:, None].long())[:, 0]   # NaN where a logit is inf, as the kernels'
     # a factor, so that a target outside the vocabulary makes its row's gradients NaN too
     loss = loss * torch.where(inside | ~scored, 1.0, torch.nan).to(loss.dtype)
@@ -105,9 +105,14 @@ def _token_losses_backward(gout, hidden, weight, targets, ignore_index, want_hid
         wide = weight.to(rows.dtype)
         seed = torch.where(scored, torch.where(inside, gout.reshape(-1), torch.nan), 0.0)[:, None]
         hot = torch.arange(vocab, device=at.device) == at[:, None]
-        grad = ((rows @ wide.t()).softmax(1) - hot.to(rows.dtype)) * seed
-        return ((grad @ wide).to(hidden.dtype).reshape(hidden.shape) if want_hidden else None,
-                (grad.t() @ rows).to(weight.dtype) if want_weight else None, None, None)
+        logits = torch.where(scored[:, None], rows @ wide.t(), 0.0)   # (zeros times an infinite weight are NaN)
+        grad = (logits.softmax(1) - hot.to(rows.dtype)) * seed
+        dhidden = dweight = None
+        if want_hidden:
+            dhidden = torch.where(scored[:, None], grad @ wide, 0.0).to(hidden.dtype).reshape(hidden.shape)
+        if want_weight:
+            dweight = (grad.t() @ rows).to(weight.dtype)
+        return dhidden, dweight, None, None
 
 
 def token_losses(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:

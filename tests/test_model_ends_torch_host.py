@@ -47,3 +47,19 @@ def test_a_logit_of_inf_leaves_no_distribution(dtype):
     want = ab.token_losses(h[0], torch.cat((w[:3], w[4:])), torch.tensor(1))
     assert torch.allclose(loss[0], want) and loss[1] == torch.inf and loss[3] == 0
     assert ab.token_losses(h, torch.full_like(w, -torch.inf), t)[:3].isnan().all()
+
+
+def test_a_row_that_is_not_scored_reaches_nothing_beside_an_infinite_weight():
+    """A word of inf that the scored rows hold at -inf: their losses are finite, and so are the weight's gradients; a row that is not
+    scored has a gradient of zeros."""
+    h, w = -torch.ones(4, 6), torch.randn(10, 6, generator=torch.Generator().manual_seed(2))
+    h[3] = torch.nan
+    w[3, 0] = torch.inf
+    t, g = torch.tensor([1, 2, -100, -100]), torch.rand(4, generator=torch.Generator().manual_seed(3))
+    h, w = h.requires_grad_(), w.requires_grad_()
+    loss = ab.token_losses(h, w, t)
+    assert loss[:2].isfinite().all() and not loss[2:].any()
+    for dh, dw in (torch.autograd.grad(loss, (h, w), g), BACKWARD["token_losses"](g, h.detach(), w.detach(), t, -100, True, True)[:2]):
+        assert not dh[2:].any() and dw.isfinite().all() and not dw[3].any()
+    loss = ab.token_losses(h, w, torch.full_like(t, -100))
+    assert not loss.any() and all(not x.any() for x in torch.autograd.grad(loss.sum(), (h, w)))
