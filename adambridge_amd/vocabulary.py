@@ -91,7 +91,7 @@ def _torch_token_losses(hidden, weight, targets, ignore_index):
     """The definition in torch operations, which hold all logits."""
     rows, scored, inside, at = _scored(hidden, targets, weight.shape[0], ignore_index)
     logits = torch.where(scored[:, None], rows @ weight.to(rows.dtype).t(), 0.0)   # (zeros times an infinite weight are NaN)
-    loss = -torch.gather(logits.log_softmax(1), 1, at[:, None].long())[:, 0]   # NaN where a logit is inf, as the kernels'
+    loss = -torch.gather(logits.log_softmax(1), 1, at[:, None])[:, 0]   # NaN where a logit is inf, as the kernels'
     # a factor, so that a target outside the vocabulary makes its row's gradients NaN too
     loss = loss * torch.where(inside | ~scored, 1.0, torch.nan).to(loss.dtype)
     return torch.where(scored, loss, 0.0).reshape(targets.shape)
@@ -140,6 +140,9 @@ def token_losses(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tens
         raise ValueError(f"hidden, weight and targets must be on one device, got {hidden.device}, {weight.device} and {targets.device}")
     if isinstance(ignore_index, bool) or not isinstance(ignore_index, int):
         raise ValueError(f"ignore_index must be an int, got {ignore_index!r}")
+    if not -(1 << 63) <= ignore_index < 1 << 63:
+        raise ValueError(f"ignore_index must be an int of 64 bits, got {ignore_index}")
+    targets = targets.long()   # an ignore_index past 32 bits is compared as it is
     if torch.is_autocast_enabled(hidden.device.type):
         cast = torch.get_autocast_dtype(hidden.device.type)
         hidden, weight = (t.to(cast) if t.is_floating_point() and t.dtype != torch.float64 else t for t in (hidden, weight))
@@ -148,7 +151,7 @@ def token_losses(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tens
     with torch.autocast(hidden.device.type, enabled=False):
         if (plain(hidden, weight) and type(targets) is torch.Tensor and 0 < targets.numel() <= _MOST_ROWS and weight.shape[0] <= _MOST_CLASSES
                 and _LEAST_SIZE[weight.dtype] <= weight.shape[1] <= _MOST_SIZE and not _observed()):
-            losses = _hip.ops().token_losses(hidden.contiguous(), weight.contiguous(), targets.long().contiguous(), ignore_index)
+            losses = _hip.ops().token_losses(hidden.contiguous(), weight.contiguous(), targets.contiguous(), ignore_index)
             if losses is not None:
                 return losses
         return _torch_token_losses(hidden, weight, targets, ignore_index)

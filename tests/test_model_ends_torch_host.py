@@ -63,3 +63,17 @@ def test_a_row_that_is_not_scored_reaches_nothing_beside_an_infinite_weight():
         assert not dh[2:].any() and dw.isfinite().all() and not dw[3].any()
     loss = ab.token_losses(h, w, torch.full_like(t, -100))
     assert not loss.any() and all(not x.any() for x in torch.autograd.grad(loss.sum(), (h, w)))
+
+
+def test_an_ignore_index_that_is_no_target_s_type():
+    """One past 32 bits ignores no row of int32 targets; one past 64 bits is refused."""
+    gen = torch.Generator().manual_seed(4)
+    h, w, t = torch.randn(4, 6, generator=gen), torch.randn(10, 6, generator=gen), torch.tensor([0, 1, 2, 3])
+    want = ab.token_losses(h, w, t)
+    for ignore in (1 << 32, 1 << 40, -(1 << 40), (1 << 63) - 1, -(1 << 63)):
+        assert torch.equal(ab.token_losses(h, w, t.int(), ignore), want) and torch.equal(ab.token_losses(h, w, t, ignore), want)
+    assert (want > 0).all()
+    for ignore in (1 << 63, -(1 << 63) - 1, 1 << 70):
+        for targets in (t, t.int()):
+            with pytest.raises(ValueError, match="ignore_index must be an int of 64 bits"):
+                ab.token_losses(h, w, targets, ignore)
