@@ -301,14 +301,16 @@ __global__ __launch_bounds__(256) void k_embed_rows(EmbedBackArgs A)
     const int start = A.starts[v0 + (lane < words ? lane : words)], next = __shfl_down(start, 1);
     // words that are not sums of their rows: the padding, and long ones
     uint64_t apart = __builtin_amdgcn_ballot_w64(lane < words && (v0 + lane == A.padding || is_long(A, start, next)));
+    const uint64_t some = __builtin_amdgcn_ballot_w64(lane < words && next > start && v0 + lane != A.padding);
     float acc[L];
     auto clear = [&]() {
 #pragma unroll
         for (int k = 0; k < L; ++k) acc[k] = 0.0f;
     };
     auto flush = [&](int w) {
+        const float by = some >> w & 1 ? A.scale : 0.0f;   // zeros without tokens, whatever the scale
 #pragma unroll
-        for (int k = 0; k < L; ++k) acc[k] *= A.scale;
+        for (int k = 0; k < L; ++k) acc[k] *= by;
         columns.stream(at<DT>(A.dweight, (v0 + w) * A.hidden), A.hidden, acc);
         clear();
     };
@@ -383,10 +385,12 @@ __global__ __launch_bounds__(256) void k_embed_few(EmbedBackArgs A)
         float acc[L];
 #pragma unroll
         for (int k = 0; k < L; ++k) acc[k] = 0.0f;
+        float by = 0.0f;   // zeros without tokens, whatever the scale
         if (v0 + w != A.padding) {
 #pragma unroll
             for (int b = 0; b < B; ++b) {
                 uint64_t mine = __builtin_amdgcn_ballot_w64(id[b] == v0 + w);
+                by = mine ? A.scale : by;
                 while (mine) {
                     raw16 row[AHEAD];
                     int n = 0, from = 0;
@@ -404,7 +408,7 @@ __global__ __launch_bounds__(256) void k_embed_few(EmbedBackArgs A)
             }
         }
 #pragma unroll
-        for (int k = 0; k < L; ++k) acc[k] *= A.scale;
+        for (int k = 0; k < L; ++k) acc[k] *= by;
         columns.stream(at<DT>(A.dweight, (v0 + w) * A.hidden), A.hidden, acc);
     }
 }

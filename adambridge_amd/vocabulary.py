@@ -31,7 +31,7 @@ def _torch_embed(ids, weight, scale, padding_idx):
     rows = wide.index_select(0, torch.where(inside, flat, 0))
     if padding_idx is not None:
         rows = torch.where((flat == padding_idx)[:, None], rows.detach(), rows)
-    y = torch.where(inside[:, None], rows * scale, torch.nan)
+    y = torch.where(inside[:, None], rows, torch.nan) * scale   # (in this order zeros go back to the rows of ids outside, whatever the scale)
     return y.to(weight.dtype).reshape(*ids.shape, hidden)
 
 

@@ -27,3 +27,18 @@ def test_a_target_outside_the_vocabulary_has_gradients_of_nan(dtype, size, rows)
         got = torch.func.grad(lambda a, b: ab.token_losses(a, b, t).sum(), argnums=(0, 1))(h.detach(), w.detach())
         assert torch.equal(got[0].isnan(), dh.isnan()) and got[1].isnan().all()
         assert torch.allclose(got[0][~bad], dh[~bad], rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("scale", [float("inf"), float("nan"), -3.0])
+@pytest.mark.parametrize("tokens,hidden", [(9, 40), (9, 3), (256, 33), (257, 40), (700, 2), (5000, 1030)])
+def test_a_scale_that_is_not_finite_reaches_its_tokens_words_only(tokens, hidden, scale, dtype):
+    """Words without tokens, the padding (the most frequent word) and ids outside the vocabulary: zeros, not -0 or NaN."""
+    ids = torch.full((tokens,), 13, device="cuda")
+    ids[1::3], ids[2::7], ids[3] = 4, 60, -1   # 60 words; 4 has every third token
+    w = torch.randn(60, hidden, device="cuda").to(dtype).requires_grad_()
+    dw, = torch.autograd.grad(ab.embed(ids, w, scale, 13), w, torch.ones(tokens, hidden, device="cuda", dtype=dtype))
+    want = (torch.full((hidden,), float((ids == 4).sum()), device="cuda") * scale).to(dtype)
+    assert torch.equal(dw[4].nan_to_num(), want.nan_to_num())
+    others = dw[torch.arange(60, device="cuda") != 4]
+    assert not others.any() and not others.signbit().any()

@@ -77,3 +77,13 @@ def test_an_ignore_index_that_is_no_target_s_type():
         for targets in (t, t.int()):
             with pytest.raises(ValueError, match="ignore_index must be an int of 64 bits"):
                 ab.token_losses(h, w, targets, ignore)
+
+
+@pytest.mark.parametrize("scale", [float("inf"), float("nan"), -3.0])
+def test_a_scale_that_is_not_finite_reaches_its_tokens_words_only(scale):
+    """Words without tokens, the padding and ids outside the vocabulary: zeros."""
+    w, ids = torch.randn(5, 4, requires_grad=True), torch.tensor([1, -1, 7, 2, 1])
+    y = ab.embed(ids, w, scale, 2)
+    assert torch.equal(y[[0, 3, 4]].detach().nan_to_num(), (w.detach()[[1, 2, 1]] * scale).nan_to_num())
+    for dw in (torch.autograd.grad(y, w, torch.ones(5, 4))[0], BACKWARD["embed"](torch.ones(5, 4), ids, 5, scale, 2)[1]):
+        assert not dw[[0, 2, 3, 4]].any() and torch.equal(dw[1].nan_to_num(), torch.full((4,), 2 * scale).nan_to_num())
