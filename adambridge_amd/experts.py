@@ -301,6 +301,15 @@ def expert_mm(x: torch.Tensor, weight: torch.Tensor, ends: torch.Tensor) -> torc
 _ACTIVATIONS = {"gelu": F.gelu, "silu": F.silu}
 
 
+def _few_tokens(x, logits, operands, top_k) -> bool:
+    """Whether the kernels take this call, once every operand's values lie one after the other."""
+    experts, inter, hidden = operands[1].shape
+    return (0 < x.shape[0] <= _FEW_TOKENS and plain(logits, *operands) and isinstance(top_k, int) and not isinstance(top_k, bool)
+            and 1 <= top_k <= min(experts, _MOST_CHOSEN) and experts <= _MOST_EXPERTS and 0 < inter <= _MOST_SIZE and 0 < hidden <= _MOST_SIZE
+            and not (torch.is_grad_enabled() and any(t.requires_grad for t in (logits, *operands)))
+            and not torch.is_autocast_enabled(x.device.type) and not _observed())
+
+
 def expert_mlp(x: torch.Tensor, logits: torch.Tensor, up: torch.Tensor, down: torch.Tensor, top_k: int,
                gate: torch.Tensor | None = None, activation: str = "gelu", normalize: bool = True) -> torch.Tensor:
     """A layer of expert MLPs: each token's sum, by the weights of ``route(logits, top_k, normalize)``, of
@@ -330,7 +339,8 @@ def expert_mlp(x: torch.Tensor, logits: torch.Tensor, up: torch.Tensor, down: to
         raise ValueError("x, logits, up, down and gate must be on one device")
     if not torch.is_autocast_enabled(x.device.type) and any(t.dtype != x.dtype for t in operands):
         raise ValueError(f"x, up, down and gate must be of one type, got {', '.join(str(t.dtype) for t in operands)}")
-    if plain(logits, *operands) and not all(t.is_contiguous() for t in (logits, *operands)) and x.shape[0] <= _FEW_TOKENS:
+    # the copies only where the kernels take the call: another lays out again what it needs
+    if _few_tokens(x, logits, operands, top_k) and not all(t.is_contiguous() for t in (logits, *operands)):
         out = _hip.ops().expert_mlp(x.contiguous(), logits.contiguous(), up.contiguous(), down.contiguous(),
                                     None if gate is None else gate.contiguous(), top_k, activation == "silu", bool(normalize))
         if out is not None:

@@ -68,3 +68,56 @@ def test_entry_point():
         assert mlp(*args) == -2
     assert mlp(p, p, f32, p, None, p, f32, *sizes, 0, 1, p, ctypes.c_void_p(264)) == -14
     assert work(f32, 16, 64, 8, 100, 8) > 64 * 16 * 100 * 4 and work(f32, 1, 64, 8, 100, 8) < 9 * 16 * 100 * 4
+
+
+def _copies(monkeypatch, call):
+    """The tensors that expert_mlp itself lays out again in ``call``, with its conditions taken as on a GPU."""
+    import sys
+
+    from adambridge_amd import experts
+
+    class Native:
+        def __getattr__(self, name):
+            return lambda *args: None   # every kernel declines: torch operations
+
+    seen, contiguous = [], torch.Tensor.contiguous
+
+    def counted(self, *args, **kwargs):
+        if sys._getframe(1).f_code is experts.expert_mlp.__code__:
+            seen.append(self)
+        return contiguous(self, *args, **kwargs)
+
+    with monkeypatch.context() as m:
+        m.setattr(experts, "plain", lambda *ts: all(t is None or t.dtype in (torch.float32, torch.bfloat16) for t in ts))
+        m.setattr(experts._hip, "ops", lambda: Native())
+        m.setattr(torch.Tensor, "contiguous", counted)
+        call()
+    return seen
+
+
+def test_operands_are_laid_out_again_only_for_a_call_that_the_kernels_take(monkeypatch):
+    """A trained call, one under autocast or observed, one of many tokens or of sizes that they do not take: expert_mm lays out what
+    it needs, and nothing is copied twice."""
+    x, logits, up, down, gate = _operands(torch.Generator().manual_seed(3), torch.float32)
+    strided = up.transpose(1, 2).contiguous().transpose(1, 2)
+    call = lambda *more, x=x, logits=logits, up=strided, down=down, top_k=2: lambda: ab.expert_mlp(x, logits, up, down, top_k, *more)
+    assert len(_copies(monkeypatch, call())) == 4 and len(_copies(monkeypatch, call(gate))) == 5
+    assert not _copies(monkeypatch, call(up=up))
+    for leaf in (x, logits, strided, down, gate):
+        leaf.requires_grad_()
+        assert not _copies(monkeypatch, call(gate))
+        with torch.no_grad():
+            assert len(_copies(monkeypatch, call(gate))) == 5
+        leaf.requires_grad_(False)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        assert not _copies(monkeypatch, call())
+    assert not _copies(monkeypatch, lambda: torch.func.vmap(lambda t: ab.expert_mlp(t, logits, strided, down, 2))(torch.stack((x, x))))
+    assert not _copies(monkeypatch, call(x=torch.cat((x, x, x)), logits=torch.cat((logits, logits, logits))))
+    assert not _copies(monkeypatch, call(x=x[:0], logits=logits[:0]))
+    half = [t.half() for t in (x, strided, down)]
+    assert not _copies(monkeypatch, call(x=half[0], up=half[1], down=half[2]))
+    wide = [torch.randn(*s) for s in ((2, 6), (2, 1030), (1030, 1, 6), (1030, 6, 1))]
+    assert not _copies(monkeypatch, call(x=wide[0].t().contiguous().t(), logits=wide[1], up=wide[2], down=wide[3]))
+    assert not _copies(monkeypatch, call(x=wide[0].t().contiguous().t(), logits=wide[1][:, :70], up=wide[2][:70], down=wide[3][:70], top_k=65))
+    with pytest.raises(ValueError, match="top_k must be an int"):
+        _copies(monkeypatch, call(top_k=True))
