@@ -6,8 +6,8 @@ A block is ``x + combine(down(gelu(up(dispatch(layer_norm(x))))))``: the package
 chooses ``top_k`` of the experts for each token, the rows' way to them, their products, and the way back, all but the
 norm in ``expert_mlp``.  Tokens come in by ``embed``; the loss is ``causal_lm_loss``, the optimizer ``AdamBridge`` (on the GPU;
 on the CPU, where its kernels do not run, torch's AdamW).  Nothing in a step waits for the device: the losses are read
-when the steps are done.  A decoded token takes one row through the model, with the sums over the tokens before kept
-from step to step; ``token_losses`` says afterwards how likely the model held each token.
+when the steps are done.  A prompt is decoded from in one pass; each token after it takes one row through the model, with the
+sums over the tokens before kept from step to step; ``token_losses`` says afterwards how likely the model held each token.
 """
 
 import argparse
@@ -44,12 +44,15 @@ class Model(torch.nn.Module):
         self.norm = torch.nn.LayerNorm(hidden)
         self.head = torch.nn.Linear(hidden, vocab, bias=False)
 
-    def forward(self, ids: torch.Tensor) -> torch.Tensor:
-        """Hidden states of ``ids`` [batch, seq], ready for the head."""
+    def forward(self, ids: torch.Tensor, sums: list[torch.Tensor] | None = None) -> torch.Tensor:
+        """Hidden states of ``ids`` [batch, seq], ready for the head.  ``sums``, if given, takes what :meth:`step` goes on from."""
         x = ab.embed(ids, self.embed.weight)
         count = torch.arange(1, ids.shape[1] + 1, device=ids.device)[:, None]
         for block in self.blocks:
-            x = block(x + (x.float().cumsum(1) / count).to(x.dtype))
+            total = x.float().cumsum(1)
+            if sums is not None:
+                sums.append(total[:, -1].clone())
+            x = block(x + (total / count).to(x.dtype))
         return ab.layer_norm(x, self.norm.weight, self.norm.bias, self.norm.eps)
 
     def step(self, ids: torch.Tensor, sums: list[torch.Tensor], count: int) -> torch.Tensor:
@@ -92,14 +95,12 @@ def train(steps: int, device: str, precision: str, batch: int = 8, seq: int = 64
 
 @torch.no_grad()
 def decode(model: Model, prompt: torch.Tensor, tokens: int) -> torch.Tensor:
-    """``tokens`` greedy tokens after ``prompt`` [seq], one at a time."""
-    sums = [torch.zeros(1, model.norm.normalized_shape[0], device=prompt.device) for _ in model.blocks]
-    ids = list(prompt[:, None])
-    for i in range(len(prompt) + tokens - 1):
-        hidden = model.step(ids[i], sums, i + 1)
-        if i + 1 == len(ids):
-            ids.append(model.head(hidden).argmax(-1))
-    return torch.cat(ids[len(prompt):])
+    """``tokens`` greedy tokens after ``prompt`` [seq]: the prompt in one pass, then one at a time."""
+    chosen, sums = [prompt[:0]], []
+    for i in range(tokens):
+        hidden = model.step(chosen[-1], sums, len(prompt) + i) if i else model(prompt[None], sums)[:, -1]
+        chosen.append(model.head(hidden).argmax(-1))
+    return torch.cat(chosen)
 
 
 @torch.no_grad()
