@@ -546,7 +546,8 @@ __global__ __launch_bounds__(256) void k_head_few(HeadArgs A)
         turn(s, even, odd);
         if (s + U < steps) turn(s + U, odd, even);
     }
-    const int64_t target = col < A.rows ? A.targets[col] - j0 : -1;
+    const int64_t target = col < A.rows ? A.targets[col] : -1;
+    const int hot = target >= j0 && target < j0 + words ? (int)(target - j0) : -1;   // (a target may be any number)
     Sums all{kHeadNegInf, 0.0f};
 #pragma unroll
     for (int n = 0; n < NG; ++n)
@@ -554,7 +555,7 @@ __global__ __launch_bounds__(256) void k_head_few(HeadArgs A)
         for (int r = 0; r < 4; ++r) {
             const int word = 16 * n + 4 * quarter + r;
             if (word >= words) acc[n][r] = kHeadNegInf;
-            else if (word == target) A.picked[col] = acc[n][r];
+            else if (word == hot) A.picked[col] = acc[n][r];
             all.m = __builtin_fmaxf(all.m, acc[n][r]);
         }
     all.m = __builtin_fmaxf(all.m, __shfl_xor(all.m, 16));

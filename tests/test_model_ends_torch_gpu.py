@@ -42,3 +42,21 @@ def test_a_scale_that_is_not_finite_reaches_its_tokens_words_only(tokens, hidden
     assert torch.equal(dw[4].nan_to_num(), want.nan_to_num())
     others = dw[torch.arange(60, device="cuda") != 4]
     assert not others.any() and not others.signbit().any()
+
+
+@pytest.mark.parametrize("rows", [6, 16, 17, 300])
+def test_targets_and_ignore_indexes_at_the_ends_of_64_bits(rows):
+    """A target of any 64 bits is outside the vocabulary, or is not scored where it is the ignore index."""
+    gen = torch.Generator("cuda").manual_seed(rows)
+    h, w = torch.randn(rows, 40, generator=gen, device="cuda"), torch.randn(700, 40, generator=gen, device="cuda")
+    clean = torch.randint(0, 700, (rows,), generator=gen, device="cuda")
+    want = ab.token_losses(h, w, clean)
+    ends = [-(1 << 63), 1 - (1 << 63), (1 << 63) - 1, -(1 << 32), 1 << 32]
+    t = clean.clone()
+    t[:5] = torch.tensor(ends, device="cuda")
+    for ignore in (-100, *ends):
+        loss = ab.token_losses(h, w, t, ignore)
+        assert torch.equal(loss[5:], want[5:])
+        assert [x.isnan().item() for x in loss[:5]] == [end != ignore for end in ends] and all(x == 0 or x.isnan() for x in loss[:5])
+    for ignore in (1 << 40, -(1 << 40)):
+        assert torch.equal(ab.token_losses(h, w, clean.int(), ignore), want)
