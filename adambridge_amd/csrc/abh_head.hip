@@ -625,7 +625,7 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_grad(HeadArgs A)
     const Operand a{at<H::DT>(A.h, (int64_t)i0 * A.hidden), A.hidden, 0, limit_i, A.hidden};
     const Operand b{at<H::DT>(A.w, (A.v0 + j0) * A.hidden), A.hidden, 0, limit_j, A.hidden};
     typename H::Sum acc[H::NI][H::NJ];
-    const int wi = H::wi(), wj = H::wj(), lane = threadIdx.x & 63;
+    const int wi = H::wi(), wj = H::wj();
     // the rows' numbers, asked for before the product, with no condition
     HeadRow facts[H::NI];
 #pragma unroll
@@ -685,7 +685,7 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_dh(HeadArgs A)
     const Operand a{at<H::DT>(A.g, (int64_t)i0 * A.pitch + k.first), A.pitch, 0, limit_i, (k.len + 7) & ~7};
     const Operand b{at<H::DT>(A.w, (A.v0 + k.first) * A.hidden), A.hidden, j0, A.hidden, k.len};
     typename H::Sum acc[H::NI][H::NJ];
-    const int wi = H::wi(), wj = H::wj(), lane = threadIdx.x & 63;
+    const int wi = H::wi(), wj = H::wj();
     if (!head_multiply<H, true, false>(lds, a, b, wi < limit_i, acc)) return;
     float* out = A.dh + ((int64_t)t.split * count + i0) * A.hidden + j0;
 #pragma unroll
@@ -722,7 +722,7 @@ __global__ __launch_bounds__(H::T, H::OCC) void k_head_dw(HeadArgs A)
     const Operand a{at<H::DT>(A.g, (int64_t)k.first * A.pitch), A.pitch, i0, A.pitch, k.len};
     const Operand b{at<H::DT>(A.h, (int64_t)k.first * A.hidden), A.hidden, j0, A.hidden, k.len};
     typename H::Sum acc[H::NI][H::NJ];
-    const int wi = H::wi(), wj = H::wj(), lane = threadIdx.x & 63;
+    const int wi = H::wi(), wj = H::wj();
     if (!head_multiply<H, false, false>(lds, a, b, wi < limit_i, acc)) return;
     if (A.splits > 1) {
         store_sums<H>(A.parts + ((int64_t)t.split * A.width + i0) * A.hidden + j0, A.hidden, limit_i, limit_j, acc, wi, wj);
