@@ -32,6 +32,7 @@ namespace abh {
 constexpr int kMlpTokens = 16, kMlpExperts = 1024, kMlpChosen = 64;
 constexpr int kMlpColumns = 16;   // a matrix instruction's
 constexpr int kUpWaves = 4, kDownWaves = 16;
+constexpr int kMlpCus = 256;
 
 // A chosen expert: which tokens chose it, and their weights.
 struct Chosen {
@@ -353,12 +354,13 @@ static void launch_up(const MlpArgs& A, const dim3 grid, int groups)
 template <int DT, bool EVEN>
 static void launch_down(const MlpArgs& A)
 {
-    // columns of a workgroup: so many that there are 256 of them, if there can be (us, 2048 columns, 16 / 8 / 4 a workgroup: one token of
-    // 8 experts of 1536 16.5 / 11.1 / 15.9, 13 tokens of 8 experts of 8192 86 / 57 / 79)
+    // Columns of a workgroup: the fewest with which a CU has one workgroup of them and not two (us of both kernels, 4 / 8 / 16: 13
+    // tokens, 2 of 8 experts of 8192, 1024 columns 64 / 74 / 103, 1536 121 / 100 / 127, 2048 133 / 114 / 138, 2560 184 / 178 / 160, 3500
+    // 238 / 204 / 194; of 4096, 4096 columns 134 / 117 / 107, 8192 270 / 225 / 209; one token of 8 experts of 1536, 1536 columns 25.8 / 21.6 / 26.8)
     const dim3 block(kDownWaves * kWave);
-    if (A.hidden >= 4096) hipLaunchKernelGGL((k_mlp_down<DT, EVEN, 16>), block_grid((A.hidden + 15) / 16), block, 0, t_stream, A);
-    else if (A.hidden >= 2048) hipLaunchKernelGGL((k_mlp_down<DT, EVEN, 8>), block_grid((A.hidden + 7) / 8), block, 0, t_stream, A);
-    else hipLaunchKernelGGL((k_mlp_down<DT, EVEN, 4>), block_grid((A.hidden + 3) / 4), block, 0, t_stream, A);
+    if (A.hidden <= 4 * kMlpCus) hipLaunchKernelGGL((k_mlp_down<DT, EVEN, 4>), block_grid((A.hidden + 3) / 4), block, 0, t_stream, A);
+    else if (A.hidden <= 8 * kMlpCus) hipLaunchKernelGGL((k_mlp_down<DT, EVEN, 8>), block_grid((A.hidden + 7) / 8), block, 0, t_stream, A);
+    else hipLaunchKernelGGL((k_mlp_down<DT, EVEN, 16>), block_grid((A.hidden + 15) / 16), block, 0, t_stream, A);
 }
 
 template <int DT>

@@ -34,7 +34,7 @@ def test_more_columns_than_workgroups_of_long_rows(inter, hidden, gated, dtype):
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 @pytest.mark.parametrize("gated", [False, True])
 @pytest.mark.parametrize("inter", [24, 33, 1030])
-@pytest.mark.parametrize("hidden", [2047, 2048, 2051, 4095, 4096, 4101, 4104, 5000])
+@pytest.mark.parametrize("hidden", [1024, 1025, 1536, 2047, 2048, 2049, 2051, 4095, 4096, 4101, 4104, 5000])
 def test_columns_of_the_result(hidden, inter, gated, dtype):
     gen = torch.Generator("cuda").manual_seed(inter + hidden)
     _check(7, 5, 3, inter, hidden, dtype, gated, "silu", True, gen)
