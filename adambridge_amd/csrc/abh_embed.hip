@@ -30,7 +30,10 @@
 namespace abh {
 
 constexpr int kRun = 4096, kSortThreads = 1024;
-constexpr int kMostWords = 8;     // of a wavefront; fewer than its lanes.  (65536 tokens, 32000 x 4096: 8 words 108 us, 16 112, 4 105)
+// Words of a wavefront, fewer than its lanes.  (us of a backward pass with 4 / 8 / 16: 65536 tokens of 32000 x 4096 BF16 215 / 224 / 225, of
+// 151936 x 896 110 / 113 / 118, of 200000 x 2048 228 / 244 / 244; 4096 of 151936 x 896 62 / 63 / 65; 2021 of 5003 x 897 FP32 17 / 17 / 17.  Without a sort, 4 / 8:
+// 8 tokens of 151936 x 896 50 / 53, 256 of 32000 x 4096 48 / 50, of 1000 x 8192 7.5 / 7.4)
+constexpr int kMostWords = 4;
 constexpr int kFewIds = 256;      // tokens whose ids every wavefront reads for itself
 constexpr int kLeastChunk = 32;   // tokens.  (the words' rows and the parts: 146 us with 32, 149 with 64)
 
