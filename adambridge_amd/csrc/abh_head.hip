@@ -897,6 +897,9 @@ struct HeadBackward {
         // parts x rows x hidden: as many as fill the CUs with tiles, or one
         dh = s.take<float>(std::max(rows * hidden, (int64_t)places_of(dh_kind) * tile_m(dh_kind) * tile_n(dh_kind)));
         grad_splits = splits_of(tiles_of(grad, rows, width), places_of(grad), hidden);
+        // two parts no more than forward (us, whole / two: 2048 rows of 3500 x 2048 BF16 149 / 158, 1000 of 7000 x 1024 94 / 108, of 7000 x
+        // 4096 211 / 212; 500 of 3500 x 1024 FP32 142 / 146)
+        if (tiles_of(grad, rows, width) * 3 > places_of(grad)) grad_splits = 1;
         dw_splits = splits_of(tiles_of(dw, width, hidden), places_of(dw), rows);
         if (tiles_of(dw, width, hidden) * 3 > places_of(dw)) dw_splits = 1;   // (1237 rows, 5003 x 333 FP32: 55 us whole, 55 + 6 in two parts)
         parts = s.take<float>(std::max(grad_splits > 1 ? grad_splits * rows * pitch : 0, dw_splits > 1 ? dw_splits * width * hidden : 0));

@@ -56,3 +56,10 @@ def test_large_fp32_tiles(rows, vocab, size):
 def test_large_tiles_of_any_rows(rows, vocab, size):
     gen = torch.Generator("cuda").manual_seed(rows + size)
     _check(*_inputs(rows, vocab, size, BF16, gen))
+
+
+# tiles of the backward pass's logits that would fit twice into the CUs' places: their sums stay whole
+@pytest.mark.parametrize("rows,vocab,size,dtype", [(1000, 7000, 1032, BF16), (1000, 7000, 1029, BF16), (500, 3500, 1030, FP32)])
+def test_tiles_that_would_fit_twice(rows, vocab, size, dtype):
+    gen = torch.Generator("cuda").manual_seed(rows + size)
+    _check(*_inputs(rows, vocab, size, dtype, gen))
