@@ -25,7 +25,7 @@ _LEAST_SIZE = {torch.bfloat16: 8, torch.float32: 4}
 def _torch_embed(ids, weight, scale, padding_idx):
     """The definition in torch operations."""
     vocab, hidden = weight.shape
-    flat = ids.reshape(-1)
+    flat = ids.reshape(-1).long()   # a vocabulary past 32 bits is compared as it is
     inside = (flat >= 0) & (flat < vocab)
     wide = weight.to(torch.promote_types(weight.dtype, torch.float32))   # before the rows are taken: their gradients are summed so
     rows = wide.index_select(0, torch.where(inside, flat, 0))
@@ -37,7 +37,7 @@ def _torch_embed(ids, weight, scale, padding_idx):
 
 def _embed_backward(gout, ids, vocab, scale, padding_idx):
     """The embedding's gradient in torch operations, differentiable in turn."""
-    flat = ids.reshape(-1)
+    flat = ids.reshape(-1).long()
     inside = (flat >= 0) & (flat < vocab)
     if padding_idx is not None:
         inside = inside & (flat != padding_idx)

@@ -87,3 +87,10 @@ def test_a_scale_that_is_not_finite_reaches_its_tokens_words_only(scale):
     assert torch.equal(y[[0, 3, 4]].detach().nan_to_num(), (w.detach()[[1, 2, 1]] * scale).nan_to_num())
     for dw in (torch.autograd.grad(y, w, torch.ones(5, 4))[0], BACKWARD["embed"](torch.ones(5, 4), ids, 5, scale, 2)[1]):
         assert not dw[[0, 2, 3, 4]].any() and torch.equal(dw[1].nan_to_num(), torch.full((4,), 2 * scale).nan_to_num())
+
+
+def test_a_vocabulary_past_32_bits_with_int32_ids():
+    """(One row of memory.)"""
+    weight = torch.full((1, 2), 3.0).expand((1 << 32) + 9, 2)
+    ids = torch.tensor([0, 7, 8, 9, (1 << 31) - 1, -1], dtype=torch.int32)
+    assert torch.equal(ab.embed(ids, weight).isnan().all(1), ids < 0)
