@@ -27,8 +27,11 @@ def _torch_embed(ids, weight, scale, padding_idx):
     vocab, hidden = weight.shape
     flat = ids.reshape(-1).long()   # a vocabulary past 32 bits is compared as it is
     inside = (flat >= 0) & (flat < vocab)
-    wide = weight.to(torch.promote_types(weight.dtype, torch.float32))   # before the rows are taken: their gradients are summed so
-    rows = wide.index_select(0, torch.where(inside, flat, 0))
+    wide, at = torch.promote_types(weight.dtype, torch.float32), torch.where(inside, flat, 0)
+    if _observed() or torch.is_grad_enabled() and weight.requires_grad:
+        rows = weight.to(wide).index_select(0, at)   # widened before the rows are taken: their gradients are summed so
+    else:
+        rows = weight.index_select(0, at).to(wide)
     if padding_idx is not None:
         rows = torch.where((flat == padding_idx)[:, None], rows.detach(), rows)
     y = torch.where(inside[:, None], rows, torch.nan) * scale   # (in this order zeros go back to the rows of ids outside, whatever the scale)

@@ -94,3 +94,18 @@ def test_a_vocabulary_past_32_bits_with_int32_ids():
     weight = torch.full((1, 2), 3.0).expand((1 << 32) + 9, 2)
     ids = torch.tensor([0, 7, 8, 9, (1 << 31) - 1, -1], dtype=torch.int32)
     assert torch.equal(ab.embed(ids, weight).isnan().all(1), ids < 0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_few_tokens_without_gradients_do_not_widen_the_table(dtype, monkeypatch):
+    """With a gradient the whole table is taken in FP32, in which its rows' gradients are summed."""
+    weight, ids = torch.randn(500, 8).to(dtype).requires_grad_(), torch.tensor([3, 499, 500, 3])
+    sizes, to = [], torch.Tensor.to
+    monkeypatch.setattr(torch.Tensor, "to", lambda self, *args, **kwargs: (sizes.append(self.numel()), to(self, *args, **kwargs))[1])
+    trained = ab.embed(ids, weight, 1.7, 3)
+    assert max(sizes) == 4000
+    sizes.clear()
+    with torch.no_grad():
+        rows = ab.embed(ids, weight, 1.7, 3)
+    assert torch.equal(ab.embed(ids, weight.detach(), 1.7, 3).nan_to_num(), rows.nan_to_num()) and max(sizes) <= 32
+    assert torch.equal(rows.nan_to_num(), trained.detach().nan_to_num())
