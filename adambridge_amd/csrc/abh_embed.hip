@@ -4,8 +4,8 @@
 //   dW[v] = scale sum of g[i] over ids[i] = v    (zeros for a word without tokens, and for the padding)
 //
 // Bytes bound both: T rows read and written; T rows read and V written, most of them zeros.  (65536 tokens of 32000 x 4096 BF16: rows
-// 125 us; gradient 46 for the order, 43 for long words' parts, 103 for the words' rows, 5.5 TB/s of the two.  4096 of 151936 x 896:
-// 4.5; 5.8, 6.6, 50, 5.4 TB/s.)
+// 124 us; gradient 47 for the order, 43 for long words' parts, 98 for the words' rows, 5.7 TB/s of the two.  4096 of 151936 x 896:
+// 4.9; 5.3, 7.0, 51, 5.5 TB/s.)
 //
 // The gradient's sums run over the tokens sorted by id, then by position, so that they have an order of their own and
 // dW is written once, by the words' rows, without atomics on values or a pass that clears it.  Text has a few words
@@ -365,8 +365,8 @@ __global__ __launch_bounds__(256) void k_embed_rows(EmbedBackArgs A)
 }
 
 // The same of a few tokens in one launch: a wavefront has all ids, four a lane, and a word's tokens are the bits of four ballots, in
-// order.  (us of a forward and backward pass, 256 tokens so / 257 sorted: 5003 words of 897 BF16 values 47 / 51, 32000 of 4096 53 / 60;
-// one word's 256 rows of 4096, which are then one wavefront's, 63 / 60.)
+// order.  (us of a forward and backward pass, 256 tokens so / 257 sorted: 5003 words of 897 BF16 values 26 / 31, 32000 of 4096 52 / 59;
+// one word's 256 rows of 897, which are then one wavefront's, 32 / 31, of 4096 59 / 60.)
 template <int DT, bool SHORT>
 __global__ __launch_bounds__(256) void k_embed_few(EmbedBackArgs A)
 {

@@ -11,10 +11,11 @@
 // dh's FP32 sums grow by G W.  So each piece of W is read once for all rows, where slices of rows would read W, and
 // add to dW, once a slice.
 //
-// Rows that are not scored cost nothing and reach nothing, whatever they hold: the scored ones are copied together first, and the
-// products end with them (how many they are is known on the device only).  The matrix products bound all of it (6 T H V operations forward
-// and backward and 2 T H V for the logits again); a few rows are the weights read once, which HBM bounds.  (16384 rows of 32000 x 4096 BF16: logits 3.4 ms,
-// 1255 TFLOP/s; G, dW and dh of a half of the words 1.72, 1.72, 1.78, 1210-1250.  8 rows of 151936 x 896: 46 us, 5.9 TB/s.)
+// Rows that are not scored reach nothing, whatever they hold: the scored ones are copied together first, and the
+// products end with them (how many they are is known on the device only); 16 rows or fewer are all multiplied, and only the losses
+// tell them apart.  The matrix products bound all of it (6 T H V operations forward
+// and backward and 2 T H V for the logits again); a few rows are the weights read once, which HBM bounds.  (16384 rows of 32000 x 4096 BF16: logits 3.3-3.4 ms,
+// 1255-1285 TFLOP/s; G, dW and dh of a half of the words 1.67-1.72, 1.68-1.72, 1.72-1.78, 1210-1290.  8 rows of 151936 x 896: 46 us, 5.9 TB/s.)
 
 #include <hip/hip_runtime.h>
 
@@ -41,6 +42,8 @@ struct Sums {
     float m, s;
 };
 
+// x - m and its product with log2 e are rounded to FP32, so that the largest logit's exponential is exact, one of e^-8 off by at most
+// 2^-20 of itself; expf, which is exact to a step, takes several instructions of each of a tile's logits to one here.
 __device__ __forceinline__ float exp_of(float x, float m) { return __builtin_amdgcn_exp2f((x - m) * kHeadLog2e); }
 // The subtrahend that stands for a maximum, so that exp(-inf + inf) is never taken.
 __device__ __forceinline__ float shift_for(float m) { return m == kHeadNegInf ? 0.0f : m; }
@@ -508,7 +511,7 @@ __global__ __launch_bounds__(256) void k_head_few(HeadArgs A)
     mm_f32x4 acc[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) acc[n] = mm_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    raw16 even[NG][U], odd[NG][U];
+    raw16 even[NG][U], odd[NG][U];   // (BF16's products are exact in FP32, and a row's sum is one chain of its size / 32 steps)
     auto load = [&](int s, raw16 (&to)[NG][U]) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -820,7 +823,9 @@ static_assert(HalfTile::BM == 256 && HalfTile::BN == 128 && WideTile::BM == Larg
 // The tile for m x n sums of so many terms.  FP32: as the expert products' rule, 64 where tiles of 128 are few.  BF16: 256 x 256;
 // dW's 256 x 128, two workgroups a CU, where their columns end closer behind the last one (us, 256 / 128 columns: dW of 2703 rows
 // and 50688 words of 896 values 286 / 240, of 16384 rows and 16128 words of 4096 1649 / 1732; the other kernels are 8-18% slower on
-// half tiles).  Four wavefronts a workgroup where the sums are long, else eight, whose epilogues hide one another's waits (us, four
+// half tiles).  Logits whose large tiles are half the CUs or fewer are on half tiles too (us of the forward call, 256 / 128 columns: 2048 rows
+// of 3328 x 4096 102 / 90, of 2816 x 1024 39 / 36, 512 of 16000 x 2048 59 / 53, 256 of 32000 x 4096 103 / 96, of 32000 x 1024 34 / 36).
+// Four wavefronts a workgroup where the sums are long, else eight, whose epilogues hide one another's waits (us, four
 // / eight: 4096 rows of 32768 words of 1024 values 321 / 303, 2048 487 / 486, 4096 853 / 901, 8192 1599 / 1705).
 enum Product { SUMS, WEIGHTS, ROWS };   // the logits, dW, dh
 static Kind kind_of(int32_t dtype, int64_t m, int64_t n, int64_t terms, Product product)

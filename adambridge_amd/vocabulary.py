@@ -123,11 +123,15 @@ def token_losses(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tens
     ``weight`` ``[vocab, size]`` (a Linear head's), ``targets`` (int64 or int32) ``[...]``; float32 ``[...]`` (float64 from float64).
 
     ``-token_losses(...)`` is the log-probability of each target.  Differentiable in ``hidden`` and ``weight``: the backward pass
-    goes through the vocabulary in pieces (its scratch beside copies of ``hidden``: half a GiB in BF16, or 4096 words for every
-    row) and computes each piece's logits again, from ``weight`` as it is then: as any saved operand, it must not be
-    written between the two passes.  Where a target is ``ignore_index`` the loss is 0 and its row reaches nothing and costs nothing,
-    whatever it holds; a target outside the vocabulary gives a loss and gradients of NaN.  ``hidden`` and ``weight`` are of
-    one type (under autocast, taken in its type, as a Linear's are).  Rows shorter than 16 bytes take torch operations."""
+    goes through the vocabulary in pieces and computes each piece's logits again, from ``weight`` as it is then: as any saved
+    operand, it must not be written between the two passes.  Its scratch: a copy of ``hidden``, FP32 sums of ``hidden``'s size, a
+    piece's gradient of at most 2^28 values (half a GiB in BF16), or 4096 words for every row.  The forward pass's: a copy of
+    ``hidden`` and 8 bytes for each row and 256 words.
+
+    Where a target is ``ignore_index`` the loss is 0 and its row reaches nothing, whatever it holds (and of more than 16 rows,
+    it is left out of the products); a target outside the vocabulary gives a loss and gradients of NaN, as a logit of inf does.
+    ``hidden`` and ``weight`` are of one type (under autocast, taken in its type, as a Linear's are).  Rows shorter than 16 bytes
+    take torch operations."""
     if torch.compiler.is_compiling():
         return _uncompiled(token_losses, hidden, weight, targets, ignore_index)
     if weight.is_cuda:
