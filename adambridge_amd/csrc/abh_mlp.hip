@@ -356,7 +356,8 @@ static void launch_down(const MlpArgs& A)
 {
     // Columns of a workgroup: the fewest with which a CU has one workgroup of them and not two (us of both kernels, 4 / 8 / 16: 13
     // tokens, 2 of 8 experts of 8192, 1024 columns 64 / 74 / 103, 1536 121 / 100 / 127, 2048 133 / 114 / 138, 2560 184 / 178 / 160, 3500
-    // 238 / 204 / 194; of 4096, 4096 columns 134 / 117 / 107, 8192 270 / 225 / 209; one token of 8 experts of 1536, 1536 columns 25.8 / 21.6 / 26.8)
+    // 238 / 204 / 194; of 4096, 4096 columns 134 / 117 / 107, 8192 270 / 225 / 209; one token of 8 experts of 1536, 1536 columns 25.8 / 21.6 / 26.8.
+    // FP32, 13 tokens of 4096: 1024 75 / 80 / 107, 1280 134 / 98 / 124, 2048 150 / 116 / 138, 2560 194 / 169 / 147, 4096 296 / 227 / 217, 6144 431 / 329 / 347)
     const dim3 block(kDownWaves * kWave);
     if (A.hidden <= 4 * kMlpCus) hipLaunchKernelGGL((k_mlp_down<DT, EVEN, 4>), block_grid((A.hidden + 3) / 4), block, 0, t_stream, A);
     else if (A.hidden <= 8 * kMlpCus) hipLaunchKernelGGL((k_mlp_down<DT, EVEN, 8>), block_grid((A.hidden + 7) / 8), block, 0, t_stream, A);
@@ -370,9 +371,9 @@ static void launch_mlp(MlpArgs& A)
     const bool down_even = A.inter % kLane<DT> == 0 && (uintptr_t)A.down % 16 == 0;
     // two groups of columns share the tokens' rows and the choice, where that leaves a CU four workgroups (us, one / two: 13 tokens of 8
     // gated experts 8192 x 2048 109 / 101; one token of 8 experts 1536 x 2048, which does not, 12.8 / 14.5)
-    const int groups = (int64_t)A.used * ((A.inter + 31) / 32) >= 4 * 256 ? 2 : 1;
+    const int groups = (int64_t)A.used * ((A.inter + 31) / 32) >= 4 * kMlpCus ? 2 : 1;
     A.columns = (A.inter + groups * kMlpColumns - 1) / (groups * kMlpColumns);
-    const dim3 grid((unsigned)std::min<int64_t>((int64_t)A.used * A.columns, 4 * 256));   // as many as the CUs hold
+    const dim3 grid((unsigned)std::min<int64_t>((int64_t)A.used * A.columns, 4 * kMlpCus));   // as many as the CUs hold
     if (up_even) launch_up<DT, true>(A, grid, groups);
     else launch_up<DT, false>(A, grid, groups);
     if (down_even) launch_down<DT, true>(A);
